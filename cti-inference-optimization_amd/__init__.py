@@ -12,6 +12,10 @@ Public surface:
   layer_norm                 the encoder's input LayerNorm over the pooled rows
   layer_norm_stats           its per-row mean and rstd only
   layer_norm_linear          the input LayerNorm and the encoder's Linear in one matrix-core kernel
+  dequantize_embedding_int8  the values that int8 rows and their scales stand for
+  rms_norm_int8, layer_norm_int8   residual addition, norm and int8 rows with scales in one pass
+  linear_int8                Linear in 8-bit integers, a scale for each token and each channel
+  gated_linear_int8          both projections of a gated feed-forward block and their product
   RepEncoder                 the reference module with the fused step and LayerNorm on this path
   collate_flat_layout, prebuild_flat_layout   host builders of the flat layout
   pack_slots, merge_batches                   GPU builders of the flat layout
@@ -24,9 +28,10 @@ from ._capi import EbagError, lib as load_library
 from .encoder import RepEncoder
 from .layout import collate_flat_layout, merge_batches, pack_slots, prebuild_flat_layout
 from .staging import InputStager, move_model_inputs_to_device
-from .ops import (PooledEmbedding, embedding_bag_pooled, fused_all_slots_embedding, fused_all_slots_embedding_int8,
-                  fused_all_slots_embedding_int8_layernorm, fused_all_slots_embedding_layernorm, fused_embedding, layer_norm, layer_norm_linear,
-                  layer_norm_stats, make_tile_order, order_bytes, quantize_embedding_int8)
+from .ops import (PooledEmbedding, dequantize_embedding_int8, embedding_bag_pooled, fused_all_slots_embedding, fused_all_slots_embedding_int8,
+                  fused_all_slots_embedding_int8_layernorm, fused_all_slots_embedding_layernorm, fused_embedding, gated_linear_int8,
+                  layer_norm, layer_norm_int8, layer_norm_linear, layer_norm_stats, linear_int8, make_tile_order,
+                  order_bytes, quantize_embedding_int8, rms_norm_int8)
 
 __all__ = [
     "EbagError",
@@ -46,6 +51,11 @@ __all__ = [
     "fused_all_slots_embedding_int8_layernorm",
     "fused_all_slots_embedding_layernorm",
     "quantize_embedding_int8",
+    "dequantize_embedding_int8",
+    "rms_norm_int8",
+    "layer_norm_int8",
+    "linear_int8",
+    "gated_linear_int8",
     "layer_norm",
     "layer_norm_stats",
     "layer_norm_linear",

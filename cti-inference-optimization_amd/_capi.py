@@ -22,6 +22,8 @@ ABI_VERSION = 5
 F32, BF16, F16, I8 = 0, 1, 2, 3
 I64, I32 = 0, 1
 SUM, MEAN = 0, 1
+RMS_NORM, LAYER_NORM = 0, 1
+GATE_NONE, GATE_SILU, GATE_GELU, GATE_RELU = 0, 1, 2, 3
 
 OK = 0
 EINVAL = -1
@@ -34,6 +36,7 @@ _STATUS_NAMES = {EINVAL: "EINVAL", EUNSUPPORTED: "EUNSUPPORTED", EHIP: "EHIP", E
 _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 _INDEX_CODE = {torch.int64: I64, torch.int32: I32}
 _POOL_CODE = {"sum": SUM, "mean": MEAN}
+_GATE_CODE = {"silu": GATE_SILU, "gelu": GATE_GELU, "relu": GATE_RELU}
 
 
 class EbagError(RuntimeError):
@@ -117,6 +120,16 @@ SIGNATURES = {
         [_P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I64, _I64, _P],
     ),
     "cti_ebag_quantize_int8": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),
+    "cti_ebag_dequantize_int8": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _I32, _P]),
+    "cti_ebag_norm_int8": (
+        ctypes.c_int,
+        [_I32, _P, _P, _P, _I64, _I64, _I32, _P, _P, _I32, ctypes.c_float, _P, _P, _P],
+    ),
+    "cti_ebag_linear_int8": (
+        ctypes.c_int,
+        [_P, _P, _I64, _I32, _P, _P, _I32, _P, _I32, _I32, _P, _I32, _P, _I64, _P],
+    ),
+    "cti_ebag_linear_int8_workspace_bytes": (ctypes.c_int64, [_I64, _I32, _I32, _I32]),
     "cti_ebag_narrow_ids": (ctypes.c_int, [_P, _I64, _P, _I32]),
     "cti_ebag_fused_all_slots_layernorm": (
         ctypes.c_int,
@@ -200,6 +213,13 @@ def pooling_code(mode: str) -> int:
         return _POOL_CODE[mode]
     except KeyError:
         raise ValueError(f"unsupported pooling {mode!r}; expected 'sum' or 'mean'") from None
+
+
+def gate_code(activation: str) -> int:
+    try:
+        return _GATE_CODE[activation]
+    except KeyError:
+        raise ValueError(f"unsupported activation {activation!r}; expected 'silu', 'gelu' or 'relu'") from None
 
 
 def current_stream_handle(device: torch.device) -> int:

@@ -93,32 +93,6 @@ __device__ __forceinline__ float group_max(float m, int lg) {
   return m;
 }
 
-// rint(RN32(v / s)) as a byte for C elements, given inv = RN32(1 / s). |v / s| < 128, so y = v * inv
-// is within 128 * 2^-23 of v / s and RN32(v / s) within 128 * 2^-24: together below 2^-15. Where y is
-// further than that from a rounding boundary (an integer + 1/2) both round to the same integer, which
-// adding 1.5 * 2^23 leaves in the low byte; else (about one element in 16,000, and every NaN) the
-// element takes the division.
-template <int C>
-__device__ __forceinline__ void quantize_chunk(const float* v, float s, float inv, uint32_t* q) {
-  constexpr float kMagic = 12582912.f;
-  bool sure = true;
-#pragma unroll
-  for (int e = 0; e < C; ++e) {
-    const float y = v[e] * inv;
-    const float t = y + kMagic;
-    q[e] = __float_as_uint(t) & 0xffu;
-    sure = sure && fabsf(y - (t - kMagic)) < 0.5f - 3.0517578125e-5f;  // false for NaN
-  }
-  if (__builtin_expect(!sure, 0)) {
-#pragma unroll
-    for (int e = 0; e < C; ++e) {
-      float r = rintf(v[e] / s);
-      r = r < -128.f ? -128.f : (r > 127.f ? 127.f : r);
-      q[e] = static_cast<uint32_t>(static_cast<int32_t>(r)) & 0xffu;
-    }
-  }
-}
-
 template <typename T, int C, int K>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const char* w, int64_t rows, int32_t chunks,
                                                                        int64_t row_bytes, int lg, int8_t* q,
@@ -221,10 +195,95 @@ void launch_quantize(const char* w, int64_t rows, int64_t dim, int64_t row_strid
   hipLaunchKernelGGL((quantize_rows_loop_kernel<T>), grid, block, 0, s, w, rows, dim, row_stride, q, scale);
 }
 
+// ---------------------------------------------------------------------------------------------
+// The way back: out[r, j] = q[r, j] * scale[r] in fp32, rounded once to the output type.
+// Both arrays are contiguous, so a thread takes 16 consecutive bytes wherever rows begin and end in
+// them, and stores 16 consecutive values. Bound by HBM (one byte read and 2 or 4 written an element).
+// ---------------------------------------------------------------------------------------------
+constexpr int kDequantElems = 16;  // per thread
+
+template <typename T, typename I>
+__global__ void __launch_bounds__(kQuantThreads) dequantize_rows_kernel(const int8_t* q, const float* scale, I total,
+                                                                        I dim, char* out, int32_t stream_out) {
+  const I e0 = (static_cast<I>(blockIdx.x) * kQuantThreads + threadIdx.x) * kDequantElems;
+  if (e0 >= total) return;
+  I row = e0 / dim;
+  I left = dim - (e0 - row * dim);  // elements of this row from e0 on
+  T* const dst = reinterpret_cast<T*>(out) + e0;
+  if (total - e0 < kDequantElems) {
+    for (I e = 0; e < total - e0; ++e, --left) {
+      if (left == 0) {
+        ++row;
+        left = dim;
+      }
+      store_one(dst + e, static_cast<float>(q[e0 + e]) * scale[row], false);
+    }
+    return;
+  }
+  typedef u32x4 u32x4_any __attribute__((aligned(1)));
+  const u32x4 raw = *reinterpret_cast<const u32x4_any*>(q + e0);
+  float s = scale[row];
+  float v[kDequantElems];
+#pragma unroll
+  for (int e = 0; e < kDequantElems; ++e) v[e] = static_cast<float>(static_cast<int8_t>(raw[e / 4] >> (8 * (e % 4))));
+  if (left >= kDequantElems) {
+#pragma unroll
+    for (int e = 0; e < kDequantElems; ++e) v[e] *= s;
+  } else {
+#pragma unroll
+    for (int e = 0; e < kDequantElems; ++e, --left) {
+      if (left == 0) {
+        s = scale[++row];
+        left = dim;
+      }
+      v[e] *= s;
+    }
+  }
+  with_stream(stream_out, [&](auto stream) { store_out<kDequantElems>(dst, v, decltype(stream)::value); });
+}
+
+template <typename T>
+void launch_dequantize(const int8_t* q, const float* scale, int64_t total, int64_t dim, char* out, hipStream_t s) {
+  constexpr int64_t kPer = int64_t{kQuantThreads} * kDequantElems;
+  const dim3 grid(static_cast<unsigned>((total + kPer - 1) / kPer)), block(kQuantThreads);
+  const int32_t stream_out = total * Elem<T>::kBytes >= kStreamOutBytes;
+  if (total + kPer <= UINT32_MAX)
+    hipLaunchKernelGGL((dequantize_rows_kernel<T, uint32_t>), grid, block, 0, s, q, scale, static_cast<uint32_t>(total),
+                       static_cast<uint32_t>(dim), out, stream_out);
+  else
+    hipLaunchKernelGGL((dequantize_rows_kernel<T, uint64_t>), grid, block, 0, s, q, scale, static_cast<uint64_t>(total),
+                       static_cast<uint64_t>(dim), out, stream_out);
+}
+
 }  // namespace
 }  // namespace cti
 
 using namespace cti;
+
+extern "C" int cti_ebag_dequantize_int8(const int8_t* q, const float* scale, int64_t rows, int64_t dim, void* out,
+                                        int32_t out_dtype, void* stream) {
+  clear_error();
+  if (out_dtype != CTI_EBAG_F32 && out_dtype != CTI_EBAG_BF16 && out_dtype != CTI_EBAG_F16)
+    return set_error(CTI_EBAG_EINVAL, "unknown dtype code %d", out_dtype);
+  if (rows < 0) return set_error(CTI_EBAG_EINVAL, "rows must be >= 0 (got %lld)", (long long)rows);
+  if (dim < 1) return set_error(CTI_EBAG_EINVAL, "dim must be >= 1 (got %lld)", (long long)dim);
+  if (rows == 0) return CTI_EBAG_OK;
+  if (!q || !scale || !out) return set_error(CTI_EBAG_EINVAL, "NULL device pointer among q/scale/out");
+  if (rows > (int64_t{1} << 40) / dim)
+    return set_error(CTI_EBAG_EUNSUPPORTED, "more than 2^40 elements (%lld x %lld)", (long long)rows, (long long)dim);
+  if (reinterpret_cast<uintptr_t>(out) % dtype_bytes(out_dtype) != 0)
+    return set_error(CTI_EBAG_EINVAL, "out is not aligned to its elements");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* const o = static_cast<char*>(out);
+  switch (out_dtype) {
+    case CTI_EBAG_F32: launch_dequantize<float>(q, scale, rows * dim, dim, o, s); break;
+    case CTI_EBAG_BF16: launch_dequantize<bf16_t>(q, scale, rows * dim, dim, o, s); break;
+    default: launch_dequantize<f16_t>(q, scale, rows * dim, dim, o, s); break;
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return set_error(CTI_EBAG_EHIP, "dequantize launch failed: %s", hipGetErrorString(e));
+  return CTI_EBAG_OK;
+}
 
 extern "C" int cti_ebag_quantize_int8(const void* weight, int32_t dtype, int64_t rows, int64_t dim,
                                       int64_t row_stride, int8_t* q, float* scale, void* stream) {

@@ -154,4 +154,47 @@ inline LinearPlan linear_plan(int64_t M, int32_t N, int32_t K, int param_bytes, 
   return linear_choose(M, N, K, param_bytes, ws_bytes < most ? ws_bytes : most);
 }
 
+// ---------------------------------------------------------------------------------------------
+// int8 Linear: t [M, N or 2 N] = q [M, K] w^T in int32, K in steps of kLinear8Step bytes.
+// ---------------------------------------------------------------------------------------------
+constexpr int kLinear8Step = 128;
+// |t| <= K * 2^14 (both operands -128 throughout) stays below 2^31
+constexpr int kLinear8MaxK = 131071;
+constexpr int kLinear8MaxN = 1 << 30;  // 2 N is an int32 too
+
+enum Linear8Form {
+  kLinear8Rows,  // few rows: operands straight to registers
+  kLinear8Tile,  // 128 x 128 tiles, K split if they are few
+};
+struct Linear8Plan {
+  Linear8Form form;
+  int splits;  // of K: 1, or as many int32 partial sums as the workspace then has to hold
+  int steps;   // per split
+};
+
+inline int64_t linear8_part_bytes(const Linear8Plan& plan, int64_t M, int32_t N, bool gated) {
+  return plan.splits > 1 ? plan.splits * M * N * (gated ? 8 : 4) : 0;
+}
+
+// Workgroups of a launch (one split).
+inline int64_t linear8_workgroups(const Linear8Plan& plan, int64_t M, int32_t N, bool gated) {
+  if (plan.form == kLinear8Rows) return linear_ceil(N, 16);
+  return linear_ceil(M, 128) * linear_ceil(N, gated ? 64 : 128);
+}
+
+inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, int64_t ws_bytes) {
+  const int nk = static_cast<int>(linear_ceil(K, kLinear8Step));
+  if (M <= 32) return {kLinear8Rows, 1, nk};
+  Linear8Plan plan{kLinear8Tile, 1, nk};
+  int64_t want = kLinearCus / linear8_workgroups(plan, M, N, gated);
+  const int64_t fit = ws_bytes / (M * N * (gated ? 8 : 4));
+  if (want > fit) want = fit;
+  if (want > nk / 2) want = nk / 2;
+  if (want > 1) {
+    plan.steps = static_cast<int>(linear_ceil(nk, want));
+    plan.splits = static_cast<int>(linear_ceil(nk, plan.steps));
+  }
+  return plan;
+}
+
 }  // namespace cti

@@ -14,6 +14,9 @@ Like the reference's Triton kernels, the pooling and the LayerNorm are forward-o
 ``quantize_int8_()`` is the reference's int8 switch (``_USE_INT8_EMB``, online_best/infer.py:893
 and :976-1026): the table is row-quantised once on the device and every later ``pooled`` reads
 the int8 rows and their fp32 scales; ``dequantize_()`` switches back to the float table.
+``quantize_linear_int8_()`` does the same with ``linear``: its weight is quantised by output channel, and
+``forward`` then normalises the pooled block straight to int8 rows (``layer_norm_int8``) and multiplies in
+8-bit integers (``linear_int8``); ``dequantize_linear_()`` switches back.
 """
 from __future__ import annotations
 
@@ -23,7 +26,8 @@ from torch import nn
 from .layout import pack_slots
 from .ops import (fused_all_slots_embedding, fused_all_slots_embedding_int8,
                   fused_all_slots_embedding_int8_layernorm, fused_all_slots_embedding_layernorm,
-                  layer_norm, layer_norm_linear, layer_norm_stats, quantize_embedding_int8)
+                  layer_norm, layer_norm_int8, layer_norm_linear, layer_norm_stats, linear_int8,
+                  quantize_embedding_int8)
 
 
 class RepEncoder(nn.Module):
@@ -36,6 +40,7 @@ class RepEncoder(nn.Module):
         self.linear = nn.Linear(in_features=slot_num * emb_dim, out_features=d_model)
         self._int8_weight = None
         self._int8_scale = None
+        self._int8_linear = None
 
     def quantize_int8_(self):
         """Quantise the table to int8 rows + fp32 row scales (online_best/infer.py:980-987)."""
@@ -45,6 +50,17 @@ class RepEncoder(nn.Module):
 
     def dequantize_(self):
         self._int8_weight = self._int8_scale = None
+        return self
+
+    def quantize_linear_int8_(self):
+        """Quantise ``linear``'s weight to int8 rows + fp32 scales, one for each output channel, as it is
+        now (call it again after the weight has changed); ``forward`` multiplies in int8 from then on."""
+        with torch.no_grad():
+            self._int8_linear = quantize_embedding_int8(self.linear.weight.detach())
+        return self
+
+    def dequantize_linear_(self):
+        self._int8_linear = None
         return self
 
     def flat_inputs(self, batch: dict):
@@ -117,8 +133,21 @@ class RepEncoder(nn.Module):
         there). It needs a bf16 table and a bf16
         ``linear`` with LayerNorm parameters in bf16 or fp32 (the reference's model after
         ``model.to(bfloat16)``, online_best/infer.py:2797).
+
+        After ``quantize_linear_int8_()`` the pooled block is normalised to int8 rows with a scale each
+        (``layer_norm_int8``) and multiplied with the int8 weight (``linear_int8``); the output has
+        ``linear``'s dtype.
         """
         lin, norm = self.linear, self.input_norm
+        if self._int8_linear is not None:
+            if fused_linear:
+                raise ValueError("fused_linear does not combine with an int8 Linear (quantize_linear_int8_)")
+            fused_embs = self.pooled(batch)
+            with torch.no_grad():
+                q, scale = layer_norm_int8(fused_embs, norm.weight.detach(), norm.bias.detach(), norm.eps)
+                return linear_int8(q, scale, *self._int8_linear,
+                                   bias=lin.bias.detach() if lin.bias is not None else None,
+                                   out_dtype=lin.weight.dtype)
         if fused_linear:
             if not (self.emb.weight.dtype == torch.bfloat16 and lin.weight.dtype == torch.bfloat16
                     and norm.weight.dtype in (torch.bfloat16, torch.float32) and norm.weight.dtype == norm.bias.dtype

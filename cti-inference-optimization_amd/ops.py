@@ -114,6 +114,57 @@ def quantize_embedding_int8(weight: torch.Tensor):
     return q, scale
 
 
+def dequantize_embedding_int8(q: torch.Tensor, scale: torch.Tensor, out_dtype: torch.dtype = torch.bfloat16,
+                              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The values that int8 rows stand for: ``q [V, D] int8``, ``scale [V] float32`` (as
+    ``quantize_embedding_int8``, ``rms_norm_int8`` and ``layer_norm_int8`` return them) to
+    ``out [V, D]`` with ``out[v, j] = q[v, j] * scale[v]`` in fp32, rounded once to ``out_dtype``
+    (bf16 by default; fp32, bf16 or fp16, or ``out``'s). Written on torch's current stream."""
+    rows, dim, dev = _check_int8_rows("q", q, "scale", scale)
+    out = _output("out", out, (rows, dim), out_dtype, dev)
+    with torch.cuda.device(dev):
+        _capi.check(_capi.lib().cti_ebag_dequantize_int8(
+            q.data_ptr(), scale.data_ptr(), rows, dim, out.data_ptr(), _capi.dtype_code(out.dtype),
+            _capi.current_stream_handle(dev)))
+    return out
+
+
+def _check_int8_rows(name: str, q, scale_name: str, scale, device: Optional[torch.device] = None):
+    """Validate int8 rows and their scales; return (rows, columns, device)."""
+    _require_device_tensor(name, q, device)
+    _require_device_tensor(scale_name, scale, q.device)
+    if q.dim() != 2 or q.shape[1] < 1:
+        raise ValueError(f"{name} must be 2-D [rows, columns >= 1], got shape {tuple(q.shape)}")
+    if q.dtype != torch.int8:
+        raise TypeError(f"{name} must be int8 (got {q.dtype})")
+    if scale.dtype != torch.float32:
+        raise TypeError(f"{scale_name} must be float32 (got {scale.dtype})")
+    _require_contiguous(name, q)
+    _require_contiguous(scale_name, scale)
+    if scale.dim() != 1 or scale.numel() != q.shape[0]:
+        raise ValueError(f"{scale_name} has shape {tuple(scale.shape)}, expected ({q.shape[0]},)")
+    return q.shape[0], q.shape[1], q.device
+
+
+def _output(name: str, out: Optional[torch.Tensor], shape, dtype: torch.dtype, dev: torch.device,
+            any_float: bool = True) -> torch.Tensor:
+    """`out`, checked, or a new tensor of `dtype`; an `out` given may have any element type of the
+    library (`any_float`), or must have `dtype`."""
+    if out is None:
+        if any_float:
+            _capi.dtype_code(dtype)
+        return torch.empty(shape, dtype=dtype, device=dev)
+    _require_device_tensor(name, out, dev)
+    _require_contiguous(name, out)
+    if tuple(out.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(out.shape)}, expected {tuple(shape)}")
+    if any_float:
+        _capi.dtype_code(out.dtype)
+    elif out.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype} (got {out.dtype})")
+    return out
+
+
 def _check_flat_layout(flat_values, val_offsets, flat_row_offsets, out, dev):
     """Validate a flat-layout batch; return the (index, offset) type codes. Ids may be int64 or
     int32; val_offsets and flat_row_offsets share one type, int64 or int32."""
@@ -820,3 +871,159 @@ def layer_norm_linear(
             _capi.dtype_code(bias.dtype) if bias is not None else _capi.F32, out.data_ptr(),
             _capi.dtype_code(out.dtype), ptr(ws), ws_bytes, _capi.current_stream_handle(dev)))
     return out
+
+
+def _norm_int8(kind: int, x, weight, bias, eps, residual, q, scale, residual_out):
+    _require_device_tensor("x", x)
+    dev = x.device
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x must be 2-D [rows, cols >= 1], got shape {tuple(x.shape)}")
+    _require_contiguous("x", x)
+    code = _capi.dtype_code(x.dtype)
+    rows, cols = x.shape
+    params = [("weight", weight)] + ([("bias", bias)] if kind == _capi.LAYER_NORM else [])
+    for name, t in params:
+        _require_device_tensor(name, t, dev)
+        _require_contiguous(name, t)
+        if t.numel() != cols:
+            raise ValueError(f"{name} has {t.numel()} elements, expected {cols}")
+        if t.dtype != weight.dtype:
+            raise TypeError(f"weight and bias dtypes differ ({weight.dtype} vs {t.dtype})")
+    param_code = _capi.dtype_code(weight.dtype)
+    if residual is None:
+        if residual_out is not None:
+            raise ValueError("residual_out needs a residual")
+    else:
+        _require_device_tensor("residual", residual, dev)
+        _require_contiguous("residual", residual)
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"residual must be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
+        residual_out = _output("residual_out", residual_out, x.shape, x.dtype, dev, any_float=False)
+    q = _output("q", q, x.shape, torch.int8, dev, any_float=False)
+    scale = _output("scale", scale, (rows,), torch.float32, dev, any_float=False)
+    ptr = (lambda t: t.data_ptr() if t is not None else None)
+    with torch.cuda.device(dev):
+        _capi.check(_capi.lib().cti_ebag_norm_int8(
+            kind, x.data_ptr(), ptr(residual), ptr(residual_out), rows, cols, code, weight.data_ptr(), ptr(bias),
+            param_code, float(eps), q.data_ptr(), scale.data_ptr(), _capi.current_stream_handle(dev)))
+    return (q, scale) if residual is None else (q, scale, residual_out)
+
+
+def rms_norm_int8(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float = 1e-5,
+    residual: Optional[torch.Tensor] = None,
+    q: Optional[torch.Tensor] = None,
+    scale: Optional[torch.Tensor] = None,
+    residual_out: Optional[torch.Tensor] = None,
+):
+    """Root-mean-square norm of the rows of ``x[rows, cols]`` (fp32, bf16 or fp16), with the addition
+    of ``residual`` before it and int8 rows with a scale each as its output, in one pass:
+
+    ``h = x + residual``; ``y = h / sqrt(mean(h^2) + eps) * weight``; then ``scale`` and ``q`` as
+    ``quantize_embedding_int8`` makes them from ``y``, all in fp32. Returns ``(q, scale)``, int8
+    ``[rows, cols]`` and fp32 ``[rows]``, or with a residual ``(q, scale, residual_out)``, where
+    ``residual_out`` is ``h`` rounded to x's dtype (the norm reads ``h`` unrounded); it may be
+    ``residual`` or ``x`` itself, the other outputs overlap no input. ``weight`` is ``[cols]`` of any
+    of the three types. A row whose statistics or normalised values are not all finite gets the
+    scale NaN and ``q`` 0. Written on torch's current stream.
+    """
+    return _norm_int8(_capi.RMS_NORM, x, weight, None, eps, residual, q, scale, residual_out)
+
+
+def layer_norm_int8(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor,
+    eps: float = 1e-5,
+    residual: Optional[torch.Tensor] = None,
+    q: Optional[torch.Tensor] = None,
+    scale: Optional[torch.Tensor] = None,
+    residual_out: Optional[torch.Tensor] = None,
+):
+    """LayerNorm of the rows of ``x[rows, cols]`` with int8 rows and a scale each as its output: as
+    ``rms_norm_int8``, with ``y = (h - mean) / sqrt(var + eps) * weight + bias`` (the encoder's input
+    norm, ``layer_norm``, before its rounding)."""
+    return _norm_int8(_capi.LAYER_NORM, x, weight, bias, eps, residual, q, scale, residual_out)
+
+
+def _linear_int8(q, scale, weight, weight_scale, bias, gate: int, out, out_dtype, split_k: bool):
+    rows, cols, dev = _check_int8_rows("q", q, "scale", scale)
+    w_rows, w_cols, _ = _check_int8_rows("weight", weight, "weight_scale", weight_scale, dev)
+    if w_cols != cols:
+        raise ValueError(f"weight has {w_cols} columns, q has {cols}")
+    if w_rows < 1:
+        raise ValueError("weight has no rows")
+    n_out = w_rows
+    if gate != _capi.GATE_NONE:
+        if w_rows % 2:
+            raise ValueError(f"weight has {w_rows} rows; expected as many gates as values (an even number)")
+        n_out = w_rows // 2
+    if bias is not None:
+        _require_device_tensor("bias", bias, dev)
+        _require_contiguous("bias", bias)
+        if bias.numel() != w_rows:
+            raise ValueError(f"bias has {bias.numel()} elements, expected {w_rows}")
+    bias_code = _capi.dtype_code(bias.dtype) if bias is not None else _capi.F32
+    out = _output("out", out, (rows, n_out), out_dtype, dev)
+    lib = _capi.lib()
+    # K split over several workgroups where few tiles would leave CUs idle: int32 partial sums in a
+    # workspace from torch's allocator (kept alive until the launches are enqueued)
+    ws_bytes = lib.cti_ebag_linear_int8_workspace_bytes(rows, cols, n_out, gate) if split_k else 0
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
+    with torch.cuda.device(dev):
+        _capi.check(lib.cti_ebag_linear_int8(
+            q.data_ptr(), scale.data_ptr(), rows, cols, weight.data_ptr(), weight_scale.data_ptr(), n_out,
+            bias.data_ptr() if bias is not None else None, bias_code, gate, out.data_ptr(),
+            _capi.dtype_code(out.dtype), ws.data_ptr() if ws is not None else None, ws_bytes,
+            _capi.current_stream_handle(dev)))
+    return out
+
+
+def linear_int8(
+    q: torch.Tensor,
+    scale: torch.Tensor,
+    weight: torch.Tensor,
+    weight_scale: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+    split_k: bool = True,
+) -> torch.Tensor:
+    """Linear in 8-bit integers on the matrix cores: ``q`` int8 ``[rows, cols]`` with ``scale`` fp32
+    ``[rows]`` (``layer_norm_int8``, ``rms_norm_int8``, ``quantize_embedding_int8``), ``weight`` int8
+    ``[out_features, cols]`` with ``weight_scale`` fp32 ``[out_features]`` (an nn.Linear's weight
+    through ``quantize_embedding_int8``), ``bias`` ``[out_features]`` of any type of the library:
+
+    ``out[m, n] = (sum_k q[m, k] * weight[n, k]) * scale[m] * weight_scale[n] + bias[n]``,
+
+    the sum exact in int32 (``cols`` at most 131071), the rest in fp32 with one rounding to
+    ``out_dtype`` (bf16 by default; or ``out``'s type). With ``split_k`` (default) a shape whose tiles
+    would leave CUs idle has K split over several workgroups (partial sums in a workspace from torch's
+    allocator); the result is the same bit for bit. Written on torch's current stream.
+    """
+    return _linear_int8(q, scale, weight, weight_scale, bias, _capi.GATE_NONE, out, out_dtype, split_k)
+
+
+def gated_linear_int8(
+    q: torch.Tensor,
+    scale: torch.Tensor,
+    weight: torch.Tensor,
+    weight_scale: torch.Tensor,
+    bias: Optional[torch.Tensor] = None,
+    activation: str = "silu",
+    out: Optional[torch.Tensor] = None,
+    out_dtype: torch.dtype = torch.bfloat16,
+    split_k: bool = True,
+) -> torch.Tensor:
+    """Both projections of a gated feed-forward block, the activation and their product in one kernel:
+    ``weight`` int8 ``[2 * hidden, cols]`` holds the gates' rows and then the values' (as do
+    ``weight_scale`` and ``bias``), and with ``v = linear_int8(...)`` unrounded
+
+    ``out[m, n] = act(v[m, n]) * v[m, hidden + n]``, ``n < hidden``,
+
+    rounded once. ``activation`` is "silu", "gelu" (exact) or "relu". The rest is as in
+    ``linear_int8``; ``quantize_embedding_int8`` makes the input of the projection back of the result.
+    """
+    return _linear_int8(q, scale, weight, weight_scale, bias, _capi.gate_code(activation), out, out_dtype, split_k)

@@ -59,6 +59,16 @@ extern "C" {
 #define CTI_EBAG_SUM 0
 #define CTI_EBAG_MEAN 1
 
+/* norms of cti_ebag_norm_int8 */
+#define CTI_EBAG_RMS_NORM 0
+#define CTI_EBAG_LAYER_NORM 1
+
+/* gates of cti_ebag_linear_int8 */
+#define CTI_EBAG_GATE_NONE 0
+#define CTI_EBAG_GATE_SILU 1 /* g / (1 + exp(-g)) */
+#define CTI_EBAG_GATE_GELU 2 /* g * (1 + erf(g / sqrt(2))) / 2 */
+#define CTI_EBAG_GATE_RELU 3 /* max(g, 0) */
+
 /* status codes */
 #define CTI_EBAG_OK 0
 #define CTI_EBAG_EINVAL (-1)      /* bad argument (null pointer, negative size, bad enum, ...) */
@@ -454,6 +464,60 @@ int cti_ebag_layernorm_linear(const void* x, int64_t rows, int32_t cols, const f
 /* Bytes of workspace cti_ebag_layernorm_linear uses at most for this shape, whatever the type of gamma
  * and beta (0: it never splits). */
 int64_t cti_ebag_layernorm_linear_workspace_bytes(int64_t rows, int32_t cols, int32_t out_features);
+
+/*
+ * The way back from cti_ebag_quantize_int8 and cti_ebag_norm_int8: out[r, j] = q[r, j] * scale[r] in fp32,
+ * rounded once to `out_dtype` (F32 / BF16 / F16). q int8 [rows, dim] and out [rows, dim] contiguous, scale
+ * fp32 [rows]; at most 2^40 elements.
+ */
+int cti_ebag_dequantize_int8(const int8_t* q, const float* scale, int64_t rows, int64_t dim, void* out,
+                             int32_t out_dtype, void* stream);
+
+/*
+ * A row norm with int8 output, in one pass over the rows:
+ *   h = x + residual                       (fp32; h = x without a residual; residual_out = h rounded to `dtype`)
+ *   CTI_EBAG_RMS_NORM:    y = h * rstd * gamma,                 rstd = 1/sqrt(sum(h^2)/cols + eps)
+ *   CTI_EBAG_LAYER_NORM:  y = (h - mean) * rstd * gamma + beta, rstd = 1/sqrt(sum((h - mean)^2)/cols + eps)
+ *   scale[r] = max(max_j |y_j| * RN32(1/127), 1e-8),  q[r, j] = clamp(rint(y_j / scale[r]), -128, 127)
+ * in fp32 (h unrounded), quantised as cti_ebag_quantize_int8 does it. A row whose statistics or normalised
+ * values are not all finite in fp32 gets scale NaN and q = 0: what is computed from it is NaN.
+ *   x, residual, residual_out  [rows, cols] contiguous, of `dtype` (F32 / BF16 / F16); residual and
+ *            residual_out both or neither; residual_out may be x or residual, else no two arrays overlap
+ *   gamma, beta  [cols] of `param_dtype` (beta ignored for the root-mean-square norm)
+ *   q        int8 [rows, cols] contiguous; scale fp32 [rows]
+ * Per-row results are deterministic for a given shape (fixed reduction order).
+ */
+int cti_ebag_norm_int8(int32_t kind, const void* x, const void* residual, void* residual_out, int64_t rows,
+                       int64_t cols, int32_t dtype, const void* gamma, const void* beta, int32_t param_dtype,
+                       float eps, int8_t* q, float* scale, void* stream);
+
+/*
+ * Linear in 8-bit integers, with a scale for each row of q (token) and each row of the weight (channel):
+ *   t[m, n] = sum_k q[m, k] * weight[n, k]                          (exact, int32)
+ *   v[m, n] = (t[m, n] * scale[m]) * weight_scale[n] + bias[n]      (fp32)
+ *   gate CTI_EBAG_GATE_NONE:  y[m, n] = v[m, n]
+ *   other gates:              y[m, n] = act(v[m, n]) * v[m, out_features + n], the two projections of a gated
+ *            feed-forward block and their product: weight, weight_scale and bias hold 2 * out_features rows,
+ *            the gates' first
+ * with one rounding to y's type.
+ *   q        int8 [rows, cols], scale fp32 [rows] (cti_ebag_norm_int8, cti_ebag_quantize_int8), contiguous
+ *   weight   int8 [out_features (gated: twice), cols] (nn.Linear's layout, quantised by row:
+ *            cti_ebag_quantize_int8), weight_scale fp32
+ *   bias     of `bias_dtype` F32 / BF16 / F16, or NULL
+ *   y        [rows, out_features] of `y_dtype` F32 / BF16 / F16, contiguous
+ *   workspace  device scratch of workspace_bytes (16-byte aligned), or NULL / 0: where few tiles would leave
+ *            CUs idle, K is split over several workgroups per tile, each writing int32 partial sums here,
+ *            and a second launch adds them; as many splits as the workspace holds, none without one
+ * cols at most 131071 (the int32 sums cannot overflow up to there), out_features at most 2^30. The integer
+ * sums are exact, so the result is the same bit for bit with any workspace.
+ */
+int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t rows, int32_t cols, const int8_t* weight,
+                         const float* weight_scale, int32_t out_features, const void* bias, int32_t bias_dtype,
+                         int32_t gate, void* y, int32_t y_dtype, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
+/* Bytes of workspace cti_ebag_linear_int8 uses at most for this shape (0: it never splits). */
+int64_t cti_ebag_linear_int8_workspace_bytes(int64_t rows, int32_t cols, int32_t out_features, int32_t gate);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,134 @@
+"""The int8 serving operators without a GPU: refusals of the C ABI and of the Python entry points (no HIP
+call is reached, the pointers are not real), and the dispatch rules of the int8 Linear."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "cti-inference-optimization_amd", "csrc")
+
+
+def _norm(c, **kw):
+    a = dict(kind=c.RMS_NORM, x=4096, res=None, out=None, rows=4, cols=64, dt=c.BF16, gamma=256, beta=256,
+             pdt=c.BF16, eps=1e-5, q=256, scale=256)
+    a.update(kw)
+    return c.lib().cti_ebag_norm_int8(a["kind"], a["x"], a["res"], a["out"], a["rows"], a["cols"], a["dt"], a["gamma"],
+                                      a["beta"], a["pdt"], a["eps"], a["q"], a["scale"], None)
+
+
+@pytest.mark.parametrize("kw,needle", [
+    (dict(kind=2), "norm"), (dict(rows=-1), "rows"), (dict(cols=0), "cols"), (dict(dt=3), "dtype"),
+    (dict(pdt=3), "parameter dtype"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
+    (dict(res=64), "together"), (dict(out=64), "together"), (dict(x=None), "NULL"), (dict(q=None), "NULL"),
+    (dict(scale=None), "NULL"), (dict(gamma=None), "NULL"), (dict(kind=1, beta=None), "beta"),
+    # 4 x 64 bf16 are 512 bytes: an output 2 bytes into an input, or 510 before it, overlaps it
+    (dict(res=65536, out=4098), "overlaps"), (dict(res=65536, out=65536 - 510), "overlaps"),
+])
+def test_norm_int8_rejects_bad_arguments(pkg, kw, needle):
+    assert _norm(pkg._capi, **kw) == pkg._capi.EINVAL
+    assert needle in pkg._capi.last_error()
+
+
+def test_norm_int8_limits(pkg):
+    c = pkg._capi
+    assert _norm(c, rows=0, x=None, q=None, scale=None, gamma=None) == c.OK
+    assert _norm(c, rows=2 ** 31) == c.EUNSUPPORTED
+
+
+def _linear(c, **kw):
+    a = dict(q=256, scale=256, rows=4, cols=64, w=256, ws=256, n=32, bias=None, bdt=c.F32, gate=c.GATE_NONE, y=256,
+             ydt=c.BF16, work=None, wb=0)
+    a.update(kw)
+    return c.lib().cti_ebag_linear_int8(a["q"], a["scale"], a["rows"], a["cols"], a["w"], a["ws"], a["n"], a["bias"],
+                                        a["bdt"], a["gate"], a["y"], a["ydt"], a["work"], a["wb"], None)
+
+
+@pytest.mark.parametrize("kw,needle", [
+    (dict(rows=-1), "rows"), (dict(cols=0), "cols"), (dict(n=0), "out_features"), (dict(gate=4), "gate"),
+    (dict(gate=-1), "gate"), (dict(ydt=3), "output dtype"), (dict(bias=64, bdt=3), "bias dtype"),
+    (dict(wb=-1), "workspace_bytes"), (dict(q=None), "NULL"), (dict(scale=None), "NULL"), (dict(w=None), "NULL"),
+    (dict(ws=None), "NULL"), (dict(y=None), "NULL"), (dict(work=8, wb=1 << 20), "aligned"),
+])
+def test_linear_int8_rejects_bad_arguments(pkg, kw, needle):
+    assert _linear(pkg._capi, **kw) == pkg._capi.EINVAL
+    assert needle in pkg._capi.last_error()
+
+
+def test_linear_int8_limits(pkg):
+    c = pkg._capi
+    assert _linear(c, rows=0, q=None, scale=None, y=None) == c.OK
+    assert _linear(c, cols=131072) == c.EUNSUPPORTED and "overflow" in c.last_error()
+    assert 131071 * 128 * 128 < 2 ** 31 <= 131072 * 128 * 128  # the largest |sum| at that width
+    assert _linear(c, rows=2 ** 31) == c.EUNSUPPORTED
+    assert _linear(c, n=2 ** 30 + 1) == c.EUNSUPPORTED
+    assert _linear(c, rows=2 ** 31 - 1, n=2 ** 30) == c.EUNSUPPORTED  # more tiles than a launch has
+
+
+def test_dequantize_int8_rejects_bad_arguments(pkg):
+    c = pkg._capi
+    f = c.lib().cti_ebag_dequantize_int8
+    #        q  scale rows dim out dtype stream
+    assert f(256, 256, 4, 8, 256, c.I8, None) == c.EINVAL and "dtype" in c.last_error()
+    assert f(256, 256, -1, 8, 256, c.BF16, None) == c.EINVAL and "rows" in c.last_error()
+    assert f(256, 256, 4, 0, 256, c.BF16, None) == c.EINVAL and "dim" in c.last_error()
+    assert f(256, None, 4, 8, 256, c.BF16, None) == c.EINVAL and "NULL" in c.last_error()
+    assert f(256, 256, 4, 8, 257, c.BF16, None) == c.EINVAL and "aligned" in c.last_error()
+    assert f(256, 256, 2 ** 30, 2 ** 11, 256, c.BF16, None) == c.EUNSUPPORTED
+    assert f(None, None, 0, 8, None, c.BF16, None) == c.OK
+
+
+def test_python_entry_points_validate_before_any_launch(pkg):
+    x, w, q, s = torch.zeros(4, 8), torch.ones(8), torch.zeros(4, 8, dtype=torch.int8), torch.ones(4)
+    for call in (lambda: pkg.rms_norm_int8(x, w), lambda: pkg.layer_norm_int8(x, w, w),
+                 lambda: pkg.linear_int8(q, s, q, s), lambda: pkg.gated_linear_int8(q, s, q, s),
+                 lambda: pkg.dequantize_embedding_int8(q, s)):
+        with pytest.raises(ValueError, match="GPU tensor"):
+            call()
+    with pytest.raises(ValueError, match="activation"):
+        pkg.gated_linear_int8(q, s, q, s, activation="tanh")
+
+
+# ------------------------------------------------------------------------------------------------
+# Dispatch
+# ------------------------------------------------------------------------------------------------
+@pytest.fixture(scope="module")
+def rules(tmp_path_factory):
+    work = tmp_path_factory.mktemp("rules8")
+    (work / "rules.cpp").write_text(
+        '#include "ebag_rules.h"\n'
+        'extern "C" int plan(int64_t M, int32_t N, int32_t K, int gated, int64_t ws, int* splits, int* steps,\n'
+        "                    int64_t* part, int64_t* groups) {\n"
+        "  const cti::Linear8Plan p = cti::linear8_plan(M, N, K, gated != 0, ws);\n"
+        "  *splits = p.splits;\n  *steps = p.steps;\n"
+        "  *part = cti::linear8_part_bytes(p, M, N, gated != 0);\n"
+        "  *groups = cti::linear8_workgroups(p, M, N, gated != 0);\n  return p.form;\n}\n")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", f"-I{CSRC}",
+                    str(work / "rules.cpp"), "-o", str(work / "rules.so")], check=True)
+    lib = ctypes.CDLL(str(work / "rules.so"))
+    I, P = ctypes.c_int64, ctypes.POINTER
+    lib.plan.argtypes = [I, ctypes.c_int32, ctypes.c_int32, ctypes.c_int, I, P(ctypes.c_int), P(ctypes.c_int), P(I), P(I)]
+
+    def plan(M, N, K, gated, ws):
+        out = ctypes.c_int(), ctypes.c_int(), I(), I()
+        form = lib.plan(M, N, K, gated, ws, *(ctypes.byref(o) for o in out))
+        return (form, *(o.value for o in out))
+
+    return plan
+
+
+@pytest.mark.parametrize("gated", [0, 1])
+def test_the_splits_cover_k_and_fit_the_workspace(rules, pkg, gated):
+    for M in (1, 16, 17, 32, 33, 64, 65, 100, 128, 500, 2048, 70000):
+        for N in (1, 16, 500, 512, 4096, 14336):
+            for K in (1, 16, 127, 128, 129, 1021, 3584, 14336, 131071):
+                query = pkg._capi.lib().cti_ebag_linear_int8_workspace_bytes(M, K, N, gated)
+                for ws in (0, 1000, M * N * (8 if gated else 4) * 3, query, 1 << 40):
+                    _, splits, steps, part, groups = rules(M, N, K, gated, ws)
+                    nk = -(-K // 128)
+                    assert splits >= 1 and steps >= 1 and groups >= 1
+                    assert (splits - 1) * steps < nk <= splits * steps  # every split has work, all of it is done
+                    assert part <= max(0, min(ws, query))
+                    assert part == (0 if splits == 1 else splits * M * N * (8 if gated else 4))
