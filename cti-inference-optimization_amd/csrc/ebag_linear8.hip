@@ -32,6 +32,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef i32x4 i32x4_any __attribute__((aligned(1)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 constexpr int kStep = kLinear8Step;  // bytes of K per step
 constexpr int kXcds = 8;
@@ -66,84 +67,177 @@ __device__ __forceinline__ float load_bias(const Linear8Params& p, int n) {
 }
 
 // act(g) in fp32: silu with exp(-|g|), which cannot overflow; gelu with erfc, without the cancellation of 1 + erf.
-__device__ __forceinline__ float activate(float g, int gate) {
-  switch (gate) {
-    case CTI_EBAG_GATE_SILU: {
-      const float e = expf(-fabsf(g));
-      return (g < 0.f ? g * e : g) / (1.0f + e);
-    }
-    case CTI_EBAG_GATE_GELU: return 0.5f * g * erfcf(g * -0.70710678118654752f);
-    default: return g < 0.f ? 0.f : g;  // NaN stays NaN
+template <int GATE>
+__device__ __forceinline__ float activate(float g) {
+  if constexpr (GATE == CTI_EBAG_GATE_SILU) {
+    const float e = expf(-fabsf(g));
+    return (g < 0.f ? g * e : g) / (1.0f + e);
+  } else if constexpr (GATE == CTI_EBAG_GATE_GELU) {
+    return 0.5f * g * erfcf(g * -0.70710678118654752f);
+  } else {
+    return g < 0.f ? 0.f : g;  // NaN stays NaN
   }
 }
 
-// Weight scales and bias of 4 consecutive columns from `row` of the weight on (`live` of them exist).
+// Weight scales and bias of C (a multiple of 4) consecutive columns from `row` of the weight on, `live` of which
+// exist (1 at least; the others repeat the last).
+template <int C>
 struct Columns {
-  f32x4 scale, bias;
+  float scale[C], bias[C];
   __device__ __forceinline__ void load(const Linear8Params& p, int row, int live) {
+    if (live >= C) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int n = row + (r < live ? r : live - 1);
-      scale[r] = p.wscale[n];
-      bias[r] = p.bias ? load_bias(p, n) : 0.f;
+      for (int i = 0; i < C; i += 4) {
+        const f32x4 v = *reinterpret_cast<const f32x4_any*>(p.wscale + row + i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) scale[i + r] = v[r];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) scale[i] = p.wscale[row + (i < live ? i : live - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) bias[i] = 0.f;
+    if (p.bias) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) bias[i] = load_bias(p, row + (i < live ? i : live - 1));
     }
   }
-  __device__ __forceinline__ f32x4 apply(const i32x4& t, float sm) const {
-    f32x4 v;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = static_cast<float>(t[r]) * sm * scale[r] + bias[r];
-    return v;
+  __device__ __forceinline__ float apply(int i, int t, float sm) const {
+    return static_cast<float>(t) * sm * scale[i] + bias[i];
   }
 };
 
-// y[m][n .. n + 4) (those below N).
-__device__ __forceinline__ void store_y4(const Linear8Params& p, int64_t m, int n, const f32x4& v) {
-  const int64_t at = m * p.N + n;
-  const int live = p.N - n;
-  if (p.y_dtype == CTI_EBAG_F32) {
-    float* const y = reinterpret_cast<float*>(p.y) + at;
-    if (live >= 4) {
-      *reinterpret_cast<f32x4_any*>(y) = v;
+// y[i], i < live, of C consecutive columns, rounded to YT.
+template <typename YT, int C>
+__device__ __forceinline__ void store_columns(char* y, int64_t at, const float* v, int live) {
+  if constexpr (std::is_same<YT, float>::value) {
+    float* const to = reinterpret_cast<float*>(y) + at;
+    if (live >= C) {
+#pragma unroll
+      for (int i = 0; i < C; i += 4) *reinterpret_cast<f32x4_any*>(to + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
     } else {
 #pragma unroll
-      for (int r = 0; r < 3; ++r)
-        if (r < live) y[r] = v[r];
+      for (int i = 0; i < C - 1; ++i)
+        if (i < live) to[i] = v[i];
+    }
+  } else {
+    uint32_t w[C / 2];
+#pragma unroll
+    for (int i = 0; i < C / 2; ++i)
+      w[i] = std::is_same<YT, bf16_t>::value ? pack_bf16x2(v[2 * i], v[2 * i + 1]) : pack_f16x2(v[2 * i], v[2 * i + 1]);
+    uint16_t* const to = reinterpret_cast<uint16_t*>(y) + at;
+    if (live >= C) {
+      if constexpr (C % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < C / 2; i += 4) *reinterpret_cast<u32x4_any*>(to + 2 * i) = u32x4{w[i], w[i + 1], w[i + 2], w[i + 3]};
+      } else {
+#pragma unroll
+        for (int i = 0; i < C / 2; i += 2) *reinterpret_cast<u32x2_any*>(to + 2 * i) = u32x2{w[i], w[i + 1]};
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C - 1; ++i)
+        if (i < live) to[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i % 2)));
+    }
+  }
+}
+
+// Runs f(gate) with the gate as a constant: one copy of what f unrolls for each.
+template <bool GATED, typename F>
+__device__ __forceinline__ void with_gate(const Linear8Params& p, F&& f) {
+  if constexpr (!GATED) {
+    f(std::integral_constant<int, CTI_EBAG_GATE_NONE>{});
+  } else {
+    switch (p.gate) {
+      case CTI_EBAG_GATE_SILU: f(std::integral_constant<int, CTI_EBAG_GATE_SILU>{}); break;
+      case CTI_EBAG_GATE_GELU: f(std::integral_constant<int, CTI_EBAG_GATE_GELU>{}); break;
+      default: f(std::integral_constant<int, CTI_EBAG_GATE_RELU>{}); break;
+    }
+  }
+}
+
+// C consecutive columns of a row from the sums t (gated: gates) and u (values).
+template <typename YT, int GATE, int C>
+__device__ __forceinline__ void emit(const Linear8Params& p, int64_t m, int n, int live, float sm, const Columns<C>& a,
+                                     const Columns<C>& b, const int* t, const int* u) {
+  float v[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    v[i] = a.apply(i, t[i], sm);
+    if constexpr (GATE != CTI_EBAG_GATE_NONE) v[i] = activate<GATE>(v[i]) * b.apply(i, u[i], sm);
+  }
+  store_columns<YT, C>(p.y, m * p.N + n, v, live);
+}
+
+// A wavefront's sums to y, or to this split's partial sums: lane l holds rows m0 + 16 a + l % 16 and of them C
+// columns side by side from n on (`live` of which exist) in acc[a][f * C / 4 ..], gated: the values' behind the gates'.
+// Scales are loaded at once and before the first is used: one at a time, between the stores, they took longer than
+// 64 steps of products.
+template <typename YT, bool GATED, int MI, int NO, int G, typename ColOf>
+__device__ __forceinline__ void epilogue(const Linear8Params& p, int64_t m0, ColOf&& col_of,
+                                         const i32x4 (&acc)[MI][GATED ? 2 * NO : NO], int split) {
+  constexpr int C = 4 * G, GROUPS = NO / G;
+  const int fr = lane_id() & 15;
+  const auto sums = [&](int a, int f, int* t) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) t[i] = acc[a][f + i / 4][i % 4];
+  };
+  if (p.part) {
+    const int64_t width = static_cast<int64_t>(p.N) * (GATED ? 2 : 1);
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+      const int n = col_of(g), live = p.N - n;
+      if (live <= 0) continue;
+      int32_t* const part = p.part + split * p.M * width + n;
+#pragma unroll
+      for (int a = 0; a < MI; ++a) {
+        const int64_t m = m0 + a * 16 + fr;
+        if (m >= p.M) continue;
+#pragma unroll
+        for (int half = 0; half < (GATED ? 2 : 1); ++half) {
+          int32_t* const to = part + m * width + static_cast<int64_t>(half) * p.N;
+#pragma unroll
+          for (int i = 0; i < C; i += 4) {
+            const i32x4 v = acc[a][half * NO + g * G + i / 4];
+            if (live >= C) {
+              *reinterpret_cast<i32x4_any*>(to + i) = v;
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (i + r < live) to[i + r] = v[r];
+            }
+          }
+        }
+      }
     }
     return;
   }
-  const bool bf = p.y_dtype == CTI_EBAG_BF16;
-  const u32x2 w = bf ? u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}
-                     : u32x2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])};
-  uint16_t* const y = reinterpret_cast<uint16_t*>(p.y) + at;
-  if (live >= 4) {
-    *reinterpret_cast<u32x2_any*>(y) = w;
-  } else {
+  float sm[MI];
 #pragma unroll
-    for (int r = 0; r < 3; ++r)
-      if (r < live) y[r] = static_cast<uint16_t>(w[r / 2] >> (16 * (r % 2)));
+  for (int a = 0; a < MI; ++a) {
+    const int64_t m = m0 + a * 16 + fr;
+    sm[a] = p.scale[m < p.M ? m : p.M - 1];
+  }
+#pragma unroll
+  for (int g = 0; g < GROUPS; ++g) {
+    const int n = col_of(g), live = p.N - n;
+    if (live <= 0) continue;
+    Columns<C> ca, cb;
+    ca.load(p, n, live);
+    if constexpr (GATED) cb.load(p, p.N + n, live);
+    with_gate<GATED>(p, [&](auto gate) {
+#pragma unroll
+      for (int a = 0; a < MI; ++a) {
+        const int64_t m = m0 + a * 16 + fr;
+        int t[C], u[C];
+        sums(a, g * G, t);
+        sums(a, (GATED ? NO : 0) + g * G, u);
+        if (m < p.M) emit<YT, decltype(gate)::value, C>(p, m, n, live, sm[a], ca, cb, t, u);
+      }
+    });
   }
 }
-
-template <bool GATED>
-struct Epilogue {
-  Columns a, b;  // b: the values' columns of the gated form
-  int n;
-  __device__ __forceinline__ void load(const Linear8Params& p, int col) {
-    n = col;
-    const int live = p.N - n < 4 ? p.N - n : 4;
-    a.load(p, n, live);
-    if constexpr (GATED) b.load(p, p.N + n, live);
-  }
-  __device__ __forceinline__ void emit(const Linear8Params& p, int64_t m, float sm, const i32x4& t, const i32x4& u) const {
-    f32x4 v = a.apply(t, sm);
-    if constexpr (GATED) {
-      const f32x4 w = b.apply(u, sm);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = activate(v[r], p.gate) * w[r];
-    }
-    store_y4(p, m, n, v);
-  }
-};
 
 // ---------------------------------------------------------------------------------------------
 // Loads
@@ -162,7 +256,7 @@ __device__ __forceinline__ i32x4 load_chunk(const int8_t* row, int k, int K) {
 // ---------------------------------------------------------------------------------------------
 // Few rows (M <= 16 MT)
 // ---------------------------------------------------------------------------------------------
-template <int W, int MT, bool GATED>
+template <typename YT, int W, int MT, bool GATED>
 __global__ void __launch_bounds__(W * kWave) linear8_rows_kernel(const Linear8Params p) {
   constexpr int NT = GATED ? 2 : 1;
   __shared__ i32x4 s_acc[W > 1 ? W : 1][MT * NT][kWave];
@@ -219,15 +313,13 @@ __global__ void __launch_bounds__(W * kWave) linear8_rows_kernel(const Linear8Pa
 #pragma unroll
         for (int i = 1; i < W; ++i) acc[c][a] += s_acc[i][a * NT + c][lane];
   }
-  const int n = n0 + fq * 4;
-  if (n >= p.N) return;
-  Epilogue<GATED> ep;
-  ep.load(p, n);
+  // lane l holds columns 4 (l / 16) .. + 4 of row l % 16
+  i32x4 sums[MT][NT];
 #pragma unroll
-  for (int a = 0; a < MT; ++a) {
-    const int64_t m = a * 16 + fr;
-    if (m < p.M) ep.emit(p, m, p.scale[m], acc[0][a], acc[NT - 1][a]);
-  }
+  for (int a = 0; a < MT; ++a)
+#pragma unroll
+    for (int c = 0; c < NT; ++c) sums[a][c] = acc[c][a];
+  epilogue<YT, GATED, MT, 1, 1>(p, 0, [&](int) { return n0 + fq * 4; }, sums, 0);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -247,7 +339,7 @@ __device__ __forceinline__ void tile_of(const Linear8Params& p, int* tm, int* tn
   *tn = rest / rows;
 }
 
-template <int BM, int BN, int WM, int WN, bool GATED>
+template <typename YT, int BM, int BN, int WM, int WN, bool GATED>
 __global__ void __launch_bounds__(WM * WN * kWave) linear8_tile_kernel(const Linear8Params p) {
   constexpr int THREADS = WM * WN * kWave;
   constexpr int TM = BM / WM, TN = BN / WN;     // a wavefront's rows and weight rows
@@ -337,68 +429,230 @@ __global__ void __launch_bounds__(WM * WN * kWave) linear8_tile_kernel(const Lin
     if (s + 1 < nk) put(buf ^ 1);
     __syncthreads();
   }
+  epilogue<YT, GATED, MI, NO, 1>(p, m0 + wm * TM, [&](int g) { return n0 + wn * NO * 16 + g * 16 + fq * 4; }, acc,
+                                 static_cast<int>(blockIdx.y));
+}
+
+// ---------------------------------------------------------------------------------------------
+// Large tiles (K a multiple of 16, 16-byte aligned operands): loads straight to LDS
+// ---------------------------------------------------------------------------------------------
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+__device__ __forceinline__ Rsrc make_rsrc(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), static_cast<short>(0), static_cast<int>(bytes),
+                                           0x00020000);  // raw buffer, 32-bit data format
+}
+// 16 bytes per lane straight to LDS, lane l's to lds + 16 l (lds the same for every lane).
+__device__ __forceinline__ void load_lds(Rsrc r, i32x4* lds, uint32_t voff, uint32_t soff) {
+#ifdef __HIP_DEVICE_COMPILE__  // the host pass has no 16-byte form
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, voff, soff, 0, 0);
+#endif
+}
+// Waits until at most N of this wavefront's loads are in flight, and for its LDS reads; then the barrier.
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");  // no instruction: keeps the compiler's order
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4 << 14));  // vmcnt(N) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <typename YT, int WM, int WN, bool GATED, bool TAIL>
+__global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_big_kernel(const Linear8Params p) {
+  constexpr int BM = 256, BN = 256, WAVES = WM * WN;
+  constexpr int TM = BM / WM, TN = BN / WN;
+  constexpr int MI = TM / 16, NI = TN / 16;
+  constexpr int kChunks = kStep / 16;
+  constexpr int PX = BM / 8 / WAVES, PW = BN / 8 / WAVES;  // loads per thread and step, 8 rows a wavefront each
+  constexpr int OUT = GATED ? BN / 2 : BN;
+  constexpr int NO = GATED ? NI / 2 : NI;    // fragments of output columns
+  constexpr int G = NO < 4 ? NO : 4;         // of them side by side: a lane holds 4 G columns of a row
+  // rows of 128 bytes, chunk c of row r in slot c ^ (r & 7) (no bank conflicts)
+  __shared__ i32x4 s0[(BM + BN) * kChunks], s1[(BM + BN) * kChunks];
+  int tm, tn;
+  tile_of(p, &tm, &tn);
+  const int64_t m0 = static_cast<int64_t>(tm) * BM;
+  const int n0 = tn * OUT;
+  const int t = static_cast<int>(threadIdx.x);
+  const int lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int wm = wave / WN, wn = wave % WN;
+  const int fr = lane & 15, fq = lane >> 4;
+
+  const int nk_all = (p.K + kStep - 1) / kStep;
+  const int ks0 = p.part ? static_cast<int>(blockIdx.y) * p.split_steps : 0;
+  const int nk = p.part ? (nk_all - ks0 < p.split_steps ? nk_all - ks0 : p.split_steps) : nk_all;
+
+  // rows past M, weight rows past N and chunks past the last row's end lie past the buffers: nothing is read (a
+  // chunk past the end of another row is the next row's; either is masked or multiplies what is not stored)
+  const int64_t mrows = p.M - m0 < BM ? p.M - m0 : BM;
+  const int64_t nrows = p.N - n0 < OUT ? p.N - n0 : OUT;
+  const Rsrc xr = make_rsrc(p.x + m0 * p.K, static_cast<uint32_t>(mrows * p.K));
+  const Rsrc wr = make_rsrc(p.w + static_cast<int64_t>(n0) * p.K, static_cast<uint32_t>(nrows * p.K));
+  const Rsrc ur = make_rsrc(p.w + (static_cast<int64_t>(GATED ? p.N : 0) + n0) * p.K, static_cast<uint32_t>(nrows * p.K));
+  // load q of wavefront w fills LDS rows 8 (w PX + q) .. + 8, lane l chunk l % 8 of row l / 8 there
+  uint32_t xoff[PX], woff[PW];
+  const int chunk = (lane & 7) ^ (lane >> 3);
 #pragma unroll
-  for (int c = 0; c < NO; ++c) {
-    const int n = n0 + wn * NO * 16 + c * 16 + fq * 4;
-    if (n >= p.N) continue;
-    if (p.part) {
-      const int64_t width = static_cast<int64_t>(p.N) * (GATED ? 2 : 1);
-      int32_t* const part = p.part + static_cast<int64_t>(blockIdx.y) * p.M * width + n;
+  for (int q = 0; q < PX; ++q) xoff[q] = static_cast<uint32_t>((wave * PX + q) * 8 + lane / 8) * p.K + chunk * 16;
 #pragma unroll
-      for (int a = 0; a < MI; ++a) {
-        const int64_t m = m0 + wm * TM + a * 16 + fr;
-        if (m >= p.M) continue;
-#pragma unroll
-        for (int half = 0; half < (GATED ? 2 : 1); ++half)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n + r < p.N) part[m * width + static_cast<int64_t>(half) * p.N + r] = acc[a][half * NO + c][r];
-      }
-      continue;
-    }
-    Epilogue<GATED> ep;
-    ep.load(p, n);
-#pragma unroll
-    for (int a = 0; a < MI; ++a) {
-      const int64_t m = m0 + wm * TM + a * 16 + fr;
-      if (m < p.M) ep.emit(p, m, p.scale[m], acc[a][c], acc[a][GATED ? NO + c : c]);
-    }
+  for (int q = 0; q < PW; ++q) {
+    // LDS row 16 f + i of a wavefront column holds column 16 (i / 4) + 4 (f % 4) + i % 4 of 64 (gated: fragments
+    // f < NO gates, the others their values), so that a lane receives 4 G columns side by side
+    const int j = (wave * PW + q) * 8 + lane / 8, f = j % TN / 16 % NO, i = j % 16;
+    const int c = j / TN * (NO * 16) + f / G * (16 * G) + 4 * G * (i / 4) + 4 * (f % G) + i % 4;
+    woff[q] = static_cast<uint32_t>(c) * p.K + chunk * 16;
   }
+  const auto issue = [&](int s, i32x4* to) {
+    const int k = (ks0 + (s < nk ? s : nk - 1)) * kStep;  // later steps are never used
+#pragma unroll
+    for (int q = 0; q < PX; ++q) load_lds(xr, to + (wave * PX + q) * kWave, xoff[q], k);
+#pragma unroll
+    for (int q = 0; q < PW; ++q) {
+      const int f = (wave * PW + q) / 2 % NI;
+      load_lds(GATED && f >= NO ? ur : wr, to + BM * kChunks + (wave * PW + q) * kWave, woff[q], k);
+    }
+  };
+  i32x4 fx[2][MI], fw[2][NI];
+  const auto read = [&](const i32x4* from, auto half) {
+    constexpr int h = decltype(half)::value;
+    const int slot = fr * kChunks + ((h * 4 + fq) ^ (fr & 7));
+#pragma unroll
+    for (int c = 0; c < NI; ++c) fw[h][c] = from[BM * kChunks + (wn * TN + c * 16) * kChunks + slot];
+#pragma unroll
+    for (int a = 0; a < MI; ++a) fx[h][a] = from[(wm * TM + a * 16) * kChunks + slot];
+  };
+  i32x4 acc[MI][NI];
+#pragma unroll
+  for (int a = 0; a < MI; ++a)
+#pragma unroll
+    for (int c = 0; c < NI; ++c) acc[a][c] = i32x4{0, 0, 0, 0};
+  const auto multiply = [&](auto half) {
+    constexpr int h = decltype(half)::value;
+#pragma unroll
+    for (int a = 0; a < MI; ++a)
+#pragma unroll
+      for (int c = 0; c < NI; ++c)
+        acc[a][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[h][c], fx[h][a], acc[a][c], 0, 0, 0);
+  };
+  constexpr std::integral_constant<int, 0> first{};
+  constexpr std::integral_constant<int, 1> second{};
+  constexpr int L = PX + PW;
+  issue(0, s0);
+  issue(1, s1);
+  wait_barrier<L>();
+  read(s0, first);
+  // Step s: the first half's fragments are in registers (or on their way), the second half's are read while the
+  // first is multiplied. Once every wavefront has them and step s + 1 has arrived, the second half is multiplied
+  // while step s + 2 is loaded over step s and the next step's first half is read.
+  const auto step = [&](int s, i32x4* mine, const i32x4* next, auto endc) {
+    constexpr bool end = decltype(endc)::value;
+    const int left = p.K - (ks0 + s) * kStep;  // bytes of K from this step on
+    const auto mask = [&](int h) {
+      if (end && s == nk - 1 && left < kStep) {
+#pragma unroll
+        for (int a = 0; a < MI; ++a)
+          if (h * 64 + fq * 16 >= left) fx[h][a] = i32x4{0, 0, 0, 0};
+      }
+    };
+    mask(0);
+    read(mine, second);
+    multiply(first);
+#pragma unroll
+    for (int i = 0; i < (MI + NI) / 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);    // products
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+    }
+    wait_barrier<0>();
+    mask(1);
+    issue(s + 2, mine);
+    read(next, first);
+    multiply(second);
+#pragma unroll
+    for (int i = 0; i < L / 2; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, 3, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);   // load
+      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // one way out of the loop: the compiler then knows at its head which loads to LDS are in flight, and adds no wait
+  constexpr std::integral_constant<bool, false> inside{};
+  constexpr std::integral_constant<bool, TAIL> end{};
+  int s = 0;
+  for (; s + 2 <= (TAIL ? nk - 1 : nk); s += 2) {
+    step(s, s0, s1, inside);
+    step(s + 1, s1, s0, inside);
+  }
+  if (s < nk) {
+    step(s, s0, s1, end);
+    if (TAIL && s + 1 < nk) step(s + 1, s1, s0, end);
+  }
+  epilogue<YT, GATED, MI, NO, G>(p, m0 + wm * TM, [&](int g) { return n0 + wn * (NO * 16) + g * (16 * G) + fq * (4 * G); },
+                                 acc, static_cast<int>(blockIdx.y));
 }
 
 // Split K: the splits' sums added, scales, bias, gate and rounding as in the tiles' epilogue; 4 columns a thread.
 constexpr int kReduceThreads = 256;
-template <bool GATED>
+template <typename YT, bool GATED>
 __global__ void __launch_bounds__(kReduceThreads) linear8_reduce_kernel(const Linear8Params p, int splits) {
   const int quads = (p.N + 3) / 4;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kReduceThreads + threadIdx.x;
   const int64_t m = i / quads;
   if (m >= p.M) return;
-  const int n = static_cast<int>(i - m * quads) * 4;
-  const int64_t width = static_cast<int64_t>(p.N) * (GATED ? 2 : 1);
-  i32x4 t[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  const int n = static_cast<int>(i - m * quads) * 4, live = p.N - n;
+  const int64_t width = static_cast<int64_t>(p.N) * (GATED ? 2 : 1), each = p.M * width;
+  int t[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
   for (int half = 0; half < (GATED ? 2 : 1); ++half) {
-    const int32_t* from = p.part + m * width + static_cast<int64_t>(half) * p.N + n;
-    for (int s = 0; s < splits; ++s, from += p.M * width)
+    const int32_t* const from = p.part + m * width + static_cast<int64_t>(half) * p.N + n;
+    if (live >= 4) {
+#pragma unroll 4
+      for (int s = 0; s < splits; ++s) {
+        const i32x4 v = *reinterpret_cast<const i32x4_any*>(from + s * each);
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (n + r < p.N) t[half][r] += from[r];
+        for (int r = 0; r < 4; ++r) t[half][r] += v[r];
+      }
+    } else {
+      for (int s = 0; s < splits; ++s)
+#pragma unroll
+        for (int r = 0; r < 3; ++r)
+          if (r < live) t[half][r] += from[s * each + r];
+    }
   }
-  Epilogue<GATED> ep;
-  ep.load(p, n);
-  ep.emit(p, m, p.scale[m], t[0], t[1]);
+  Columns<4> ca, cb;
+  ca.load(p, n, live);
+  if constexpr (GATED) cb.load(p, p.N + n, live);
+  with_gate<GATED>(p, [&](auto gate) {
+    emit<YT, decltype(gate)::value, 4>(p, m, n, live, p.scale[m], ca, cb, t[0], t[1]);
+  });
 }
 
 // ---------------------------------------------------------------------------------------------
 // Launch
 // ---------------------------------------------------------------------------------------------
-template <bool GATED>
+template <typename YT, bool GATED>
 hipError_t launch(Linear8Params p, const Linear8Plan& plan, hipStream_t s) {
   if (plan.form == kLinear8Rows) {
     const dim3 grid(static_cast<unsigned>((p.N + 15) / 16));
-    if (p.M <= 16) hipLaunchKernelGGL((linear8_rows_kernel<8, 1, GATED>), grid, dim3(8 * kWave), 0, s, p);
-    else hipLaunchKernelGGL((linear8_rows_kernel<8, 2, GATED>), grid, dim3(8 * kWave), 0, s, p);
+    p.part = nullptr;
+    if (p.M <= 16) hipLaunchKernelGGL((linear8_rows_kernel<YT, 8, 1, GATED>), grid, dim3(8 * kWave), 0, s, p);
+    else hipLaunchKernelGGL((linear8_rows_kernel<YT, 8, 2, GATED>), grid, dim3(8 * kWave), 0, s, p);
+    return hipGetLastError();
+  }
+  if (p.M > 1024 && p.K % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0) {
+    p.tiles_m = static_cast<int32_t>((p.M + 255) / 256);
+    p.tiles_n = (p.N + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
+    p.part = nullptr;
+    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.tiles_m) * p.tiles_n));
+    if (p.K % kStep == 0) hipLaunchKernelGGL((linear8_big_kernel<YT, 2, 4, GATED, false>), grid, dim3(8 * kWave), 0, s, p);
+    else hipLaunchKernelGGL((linear8_big_kernel<YT, 2, 4, GATED, true>), grid, dim3(8 * kWave), 0, s, p);
     return hipGetLastError();
   }
   constexpr int BM = 128, BN = 128, OUT = GATED ? BN / 2 : BN;
@@ -407,15 +661,24 @@ hipError_t launch(Linear8Params p, const Linear8Plan& plan, hipStream_t s) {
   p.split_steps = plan.steps;
   if (plan.splits <= 1) p.part = nullptr;
   const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.tiles_m) * p.tiles_n), static_cast<unsigned>(plan.splits));
-  hipLaunchKernelGGL((linear8_tile_kernel<BM, BN, 2, 2, GATED>), grid, dim3(4 * kWave), 0, s, p);
+  hipLaunchKernelGGL((linear8_tile_kernel<YT, BM, BN, 2, 2, GATED>), grid, dim3(4 * kWave), 0, s, p);
   if (p.part) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int64_t threads = p.M * ((p.N + 3) / 4);
-    hipLaunchKernelGGL((linear8_reduce_kernel<GATED>), dim3(static_cast<unsigned>((threads + kReduceThreads - 1) / kReduceThreads)),
+    hipLaunchKernelGGL((linear8_reduce_kernel<YT, GATED>), dim3(static_cast<unsigned>((threads + kReduceThreads - 1) / kReduceThreads)),
                        dim3(kReduceThreads), 0, s, p, plan.splits);
   }
   return hipGetLastError();
+}
+
+template <bool GATED>
+hipError_t launch_typed(const Linear8Params& p, const Linear8Plan& plan, hipStream_t s) {
+  switch (p.y_dtype) {
+    case CTI_EBAG_F32: return launch<float, GATED>(p, plan, s);
+    case CTI_EBAG_BF16: return launch<bf16_t, GATED>(p, plan, s);
+    default: return launch<f16_t, GATED>(p, plan, s);
+  }
 }
 
 bool float_dtype(int32_t dt) { return dt == CTI_EBAG_F32 || dt == CTI_EBAG_BF16 || dt == CTI_EBAG_F16; }
@@ -475,7 +738,7 @@ extern "C" int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t
   p.y_dtype = y_dtype;
   p.gate = gate;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const hipError_t e = gated ? launch<true>(p, plan, s) : launch<false>(p, plan, s);
+  const hipError_t e = gated ? launch_typed<true>(p, plan, s) : launch_typed<false>(p, plan, s);
   if (e != hipSuccess) return set_error(CTI_EBAG_EHIP, "linear launch failed: %s", hipGetErrorString(e));
   return CTI_EBAG_OK;
 }
