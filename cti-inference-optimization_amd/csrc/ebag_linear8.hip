@@ -44,10 +44,11 @@ struct Linear8Params {
   const float* wscale;  // [N or 2 N]
   const void* bias;     // [N or 2 N] or NULL
   char* y;              // [M, N]
-  int32_t* part;        // split K: int32 partial sums [splits, M, N or 2 N]; NULL: no split
+  int32_t* part;        // split K: int32 partial sums [splits, M, columns of this launch (gated: twice)]; NULL: no split
   int64_t M;
   int32_t N;            // columns of y
-  int32_t K;
+  int32_t K;            // bytes of a row of x and w
+  int32_t n_begin, n_end;  // columns of y of this launch
   int32_t tiles_m, tiles_n;
   int32_t split_steps;  // split K: steps per split; split s is blockIdx.y
   int32_t bias_dtype, y_dtype;
@@ -170,36 +171,31 @@ __device__ __forceinline__ void emit(const Linear8Params& p, int64_t m, int n, i
   store_columns<YT, C>(p.y, m * p.N + n, v, live);
 }
 
-// A wavefront's sums to y, or to this split's partial sums: lane l holds rows m0 + 16 a + l % 16 and of them C
-// columns side by side from n on (`live` of which exist) in acc[a][f * C / 4 ..], gated: the values' behind the gates'.
-// Scales are loaded at once and before the first is used: one at a time, between the stores, they took longer than
-// 64 steps of products.
-template <typename YT, bool GATED, int MI, int NO, int G, typename ColOf>
-__device__ __forceinline__ void epilogue(const Linear8Params& p, int64_t m0, ColOf&& col_of,
-                                         const i32x4 (&acc)[MI][GATED ? 2 * NO : NO], int split) {
-  constexpr int C = 4 * G, GROUPS = NO / G;
-  const int fr = lane_id() & 15;
-  const auto sums = [&](int a, int f, int* t) {
-#pragma unroll
-    for (int i = 0; i < C; ++i) t[i] = acc[a][f + i / 4][i % 4];
-  };
+// A wavefront's sums to y, or to this split's partial sums: lane l holds rows m0 + R a + l % R, a < MI, and of each
+// GROUPS times C columns side by side from col_of(g) on; sum(a, g, half, i) is the sum of column i of group g (half 1:
+// of the gated form's values). Scales are loaded at once and before the first is used: one at a time, between the
+// stores, they took 38 us a 256 x 256 tile, longer than 8,192 of K.
+template <typename YT, bool GATED, int R, int MI, int GROUPS, int C, typename ColOf, typename Sum>
+__device__ __forceinline__ void epilogue(const Linear8Params& p, int64_t m0, ColOf&& col_of, Sum&& sum, int split) {
+  constexpr int H = GATED ? 2 : 1;
+  const int row = lane_id() % R;
   if (p.part) {
-    const int64_t width = static_cast<int64_t>(p.N) * (GATED ? 2 : 1);
+    const int64_t cols = p.n_end - p.n_begin, width = cols * H;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
-      const int n = col_of(g), live = p.N - n;
+      const int n = col_of(g), live = p.n_end - n;
       if (live <= 0) continue;
-      int32_t* const part = p.part + split * p.M * width + n;
+      int32_t* const part = p.part + split * p.M * width + n - p.n_begin;
 #pragma unroll
       for (int a = 0; a < MI; ++a) {
-        const int64_t m = m0 + a * 16 + fr;
+        const int64_t m = m0 + a * R + row;
         if (m >= p.M) continue;
 #pragma unroll
-        for (int half = 0; half < (GATED ? 2 : 1); ++half) {
-          int32_t* const to = part + m * width + static_cast<int64_t>(half) * p.N;
+        for (int half = 0; half < H; ++half) {
+          int32_t* const to = part + m * width + half * cols;
 #pragma unroll
           for (int i = 0; i < C; i += 4) {
-            const i32x4 v = acc[a][half * NO + g * G + i / 4];
+            const i32x4 v = {sum(a, g, half, i), sum(a, g, half, i + 1), sum(a, g, half, i + 2), sum(a, g, half, i + 3)};
             if (live >= C) {
               *reinterpret_cast<i32x4_any*>(to + i) = v;
             } else {
@@ -216,12 +212,12 @@ __device__ __forceinline__ void epilogue(const Linear8Params& p, int64_t m0, Col
   float sm[MI];
 #pragma unroll
   for (int a = 0; a < MI; ++a) {
-    const int64_t m = m0 + a * 16 + fr;
+    const int64_t m = m0 + a * R + row;
     sm[a] = p.scale[m < p.M ? m : p.M - 1];
   }
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
-    const int n = col_of(g), live = p.N - n;
+    const int n = col_of(g), live = p.n_end - n;
     if (live <= 0) continue;
     Columns<C> ca, cb;
     ca.load(p, n, live);
@@ -229,10 +225,13 @@ __device__ __forceinline__ void epilogue(const Linear8Params& p, int64_t m0, Col
     with_gate<GATED>(p, [&](auto gate) {
 #pragma unroll
       for (int a = 0; a < MI; ++a) {
-        const int64_t m = m0 + a * 16 + fr;
+        const int64_t m = m0 + a * R + row;
         int t[C], u[C];
-        sums(a, g * G, t);
-        sums(a, (GATED ? NO : 0) + g * G, u);
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          t[i] = sum(a, g, 0, i);
+          u[i] = sum(a, g, H - 1, i);
+        }
         if (m < p.M) emit<YT, decltype(gate)::value, C>(p, m, n, live, sm[a], ca, cb, t, u);
       }
     });
@@ -242,29 +241,49 @@ __device__ __forceinline__ void epilogue(const Linear8Params& p, int64_t m0, Col
 // ---------------------------------------------------------------------------------------------
 // Loads
 // ---------------------------------------------------------------------------------------------
-// 16 bytes of a row at byte k; what lies past K is zero. Rows start at any address (the vector loads of
-// gfx950 take any); only the row's last bytes, if fewer than 16, are loaded one by one.
+// 16 bytes of a row at byte k; what lies past K is zero. Rows start at any address (the vector loads of gfx950
+// take any). A row's last bytes, if fewer than 16, are the end of its last 16 moved down: 40 rows of 333 by 1,000
+// outputs took 17 us with them loaded one by one (rows of less than 16 bytes are).
 __device__ __forceinline__ i32x4 load_chunk(const int8_t* row, int k, int K) {
   if (k + 16 <= K) return *reinterpret_cast<const i32x4_any*>(row + k);
   i32x4 v = {0, 0, 0, 0};
+  if (k >= K) return v;
+  if (K < 16) {
 #pragma unroll
-  for (int b = 0; b < 15; ++b)
-    if (k + b < K) v[b / 4] |= static_cast<int>(static_cast<uint32_t>(static_cast<uint8_t>(row[k + b])) << (8 * (b % 4)));
+    for (int b = 0; b < 15; ++b)
+      if (b < K) v[b / 4] |= static_cast<int>(static_cast<uint32_t>(static_cast<uint8_t>(row[b])) << (8 * (b % 4)));
+    return v;
+  }
+  const i32x4 e = *reinterpret_cast<const i32x4_any*>(row + K - 16);
+  const int by = k + 16 - K;  // bytes to drop, 1 to 15
+  const uint32_t w[8] = {static_cast<uint32_t>(e[0]), static_cast<uint32_t>(e[1]), static_cast<uint32_t>(e[2]),
+                         static_cast<uint32_t>(e[3]), 0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t lo = w[i], hi = w[i + 1];  // words i + by / 4 and the next
+#pragma unroll
+    for (int j = 1; j < 4; ++j) {
+      lo = by / 4 == j ? w[i + j] : lo;
+      hi = by / 4 == j ? w[i + j + 1 < 8 ? i + j + 1 : 7] : hi;
+    }
+    v[i] = static_cast<int>(__builtin_amdgcn_alignbyte(hi, lo, static_cast<uint32_t>(by) & 3u));
+  }
   return v;
 }
 
 // ---------------------------------------------------------------------------------------------
 // Few rows (M <= 16 MT)
 // ---------------------------------------------------------------------------------------------
-template <typename YT, int W, int MT, bool GATED>
+template <typename YT, int W, int MT, int U, bool GATED>
 __global__ void __launch_bounds__(W * kWave) linear8_rows_kernel(const Linear8Params p) {
   constexpr int NT = GATED ? 2 : 1;
   __shared__ i32x4 s_acc[W > 1 ? W : 1][MT * NT][kWave];
   const int t = static_cast<int>(threadIdx.x);
-  const int lane = t & (kWave - 1), wave = t / kWave;
+  const int lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int fr = lane & 15, fq = lane >> 4;
-  const int n0 = static_cast<int>(blockIdx.x) * 16;
-  const int nr = n0 + fr < p.N ? n0 + fr : p.N - 1;  // columns past N repeat the last: not stored
+  const int n0 = p.n_begin + static_cast<int>(blockIdx.x) * 16;
+  // columns past the last and rows past M repeat the last: not stored
+  const int nr = n0 + fr < p.n_end ? n0 + fr : p.n_end - 1;
   const int8_t* wrow[NT];
   const int8_t* xrow[MT];
 #pragma unroll
@@ -279,25 +298,52 @@ __global__ void __launch_bounds__(W * kWave) linear8_rows_kernel(const Linear8Pa
   for (int c = 0; c < NT; ++c)
 #pragma unroll
     for (int a = 0; a < MT; ++a) acc[c][a] = i32x4{0, 0, 0, 0};
-  // a step of 128 bytes: the lane's two chunks are 32 bytes side by side
-  const int nk = (p.K + kStep - 1) / kStep;
-  for (int s = wave; s < nk; s += W) {
-    const int k = s * kStep + fq * 32;
-    i32x4 fw[NT][2], fx[MT][2];
+  // Steps of 128 bytes of K, of which the lane's two chunks are 32 bytes side by side; wavefront w takes steps w,
+  // w + W, ..., U of them at a time with all their loads in flight (those past the last whole step load it again
+  // and multiply by zero).
+  // (K split over workgroups: of this split's steps)
+  const int nk_all = p.K / kStep;
+  const int ks0 = p.part ? static_cast<int>(blockIdx.y) * p.split_steps : 0;
+  const int whole = p.part && ks0 + p.split_steps < nk_all ? ks0 + p.split_steps : nk_all;
+  for (int s = ks0 + wave; s < whole; s += W * U) {
+    i32x4 fw[U][NT][2], fx[U][MT][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int u = 0; u < U; ++u) {
+      const int su = s + u * W;
+      const int k = (su < whole ? su : whole - 1) * kStep + fq * 32;
 #pragma unroll
-      for (int c = 0; c < NT; ++c) fw[c][h] = load_chunk(wrow[c], k + h * 16, p.K);
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int a = 0; a < MT; ++a) fx[a][h] = load_chunk(xrow[a], k + h * 16, p.K);
+        for (int c = 0; c < NT; ++c) fw[u][c][h] = *reinterpret_cast<const i32x4_any*>(wrow[c] + k + h * 16);
+#pragma unroll
+        for (int a = 0; a < MT; ++a) fx[u][a][h] = *reinterpret_cast<const i32x4_any*>(xrow[a] + k + h * 16);
+      }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int c = 0; c < NT; ++c)
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int a = 0; a < MT; ++a)
-          acc[c][a] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[c][h], fx[a][h], acc[c][a], 0, 0, 0);
+        for (int a = 0; a < MT; ++a) {
+          const i32x4 x = s + u * W < whole ? fx[u][a][h] : i32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int c = 0; c < NT; ++c) acc[c][a] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u][c][h], x, acc[c][a], 0, 0, 0);
+        }
+  }
+  if (p.K % kStep != 0 && wave == nk_all % W && (!p.part || blockIdx.y + 1 == gridDim.y)) {  // the rest of K
+    const int k = nk_all * kStep + fq * 32;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      i32x4 fw[NT];
+#pragma unroll
+      for (int c = 0; c < NT; ++c) fw[c] = load_chunk(wrow[c], k + h * 16, p.K);
+#pragma unroll
+      for (int a = 0; a < MT; ++a) {
+        const i32x4 x = load_chunk(xrow[a], k + h * 16, p.K);
+#pragma unroll
+        for (int c = 0; c < NT; ++c) acc[c][a] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[c], x, acc[c][a], 0, 0, 0);
+      }
+    }
   }
   if constexpr (W > 1) {
 #pragma unroll
@@ -314,12 +360,9 @@ __global__ void __launch_bounds__(W * kWave) linear8_rows_kernel(const Linear8Pa
         for (int i = 1; i < W; ++i) acc[c][a] += s_acc[i][a * NT + c][lane];
   }
   // lane l holds columns 4 (l / 16) .. + 4 of row l % 16
-  i32x4 sums[MT][NT];
-#pragma unroll
-  for (int a = 0; a < MT; ++a)
-#pragma unroll
-    for (int c = 0; c < NT; ++c) sums[a][c] = acc[c][a];
-  epilogue<YT, GATED, MT, 1, 1>(p, 0, [&](int) { return n0 + fq * 4; }, sums, 0);
+  epilogue<YT, GATED, 16, MT, 1, 4>(p, 0, [&](int) { return n0 + fq * 4; },
+                                    [&](int a, int, int half, int i) { return acc[half][a][i]; },
+                                    static_cast<int>(blockIdx.y));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -356,7 +399,7 @@ __global__ void __launch_bounds__(WM * WN * kWave) linear8_tile_kernel(const Lin
   int tm, tn;
   tile_of(p, &tm, &tn);
   const int64_t m0 = static_cast<int64_t>(tm) * BM;
-  const int n0 = tn * OUT;
+  const int n0 = p.n_begin + tn * OUT;
   const int t = static_cast<int>(threadIdx.x);
   const int lane = t & (kWave - 1), wave = t / kWave;
   const int wm = wave / WN, wn = wave % WN;
@@ -381,7 +424,7 @@ __global__ void __launch_bounds__(WM * WN * kWave) linear8_tile_kernel(const Lin
     } else {
       n = n0 + j;
     }
-    wrow[q] = p.w + (static_cast<int64_t>(half) * p.N + (n < p.N ? n : p.N - 1)) * p.K;
+    wrow[q] = p.w + (static_cast<int64_t>(half) * p.N + (n < p.n_end ? n : p.n_end - 1)) * p.K;
   }
   const int nk_all = (p.K + kStep - 1) / kStep;
   const int ks0 = p.part ? static_cast<int>(blockIdx.y) * p.split_steps : 0;
@@ -429,8 +472,9 @@ __global__ void __launch_bounds__(WM * WN * kWave) linear8_tile_kernel(const Lin
     if (s + 1 < nk) put(buf ^ 1);
     __syncthreads();
   }
-  epilogue<YT, GATED, MI, NO, 1>(p, m0 + wm * TM, [&](int g) { return n0 + wn * NO * 16 + g * 16 + fq * 4; }, acc,
-                                 static_cast<int>(blockIdx.y));
+  epilogue<YT, GATED, 16, MI, NO, 4>(p, m0 + wm * TM, [&](int g) { return n0 + wn * NO * 16 + g * 16 + fq * 4; },
+                                     [&](int a, int g, int half, int i) { return acc[a][half * NO + g][i]; },
+                                     static_cast<int>(blockIdx.y));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -458,22 +502,147 @@ __device__ __forceinline__ void wait_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <typename YT, int WM, int WN, bool GATED, bool TAIL>
+// Tiles of BM x BN with WM x WN wavefronts, a ring of four steps: a step's loads are issued three steps ahead. For
+// tiles that are few, or short in K once it is split: what counts is bytes in flight.
+template <typename YT, int BM, int BN, int WM, int WN, bool GATED>
+__global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_ring_kernel(const Linear8Params p) {
+  constexpr int WAVES = WM * WN;
+  constexpr int TM = BM / WM, TN = BN / WN;
+  constexpr int MI = TM / 16, NI = TN / 16;
+  constexpr int kChunks = kStep / 16;
+  constexpr int PX = BM / 8 / WAVES, PW = BN / 8 / WAVES;  // loads per thread and step, 8 rows a wavefront each
+  constexpr int OUT = GATED ? BN / 2 : BN;
+  constexpr int NO = GATED ? NI / 2 : NI;
+  constexpr int G = std::is_same<YT, float>::value || NO < 2 ? 1 : 2;
+  static_assert(PX >= 1 && PW >= 1 && NO >= 1 && (!GATED || PW == 1 || NI % 2 == 0), "tile shape");
+  __shared__ i32x4 s0[(BM + BN) * kChunks], s1[(BM + BN) * kChunks], s2[(BM + BN) * kChunks], s3[(BM + BN) * kChunks];
+  int tm, tn;
+  tile_of(p, &tm, &tn);
+  const int64_t m0 = static_cast<int64_t>(tm) * BM;
+  const int n0 = p.n_begin + tn * OUT;
+  const int t = static_cast<int>(threadIdx.x);
+  const int lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int wm = wave / WN, wn = wave % WN;
+  const int fr = lane & 15, fq = lane >> 4;
+  const int nk_all = (p.K + kStep - 1) / kStep;
+  const int ks0 = p.part ? static_cast<int>(blockIdx.y) * p.split_steps : 0;
+  const int nk = p.part ? (nk_all - ks0 < p.split_steps ? nk_all - ks0 : p.split_steps) : nk_all;
+
+  const int64_t mrows = p.M - m0 < BM ? p.M - m0 : BM;
+  const int64_t nrows = p.n_end - n0 < OUT ? p.n_end - n0 : OUT;
+  const Rsrc xr = make_rsrc(p.x + m0 * p.K, static_cast<uint32_t>(mrows * p.K));
+  const Rsrc wr = make_rsrc(p.w + static_cast<int64_t>(n0) * p.K, static_cast<uint32_t>(nrows * p.K));
+  const Rsrc ur = make_rsrc(p.w + (static_cast<int64_t>(GATED ? p.N : 0) + n0) * p.K, static_cast<uint32_t>(nrows * p.K));
+  uint32_t xoff[PX], woff[PW];
+  const int chunk = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+  for (int q = 0; q < PX; ++q) xoff[q] = static_cast<uint32_t>((wave * PX + q) * 8 + lane / 8) * p.K + chunk * 16;
+#pragma unroll
+  for (int q = 0; q < PW; ++q) {
+    const int j = (wave * PW + q) * 8 + lane / 8, f = j % TN / 16 % NO, i = j % 16;
+    const int c = j / TN * (NO * 16) + f / G * (16 * G) + 4 * G * (i / 4) + 4 * (f % G) + i % 4;
+    woff[q] = static_cast<uint32_t>(c) * p.K + chunk * 16;
+  }
+  const auto issue = [&](int s, i32x4* to) {
+    const int k = (ks0 + (s < nk ? s : nk - 1)) * kStep;  // later steps are never used
+#pragma unroll
+    for (int q = 0; q < PX; ++q) load_lds(xr, to + (wave * PX + q) * kWave, xoff[q], k);
+#pragma unroll
+    for (int q = 0; q < PW; ++q) {
+      const int f = (wave * PW + q) / 2 % NI;
+      load_lds(GATED && f >= NO ? ur : wr, to + BM * kChunks + (wave * PW + q) * kWave, woff[q], k);
+    }
+  };
+  i32x4 acc[MI][NI];
+#pragma unroll
+  for (int a = 0; a < MI; ++a)
+#pragma unroll
+    for (int c = 0; c < NI; ++c) acc[a][c] = i32x4{0, 0, 0, 0};
+  constexpr int L = PX + PW;
+  issue(0, s0);
+  issue(1, s1);
+  issue(2, s2);
+  const auto step = [&](int s, const i32x4* mine, i32x4* free, auto endc) {
+    constexpr bool end = decltype(endc)::value;
+    wait_barrier<2 * L>();
+    issue(s + 3, free);  // over step s - 1, which every wavefront has read
+    const int left = p.K - (ks0 + s) * kStep;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int slot = fr * kChunks + ((h * 4 + fq) ^ (fr & 7));
+      i32x4 fw[NI], fx[MI];
+#pragma unroll
+      for (int c = 0; c < NI; ++c) fw[c] = mine[BM * kChunks + (wn * TN + c * 16) * kChunks + slot];
+#pragma unroll
+      for (int a = 0; a < MI; ++a) fx[a] = mine[(wm * TM + a * 16) * kChunks + slot];
+      if (end && left < kStep) {  // the rest of K
+#pragma unroll
+        for (int a = 0; a < MI; ++a)
+          if (h * 64 + fq * 16 >= left) fx[a] = i32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int a = 0; a < MI; ++a)
+#pragma unroll
+        for (int c = 0; c < NI; ++c)
+          acc[a][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[c], fx[a], acc[a][c], 0, 0, 0);
+    }
+  };
+  constexpr std::integral_constant<bool, false> inside{};
+  constexpr std::integral_constant<bool, true> end{};
+  int s = 0;
+  for (; s + 4 < nk; s += 4) {
+    step(s, s0, s3, inside);
+    step(s + 1, s1, s0, inside);
+    step(s + 2, s2, s1, inside);
+    step(s + 3, s3, s2, inside);
+  }
+  // one to four steps, the last of which may be the rest of K
+  step(s, s0, s3, end);
+  if (s + 1 < nk) {
+    step(s + 1, s1, s0, end);
+    if (s + 2 < nk) {
+      step(s + 2, s2, s1, end);
+      if (s + 3 < nk) step(s + 3, s3, s2, end);
+    }
+  }
+  epilogue<YT, GATED, 16, MI, NO / G, 4 * G>(
+      p, m0 + wm * TM, [&](int g) { return n0 + wn * (NO * 16) + g * (16 * G) + fq * (4 * G); },
+      [&](int a, int g, int half, int i) { return acc[a][half * NO + g * G + i / 4][i % 4]; }, static_cast<int>(blockIdx.y));
+}
+
+// Asks the scheduler for P products with R LDS reads and L loads spread evenly between them.
+template <int P, int R, int L, int I = 0>
+__device__ __forceinline__ void interleave() {
+  if constexpr (I < P) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // product
+    // reads come in the first three quarters: the next products need them
+    constexpr int r = (I + 1) * R * 4 / (P * 3) > R ? R : (I + 1) * R * 4 / (P * 3);
+    constexpr int r0 = I * R * 4 / (P * 3) > R ? R : I * R * 4 / (P * 3);
+    if constexpr (r > r0) __builtin_amdgcn_sched_group_barrier(0x100, r - r0, 0);
+    constexpr int l = (I + 1) * L / P, l0 = I * L / P;
+    if constexpr (l > l0) __builtin_amdgcn_sched_group_barrier(0x20, l - l0, 0);
+    interleave<P, R, L, I + 1>();
+  }
+}
+
+template <typename YT, int BM, int BN, int WM, int WN, bool GATED, bool TAIL>
 __global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_big_kernel(const Linear8Params p) {
-  constexpr int BM = 256, BN = 256, WAVES = WM * WN;
+  constexpr int WAVES = WM * WN;
   constexpr int TM = BM / WM, TN = BN / WN;
   constexpr int MI = TM / 16, NI = TN / 16;
   constexpr int kChunks = kStep / 16;
   constexpr int PX = BM / 8 / WAVES, PW = BN / 8 / WAVES;  // loads per thread and step, 8 rows a wavefront each
   constexpr int OUT = GATED ? BN / 2 : BN;
   constexpr int NO = GATED ? NI / 2 : NI;    // fragments of output columns
-  constexpr int G = NO < 4 ? NO : 4;         // of them side by side: a lane holds 4 G columns of a row
+  // G fragments of columns side by side, so that a lane holds 16 bytes of a row and four lanes store 64 in a row (32
+  // bytes a lane, stored in two halves with gaps: 8192 x 8192 -> 4096 took ? us)
+  constexpr int G = std::is_same<YT, float>::value || NO < 2 ? 1 : 2;
   // rows of 128 bytes, chunk c of row r in slot c ^ (r & 7) (no bank conflicts)
   __shared__ i32x4 s0[(BM + BN) * kChunks], s1[(BM + BN) * kChunks];
   int tm, tn;
   tile_of(p, &tm, &tn);
   const int64_t m0 = static_cast<int64_t>(tm) * BM;
-  const int n0 = tn * OUT;
+  const int n0 = p.n_begin + tn * OUT;
   const int t = static_cast<int>(threadIdx.x);
   const int lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int wm = wave / WN, wn = wave % WN;
@@ -486,7 +655,7 @@ __global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_big_kernel(const L
   // rows past M, weight rows past N and chunks past the last row's end lie past the buffers: nothing is read (a
   // chunk past the end of another row is the next row's; either is masked or multiplies what is not stored)
   const int64_t mrows = p.M - m0 < BM ? p.M - m0 : BM;
-  const int64_t nrows = p.N - n0 < OUT ? p.N - n0 : OUT;
+  const int64_t nrows = p.n_end - n0 < OUT ? p.n_end - n0 : OUT;
   const Rsrc xr = make_rsrc(p.x + m0 * p.K, static_cast<uint32_t>(mrows * p.K));
   const Rsrc wr = make_rsrc(p.w + static_cast<int64_t>(n0) * p.K, static_cast<uint32_t>(nrows * p.K));
   const Rsrc ur = make_rsrc(p.w + (static_cast<int64_t>(GATED ? p.N : 0) + n0) * p.K, static_cast<uint32_t>(nrows * p.K));
@@ -497,8 +666,8 @@ __global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_big_kernel(const L
   for (int q = 0; q < PX; ++q) xoff[q] = static_cast<uint32_t>((wave * PX + q) * 8 + lane / 8) * p.K + chunk * 16;
 #pragma unroll
   for (int q = 0; q < PW; ++q) {
-    // LDS row 16 f + i of a wavefront column holds column 16 (i / 4) + 4 (f % 4) + i % 4 of 64 (gated: fragments
-    // f < NO gates, the others their values), so that a lane receives 4 G columns side by side
+    // LDS row 16 f + i of a wavefront column holds column 4 G (i / 4) + 4 (f % G) + i % 4 of each 16 G (gated:
+    // fragments f < NO gates, the others their values), so that a lane receives 4 G columns side by side
     const int j = (wave * PW + q) * 8 + lane / 8, f = j % TN / 16 % NO, i = j % 16;
     const int c = j / TN * (NO * 16) + f / G * (16 * G) + 4 * G * (i / 4) + 4 * (f % G) + i % 4;
     woff[q] = static_cast<uint32_t>(c) * p.K + chunk * 16;
@@ -558,28 +727,13 @@ __global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_big_kernel(const L
     mask(0);
     read(mine, second);
     multiply(first);
-#pragma unroll
-    for (int i = 0; i < (MI + NI) / 2; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);    // products
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
-    }
+    interleave<MI * NI, MI + NI, 0>();
     wait_barrier<0>();
     mask(1);
     issue(s + 2, mine);
     read(next, first);
     multiply(second);
-#pragma unroll
-    for (int i = 0; i < L / 2; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x8, 3, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);   // load
-      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
+    interleave<MI * NI, MI + NI, L>();
     __builtin_amdgcn_sched_barrier(0);
   };
   // one way out of the loop: the compiler then knows at its head which loads to LDS are in flight, and adds no wait
@@ -594,30 +748,36 @@ __global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_big_kernel(const L
     step(s, s0, s1, end);
     if (TAIL && s + 1 < nk) step(s + 1, s1, s0, end);
   }
-  epilogue<YT, GATED, MI, NO, G>(p, m0 + wm * TM, [&](int g) { return n0 + wn * (NO * 16) + g * (16 * G) + fq * (4 * G); },
-                                 acc, static_cast<int>(blockIdx.y));
+  epilogue<YT, GATED, 16, MI, NO / G, 4 * G>(
+      p, m0 + wm * TM, [&](int g) { return n0 + wn * (NO * 16) + g * (16 * G) + fq * (4 * G); },
+      [&](int a, int g, int half, int i) { return acc[a][half * NO + g * G + i / 4][i % 4]; }, static_cast<int>(blockIdx.y));
 }
 
 // Split K: the splits' sums added, scales, bias, gate and rounding as in the tiles' epilogue; 4 columns a thread.
 constexpr int kReduceThreads = 256;
 template <typename YT, bool GATED>
 __global__ void __launch_bounds__(kReduceThreads) linear8_reduce_kernel(const Linear8Params p, int splits) {
-  const int quads = (p.N + 3) / 4;
+  const int64_t cols = p.n_end - p.n_begin, quads = (cols + 3) / 4;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kReduceThreads + threadIdx.x;
   const int64_t m = i / quads;
   if (m >= p.M) return;
-  const int n = static_cast<int>(i - m * quads) * 4, live = p.N - n;
-  const int64_t width = static_cast<int64_t>(p.N) * (GATED ? 2 : 1), each = p.M * width;
+  const int at = static_cast<int>(i - m * quads) * 4, n = p.n_begin + at, live = p.n_end - n;
+  const int64_t width = cols * (GATED ? 2 : 1), each = p.M * width;
   int t[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
 #pragma unroll
   for (int half = 0; half < (GATED ? 2 : 1); ++half) {
-    const int32_t* const from = p.part + m * width + static_cast<int64_t>(half) * p.N + n;
+    const int32_t* const from = p.part + m * width + half * cols + at;
     if (live >= 4) {
-#pragma unroll 4
-      for (int s = 0; s < splits; ++s) {
-        const i32x4 v = *reinterpret_cast<const i32x4_any*>(from + s * each);
+      constexpr int kAhead = 8;  // loads in flight
+      for (int s = 0; s < splits; s += kAhead) {
+        i32x4 v[kAhead];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) t[half][r] += v[r];
+        for (int j = 0; j < kAhead; ++j)
+          v[j] = *reinterpret_cast<const i32x4_any*>(from + (s + j < splits ? s + j : splits - 1) * each);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) t[half][r] += s + j < splits ? v[j][r] : 0;
       }
     } else {
       for (int s = 0; s < splits; ++s)
@@ -634,50 +794,96 @@ __global__ void __launch_bounds__(kReduceThreads) linear8_reduce_kernel(const Li
   });
 }
 
+// Rows of K bytes at any address to rows of a whole number of steps, the rest zero: x, then the weight. A copy of both
+// (read once, written once) costs less than tiles of operands that cannot be loaded straight to LDS.
+constexpr int kPadThreads = 256;
+__global__ void __launch_bounds__(kPadThreads) linear8_pad_kernel(const int8_t* x, const int8_t* w, int64_t x_rows,
+                                                                  int64_t rows, int32_t K, int32_t chunks, i32x4* out) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kPadThreads + threadIdx.x;
+  const int64_t row = i / chunks;
+  if (row >= rows) return;
+  const int8_t* const from = row < x_rows ? x + row * K : w + (row - x_rows) * K;
+  out[i] = load_chunk(from, static_cast<int>(i - row * chunks) * 16, K);
+}
+
 // ---------------------------------------------------------------------------------------------
 // Launch
 // ---------------------------------------------------------------------------------------------
 template <typename YT, bool GATED>
-hipError_t launch(Linear8Params p, const Linear8Plan& plan, hipStream_t s) {
-  if (plan.form == kLinear8Rows) {
-    const dim3 grid(static_cast<unsigned>((p.N + 15) / 16));
-    p.part = nullptr;
-    if (p.M <= 16) hipLaunchKernelGGL((linear8_rows_kernel<YT, 8, 1, GATED>), grid, dim3(8 * kWave), 0, s, p);
-    else hipLaunchKernelGGL((linear8_rows_kernel<YT, 8, 2, GATED>), grid, dim3(8 * kWave), 0, s, p);
-    return hipGetLastError();
+hipError_t launch_part(Linear8Params p, const Linear8Part& part, int32_t* work, hipStream_t s) {
+  p.n_begin = part.n_begin;
+  p.n_end = part.n_end;
+  p.split_steps = part.steps;
+  p.part = part.splits > 1 ? work : nullptr;
+  const Linear8Tile tile = linear8_tile(part.form, p.M);
+  const int out = GATED && part.form != kLinear8Rows ? tile.cols / 2 : tile.cols;
+  p.tiles_m = static_cast<int32_t>(linear_ceil(p.M, tile.rows));
+  p.tiles_n = static_cast<int32_t>(linear_ceil(p.n_end - p.n_begin, out));
+  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.tiles_m) * p.tiles_n), static_cast<unsigned>(part.splits));
+  const auto go = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, grid, dim3(waves * kWave), 0, s, p); };
+  const bool whole = p.K % kStep == 0;
+  switch (part.form) {
+    case kLinear8Rows: {
+      const auto rows = [&](auto mt) {
+        constexpr int MT = decltype(mt)::value;
+        // the steps of a split in one batch of loads where they are few
+        if (part.steps <= 4) go(linear8_rows_kernel<YT, 4, MT, 1, GATED>, 4);
+        else if (part.steps <= 8) go(linear8_rows_kernel<YT, 4, MT, 2, GATED>, 4);
+        else if (part.steps <= 16) go(linear8_rows_kernel<YT, 4, MT, 4, GATED>, 4);
+        else go(linear8_rows_kernel<YT, 8, MT, 4, GATED>, 8);
+      };
+      if (p.M <= 16) rows(std::integral_constant<int, 1>{});
+      else rows(std::integral_constant<int, 2>{});
+      break;
+    }
+    case kLinear8Any: go(linear8_tile_kernel<YT, 128, 128, 2, 2, GATED>, 4); break;
+    case kLinear8Ring64: go(linear8_ring_kernel<YT, 64, 64, 2, 2, GATED>, 4); break;
+    case kLinear8Ring128: go(linear8_ring_kernel<YT, 64, 128, 1, 4, GATED>, 4); break;
+    case kLinear8Tile128:
+      if (whole) go(linear8_big_kernel<YT, 128, 128, 2, 4, GATED, false>, 8);
+      else go(linear8_big_kernel<YT, 128, 128, 2, 4, GATED, true>, 8);
+      break;
+    case kLinear8Tile256:
+      if (whole) go(linear8_big_kernel<YT, 256, 256, 2, 4, GATED, false>, 8);
+      else go(linear8_big_kernel<YT, 256, 256, 2, 4, GATED, true>, 8);
+      break;
   }
-  if (p.M > 1024 && p.K % 16 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && reinterpret_cast<uintptr_t>(p.w) % 16 == 0) {
-    p.tiles_m = static_cast<int32_t>((p.M + 255) / 256);
-    p.tiles_n = (p.N + (GATED ? 127 : 255)) / (GATED ? 128 : 256);
-    p.part = nullptr;
-    const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.tiles_m) * p.tiles_n));
-    if (p.K % kStep == 0) hipLaunchKernelGGL((linear8_big_kernel<YT, 2, 4, GATED, false>), grid, dim3(8 * kWave), 0, s, p);
-    else hipLaunchKernelGGL((linear8_big_kernel<YT, 2, 4, GATED, true>), grid, dim3(8 * kWave), 0, s, p);
-    return hipGetLastError();
-  }
-  constexpr int BM = 128, BN = 128, OUT = GATED ? BN / 2 : BN;
-  p.tiles_m = static_cast<int32_t>((p.M + BM - 1) / BM);
-  p.tiles_n = (p.N + OUT - 1) / OUT;
-  p.split_steps = plan.steps;
-  if (plan.splits <= 1) p.part = nullptr;
-  const dim3 grid(static_cast<unsigned>(static_cast<int64_t>(p.tiles_m) * p.tiles_n), static_cast<unsigned>(plan.splits));
-  hipLaunchKernelGGL((linear8_tile_kernel<YT, BM, BN, 2, 2, GATED>), grid, dim3(4 * kWave), 0, s, p);
   if (p.part) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t threads = p.M * ((p.N + 3) / 4);
+    const int64_t threads = p.M * ((p.n_end - p.n_begin + 3) / 4);
     hipLaunchKernelGGL((linear8_reduce_kernel<YT, GATED>), dim3(static_cast<unsigned>((threads + kReduceThreads - 1) / kReduceThreads)),
-                       dim3(kReduceThreads), 0, s, p, plan.splits);
+                       dim3(kReduceThreads), 0, s, p, part.splits);
   }
   return hipGetLastError();
 }
 
+template <typename YT, bool GATED>
+hipError_t launch(Linear8Params p, const Linear8Plan& plan, char* work, hipStream_t s) {
+  if (plan.padded) {
+    const int64_t wrows = static_cast<int64_t>(p.N) * (GATED ? 2 : 1), rows = p.M + wrows;
+    const int32_t to = static_cast<int32_t>(linear_ceil(p.K, kStep) * kStep), chunks = to / 16;
+    hipLaunchKernelGGL(linear8_pad_kernel, dim3(static_cast<unsigned>(linear_ceil(rows * chunks, kPadThreads))),
+                       dim3(kPadThreads), 0, s, p.x, p.w, p.M, rows, p.K, chunks, reinterpret_cast<i32x4*>(work));
+    p.x = reinterpret_cast<const int8_t*>(work);
+    p.w = p.x + p.M * to;
+    p.K = to;
+    work += rows * to;
+  }
+  // (parts run one after the other: they may share the space for partial sums)
+  for (int i = 0; i < plan.parts; ++i) {
+    const hipError_t e = launch_part<YT, GATED>(p, plan.part[i], reinterpret_cast<int32_t*>(work), s);
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
 template <bool GATED>
-hipError_t launch_typed(const Linear8Params& p, const Linear8Plan& plan, hipStream_t s) {
+hipError_t launch_typed(const Linear8Params& p, const Linear8Plan& plan, char* work, hipStream_t s) {
   switch (p.y_dtype) {
-    case CTI_EBAG_F32: return launch<float, GATED>(p, plan, s);
-    case CTI_EBAG_BF16: return launch<bf16_t, GATED>(p, plan, s);
-    default: return launch<f16_t, GATED>(p, plan, s);
+    case CTI_EBAG_F32: return launch<float, GATED>(p, plan, work, s);
+    case CTI_EBAG_BF16: return launch<bf16_t, GATED>(p, plan, work, s);
+    default: return launch<f16_t, GATED>(p, plan, work, s);
   }
 }
 
@@ -693,8 +899,7 @@ extern "C" int64_t cti_ebag_linear_int8_workspace_bytes(int64_t rows, int32_t co
       out_features > kLinear8MaxN || gate < CTI_EBAG_GATE_NONE || gate > CTI_EBAG_GATE_RELU)
     return 0;
   const bool gated = gate != CTI_EBAG_GATE_NONE;
-  const Linear8Plan plan = linear8_plan(rows, out_features, cols, gated, INT64_MAX);
-  return linear8_part_bytes(plan, rows, out_features, gated);
+  return linear8_workspace_bytes(rows, out_features, cols, gated);
 }
 
 extern "C" int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t rows, int32_t cols, const int8_t* weight,
@@ -720,8 +925,9 @@ extern "C" int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return set_error(CTI_EBAG_EINVAL, "workspace is not 16-byte aligned");
   const bool gated = gate != CTI_EBAG_GATE_NONE;
-  const Linear8Plan plan = linear8_plan(rows, out_features, cols, gated, workspace ? workspace_bytes : 0);
-  if (linear8_workgroups(plan, rows, out_features, gated) > INT32_MAX)
+  const bool aligned = cols % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0;
+  const Linear8Plan plan = linear8_plan(rows, out_features, cols, gated, aligned, workspace ? workspace_bytes : 0);
+  if (linear8_workgroups(plan, rows, gated) > INT32_MAX)
     return set_error(CTI_EBAG_EUNSUPPORTED, "too many output tiles (%lld x %d)", (long long)rows, out_features);
   Linear8Params p = {};
   p.x = q;
@@ -730,7 +936,6 @@ extern "C" int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t
   p.wscale = weight_scale;
   p.bias = bias;
   p.y = static_cast<char*>(y);
-  p.part = static_cast<int32_t*>(workspace);
   p.M = rows;
   p.N = out_features;
   p.K = cols;
@@ -738,7 +943,8 @@ extern "C" int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t
   p.y_dtype = y_dtype;
   p.gate = gate;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const hipError_t e = gated ? launch_typed<true>(p, plan, s) : launch_typed<false>(p, plan, s);
+  char* const work = static_cast<char*>(workspace);
+  const hipError_t e = gated ? launch_typed<true>(p, plan, work, s) : launch_typed<false>(p, plan, work, s);
   if (e != hipSuccess) return set_error(CTI_EBAG_EHIP, "linear launch failed: %s", hipGetErrorString(e));
   return CTI_EBAG_OK;
 }

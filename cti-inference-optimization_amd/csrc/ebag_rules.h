@@ -164,37 +164,94 @@ constexpr int kLinear8MaxN = 1 << 30;  // 2 N is an int32 too
 
 enum Linear8Form {
   kLinear8Rows,  // few rows: operands straight to registers
-  kLinear8Tile,  // 128 x 128 tiles, K split if they are few
+  kLinear8Any,   // 128 x 128 tiles of operands at any address, any K
+  // K a multiple of 16, 16-byte aligned operands, loaded straight to LDS:
+  kLinear8Ring64,   // 64 x 64 tiles
+  kLinear8Ring128,  // 64 x 128 tiles
+  kLinear8Tile128,  // 128 x 128 tiles
+  kLinear8Tile256,  // 256 x 256 tiles
 };
-struct Linear8Plan {
+// One launch (two with splits): columns n_begin .. n_end of y.
+struct Linear8Part {
   Linear8Form form;
   int splits;  // of K: 1, or as many int32 partial sums as the workspace then has to hold
   int steps;   // per split
+  int32_t n_begin, n_end;
+};
+struct Linear8Plan {
+  int parts;
+  Linear8Part part[2];
+  bool padded;  // operands are copied to rows of whole steps first
+};
+struct Linear8Tile {
+  int rows, cols;  // of weight rows; the gated form's tiles hold as many gates as values, but for few rows
 };
 
-inline int64_t linear8_part_bytes(const Linear8Plan& plan, int64_t M, int32_t N, bool gated) {
-  return plan.splits > 1 ? plan.splits * M * N * (gated ? 8 : 4) : 0;
+inline Linear8Tile linear8_tile(Linear8Form form, int64_t M) {
+  switch (form) {
+    case kLinear8Rows: return {M <= 16 ? 16 : 32, 16};
+    case kLinear8Ring64: return {64, 64};
+    case kLinear8Ring128: return {64, 128};
+    case kLinear8Tile256: return {256, 256};
+    default: return {128, 128};
+  }
 }
 
-// Workgroups of a launch (one split).
-inline int64_t linear8_workgroups(const Linear8Plan& plan, int64_t M, int32_t N, bool gated) {
-  if (plan.form == kLinear8Rows) return linear_ceil(N, 16);
-  return linear_ceil(M, 128) * linear_ceil(N, gated ? 64 : 128);
+// Bytes of the copies of padded operands, and of a plan's workspace.
+inline int64_t linear8_pad_bytes(int64_t M, int32_t N, int32_t K, bool gated) {
+  return (M + static_cast<int64_t>(N) * (gated ? 2 : 1)) * linear_ceil(K, kLinear8Step) * kLinear8Step;
+}
+inline int64_t linear8_part_bytes(const Linear8Part& part, int64_t M, bool gated) {
+  return part.splits > 1 ? part.splits * M * (part.n_end - part.n_begin) * (gated ? 8 : 4) : 0;
+}
+inline int64_t linear8_plan_bytes(const Linear8Plan& plan, int64_t M, int32_t N, int32_t K, bool gated) {
+  int64_t most = 0;  // the parts run one after the other
+  for (int i = 0; i < plan.parts; ++i) {
+    const int64_t b = linear8_part_bytes(plan.part[i], M, gated);
+    if (b > most) most = b;
+  }
+  return most + (plan.padded ? linear8_pad_bytes(M, N, K, gated) : 0);
 }
 
-inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, int64_t ws_bytes) {
+// Tiles of `cols` columns of y.
+inline int64_t linear8_tiles(Linear8Form form, int64_t M, int64_t cols, bool gated) {
+  const Linear8Tile tile = linear8_tile(form, M);
+  return linear_ceil(M, tile.rows) * linear_ceil(cols, gated && form != kLinear8Rows ? tile.cols / 2 : tile.cols);
+}
+// The most workgroups of a launch (of one split).
+inline int64_t linear8_workgroups(const Linear8Plan& plan, int64_t M, bool gated) {
+  int64_t most = 0;
+  for (int i = 0; i < plan.parts; ++i) {
+    const int64_t t = linear8_tiles(plan.part[i].form, M, plan.part[i].n_end - plan.part[i].n_begin, gated);
+    if (t > most) most = t;
+  }
+  return most;
+}
+
+inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, bool aligned, int64_t ws_bytes) {
   const int nk = static_cast<int>(linear_ceil(K, kLinear8Step));
-  if (M <= 32) return {kLinear8Rows, 1, nk};
-  Linear8Plan plan{kLinear8Tile, 1, nk};
-  int64_t want = kLinearCus / linear8_workgroups(plan, M, N, gated);
+  Linear8Plan plan{1, {{kLinear8Any, 1, nk, 0, N}, {}}, false};
+  Linear8Part& part = plan.part[0];
+  if (M > 16 && !aligned && ws_bytes >= linear8_pad_bytes(M, N, K, gated)) {
+    plan.padded = aligned = true;
+    ws_bytes -= linear8_pad_bytes(M, N, K, gated);
+  }
+  if (M <= 16) part.form = kLinear8Rows;
+  else if (aligned) part.form = M <= 64 ? kLinear8Ring64 : M <= 256 ? kLinear8Ring128 : M <= 2048 ? kLinear8Tile128 : kLinear8Tile256;
+  int64_t want = kLinearCus / linear8_tiles(part.form, M, N, gated);
   const int64_t fit = ws_bytes / (M * N * (gated ? 8 : 4));
   if (want > fit) want = fit;
   if (want > nk / 2) want = nk / 2;
   if (want > 1) {
-    plan.steps = static_cast<int>(linear_ceil(nk, want));
-    plan.splits = static_cast<int>(linear_ceil(nk, plan.steps));
+    part.steps = static_cast<int>(linear_ceil(nk, want));
+    part.splits = static_cast<int>(linear_ceil(nk, part.steps));
   }
   return plan;
+}
+
+// Bytes of workspace that a shape's operands, at 16-byte aligned addresses, are given at most.
+inline int64_t linear8_workspace_bytes(int64_t M, int32_t N, int32_t K, bool gated) {
+  return linear8_plan_bytes(linear8_plan(M, N, K, gated, K % 16 == 0, INT64_MAX), M, N, K, gated);
 }
 
 }  // namespace cti

@@ -19,6 +19,7 @@ Both validate their arguments on the host (no device synchronisation) and raise 
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from typing import Optional, Sequence
 
@@ -120,49 +121,75 @@ def dequantize_embedding_int8(q: torch.Tensor, scale: torch.Tensor, out_dtype: t
     ``quantize_embedding_int8``, ``rms_norm_int8`` and ``layer_norm_int8`` return them) to
     ``out [V, D]`` with ``out[v, j] = q[v, j] * scale[v]`` in fp32, rounded once to ``out_dtype``
     (bf16 by default; fp32, bf16 or fp16, or ``out``'s). Written on torch's current stream."""
-    rows, dim, dev = _check_int8_rows("q", q, "scale", scale)
-    out = _output("out", out, (rows, dim), out_dtype, dev)
-    with torch.cuda.device(dev):
-        _capi.check(_capi.lib().cti_ebag_dequantize_int8(
-            q.data_ptr(), scale.data_ptr(), rows, dim, out.data_ptr(), _capi.dtype_code(out.dtype),
-            _capi.current_stream_handle(dev)))
+    rows, dim, index = _check_int8_rows("q", q, "scale", scale)
+    out, code = _float_output(out, rows, dim, out_dtype, q, index)
+    _launch(index, _capi.lib().cti_ebag_dequantize_int8, q.data_ptr(), scale.data_ptr(), rows, dim, out.data_ptr(), code)
     return out
 
 
-def _check_int8_rows(name: str, q, scale_name: str, scale, device: Optional[torch.device] = None):
-    """Validate int8 rows and their scales; return (rows, columns, device)."""
-    _require_device_tensor(name, q, device)
-    _require_device_tensor(scale_name, scale, q.device)
+# The int8 operators take a few microseconds on the GPU, as long as a call's way through Python takes: their checks
+# go by device indexes, build no device or stream objects, and allocate in the forms of torch.empty that return soonest.
+def _require_on(name: str, t, index: Optional[int] = None) -> int:
+    """`t` is a contiguous GPU tensor (on device `index`); return its device's index."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or (index is not None and t.get_device() != index):
+        _require_device_tensor(name, t, None if index is None else torch.device("cuda", index))
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.get_device()
+
+
+def _launch(index: int, fn, *args) -> None:
+    """Call a C entry point with `args` and torch's current stream on device `index`, with that device the
+    current one."""
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status != _capi.OK:
+        _capi.check(status)
+
+
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a Stream object
+    _raw_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811
+
+
+def _check_int8_rows(name: str, q, scale_name: str, scale, index: Optional[int] = None):
+    """Validate int8 rows and their scales; return (rows, columns, device index)."""
+    index = _require_on(name, q, index)
+    _require_on(scale_name, scale, index)
     if q.dim() != 2 or q.shape[1] < 1:
         raise ValueError(f"{name} must be 2-D [rows, columns >= 1], got shape {tuple(q.shape)}")
-    if q.dtype != torch.int8:
+    if q.dtype is not torch.int8:
         raise TypeError(f"{name} must be int8 (got {q.dtype})")
-    if scale.dtype != torch.float32:
+    if scale.dtype is not torch.float32:
         raise TypeError(f"{scale_name} must be float32 (got {scale.dtype})")
-    _require_contiguous(name, q)
-    _require_contiguous(scale_name, scale)
-    if scale.dim() != 1 or scale.numel() != q.shape[0]:
-        raise ValueError(f"{scale_name} has shape {tuple(scale.shape)}, expected ({q.shape[0]},)")
-    return q.shape[0], q.shape[1], q.device
+    rows, cols = q.shape
+    if scale.dim() != 1 or scale.numel() != rows:
+        raise ValueError(f"{scale_name} has shape {tuple(scale.shape)}, expected ({rows},)")
+    return rows, cols, index
 
 
-def _output(name: str, out: Optional[torch.Tensor], shape, dtype: torch.dtype, dev: torch.device,
-            any_float: bool = True) -> torch.Tensor:
-    """`out`, checked, or a new tensor of `dtype`; an `out` given may have any element type of the
-    library (`any_float`), or must have `dtype`."""
+def _float_output(out: Optional[torch.Tensor], rows: int, cols: int, dtype: torch.dtype, like: torch.Tensor, index: int):
+    """`out`, checked, or a new tensor of `dtype` on the device of `like`; and its type's code."""
     if out is None:
-        if any_float:
-            _capi.dtype_code(dtype)
-        return torch.empty(shape, dtype=dtype, device=dev)
-    _require_device_tensor(name, out, dev)
-    _require_contiguous(name, out)
-    if tuple(out.shape) != tuple(shape):
+        return torch.empty(rows, cols, dtype=dtype, device=like.device), _capi.dtype_code(dtype)
+    _require_on("out", out, index)
+    if out.dim() != 2 or out.shape[0] != rows or out.shape[1] != cols:
+        raise ValueError(f"out has shape {tuple(out.shape)}, expected ({rows}, {cols})")
+    return out, _capi.dtype_code(out.dtype)
+
+
+def _check_output(name: str, out: torch.Tensor, shape, dtype: torch.dtype, index: int) -> None:
+    _require_on(name, out, index)
+    if out.shape != shape:
         raise ValueError(f"{name} has shape {tuple(out.shape)}, expected {tuple(shape)}")
-    if any_float:
-        _capi.dtype_code(out.dtype)
-    elif out.dtype != dtype:
+    if out.dtype != dtype:
         raise TypeError(f"{name} must be {dtype} (got {out.dtype})")
-    return out
 
 
 def _check_flat_layout(flat_values, val_offsets, flat_row_offsets, out, dev):
@@ -874,38 +901,45 @@ def layer_norm_linear(
 
 
 def _norm_int8(kind: int, x, weight, bias, eps, residual, q, scale, residual_out):
-    _require_device_tensor("x", x)
-    dev = x.device
+    index = _require_on("x", x)
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x must be 2-D [rows, cols >= 1], got shape {tuple(x.shape)}")
-    _require_contiguous("x", x)
-    code = _capi.dtype_code(x.dtype)
+    dtype = x.dtype
+    code = _capi.dtype_code(dtype)
     rows, cols = x.shape
-    params = [("weight", weight)] + ([("bias", bias)] if kind == _capi.LAYER_NORM else [])
-    for name, t in params:
-        _require_device_tensor(name, t, dev)
-        _require_contiguous(name, t)
-        if t.numel() != cols:
-            raise ValueError(f"{name} has {t.numel()} elements, expected {cols}")
-        if t.dtype != weight.dtype:
-            raise TypeError(f"weight and bias dtypes differ ({weight.dtype} vs {t.dtype})")
+    _require_on("weight", weight, index)
+    if weight.numel() != cols:
+        raise ValueError(f"weight has {weight.numel()} elements, expected {cols}")
     param_code = _capi.dtype_code(weight.dtype)
-    if residual is None:
-        if residual_out is not None:
-            raise ValueError("residual_out needs a residual")
+    bias_ptr = res_ptr = res_out_ptr = None
+    if kind == _capi.LAYER_NORM:
+        _require_on("bias", bias, index)
+        if bias.numel() != cols:
+            raise ValueError(f"bias has {bias.numel()} elements, expected {cols}")
+        if bias.dtype != weight.dtype:
+            raise TypeError(f"weight and bias dtypes differ ({weight.dtype} vs {bias.dtype})")
+        bias_ptr = bias.data_ptr()
+    if residual is not None:
+        _require_on("residual", residual, index)
+        if residual.shape != x.shape or residual.dtype != dtype:
+            raise ValueError(f"residual must be {tuple(x.shape)} {dtype}, got {tuple(residual.shape)} {residual.dtype}")
+        if residual_out is None:
+            residual_out = torch.empty(rows, cols, dtype=dtype, device=x.device)
+        else:
+            _check_output("residual_out", residual_out, x.shape, dtype, index)
+        res_ptr, res_out_ptr = residual.data_ptr(), residual_out.data_ptr()
+    elif residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    if q is None:
+        q = torch.empty(rows, cols, dtype=torch.int8, device=x.device)
     else:
-        _require_device_tensor("residual", residual, dev)
-        _require_contiguous("residual", residual)
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError(f"residual must be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
-        residual_out = _output("residual_out", residual_out, x.shape, x.dtype, dev, any_float=False)
-    q = _output("q", q, x.shape, torch.int8, dev, any_float=False)
-    scale = _output("scale", scale, (rows,), torch.float32, dev, any_float=False)
-    ptr = (lambda t: t.data_ptr() if t is not None else None)
-    with torch.cuda.device(dev):
-        _capi.check(_capi.lib().cti_ebag_norm_int8(
-            kind, x.data_ptr(), ptr(residual), ptr(residual_out), rows, cols, code, weight.data_ptr(), ptr(bias),
-            param_code, float(eps), q.data_ptr(), scale.data_ptr(), _capi.current_stream_handle(dev)))
+        _check_output("q", q, x.shape, torch.int8, index)
+    if scale is None:
+        scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    else:
+        _check_output("scale", scale, (rows,), torch.float32, index)
+    _launch(index, _capi.lib().cti_ebag_norm_int8, kind, x.data_ptr(), res_ptr, res_out_ptr, rows, cols, code,
+            weight.data_ptr(), bias_ptr, param_code, eps, q.data_ptr(), scale.data_ptr())
     return (q, scale) if residual is None else (q, scale, residual_out)
 
 
@@ -949,8 +983,8 @@ def layer_norm_int8(
 
 
 def _linear_int8(q, scale, weight, weight_scale, bias, gate: int, out, out_dtype, split_k: bool):
-    rows, cols, dev = _check_int8_rows("q", q, "scale", scale)
-    w_rows, w_cols, _ = _check_int8_rows("weight", weight, "weight_scale", weight_scale, dev)
+    rows, cols, index = _check_int8_rows("q", q, "scale", scale)
+    w_rows, w_cols, _ = _check_int8_rows("weight", weight, "weight_scale", weight_scale, index)
     if w_cols != cols:
         raise ValueError(f"weight has {w_cols} columns, q has {cols}")
     if w_rows < 1:
@@ -960,25 +994,28 @@ def _linear_int8(q, scale, weight, weight_scale, bias, gate: int, out, out_dtype
         if w_rows % 2:
             raise ValueError(f"weight has {w_rows} rows; expected as many gates as values (an even number)")
         n_out = w_rows // 2
+    bias_ptr, bias_code = None, _capi.F32
     if bias is not None:
-        _require_device_tensor("bias", bias, dev)
-        _require_contiguous("bias", bias)
+        _require_on("bias", bias, index)
         if bias.numel() != w_rows:
             raise ValueError(f"bias has {bias.numel()} elements, expected {w_rows}")
-    bias_code = _capi.dtype_code(bias.dtype) if bias is not None else _capi.F32
-    out = _output("out", out, (rows, n_out), out_dtype, dev)
-    lib = _capi.lib()
+        bias_ptr, bias_code = bias.data_ptr(), _capi.dtype_code(bias.dtype)
+    out, code = _float_output(out, rows, n_out, out_dtype, q, index)
     # K split over several workgroups where few tiles would leave CUs idle: int32 partial sums in a
     # workspace from torch's allocator (kept alive until the launches are enqueued)
-    ws_bytes = lib.cti_ebag_linear_int8_workspace_bytes(rows, cols, n_out, gate) if split_k else 0
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes > 0 else None
-    with torch.cuda.device(dev):
-        _capi.check(lib.cti_ebag_linear_int8(
-            q.data_ptr(), scale.data_ptr(), rows, cols, weight.data_ptr(), weight_scale.data_ptr(), n_out,
-            bias.data_ptr() if bias is not None else None, bias_code, gate, out.data_ptr(),
-            _capi.dtype_code(out.dtype), ws.data_ptr() if ws is not None else None, ws_bytes,
-            _capi.current_stream_handle(dev)))
+    ws, ws_ptr, ws_bytes = None, None, _linear_int8_workspace(rows, cols, n_out, gate) if split_k else 0
+    if ws_bytes > 0:
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        ws_ptr = ws.data_ptr()
+    _launch(index, _capi.lib().cti_ebag_linear_int8, q.data_ptr(), scale.data_ptr(), rows, cols, weight.data_ptr(),
+            weight_scale.data_ptr(), n_out, bias_ptr, bias_code, gate, out.data_ptr(), code, ws_ptr, ws_bytes)
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_int8_workspace(rows: int, cols: int, n_out: int, gate: int) -> int:
+    """The library's query, which goes by these sizes alone."""
+    return _capi.lib().cti_ebag_linear_int8_workspace_bytes(rows, cols, n_out, gate)
 
 
 def linear_int8(

@@ -94,41 +94,61 @@ def test_python_entry_points_validate_before_any_launch(pkg):
 # ------------------------------------------------------------------------------------------------
 # Dispatch
 # ------------------------------------------------------------------------------------------------
+class _Part(ctypes.Structure):
+    _fields_ = [("form", ctypes.c_int), ("splits", ctypes.c_int), ("steps", ctypes.c_int),
+                ("n_begin", ctypes.c_int32), ("n_end", ctypes.c_int32)]
+
+
+class _Plan(ctypes.Structure):
+    _fields_ = [("parts", ctypes.c_int), ("part", _Part * 2), ("padded", ctypes.c_bool)]
+
+
 @pytest.fixture(scope="module")
 def rules(tmp_path_factory):
     work = tmp_path_factory.mktemp("rules8")
     (work / "rules.cpp").write_text(
         '#include "ebag_rules.h"\n'
-        'extern "C" int plan(int64_t M, int32_t N, int32_t K, int gated, int64_t ws, int* splits, int* steps,\n'
-        "                    int64_t* part, int64_t* groups) {\n"
-        "  const cti::Linear8Plan p = cti::linear8_plan(M, N, K, gated != 0, ws);\n"
-        "  *splits = p.splits;\n  *steps = p.steps;\n"
-        "  *part = cti::linear8_part_bytes(p, M, N, gated != 0);\n"
-        "  *groups = cti::linear8_workgroups(p, M, N, gated != 0);\n  return p.form;\n}\n")
+        'extern "C" void plan(int64_t M, int32_t N, int32_t K, int gated, int aligned, int64_t ws, cti::Linear8Plan* p,\n'
+        "                     int64_t* bytes, int64_t* groups) {\n"
+        "  *p = cti::linear8_plan(M, N, K, gated != 0, aligned != 0, ws);\n"
+        "  *bytes = cti::linear8_plan_bytes(*p, M, N, K, gated != 0);\n"
+        "  *groups = cti::linear8_workgroups(*p, M, gated != 0);\n}\n")
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", f"-I{CSRC}",
                     str(work / "rules.cpp"), "-o", str(work / "rules.so")], check=True)
     lib = ctypes.CDLL(str(work / "rules.so"))
     I, P = ctypes.c_int64, ctypes.POINTER
-    lib.plan.argtypes = [I, ctypes.c_int32, ctypes.c_int32, ctypes.c_int, I, P(ctypes.c_int), P(ctypes.c_int), P(I), P(I)]
+    lib.plan.argtypes = [I, ctypes.c_int32, ctypes.c_int32, ctypes.c_int, ctypes.c_int, I, P(_Plan), P(I), P(I)]
+    lib.plan.restype = None
 
-    def plan(M, N, K, gated, ws):
-        out = ctypes.c_int(), ctypes.c_int(), I(), I()
-        form = lib.plan(M, N, K, gated, ws, *(ctypes.byref(o) for o in out))
-        return (form, *(o.value for o in out))
+    def plan(M, N, K, gated, aligned, ws):
+        p, nbytes, groups = _Plan(), I(), I()
+        lib.plan(M, N, K, gated, aligned, ws, ctypes.byref(p), ctypes.byref(nbytes), ctypes.byref(groups))
+        return p, nbytes.value, groups.value
 
     return plan
 
 
 @pytest.mark.parametrize("gated", [0, 1])
-def test_the_splits_cover_k_and_fit_the_workspace(rules, pkg, gated):
-    for M in (1, 16, 17, 32, 33, 64, 65, 100, 128, 500, 2048, 70000):
-        for N in (1, 16, 500, 512, 4096, 14336):
+def test_plans_cover_the_product_and_fit_the_workspace(rules, pkg, gated):
+    for M in (1, 16, 17, 32, 33, 64, 65, 100, 128, 500, 2048, 8000, 70000):
+        for N in (1, 16, 500, 512, 4096, 4100, 14336):
             for K in (1, 16, 127, 128, 129, 1021, 3584, 14336, 131071):
                 query = pkg._capi.lib().cti_ebag_linear_int8_workspace_bytes(M, K, N, gated)
                 for ws in (0, 1000, M * N * (8 if gated else 4) * 3, query, 1 << 40):
-                    _, splits, steps, part, groups = rules(M, N, K, gated, ws)
-                    nk = -(-K // 128)
-                    assert splits >= 1 and steps >= 1 and groups >= 1
-                    assert (splits - 1) * steps < nk <= splits * steps  # every split has work, all of it is done
-                    assert part <= max(0, min(ws, query))
-                    assert part == (0 if splits == 1 else splits * M * N * (8 if gated else 4))
+                    for aligned in (0, 1) if K % 16 == 0 else (0,):
+                        plan, nbytes, groups = rules(M, N, K, gated, aligned, ws)
+                        assert 1 <= plan.parts <= 2 and groups >= 1
+                        at = 0
+                        for part in plan.part[:plan.parts]:
+                            assert part.n_begin == at < part.n_end  # the parts' columns, side by side
+                            at = part.n_end
+                            nk = -(-K // 128)
+                            # every split has work, all of it is done
+                            assert (part.splits - 1) * part.steps < nk <= part.splits * part.steps
+                            # direct loads only of aligned rows of whole 16-byte chunks; few rows fit their fragments
+                            assert aligned or plan.padded or part.form in (0, 1)
+                            assert part.form != 0 or M <= 32
+                        assert at == N
+                        assert nbytes <= ws
+                        if bool(aligned) == (K % 16 == 0):
+                            assert nbytes <= query
