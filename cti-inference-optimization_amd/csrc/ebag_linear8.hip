@@ -44,7 +44,7 @@ struct Linear8Params {
   const float* wscale;  // [N or 2 N]
   const void* bias;     // [N or 2 N] or NULL
   char* y;              // [M, N]
-  int32_t* part;        // split K: int32 partial sums [splits, M, columns of this launch (gated: twice)]; NULL: no split
+  int32_t* part;        // split K: int32 partial sums [splits, M, linear8_part_cols() (gated: twice)]; NULL: no split
   int64_t M;
   int32_t N;            // columns of y
   int32_t K;            // bytes of a row of x and w
@@ -180,7 +180,7 @@ __device__ __forceinline__ void epilogue(const Linear8Params& p, int64_t m0, Col
   constexpr int H = GATED ? 2 : 1;
   const int row = lane_id() % R;
   if (p.part) {
-    const int64_t cols = p.n_end - p.n_begin, width = cols * H;
+    const int64_t cols = linear8_part_cols(p.n_end - p.n_begin), width = cols * H;
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       const int n = col_of(g), live = p.n_end - n;
@@ -195,14 +195,10 @@ __device__ __forceinline__ void epilogue(const Linear8Params& p, int64_t m0, Col
           int32_t* const to = part + m * width + half * cols;
 #pragma unroll
           for (int i = 0; i < C; i += 4) {
-            const i32x4 v = {sum(a, g, half, i), sum(a, g, half, i + 1), sum(a, g, half, i + 2), sum(a, g, half, i + 3)};
-            if (live >= C) {
-              *reinterpret_cast<i32x4_any*>(to + i) = v;
-            } else {
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (i + r < live) to[i + r] = v[r];
-            }
+            // (a row's space is whole vectors: what lies past its columns is never used)
+            if (i < live)
+              *reinterpret_cast<i32x4*>(to + i) =
+                  i32x4{sum(a, g, half, i), sum(a, g, half, i + 1), sum(a, g, half, i + 2), sum(a, g, half, i + 3)};
           }
         }
       }
@@ -757,7 +753,7 @@ __global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_big_kernel(const L
 constexpr int kReduceThreads = 256;
 template <typename YT, bool GATED>
 __global__ void __launch_bounds__(kReduceThreads) linear8_reduce_kernel(const Linear8Params p, int splits) {
-  const int64_t cols = p.n_end - p.n_begin, quads = (cols + 3) / 4;
+  const int64_t cols = linear8_part_cols(p.n_end - p.n_begin), quads = cols / 4;
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kReduceThreads + threadIdx.x;
   const int64_t m = i / quads;
   if (m >= p.M) return;
@@ -767,23 +763,16 @@ __global__ void __launch_bounds__(kReduceThreads) linear8_reduce_kernel(const Li
 #pragma unroll
   for (int half = 0; half < (GATED ? 2 : 1); ++half) {
     const int32_t* const from = p.part + m * width + half * cols + at;
-    if (live >= 4) {
-      constexpr int kAhead = 8;  // loads in flight
-      for (int s = 0; s < splits; s += kAhead) {
-        i32x4 v[kAhead];
+    constexpr int kAhead = 8;  // loads in flight
+    for (int s = 0; s < splits; s += kAhead) {
+      i32x4 v[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-          v[j] = *reinterpret_cast<const i32x4_any*>(from + (s + j < splits ? s + j : splits - 1) * each);
+      for (int j = 0; j < kAhead; ++j)
+        v[j] = *reinterpret_cast<const i32x4*>(from + (s + j < splits ? s + j : splits - 1) * each);
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j)
+      for (int j = 0; j < kAhead; ++j)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) t[half][r] += s + j < splits ? v[j][r] : 0;
-      }
-    } else {
-      for (int s = 0; s < splits; ++s)
-#pragma unroll
-        for (int r = 0; r < 3; ++r)
-          if (r < live) t[half][r] += from[s * each + r];
+        for (int r = 0; r < 4; ++r) t[half][r] += s + j < splits ? v[j][r] : 0;
     }
   }
   Columns<4> ca, cb;
@@ -837,8 +826,7 @@ hipError_t launch_part(Linear8Params p, const Linear8Part& part, int32_t* work, 
       break;
     }
     case kLinear8Any: go(linear8_tile_kernel<YT, 128, 128, 2, 2, GATED>, 4); break;
-    case kLinear8Ring64: go(linear8_ring_kernel<YT, 64, 64, 2, 2, GATED>, 4); break;
-    case kLinear8Ring128: go(linear8_ring_kernel<YT, 64, 128, 1, 4, GATED>, 4); break;
+    case kLinear8Ring: go(linear8_ring_kernel<YT, 64, 64, 2, 2, GATED>, 4); break;
     case kLinear8Tile128:
       if (whole) go(linear8_big_kernel<YT, 128, 128, 2, 4, GATED, false>, 8);
       else go(linear8_big_kernel<YT, 128, 128, 2, 4, GATED, true>, 8);
@@ -851,7 +839,7 @@ hipError_t launch_part(Linear8Params p, const Linear8Part& part, int32_t* work, 
   if (p.part) {
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t threads = p.M * ((p.n_end - p.n_begin + 3) / 4);
+    const int64_t threads = p.M * (linear8_part_cols(p.n_end - p.n_begin) / 4);
     hipLaunchKernelGGL((linear8_reduce_kernel<YT, GATED>), dim3(static_cast<unsigned>((threads + kReduceThreads - 1) / kReduceThreads)),
                        dim3(kReduceThreads), 0, s, p, part.splits);
   }

@@ -38,7 +38,7 @@ struct LinearPlan {
   int steps;   // per split (even)
 };
 
-inline int64_t linear_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+constexpr int64_t linear_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Column fragments per wavefront of the band form: 8 wavefronts cover N = 256, 384 or 512 columns.
 inline int linear_band_fragments(int32_t N) { return N <= 256 ? 2 : (N <= 384 ? 3 : 4); }
@@ -166,8 +166,7 @@ enum Linear8Form {
   kLinear8Rows,  // few rows: operands straight to registers
   kLinear8Any,   // 128 x 128 tiles of operands at any address, any K
   // K a multiple of 16, 16-byte aligned operands, loaded straight to LDS:
-  kLinear8Ring64,   // 64 x 64 tiles
-  kLinear8Ring128,  // 64 x 128 tiles
+  kLinear8Ring,     // 64 x 64 tiles, a ring of four steps
   kLinear8Tile128,  // 128 x 128 tiles
   kLinear8Tile256,  // 256 x 256 tiles
 };
@@ -190,8 +189,7 @@ struct Linear8Tile {
 inline Linear8Tile linear8_tile(Linear8Form form, int64_t M) {
   switch (form) {
     case kLinear8Rows: return {M <= 16 ? 16 : 32, 16};
-    case kLinear8Ring64: return {64, 64};
-    case kLinear8Ring128: return {64, 128};
+    case kLinear8Ring: return {64, 64};
     case kLinear8Tile256: return {256, 256};
     default: return {128, 128};
   }
@@ -201,8 +199,10 @@ inline Linear8Tile linear8_tile(Linear8Form form, int64_t M) {
 inline int64_t linear8_pad_bytes(int64_t M, int32_t N, int32_t K, bool gated) {
   return (M + static_cast<int64_t>(N) * (gated ? 2 : 1)) * linear_ceil(K, kLinear8Step) * kLinear8Step;
 }
+// (partial sums: rows of whole 16-byte vectors)
+constexpr int64_t linear8_part_cols(int64_t cols) { return linear_ceil(cols, 4) * 4; }
 inline int64_t linear8_part_bytes(const Linear8Part& part, int64_t M, bool gated) {
-  return part.splits > 1 ? part.splits * M * (part.n_end - part.n_begin) * (gated ? 8 : 4) : 0;
+  return part.splits > 1 ? part.splits * M * linear8_part_cols(part.n_end - part.n_begin) * (gated ? 8 : 4) : 0;
 }
 inline int64_t linear8_plan_bytes(const Linear8Plan& plan, int64_t M, int32_t N, int32_t K, bool gated) {
   int64_t most = 0;  // the parts run one after the other
@@ -228,23 +228,122 @@ inline int64_t linear8_workgroups(const Linear8Plan& plan, int64_t M, bool gated
   return most;
 }
 
-inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, bool aligned, int64_t ws_bytes) {
-  const int nk = static_cast<int>(linear_ceil(K, kLinear8Step));
-  Linear8Plan plan{1, {{kLinear8Any, 1, nk, 0, N}, {}}, false};
-  Linear8Part& part = plan.part[0];
-  if (M > 16 && !aligned && ws_bytes >= linear8_pad_bytes(M, N, K, gated)) {
-    plan.padded = aligned = true;
-    ws_bytes -= linear8_pad_bytes(M, N, K, gated);
+// The estimated time (us) of one part. Workgroups run `slots` at a time (what fits the CUs); a round takes a fixed
+// time and a time per step, which grows from `step` to `full` as the round fills the chip. What the operands, the
+// output (more where rows of y are not whole 16-byte stores) and the partial sums of a split take beyond that is
+// added per million bytes or elements. Fitted to 94,000 timings of 16,000 random shapes (1 to 16,384 rows, 16 to
+// 16,384 outputs, K from 64 to 16,384, plain and gated); the plan chosen is on average 1.2% off the best of all
+// forms and splits (5% for rows of odd widths up to 32 rows). Measured, in us, rows | rings | 128 tiles | 256 tiles:
+//   16 x 1024 -> 1024: 3.1 | 4.9 | - | -            32 x 4096 -> 4096: 9.5 | 9.0 | - | -
+//   1024 x 1024 -> 1024: - | 6.5 | 7.7 | 15.8       2048 x 4096 -> 4096: - | 62 | 38.9 | 52.4
+//   4096 x 3584 -> 512: - | 13.7 | 21.1 | 36.6      8192 x 8192 -> 4096: - | 393 | 268 | 202
+inline double linear8_time(const Linear8Part& part, int64_t M, int32_t K, bool gated) {
+  struct Cost {
+    double launch, fixed, step, full, bytes, split, sums, out, out_odd;
+    int slots;
+  };
+  const int64_t cols = part.n_end - part.n_begin, wrows = cols * (gated ? 2 : 1);
+  const auto cost = [&]() -> Cost {
+    switch (part.form) {
+      case kLinear8Rows: return {2.64, 0.0, 0.076, 0.139, 0.087, 2.24, 1.22, 0.53, 0.34, 512};
+      case kLinear8Any: return {3.92, 2.90, 1.033, 1.655, 0.074, 0.13, 1.90, 0.88, 0.18, 512};
+      case kLinear8Ring: return {1.39, 1.91, 0.158, 0.417, 0.031, 1.95, 2.90, 0.13, 0.27, 512};
+      case kLinear8Tile128: return {0.93, 2.52, 0.449, 1.005, 0.062, 1.64, 2.27, 0.39, 0.37, 512};
+      default: return {1.00, 6.07, 1.060, 1.554, 0.0, 0.57, 1.53, 0.33, 0.47, 256};
+    }
+  }();
+  double slow = 1.0;
+  if (part.form == kLinear8Rows) {
+    if (M > 16) slow *= 1.82;         // two fragments of rows
+    if (gated) slow *= 2.09;
+    if (K % 16 != 0) slow *= 2.81;    // unaligned loads
   }
-  if (M <= 16) part.form = kLinear8Rows;
-  else if (aligned) part.form = M <= 64 ? kLinear8Ring64 : M <= 256 ? kLinear8Ring128 : M <= 2048 ? kLinear8Tile128 : kLinear8Tile256;
-  int64_t want = kLinearCus / linear8_tiles(part.form, M, N, gated);
-  const int64_t fit = ws_bytes / (M * N * (gated ? 8 : 4));
-  if (want > fit) want = fit;
-  if (want > nk / 2) want = nk / 2;
-  if (want > 1) {
-    part.steps = static_cast<int>(linear_ceil(nk, want));
-    part.splits = static_cast<int>(linear_ceil(nk, part.steps));
+  const int64_t groups = linear8_tiles(part.form, M, cols, gated) * part.splits;
+  const int64_t rounds = groups / cost.slots;
+  const double filled = static_cast<double>(groups % cost.slots) / cost.slots;
+  const double mn = 1e-6 * M * cols;
+  double t = cost.launch + rounds * (cost.fixed + cost.full * slow * part.steps);
+  if (filled > 0) t += cost.fixed + (cost.step + (cost.full - cost.step) * filled) * slow * part.steps;
+  if (part.splits > 1) t += cost.split + cost.sums * 1e-6 * M * wrows * part.splits;
+  return t + cost.bytes * 1e-6 * (wrows + M) * K + (cols % 8 == 0 ? cost.out : cost.out + cost.out_odd) * mn;
+}
+
+// What the host needs for a call, and for each launch beyond the first: a plan that is faster than that on the GPU
+// gains nothing.
+constexpr double kLinear8Host = 7.5, kLinear8HostLaunch = 3.5;
+
+// The best single part for columns n_begin .. n_end: its form and splits (at most as many as ws_bytes hold partial
+// sums of), and its estimated time.
+inline Linear8Part linear8_best(int64_t M, int32_t n_begin, int32_t n_end, int32_t K, bool gated, bool aligned,
+                                int64_t ws_bytes, double* time) {
+  const int nk = static_cast<int>(linear_ceil(K, kLinear8Step));
+  Linear8Part best{kLinear8Any, 1, nk, n_begin, n_end};
+  double best_cost = -1.0;
+  for (int f = kLinear8Rows; f <= kLinear8Tile256; ++f) {
+    const Linear8Form form = static_cast<Linear8Form>(f);
+    if (form == kLinear8Rows ? M > 32 : form != kLinear8Any && !aligned) continue;
+    const int64_t tiles = linear8_tiles(form, M, n_end - n_begin, gated);
+    for (int want = 1; want <= 32; want *= 2) {
+      Linear8Part part{form, 1, nk, n_begin, n_end};
+      if (want > 1) {
+        if (want > nk / 2 || tiles * want > 1024) break;
+        part.steps = static_cast<int>(linear_ceil(nk, want));
+        part.splits = static_cast<int>(linear_ceil(nk, part.steps));
+        if (linear8_part_bytes(part, M, gated) > ws_bytes) break;
+      }
+      const double t = linear8_time(part, M, K, gated);
+      const double host = kLinear8Host + (part.splits > 1 ? kLinear8HostLaunch : 0.0);
+      const double cost = t > host ? t : host + 1e-3 * t;  // level with the host: the fewest launches, then the GPU's time
+      if (best_cost < 0 || cost < best_cost) {
+        best_cost = cost;
+        best = part;
+        *time = t;
+      }
+    }
+  }
+  return best;
+}
+
+inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, bool aligned, int64_t ws_bytes) {
+  Linear8Plan plan{1, {}, false};
+  double time = 0;
+  plan.part[0] = linear8_best(M, 0, N, K, gated, aligned, ws_bytes, &time);
+  // Operands of odd widths (or addresses) copied to rows of whole steps first: 40 x 333 -> 1000: 10.7 | 7.9 us; 2000 x 4094
+  // -> 4096: 66 | 54 us.
+  const int64_t pad = linear8_pad_bytes(M, N, K, gated);
+  if (!aligned && ws_bytes >= pad) {
+    const int32_t to = static_cast<int32_t>(linear_ceil(K, kLinear8Step) * kLinear8Step);
+    double t = 0;
+    const Linear8Part part = linear8_best(M, 0, N, to, gated, true, ws_bytes - pad, &t);
+    t += 2.5 + 0.35e-6 * pad;
+    const auto cost = [](double t, int launches) {
+      const double host = kLinear8Host + kLinear8HostLaunch * (launches - 1);
+      return t > host ? t : host + 1e-3 * t;
+    };
+    if (cost(t, part.splits > 1 ? 3 : 2) < cost(time, plan.part[0].splits > 1 ? 2 : 1)) {
+      plan.part[0] = part;
+      plan.padded = aligned = true;
+      time = t;
+      K = to;
+      ws_bytes -= pad;
+    }
+  }
+  // Rounds of 256 x 256 tiles that fill the chip, and the columns left over in a form of their own: 8192 x 8192 -> 4352:
+  // 17 columns of 32 tiles are two rounds and a rest of 32.
+  if (aligned) {
+    const int64_t rows = linear_ceil(M, 256), wide = gated ? 128 : 256, tiles = rows * linear_ceil(N, wide);
+    const int64_t whole = tiles / kLinearCus * kLinearCus / rows * wide;  // columns of the whole rounds
+    if (tiles > kLinearCus && whole > 0 && whole < N) {
+      const int nk = static_cast<int>(linear_ceil(K, kLinear8Step));
+      const Linear8Part first{kLinear8Tile256, 1, nk, 0, static_cast<int32_t>(whole)};
+      double rest = 0;
+      const Linear8Part second = linear8_best(M, first.n_end, N, K, gated, true, ws_bytes, &rest);
+      if (linear8_time(first, M, K, gated) + rest < 0.95 * time) {
+        plan.parts = 2;
+        plan.part[0] = first;
+        plan.part[1] = second;
+      }
+    }
   }
   return plan;
 }
