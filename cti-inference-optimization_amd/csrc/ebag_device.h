@@ -397,4 +397,41 @@ __device__ __forceinline__ void quantize_chunk(const float* v, float s, float in
   }
 }
 
+// 16, 8 and 4 bytes at any address (the vector loads and stores of gfx950 take any).
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+typedef u32x2 u32x2_any __attribute__((aligned(1)));
+typedef uint32_t u32_any __attribute__((aligned(1)));
+
+__device__ __forceinline__ uint4 load16_any(const char* p) {
+  const u32x4 v = *reinterpret_cast<const u32x4_any*>(p);
+  return make_uint4(v.x, v.y, v.z, v.w);
+}
+
+// Maximum over the workgroup of non-negative values' bits (NaN above infinity above every number).
+template <int WAVES>
+__device__ __forceinline__ uint32_t block_max_bits(uint32_t v, uint32_t* s_red) {
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) {
+    const uint32_t o = static_cast<uint32_t>(shfl_i32(static_cast<int>(v), lane_id() ^ m));
+    v = o > v ? o : v;
+  }
+  if constexpr (WAVES > 1) {
+    if (lane_id() == 0) s_red[threadIdx.x / kWave] = v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) v = s_red[i] > v ? s_red[i] : v;
+  }
+  return v;
+}
+
+// VEC bytes, values as quantize_chunk leaves them.
+template <int VEC>
+__device__ __forceinline__ void store_bytes(int8_t* dst, const uint32_t* b) {
+  uint32_t w[VEC / 4];
+#pragma unroll
+  for (int i = 0; i < VEC / 4; ++i) w[i] = b[4 * i] | (b[4 * i + 1] << 8) | (b[4 * i + 2] << 16) | (b[4 * i + 3] << 24);
+  if constexpr (VEC == 4) *reinterpret_cast<u32_any*>(dst) = w[0];
+  else *reinterpret_cast<u32x2_any*>(dst) = u32x2{w[0], w[1]};
+}
+
 }  // namespace cti

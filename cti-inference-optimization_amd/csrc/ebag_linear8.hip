@@ -31,8 +31,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef i32x4 i32x4_any __attribute__((aligned(1)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
-typedef u32x2 u32x2_any __attribute__((aligned(2)));
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
 
 constexpr int kStep = kLinear8Step;  // bytes of K per step
 constexpr int kXcds = 8;

@@ -106,12 +106,10 @@ def quantize_embedding_int8(weight: torch.Tensor):
         raise ValueError("weight must be a row-major 2-D tensor with unit column stride")
     rows, dim = weight.shape
     dev = weight.device
-    q = torch.empty((rows, dim), dtype=torch.int8, device=dev)
+    q = torch.empty(rows, dim, dtype=torch.int8, device=dev)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _capi.check(_capi.lib().cti_ebag_quantize_int8(
-            weight.data_ptr(), _capi.dtype_code(weight.dtype), rows, dim, weight.stride(0), q.data_ptr(),
-            scale.data_ptr(), _capi.current_stream_handle(dev)))
+    _launch(dev.index, _capi.lib().cti_ebag_quantize_int8, weight.data_ptr(), _capi.dtype_code(weight.dtype), rows, dim,
+            weight.stride(0), q.data_ptr(), scale.data_ptr())
     return q, scale
 
 

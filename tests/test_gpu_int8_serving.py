@@ -631,3 +631,23 @@ def test_python_refusals(pkg, dev):
     flat = torch.zeros(4 * 64 + 1, device=dev)
     with pytest.raises(pkg.EbagError, match="overlaps"):
         pkg.rms_norm_int8(flat[:-1].view(4, 64), g, residual=x, residual_out=flat[1:].view(4, 64))
+
+
+@pytest.mark.parametrize("dim", [513, 1000, 1021, 2048, 4097, 5632, 14336, 16391, 32768, 40000])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_wide_rows_are_quantised_as_narrow_ones(pkg, dev, dim, dt):
+    """Bit for bit the expression that quantize_embedding_int8 states, rows with a stride and odd addresses too."""
+    g = _gen(dim)
+    x = torch.randn(37, dim, generator=g) * torch.exp(torch.randn(37, 1, generator=g))
+    x[5] = 0
+    x[7, dim - 1] = 50.0
+    x = x.to(dt)
+    for shift, pad in ((0, 0), (1, 0), (0, 5), (3, 8)):
+        print(f"wide rows dim={dim} {dt} shift={shift} pad={pad}", flush=True)
+        base = torch.zeros(37 * (dim + pad) + shift, dtype=dt, device=dev)
+        view = base[shift:].view(37, dim + pad)[:, :dim]
+        view.copy_(x)
+        q, s = pkg.quantize_embedding_int8(view)
+        want_s = torch.clamp(x.float().abs().amax(1) * np.float32(1 / 127), min=np.float32(1e-8))
+        want_q = torch.clamp(torch.round(x.float() / want_s[:, None]), -128, 127).to(torch.int8)
+        assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu(), want_q)
