@@ -68,11 +68,39 @@ struct Params {
   }
 };
 
+// The larger of m and every |v|, NaN if any is: one instruction for two of them.
+template <int N>
+__device__ __forceinline__ float top_of(float m, const float* v) {
+#pragma unroll
+  for (int e = 0; e < N; e += 2)
+    m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(__builtin_fabsf(v[e]), __builtin_fabsf(v[e + 1])), m);
+  return m;
+}
+
 // The scale of a row whose largest |y| has these bits; NaN for infinity and NaN.
 __device__ __forceinline__ float scale_of(uint32_t bits) {
   const float s = __uint_as_float(bits) * (1.0f / 127.0f);
   if (bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
   return s < 1e-8f ? 1e-8f : s;
+}
+
+// VEC bytes rint(v / s), given inv = RN32(1 / s): the product with inv is exact inside the addition of 1.5 * 2^23, which
+// leaves the nearest integer in the low byte, so a byte differs from the quotient's only where v / s is within 2^-17 of
+// the middle of two. |v / s| <= 127 (1 + 2^-22). `live` false (the row's scale is NaN): zeros.
+template <int VEC>
+__device__ __forceinline__ void store_quantised(int8_t* dst, const float* v, float inv, bool live) {
+  constexpr float kMagic = 12582912.f;
+  uint32_t w[VEC / 4];
+#pragma unroll
+  for (int i = 0; i < VEC / 4; ++i) {
+    uint32_t b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = __float_as_uint(__builtin_fmaf(v[4 * i + e], inv, kMagic));
+    const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0c0c0400u);
+    w[i] = live ? __builtin_amdgcn_perm(hi, lo, 0x05040100u) : 0u;
+  }
+  if constexpr (VEC == 4) *reinterpret_cast<u32_any*>(dst) = w[0];
+  else *reinterpret_cast<u32x2_any*>(dst) = u32x2{w[0], w[1]};
 }
 
 // 1 / sqrt(var + eps); NaN where the sum of squares left fp32's range (it would give a row of zeros).
@@ -125,10 +153,8 @@ __global__ void __launch_bounds__(WAVES * kWave) norm8_rows_kernel(const Norm8Pa
     }
   }
   float v[K][VEC];
-  float s = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int i = t + k * THREADS;
     unpack16(rx[k], v[k], T{});
     if (p.res) {
       float r[VEC];
@@ -136,32 +162,44 @@ __global__ void __launch_bounds__(WAVES * kWave) norm8_rows_kernel(const Norm8Pa
 #pragma unroll
       for (int e = 0; e < VEC; ++e) v[k][e] += r[e];
     }
-    // the elements that this vector shares with the one before it do not count (vectors past the row hold 0)
-    const int shared = i == nfull ? VEC - rest : 0;
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const float c = e >= shared ? v[k][e] : 0.f;
-      s += p.layer ? c : c * c;
-    }
   }
-  const float n = static_cast<float>(cols);
-  s = block_sum<WAVES>(s, s_sum) / n;
-  float mean = 0.f;
-  if (p.layer) {
-    mean = s;
-    s = 0.f;
+  // f over the elements that count: not those that the last vector shares with the one before it, and where `beyond`
+  // is set not those of vectors past the row (which hold 0)
+  const auto each = [&](bool beyond, auto&& f) {
+    if (rest == 0) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int i = t + k * THREADS;
-      const int shared = i < nfull ? 0 : (i < nvec ? VEC - rest : VEC);
+      for (int k = 0; k < K; ++k) {
+        if (beyond && t + k * THREADS >= nvec) continue;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float d = e >= shared ? v[k][e] - mean : 0.f;
-        s += d * d;
+        for (int e = 0; e < VEC; ++e) f(v[k][e], true);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int i = t + k * THREADS;
+        const int shared = i < nfull ? 0 : (i < nvec ? VEC - rest : (beyond ? VEC : 0));
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f(v[k][e], e >= shared);
       }
     }
-    s = block_sum<WAVES>(s, s_sum) / n;
+  };
+  const float n = static_cast<float>(cols);
+  float mean = 0.f, s = 0.f;
+  if (p.layer) {
+    each(false, [&](float& x, bool counts) { s += counts ? x : 0.f; });
+    mean = block_sum<WAVES>(s, s_sum) / n;
+    s = 0.f;
+    each(true, [&](float& x, bool counts) {
+      const float d = counts ? x - mean : 0.f;
+      s = __builtin_fmaf(d, d, s);
+    });
+  } else {
+    each(false, [&](float& x, bool counts) {
+      const float c = counts ? x : 0.f;
+      s = __builtin_fmaf(c, c, s);
+    });
   }
+  s = block_sum<WAVES>(s, s_sum) / n;
   const float rstd = rstd_of(s, p.eps);
   if (p.res) {
     with_stream(p.stream_out, [&](auto stream) {
@@ -176,7 +214,7 @@ __global__ void __launch_bounds__(WAVES * kWave) norm8_rows_kernel(const Norm8Pa
       }
     });
   }
-  uint32_t top = 0u;
+  float top = 0.f;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int i = t + k * THREADS;
@@ -187,31 +225,101 @@ __global__ void __launch_bounds__(WAVES * kWave) norm8_rows_kernel(const Norm8Pa
         if (p.layer) bt[0].load(p.beta, first(i));
       }
       gm[kEarly ? k : 0].unpack(g);
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[k][e] = (v[k][e] - mean) * rstd * g[e];
       if (p.layer) {
         bt[kEarly ? k : 0].unpack(b);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[k][e] += b[e];
-      }
+        for (int e = 0; e < VEC; ++e) v[k][e] = __builtin_fmaf((v[k][e] - mean) * rstd, g[e], b[e]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const uint32_t a = __float_as_uint(v[k][e]) & 0x7fffffffu;
-        top = a > top ? a : top;
+        for (int e = 0; e < VEC; ++e) v[k][e] = v[k][e] * rstd * g[e];
       }
+      top = top_of<VEC>(top, v[k]);
     }
   }
-  const float sc = scale_of(block_max_bits<WAVES>(top, s_max));
+  const float sc = scale_of(block_max_bits<WAVES>(__float_as_uint(top) & 0x7fffffffu, s_max));
   if (t == 0) p.scale[row] = sc;
   const float inv = 1.0f / sc;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int i = t + k * THREADS;
-    if (i < nvec) {
-      uint32_t b[VEC];
-      quantize_chunk<VEC>(v[k], sc, inv, b);
-      store_bytes<VEC>(p.q + at + first(i), b);
+    if (i < nvec) store_quantised<VEC>(p.q + at + first(i), v[k], inv, sc == sc);
+  }
+}
+
+// Narrow rows: a group of 1 << lg lanes holds a row, a vector a lane; a wavefront has 64 >> lg rows side by side.
+// (32,768 rows of 64 bf16 took ? us with a wavefront for each.)
+constexpr int kNarrowWaves = 4;
+template <typename T, typename PT>
+__global__ void __launch_bounds__(kNarrowWaves * kWave) norm8_narrow_kernel(const Norm8Params p, int64_t rows, int lg) {
+  constexpr int VEC = 16 / Elem<T>::kBytes;
+  const int lane = lane_id(), i = lane & ((1 << lg) - 1);
+  const int64_t row = ((static_cast<int64_t>(blockIdx.x) * kNarrowWaves + threadIdx.x / kWave) << (6 - lg)) + (lane >> lg);
+  const int cols = static_cast<int>(p.cols);
+  const int nfull = cols / VEC, rest = cols % VEC;
+  const bool live = row < rows && i < nfull + (rest != 0);  // (lanes stay: the sums are taken across lanes)
+  const int first = i < nfull ? i * VEC : cols - VEC;
+  const int64_t at = row * cols + first;
+  uint4 rx = make_uint4(0u, 0u, 0u, 0u), rr = rx;
+  Params<PT, VEC> gm = {}, bt = {};
+  if (live) {
+    rx = load16_any(p.x + at * Elem<T>::kBytes);
+    if (p.res) rr = load16_any(p.res + at * Elem<T>::kBytes);
+    gm.load(p.gamma, first);
+    if (p.layer) bt.load(p.beta, first);
+  }
+  float v[VEC];
+  unpack16(rx, v, T{});
+  if (p.res) {
+    float r[VEC];
+    unpack16(rr, r, T{});
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] += r[e];
+  }
+  const auto group_sum = [&](float s) {
+    for (int m = 1; m < (1 << lg); m <<= 1) s += shfl_xor_f32(s, m);
+    return s;
+  };
+  const int shared = !live ? VEC : (i == nfull ? VEC - rest : 0);  // elements that do not count
+  const float n = static_cast<float>(cols);
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    const float c = e >= shared ? v[e] : 0.f;
+    s = p.layer ? s + c : __builtin_fmaf(c, c, s);
+  }
+  s = group_sum(s) / n;
+  float mean = 0.f;
+  if (p.layer) {
+    mean = s;
+    s = 0.f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float d = e >= shared ? v[e] - mean : 0.f;
+      s += d * d;
     }
+    s = group_sum(s) / n;
+  }
+  const float rstd = rstd_of(s, p.eps);
+  if (live && p.res) {
+    u32x4_any* const dst = reinterpret_cast<u32x4_any*>(p.res_out + at * Elem<T>::kBytes);
+    if (p.stream_out) __builtin_nontemporal_store(pack16(v, T{}), dst);
+    else *dst = pack16(v, T{});
+  }
+  float g[VEC], b[VEC];
+  gm.unpack(g);
+  bt.unpack(b);
+#pragma unroll
+  for (int e = 0; e < VEC; ++e)
+    v[e] = p.layer ? __builtin_fmaf((v[e] - mean) * rstd, g[e], b[e]) : v[e] * rstd * g[e];
+  uint32_t top = live ? __float_as_uint(top_of<VEC>(0.f, v)) & 0x7fffffffu : 0u;
+  for (int m = 1; m < (1 << lg); m <<= 1) {
+    const uint32_t o = static_cast<uint32_t>(shfl_i32(static_cast<int>(top), lane ^ m));
+    top = o > top ? o : top;
+  }
+  const float sc = scale_of(top);
+  if (live) {
+    if (i == 0) p.scale[row] = sc;
+    store_quantised<VEC>(p.q + at, v, 1.0f / sc, sc == sc);
   }
 }
 
@@ -255,16 +363,14 @@ __global__ void __launch_bounds__(kLoopThreads) norm8_loop_kernel(const Norm8Par
   T* const ro = reinterpret_cast<T*>(p.res_out);
   for (int64_t c = threadIdx.x; c < p.cols; c += kLoopThreads) {
     const float hc = h(c);
-    float v = y(c, hc);
-    uint32_t b;
-    quantize_chunk<1>(&v, sc, inv, &b);
-    p.q[at + c] = static_cast<int8_t>(b);
+    p.q[at + c] = sc == sc ? static_cast<int8_t>(rintf(y(c, hc) * inv)) : static_cast<int8_t>(0);
     if (p.res) store_one(ro + at + c, hc, false);
   }
 }
 
-// The fewest registers that hold the row: with rows enough to fill the card a wavefront takes up to 8
-// vectors per lane (no barrier up to 512 vectors), with fewer rows more wavefronts share one.
+// Wavefronts per row: the time of a row alone counts while rows are few, and a wavefront with 8 vectors per lane leaves too
+// little else on its SIMD (16,384 rows of 4,096 bf16 with a residual: 82 us with 4 wavefronts of 2 vectors per lane,
+// 88 with 4 of 4, 101 with one of 8; one row: 4.4 us with 8 of 1, 5.2 with 4 of 2, 9.3 with one of 8).
 template <typename T, typename PT>
 hipError_t launch_norm8(const Norm8Params& p, int64_t rows, hipStream_t s) {
   constexpr int VEC = 16 / Elem<T>::kBytes;
@@ -280,26 +386,29 @@ hipError_t launch_norm8(const Norm8Params& p, int64_t rows, hipStream_t s) {
   constexpr integral_constant<int, 4> n4{};
   constexpr integral_constant<int, 8> n8{};
   constexpr integral_constant<int, 16> n16{};
-  const bool few = rows < 1024;
+  const bool few = rows < 1536;  // too few to fill the card with 8 wavefronts each
   if (p.cols < VEC || nvec > 64 * kWave) {
     hipLaunchKernelGGL((norm8_loop_kernel<T, PT>), grid, dim3(kLoopThreads), 0, s, p);
+  } else if (nvec <= kWave / 2) {
+    int lg = 0;
+    while ((1 << lg) < nvec) ++lg;
+    const int64_t per = static_cast<int64_t>(kNarrowWaves) << (6 - lg);
+    hipLaunchKernelGGL((norm8_narrow_kernel<T, PT>), dim3(static_cast<unsigned>((rows + per - 1) / per)),
+                       dim3(kNarrowWaves * kWave), 0, s, p, rows, lg);
   } else if (nvec <= kWave) {
     go(n1, n1);
-  } else if (few) {
-    if (nvec <= 4 * kWave) go(n1, n4);
-    else if (nvec <= 16 * kWave) go(n1, n16);
-    else if (nvec <= 32 * kWave) go(n2, n16);
-    else go(n4, n16);
   } else if (nvec <= 2 * kWave) {
-    go(n2, n1);
+    go(n1, n2);
   } else if (nvec <= 4 * kWave) {
-    go(n4, n1);
+    go(n1, n4);
   } else if (nvec <= 8 * kWave) {
-    go(n8, n1);
+    if (few) go(n1, n8);
+    else go(n2, n4);
   } else if (nvec <= 16 * kWave) {
-    go(n4, n4);
+    go(n2, n8);
   } else if (nvec <= 32 * kWave) {
-    go(n8, n4);
+    if (few) go(n2, n16);
+    else go(n4, n8);
   } else {
     go(n4, n16);
   }

@@ -266,53 +266,70 @@ void launch_quantize(const char* w, int64_t rows, int64_t dim, int64_t row_strid
 
 // ---------------------------------------------------------------------------------------------
 // The way back: out[r, j] = q[r, j] * scale[r] in fp32, rounded once to the output type.
-// Both arrays are contiguous, so a thread takes 16 consecutive bytes wherever rows begin and end in
-// them, and stores 16 consecutive values. Bound by HBM (one byte read and 2 or 4 written an element).
+// Both arrays are contiguous, so a chunk is as many consecutive elements as 16 bytes of output hold, wherever rows
+// begin and end in them, and a wavefront's chunks are side by side (with 64 bytes a lane in four stores, 8,192 x 8,192
+// to fp32 took 202 us). Bound by HBM (one byte read and 2 or 4 written an element).
 // ---------------------------------------------------------------------------------------------
-constexpr int kDequantElems = 16;  // per thread
+constexpr int kDequantChunks = 4;  // per thread
 
 template <typename T, typename I>
 __global__ void __launch_bounds__(kQuantThreads) dequantize_rows_kernel(const int8_t* q, const float* scale, I total,
                                                                         I dim, char* out, int32_t stream_out) {
-  const I e0 = (static_cast<I>(blockIdx.x) * kQuantThreads + threadIdx.x) * kDequantElems;
-  if (e0 >= total) return;
-  I row = e0 / dim;
-  I left = dim - (e0 - row * dim);  // elements of this row from e0 on
-  T* const dst = reinterpret_cast<T*>(out) + e0;
-  if (total - e0 < kDequantElems) {
-    for (I e = 0; e < total - e0; ++e, --left) {
-      if (left == 0) {
-        ++row;
-        left = dim;
-      }
-      store_one(dst + e, static_cast<float>(q[e0 + e]) * scale[row], false);
-    }
-    return;
+  constexpr int C = 16 / Elem<T>::kBytes;
+  using V = std::conditional_t<C == 4, u32_any, u32x2_any>;
+  const I first = static_cast<I>(blockIdx.x) * (kQuantThreads * kDequantChunks) + threadIdx.x;
+  V raw[kDequantChunks];
+#pragma unroll
+  for (int u = 0; u < kDequantChunks; ++u) {
+    const I e0 = (first + u * kQuantThreads) * C;
+    raw[u] = V{};
+    if (e0 + C <= total) raw[u] = *reinterpret_cast<const V*>(q + e0);
   }
-  const u32x4 raw = *reinterpret_cast<const u32x4_any*>(q + e0);
-  float s = scale[row];
-  float v[kDequantElems];
 #pragma unroll
-  for (int e = 0; e < kDequantElems; ++e) v[e] = static_cast<float>(static_cast<int8_t>(raw[e / 4] >> (8 * (e % 4))));
-  if (left >= kDequantElems) {
-#pragma unroll
-    for (int e = 0; e < kDequantElems; ++e) v[e] *= s;
-  } else {
-#pragma unroll
-    for (int e = 0; e < kDequantElems; ++e, --left) {
-      if (left == 0) {
-        s = scale[++row];
-        left = dim;
+  for (int u = 0; u < kDequantChunks; ++u) {
+    const I e0 = (first + u * kQuantThreads) * C;
+    if (e0 >= total) return;
+    I row = e0 / dim;
+    I left = dim - (e0 - row * dim);  // elements of this row from e0 on
+    T* const dst = reinterpret_cast<T*>(out) + e0;
+    if (e0 + C > total) {
+      for (I e = 0; e < total - e0; ++e, --left) {
+        if (left == 0) {
+          ++row;
+          left = dim;
+        }
+        store_one(dst + e, static_cast<float>(q[e0 + e]) * scale[row], false);
       }
-      v[e] *= s;
+      return;
     }
+    float s = scale[row], v[C];
+#pragma unroll
+    for (int e = 0; e < C; ++e) {
+      uint32_t w;
+      if constexpr (C == 4) w = raw[u];
+      else w = raw[u][e / 4];
+      v[e] = static_cast<float>(static_cast<int8_t>(w >> (8 * (e % 4))));
+    }
+    if (left >= C) {
+#pragma unroll
+      for (int e = 0; e < C; ++e) v[e] *= s;
+    } else {
+#pragma unroll
+      for (int e = 0; e < C; ++e, --left) {
+        if (left == 0) {
+          s = scale[++row];
+          left = dim;
+        }
+        v[e] *= s;
+      }
+    }
+    with_stream(stream_out, [&](auto stream) { store_out<C>(dst, v, decltype(stream)::value); });
   }
-  with_stream(stream_out, [&](auto stream) { store_out<kDequantElems>(dst, v, decltype(stream)::value); });
 }
 
 template <typename T>
 void launch_dequantize(const int8_t* q, const float* scale, int64_t total, int64_t dim, char* out, hipStream_t s) {
-  constexpr int64_t kPer = int64_t{kQuantThreads} * kDequantElems;
+  constexpr int64_t kPer = int64_t{kQuantThreads} * kDequantChunks * (16 / Elem<T>::kBytes);
   const dim3 grid(static_cast<unsigned>((total + kPer - 1) / kPer)), block(kQuantThreads);
   const int32_t stream_out = total * Elem<T>::kBytes >= kStreamOutBytes;
   if (total + kPer <= UINT32_MAX)
