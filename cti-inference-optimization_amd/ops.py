@@ -125,8 +125,9 @@ def dequantize_embedding_int8(q: torch.Tensor, scale: torch.Tensor, out_dtype: t
     return out
 
 
-# The int8 operators take a few microseconds on the GPU, as long as a call's way through Python takes: their checks
-# go by device indexes, build no device or stream objects, and allocate in the forms of torch.empty that return soonest.
+# The int8 operators take a few microseconds on the GPU, as long as a call's way through Python takes. So their checks are
+# one expression each, explained only when it fails; devices are compared by index, no device or stream objects are built,
+# and memory comes from the forms of torch.empty that return soonest.
 def _require_on(name: str, t, index: Optional[int] = None) -> int:
     """`t` is a contiguous GPU tensor (on device `index`); return its device's index."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or (index is not None and t.get_device() != index):
@@ -136,28 +137,37 @@ def _require_on(name: str, t, index: Optional[int] = None) -> int:
     return t.get_device()
 
 
-def _launch(index: int, fn, *args) -> None:
-    """Call a C entry point with `args` and torch's current stream on device `index`, with that device the
-    current one."""
-    if index == torch.cuda.current_device():
-        status = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, _raw_stream(index))
-    if status != _capi.OK:
-        _capi.check(status)
-
-
 def _raw_stream(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
 
-if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a Stream object
+_current_device = torch.cuda.current_device
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same without a Stream object; the tensors are there: torch.cuda is up
     _raw_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811
+    _current_device = torch._C._cuda_getDevice
+
+
+def _launch(index: int, fn, *args) -> None:
+    """Call a C entry point with `args` and torch's current stream on device `index`, with that device the
+    current one."""
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        _capi.check(status)
 
 
 def _check_int8_rows(name: str, q, scale_name: str, scale, index: Optional[int] = None):
     """Validate int8 rows and their scales; return (rows, columns, device index)."""
+    if (isinstance(q, torch.Tensor) and isinstance(scale, torch.Tensor) and q.is_cuda and scale.is_cuda
+            and q.dtype is torch.int8 and scale.dtype is torch.float32 and q.is_contiguous() and scale.is_contiguous()
+            and q.dim() == 2 and scale.dim() == 1):
+        rows, cols = q.shape
+        at = q.get_device()
+        if scale.numel() == rows and cols >= 1 and scale.get_device() == at and (index is None or index == at):
+            return rows, cols, at
     index = _require_on(name, q, index)
     _require_on(scale_name, scale, index)
     if q.dim() != 2 or q.shape[1] < 1:
@@ -166,10 +176,7 @@ def _check_int8_rows(name: str, q, scale_name: str, scale, index: Optional[int] 
         raise TypeError(f"{name} must be int8 (got {q.dtype})")
     if scale.dtype is not torch.float32:
         raise TypeError(f"{scale_name} must be float32 (got {scale.dtype})")
-    rows, cols = q.shape
-    if scale.dim() != 1 or scale.numel() != rows:
-        raise ValueError(f"{scale_name} has shape {tuple(scale.shape)}, expected ({rows},)")
-    return rows, cols, index
+    raise ValueError(f"{scale_name} has shape {tuple(scale.shape)}, expected ({q.shape[0]},)")
 
 
 def _float_output(out: Optional[torch.Tensor], rows: int, cols: int, dtype: torch.dtype, like: torch.Tensor, index: int):

@@ -267,6 +267,31 @@ def test_linear_is_exact(pkg, dev, rows, cols, n):
             assert torch.equal(got.cpu(), want), (split, int((got.cpu() != want).sum()))
 
 
+# Products too large for the CPU: every form of the large plans (256 x 256 tiles with and without a rest of K, a rest of
+# columns in another form, operands copied to whole steps), against float64 on the device.
+LARGE = [(8192, 256, 2048, False), (4100, 640, 4100, False), (4100, 272, 4100, False), (4096, 1000, 4200, False),
+         (8000, 130, 4099, False), (2500, 1040, 2049, False), (4100, 640, 2050, True), (4096, 1008, 2176, True),
+         (3001, 333, 1500, True), (8192, 512, 1024, True), (2048, 2048, 2048, False)]
+
+
+@pytest.mark.parametrize("rows,cols,n,gated", LARGE)
+def test_large_products(pkg, dev, rows, cols, n, gated):
+    print(f"large rows={rows} cols={cols} n={n} gated={gated}", flush=True)
+    wrows = 2 * n if gated else n
+    q, s, w, ws, bias = (t.to(dev) for t in _operands(rows, cols, wrows, rows + n))
+    t = q.double() @ w.double().t().contiguous()
+    v = (t.float() * s[:, None]) * ws[None, :] + bias[None, :]  # as _value: one rounding an operation
+    for odt in (torch.bfloat16, torch.float32):
+        if gated:
+            got = pkg.gated_linear_int8(q, s, w, ws, bias, activation="relu", out_dtype=odt)
+            want = torch.clamp(v[:, :n], min=0.0) * v[:, n:]
+        else:
+            got = pkg.linear_int8(q, s, w, ws, bias, out_dtype=odt)
+            want = v
+        torch.cuda.synchronize()
+        assert torch.equal(got, want.to(odt)), int((got != want.to(odt)).sum())
+
+
 @pytest.mark.parametrize("rows,cols,n", [(1, 131071, 20), (40, 131071, 24), (300, 131071, 40)])
 def test_the_largest_sums_do_not_overflow(pkg, dev, rows, cols, n):
     print(f"largest sums rows={rows}", flush=True)

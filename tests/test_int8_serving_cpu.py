@@ -152,3 +152,21 @@ def test_plans_cover_the_product_and_fit_the_workspace(rules, pkg, gated):
                         assert nbytes <= ws
                         if bool(aligned) == (K % 16 == 0):
                             assert nbytes <= query
+
+
+def test_the_gpu_tests_reach_every_plan(rules):
+    """Each form, K split and whole, copied operands, and a rest of columns in a form of its own."""
+    import test_gpu_int8_serving as g
+
+    seen = set()
+    shapes = [(m, k, n, 0) for m, k, n in g.SHAPES] + [(m, k, n, int(gated)) for m, k, n, gated in g.LARGE]
+    for M, K, N, gated in shapes:
+        plan, _, _ = rules(M, N, K, gated, K % 16 == 0, 1 << 62)
+        for i, part in enumerate(plan.part[:plan.parts]):
+            seen |= {("form", part.form), ("split", part.form in (0, 2) and part.splits > 1), ("padded", bool(plan.padded)),
+                     ("part", i), ("rest of K", part.form, K % 128 != 0 and not plan.padded)}
+        if not gated:  # without a workspace
+            seen |= {("form", rules(M, N, K, 0, K % 16 == 0, 0)[0].part[0].form)}
+    want = {("form", f) for f in range(5)} | {("split", True), ("padded", True), ("part", 1)}
+    want |= {("rest of K", f, tail) for f in (0, 2, 3, 4) for tail in (False, True)}
+    assert want - seen == set()
