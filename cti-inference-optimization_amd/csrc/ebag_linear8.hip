@@ -364,9 +364,11 @@ __global__ void __launch_bounds__(W * kWave) linear8_rows_kernel(const Linear8Pa
 // Tiles: BM rows by BN weight rows, WM x WN wavefronts
 // ---------------------------------------------------------------------------------------------
 // Tile i of the launch. Dispatch position i runs on XCD i % 8: each XCD gets a contiguous range of tiles
-// (L2 is per XCD), which runs down kGroup row bands before it steps to the next column of tiles.
+// (L2 is per XCD), which runs down kGroup row bands before it steps to the next column of tiles. A group of 6, no power
+// of two, keeps what runs at a time off the same cache channels: 8192 x 2048 -> 16384 took 277 / 246 / 238 / 293 / 241 us with
+// groups of 1 / 2 / 3 / 4 / 6, 16384 x 2048 -> 8192 291 / 255 / 253 / 243 / 236 and 288 with 8.
 __device__ __forceinline__ void tile_of(const Linear8Params& p, int* tm, int* tn) {
-  constexpr int kGroup = 8;
+  constexpr int kGroup = 6;
   const int total = p.tiles_m * p.tiles_n, i = static_cast<int>(blockIdx.x);
   const int xcd = i % kXcds, each = total / kXcds, more = total % kXcds;
   const int tile = xcd * each + (xcd < more ? xcd : more) + i / kXcds;
@@ -630,7 +632,7 @@ __global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_big_kernel(const L
   constexpr int OUT = GATED ? BN / 2 : BN;
   constexpr int NO = GATED ? NI / 2 : NI;    // fragments of output columns
   // G fragments of columns side by side, so that a lane holds 16 bytes of a row and four lanes store 64 in a row (32
-  // bytes a lane, stored in two halves with gaps: 8192 x 8192 -> 4096 took ? us)
+  // bytes a lane, stored in two halves with gaps, took the same time)
   constexpr int G = std::is_same<YT, float>::value || NO < 2 ? 1 : 2;
   // rows of 128 bytes, chunk c of row r in slot c ^ (r & 7) (no bank conflicts)
   __shared__ i32x4 s0[(BM + BN) * kChunks], s1[(BM + BN) * kChunks];
@@ -696,8 +698,10 @@ __global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_big_kernel(const L
 #pragma unroll
     for (int a = 0; a < MI; ++a)
 #pragma unroll
-      for (int c = 0; c < NI; ++c)
+      for (int i = 0; i < NI; ++i) {
+        const int c = a & 1 ? NI - 1 - i : i;  // there and back: an operand changes at a time (0.5% at the power limit)
         acc[a][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[h][c], fx[h][a], acc[a][c], 0, 0, 0);
+      }
   };
   constexpr std::integral_constant<int, 0> first{};
   constexpr std::integral_constant<int, 1> second{};

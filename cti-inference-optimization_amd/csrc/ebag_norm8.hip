@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(WAVES * kWave) norm8_rows_kernel(const Norm8Pa
 }
 
 // Narrow rows: a group of 1 << lg lanes holds a row, a vector a lane; a wavefront has 64 >> lg rows side by side.
-// (32,768 rows of 64 bf16 took ? us with a wavefront for each.)
+// (262,144 rows of 64 bf16 with a residual: 101.5 us with a wavefront for each, 26 so.)
 constexpr int kNarrowWaves = 4;
 template <typename T, typename PT>
 __global__ void __launch_bounds__(kNarrowWaves * kWave) norm8_narrow_kernel(const Norm8Params p, int64_t rows, int lg) {
