@@ -13,11 +13,15 @@
 // t[m0 + l % 16][n0 + 4 (l / 16) + r], r < 4: four consecutive columns of one row.
 //
 // Forms, chosen by linear8_plan:
-//   rows   few rows: bound by reading the weight once. A wavefront owns 16 columns (gated: 16 gates and
-//          their 16 values) and a share of K, weights and rows straight to registers; the wavefronts of a
-//          workgroup split K and add their sums through LDS.
-//   tiles  both operands through LDS. When the tiles would leave CUs idle, K is split over workgroups,
-//          each writing int32 partial sums to the caller's workspace, added by a second kernel.
+//   rows   few rows or few outputs: bound by reading the weight, or by the way to memory and back. A workgroup owns
+//          16 rows by 16 columns (gated: 16 gates and their 16 values); its wavefronts split K, load both operands
+//          straight to registers and add their sums through LDS.
+//   ring   64 x 64 tiles through LDS, a ring of four steps loaded straight to it.
+//   tiles  128 x 128 and 256 x 256 tiles, two steps in LDS, fragments read half a step ahead.
+//   any    128 x 128 tiles of operands at any address and any width, through registers: without a workspace. With one,
+//          operands of odd widths are copied to rows of whole steps first.
+// Where tiles would leave CUs idle, K is split over workgroups, each writing int32 partial sums to the caller's
+// workspace, added by a second kernel.
 #include <stdint.h>
 
 #include "ebag_device.h"
@@ -267,32 +271,28 @@ __device__ __forceinline__ i32x4 load_chunk(const int8_t* row, int k, int K) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Few rows (M <= 16 MT)
+// Few rows, or few outputs: 16 rows by 16 columns (gated: of gates and of values) a workgroup
 // ---------------------------------------------------------------------------------------------
-template <typename YT, int W, int MT, int U, bool GATED>
+template <typename YT, int W, int U, bool GATED>
 __global__ void __launch_bounds__(W * kWave) linear8_rows_kernel(const Linear8Params p) {
   constexpr int NT = GATED ? 2 : 1;
-  __shared__ i32x4 s_acc[W > 1 ? W : 1][MT * NT][kWave];
+  __shared__ i32x4 s_acc[W][NT][kWave];
   const int t = static_cast<int>(threadIdx.x);
   const int lane = t & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(t / kWave);
   const int fr = lane & 15, fq = lane >> 4;
-  const int n0 = p.n_begin + static_cast<int>(blockIdx.x) * 16;
+  const int tile_m = static_cast<int>(blockIdx.x) / p.tiles_n;
+  const int n0 = p.n_begin + (static_cast<int>(blockIdx.x) - tile_m * p.tiles_n) * 16;
+  const int64_t m0 = static_cast<int64_t>(tile_m) * 16;
   // columns past the last and rows past M repeat the last: not stored
-  const int nr = n0 + fr < p.n_end ? n0 + fr : p.n_end - 1;
+  const int n = n0 + fr < p.n_end ? n0 + fr : p.n_end - 1;
+  const int64_t m = m0 + fr < p.M ? m0 + fr : p.M - 1;
+  const int8_t* const xrow = p.x + m * p.K;
   const int8_t* wrow[NT];
-  const int8_t* xrow[MT];
 #pragma unroll
-  for (int c = 0; c < NT; ++c) wrow[c] = p.w + (static_cast<int64_t>(c) * p.N + nr) * p.K;
+  for (int c = 0; c < NT; ++c) wrow[c] = p.w + (static_cast<int64_t>(c) * p.N + n) * p.K;
+  i32x4 acc[NT];
 #pragma unroll
-  for (int a = 0; a < MT; ++a) {
-    const int64_t m = a * 16 + fr;
-    xrow[a] = p.x + (m < p.M ? m : p.M - 1) * p.K;
-  }
-  i32x4 acc[NT][MT];
-#pragma unroll
-  for (int c = 0; c < NT; ++c)
-#pragma unroll
-    for (int a = 0; a < MT; ++a) acc[c][a] = i32x4{0, 0, 0, 0};
+  for (int c = 0; c < NT; ++c) acc[c] = i32x4{0, 0, 0, 0};
   // Steps of 128 bytes of K, of which the lane's two chunks are 32 bytes side by side; wavefront w takes steps w,
   // w + W, ..., U of them at a time with all their loads in flight (those past the last whole step load it again
   // and multiply by zero).
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(W * kWave) linear8_rows_kernel(const Linear8Pa
   const int ks0 = p.part ? static_cast<int>(blockIdx.y) * p.split_steps : 0;
   const int whole = p.part && ks0 + p.split_steps < nk_all ? ks0 + p.split_steps : nk_all;
   for (int s = ks0 + wave; s < whole; s += W * U) {
-    i32x4 fw[U][NT][2], fx[U][MT][2];
+    i32x4 fw[U][NT][2], fx[U][2];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int su = s + u * W;
@@ -310,54 +310,39 @@ __global__ void __launch_bounds__(W * kWave) linear8_rows_kernel(const Linear8Pa
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int c = 0; c < NT; ++c) fw[u][c][h] = *reinterpret_cast<const i32x4_any*>(wrow[c] + k + h * 16);
-#pragma unroll
-        for (int a = 0; a < MT; ++a) fx[u][a][h] = *reinterpret_cast<const i32x4_any*>(xrow[a] + k + h * 16);
+        fx[u][h] = *reinterpret_cast<const i32x4_any*>(xrow + k + h * 16);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);  // every load before the first product
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        const i32x4 x = s + u * W < whole ? fx[u][h] : i32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int a = 0; a < MT; ++a) {
-          const i32x4 x = s + u * W < whole ? fx[u][a][h] : i32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int c = 0; c < NT; ++c) acc[c][a] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u][c][h], x, acc[c][a], 0, 0, 0);
-        }
+        for (int c = 0; c < NT; ++c) acc[c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[u][c][h], x, acc[c], 0, 0, 0);
+      }
   }
   if (p.K % kStep != 0 && wave == nk_all % W && (!p.part || blockIdx.y + 1 == gridDim.y)) {  // the rest of K
     const int k = nk_all * kStep + fq * 32;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      i32x4 fw[NT];
+      const i32x4 x = load_chunk(xrow, k + h * 16, p.K);
 #pragma unroll
-      for (int c = 0; c < NT; ++c) fw[c] = load_chunk(wrow[c], k + h * 16, p.K);
-#pragma unroll
-      for (int a = 0; a < MT; ++a) {
-        const i32x4 x = load_chunk(xrow[a], k + h * 16, p.K);
-#pragma unroll
-        for (int c = 0; c < NT; ++c) acc[c][a] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[c], x, acc[c][a], 0, 0, 0);
-      }
+      for (int c = 0; c < NT; ++c)
+        acc[c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(load_chunk(wrow[c], k + h * 16, p.K), x, acc[c], 0, 0, 0);
     }
   }
-  if constexpr (W > 1) {
 #pragma unroll
-    for (int c = 0; c < NT; ++c)
+  for (int c = 0; c < NT; ++c) s_acc[wave][c][lane] = acc[c];
+  __syncthreads();
+  if (wave != 0) return;
 #pragma unroll
-      for (int a = 0; a < MT; ++a) s_acc[wave][a * NT + c][lane] = acc[c][a];
-    __syncthreads();
-    if (wave != 0) return;
+  for (int c = 0; c < NT; ++c)
 #pragma unroll
-    for (int c = 0; c < NT; ++c)
-#pragma unroll
-      for (int a = 0; a < MT; ++a)
-#pragma unroll
-        for (int i = 1; i < W; ++i) acc[c][a] += s_acc[i][a * NT + c][lane];
-  }
-  // lane l holds columns 4 (l / 16) .. + 4 of row l % 16
-  epilogue<YT, GATED, 16, MT, 1, 4>(p, 0, [&](int) { return n0 + fq * 4; },
-                                    [&](int a, int, int half, int i) { return acc[half][a][i]; },
-                                    static_cast<int>(blockIdx.y));
+    for (int i = 1; i < W; ++i) acc[c] += s_acc[i][c][lane];
+  epilogue<YT, GATED, 16, 1, 1, 4>(p, m0, [&](int) { return n0 + fq * 4; },
+                                   [&](int, int, int half, int i) { return acc[half][i]; }, static_cast<int>(blockIdx.y));
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -807,7 +792,7 @@ hipError_t launch_part(Linear8Params p, const Linear8Part& part, int32_t* work, 
   p.n_end = part.n_end;
   p.split_steps = part.steps;
   p.part = part.splits > 1 ? work : nullptr;
-  const Linear8Tile tile = linear8_tile(part.form, p.M);
+  const Linear8Tile tile = linear8_tile(part.form);
   const int out = GATED && part.form != kLinear8Rows ? tile.cols / 2 : tile.cols;
   p.tiles_m = static_cast<int32_t>(linear_ceil(p.M, tile.rows));
   p.tiles_n = static_cast<int32_t>(linear_ceil(p.n_end - p.n_begin, out));
@@ -815,19 +800,14 @@ hipError_t launch_part(Linear8Params p, const Linear8Part& part, int32_t* work, 
   const auto go = [&](auto kernel, int waves) { hipLaunchKernelGGL(kernel, grid, dim3(waves * kWave), 0, s, p); };
   const bool whole = p.K % kStep == 0;
   switch (part.form) {
-    case kLinear8Rows: {
-      const auto rows = [&](auto mt) {
-        constexpr int MT = decltype(mt)::value;
-        // the steps of a split in one batch of loads where they are few
-        if (part.steps <= 4) go(linear8_rows_kernel<YT, 4, MT, 1, GATED>, 4);
-        else if (part.steps <= 8) go(linear8_rows_kernel<YT, 4, MT, 2, GATED>, 4);
-        else if (part.steps <= 16) go(linear8_rows_kernel<YT, 4, MT, 4, GATED>, 4);
-        else go(linear8_rows_kernel<YT, 8, MT, 4, GATED>, 8);
-      };
-      if (p.M <= 16) rows(std::integral_constant<int, 1>{});
-      else rows(std::integral_constant<int, 2>{});
+    case kLinear8Rows:
+      // the steps of a split in one batch of loads where they are few
+      if (part.steps <= 4) go(linear8_rows_kernel<YT, 4, 1, GATED>, 4);
+      else if (part.steps <= 8) go(linear8_rows_kernel<YT, 4, 2, GATED>, 4);
+      else if (part.steps <= 16) go(linear8_rows_kernel<YT, 4, 4, GATED>, 4);
+      else if (part.steps <= 32) go(linear8_rows_kernel<YT, 8, 4, GATED>, 8);
+      else go(linear8_rows_kernel<YT, 16, 4, GATED>, 16);
       break;
-    }
     case kLinear8Any: go(linear8_tile_kernel<YT, 128, 128, 2, 2, GATED>, 4); break;
     case kLinear8Ring: go(linear8_ring_kernel<YT, 64, 64, 2, 2, GATED>, 4); break;
     case kLinear8Tile128:

@@ -163,7 +163,7 @@ constexpr int kLinear8MaxK = 131071;
 constexpr int kLinear8MaxN = 1 << 30;  // 2 N is an int32 too
 
 enum Linear8Form {
-  kLinear8Rows,  // few rows: operands straight to registers
+  kLinear8Rows,  // 16 rows x 16 outputs, operands straight to registers, K over the wavefronts of a workgroup
   kLinear8Any,   // 128 x 128 tiles of operands at any address, any K
   // K a multiple of 16, 16-byte aligned operands, loaded straight to LDS:
   kLinear8Ring,     // 64 x 64 tiles, a ring of four steps
@@ -183,12 +183,12 @@ struct Linear8Plan {
   bool padded;  // operands are copied to rows of whole steps first
 };
 struct Linear8Tile {
-  int rows, cols;  // of weight rows; the gated form's tiles hold as many gates as values, but for few rows
+  int rows, cols;  // weight rows (gated: as many gates as values); of the rows forms outputs
 };
 
-inline Linear8Tile linear8_tile(Linear8Form form, int64_t M) {
+inline Linear8Tile linear8_tile(Linear8Form form) {
   switch (form) {
-    case kLinear8Rows: return {M <= 16 ? 16 : 32, 16};
+    case kLinear8Rows: return {16, 16};
     case kLinear8Ring: return {64, 64};
     case kLinear8Tile256: return {256, 256};
     default: return {128, 128};
@@ -215,7 +215,7 @@ inline int64_t linear8_plan_bytes(const Linear8Plan& plan, int64_t M, int32_t N,
 
 // Tiles of `cols` columns of y.
 inline int64_t linear8_tiles(Linear8Form form, int64_t M, int64_t cols, bool gated) {
-  const Linear8Tile tile = linear8_tile(form, M);
+  const Linear8Tile tile = linear8_tile(form);
   return linear_ceil(M, tile.rows) * linear_ceil(cols, gated && form != kLinear8Rows ? tile.cols / 2 : tile.cols);
 }
 // The most workgroups of a launch (of one split).
@@ -231,12 +231,12 @@ inline int64_t linear8_workgroups(const Linear8Plan& plan, int64_t M, bool gated
 // The estimated time (us) of one part. Workgroups run `slots` at a time (what fits the CUs); a round takes a fixed
 // time and a time per step, which grows from `step` to `full` as the round fills the chip. What the operands, the
 // output (more where rows of y are not whole 16-byte stores) and the partial sums of a split take beyond that is
-// added per million bytes or elements. Fitted to 94,000 timings of 16,000 random shapes (1 to 16,384 rows, 16 to
-// 16,384 outputs, K from 64 to 16,384, plain and gated); the plan chosen is on average 1.2% off the best of all
-// forms and splits (5% for rows of odd widths up to 32 rows). Measured, in us, rows | rings | 128 tiles | 256 tiles:
-//   16 x 1024 -> 1024: 3.1 | 4.9 | - | -            32 x 4096 -> 4096: 9.5 | 9.0 | - | -
+// added per million bytes or elements. Fitted to 61,000 timings of 9,000 random shapes (1 to 16,384 rows, 16 to 16,384
+// outputs, K from 64 to 16,384, plain and gated); the plan chosen is on average 1.4% off the best of all forms and
+// splits (4% for rows of odd widths). Measured, in us, rows | ring | 128 tiles | 256 tiles:
+//   16 x 4096 -> 4096: 7.0 | 11.2 | - | -           64 x 4096 -> 4096: 18.5 | 12.5 | - | -
 //   1024 x 1024 -> 1024: - | 6.5 | 7.7 | 15.8       2048 x 4096 -> 4096: - | 62 | 38.9 | 52.4
-//   4096 x 3584 -> 512: - | 13.7 | 21.1 | 36.6      8192 x 8192 -> 4096: - | 393 | 268 | 202
+//   4096 x 3584 -> 512: - | 13.7 | 21.1 | 36.6      8192 x 8192 -> 4096: - | 393 | 268 | 195
 inline double linear8_time(const Linear8Part& part, int64_t M, int32_t K, bool gated) {
   struct Cost {
     double launch, fixed, step, full, bytes, split, sums, out, out_odd;
@@ -245,18 +245,17 @@ inline double linear8_time(const Linear8Part& part, int64_t M, int32_t K, bool g
   const int64_t cols = part.n_end - part.n_begin, wrows = cols * (gated ? 2 : 1);
   const auto cost = [&]() -> Cost {
     switch (part.form) {
-      case kLinear8Rows: return {2.64, 0.0, 0.076, 0.139, 0.087, 2.24, 1.22, 0.53, 0.34, 512};
-      case kLinear8Any: return {3.92, 2.90, 1.033, 1.655, 0.074, 0.13, 1.90, 0.88, 0.18, 512};
-      case kLinear8Ring: return {1.39, 1.91, 0.158, 0.417, 0.031, 1.95, 2.90, 0.13, 0.27, 512};
-      case kLinear8Tile128: return {0.93, 2.52, 0.449, 1.005, 0.062, 1.64, 2.27, 0.39, 0.37, 512};
-      default: return {1.00, 6.07, 1.060, 1.554, 0.0, 0.57, 1.53, 0.33, 0.47, 256};
+      case kLinear8Rows: return {2.56, 0.0, 0.108, 0.275, 0.0, 2.35, 1.05, 0.38, 0.26, 512};
+      case kLinear8Any: return {3.54, 2.97, 1.052, 1.566, 0.078, 0.31, 1.97, 1.06, 0.0, 512};
+      case kLinear8Ring: return {1.40, 1.86, 0.158, 0.412, 0.032, 2.03, 2.81, 0.19, 0.30, 512};
+      case kLinear8Tile128: return {1.60, 1.72, 0.420, 1.025, 0.066, 1.79, 2.25, 0.48, 0.46, 512};
+      default: return {2.82, 3.06, 1.081, 1.624, 0.0, 1.35, 1.98, 0.54, 0.49, 256};
     }
   }();
   double slow = 1.0;
   if (part.form == kLinear8Rows) {
-    if (M > 16) slow *= 1.82;         // two fragments of rows
-    if (gated) slow *= 2.09;
-    if (K % 16 != 0) slow *= 2.81;    // unaligned loads
+    if (gated) slow *= 1.78;
+    if (K % 16 != 0) slow *= 2.33;  // unaligned loads
   }
   const int64_t groups = linear8_tiles(part.form, M, cols, gated) * part.splits;
   const int64_t rounds = groups / cost.slots;
@@ -281,7 +280,7 @@ inline Linear8Part linear8_best(int64_t M, int32_t n_begin, int32_t n_end, int32
   double best_cost = -1.0;
   for (int f = kLinear8Rows; f <= kLinear8Tile256; ++f) {
     const Linear8Form form = static_cast<Linear8Form>(f);
-    if (form == kLinear8Rows ? M > 32 : form != kLinear8Any && !aligned) continue;
+    if (form != kLinear8Rows && form != kLinear8Any && !aligned) continue;
     const int64_t tiles = linear8_tiles(form, M, n_end - n_begin, gated);
     for (int want = 1; want <= 32; want *= 2) {
       Linear8Part part{form, 1, nk, n_begin, n_end};
@@ -315,7 +314,7 @@ inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, boo
     const int32_t to = static_cast<int32_t>(linear_ceil(K, kLinear8Step) * kLinear8Step);
     double t = 0;
     const Linear8Part part = linear8_best(M, 0, N, to, gated, true, ws_bytes - pad, &t);
-    t += 2.5 + 0.35e-6 * pad;
+    t += 2.5 + 0.37e-6 * pad;
     const auto cost = [](double t, int launches) {
       const double host = kLinear8Host + kLinear8HostLaunch * (launches - 1);
       return t > host ? t : host + 1e-3 * t;
