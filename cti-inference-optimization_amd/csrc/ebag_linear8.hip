@@ -214,27 +214,33 @@ __device__ __forceinline__ void epilogue(const Linear8Params& p, int64_t m0, Col
     const int64_t m = m0 + a * R + row;
     sm[a] = p.scale[m < p.M ? m : p.M - 1];
   }
+  Columns<C> ca[GROUPS], cb[GROUPS];
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) {
     const int n = col_of(g), live = p.n_end - n;
     if (live <= 0) continue;
-    Columns<C> ca, cb;
-    ca.load(p, n, live);
-    if constexpr (GATED) cb.load(p, p.N + n, live);
-    with_gate<GATED>(p, [&](auto gate) {
+    ca[g].load(p, n, live);
+    if constexpr (GATED) cb[g].load(p, p.N + n, live);
+  }
+  with_gate<GATED>(p, [&](auto gate) {
 #pragma unroll
-      for (int a = 0; a < MI; ++a) {
-        const int64_t m = m0 + a * R + row;
+    for (int a = 0; a < MI; ++a) {
+      const int64_t m = m0 + a * R + row;
+      if (m >= p.M) continue;
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {  // a row's groups one after the other: they share cache lines
+        const int n = col_of(g), live = p.n_end - n;
+        if (live <= 0) continue;
         int t[C], u[C];
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           t[i] = sum(a, g, 0, i);
           u[i] = sum(a, g, H - 1, i);
         }
-        if (m < p.M) emit<YT, decltype(gate)::value, C>(p, m, n, live, sm[a], ca, cb, t, u);
+        emit<YT, decltype(gate)::value, C>(p, m, n, live, sm[a], ca[g], cb[g], t, u);
       }
-    });
-  }
+    }
+  });
 }
 
 // ---------------------------------------------------------------------------------------------
