@@ -13,7 +13,11 @@ global offsets ``offsets[F*B+1]``, sum or mean pooling, and an explicit output d
 pair (online_best/infer.py:895-942). A table argument of the general entry points may also be an
 int8 pair ``(q [V, D] int8, scale [V] float32)``; its rows pool as ``acc = fma(q, scale, acc)``.
 
-Both validate their arguments on the host (no device synchronisation) and raise ``ValueError``
+``rms_norm_int8``, ``layer_norm_int8``, ``linear_int8``, ``gated_linear_int8`` and
+``dequantize_embedding_int8`` carry int8 rows with a scale each on into the encoder's Linear and the
+feed-forward blocks behind it.
+
+All validate their arguments on the host (no device synchronisation) and raise ``ValueError``
 / ``TypeError`` for malformed calls and ``EbagError`` when the C ABI reports a failure.
 """
 from __future__ import annotations
