@@ -36,7 +36,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef i32x4 i32x4_any __attribute__((aligned(1)));
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
-
 constexpr int kStep = kLinear8Step;  // bytes of K per step
 constexpr int kXcds = 8;
 
@@ -177,7 +176,7 @@ __device__ __forceinline__ void emit(const Linear8Params& p, int64_t m, int n, i
 // A wavefront's sums to y, or to this split's partial sums: lane l holds rows m0 + R a + l % R, a < MI, and of each
 // GROUPS times C columns side by side from col_of(g) on; sum(a, g, half, i) is the sum of column i of group g (half 1:
 // of the gated form's values). Scales are loaded at once and before the first is used: one at a time, between the
-// stores, they took 38 us a 256 x 256 tile, longer than 8,192 of K.
+// stores, they took 38 us a 256 x 256 tile, as long as 3,500 of K.
 template <typename YT, bool GATED, int R, int MI, int GROUPS, int C, typename ColOf, typename Sum>
 __device__ __forceinline__ void epilogue(const Linear8Params& p, int64_t m0, ColOf&& col_of, Sum&& sum, int split) {
   constexpr int H = GATED ? 2 : 1;
@@ -352,7 +351,7 @@ __global__ void __launch_bounds__(W * kWave) linear8_rows_kernel(const Linear8Pa
 }
 
 // ---------------------------------------------------------------------------------------------
-// Tiles: BM rows by BN weight rows, WM x WN wavefronts
+// Tiles of operands at any address: BM rows by BN weight rows, WM x WN wavefronts
 // ---------------------------------------------------------------------------------------------
 // Tile i of the launch. Dispatch position i runs on XCD i % 8: each XCD gets a contiguous range of tiles
 // (L2 is per XCD), which runs down kGroup row bands before it steps to the next column of tiles. A group of 6, no power

@@ -255,7 +255,7 @@ inline double linear8_time(const Linear8Part& part, int64_t M, int32_t K, bool g
   double slow = 1.0;
   if (part.form == kLinear8Rows) {
     if (gated) slow *= 1.78;
-    if (K % 16 != 0) slow *= 2.33;  // unaligned loads
+    if (K % 4 != 0) slow *= 2.33;  // loads at odd addresses (at multiples of 4 they cost nothing)
   }
   const int64_t groups = linear8_tiles(part.form, M, cols, gated) * part.splits;
   const int64_t rounds = groups / cost.slots;
@@ -307,8 +307,8 @@ inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, boo
   Linear8Plan plan{1, {}, false};
   double time = 0;
   plan.part[0] = linear8_best(M, 0, N, K, gated, aligned, ws_bytes, &time);
-  // Operands of odd widths (or addresses) copied to rows of whole steps first: 40 x 333 -> 1000: 10.7 | 7.9 us; 2000 x 4094
-  // -> 4096: 66 | 54 us.
+  // Operands of odd widths (or addresses) copied to rows of whole steps first (us, not copied | copied): 1531 x 1021 ->
+  // 777: 17.7 | 10.9; 2000 x 4094 -> 4096: 57.7 | 52.7; 500 x 8191 -> 2000: 88.9 | 29.1.
   const int64_t pad = linear8_pad_bytes(M, N, K, gated);
   if (!aligned && ws_bytes >= pad) {
     const int32_t to = static_cast<int32_t>(linear_ceil(K, kLinear8Step) * kLinear8Step);

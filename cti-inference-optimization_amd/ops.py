@@ -1010,8 +1010,8 @@ def _linear_int8(q, scale, weight, weight_scale, bias, gate: int, out, out_dtype
             raise ValueError(f"bias has {bias.numel()} elements, expected {w_rows}")
         bias_ptr, bias_code = bias.data_ptr(), _capi.dtype_code(bias.dtype)
     out, code = _float_output(out, rows, n_out, out_dtype, q, index)
-    # K split over several workgroups where few tiles would leave CUs idle: int32 partial sums in a
-    # workspace from torch's allocator (kept alive until the launches are enqueued)
+    # partial sums of a split K, copies of operands of odd widths: in a workspace from torch's allocator
+    # (kept alive until the launches are enqueued)
     ws, ws_ptr, ws_bytes = None, None, _linear_int8_workspace(rows, cols, n_out, gate) if split_k else 0
     if ws_bytes > 0:
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
@@ -1045,9 +1045,10 @@ def linear_int8(
     ``out[m, n] = (sum_k q[m, k] * weight[n, k]) * scale[m] * weight_scale[n] + bias[n]``,
 
     the sum exact in int32 (``cols`` at most 131071), the rest in fp32 with one rounding to
-    ``out_dtype`` (bf16 by default; or ``out``'s type). With ``split_k`` (default) a shape whose tiles
-    would leave CUs idle has K split over several workgroups (partial sums in a workspace from torch's
-    allocator); the result is the same bit for bit. Written on torch's current stream.
+    ``out_dtype`` (bf16 by default; or ``out``'s type). With ``split_k`` (default) a workspace from torch's
+    allocator lets a shape whose tiles would leave CUs idle have K split over several workgroups, and
+    operands of odd widths be copied to whole steps first, where that is faster; the result is the same
+    bit for bit. Written on torch's current stream.
     """
     return _linear_int8(q, scale, weight, weight_scale, bias, _capi.GATE_NONE, out, out_dtype, split_k)
 

@@ -505,9 +505,10 @@ int cti_ebag_norm_int8(int32_t kind, const void* x, const void* residual, void* 
  *            cti_ebag_quantize_int8), weight_scale fp32
  *   bias     of `bias_dtype` F32 / BF16 / F16, or NULL
  *   y        [rows, out_features] of `y_dtype` F32 / BF16 / F16, contiguous
- *   workspace  device scratch of workspace_bytes (16-byte aligned), or NULL / 0: where few tiles would leave
- *            CUs idle, K is split over several workgroups per tile, each writing int32 partial sums here,
- *            and a second launch adds them; as many splits as the workspace holds, none without one
+ *   workspace  device scratch of workspace_bytes (16-byte aligned), or NULL / 0. Where few tiles would leave
+ *            CUs idle, K is split over several workgroups per tile, each writing int32 partial sums here, and a
+ *            second launch adds them; operands whose rows are no multiple of 16 bytes, or that start at no
+ *            16-byte address, are first copied here to rows of a multiple of 128. What does not fit is not done.
  * cols at most 131071 (the int32 sums cannot overflow up to there), out_features at most 2^30. The integer
  * sums are exact, so the result is the same bit for bit with any workspace.
  */
@@ -516,7 +517,8 @@ int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t rows, int3
                          int32_t gate, void* y, int32_t y_dtype, void* workspace, int64_t workspace_bytes,
                          void* stream);
 
-/* Bytes of workspace cti_ebag_linear_int8 uses at most for this shape (0: it never splits). */
+/* Bytes of workspace cti_ebag_linear_int8 uses at most for this shape, q and weight at 16-byte aligned addresses
+ * (0: none). */
 int64_t cti_ebag_linear_int8_workspace_bytes(int64_t rows, int32_t cols, int32_t out_features, int32_t gate);
 
 #ifdef __cplusplus
