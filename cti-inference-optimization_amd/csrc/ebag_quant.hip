@@ -227,13 +227,16 @@ template <typename T>
 bool launch_wide(const char* w, int64_t rows, int64_t dim, int64_t row_stride, int8_t* q, float* scale, hipStream_t s) {
   constexpr int VEC = 16 / Elem<T>::kBytes;
   const int64_t vecs = (dim + VEC - 1) / VEC;
-  if (vecs <= kWave || vecs > 64 * kWave || rows > INT32_MAX) return false;
-  const dim3 grid(static_cast<unsigned>(rows));
+  if (vecs <= kWave || vecs > 64 * kWave) return false;
   const int64_t rb = row_stride * Elem<T>::kBytes;
   const auto go = [&](auto k, auto waves) {
     constexpr int W = decltype(waves)::value;
-    hipLaunchKernelGGL((quantize_wide_kernel<T, decltype(k)::value, W>), grid, dim3(W * kWave), 0, s, w,
-                       static_cast<int32_t>(dim), rb, q, scale);
+    constexpr int64_t kRows = UINT32_MAX / (W * kWave);  // a launch has fewer than 2^32 threads
+    for (int64_t r = 0; r < rows; r += kRows) {
+      const dim3 grid(static_cast<unsigned>(rows - r < kRows ? rows - r : kRows));
+      hipLaunchKernelGGL((quantize_wide_kernel<T, decltype(k)::value, W>), grid, dim3(W * kWave), 0, s, w + r * rb,
+                         static_cast<int32_t>(dim), rb, q + r * dim, scale + r);
+    }
   };
   constexpr std::integral_constant<int, 1> n1{};
   constexpr std::integral_constant<int, 2> n2{};

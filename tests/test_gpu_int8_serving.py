@@ -676,3 +676,20 @@ def test_wide_rows_are_quantised_as_narrow_ones(pkg, dev, dim, dt):
         want_s = torch.clamp(x.float().abs().amax(1) * np.float32(1 / 127), min=np.float32(1e-8))
         want_q = torch.clamp(torch.round(x.float() / want_s[:, None]), -128, 127).to(torch.int8)
         assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu(), want_q)
+
+
+def test_more_wide_rows_than_a_launch_has(pkg, dev):
+    """A workgroup of 256 threads a row: 2^24 rows and more are 2^32 threads, which no launch has."""
+    rows, dim = 2 ** 24 + 5, 513
+    w = torch.zeros(rows, dim, dtype=torch.bfloat16, device=dev)
+    g = _gen(4)
+    at = torch.tensor([0, 2 ** 24 - 2, 2 ** 24 - 1, 2 ** 24, rows - 1])
+    some = torch.randn(len(at), dim, generator=g).to(torch.bfloat16)
+    w[at.to(dev)] = some.to(dev)
+    print("more wide rows than a launch has", flush=True)
+    q, s = pkg.quantize_embedding_int8(w)
+    torch.cuda.synchronize()
+    del w
+    want_q, want_s = pkg.quantize_embedding_int8(some.to(dev))
+    assert torch.equal(q[at.to(dev)], want_q) and torch.equal(s[at.to(dev)], want_s)
+    assert int((s != np.float32(1e-8)).sum()) == len(at)
