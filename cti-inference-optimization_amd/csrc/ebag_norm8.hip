@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(kLoopThreads) norm8_loop_kernel(const Norm8Par
 // little else on its SIMD (16,384 rows of 4,096 bf16 with a residual: 82 us with 4 wavefronts of 2 vectors per lane,
 // 88 with 4 of 4, 101 with one of 8; one row: 4.4 us with 8 of 1, 5.2 with 4 of 2, 9.3 with one of 8).
 template <typename T, typename PT>
-hipError_t launch_norm8(const Norm8Params& p, int64_t rows, hipStream_t s) {
+hipError_t launch_norm8_rows(const Norm8Params& p, int64_t rows, hipStream_t s) {
   constexpr int VEC = 16 / Elem<T>::kBytes;
   const int64_t nvec = (p.cols + VEC - 1) / VEC;
   const dim3 grid(static_cast<unsigned>(rows));
@@ -413,6 +413,25 @@ hipError_t launch_norm8(const Norm8Params& p, int64_t rows, hipStream_t s) {
     go(n4, n16);
   }
   return hipGetLastError();
+}
+
+// A launch has fewer than 2^32 threads: at most so many rows of up to 1,024 threads in one.
+constexpr int64_t kNorm8Rows = UINT32_MAX / 1024;
+template <typename T, typename PT>
+hipError_t launch_norm8(Norm8Params p, int64_t rows, hipStream_t s) {
+  for (; rows > kNorm8Rows; rows -= kNorm8Rows) {
+    const hipError_t e = launch_norm8_rows<T, PT>(p, kNorm8Rows, s);
+    if (e != hipSuccess) return e;
+    const int64_t bytes = kNorm8Rows * p.cols * Elem<T>::kBytes;
+    p.x += bytes;
+    if (p.res) {
+      p.res += bytes;
+      p.res_out += bytes;
+    }
+    p.q += kNorm8Rows * p.cols;
+    p.scale += kNorm8Rows;
+  }
+  return launch_norm8_rows<T, PT>(p, rows, s);
 }
 
 template <typename T>

@@ -693,3 +693,20 @@ def test_more_wide_rows_than_a_launch_has(pkg, dev):
     want_q, want_s = pkg.quantize_embedding_int8(some.to(dev))
     assert torch.equal(q[at.to(dev)], want_q) and torch.equal(s[at.to(dev)], want_s)
     assert int((s != np.float32(1e-8)).sum()) == len(at)
+
+
+@pytest.mark.parametrize("cols", [3, 40])
+def test_more_norm_rows_than_a_launch_has(pkg, dev, cols):
+    """Up to 1,024 threads a row, fewer than 2^32 in a launch: the rows of several launches."""
+    rows = 2 ** 24 + 5
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=dev)
+    edge = (2 ** 32 - 1) // 1024  # the first launch's rows, if it has as many as 1,024 threads for each allow
+    at = torch.tensor([0, edge - 1, edge, 2 * edge - 1, 2 * edge, 4 * edge, 2 ** 24 - 1, 2 ** 24, rows - 1])
+    some = torch.randn(len(at), cols, generator=_gen(5)).to(torch.bfloat16)
+    x[at.to(dev)] = some.to(dev)
+    w = torch.ones(cols)
+    print(f"more norm rows than a launch has, {cols} wide", flush=True)
+    q, s, h = pkg.rms_norm_int8(x, w.to(dev), residual=x, residual_out=x)
+    torch.cuda.synchronize()
+    _check_norm((q[at.to(dev)], s[at.to(dev)], h[at.to(dev)]), some, some, w, None, 1e-5, False)
+    assert int((s != np.float32(1e-8)).sum()) == len(at) and int(h.any(1).sum()) == len(at)
