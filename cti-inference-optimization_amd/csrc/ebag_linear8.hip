@@ -902,17 +902,18 @@ extern "C" int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t
     return set_error(CTI_EBAG_EINVAL, "workspace is not 16-byte aligned");
   const bool gated = gate != CTI_EBAG_GATE_NONE;
   const bool aligned = cols % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0;
-  const Linear8Plan plan = linear8_plan(rows, out_features, cols, gated, aligned, workspace ? workspace_bytes : 0);
-  if (linear8_workgroups(plan, rows, gated) > INT32_MAX)
+  const int64_t ws_bytes = workspace ? workspace_bytes : 0;
+  const auto plan_of = [&](int64_t m) { return linear8_plan(m, out_features, cols, gated, aligned, ws_bytes); };
+  // launches of kLinear8LaunchRows rows, and of those left
+  const int64_t rest = rows % kLinear8LaunchRows, whole = rows - rest;
+  const Linear8Plan plan = whole ? plan_of(kLinear8LaunchRows) : Linear8Plan{}, last = rest ? plan_of(rest) : Linear8Plan{};
+  if (linear8_workgroups(plan, kLinear8LaunchRows, gated) > kLinear8MaxTiles ||
+      linear8_workgroups(last, rest, gated) > kLinear8MaxTiles)
     return set_error(CTI_EBAG_EUNSUPPORTED, "too many output tiles (%lld x %d)", (long long)rows, out_features);
   Linear8Params p = {};
-  p.x = q;
-  p.scale = scale;
   p.w = weight;
   p.wscale = weight_scale;
   p.bias = bias;
-  p.y = static_cast<char*>(y);
-  p.M = rows;
   p.N = out_features;
   p.K = cols;
   p.bias_dtype = bias_dtype;
@@ -920,7 +921,14 @@ extern "C" int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t
   p.gate = gate;
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* const work = static_cast<char*>(workspace);
-  const hipError_t e = gated ? launch_typed<true>(p, plan, work, s) : launch_typed<false>(p, plan, work, s);
-  if (e != hipSuccess) return set_error(CTI_EBAG_EHIP, "linear launch failed: %s", hipGetErrorString(e));
+  for (int64_t m = 0; m < rows; m += kLinear8LaunchRows) {
+    const Linear8Plan& of = m < whole ? plan : last;
+    p.M = m < whole ? kLinear8LaunchRows : rest;
+    p.x = q + m * cols;
+    p.scale = scale + m;
+    p.y = static_cast<char*>(y) + m * out_features * dtype_bytes(y_dtype);
+    const hipError_t e = gated ? launch_typed<true>(p, of, work, s) : launch_typed<false>(p, of, work, s);
+    if (e != hipSuccess) return set_error(CTI_EBAG_EHIP, "linear launch failed: %s", hipGetErrorString(e));
+  }
   return CTI_EBAG_OK;
 }

@@ -228,6 +228,11 @@ inline int64_t linear8_workgroups(const Linear8Plan& plan, int64_t M, bool gated
   return most;
 }
 
+// Rows of x in a launch, more take several: a launch has fewer than 2^32 threads, up to 1,024 a workgroup, and the copy of operands of odd widths
+// stays small beside what they were made from. (A launch of 2^20 rows leaves at most 1 round of tiles in 16 unfilled.)
+constexpr int64_t kLinear8LaunchRows = int64_t{1} << 20;
+constexpr int64_t kLinear8MaxTiles = UINT32_MAX / 1024;
+
 // The estimated time (us) of one part. Workgroups run `slots` at a time (what fits the CUs); a round takes a fixed
 // time and a time per step, which grows from `step` to `full` as the round fills the chip. What the operands, the
 // output (more where rows of y are not whole 16-byte stores) and the partial sums of a split take beyond that is
@@ -310,7 +315,7 @@ inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, boo
   // Operands of odd widths (or addresses) copied to rows of whole steps first (us, not copied | copied): 1531 x 1021 ->
   // 777: 17.7 | 10.9; 2000 x 4094 -> 4096: 57.7 | 52.7; 500 x 8191 -> 2000: 88.9 | 29.1.
   const int64_t pad = linear8_pad_bytes(M, N, K, gated);
-  if (!aligned && ws_bytes >= pad) {
+  if (!aligned && ws_bytes >= pad && pad / 16 < UINT32_MAX - 1024) {  // (a thread copies 16 bytes)
     const int32_t to = static_cast<int32_t>(linear_ceil(K, kLinear8Step) * kLinear8Step);
     double t = 0;
     const Linear8Part part = linear8_best(M, 0, N, to, gated, true, ws_bytes - pad, &t);
@@ -349,7 +354,11 @@ inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, boo
 
 // Bytes of workspace that a shape's operands, at 16-byte aligned addresses, are given at most.
 inline int64_t linear8_workspace_bytes(int64_t M, int32_t N, int32_t K, bool gated) {
-  return linear8_plan_bytes(linear8_plan(M, N, K, gated, K % 16 == 0, INT64_MAX), M, N, K, gated);
+  const auto of = [&](int64_t rows) {
+    return rows > 0 ? linear8_plan_bytes(linear8_plan(rows, N, K, gated, K % 16 == 0, INT64_MAX), rows, N, K, gated) : 0;
+  };
+  const int64_t rest = of(M % kLinear8LaunchRows), whole = M >= kLinear8LaunchRows ? of(kLinear8LaunchRows) : 0;
+  return rest > whole ? rest : whole;
 }
 
 }  // namespace cti

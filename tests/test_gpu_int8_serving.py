@@ -710,3 +710,23 @@ def test_more_norm_rows_than_a_launch_has(pkg, dev, cols):
     torch.cuda.synchronize()
     _check_norm((q[at.to(dev)], s[at.to(dev)], h[at.to(dev)]), some, some, w, None, 1e-5, False)
     assert int((s != np.float32(1e-8)).sum()) == len(at) and int(h.any(1).sum()) == len(at)
+
+
+@pytest.mark.parametrize("cols", [20, 32])
+def test_more_product_rows_than_a_launch_takes(pkg, dev, cols):
+    """2^20 rows a launch: the rows of three, the last of a few."""
+    rows, n = 2 ** 21 + 37, 24
+    q, s, w, ws, bias = _operands(rows, cols, n, 7)
+    args = [t.to(dev) for t in (q, s, w, ws)]
+    print(f"more product rows than a launch takes, {cols} wide", flush=True)
+    y = pkg.linear_int8(*args, bias=bias.to(dev))
+    torch.cuda.synchronize()
+    at = torch.cat([torch.arange(70), *(torch.arange(e - 70, e + 37) for e in (2 ** 20, 2 ** 21))])
+    assert torch.equal(y[at.to(dev)].cpu(), torch.from_numpy(_value(q[at], s[at], w, ws, bias)).to(torch.bfloat16))
+    # every other row against the same product of the rows around it
+    for lo in range(0, rows, 300000):
+        part = pkg.linear_int8(args[0][lo:lo + 300000], args[1][lo:lo + 300000], *args[2:], bias=bias.to(dev))
+        assert torch.equal(y[lo:lo + 300000], part)
+    z = pkg.gated_linear_int8(*args, bias=bias.to(dev))
+    assert torch.equal(z[2 ** 20 - 9:2 ** 20 + 9], pkg.gated_linear_int8(args[0][2 ** 20 - 9:2 ** 20 + 9], args[1][2 ** 20 - 9:2 ** 20 + 9],
+                                                                         *args[2:], bias=bias.to(dev)))

@@ -67,6 +67,18 @@ def test_linear_int8_limits(pkg):
     assert _linear(c, rows=2 ** 31 - 1, n=2 ** 30) == c.EUNSUPPORTED  # more tiles than a launch has
 
 
+def test_tall_products_take_several_launches(pkg):
+    """The copy of operands of odd widths does not grow with the rows past those of a launch; a workspace serves the
+    rows of each launch; too many tiles are refused before any launch."""
+    c = pkg._capi
+    f = c.lib().cti_ebag_linear_int8_workspace_bytes
+    for cols, n, gate in ((17, 64, c.GATE_NONE), (1021, 777, c.GATE_NONE), (17, 64, c.GATE_SILU)):
+        most = max(f(2 ** 20, cols, n, gate), f(5, cols, n, gate))
+        assert f(2 ** 31 - 2 ** 20 + 5, cols, n, gate) == most
+    assert f(2 ** 20, 1021, 777, c.GATE_NONE) == (2 ** 20 + 777) * 1024  # copied to rows of whole steps
+    assert _linear(c, rows=1, cols=16, n=2 ** 30) == c.EUNSUPPORTED and "tiles" in c.last_error()
+
+
 def test_dequantize_int8_rejects_bad_arguments(pkg):
     c = pkg._capi
     f = c.lib().cti_ebag_dequantize_int8
