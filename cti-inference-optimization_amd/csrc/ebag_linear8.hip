@@ -490,7 +490,9 @@ __device__ __forceinline__ void wait_barrier() {
 }
 
 // Tiles of BM x BN with WM x WN wavefronts, a ring of four steps: a step's loads are issued three steps ahead. For
-// tiles that are few, or short in K once it is split: what counts is bytes in flight.
+// tiles that are few, or short in K once it is split: what counts is bytes in flight, and for rounds that fill the card
+// bytes from L2 (4096 x 3584 -> 512: 512 tiles of 64 x 64, two to a CU, load 32 KB for each product of 128 x 64 x 128 on a CU
+// and take 15.2 us; 256 of 128 x 64 load 24 and take 12.7; 2048 x 5632 -> 2048 as 256 tiles of 128 x 128 26.7).
 template <typename YT, int BM, int BN, int WM, int WN, bool GATED>
 __global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_ring_kernel(const Linear8Params p) {
   constexpr int WAVES = WM * WN;
@@ -823,6 +825,9 @@ hipError_t launch_part(Linear8Params p, const Linear8Part& part, int32_t* work, 
       if (whole) go(linear8_big_kernel<YT, 256, 256, 2, 4, GATED, false>, 8);
       else go(linear8_big_kernel<YT, 256, 256, 2, 4, GATED, true>, 8);
       break;
+    case kLinear8RingTall: go(linear8_ring_kernel<YT, 128, 64, 4, 2, GATED>, 8); break;
+    case kLinear8Ring128: go(linear8_ring_kernel<YT, 128, 128, 4, 2, GATED>, 8); break;
+    case kLinear8Forms: return hipErrorInvalidValue;
   }
   if (p.part) {
     const hipError_t e = hipGetLastError();

@@ -166,9 +166,13 @@ enum Linear8Form {
   kLinear8Rows,  // 16 rows x 16 outputs, operands straight to registers, K over the wavefronts of a workgroup
   kLinear8Any,   // 128 x 128 tiles of operands at any address, any K
   // K a multiple of 16, 16-byte aligned operands, loaded straight to LDS:
-  kLinear8Ring,     // 64 x 64 tiles, a ring of four steps
-  kLinear8Tile128,  // 128 x 128 tiles
-  kLinear8Tile256,  // 256 x 256 tiles
+  kLinear8Ring,     // 64 x 64 tiles, a ring of four steps, two to a CU
+  kLinear8Tile128,  // 128 x 128 tiles, two steps, two to a CU
+  kLinear8Tile256,  // 256 x 256 tiles, two steps, one to a CU
+  // rings of four steps, one tile to a CU, when there are about as many tiles as CUs:
+  kLinear8RingTall,  // 128 x 64 tiles
+  kLinear8Ring128,   // 128 x 128 tiles
+  kLinear8Forms,
 };
 // One launch (two with splits): columns n_begin .. n_end of y.
 struct Linear8Part {
@@ -190,6 +194,7 @@ inline Linear8Tile linear8_tile(Linear8Form form) {
   switch (form) {
     case kLinear8Rows: return {16, 16};
     case kLinear8Ring: return {64, 64};
+    case kLinear8RingTall: return {128, 64};
     case kLinear8Tile256: return {256, 256};
     default: return {128, 128};
   }
@@ -236,12 +241,14 @@ constexpr int64_t kLinear8MaxTiles = UINT32_MAX / 1024;
 // The estimated time (us) of one part. Workgroups run `slots` at a time (what fits the CUs); a round takes a fixed
 // time and a time per step, which grows from `step` to `full` as the round fills the chip. What the operands, the
 // output (more where rows of y are not whole 16-byte stores) and the partial sums of a split take beyond that is
-// added per million bytes or elements. Fitted to 61,000 timings of 9,000 random shapes (1 to 16,384 rows, 16 to 16,384
-// outputs, K from 64 to 16,384, plain and gated); the plan chosen is on average 1.4% off the best of all forms and
-// splits (4% for rows of odd widths). Measured, in us, rows | ring | 128 tiles | 256 tiles:
-//   16 x 4096 -> 4096: 7.0 | 11.2 | - | -           64 x 4096 -> 4096: 18.5 | 12.5 | - | -
-//   1024 x 1024 -> 1024: - | 6.5 | 7.7 | 15.8       2048 x 4096 -> 4096: - | 62 | 38.9 | 52.4
-//   4096 x 3584 -> 512: - | 13.7 | 21.1 | 36.6      8192 x 8192 -> 4096: - | 393 | 268 | 195
+// added per million bytes or elements. Fitted to 84,000 timings of 10,600 random shapes (64 to 16,384 rows and outputs, K
+// from 64 to 16,384, plain and gated), the first two forms to 61,000 of 9,000 from one row and one output on; the plan chosen
+// is on average 1.1% off the best of all forms and splits (4% for rows of odd widths). Measured, in us, rows | ring |
+// tall ring | 128 ring | 128 tiles | 256 tiles:
+//   16 x 4096 -> 4096: 7.0 | 11.2 | - | - | - | -              64 x 4096 -> 4096: 18.5 | 12.5 | - | - | - | -
+//   300 x 3584 -> 512: - | 8.3 | 9.3 | - | - | -               4096 x 3584 -> 512: - | 15.2 | 12.7 | 16.0 | 21.6 | 37.3
+//   2048 x 2048 -> 2048: - | 17.6 | 14.8 | 13.5 | 13.2 | 24.6  2048 x 5632 -> 2048: - | 45 | 38 | 27 | 36 | 55
+//   2048 x 4096 -> 4096: - | 54 | 48 | 37.7 | 34.4 | 43.6      8192 x 8192 -> 4096: - | 393 | - | - | 268 | 195
 inline double linear8_time(const Linear8Part& part, int64_t M, int32_t K, bool gated) {
   struct Cost {
     double launch, fixed, step, full, bytes, split, sums, out, out_odd;
@@ -252,9 +259,11 @@ inline double linear8_time(const Linear8Part& part, int64_t M, int32_t K, bool g
     switch (part.form) {
       case kLinear8Rows: return {2.56, 0.0, 0.108, 0.275, 0.0, 2.35, 1.05, 0.38, 0.26, 512};
       case kLinear8Any: return {3.54, 2.97, 1.052, 1.566, 0.078, 0.31, 1.97, 1.06, 0.0, 512};
-      case kLinear8Ring: return {1.40, 1.86, 0.158, 0.412, 0.032, 2.03, 2.81, 0.19, 0.30, 512};
-      case kLinear8Tile128: return {1.60, 1.72, 0.420, 1.025, 0.066, 1.79, 2.25, 0.48, 0.46, 512};
-      default: return {2.82, 3.06, 1.081, 1.624, 0.0, 1.35, 1.98, 0.54, 0.49, 256};
+      case kLinear8Ring: return {1.38, 2.11, 0.156, 0.408, 0.034, 1.97, 2.48, 0.04, 0.25, 512};
+      case kLinear8Tile128: return {0.96, 2.91, 0.540, 0.987, 0.032, 1.99, 1.96, 0.27, 0.36, 512};
+      case kLinear8RingTall: return {1.49, 2.21, 0.221, 0.322, 0.042, 2.36, 1.82, 0.0, 0.35, 256};
+      case kLinear8Ring128: return {1.65, 3.16, 0.307, 0.496, 0.027, 2.30, 1.59, 0.0, 0.37, 256};
+      default: return {2.70, 6.86, 0.984, 1.617, 0.0, 3.21, 1.02, 0.04, 0.44, 256};
     }
   }();
   double slow = 1.0;
@@ -283,7 +292,7 @@ inline Linear8Part linear8_best(int64_t M, int32_t n_begin, int32_t n_end, int32
   const int nk = static_cast<int>(linear_ceil(K, kLinear8Step));
   Linear8Part best{kLinear8Any, 1, nk, n_begin, n_end};
   double best_cost = -1.0;
-  for (int f = kLinear8Rows; f <= kLinear8Tile256; ++f) {
+  for (int f = kLinear8Rows; f < kLinear8Forms; ++f) {
     const Linear8Form form = static_cast<Linear8Form>(f);
     if (form != kLinear8Rows && form != kLinear8Any && !aligned) continue;
     const int64_t tiles = linear8_tiles(form, M, n_end - n_begin, gated);

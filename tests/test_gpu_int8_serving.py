@@ -271,7 +271,11 @@ def test_linear_is_exact(pkg, dev, rows, cols, n):
 # columns in another form, operands copied to whole steps), against float64 on the device.
 LARGE = [(8192, 256, 2048, False), (4100, 640, 4100, False), (4100, 272, 4100, False), (4096, 1000, 4200, False),
          (8000, 130, 4099, False), (2500, 1040, 2049, False), (4100, 640, 2050, True), (4096, 1008, 2176, True),
-         (3001, 333, 1500, True), (8192, 512, 1024, True), (2048, 2048, 2048, False)]
+         (3001, 333, 1500, True), (8192, 512, 1024, True), (2048, 2048, 2048, False),
+         # about as many tiles as CUs, or K split over as many: the rings of one tile to a CU
+         (4096, 3584, 512, False), (2000, 1040, 1003, False), (1000, 8192, 1000, False), (600, 16016, 700, False),
+         (512, 4096, 2048, True), (700, 9216, 500, True), (520, 3600, 4100, False), (900, 12304, 900, False),
+         (500, 1040, 2100, True), (2048, 2048, 1024, True), (300, 15360, 2500, False)]
 
 
 @pytest.mark.parametrize("rows,cols,n,gated", LARGE)

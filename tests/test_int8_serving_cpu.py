@@ -181,3 +181,15 @@ def test_the_gpu_tests_reach_every_plan(rules):
     want = {("form", f) for f in range(5)} | {("split", True), ("padded", True), ("part", 1)}
     want |= {("rest of K", f, tail) for f in (0, 2, 3, 4) for tail in (False, True)}
     assert want - seen == set()
+
+
+def test_the_gpu_tests_reach_every_plan_of_the_rings(rules):
+    """128 x 64 and 128 x 128 rings of four steps: plain and gated, with and without a rest of K, K split and whole."""
+    import test_gpu_int8_serving as g
+
+    seen = set()
+    for M, K, N, gated in g.LARGE:
+        plan, _, _ = rules(M, N, K, int(gated), K % 16 == 0, 1 << 62)
+        for part in plan.part[:plan.parts]:
+            seen |= {(part.form, "gated", gated), (part.form, "rest", K % 128 != 0), (part.form, "split", part.splits > 1)}
+    assert {(f, what, x) for f in (5, 6) for what in ("gated", "rest", "split") for x in (False, True)} - seen == set()
