@@ -16,7 +16,7 @@
 //   rows   few rows or few outputs: bound by reading the weight, or by the way to memory and back. A workgroup owns
 //          16 rows by 16 columns (gated: 16 gates and their 16 values); its wavefronts split K, load both operands
 //          straight to registers and add their sums through LDS.
-//   ring   64 x 64 tiles through LDS, a ring of four steps loaded straight to it.
+//   rings  tiles through LDS, a ring of four steps loaded straight to it: 64 x 64, two to a CU; 128 x 64 and 128 x 128, one.
 //   tiles  128 x 128 and 256 x 256 tiles, two steps in LDS, fragments read half a step ahead.
 //   any    128 x 128 tiles of operands at any address and any width, through registers: without a workspace. With one,
 //          operands of odd widths are copied to rows of whole steps first.
@@ -492,7 +492,8 @@ __device__ __forceinline__ void wait_barrier() {
 // Tiles of BM x BN with WM x WN wavefronts, a ring of four steps: a step's loads are issued three steps ahead. For
 // tiles that are few, or short in K once it is split: what counts is bytes in flight, and for rounds that fill the card
 // bytes from L2 (4096 x 3584 -> 512: 512 tiles of 64 x 64, two to a CU, load 32 KB for each product of 128 x 64 x 128 on a CU
-// and take 15.2 us; 256 of 128 x 64 load 24 and take 12.7; 2048 x 5632 -> 2048 as 256 tiles of 128 x 128 26.7).
+// and take 15.2 us; 256 of 128 x 64 load 24 and take 12.7; 2048 x 5632 -> 2048 as 256 tiles of 128 x 128 26.7, its matrix
+// cores busy half of that, 34 bytes a clock and CU loaded). Fragments read half a step ahead as below gained nothing here.
 template <typename YT, int BM, int BN, int WM, int WN, bool GATED>
 __global__ void __launch_bounds__(WM * WN * kWave, 1) linear8_ring_kernel(const Linear8Params p) {
   constexpr int WAVES = WM * WN;
