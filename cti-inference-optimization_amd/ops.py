@@ -122,7 +122,8 @@ def dequantize_embedding_int8(q: torch.Tensor, scale: torch.Tensor, out_dtype: t
     """The values that int8 rows stand for: ``q [V, D] int8``, ``scale [V] float32`` (as
     ``quantize_embedding_int8``, ``rms_norm_int8`` and ``layer_norm_int8`` return them) to
     ``out [V, D]`` with ``out[v, j] = q[v, j] * scale[v]`` in fp32, rounded once to ``out_dtype``
-    (bf16 by default; fp32, bf16 or fp16, or ``out``'s). Written on torch's current stream."""
+    (bf16 by default; fp32, bf16 or fp16, or ``out``'s); ``out`` overlaps no input. Written on torch's
+    current stream."""
     rows, dim, index = _check_int8_rows("q", q, "scale", scale)
     out, code = _float_output(out, rows, dim, out_dtype, q, index)
     _launch(index, _capi.lib().cti_ebag_dequantize_int8, q.data_ptr(), scale.data_ptr(), rows, dim, out.data_ptr(), code)
@@ -1048,7 +1049,7 @@ def linear_int8(
     ``out_dtype`` (bf16 by default; or ``out``'s type). With ``split_k`` (default) a workspace from torch's
     allocator lets a shape whose tiles would leave CUs idle have K split over several workgroups, and
     operands of odd widths be copied to whole steps first, where that is faster; the result is the same
-    bit for bit. Written on torch's current stream.
+    bit for bit. ``out`` overlaps no input. Written on torch's current stream.
     """
     return _linear_int8(q, scale, weight, weight_scale, bias, _capi.GATE_NONE, out, out_dtype, split_k)
 
