@@ -992,6 +992,10 @@ def layer_norm_int8(
     return _norm_int8(_capi.LAYER_NORM, x, weight, bias, eps, residual, q, scale, residual_out)
 
 
+# The library's limits. It takes both as 32-bit numbers and ctypes drops the bits above, so what is past them must not get there.
+_LINEAR_INT8_MAX_COLS, _LINEAR_INT8_MAX_OUT = 131071, 1 << 30
+
+
 def _linear_int8(q, scale, weight, weight_scale, bias, gate: int, out, out_dtype, split_k: bool):
     rows, cols, index = _check_int8_rows("q", q, "scale", scale)
     w_rows, w_cols, _ = _check_int8_rows("weight", weight, "weight_scale", weight_scale, index)
@@ -1004,6 +1008,10 @@ def _linear_int8(q, scale, weight, weight_scale, bias, gate: int, out, out_dtype
         if w_rows % 2:
             raise ValueError(f"weight has {w_rows} rows; expected as many gates as values (an even number)")
         n_out = w_rows // 2
+    if cols > _LINEAR_INT8_MAX_COLS or n_out > _LINEAR_INT8_MAX_OUT:
+        what, size, most = (("cols", cols, _LINEAR_INT8_MAX_COLS) if cols > _LINEAR_INT8_MAX_COLS
+                            else ("out_features", n_out, _LINEAR_INT8_MAX_OUT))
+        raise _capi.EbagError(_capi.EUNSUPPORTED, f"{what} {size} > {most}")
     bias_ptr, bias_code = None, _capi.F32
     if bias is not None:
         _require_on("bias", bias, index)
