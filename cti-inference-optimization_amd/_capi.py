@@ -120,6 +120,7 @@ SIGNATURES = {
         [_P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I64, _I64, _P],
     ),
     "cti_ebag_quantize_int8": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),
+    "cti_ebag_quantize_activations_int8": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),
     "cti_ebag_dequantize_int8": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _I32, _P]),
     "cti_ebag_norm_int8": (
         ctypes.c_int,

@@ -5,7 +5,8 @@
 //                                        multiply by the scalar's fp32 reciprocal; then
 //                                        torch.clamp(scale, min=1e-8))
 //   q[r, j] = clamp(rint(w[r, j] / s), -128, 127)   (IEEE fp32 division, round half to even)
-// Results are bit-identical to that expression for finite tables.
+// Results are bit-identical to that expression for finite tables. In a table, NaN is left out of m (and becomes q = 0);
+// rows of activations may not lose it (nan_rows): one with NaN or infinity in it gets the scale NaN and q = 0.
 //
 // A streaming pass: each element is read once and written once as a byte. Bound by HBM (2M rows of
 // 128 bf16: 512 MB read, 264 MB written), so a lane group reads its row as 16-byte vectors, keeps
@@ -25,20 +26,56 @@ constexpr int kQuantRowsPerBlock = kQuantThreads / kWave;  // wavefronts per wor
 // Row sets a wavefront of the chunk form has in flight: 4 loads per lane.
 constexpr int rows_in_flight(int chunks_per_lane) { return 4 / chunks_per_lane; }
 
+// The largest of m and every |v|, NaN if any is. (v_maximum3_f32: two elements an instruction.)
+template <int N>
+__device__ __forceinline__ float max_abs(float m, const float* v) {
+  if constexpr (N == 1) return __builtin_elementwise_maximum(m, __builtin_fabsf(v[0]));
+#pragma unroll
+  for (int e = 0; e + 1 < N; e += 2)
+    m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(__builtin_fabsf(v[e]), __builtin_fabsf(v[e + 1])), m);
+  return m;
+}
+// The largest of m and of the |v| that are not NaN: taken again where a table's row has NaN.
+template <int N>
+__device__ __forceinline__ float max_abs_numbers(float m, const float* v) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) m = fmaxf(m, __builtin_fabsf(v[e]));
+  return m;
+}
+// The bits of such a maximum: ordered as the values are, NaN above infinity, so that maxima over lanes keep it.
+constexpr uint32_t kInfBits = 0x7f800000u;
+__device__ __forceinline__ uint32_t max_bits(float m) { return __float_as_uint(m) & 0x7fffffffu; }
+
+__device__ __forceinline__ float row_scale(uint32_t bits, bool nan_rows) {
+  const float s = __uint_as_float(bits) * (1.0f / 127.0f);
+  if (nan_rows && bits >= kInfBits) return __uint_as_float(0x7fc00000u);
+  return s < 1e-8f ? 1e-8f : s;
+}
+
 // Any width and alignment: one wavefront per row, the row read twice.
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_loop_kernel(const char* w, int64_t rows, int64_t dim,
-                                                                       int64_t row_stride, int8_t* q, float* scale) {
+                                                                       int64_t row_stride, bool nan_rows, int8_t* q,
+                                                                       float* scale) {
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kQuantRowsPerBlock + threadIdx.x / kWave;
   if (row >= rows) return;  // uniform over the wavefront
   const int lane = lane_id();
   const char* wr = w + row * row_stride * Elem<T>::kBytes;
   float m = 0.f;
-  for (int64_t c = lane; c < dim; c += kWave) m = fmaxf(m, fabsf(Elem<T>::load(wr + c * Elem<T>::kBytes)));
-#pragma unroll
-  for (int k = 1; k < kWave; k <<= 1) m = fmaxf(m, shfl_xor_f32(m, k));
-  float s = m * (1.0f / 127.0f);
-  s = s < 1e-8f ? 1e-8f : s;
+  for (int64_t c = lane; c < dim; c += kWave) {
+    const float v = Elem<T>::load(wr + c * Elem<T>::kBytes);
+    m = max_abs<1>(m, &v);
+  }
+  uint32_t top = block_max_bits<1>(max_bits(m), nullptr);
+  if (top > kInfBits && !nan_rows) {  // the same in every lane
+    m = 0.f;
+    for (int64_t c = lane; c < dim; c += kWave) {
+      const float v = Elem<T>::load(wr + c * Elem<T>::kBytes);
+      m = max_abs_numbers<1>(m, &v);
+    }
+    top = block_max_bits<1>(max_bits(m), nullptr);
+  }
+  const float s = row_scale(top, nan_rows);
   if (lane == 0) scale[row] = s;
   int8_t* qr = q + row * dim;
   for (int64_t c = lane; c < dim; c += kWave) {
@@ -78,24 +115,26 @@ __device__ __forceinline__ void unpack_chunk(const typename Chunk<C * Elem<T>::k
   for (int e = 0; e < C; ++e) v[e] = t[e];
 }
 
-// Maximum over each aligned group of 1 << lg lanes, in every lane of the group (m >= 0): lane moves
-// inside 16 lanes on the VALU (DPP), across them through LDS.
-__device__ __forceinline__ float group_max(float m, int lg) {
-  const auto dpp = [](float x, auto ctrl) {
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
+// Maximum over each aligned group of 1 << lg lanes, in every lane of the group: lane moves inside 16 lanes on the VALU
+// (DPP), across them through LDS.
+__device__ __forceinline__ uint32_t group_max(uint32_t m, int lg) {
+  const auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+  const auto dpp = [](uint32_t x, auto ctrl) {
+    return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), decltype(ctrl)::value, 0xf, 0xf, true));
   };
-  if (lg > 0) m = fmaxf(m, dpp(m, std::integral_constant<int, 0xb1>{}));   // quad_perm: lane ^ 1
-  if (lg > 1) m = fmaxf(m, dpp(m, std::integral_constant<int, 0x4e>{}));   // quad_perm: lane ^ 2
-  if (lg > 2) m = fmaxf(m, dpp(m, std::integral_constant<int, 0x141>{}));  // row_half_mirror
-  if (lg > 3) m = fmaxf(m, dpp(m, std::integral_constant<int, 0x140>{}));  // row_mirror
-  if (lg > 4) m = fmaxf(m, shfl_xor_f32(m, 16));
-  if (lg > 5) m = fmaxf(m, shfl_xor_f32(m, 32));
+  const auto other = [](uint32_t x, int by) { return static_cast<uint32_t>(shfl_i32(static_cast<int>(x), lane_id() ^ by)); };
+  if (lg > 0) m = larger(m, dpp(m, std::integral_constant<int, 0xb1>{}));   // quad_perm: lane ^ 1
+  if (lg > 1) m = larger(m, dpp(m, std::integral_constant<int, 0x4e>{}));   // quad_perm: lane ^ 2
+  if (lg > 2) m = larger(m, dpp(m, std::integral_constant<int, 0x141>{}));  // row_half_mirror
+  if (lg > 3) m = larger(m, dpp(m, std::integral_constant<int, 0x140>{}));  // row_mirror
+  if (lg > 4) m = larger(m, other(m, 16));
+  if (lg > 5) m = larger(m, other(m, 32));
   return m;
 }
 
 template <typename T, int C, int K>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const char* w, int64_t rows, int32_t chunks,
-                                                                       int64_t row_bytes, int lg, int8_t* q,
+                                                                       int64_t row_bytes, int lg, bool nan_rows, int8_t* q,
                                                                        float* scale) {
   using V = typename Chunk<C * Elem<T>::kBytes>::type;
   constexpr int kRows = rows_in_flight(K);
@@ -123,12 +162,16 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const char
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       unpack_chunk<T, C>(raw[u][k], v[k]);
-#pragma unroll
-      for (int e = 0; e < C; ++e) m = fmaxf(m, fabsf(v[k][e]));
+      m = max_abs<C>(m, v[k]);
     }
-    m = group_max(m, lg);
-    float s = m * (1.0f / 127.0f);
-    s = s < 1e-8f ? 1e-8f : s;
+    uint32_t top = group_max(max_bits(m), lg);
+    if (__builtin_expect(__ballot(top > kInfBits) != 0 && !nan_rows, 0)) {  // (a whole wavefront: lanes read each other)
+      m = 0.f;
+#pragma unroll
+      for (int k = 0; k < K; ++k) m = max_abs_numbers<C>(m, v[k]);
+      top = group_max(max_bits(m), lg);
+    }
+    const float s = row_scale(top, nan_rows);
     const float inv = 1.0f / s;
     if (row < rows && sl == 0) scale[row] = s;
 #pragma unroll
@@ -159,7 +202,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const char
 // and the row is at most 4 chunks per lane of a wavefront (single elements: 2; 200,000 rows of 129 /
 // 191 / 255 bf16 took 62 / 68 / 82 us at 4, the loop kernel 59 / 64 / 79); false: not this form.
 template <typename T, int C>
-bool launch_chunks(const char* w, int64_t rows, int64_t dim, int64_t row_stride, int8_t* q, float* scale,
+bool launch_chunks(const char* w, int64_t rows, int64_t dim, int64_t row_stride, bool nan_rows, int8_t* q, float* scale,
                    hipStream_t s) {
   constexpr int BYTES = C * Elem<T>::kBytes;
   if (dim % C != 0 || (row_stride * Elem<T>::kBytes) % BYTES != 0 || reinterpret_cast<uintptr_t>(w) % BYTES != 0 ||
@@ -172,10 +215,10 @@ bool launch_chunks(const char* w, int64_t rows, int64_t dim, int64_t row_stride,
   const int64_t per_block = static_cast<int64_t>(kQuantRowsPerBlock) * (kWave >> lg) * rows_in_flight(K);
   const dim3 grid(static_cast<unsigned>((rows + per_block - 1) / per_block)), block(kQuantThreads);
   const int64_t rb = row_stride * Elem<T>::kBytes;
-  if (K == 1) hipLaunchKernelGGL((quantize_rows_kernel<T, C, 1>), grid, block, 0, s, w, rows, chunks, rb, lg, q, scale);
-  if (K == 2) hipLaunchKernelGGL((quantize_rows_kernel<T, C, 2>), grid, block, 0, s, w, rows, chunks, rb, lg, q, scale);
+  if (K == 1) hipLaunchKernelGGL((quantize_rows_kernel<T, C, 1>), grid, block, 0, s, w, rows, chunks, rb, lg, nan_rows, q, scale);
+  if (K == 2) hipLaunchKernelGGL((quantize_rows_kernel<T, C, 2>), grid, block, 0, s, w, rows, chunks, rb, lg, nan_rows, q, scale);
   if constexpr (C > 1) {
-    if (K == 4) hipLaunchKernelGGL((quantize_rows_kernel<T, C, 4>), grid, block, 0, s, w, rows, chunks, rb, lg, q, scale);
+    if (K == 4) hipLaunchKernelGGL((quantize_rows_kernel<T, C, 4>), grid, block, 0, s, w, rows, chunks, rb, lg, nan_rows, q, scale);
   }
   return true;
 }
@@ -186,7 +229,7 @@ bool launch_chunks(const char* w, int64_t rows, int64_t dim, int64_t row_stride,
 // loop kernel (one wavefront a row, 2-byte loads, the row read twice), 10.2 in this; one row of 4,096: 18.6 and 5.0.
 template <typename T, int K, int WAVES>
 __global__ void __launch_bounds__(WAVES * kWave) quantize_wide_kernel(const char* w, int32_t dim, int64_t row_bytes,
-                                                                      int8_t* q, float* scale) {
+                                                                      bool nan_rows, int8_t* q, float* scale) {
   constexpr int VEC = 16 / Elem<T>::kBytes, THREADS = WAVES * kWave;
   __shared__ uint32_t s_max[WAVES];
   const int64_t row = blockIdx.x;
@@ -205,11 +248,17 @@ __global__ void __launch_bounds__(WAVES * kWave) quantize_wide_kernel(const char
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     unpack16(raw[k], v[k], T{});
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) m = fmaxf(m, fabsf(v[k][e]));  // (NaN is left out, as in the other forms)
+    m = max_abs<VEC>(m, v[k]);
   }
-  float s = __uint_as_float(block_max_bits<WAVES>(__float_as_uint(m), s_max)) * (1.0f / 127.0f);
-  s = s < 1e-8f ? 1e-8f : s;
+  uint32_t top = block_max_bits<WAVES>(max_bits(m), s_max);
+  if (__builtin_expect(top > kInfBits && !nan_rows, 0)) {  // the same in every thread
+    m = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) m = max_abs_numbers<VEC>(m, v[k]);
+    __syncthreads();  // every wavefront has read the first maximum
+    top = block_max_bits<WAVES>(max_bits(m), s_max);
+  }
+  const float s = row_scale(top, nan_rows);
   const float inv = 1.0f / s;
   if (t == 0) scale[row] = s;
 #pragma unroll
@@ -224,7 +273,8 @@ __global__ void __launch_bounds__(WAVES * kWave) quantize_wide_kernel(const char
 }
 
 template <typename T>
-bool launch_wide(const char* w, int64_t rows, int64_t dim, int64_t row_stride, int8_t* q, float* scale, hipStream_t s) {
+bool launch_wide(const char* w, int64_t rows, int64_t dim, int64_t row_stride, bool nan_rows, int8_t* q, float* scale,
+                 hipStream_t s) {
   constexpr int VEC = 16 / Elem<T>::kBytes;
   const int64_t vecs = (dim + VEC - 1) / VEC;
   if (vecs <= kWave || vecs > 64 * kWave) return false;
@@ -235,7 +285,7 @@ bool launch_wide(const char* w, int64_t rows, int64_t dim, int64_t row_stride, i
     for (int64_t r = 0; r < rows; r += kRows) {
       const dim3 grid(static_cast<unsigned>(rows - r < kRows ? rows - r : kRows));
       hipLaunchKernelGGL((quantize_wide_kernel<T, decltype(k)::value, W>), grid, dim3(W * kWave), 0, s, w + r * rb,
-                         static_cast<int32_t>(dim), rb, q + r * dim, scale + r);
+                         static_cast<int32_t>(dim), rb, nan_rows, q + r * dim, scale + r);
     }
   };
   constexpr std::integral_constant<int, 1> n1{};
@@ -253,18 +303,18 @@ bool launch_wide(const char* w, int64_t rows, int64_t dim, int64_t row_stride, i
 // The widest chunks that fit; wider rows than they cover take the wide kernel, what that does not cover either the
 // loop kernel.
 template <typename T>
-void launch_quantize(const char* w, int64_t rows, int64_t dim, int64_t row_stride, int8_t* q, float* scale,
+void launch_quantize(const char* w, int64_t rows, int64_t dim, int64_t row_stride, bool nan_rows, int8_t* q, float* scale,
                      hipStream_t s) {
   constexpr int kMax = 16 / Elem<T>::kBytes;
-  if (launch_chunks<T, kMax>(w, rows, dim, row_stride, q, scale, s)) return;
-  if (launch_chunks<T, kMax / 2>(w, rows, dim, row_stride, q, scale, s)) return;
-  if (launch_chunks<T, kMax / 4>(w, rows, dim, row_stride, q, scale, s)) return;
+  if (launch_chunks<T, kMax>(w, rows, dim, row_stride, nan_rows, q, scale, s)) return;
+  if (launch_chunks<T, kMax / 2>(w, rows, dim, row_stride, nan_rows, q, scale, s)) return;
+  if (launch_chunks<T, kMax / 4>(w, rows, dim, row_stride, nan_rows, q, scale, s)) return;
   if constexpr (kMax == 8) {
-    if (launch_chunks<T, 1>(w, rows, dim, row_stride, q, scale, s)) return;
+    if (launch_chunks<T, 1>(w, rows, dim, row_stride, nan_rows, q, scale, s)) return;
   }
-  if (launch_wide<T>(w, rows, dim, row_stride, q, scale, s)) return;
+  if (launch_wide<T>(w, rows, dim, row_stride, nan_rows, q, scale, s)) return;
   const dim3 grid(static_cast<unsigned>((rows + kQuantRowsPerBlock - 1) / kQuantRowsPerBlock)), block(kQuantThreads);
-  hipLaunchKernelGGL((quantize_rows_loop_kernel<T>), grid, block, 0, s, w, rows, dim, row_stride, q, scale);
+  hipLaunchKernelGGL((quantize_rows_loop_kernel<T>), grid, block, 0, s, w, rows, dim, row_stride, nan_rows, q, scale);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -373,8 +423,8 @@ extern "C" int cti_ebag_dequantize_int8(const int8_t* q, const float* scale, int
   return CTI_EBAG_OK;
 }
 
-extern "C" int cti_ebag_quantize_int8(const void* weight, int32_t dtype, int64_t rows, int64_t dim,
-                                      int64_t row_stride, int8_t* q, float* scale, void* stream) {
+static int quantize(const void* weight, int32_t dtype, int64_t rows, int64_t dim, int64_t row_stride, bool nan_rows,
+                    int8_t* q, float* scale, void* stream) {
   clear_error();
   if (dtype != CTI_EBAG_F32 && dtype != CTI_EBAG_BF16 && dtype != CTI_EBAG_F16)
     return set_error(CTI_EBAG_EINVAL, "unknown dtype code %d", dtype);
@@ -388,11 +438,21 @@ extern "C" int cti_ebag_quantize_int8(const void* weight, int32_t dtype, int64_t
   hipStream_t s = static_cast<hipStream_t>(stream);
   const char* w = static_cast<const char*>(weight);
   switch (dtype) {
-    case CTI_EBAG_F32: launch_quantize<float>(w, rows, dim, row_stride, q, scale, s); break;
-    case CTI_EBAG_BF16: launch_quantize<bf16_t>(w, rows, dim, row_stride, q, scale, s); break;
-    default: launch_quantize<f16_t>(w, rows, dim, row_stride, q, scale, s); break;
+    case CTI_EBAG_F32: launch_quantize<float>(w, rows, dim, row_stride, nan_rows, q, scale, s); break;
+    case CTI_EBAG_BF16: launch_quantize<bf16_t>(w, rows, dim, row_stride, nan_rows, q, scale, s); break;
+    default: launch_quantize<f16_t>(w, rows, dim, row_stride, nan_rows, q, scale, s); break;
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(CTI_EBAG_EHIP, "quantize launch failed: %s", hipGetErrorString(e));
   return CTI_EBAG_OK;
+}
+
+extern "C" int cti_ebag_quantize_int8(const void* weight, int32_t dtype, int64_t rows, int64_t dim,
+                                      int64_t row_stride, int8_t* q, float* scale, void* stream) {
+  return quantize(weight, dtype, rows, dim, row_stride, false, q, scale, stream);
+}
+
+extern "C" int cti_ebag_quantize_activations_int8(const void* x, int32_t dtype, int64_t rows, int64_t dim,
+                                                  int64_t row_stride, int8_t* q, float* scale, void* stream) {
+  return quantize(x, dtype, rows, dim, row_stride, true, q, scale, stream);
 }

@@ -54,9 +54,11 @@ class RepEncoder(nn.Module):
 
     def quantize_linear_int8_(self):
         """Quantise ``linear``'s weight to int8 rows + fp32 scales, one for each output channel, as it is
-        now (call it again after the weight has changed); ``forward`` multiplies in int8 from then on."""
+        now (call it again after the weight has changed or the module has moved); ``forward`` multiplies in
+        int8 from then on and no longer calls ``linear`` itself, nor its hooks. A channel whose weights are
+        not all finite gives NaN."""
         with torch.no_grad():
-            self._int8_linear = quantize_embedding_int8(self.linear.weight.detach())
+            self._int8_linear = quantize_embedding_int8(self.linear.weight.detach(), nan_rows=True)
         return self
 
     def dequantize_linear_(self):

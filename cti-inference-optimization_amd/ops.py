@@ -96,14 +96,18 @@ def _table_descs(tables):
     return descs, dev, code, col, tdt
 
 
-def quantize_embedding_int8(weight: torch.Tensor):
-    """Row-quantise a GPU table to int8: ``(q [V, D] int8, scale [V] float32)``.
+def quantize_embedding_int8(weight: torch.Tensor, nan_rows: bool = False):
+    """Row-quantise a GPU table, or rows of activations, to int8: ``(q [V, D] int8, scale [V] float32)``.
 
     Mirrors online_best/infer.py:895-901 as torch evaluates it on the device:
     ``scale = max(max_j |w_j| * fp32(1/127), 1e-8)`` (torch turns the division by the Python
     scalar 127.0 into a multiply by its fp32 reciprocal), ``q = clamp(round_half_even(w / scale),
     -128, 127)``, all in fp32; bit-identical to that expression for finite tables. ``weight`` is
     fp32 / bf16 / fp16 with unit column stride.
+
+    Tables are finite: NaN is left out of a row's maximum and becomes 0. Activations need not be, and
+    NaN must not get lost in them: with ``nan_rows`` a row with NaN or infinity in it gets the scale NaN
+    and ``q`` 0, as the int8 norms give it, so that its products are NaN. Other rows are the same.
     """
     _require_device_tensor("weight", weight)
     if weight.dim() != 2 or weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
@@ -112,7 +116,8 @@ def quantize_embedding_int8(weight: torch.Tensor):
     dev = weight.device
     q = torch.empty(rows, dim, dtype=torch.int8, device=dev)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
-    _launch(dev.index, _capi.lib().cti_ebag_quantize_int8, weight.data_ptr(), _capi.dtype_code(weight.dtype), rows, dim,
+    lib = _capi.lib()
+    _launch(dev.index, lib.cti_ebag_quantize_activations_int8 if nan_rows else lib.cti_ebag_quantize_int8, weight.data_ptr(), _capi.dtype_code(weight.dtype), rows, dim,
             weight.stride(0), q.data_ptr(), scale.data_ptr())
     return q, scale
 
@@ -1080,6 +1085,7 @@ def gated_linear_int8(
     ``out[m, n] = act(v[m, n]) * v[m, hidden + n]``, ``n < hidden``,
 
     rounded once. ``activation`` is "silu", "gelu" (exact) or "relu". The rest is as in
-    ``linear_int8``; ``quantize_embedding_int8`` makes the input of the projection back of the result.
+    ``linear_int8``; ``quantize_embedding_int8(out, nan_rows=True)`` makes the input of the projection
+    back of the result.
     """
     return _linear_int8(q, scale, weight, weight_scale, bias, _capi.gate_code(activation), out, out_dtype, split_k)

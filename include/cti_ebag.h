@@ -408,10 +408,18 @@ int64_t cti_ebag_stage_offset(const int64_t* counts, int32_t n_parts, int32_t ds
  *   scalar 127.0 is a multiply by its fp32 reciprocal there), q[r, j] = clamp(rint(w / s), -128, 127)
  * with IEEE fp32 division and round half to even, bit for bit.
  *   weight  [rows, row_stride] of `dtype` (F32/BF16/F16), first `dim` columns used
- *   q       int8 [rows, dim] (contiguous), scale fp32 [rows]. Tables must be finite.
+ *   q       int8 [rows, dim] (contiguous), scale fp32 [rows]. Tables must be finite: NaN is left out of
+ *           m and its q is 0.
  */
 int cti_ebag_quantize_int8(const void* weight, int32_t dtype, int64_t rows, int64_t dim, int64_t row_stride,
                            int8_t* q, float* scale, void* stream);
+
+/*
+ * The same for rows that need not be finite, as a model's activations: a row with NaN or infinity in it gets scale
+ * NaN and q = 0, as from cti_ebag_norm_int8, so what is computed from it is NaN. Finite rows as above, bit for bit.
+ */
+int cti_ebag_quantize_activations_int8(const void* x, int32_t dtype, int64_t rows, int64_t dim, int64_t row_stride,
+                                       int8_t* q, float* scale, void* stream);
 
 /*
  * Row LayerNorm over the pooled block, a drop-in for the launch
