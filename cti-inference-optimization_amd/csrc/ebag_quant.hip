@@ -227,6 +227,8 @@ bool launch_chunks(const char* w, int64_t rows, int64_t dim, int64_t row_stride,
 // t + THREADS, ... (K of them), at any alignment; the last vector ends with the row and overlaps the one before it where
 // the row is no whole number of them (the bytes both store are the same). 2,048 rows of 5,632 bf16: 57.7 us in the
 // loop kernel (one wavefront a row, 2-byte loads, the row read twice), 10.2 in this; one row of 4,096: 18.6 and 5.0.
+// Up to 128 vectors take two wavefronts (200,000 rows of 257 fp32: 94 us in the loop kernel, 102 by four wavefronts of
+// which three are idle, 67 by two; of 1,021 bf16 410, 182 and 134).
 template <typename T, int K, int WAVES>
 __global__ void __launch_bounds__(WAVES * kWave) quantize_wide_kernel(const char* w, int32_t dim, int64_t row_bytes,
                                                                       bool nan_rows, int8_t* q, float* scale) {
@@ -292,7 +294,8 @@ bool launch_wide(const char* w, int64_t rows, int64_t dim, int64_t row_stride, b
   constexpr std::integral_constant<int, 2> n2{};
   constexpr std::integral_constant<int, 4> n4{};
   constexpr std::integral_constant<int, 16> n16{};
-  if (vecs <= 4 * kWave) go(n1, n4);
+  if (vecs <= 2 * kWave) go(n1, n2);
+  else if (vecs <= 4 * kWave) go(n1, n4);
   else if (vecs <= 8 * kWave) go(n2, n4);
   else if (vecs <= 16 * kWave) go(n4, n4);
   else if (vecs <= 32 * kWave) go(n2, n16);
