@@ -810,11 +810,15 @@ hipError_t launch_part(Linear8Params p, const Linear8Part& part, int32_t* work, 
   switch (part.form) {
     case kLinear8Rows:
       // the steps of a split in one batch of loads where they are few
-      if (part.steps <= 4) go(linear8_rows_kernel<YT, 4, 1, GATED>, 4);
-      else if (part.steps <= 8) go(linear8_rows_kernel<YT, 4, 2, GATED>, 4);
-      else if (part.steps <= 16) go(linear8_rows_kernel<YT, 4, 4, GATED>, 4);
-      else if (part.steps <= 32) go(linear8_rows_kernel<YT, 8, 4, GATED>, 8);
-      else go(linear8_rows_kernel<YT, 16, 4, GATED>, 16);
+      switch (linear8_rows_waves(part.steps)) {
+        case 4:
+          if (part.steps <= 4) go(linear8_rows_kernel<YT, 4, 1, GATED>, 4);
+          else if (part.steps <= 8) go(linear8_rows_kernel<YT, 4, 2, GATED>, 4);
+          else go(linear8_rows_kernel<YT, 4, 4, GATED>, 4);
+          break;
+        case 8: go(linear8_rows_kernel<YT, 8, 4, GATED>, 8); break;
+        default: go(linear8_rows_kernel<YT, 16, 4, GATED>, 16);
+      }
       break;
     case kLinear8Any: go(linear8_tile_kernel<YT, 128, 128, 2, 2, GATED>, 4); break;
     case kLinear8Ring: go(linear8_ring_kernel<YT, 64, 64, 2, 2, GATED>, 4); break;
@@ -881,6 +885,7 @@ extern "C" int64_t cti_ebag_linear_int8_workspace_bytes(int64_t rows, int32_t co
       out_features > kLinear8MaxN || gate < CTI_EBAG_GATE_NONE || gate > CTI_EBAG_GATE_RELU)
     return 0;
   const bool gated = gate != CTI_EBAG_GATE_NONE;
+  if (out_features > linear8_max_out(gated)) return 0;
   return linear8_workspace_bytes(rows, out_features, cols, gated);
 }
 
@@ -907,15 +912,14 @@ extern "C" int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return set_error(CTI_EBAG_EINVAL, "workspace is not 16-byte aligned");
   const bool gated = gate != CTI_EBAG_GATE_NONE;
+  if (out_features > linear8_max_out(gated))
+    return set_error(CTI_EBAG_EUNSUPPORTED, "too many output tiles (%lld x %d)", (long long)rows, out_features);
   const bool aligned = cols % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 && reinterpret_cast<uintptr_t>(weight) % 16 == 0;
   const int64_t ws_bytes = workspace ? workspace_bytes : 0;
   const auto plan_of = [&](int64_t m) { return linear8_plan(m, out_features, cols, gated, aligned, ws_bytes); };
-  // launches of kLinear8LaunchRows rows, and of those left
-  const int64_t rest = rows % kLinear8LaunchRows, whole = rows - rest;
-  const Linear8Plan plan = whole ? plan_of(kLinear8LaunchRows) : Linear8Plan{}, last = rest ? plan_of(rest) : Linear8Plan{};
-  if (linear8_workgroups(plan, kLinear8LaunchRows, gated) > kLinear8MaxTiles ||
-      linear8_workgroups(last, rest, gated) > kLinear8MaxTiles)
-    return set_error(CTI_EBAG_EUNSUPPORTED, "too many output tiles (%lld x %d)", (long long)rows, out_features);
+  // launches of `most` rows, and of those left
+  const int64_t most = linear8_launch_rows(out_features, gated), rest = rows % most, whole = rows - rest;
+  const Linear8Plan plan = whole ? plan_of(most) : Linear8Plan{}, last = rest ? plan_of(rest) : Linear8Plan{};
   Linear8Params p = {};
   p.w = weight;
   p.wscale = weight_scale;
@@ -927,9 +931,9 @@ extern "C" int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t
   p.gate = gate;
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* const work = static_cast<char*>(workspace);
-  for (int64_t m = 0; m < rows; m += kLinear8LaunchRows) {
+  for (int64_t m = 0; m < rows; m += most) {
     const Linear8Plan& of = m < whole ? plan : last;
-    p.M = m < whole ? kLinear8LaunchRows : rest;
+    p.M = m < whole ? most : rest;
     p.x = q + m * cols;
     p.scale = scale + m;
     p.y = static_cast<char*>(y) + m * out_features * dtype_bytes(y_dtype);

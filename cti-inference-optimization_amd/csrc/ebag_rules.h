@@ -223,7 +223,7 @@ inline int64_t linear8_tiles(Linear8Form form, int64_t M, int64_t cols, bool gat
   const Linear8Tile tile = linear8_tile(form);
   return linear_ceil(M, tile.rows) * linear_ceil(cols, gated && form != kLinear8Rows ? tile.cols / 2 : tile.cols);
 }
-// The most workgroups of a launch (of one split).
+// The most workgroups of a plan's launches (of one split).
 inline int64_t linear8_workgroups(const Linear8Plan& plan, int64_t M, bool gated) {
   int64_t most = 0;
   for (int i = 0; i < plan.parts; ++i) {
@@ -233,10 +233,25 @@ inline int64_t linear8_workgroups(const Linear8Plan& plan, int64_t M, bool gated
   return most;
 }
 
-// Rows of x in a launch, more take several: a launch has fewer than 2^32 threads, up to 1,024 a workgroup, and the copy of operands of odd widths
-// stays small beside what they were made from. (A launch of 2^20 rows leaves at most 1 round of tiles in 16 unfilled.)
+// A launch has fewer than 2^32 threads: the most workgroups of one, by their threads (those of the rows form go by the
+// steps of K that it has, see linear8_rows_waves).
+constexpr int linear8_rows_waves(int steps) { return steps <= 16 ? 4 : steps <= 32 ? 8 : 16; }
+inline int64_t linear8_max_tiles(Linear8Form form, int steps) {
+  const int waves = form == kLinear8Rows ? linear8_rows_waves(steps) : form == kLinear8Any || form == kLinear8Ring ? 4 : 8;
+  return UINT32_MAX / (waves * 64);
+}
+// Outputs that are taken, whatever the operands' addresses and the workspace: so many that a row of 256 x 256 tiles has no
+// more workgroups than a launch of 1,024 threads each.
+inline int64_t linear8_max_out(bool gated) { return static_cast<int64_t>(UINT32_MAX / 1024) * (gated ? 128 : 256); }
+// Rows of x in a launch, more take several: so the copy of operands of odd widths stays small beside what they were made
+// from (a launch of 2^20 rows leaves at most 1 round of tiles in 16 unfilled), and for outputs past 2^18 (gated 2^17) the
+// form that takes every operand has a launch (of 128 rows it has one for every number of outputs that is taken).
 constexpr int64_t kLinear8LaunchRows = int64_t{1} << 20;
-constexpr int64_t kLinear8MaxTiles = UINT32_MAX / 1024;
+inline int64_t linear8_launch_rows(int32_t N, bool gated) {
+  int64_t rows = kLinear8LaunchRows;
+  while (linear8_tiles(kLinear8Any, rows, N, gated) > linear8_max_tiles(kLinear8Any, 0)) rows /= 2;
+  return rows;
+}
 
 // The estimated time (us) of one part. Workgroups run `slots` at a time (what fits the CUs); a round takes a fixed
 // time and a time per step, which grows from `step` to `full` as the round fills the chip. What the operands, the
@@ -296,6 +311,7 @@ inline Linear8Part linear8_best(int64_t M, int32_t n_begin, int32_t n_end, int32
     const Linear8Form form = static_cast<Linear8Form>(f);
     if (form != kLinear8Rows && form != kLinear8Any && !aligned) continue;
     const int64_t tiles = linear8_tiles(form, M, n_end - n_begin, gated);
+    if (tiles > linear8_max_tiles(form, nk)) continue;  // (never the form for any operand: linear8_launch_rows)
     for (int want = 1; want <= 32; want *= 2) {
       Linear8Part part{form, 1, nk, n_begin, n_end};
       if (want > 1) {
@@ -346,7 +362,7 @@ inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, boo
   if (aligned) {
     const int64_t rows = linear_ceil(M, 256), wide = gated ? 128 : 256, tiles = rows * linear_ceil(N, wide);
     const int64_t whole = tiles / kLinearCus * kLinearCus / rows * wide;  // columns of the whole rounds
-    if (tiles > kLinearCus && whole > 0 && whole < N) {
+    if (tiles > kLinearCus && whole > 0 && whole < N && rows * (whole / wide) <= linear8_max_tiles(kLinear8Tile256, 0)) {
       const int nk = static_cast<int>(linear_ceil(K, kLinear8Step));
       const Linear8Part first{kLinear8Tile256, 1, nk, 0, static_cast<int32_t>(whole)};
       double rest = 0;
@@ -366,7 +382,7 @@ inline int64_t linear8_workspace_bytes(int64_t M, int32_t N, int32_t K, bool gat
   const auto of = [&](int64_t rows) {
     return rows > 0 ? linear8_plan_bytes(linear8_plan(rows, N, K, gated, K % 16 == 0, INT64_MAX), rows, N, K, gated) : 0;
   };
-  const int64_t rest = of(M % kLinear8LaunchRows), whole = M >= kLinear8LaunchRows ? of(kLinear8LaunchRows) : 0;
+  const int64_t most = linear8_launch_rows(N, gated), rest = of(M % most), whole = M >= most ? of(most) : 0;
   return rest > whole ? rest : whole;
 }
 

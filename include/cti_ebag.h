@@ -517,8 +517,8 @@ int cti_ebag_norm_int8(int32_t kind, const void* x, const void* residual, void* 
  *            CUs idle, K is split over several workgroups per tile, each writing int32 partial sums here, and a
  *            second launch adds them; operands whose rows are no multiple of 16 bytes, or that start at no
  *            16-byte address, are first copied here to rows of a multiple of 128. What does not fit is not done.
- * cols at most 131071 (the int32 sums cannot overflow up to there), out_features at most 2^30 and of no more than
- * 2^22 - 1 tiles of the output (of 16 x 16 elements where rows are few). The integer
+ * cols at most 131071 (the int32 sums cannot overflow up to there), out_features at most 2^22 - 1 tiles of 256 rows of
+ * the weight (2^30 - 256; gated 2^29 - 128), wherever the operands lie and with any workspace. The integer
  * sums are exact, so the result is the same bit for bit with any workspace.
  */
 int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t rows, int32_t cols, const int8_t* weight,
