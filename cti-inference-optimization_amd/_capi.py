@@ -131,6 +131,7 @@ SIGNATURES = {
         [_P, _P, _I64, _I32, _P, _P, _I32, _P, _I32, _I32, _P, _I32, _P, _I64, _P],
     ),
     "cti_ebag_linear_int8_workspace_bytes": (ctypes.c_int64, [_I64, _I32, _I32, _I32]),
+    "cti_ebag_linear_int8_workspace_bytes_unaligned": (ctypes.c_int64, [_I64, _I32, _I32, _I32]),
     "cti_ebag_narrow_ids": (ctypes.c_int, [_P, _I64, _P, _I32]),
     "cti_ebag_fused_all_slots_layernorm": (
         ctypes.c_int,

@@ -880,13 +880,21 @@ bool float_dtype(int32_t dt) { return dt == CTI_EBAG_F32 || dt == CTI_EBAG_BF16 
 
 using namespace cti;
 
-extern "C" int64_t cti_ebag_linear_int8_workspace_bytes(int64_t rows, int32_t cols, int32_t out_features, int32_t gate) {
-  if (rows < 1 || rows > INT32_MAX || cols < 1 || cols > kLinear8MaxK || out_features < 1 ||
-      out_features > kLinear8MaxN || gate < CTI_EBAG_GATE_NONE || gate > CTI_EBAG_GATE_RELU)
-    return 0;
+static int64_t workspace_bytes(int64_t rows, int32_t cols, int32_t out_features, int32_t gate, bool aligned) {
   const bool gated = gate != CTI_EBAG_GATE_NONE;
-  if (out_features > linear8_max_out(gated)) return 0;
-  return linear8_workspace_bytes(rows, out_features, cols, gated);
+  if (rows < 1 || rows > INT32_MAX || cols < 1 || cols > kLinear8MaxK || out_features < 1 ||
+      out_features > linear8_max_out(gated) || gate < CTI_EBAG_GATE_NONE || gate > CTI_EBAG_GATE_RELU)
+    return 0;
+  return linear8_workspace_bytes(rows, out_features, cols, gated, aligned);
+}
+
+extern "C" int64_t cti_ebag_linear_int8_workspace_bytes(int64_t rows, int32_t cols, int32_t out_features, int32_t gate) {
+  return workspace_bytes(rows, cols, out_features, gate, true);
+}
+
+extern "C" int64_t cti_ebag_linear_int8_workspace_bytes_unaligned(int64_t rows, int32_t cols, int32_t out_features,
+                                                                  int32_t gate) {
+  return workspace_bytes(rows, cols, out_features, gate, false);
 }
 
 extern "C" int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t rows, int32_t cols, const int8_t* weight,

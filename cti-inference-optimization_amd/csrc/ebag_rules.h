@@ -377,10 +377,10 @@ inline Linear8Plan linear8_plan(int64_t M, int32_t N, int32_t K, bool gated, boo
   return plan;
 }
 
-// Bytes of workspace that a shape's operands, at 16-byte aligned addresses, are given at most.
-inline int64_t linear8_workspace_bytes(int64_t M, int32_t N, int32_t K, bool gated) {
+// Bytes of workspace that a shape's operands, at 16-byte aligned addresses or others, are given at most.
+inline int64_t linear8_workspace_bytes(int64_t M, int32_t N, int32_t K, bool gated, bool aligned) {
   const auto of = [&](int64_t rows) {
-    return rows > 0 ? linear8_plan_bytes(linear8_plan(rows, N, K, gated, K % 16 == 0, INT64_MAX), rows, N, K, gated) : 0;
+    return rows > 0 ? linear8_plan_bytes(linear8_plan(rows, N, K, gated, aligned && K % 16 == 0, INT64_MAX), rows, N, K, gated) : 0;
   };
   const int64_t most = linear8_launch_rows(N, gated), rest = of(M % most), whole = M >= most ? of(most) : 0;
   return rest > whole ? rest : whole;

@@ -1024,21 +1024,26 @@ def _linear_int8(q, scale, weight, weight_scale, bias, gate: int, out, out_dtype
             raise ValueError(f"bias has {bias.numel()} elements, expected {w_rows}")
         bias_ptr, bias_code = bias.data_ptr(), _capi.dtype_code(bias.dtype)
     out, code = _float_output(out, rows, n_out, out_dtype, q, index)
-    # partial sums of a split K, copies of operands of odd widths: in a workspace from torch's allocator
+    # partial sums of a split K, copies of operands of odd widths or addresses: in a workspace from torch's allocator
     # (kept alive until the launches are enqueued)
-    ws, ws_ptr, ws_bytes = None, None, _linear_int8_workspace(rows, cols, n_out, gate) if split_k else 0
-    if ws_bytes > 0:
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-        ws_ptr = ws.data_ptr()
-    _launch(index, _capi.lib().cti_ebag_linear_int8, q.data_ptr(), scale.data_ptr(), rows, cols, weight.data_ptr(),
+    q_ptr, w_ptr = q.data_ptr(), weight.data_ptr()
+    ws, ws_ptr, ws_bytes = None, None, 0
+    if split_k:
+        ws_bytes = _linear_int8_workspace(rows, cols, n_out, gate, (q_ptr | w_ptr) % 16 == 0)
+        if ws_bytes > 0:
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+            ws_ptr = ws.data_ptr()
+    _launch(index, _capi.lib().cti_ebag_linear_int8, q_ptr, scale.data_ptr(), rows, cols, w_ptr,
             weight_scale.data_ptr(), n_out, bias_ptr, bias_code, gate, out.data_ptr(), code, ws_ptr, ws_bytes)
     return out
 
 
 @functools.lru_cache(maxsize=4096)
-def _linear_int8_workspace(rows: int, cols: int, n_out: int, gate: int) -> int:
-    """The library's query, which goes by these sizes alone."""
-    return _capi.lib().cti_ebag_linear_int8_workspace_bytes(rows, cols, n_out, gate)
+def _linear_int8_workspace(rows: int, cols: int, n_out: int, gate: int, aligned: bool) -> int:
+    """The library's query, which goes by these sizes and whether q and the weight lie at 16-byte addresses alone."""
+    lib = _capi.lib()
+    query = lib.cti_ebag_linear_int8_workspace_bytes if aligned else lib.cti_ebag_linear_int8_workspace_bytes_unaligned
+    return query(rows, cols, n_out, gate)
 
 
 def linear_int8(
@@ -1061,8 +1066,8 @@ def linear_int8(
     the sum exact in int32 (``cols`` at most 131071), the rest in fp32 with one rounding to
     ``out_dtype`` (bf16 by default; or ``out``'s type). With ``split_k`` (default) a workspace from torch's
     allocator lets a shape whose tiles would leave CUs idle have K split over several workgroups, and
-    operands of odd widths be copied to whole steps first, where that is faster; the result is the same
-    bit for bit. ``out`` overlaps no input. Written on torch's current stream.
+    operands of odd widths or at odd addresses be copied to whole steps first, where that is faster; the
+    result is the same bit for bit. ``out`` overlaps no input. Written on torch's current stream.
     """
     return _linear_int8(q, scale, weight, weight_scale, bias, _capi.GATE_NONE, out, out_dtype, split_k)
 

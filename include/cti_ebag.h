@@ -530,6 +530,9 @@ int cti_ebag_linear_int8(const int8_t* q, const float* scale, int64_t rows, int3
  * (0: none). */
 int64_t cti_ebag_linear_int8_workspace_bytes(int64_t rows, int32_t cols, int32_t out_features, int32_t gate);
 
+/* The same where q or weight starts at no 16-byte address (both are copied to the workspace where that is faster). */
+int64_t cti_ebag_linear_int8_workspace_bytes_unaligned(int64_t rows, int32_t cols, int32_t out_features, int32_t gate);
+
 #ifdef __cplusplus
 }
 #endif
