@@ -424,6 +424,13 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t v, uint32_t* s_red) 
   return v;
 }
 
+// v as an fp32 number: without it the compiler takes a product and its conversion to fp16 in one instruction, which rounds
+// the exact product once, and what one kernel takes so another rounds twice.
+__device__ __forceinline__ float as_f32(float v) {
+  asm("" : "+v"(v));
+  return v;
+}
+
 // VEC bytes, values as quantize_chunk leaves them.
 template <int VEC>
 __device__ __forceinline__ void store_bytes(int8_t* dst, const uint32_t* b) {

@@ -168,7 +168,7 @@ __device__ __forceinline__ void emit(const Linear8Params& p, int64_t m, int n, i
 #pragma unroll
   for (int i = 0; i < C; ++i) {
     v[i] = a.apply(i, t[i], sm);
-    if constexpr (GATE != CTI_EBAG_GATE_NONE) v[i] = activate<GATE>(v[i]) * b.apply(i, u[i], sm);
+    if constexpr (GATE != CTI_EBAG_GATE_NONE) v[i] = as_f32(activate<GATE>(v[i]) * b.apply(i, u[i], sm));
   }
   store_columns<YT, C>(p.y, m * p.N + n, v, live);
 }

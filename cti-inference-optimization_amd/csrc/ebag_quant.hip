@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_rows_kernel(const in
           ++row;
           left = dim;
         }
-        store_one(dst + e, static_cast<float>(q[e0 + e]) * scale[row], false);
+        store_one(dst + e, as_f32(static_cast<float>(q[e0 + e]) * scale[row]), false);
       }
       return;
     }
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_rows_kernel(const in
     }
     if (left >= C) {
 #pragma unroll
-      for (int e = 0; e < C; ++e) v[e] *= s;
+      for (int e = 0; e < C; ++e) v[e] = as_f32(v[e] * s);
     } else {
 #pragma unroll
       for (int e = 0; e < C; ++e, --left) {
@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_rows_kernel(const in
           s = scale[++row];
           left = dim;
         }
-        v[e] *= s;
+        v[e] = as_f32(v[e] * s);
       }
     }
     with_stream(stream_out, [&](auto stream) { store_out<C>(dst, v, decltype(stream)::value); });

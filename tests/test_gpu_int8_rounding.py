@@ -52,3 +52,24 @@ def test_norms_round_quotients(pkg, dev, rows, cols, dt):
         assert (scale.cpu().numpy() == s).all()
         off = got.cpu() != want_q
         assert not off.any(), (layer, int(off.sum()))
+
+
+def test_read_back_is_rounded_to_fp32_and_then_to_fp16(pkg, dev):
+    """Scales of which q * scale in fp32 is the middle of two fp16 numbers while the product itself is not: the last
+    elements of an array, which are taken one by one, as well as whole vectors."""
+    rng = np.random.default_rng(0)
+    q = rng.integers(1, 128, 4_000_000).astype(np.int8)
+    s = rng.uniform(0.001, 1, q.size).astype(np.float32)
+    exact = q.astype(np.float64) * s  # 8 and 24 bits: exact
+    twice = (q * s).astype(np.float32).astype(np.float16)
+    at = np.flatnonzero(twice != exact.astype(np.float16))[:200]
+    assert len(at) > 50
+    q, s, twice = (torch.from_numpy(a[at]).to(dev) for a in (q, s, twice))
+    for n in (1, 3, 8, 11, 16, len(at)):
+        print(f"read back {n}", flush=True)
+        for lo in range(0, len(at) - n + 1, n):
+            got = pkg.dequantize_embedding_int8(q[lo:lo + n].view(n, 1), s[lo:lo + n], torch.float16)
+            assert torch.equal(got[:, 0], twice[lo:lo + n]), (n, lo)
+    # rows of 5 such elements of one scale each
+    wide = q[:, None].expand(-1, 5).contiguous()
+    assert torch.equal(pkg.dequantize_embedding_int8(wide, s, torch.float16), twice[:, None].expand(-1, 5))
