@@ -22,6 +22,7 @@
 
 #include "ebag_device.h"
 #include "ebag_internal.h"
+#include "ebag_rules.h"
 
 namespace cti {
 namespace {
@@ -396,17 +397,15 @@ __global__ void __launch_bounds__(kLoopThreads) norm8_loop_kernel(const Norm8Par
   }
 }
 
-// Wavefronts per row: the time of a row alone counts while rows are few, and a wavefront with 8 vectors per lane leaves too
-// little else on its SIMD (16,384 rows of 4,096 bf16 with a residual: 82 us with 4 wavefronts of 2 vectors per lane,
-// 88 with 4 of 4, 101 with one of 8; one row: 4.4 us with 8 of 1, 5.2 with 4 of 2, 9.3 with one of 8).
 template <typename T, typename PT>
 hipError_t launch_norm8_rows(const Norm8Params& p, int64_t rows, hipStream_t s) {
   constexpr int VEC = 16 / Elem<T>::kBytes;
-  const int64_t nvec = (p.cols + VEC - 1) / VEC;
+  const Norm8Form form = norm8_form(rows, p.cols, VEC);
   const dim3 grid(static_cast<unsigned>(rows));
-  const auto go = [&](auto k, auto waves) {
+  const auto rows_form = [&](auto k, auto waves) {
     constexpr int K = decltype(k)::value, W = decltype(waves)::value;
-    hipLaunchKernelGGL((norm8_rows_kernel<T, PT, K, W>), grid, dim3(W * kWave), 0, s, p);
+    if (form.vectors == K && form.waves == W)
+      hipLaunchKernelGGL((norm8_rows_kernel<T, PT, K, W>), grid, dim3(W * kWave), 0, s, p);
   };
   using std::integral_constant;
   constexpr integral_constant<int, 1> n1{};
@@ -414,31 +413,24 @@ hipError_t launch_norm8_rows(const Norm8Params& p, int64_t rows, hipStream_t s) 
   constexpr integral_constant<int, 4> n4{};
   constexpr integral_constant<int, 8> n8{};
   constexpr integral_constant<int, 16> n16{};
-  const bool few = rows < 1536;  // too few to fill the card with 8 wavefronts each
-  if (p.cols < VEC || nvec > 64 * kWave) {
+  if (form.vectors == 0) {
     hipLaunchKernelGGL((norm8_loop_kernel<T, PT>), grid, dim3(kLoopThreads), 0, s, p);
-  } else if (nvec <= kWave / 2) {
+  } else if (form.waves == 0) {
     int lg = 0;
-    while ((1 << lg) < nvec) ++lg;
+    while ((VEC << lg) < p.cols) ++lg;
     const int64_t per = static_cast<int64_t>(kNarrowWaves) << (6 - lg);
     hipLaunchKernelGGL((norm8_narrow_kernel<T, PT>), dim3(static_cast<unsigned>((rows + per - 1) / per)),
                        dim3(kNarrowWaves * kWave), 0, s, p, rows, lg);
-  } else if (nvec <= kWave) {
-    go(n1, n1);
-  } else if (nvec <= 2 * kWave) {
-    go(n1, n2);
-  } else if (nvec <= 4 * kWave) {
-    go(n1, n4);
-  } else if (nvec <= 8 * kWave) {
-    if (few) go(n1, n8);
-    else go(n2, n4);
-  } else if (nvec <= 16 * kWave) {
-    go(n2, n8);
-  } else if (nvec <= 32 * kWave) {
-    if (few) go(n2, n16);
-    else go(n4, n8);
   } else {
-    go(n4, n16);
+    rows_form(n1, n1);
+    rows_form(n1, n2);
+    rows_form(n1, n4);
+    rows_form(n1, n8);
+    rows_form(n2, n4);
+    rows_form(n2, n8);
+    rows_form(n2, n16);
+    rows_form(n4, n8);
+    rows_form(n4, n16);
   }
   return hipGetLastError();
 }

@@ -386,4 +386,29 @@ inline int64_t linear8_workspace_bytes(int64_t M, int32_t N, int32_t K, bool gat
   return rest > whole ? rest : whole;
 }
 
+// ---------------------------------------------------------------------------------------------
+// int8 norms
+// ---------------------------------------------------------------------------------------------
+// A row in the registers of `waves` wavefronts, `vectors` of 16 bytes (`vec` elements) a lane; waves 0: in a group of lanes
+// of one wavefront, a vector each; vectors 0: rows of less than a vector or more than the registers hold, in a loop.
+// The time of a row alone counts while rows are few, and a wavefront with 8 vectors per lane leaves too little else on its
+// SIMD (16,384 rows of 4,096 bf16 with a residual: 82 us with 4 wavefronts of 2 vectors per lane, 88 with 4 of 4, 101 with
+// one of 8; one row: 4.4 us with 8 of 1, 5.2 with 4 of 2, 9.3 with one of 8).
+struct Norm8Form {
+  int vectors, waves;
+};
+inline Norm8Form norm8_form(int64_t rows, int64_t cols, int vec) {
+  const int64_t n = linear_ceil(cols, vec);  // vectors of a row
+  const bool few = rows < 1536;              // too few to fill the card with 8 wavefronts each
+  if (cols < vec || n > 4096) return {0, 0};
+  if (n <= 32) return {1, 0};
+  if (n <= 64) return {1, 1};
+  if (n <= 128) return {1, 2};
+  if (n <= 256) return {1, 4};
+  if (n <= 512) return few ? Norm8Form{1, 8} : Norm8Form{2, 4};
+  if (n <= 1024) return {2, 8};
+  if (n <= 2048) return few ? Norm8Form{2, 16} : Norm8Form{4, 8};
+  return {4, 16};
+}
+
 }  // namespace cti
