@@ -410,8 +410,10 @@ extern "C" int cti_ebag_dequantize_int8(const int8_t* q, const float* scale, int
   if (dim < 1) return set_error(CTI_EBAG_EINVAL, "dim must be >= 1 (got %lld)", (long long)dim);
   if (rows == 0) return CTI_EBAG_OK;
   if (!q || !scale || !out) return set_error(CTI_EBAG_EINVAL, "NULL device pointer among q/scale/out");
-  if (rows > (int64_t{1} << 40) / dim)
-    return set_error(CTI_EBAG_EUNSUPPORTED, "more than 2^40 elements (%lld x %lld)", (long long)rows, (long long)dim);
+  // a launch has fewer than 2^32 threads
+  const int64_t most = UINT32_MAX / kQuantThreads * (int64_t{kQuantThreads} * kDequantChunks * 16 / dtype_bytes(out_dtype));
+  if (rows > most / dim)
+    return set_error(CTI_EBAG_EUNSUPPORTED, "more than %lld elements (%lld x %lld)", (long long)most, (long long)rows, (long long)dim);
   if (reinterpret_cast<uintptr_t>(out) % dtype_bytes(out_dtype) != 0)
     return set_error(CTI_EBAG_EINVAL, "out is not aligned to its elements");
   hipStream_t s = static_cast<hipStream_t>(stream);

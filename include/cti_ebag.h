@@ -476,7 +476,7 @@ int64_t cti_ebag_layernorm_linear_workspace_bytes(int64_t rows, int32_t cols, in
 /*
  * The way back from cti_ebag_quantize_int8 and cti_ebag_norm_int8: out[r, j] = q[r, j] * scale[r] in fp32,
  * rounded once to `out_dtype` (F32 / BF16 / F16). q int8 [rows, dim] and out [rows, dim] contiguous, scale
- * fp32 [rows]; at most 2^40 elements.
+ * fp32 [rows]; at most 2^36 - 4096 elements to F32 and 2^37 - 8192 to the others.
  */
 int cti_ebag_dequantize_int8(const int8_t* q, const float* scale, int64_t rows, int64_t dim, void* out,
                              int32_t out_dtype, void* stream);

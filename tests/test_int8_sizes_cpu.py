@@ -81,3 +81,12 @@ def test_unaligned_workspaces(pkg, cols):
                 assert (a == b) if cols % 16 else a >= 0 and b >= 0
                 if not 1 <= rows < 2 ** 31 or not 1 <= n < 2 ** 30 or gate == 4:
                     assert a == b == 0
+
+
+@pytest.mark.parametrize("dtype,most", [("F32", 2 ** 36 - 4096), ("BF16", 2 ** 37 - 8192), ("F16", 2 ** 37 - 8192)])
+def test_read_back_of_more_elements_than_a_launch_has(pkg, dtype, most):
+    """256 threads a workgroup of 1,024 chunks of 16 bytes of output, and fewer than 2^32 threads: refused before a launch."""
+    c = pkg._capi
+    for rows, dim in ((most + 1, 1), (most // 4096 + 1, 4096), (2 ** 39, 2), (1, 2 ** 62), (2 ** 62, 3)):
+        status = c.lib().cti_ebag_dequantize_int8(256, 256, rows, dim, 256, getattr(c, dtype), None)
+        assert status == c.EUNSUPPORTED and "elements" in c.last_error(), (rows, dim)
