@@ -297,7 +297,8 @@ inline double linear8_time(const Linear8Part& part, int64_t M, int32_t K, bool g
 }
 
 // What the host needs for a call, and for each launch beyond the first: a plan that is faster than that on the GPU
-// gains nothing.
+// gains nothing where calls follow each other (where a graph is replayed it would: 1 x 9856 -> 80 by the plan of fewest launches
+// is estimated at 11.0 us, 5.4 by the fastest).
 constexpr double kLinear8Host = 7.5, kLinear8HostLaunch = 3.5;
 
 // The best single part for columns n_begin .. n_end: its form and splits (at most as many as ws_bytes hold partial
