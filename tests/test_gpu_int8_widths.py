@@ -23,3 +23,20 @@ def test_quantiser_at_the_edges_of_its_forms(pkg, dev, vectors, dt):
             view.copy_(x)
             q, s = pkg.quantize_embedding_int8(view)
             assert torch.equal(s.cpu(), want_s) and torch.equal(q.cpu(), want_q)
+
+
+def test_more_rows_than_a_launch_of_four_wavefronts_has(pkg, dev):
+    """256 threads a row from 129 vectors on: 2^24 rows are 2^32 threads, which no launch has."""
+    rows, dim = 2 ** 24 + 5, 1032
+    w = torch.zeros(rows, dim, dtype=torch.bfloat16, device=dev)
+    at = torch.tensor([0, 2 ** 24 - 2, 2 ** 24 - 1, 2 ** 24, rows - 1], device=dev)
+    some = torch.randn(len(at), dim, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).to(dev)
+    w[at] = some
+    print("more rows than a launch of four wavefronts has", flush=True)
+    for nan_rows in (False, True):
+        q, s = pkg.quantize_embedding_int8(w, nan_rows=nan_rows)
+        torch.cuda.synchronize()
+        want_q, want_s = pkg.quantize_embedding_int8(some)
+        assert torch.equal(q[at], want_q) and torch.equal(s[at], want_s)
+        assert int((s != np.float32(1e-8)).sum()) == len(at)
+        del q
