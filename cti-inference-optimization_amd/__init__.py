@@ -16,6 +16,12 @@ Public surface:
   rms_norm_int8, layer_norm_int8   residual addition, norm and int8 rows with scales in one pass
   linear_int8                Linear in 8-bit integers, a scale for each token and each channel
   gated_linear_int8          both projections of a gated feed-forward block and their product
+  embedding_lookup           rows of a table, scaled, and the table's gradient by sorted ids
+  embedding_lookup_backward, embedding_bag_backward, fused_all_slots_embedding_backward
+                             gradients of tables behind lookups and pooled bags: whole, or the rows that occur
+  embedding_bag_train, fused_embedding_train   the pooled step, differentiable in its tables
+  dropout, dropout_backward  dropout from a counter-based generator, its mask never stored
+  dropout_add_layer_norm, dropout_add_layer_norm_backward   dropout, residual addition and LayerNorm in one pass
   RepEncoder                 the reference module with the fused step and LayerNorm on this path
   collate_flat_layout, prebuild_flat_layout   host builders of the flat layout
   pack_slots, merge_batches                   GPU builders of the flat layout
@@ -32,6 +38,9 @@ from .ops import (PooledEmbedding, dequantize_embedding_int8, embedding_bag_pool
                   fused_all_slots_embedding_int8_layernorm, fused_all_slots_embedding_layernorm, fused_embedding, gated_linear_int8,
                   layer_norm, layer_norm_int8, layer_norm_linear, layer_norm_stats, linear_int8, make_tile_order,
                   order_bytes, quantize_embedding_int8, rms_norm_int8)
+from .training import (dropout, dropout_add_layer_norm, dropout_add_layer_norm_backward, dropout_backward, embedding_bag_backward,
+                       embedding_bag_train, embedding_lookup, embedding_lookup_backward, fused_all_slots_embedding_backward,
+                       fused_embedding_train)
 
 __all__ = [
     "EbagError",
@@ -59,6 +68,16 @@ __all__ = [
     "layer_norm",
     "layer_norm_stats",
     "layer_norm_linear",
+    "embedding_lookup",
+    "embedding_lookup_backward",
+    "embedding_bag_backward",
+    "embedding_bag_train",
+    "fused_all_slots_embedding_backward",
+    "fused_embedding_train",
+    "dropout",
+    "dropout_backward",
+    "dropout_add_layer_norm",
+    "dropout_add_layer_norm_backward",
     "make_tile_order",
     "order_bytes",
     "workloads",

@@ -155,6 +155,35 @@ SIGNATURES = {
         ctypes.c_int,
         [_P, _I32, _P, _P, _I32, _P, _I32, _P, _P, _I32, _I64, _I32, _I32, _I64, _I64, _P],
     ),
+    "cti_ebag_lookup": (ctypes.c_int, [_P, _I32, _I64, _P, _I32, _I64, _I64, _I32, ctypes.c_float, _P, _I32, _P]),
+    "cti_ebag_lookup_backward": (
+        ctypes.c_int,
+        [_P, _I32, _P, _I32, _I64, _I64, _I32, ctypes.c_float, _I64, _P, _I32, _P, _P, _I64, _P, _I64, _P],
+    ),
+    "cti_ebag_fused_all_slots_backward": (
+        ctypes.c_int,
+        [_P, _I32, _P, _I32, _P, _P, _I32, _I64, _I32, _I32, _I64, _I64, _I32, _I64, _P, _I32, _P, _P, _I64, _P, _I64, _P],
+    ),
+    "cti_ebag_backward": (
+        ctypes.c_int,
+        [_P, _I32, _I64, _P, _I32, _I64, _P, _I64, _I32, ctypes.POINTER(Table), _I32, _I64, _I32, _P, _P, _P, _I64, _P, _I64, _P],
+    ),
+    "cti_ebag_backward_workspace_bytes": (ctypes.c_int64, [_I64, _I64, _I64, _I32, _I32]),
+    "cti_ebag_dropout": (
+        ctypes.c_int,
+        [_P, _P, _P, _I64, _I64, _I32, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, _P, _P],
+    ),
+    "cti_ebag_dropout_layernorm": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _I64, _I64, _I32, _P, _P, _I32, ctypes.c_float, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, _P,
+         _P, _P, _P],
+    ),
+    "cti_ebag_dropout_layernorm_backward": (
+        ctypes.c_int,
+        [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _I32, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, _P, _P, _P, _P, _P,
+         _P, _I64, _P],
+    ),
+    "cti_ebag_dropout_layernorm_backward_workspace_bytes": (ctypes.c_int64, [_I64, _I64]),
 }
 
 _lib = None

@@ -1,0 +1,1261 @@
+// Embedding lookup with a scale, and the gradients of tables behind lookups and pooled bags, for MI355X
+// (gfx950).
+//
+//   lookup:    out[i] = scale * W[clamp(id_i)]                    fp32, one rounding
+//   gradient:  dW[v] = scale * sum_{i: clamp(id_i) = v} w_i g[u_i]
+// u_i is the gradient's row that id i contributed to (the id's own position, or its bag), w_i is 1 or, under
+// mean pooling, 1 / length of the bag. No contribution is added by an atomic: the ids are sorted (stably, so
+// in order of position), and each table row's contributions are added in fp32 in an order that the sizes
+// alone fix, rounded once. Rows are the same bits in every run.
+//
+// 1. Keys: (table's first row number + clamped id, u) for each id; ids of the padding row and ids in no bag
+//    get the key `total`, which sorts last and is dropped. Bags are found from their starts in the tile.
+// 2. A radix sort by digits of at most 8 bits, least significant first, in tiles of 4,096: counts of every
+//    tile, then ranks within the tile (one ballot a bit finds the lanes of a wavefront that hold the same
+//    digit), the tile put in order in LDS and written out in runs. Every tile adds up the counts of the
+//    others itself where they are few (no further launch), else a scan kernel does. A single tile is sorted
+//    in LDS, all digits in one launch.
+// 3. Sums: a workgroup takes a run of the sorted list, lane groups that cover a row's columns walk shares of
+//    it, several rows' loads in flight, and write a table row where its key ends inside the share. What
+//    crosses shares is added in LDS, what crosses workgroups goes to the workspace as fp32 rows, at most two
+//    a workgroup, and a second kernel adds these up.
+#include <stdint.h>
+
+#include "ebag_train.h"
+
+namespace cti {
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// Lookup
+// ---------------------------------------------------------------------------------------------
+constexpr int kLookupThreads = 256;
+
+struct LookupParams {
+  const void* ids;
+  const char* weight;
+  char* out;
+  int64_t rows;
+  int64_t row_bytes;  // between rows of the table
+  int32_t dim;
+  int32_t ids64;
+  uint32_t chunks;    // of this launch
+  uint32_t per_row;   // chunks of 8 columns a row
+  ChunkDivide div;
+  float scale;
+  int32_t stream_out;
+};
+
+// An id of either type, clamped to a table's rows.
+__device__ __forceinline__ int64_t load_id(const void* ids, int32_t ids64, int64_t i, int64_t rows) {
+  const int64_t id = ids64 ? static_cast<const int64_t*>(ids)[i] : static_cast<int64_t>(static_cast<const int32_t*>(ids)[i]);
+  return clamp_i64(id, 0, rows - 1);
+}
+
+// A thread takes 8 columns of a row. Bound by HBM where the rows are many, by the latency of an id's load
+// and a row's behind it where they are few.
+template <typename T, typename OT>
+__global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupParams p) {
+  const uint32_t c = blockIdx.x * kLookupThreads + threadIdx.x;
+  if (c >= p.chunks) return;
+  const uint32_t i = p.div.quotient(c);
+  const int col = static_cast<int>(c - i * p.per_row) * 8;
+  const int64_t id = load_id(p.ids, p.ids64, i, p.rows);
+  float v[8];
+  const int live = p.dim - col;
+  load8<T>(p.weight + id * p.row_bytes + static_cast<int64_t>(col) * Elem<T>::kBytes, live, v);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= p.scale;
+  with_stream(p.stream_out, [&](auto stream) {
+    store8<OT, decltype(stream)::value>(p.out + (static_cast<int64_t>(i) * p.dim + col) * Elem<OT>::kBytes, live, v);
+  });
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradient: keys
+// ---------------------------------------------------------------------------------------------
+constexpr int kTile = kGradTile;  // keys a workgroup sorts
+constexpr int kSortThreads = 512;
+constexpr int kSortWaves = kSortThreads / kWave;
+constexpr int kItems = kTile / kSortThreads;  // keys a thread
+constexpr int kDigits = 256;
+constexpr int kMaxFields = 64;
+
+// Where the ids' bags and tables are.
+struct GradSource {
+  const void* ids;
+  const void* val_offsets;  // reference layout: first id of each slot; NULL: global offsets
+  const void* offsets;      // row offsets [F * (B + 1)], or global [F * B + 1]; NULL: a lookup, u_i = i
+  float* inv_len;           // mean pooling: 1 / length of bag u is written here; NULL: sum
+  int64_t n;
+  int64_t batch;
+  int64_t bags;             // F * B
+  int32_t fields;
+  int32_t ids64;
+  int32_t offs64;
+  int32_t per_field;        // base / rows below hold for each field; else base 0 and rows[0] for all
+  uint32_t total;           // rows of all tables: the key of what is dropped
+  ChunkDivide by_batch;
+  int64_t padding;          // -1: none
+  uint32_t base[kMaxFields];
+  uint32_t rows[kMaxFields];
+};
+
+__device__ __forceinline__ int64_t load_off(const void* p, int32_t is64, int64_t i) {
+  return is64 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
+}
+
+// First id of bag j = f * B + b, clipped to [0, n]; bag j's end is that of the next offset.
+__device__ __forceinline__ int64_t bag_edge(const GradSource& s, int64_t j, int end) {
+  int64_t v;
+  if (s.val_offsets) {
+    const int64_t f = s.by_batch.quotient(static_cast<uint32_t>(j));
+    v = load_off(s.val_offsets, s.offs64, f) + load_off(s.offsets, s.offs64, j + f + end);
+  } else {
+    v = load_off(s.offsets, s.offs64, j + end);
+  }
+  return clamp_i64(v, 0, s.n);
+}
+
+// How many bags start at or before p (the bags start in order): a search of 64 places a step. Called by a
+// whole wavefront, p uniform.
+__device__ __forceinline__ int64_t bags_started(const GradSource& s, int64_t p) {
+  int64_t lo = 0, hi = s.bags;  // the answer lies in [lo, hi]
+  while (lo < hi) {
+    const int64_t step = (hi - lo + kWave - 1) / kWave;
+    const int64_t j = lo + step * (lane_id() + 1) - 1;  // lane's last bag of its share
+    const bool started = j < hi && bag_edge(s, j, 0) <= p;
+    const int k = __popcll(__ballot(started));
+    lo += step * k;
+    const int64_t top = lo + step - 1;  // this bag has not started, or is past the end
+    if (top < hi) hi = top;
+  }
+  return lo;
+}
+
+// The key of id i of field f.
+__device__ __forceinline__ uint32_t grad_key(const GradSource& s, int64_t i, int f) {
+  const uint32_t at = s.per_field ? f : 0;
+  const int64_t id = load_id(s.ids, s.ids64, i, s.rows[at]);
+  return id == s.padding ? s.total : s.base[at] + static_cast<uint32_t>(id);
+}
+
+constexpr int kMostBags = 4 * kTile;  // bags whose starts a tile looks through; with more, each id searches
+
+// Keys and u of the tile's ids: item k of a thread is id tile * kTile + item_index(k). s_bag: kTile words.
+__device__ __forceinline__ int item_index(int k) {
+  return (static_cast<int>(threadIdx.x) / kWave) * (kItems * kWave) + k * kWave + lane_id();
+}
+
+__device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uint32_t* key, uint32_t* unit, int32_t* s_bag,
+                                          int64_t* s_range) {
+  const int64_t first = tile * kTile;
+  if (!s.offsets) {
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int64_t i = first + item_index(k);
+      key[k] = i < s.n ? grad_key(s, i, 0) : 0xffffffffu;
+      unit[k] = static_cast<uint32_t>(i);
+    }
+    return;
+  }
+  const int t = static_cast<int>(threadIdx.x);
+  const int64_t last = first + kTile < s.n ? first + kTile : s.n;
+  if (t < 2 * kWave) {
+    const int64_t r = bags_started(s, t < kWave ? first : last - 1);
+    if (lane_id() == 0) s_range[t / kWave] = r;
+  }
+  for (int i = t; i < kTile; i += kSortThreads) s_bag[i] = 0;
+  __syncthreads();
+  // bags [lo, hi) start in the tile after its first id; bag lo - 1 (or none) holds the first one
+  const int64_t lo = s_range[0], hi = s_range[1];
+  const bool scan = hi - lo <= kMostBags;
+  if (scan) {
+    // s_bag[p] = 1 + the last of them that starts at p, relative to lo; then the largest up to each place
+    for (int64_t j = lo + t; j < hi; j += kSortThreads) {
+      const int64_t at = bag_edge(s, j, 0) - first;
+      if (at >= 0 && at < kTile) atomicMax(&s_bag[at], static_cast<int32_t>(j - lo) + 1);
+    }
+    __syncthreads();
+    constexpr int kRun = kTile / kSortThreads;
+    int32_t m[kRun], top = 0;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      const int32_t b = s_bag[t * kRun + k];
+      top = b > top ? b : top;
+      m[k] = top;
+    }
+    int32_t before = top;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const int32_t o = shfl_i32(before, lane_id() - d);
+      if (lane_id() >= d) before = o > before ? o : before;
+    }
+    __shared__ int32_t s_top[kSortWaves];
+    if (lane_id() == kWave - 1) s_top[t / kWave] = before;
+    int32_t carry = shfl_i32(before, lane_id() - 1);
+    if (lane_id() == 0) carry = 0;
+    __syncthreads();
+    for (int w = 0; w < t / kWave; ++w) carry = s_top[w] > carry ? s_top[w] : carry;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) s_bag[t * kRun + k] = m[k] > carry ? m[k] : carry;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = first + item_index(k);
+    key[k] = 0xffffffffu;
+    unit[k] = 0u;
+    if (i >= s.n) continue;
+    int64_t j;
+    if (scan) {
+      j = lo - 1 + s_bag[item_index(k)];
+    } else {
+      int64_t a = lo, b = hi;  // bags started at or before i
+      while (a < b) {
+        const int64_t mid = (a + b) / 2;
+        if (bag_edge(s, mid, 0) <= i) a = mid + 1;
+        else b = mid;
+      }
+      j = a - 1;
+    }
+    key[k] = s.total;
+    if (j < 0 || j >= s.bags || i >= bag_edge(s, j, 1)) continue;  // in no bag
+    const int64_t f = s.by_batch.quotient(static_cast<uint32_t>(j));
+    key[k] = grad_key(s, i, static_cast<int>(f));
+    unit[k] = static_cast<uint32_t>((j - f * s.batch) * s.fields + f);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradient: sort
+// ---------------------------------------------------------------------------------------------
+struct SortBuffers {
+  uint32_t* key;
+  uint32_t* unit;
+};
+
+// Exclusive sums over the first kDigits threads' values (the others pass 0); s_scan: kSortWaves words.
+__device__ __forceinline__ uint32_t digit_scan(uint32_t v, uint32_t* s_scan) {
+  const int t = static_cast<int>(threadIdx.x);
+  uint32_t x = v;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const uint32_t o = static_cast<uint32_t>(shfl_i32(static_cast<int>(x), lane_id() - d));
+    if (lane_id() >= d) x += o;
+  }
+  __syncthreads();
+  if (lane_id() == kWave - 1) s_scan[t / kWave] = x;
+  __syncthreads();
+  uint32_t before = 0;
+#pragma unroll
+  for (int w = 0; w < kDigits / kWave; ++w) before += w < t / kWave ? s_scan[w] : 0u;
+  return before + x - v;
+}
+
+// Places of the tile's keys in the tile sorted by one digit (stable): place[k] of item k. s_start[d] is the
+// first place of digit d.
+__device__ __forceinline__ void tile_places(const uint32_t* key, int shift, int bits, uint32_t* place, uint32_t* s_hist,
+                                            uint32_t* s_start, uint32_t* s_scan) {
+  const int t = static_cast<int>(threadIdx.x), w = t / kWave;
+  const uint32_t mask = (1u << bits) - 1u;
+  for (int i = t; i < kSortWaves * kDigits; i += kSortThreads) s_hist[i] = 0u;
+  __syncthreads();
+  volatile uint32_t* const mine = s_hist + w * kDigits;
+  const uint64_t below = (uint64_t{1} << lane_id()) - 1;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const uint32_t d = (key[k] >> shift) & mask;
+    uint64_t same = ~uint64_t{0};
+    for (int b = 0; b < bits; ++b) {
+      const bool one = (d >> b) & 1u;
+      const uint64_t ones = __ballot(one);
+      same &= one ? ones : ~ones;
+    }
+    const uint32_t seen = mine[d];
+    const uint32_t rank = static_cast<uint32_t>(__popcll(same & below));
+    place[k] = seen + rank;
+    __builtin_amdgcn_wave_barrier();
+    if (rank == 0) mine[d] = seen + static_cast<uint32_t>(__popcll(same));
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  uint32_t sum = 0;
+  if (t < kDigits) {
+#pragma unroll
+    for (int i = 0; i < kSortWaves; ++i) {
+      const uint32_t c = s_hist[i * kDigits + t];
+      s_hist[i * kDigits + t] = sum;
+      sum += c;
+    }
+  }
+  const uint32_t start = digit_scan(sum, s_scan);
+  if (t < kDigits) s_start[t] = start;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const uint32_t d = (key[k] >> shift) & mask;
+    place[k] += s_start[d] + s_hist[w * kDigits + d];
+  }
+}
+
+// All ids in one tile: keys and every digit in one launch.
+__global__ void __launch_bounds__(kSortThreads) grad_sort_tile_kernel(const GradSource s, SortBuffers out, int bits) {
+  __shared__ uint32_t s_key[kTile], s_unit[kTile];
+  __shared__ uint32_t s_hist[kSortWaves * kDigits], s_start[kDigits], s_scan[kSortWaves];
+  __shared__ int64_t s_range[2];
+  uint32_t key[kItems], unit[kItems], place[kItems];
+  tile_keys(s, 0, key, unit, reinterpret_cast<int32_t*>(s_key), s_range);
+  for (int shift = 0; shift < bits; shift += 8) {
+    const int now = bits - shift < 8 ? bits - shift : 8;
+    tile_places(key, shift, now, place, s_hist, s_start, s_scan);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      s_key[place[k]] = key[k];
+      s_unit[place[k]] = unit[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      key[k] = s_key[item_index(k)];
+      unit[k] = s_unit[item_index(k)];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int i = item_index(k);
+    if (i < s.n) {
+      out.key[i] = key[k];
+      out.unit[i] = unit[k];
+    }
+  }
+}
+
+__device__ __forceinline__ void tile_count(const uint32_t* key, int64_t live, int shift, int bits, uint32_t* counts,
+                                           uint32_t* s_hist) {
+  const int t = static_cast<int>(threadIdx.x);
+  const uint32_t mask = (1u << bits) - 1u;
+  __syncthreads();
+  for (int i = t; i < kDigits; i += kSortThreads) s_hist[i] = 0u;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kItems; ++k)
+    if (item_index(k) < live) atomicAdd(&s_hist[(key[k] >> shift) & mask], 1u);
+  __syncthreads();
+  for (int i = t; i < kDigits; i += kSortThreads) counts[i] = s_hist[i];
+}
+
+// Keys of every tile and the counts of their first digit.
+__global__ void __launch_bounds__(kSortThreads) grad_keys_kernel(const GradSource s, SortBuffers out, uint32_t* counts, int bits) {
+  __shared__ int32_t s_bag[kTile];
+  __shared__ uint32_t s_hist[kDigits];
+  __shared__ int64_t s_range[2];
+  uint32_t key[kItems], unit[kItems];
+  tile_keys(s, blockIdx.x, key, unit, s_bag, s_range);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kTile;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = first + item_index(k);
+    if (i < s.n) {
+      out.key[i] = key[k];
+      out.unit[i] = unit[k];
+    }
+  }
+  tile_count(key, s.n - first, 0, bits, counts + static_cast<int64_t>(blockIdx.x) * kDigits, s_hist);
+}
+
+__global__ void __launch_bounds__(kSortThreads) grad_count_kernel(const uint32_t* keys, int64_t n, int shift, int bits,
+                                                                  uint32_t* counts) {
+  __shared__ uint32_t s_hist[kDigits];
+  uint32_t key[kItems];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kTile;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = first + item_index(k);
+    key[k] = i < n ? keys[i] : 0u;
+  }
+  tile_count(key, n - first, shift, bits, counts + static_cast<int64_t>(blockIdx.x) * kDigits, s_hist);
+}
+
+// counts[tile][digit] -> how many of the digit lie in tiles before it; totals[digit]. A workgroup takes four
+// digits, a thread a run of tiles.
+constexpr int kScanThreads = 256;
+__global__ void __launch_bounds__(kScanThreads) grad_scan_kernel(uint32_t* counts, uint32_t* totals, int64_t tiles) {
+  __shared__ uint4 s_sum[kScanThreads];
+  const int t = static_cast<int>(threadIdx.x);
+  const int64_t per = (tiles + kScanThreads - 1) / kScanThreads;
+  const int64_t a = per * t < tiles ? per * t : tiles, b = a + per < tiles ? a + per : tiles;
+  uint4* const col = reinterpret_cast<uint4*>(counts) + blockIdx.x;
+  uint4 sum = make_uint4(0u, 0u, 0u, 0u);
+  for (int64_t i = a; i < b; ++i) {
+    const uint4 c = col[i * (kDigits / 4)];
+    sum.x += c.x, sum.y += c.y, sum.z += c.z, sum.w += c.w;
+  }
+  s_sum[t] = sum;
+  __syncthreads();
+  uint4 before = make_uint4(0u, 0u, 0u, 0u);
+  for (int i = 0; i < kScanThreads; ++i) {
+    if (i == t) sum = before;
+    const uint4 c = s_sum[i];
+    before.x += c.x, before.y += c.y, before.z += c.z, before.w += c.w;
+  }
+  if (t == 0) reinterpret_cast<uint4*>(totals)[blockIdx.x] = before;
+  for (int64_t i = a; i < b; ++i) {
+    const uint4 c = col[i * (kDigits / 4)];
+    col[i * (kDigits / 4)] = sum;
+    sum.x += c.x, sum.y += c.y, sum.z += c.z, sum.w += c.w;
+  }
+}
+
+// One digit: the tile in order, written to its places. totals NULL: counts are the tiles' own.
+__global__ void __launch_bounds__(kSortThreads) grad_scatter_kernel(SortBuffers in, SortBuffers out, int64_t n, int shift, int bits,
+                                                                    const uint32_t* counts, const uint32_t* totals, int tiles) {
+  __shared__ uint32_t s_key[kTile], s_unit[kTile];
+  __shared__ uint32_t s_hist[kSortWaves * kDigits], s_start[kDigits], s_scan[kSortWaves], s_base[kDigits];
+  const int t = static_cast<int>(threadIdx.x), tile = static_cast<int>(blockIdx.x);
+  const int64_t first = static_cast<int64_t>(tile) * kTile;
+  uint32_t key[kItems], unit[kItems], place[kItems];
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = first + item_index(k);
+    key[k] = i < n ? in.key[i] : 0xffffffffu;
+    unit[k] = i < n ? in.unit[i] : 0u;
+  }
+  uint32_t before = 0, total = 0;
+  if (totals) {
+    if (t < kDigits) {
+      before = counts[static_cast<int64_t>(tile) * kDigits + t];
+      total = totals[t];
+    }
+  } else {
+    // a wavefront adds up every kSortWaves-th tile, a lane four digits
+    const uint4* const c4 = reinterpret_cast<const uint4*>(counts);
+    uint4 b4 = make_uint4(0u, 0u, 0u, 0u), t4 = b4;
+#pragma unroll 8
+    for (int i = t / kWave; i < tiles; i += kSortWaves) {
+      const uint4 c = c4[i * (kDigits / 4) + lane_id()];
+      t4.x += c.x, t4.y += c.y, t4.z += c.z, t4.w += c.w;
+      if (i < tile) b4.x += c.x, b4.y += c.y, b4.z += c.z, b4.w += c.w;
+    }
+    reinterpret_cast<uint4*>(s_key)[t] = b4;  // [wavefront][digit]
+    reinterpret_cast<uint4*>(s_unit)[t] = t4;
+    __syncthreads();
+    if (t < kDigits) {
+#pragma unroll
+      for (int w = 0; w < kSortWaves; ++w) {
+        before += s_key[w * kDigits + t];
+        total += s_unit[w * kDigits + t];
+      }
+    }
+  }
+  const uint32_t digits_before = digit_scan(total, s_scan);
+  if (t < kDigits) s_base[t] = digits_before + before;
+  tile_places(key, shift, bits, place, s_hist, s_start, s_scan);
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    s_key[place[k]] = key[k];
+    s_unit[place[k]] = unit[k];
+  }
+  __syncthreads();
+  const uint32_t mask = (1u << bits) - 1u;
+  const int64_t live = n - first;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int i = item_index(k);
+    if (i < live) {  // keys past the end are the tile's last: their digit is the largest and they come last
+      const uint32_t v = s_key[i], d = (v >> shift) & mask;
+      const uint32_t to = s_base[d] + static_cast<uint32_t>(i) - s_start[d];
+      out.key[to] = v;
+      out.unit[to] = s_unit[i];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradient: sums
+// ---------------------------------------------------------------------------------------------
+constexpr int kSumThreads = 256;
+constexpr int kSumMost = 2048;  // ids a workgroup takes at most
+constexpr int kSumAhead = 8;    // rows a lane group loads at once
+
+struct SumParams {
+  const char* grad;
+  const uint32_t* key;
+  const uint32_t* unit;
+  const float* inv_len;
+  const uint32_t* heads;  // compact: distinct keys that begin in each workgroup's run (or before it: scanned)
+  int32_t heads_scanned;
+  uint32_t* last_rank;    // compact: the last key's number of each workgroup's run
+  char* out;              // dense (one table) or compact rows
+  int64_t* rows_out;      // compact
+  int64_t* count_out;
+  float* partial;         // [columns' block][workgroup][2][slots]: what the run before began, what goes on behind
+  int64_t n;
+  int64_t grad_stride;    // elements between units' groups of `fields` (per-field), else dim
+  uint32_t total;
+  int32_t dim;            // the widest field's
+  int32_t log_lanes;      // lanes that cover a block of columns
+  int32_t run;            // ids a lane group
+  int32_t workgroups;
+  float scale;
+  int32_t fields;
+  ChunkDivide by_fields;
+};
+// A table for each field.
+struct SumFields {
+  char* data[kMaxFields];
+  int64_t stride[kMaxFields];
+  uint32_t base[kMaxFields];
+  int32_t dim[kMaxFields];
+  int32_t col[kMaxFields];
+};
+struct NoFields {};
+
+// Distinct keys that begin in each run of `ids`.
+__global__ void __launch_bounds__(kSumThreads) grad_heads_kernel(const uint32_t* key, int64_t n, uint32_t total, int ids,
+                                                                 uint32_t* heads) {
+  __shared__ uint32_t s_sum[kSumThreads / kWave];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * ids;
+  uint32_t c = 0;
+  for (int i = static_cast<int>(threadIdx.x); i < ids; i += kSumThreads) {
+    const int64_t at = first + i;
+    if (at < n) {
+      const uint32_t k = key[at];
+      c += k < total && (at == 0 || key[at - 1] != k) ? 1u : 0u;
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) c += static_cast<uint32_t>(shfl_i32(static_cast<int>(c), lane_id() ^ m));
+  if (lane_id() == 0) s_sum[threadIdx.x / kWave] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    c = 0;
+#pragma unroll
+    for (int w = 0; w < kSumThreads / kWave; ++w) c += s_sum[w];
+    heads[blockIdx.x] = c;
+  }
+}
+
+// heads[i] -> their sum before i, heads[count] the whole: one workgroup.
+__global__ void __launch_bounds__(kScanThreads) grad_heads_scan_kernel(uint32_t* heads, int64_t count) {
+  __shared__ uint32_t s_sum[kScanThreads];
+  const int t = static_cast<int>(threadIdx.x);
+  const int64_t per = (count + kScanThreads - 1) / kScanThreads;
+  const int64_t a = per * t < count ? per * t : count, b = a + per < count ? a + per : count;
+  uint32_t sum = 0;
+  for (int64_t i = a; i < b; ++i) sum += heads[i];
+  s_sum[t] = sum;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int i = 0; i < kScanThreads; ++i) {
+    if (i == t) sum = before;
+    before += s_sum[i];
+  }
+  if (t == 0) heads[count] = before;
+  for (int64_t i = a; i < b; ++i) {
+    const uint32_t c = heads[i];
+    heads[i] = sum;
+    sum += c;
+  }
+}
+
+// Columns of lane `lane` of block `block`: VEC from the first on; the last vector ends with the row and
+// overlaps the one before it (both come to the same sums). A row narrower than a vector is lane 0's.
+template <int VEC>
+__device__ __forceinline__ int first_column(int block, int lane, int dim) {
+  const int c = (block * kWave + lane) * VEC;
+  if (c >= dim) return -1;
+  return c + VEC <= dim ? c : (dim >= VEC ? dim - VEC : 0);
+}
+
+template <typename T, typename OT, typename FIELDS>
+struct Sums {
+  static constexpr int VEC = 16 / Elem<T>::kBytes;
+  static constexpr bool kPerField = !std::is_same<FIELDS, NoFields>::value;
+
+  // Element col of unit's row, and that row's width.
+  __device__ static __forceinline__ const char* row(const SumParams& p, const FIELDS& fs, uint32_t unit, int* dim) {
+    if constexpr (kPerField) {
+      const uint32_t b = p.by_fields.quotient(unit), f = unit - b * static_cast<uint32_t>(p.fields);
+      *dim = fs.dim[f];
+      return p.grad + (static_cast<int64_t>(b) * p.grad_stride + fs.col[f]) * Elem<T>::kBytes;
+    } else {
+      *dim = p.dim;
+      return p.grad + static_cast<int64_t>(unit) * p.dim * Elem<T>::kBytes;
+    }
+  }
+  // The row that a key's sum goes to; rank: its number among the distinct keys.
+  __device__ static __forceinline__ char* target(const SumParams& p, const FIELDS& fs, uint32_t key, uint32_t unit, uint32_t rank) {
+    if (p.rows_out) return p.out + static_cast<int64_t>(rank) * p.dim * Elem<OT>::kBytes;
+    if constexpr (kPerField) {
+      const uint32_t f = unit - p.by_fields.quotient(unit) * static_cast<uint32_t>(p.fields);
+      return fs.data[f] + static_cast<int64_t>(key - fs.base[f]) * fs.stride[f] * Elem<OT>::kBytes;
+    } else {
+      return p.out + static_cast<int64_t>(key) * p.dim * Elem<OT>::kBytes;
+    }
+  }
+  __device__ static __forceinline__ int width(const SumParams& p, const FIELDS& fs, uint32_t unit) {
+    if constexpr (kPerField) return fs.dim[unit - p.by_fields.quotient(unit) * static_cast<uint32_t>(p.fields)];
+    else return p.dim;
+  }
+};
+
+// A workgroup's run of the sorted ids: `run` for each of its kSumThreads >> log_lanes lane groups.
+// blockIdx.x: the run; blockIdx.y: the block of 64 vectors of columns.
+template <typename T, typename OT, typename FIELDS>
+__global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p, const FIELDS fs) {
+  using S = Sums<T, OT, FIELDS>;
+  constexpr int VEC = S::VEC;
+  __shared__ uint32_t s_key[kSumMost + 2];  // one before, one behind
+  __shared__ uint32_t s_unit[kSumMost];
+  __shared__ uint32_t s_rank[kSumMost];
+  __shared__ float s_part[2][kSumThreads * VEC];  // of each lane group: what a group before began; what goes on
+  __shared__ uint8_t s_flag[2][kSumThreads];      // 1: there is one; 2: it goes on behind the group, too
+  __shared__ uint32_t s_wave[kSumThreads / kWave], s_sum[2][kSumThreads / kWave];
+  const int t = static_cast<int>(threadIdx.x), lanes = 1 << p.log_lanes, groups = kSumThreads >> p.log_lanes;
+  const int ids = groups * p.run, block = static_cast<int>(blockIdx.y);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * ids;
+  const int live = static_cast<int>(p.n - first < ids ? p.n - first : ids);
+  for (int i = t; i < live + 2; i += kSumThreads) {
+    const int64_t at = first + i - 1;
+    s_key[i] = at >= 0 && at < p.n ? p.key[at] : 0xffffffffu;  // no key is that large
+    if (i < live) s_unit[i] = p.unit[first + i];
+  }
+  uint32_t begun = 0;  // distinct keys before this run
+  if (p.rows_out) {
+    uint32_t all = 0;
+    if (p.heads_scanned) {
+      begun = p.heads[blockIdx.x];
+      all = p.heads[p.workgroups];
+    } else {
+      for (int i = t; i < p.workgroups; i += kSumThreads) {
+        const uint32_t c = p.heads[i];
+        all += c;
+        begun += i < static_cast<int>(blockIdx.x) ? c : 0u;
+      }
+#pragma unroll
+      for (int m = 1; m < kWave; m <<= 1) {
+        all += static_cast<uint32_t>(shfl_i32(static_cast<int>(all), lane_id() ^ m));
+        begun += static_cast<uint32_t>(shfl_i32(static_cast<int>(begun), lane_id() ^ m));
+      }
+      if (lane_id() == 0) {
+        s_sum[0][t / kWave] = all;
+        s_sum[1][t / kWave] = begun;
+      }
+      __syncthreads();
+      all = begun = 0;
+#pragma unroll
+      for (int w = 0; w < kSumThreads / kWave; ++w) {
+        all += s_sum[0][w];
+        begun += s_sum[1][w];
+      }
+    }
+    if (blockIdx.x == 0 && block == 0 && t == 0) *p.count_out = all;
+  }
+  __syncthreads();
+  if (p.rows_out) {
+    // s_rank[i]: the number of id i's key among all distinct ones
+    const int per = (ids + kSumThreads - 1) / kSumThreads;
+    const int a = t * per;
+    uint32_t c = 0;
+    for (int i = a; i < a + per && i < live; ++i) c += s_key[i + 1] < p.total && s_key[i + 1] != s_key[i] ? 1u : 0u;
+    uint32_t x = c;
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) {
+      const uint32_t o = static_cast<uint32_t>(shfl_i32(static_cast<int>(x), lane_id() - d));
+      if (lane_id() >= d) x += o;
+    }
+    if (lane_id() == kWave - 1) s_wave[t / kWave] = x;
+    __syncthreads();
+    uint32_t rank = begun + x - c;
+    for (int w = 0; w < t / kWave; ++w) rank += s_wave[w];
+    for (int i = a; i < a + per && i < live; ++i) {
+      const uint32_t k = s_key[i + 1];
+      if (k < p.total && k != s_key[i]) {
+        if (block == 0) p.rows_out[rank] = k;
+        ++rank;
+      }
+      s_rank[i] = rank - 1u;  // of a key that began before the run: begun - 1
+    }
+    if (a < live && live <= a + per && block == 0) p.last_rank[blockIdx.x] = rank - 1u;
+    __syncthreads();
+  }
+
+  // Each lane group walks its ids. The row of a key is written where the key ends, unless it began in a group before.
+  const int g = t >> p.log_lanes, lane = t & (lanes - 1);
+  const int a = g * p.run, b = a + p.run < live ? a + p.run : live;
+  int flag0 = 0, flag1 = 0;
+  float acc[VEC];
+  if (a < b) {
+    uint32_t cur = s_key[a + 1];
+    bool open = cur == s_key[a];  // began before
+    int at = a;                   // an id of the current key
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+    const auto finish = [&](int i) {  // the key of id i ends
+      if (open) {
+        flag0 = 1;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s_part[0][t * VEC + e] = acc[e];
+      } else if (cur < p.total) {
+        const uint32_t unit = s_unit[i];
+        const int dim = S::width(p, fs, unit), c0 = first_column<VEC>(block, lane, dim);
+        if (c0 >= 0) {
+          char* const row = S::target(p, fs, cur, unit, p.rows_out ? s_rank[i] : 0u);
+          float v[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[e] = acc[e] * p.scale;
+          store_vec<OT, VEC>(row + static_cast<int64_t>(c0) * Elem<OT>::kBytes, dim - c0, v);
+        }
+      }
+      open = false;
+    };
+    for (int i0 = a; i0 < b; i0 += kSumAhead) {
+      uint4 raw[kSumAhead];
+      float w[kSumAhead];
+#pragma unroll
+      for (int u = 0; u < kSumAhead; ++u) {
+        const int i = i0 + u;
+        raw[u] = make_uint4(0u, 0u, 0u, 0u);
+        w[u] = 1.f;
+        if (i < b && s_key[i + 1] < p.total) {
+          const uint32_t unit = s_unit[i];
+          int dim;
+          const char* const row = S::row(p, fs, unit, &dim);
+          const int c0 = first_column<VEC>(block, lane, dim);
+          if (c0 >= 0) raw[u] = load_raw<T, VEC>(row + static_cast<int64_t>(c0) * Elem<T>::kBytes, dim - c0);
+          if (p.inv_len) w[u] = p.inv_len[unit];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kSumAhead; ++u) {
+        const int i = i0 + u;
+        if (i < b) {
+          const uint32_t k = s_key[i + 1];
+          if (k != cur) {
+            finish(at);
+            cur = k;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
+          }
+          at = i;
+          float v[VEC];
+          unpack16(raw[u], v, T{});
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) acc[e] = __builtin_fmaf(v[e], w[u], acc[e]);
+        }
+      }
+    }
+    if (s_key[b + 1] == cur && cur < p.total) {  // goes on behind the group
+      const int which = open ? 0 : 1;
+      if (open) flag0 = 2;
+      else flag1 = 1;
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) s_part[which][t * VEC + e] = acc[e];
+    } else {
+      finish(at);
+    }
+  }
+  if (lane == 0) {
+    s_flag[0][g] = static_cast<uint8_t>(flag0);
+    s_flag[1][g] = static_cast<uint8_t>(flag1);
+  }
+  __syncthreads();
+
+  // Keys that cross lane groups, in the groups' order: a thread adds up one column's parts.
+  const int slots = lanes * VEC;
+  float* const mine = p.partial + (static_cast<int64_t>(block) * p.workgroups + blockIdx.x) * 2 * slots;
+  for (int slot = t; slot < slots; slot += kSumThreads) {
+    bool before = live > 0 && s_key[1] == s_key[0];  // the key began before this workgroup's run
+    bool carrying = before;
+    float carry = 0.f;
+    const int l = slot / VEC, e = slot % VEC;
+    for (int w = 0; w < groups; ++w) {
+      const int f0 = s_flag[0][w];
+      if (f0) {
+        carry += s_part[0][w * slots + slot];
+        if (f0 == 1) {
+          if (before) {
+            mine[slot] = carry;
+          } else if (s_key[w * p.run + 1] < p.total) {
+            const int i = w * p.run;
+            const uint32_t unit = s_unit[i];
+            const int dim = S::width(p, fs, unit), c0 = first_column<VEC>(block, l, dim);
+            if (c0 >= 0 && c0 + e < dim)
+              store_one(reinterpret_cast<OT*>(S::target(p, fs, s_key[i + 1], unit, p.rows_out ? s_rank[i] : 0u)) + c0 + e,
+                        carry * p.scale, false);
+          }
+          before = carrying = false;
+          carry = 0.f;
+        }
+      }
+      if (s_flag[1][w]) {
+        carry = s_part[1][w * slots + slot];
+        carrying = true;
+      }
+    }
+    if (carrying) mine[before ? slot : slots + slot] = carry;
+  }
+}
+
+// Keys that cross workgroups: the workgroup in whose run one begins and goes on adds up its own part and, in order of the
+// runs, those of the runs it crosses.
+template <typename T, typename OT, typename FIELDS>
+__global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams p, const FIELDS fs) {
+  using S = Sums<T, OT, FIELDS>;
+  constexpr int VEC = S::VEC;
+  __shared__ float4 s_part[kSumThreads];
+  const int t = static_cast<int>(threadIdx.x), lanes = 1 << p.log_lanes, groups = kSumThreads >> p.log_lanes;
+  const int64_t ids = static_cast<int64_t>(groups) * p.run, first = static_cast<int64_t>(blockIdx.x) * ids;
+  const int block = static_cast<int>(blockIdx.y);
+  const int64_t next = first + ids;
+  if (next >= p.n) return;
+  const uint32_t key = p.key[next - 1];
+  if (key >= p.total || p.key[next] != key) return;                 // ends with the run
+  if (first > 0 && p.key[first] == key && p.key[first - 1] == key) return;  // began in a run before
+  // runs that begin with the key
+  int follow = 0;
+  for (int at = static_cast<int>(blockIdx.x) + 1;; at += kSumThreads) {
+    const int64_t i = static_cast<int64_t>(at + t) * ids;
+    const int c = __syncthreads_count(at + t < p.workgroups && i < p.n && p.key[i] == key);
+    follow += c;
+    if (c < kSumThreads) break;
+  }
+  const int slots = lanes * VEC, quads = slots / 4, rows = kSumThreads / quads;  // rows of parts side by side
+  const int64_t row_floats = 2 * static_cast<int64_t>(slots);
+  const float* const mine = p.partial + (static_cast<int64_t>(block) * p.workgroups + blockIdx.x) * row_floats;
+  const int q = t % quads, r = t / quads;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int h = r; h < follow; h += rows) {
+    const float4 v = *reinterpret_cast<const float4*>(mine + (h + 1) * row_floats + q * 4);
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  }
+  s_part[t] = sum;
+  __syncthreads();
+  if (t >= quads) return;
+  sum = *reinterpret_cast<const float4*>(mine + slots + q * 4);
+  for (int i = 0; i < rows; ++i) {
+    const float4 v = s_part[i * quads + q];
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  }
+  const uint32_t rank = p.rows_out ? p.last_rank[blockIdx.x] : 0u;
+  const uint32_t unit = p.unit[next - 1];
+  const int dim = S::width(p, fs, unit);
+  const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+  OT* const row = reinterpret_cast<OT*>(S::target(p, fs, key, unit, rank));
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int slot = q * 4 + k, c0 = first_column<VEC>(block, slot / VEC, dim);
+    if (c0 >= 0 && c0 + slot % VEC < dim) store_one(row + c0 + slot % VEC, v[k] * p.scale, false);
+  }
+}
+
+// 1 / length of every bag (1 for empty ones: no id reads it).
+__global__ void __launch_bounds__(256) grad_lengths_kernel(const GradSource s) {
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (j >= s.bags) return;
+  const int64_t len = bag_edge(s, j, 1) - bag_edge(s, j, 0), f = s.by_batch.quotient(static_cast<uint32_t>(j));
+  s.inv_len[(j - f * s.batch) * s.fields + f] = len > 0 ? 1.0f / static_cast<float>(len) : 1.0f;
+}
+
+// Rows of zeros: blockIdx.y is the table.
+struct FillParams {
+  char* data[kMaxFields];
+  int64_t rows[kMaxFields];
+  int64_t row_bytes[kMaxFields];   // to clear
+  int64_t row_stride[kMaxFields];  // bytes
+};
+__global__ void __launch_bounds__(256) grad_fill_rows_kernel(const FillParams p) {
+  const int f = static_cast<int>(blockIdx.y);
+  char* const data = p.data[f];
+  if (!data) return;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, all = static_cast<int64_t>(gridDim.x) * 256;
+  if (p.row_stride[f] == p.row_bytes[f]) {
+    const int64_t bytes = p.rows[f] * p.row_bytes[f], whole = bytes / 16;
+    for (int64_t i = at; i < whole; i += all) *reinterpret_cast<u32x4_any*>(data + i * 16) = u32x4{0u, 0u, 0u, 0u};
+    for (int64_t i = whole * 16 + at * 2; i < bytes; i += all * 2) *reinterpret_cast<uint16_t*>(data + i) = 0;
+    return;
+  }
+  for (int64_t r = at / kWave; r < p.rows[f]; r += all / kWave)
+    for (int64_t i = lane_id() * 2; i < p.row_bytes[f]; i += kWave * 2)
+      *reinterpret_cast<uint16_t*>(data + r * p.row_stride[f] + i) = 0;
+}
+__global__ void __launch_bounds__(256) grad_fill_numbers_kernel(int64_t* rows, int64_t capacity, int64_t* count) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  for (int64_t i = at; i < capacity; i += static_cast<int64_t>(gridDim.x) * 256) rows[i] = -1;
+  if (at == 0) *count = 0;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------------
+struct GradCall {
+  GradSource src{};
+  SumParams sum{};
+  SumFields fields{};
+  bool per_field = false;
+  int32_t grad_dtype = 0, out_dtype = 0;
+  int64_t capacity = 0;
+  void* workspace = nullptr;
+  int64_t workspace_bytes = 0;
+};
+
+template <typename T, typename OT, typename FIELDS>
+void launch_sums(const SumParams& p, const FIELDS& fs, int blocks, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(p.workgroups), static_cast<unsigned>(blocks));
+  hipLaunchKernelGGL((grad_sum_kernel<T, OT, FIELDS>), grid, dim3(kSumThreads), 0, s, p, fs);
+  if (p.workgroups > 1) hipLaunchKernelGGL((grad_join_kernel<T, OT, FIELDS>), grid, dim3(kSumThreads), 0, s, p, fs);
+}
+template <typename T, typename OT>
+void launch_sums_for(const GradCall& c, int blocks, hipStream_t s) {
+  if (c.per_field) launch_sums<T, OT, SumFields>(c.sum, c.fields, blocks, s);
+  else launch_sums<T, OT, NoFields>(c.sum, NoFields{}, blocks, s);
+}
+template <typename T>
+void launch_sums_typed(const GradCall& c, int blocks, hipStream_t s) {
+  switch (c.out_dtype) {
+    case CTI_EBAG_F32: launch_sums_for<T, float>(c, blocks, s); break;
+    case CTI_EBAG_BF16: launch_sums_for<T, bf16_t>(c, blocks, s); break;
+    default: launch_sums_for<T, f16_t>(c, blocks, s); break;
+  }
+}
+
+// The sort and the sums of a call whose arguments are checked.
+int run_gradient(GradCall& c, hipStream_t s) {
+  const int64_t n = c.src.n;
+  const bool compact = c.sum.rows_out != nullptr;
+  if (compact) {
+    const int64_t blocks = (c.capacity + 255) / 256;
+    hipLaunchKernelGGL(grad_fill_numbers_kernel, dim3(static_cast<unsigned>(blocks < 1 ? 1 : blocks > 1024 ? 1024 : blocks)), dim3(256),
+                       0, s, c.sum.rows_out, c.capacity, c.sum.count_out);
+  } else {
+    FillParams f{};
+    const int eb = dtype_bytes(c.out_dtype), tables = c.per_field ? c.src.fields : 1;
+    int64_t most = 0;
+    for (int i = 0; i < tables; ++i) {
+      f.data[i] = c.per_field ? c.fields.data[i] : c.sum.out;
+      f.rows[i] = c.src.rows[i];
+      f.row_bytes[i] = static_cast<int64_t>(c.per_field ? c.fields.dim[i] : c.sum.dim) * eb;
+      f.row_stride[i] = c.per_field ? c.fields.stride[i] * eb : f.row_bytes[i];
+      for (int k = 0; k < i; ++k)
+        if (f.data[k] == f.data[i]) f.data[i] = nullptr;  // fields that share a table
+      if (f.data[i] && f.rows[i] * f.row_bytes[i] > most) most = f.rows[i] * f.row_bytes[i];
+    }
+    int64_t blocks = (most + 16 * 256 - 1) / (16 * 256);
+    if (blocks > 4096) blocks = 4096;
+    hipLaunchKernelGGL(grad_fill_rows_kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(tables)), dim3(256), 0, s, f);
+  }
+  if (n == 0) return check_launch("gradient");
+
+  c.src.by_batch = ChunkDivide::by(static_cast<uint32_t>(c.src.batch));
+  const GradPlan plan = grad_plan(n, c.src.inv_len ? c.src.bags : 0, c.sum.dim, dtype_bytes(c.grad_dtype), c.src.total);
+  char* const ws = static_cast<char*>(c.workspace);
+  SortBuffers buf[2] = {{reinterpret_cast<uint32_t*>(ws + plan.key[0]), reinterpret_cast<uint32_t*>(ws + plan.unit[0])},
+                        {reinterpret_cast<uint32_t*>(ws + plan.key[1]), reinterpret_cast<uint32_t*>(ws + plan.unit[1])}};
+  uint32_t* const counts = reinterpret_cast<uint32_t*>(ws + plan.counts);
+  uint32_t* const totals = reinterpret_cast<uint32_t*>(ws + plan.totals);
+  if (c.src.inv_len) {
+    c.src.inv_len = reinterpret_cast<float*>(ws + plan.inv_len);
+    c.sum.inv_len = c.src.inv_len;
+    hipLaunchKernelGGL(grad_lengths_kernel, dim3(static_cast<unsigned>((c.src.bags + 255) / 256)), dim3(256), 0, s, c.src);
+  }
+  int at = 0;
+  if (plan.tiles == 1) {
+    hipLaunchKernelGGL(grad_sort_tile_kernel, dim3(1), dim3(kSortThreads), 0, s, c.src, buf[0], plan.bits);
+  } else {
+    const dim3 tiles(static_cast<unsigned>(plan.tiles));
+    const bool scan = plan.tiles > kGradTilesUnscanned;
+    for (int shift = 0; shift < plan.bits; shift += plan.digit_bits) {
+      const int bits = plan.bits - shift < plan.digit_bits ? plan.bits - shift : plan.digit_bits;
+      if (shift == 0) {
+        hipLaunchKernelGGL(grad_keys_kernel, tiles, dim3(kSortThreads), 0, s, c.src, buf[0], counts, bits);
+      } else {
+        hipLaunchKernelGGL(grad_count_kernel, tiles, dim3(kSortThreads), 0, s, buf[at].key, n, shift, bits, counts);
+      }
+      if (scan) hipLaunchKernelGGL(grad_scan_kernel, dim3(kDigits / 4), dim3(kScanThreads), 0, s, counts, totals, plan.tiles);
+      hipLaunchKernelGGL(grad_scatter_kernel, tiles, dim3(kSortThreads), 0, s, buf[at], buf[1 - at], n, shift, bits, counts,
+                         scan ? totals : nullptr, static_cast<int>(plan.tiles));
+      at = 1 - at;
+    }
+  }
+  SumParams& p = c.sum;
+  p.key = buf[at].key;
+  p.unit = buf[at].unit;
+  p.n = n;
+  p.total = c.src.total;
+  p.partial = reinterpret_cast<float*>(ws + plan.partial);
+  p.log_lanes = plan.log_lanes;
+  p.run = plan.run;
+  p.workgroups = static_cast<int32_t>(plan.workgroups);
+  p.fields = c.src.fields;
+  p.by_fields = ChunkDivide::by(static_cast<uint32_t>(c.src.fields));
+  if (compact) {
+    uint32_t* const heads = reinterpret_cast<uint32_t*>(ws + plan.heads);
+    p.heads = heads;
+    p.last_rank = reinterpret_cast<uint32_t*>(ws + plan.last_rank);
+    hipLaunchKernelGGL(grad_heads_kernel, dim3(static_cast<unsigned>(plan.workgroups)), dim3(kSumThreads), 0, s, p.key, n, p.total,
+                       static_cast<int>(plan.run * (kSumThreads >> plan.log_lanes)), heads);
+    p.heads_scanned = plan.workgroups > kGradHeadsUnscanned;
+    if (p.heads_scanned)
+      hipLaunchKernelGGL(grad_heads_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, heads, plan.workgroups);
+  }
+  switch (c.grad_dtype) {
+    case CTI_EBAG_F32: launch_sums_typed<float>(c, plan.blocks, s); break;
+    case CTI_EBAG_BF16: launch_sums_typed<bf16_t>(c, plan.blocks, s); break;
+    default: launch_sums_typed<f16_t>(c, plan.blocks, s); break;
+  }
+  return check_launch("gradient");
+}
+
+// Checks that every form of the gradient shares. `rows`: of all tables; padding may be -1.
+int check_gradient(int32_t grad_dtype, int32_t out_dtype, int32_t index_type, int64_t n, int64_t units, int64_t dim,
+                   bool compact, const int64_t* count_out, int64_t rows, int64_t capacity) {
+  if (!float_dtype(grad_dtype)) return set_error(CTI_EBAG_EINVAL, "unknown gradient dtype code %d", grad_dtype);
+  if (!float_dtype(out_dtype)) return set_error(CTI_EBAG_EINVAL, "unknown output dtype code %d", out_dtype);
+  if (index_type != CTI_EBAG_I64 && index_type != CTI_EBAG_I32) return set_error(CTI_EBAG_EINVAL, "unknown index type %d", index_type);
+  if (n < 0) return set_error(CTI_EBAG_EINVAL, "the number of ids must be >= 0 (got %lld)", (long long)n);
+  if (dim < 1) return set_error(CTI_EBAG_EINVAL, "dim must be >= 1 (got %lld)", (long long)dim);
+  if (dim > kGradMostDim) return set_error(CTI_EBAG_EUNSUPPORTED, "dim %lld > 2^22", (long long)dim);
+  if (rows < 1) return set_error(CTI_EBAG_EINVAL, "rows must be >= 1 (got %lld)", (long long)rows);
+  if (rows >= kGradMostRows) return set_error(CTI_EBAG_EUNSUPPORTED, "%lld rows of tables (2^31 - 1 at most)", (long long)rows);
+  if (n > kGradMostIds || units > kGradMostIds)
+    return set_error(CTI_EBAG_EUNSUPPORTED, "%lld ids in %lld bags (2^30 of each at most)", (long long)n, (long long)units);
+  if (compact != (count_out != nullptr)) return set_error(CTI_EBAG_EINVAL, "rows_out and count_out are given together or not at all");
+  if (compact && capacity < (n < rows ? n : rows))
+    return set_error(CTI_EBAG_EINVAL, "capacity %lld for the rows of %lld ids in tables of %lld", (long long)capacity, (long long)n,
+                     (long long)rows);
+  return CTI_EBAG_OK;
+}
+
+int check_workspace(const GradCall& c, int64_t bags, int64_t dim) {
+  if (c.src.n == 0) return CTI_EBAG_OK;
+  const int64_t need = grad_plan(c.src.n, bags, dim, 2, c.src.total).bytes, need4 = grad_plan(c.src.n, bags, dim, 4, c.src.total).bytes;
+  const int64_t most = need > need4 ? need : need4;
+  if (!c.workspace || c.workspace_bytes < most)
+    return set_error(CTI_EBAG_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)(c.workspace ? c.workspace_bytes : 0),
+                     (long long)most);
+  if (reinterpret_cast<uintptr_t>(c.workspace) % 16) return set_error(CTI_EBAG_EINVAL, "workspace is not 16-byte aligned");
+  return CTI_EBAG_OK;
+}
+
+}  // namespace
+}  // namespace cti
+
+using namespace cti;
+
+extern "C" int cti_ebag_lookup(const void* ids, int32_t index_type, int64_t n, const void* weight, int32_t dtype, int64_t rows,
+                               int64_t row_stride, int32_t dim, float scale, void* out, int32_t out_dtype, void* stream) {
+  clear_error();
+  if (!float_dtype(dtype)) return set_error(CTI_EBAG_EINVAL, "unknown table dtype code %d", dtype);
+  if (!float_dtype(out_dtype)) return set_error(CTI_EBAG_EINVAL, "unknown output dtype code %d", out_dtype);
+  if (index_type != CTI_EBAG_I64 && index_type != CTI_EBAG_I32) return set_error(CTI_EBAG_EINVAL, "unknown index type %d", index_type);
+  if (n < 0) return set_error(CTI_EBAG_EINVAL, "the number of ids must be >= 0 (got %lld)", (long long)n);
+  if (dim < 1) return set_error(CTI_EBAG_EINVAL, "dim must be >= 1 (got %d)", dim);
+  if (rows < 1) return set_error(CTI_EBAG_EINVAL, "rows must be >= 1 (got %lld)", (long long)rows);
+  if (row_stride < dim) return set_error(CTI_EBAG_EINVAL, "row_stride %lld < dim %d", (long long)row_stride, dim);
+  if (n == 0) return CTI_EBAG_OK;
+  if (!ids || !weight || !out) return set_error(CTI_EBAG_EINVAL, "NULL device pointer among ids/weight/out");
+  LookupParams p;
+  p.weight = static_cast<const char*>(weight);
+  p.rows = rows;
+  p.row_bytes = row_stride * dtype_bytes(dtype);
+  p.dim = dim;
+  p.ids64 = index_type == CTI_EBAG_I64;
+  p.per_row = (static_cast<uint32_t>(dim) + 7) / 8;
+  p.div = ChunkDivide::by(p.per_row);
+  p.scale = scale;
+  p.stream_out = n * dim * dtype_bytes(out_dtype) >= kStreamOutBytes;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t per_launch = kMostChunks / p.per_row;  // rows
+  for (int64_t i = 0; i < n; i += per_launch) {
+    const int64_t now = n - i < per_launch ? n - i : per_launch;
+    p.ids = static_cast<const char*>(ids) + i * (p.ids64 ? 8 : 4);
+    p.out = static_cast<char*>(out) + i * dim * dtype_bytes(out_dtype);
+    p.chunks = static_cast<uint32_t>(now * p.per_row);
+    const dim3 grid((p.chunks + kLookupThreads - 1) / kLookupThreads), block(kLookupThreads);
+    with_types(dtype, out_dtype, [&](auto t, auto o) {
+      hipLaunchKernelGGL((lookup_kernel<decltype(t), decltype(o)>), grid, block, 0, s, p);
+    });
+  }
+  return check_launch("lookup");
+}
+
+extern "C" int64_t cti_ebag_backward_workspace_bytes(int64_t nnz, int64_t bags, int64_t rows, int32_t dim, int32_t pooling) {
+  if (nnz <= 0 || bags < 0 || rows < 1 || dim < 1 || nnz > kGradMostIds || bags > kGradMostIds || rows >= kGradMostRows) return 0;
+  const int64_t b = pooling == CTI_EBAG_MEAN ? bags : 0;
+  const int64_t two = grad_plan(nnz, b, dim, 2, static_cast<uint32_t>(rows)).bytes;
+  const int64_t four = grad_plan(nnz, b, dim, 4, static_cast<uint32_t>(rows)).bytes;
+  return two > four ? two : four;
+}
+
+extern "C" int cti_ebag_lookup_backward(const void* grad, int32_t grad_dtype, const void* ids, int32_t index_type, int64_t n,
+                                        int64_t rows, int32_t dim, float scale, int64_t padding_idx, void* out, int32_t out_dtype,
+                                        int64_t* rows_out, int64_t* count_out, int64_t capacity, void* workspace,
+                                        int64_t workspace_bytes, void* stream) {
+  clear_error();
+  int rc = check_gradient(grad_dtype, out_dtype, index_type, n, n, dim, rows_out != nullptr, count_out, rows, capacity);
+  if (rc != CTI_EBAG_OK) return rc;
+  if (padding_idx < -1 || padding_idx >= rows)
+    return set_error(CTI_EBAG_EINVAL, "padding_idx %lld outside [0, %lld)", (long long)padding_idx, (long long)rows);
+  if ((n > 0 && (!grad || !ids)) || (!out && (n > 0 || !rows_out)))
+    return set_error(CTI_EBAG_EINVAL, "NULL device pointer among grad/ids/out");
+  GradCall c;
+  c.src.ids = ids;
+  c.src.n = n;
+  c.src.batch = n;
+  c.src.bags = n;
+  c.src.fields = 1;
+  c.src.ids64 = index_type == CTI_EBAG_I64;
+  c.src.total = static_cast<uint32_t>(rows);
+  c.src.padding = padding_idx;
+  c.src.rows[0] = static_cast<uint32_t>(rows);
+  c.sum.grad = static_cast<const char*>(grad);
+  c.sum.dim = dim;
+  c.sum.scale = scale;
+  c.sum.out = static_cast<char*>(out);
+  c.sum.rows_out = rows_out;
+  c.sum.count_out = count_out;
+  c.grad_dtype = grad_dtype;
+  c.out_dtype = out_dtype;
+  c.capacity = capacity;
+  c.workspace = workspace;
+  c.workspace_bytes = workspace_bytes;
+  rc = check_workspace(c, 0, dim);
+  return rc != CTI_EBAG_OK ? rc : run_gradient(c, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int cti_ebag_fused_all_slots_backward(const void* grad, int32_t grad_dtype, const void* values, int32_t index_type,
+                                                 const void* val_offsets, const void* row_offsets, int32_t offset_type,
+                                                 int64_t batch_size, int32_t num_slots, int32_t emb_dim, int64_t max_idx,
+                                                 int64_t nnz, int32_t pooling, int64_t padding_idx, void* out, int32_t out_dtype,
+                                                 int64_t* rows_out, int64_t* count_out, int64_t capacity, void* workspace,
+                                                 int64_t workspace_bytes, void* stream) {
+  clear_error();
+  if (batch_size < 0) return set_error(CTI_EBAG_EINVAL, "batch_size must be >= 0 (got %lld)", (long long)batch_size);
+  if (num_slots < 0) return set_error(CTI_EBAG_EINVAL, "num_slots must be >= 0 (got %d)", num_slots);
+  if (max_idx < 0) return set_error(CTI_EBAG_EINVAL, "max_idx must be >= 0 (got %lld)", (long long)max_idx);
+  if (offset_type != CTI_EBAG_I64 && offset_type != CTI_EBAG_I32) return set_error(CTI_EBAG_EINVAL, "unknown offset type %d", offset_type);
+  if (pooling != CTI_EBAG_SUM && pooling != CTI_EBAG_MEAN) return set_error(CTI_EBAG_EINVAL, "unknown pooling mode %d", pooling);
+  if (batch_size > kGradMostIds) return set_error(CTI_EBAG_EUNSUPPORTED, "batch_size %lld (2^30 at most)", (long long)batch_size);
+  if (max_idx >= kGradMostRows) return set_error(CTI_EBAG_EUNSUPPORTED, "max_idx %lld", (long long)max_idx);
+  const int64_t rows = max_idx + 1, bags = batch_size * num_slots;
+  int rc = check_gradient(grad_dtype, out_dtype, index_type, nnz, bags, emb_dim, rows_out != nullptr, count_out, rows, capacity);
+  if (rc != CTI_EBAG_OK) return rc;
+  if (padding_idx < -1 || padding_idx >= rows)
+    return set_error(CTI_EBAG_EINVAL, "padding_idx %lld outside [0, %lld)", (long long)padding_idx, (long long)rows);
+  const bool any = nnz > 0 && bags > 0;
+  if ((any && (!grad || !values || !val_offsets || !row_offsets)) || (!out && (any || !rows_out)))
+    return set_error(CTI_EBAG_EINVAL, "NULL device pointer among grad/values/val_offsets/row_offsets/out");
+  GradCall c;
+  c.src.ids = values;
+  c.src.val_offsets = val_offsets;
+  c.src.offsets = row_offsets;
+  c.src.n = any ? nnz : 0;
+  c.src.batch = batch_size;
+  c.src.bags = bags;
+  c.src.fields = num_slots > 0 ? num_slots : 1;
+  c.src.ids64 = index_type == CTI_EBAG_I64;
+  c.src.offs64 = offset_type == CTI_EBAG_I64;
+  c.src.total = static_cast<uint32_t>(rows);
+  c.src.padding = padding_idx;
+  c.src.rows[0] = static_cast<uint32_t>(rows);
+  c.src.inv_len = pooling == CTI_EBAG_MEAN ? static_cast<float*>(workspace) : nullptr;
+  c.sum.grad = static_cast<const char*>(grad);
+  c.sum.dim = emb_dim;
+  c.sum.scale = 1.f;
+  c.sum.out = static_cast<char*>(out);
+  c.sum.rows_out = rows_out;
+  c.sum.count_out = count_out;
+  c.grad_dtype = grad_dtype;
+  c.out_dtype = out_dtype;
+  c.capacity = capacity;
+  c.workspace = workspace;
+  c.workspace_bytes = workspace_bytes;
+  rc = check_workspace(c, pooling == CTI_EBAG_MEAN ? bags : 0, emb_dim);
+  return rc != CTI_EBAG_OK ? rc : run_gradient(c, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int cti_ebag_backward(const void* grad, int32_t grad_dtype, int64_t grad_row_stride, const void* values,
+                                 int32_t index_type, int64_t nnz, const int64_t* offsets, int64_t batch_size, int32_t num_fields,
+                                 const cti_ebag_table* tables, int32_t pooling, int64_t padding_idx, int32_t out_dtype, void* out,
+                                 int64_t* rows_out, int64_t* count_out, int64_t capacity, void* workspace, int64_t workspace_bytes,
+                                 void* stream) {
+  clear_error();
+  if (batch_size < 0) return set_error(CTI_EBAG_EINVAL, "batch_size must be >= 0 (got %lld)", (long long)batch_size);
+  if (num_fields < 1) return set_error(CTI_EBAG_EINVAL, "num_fields must be >= 1 (got %d)", num_fields);
+  if (num_fields > kMaxFields) return set_error(CTI_EBAG_EUNSUPPORTED, "num_fields %d > %d", num_fields, kMaxFields);
+  if (!tables) return set_error(CTI_EBAG_EINVAL, "tables is NULL");
+  if (pooling != CTI_EBAG_SUM && pooling != CTI_EBAG_MEAN) return set_error(CTI_EBAG_EINVAL, "unknown pooling mode %d", pooling);
+  if (batch_size > kGradMostIds) return set_error(CTI_EBAG_EUNSUPPORTED, "batch_size %lld (2^30 at most)", (long long)batch_size);
+  const bool compact = rows_out != nullptr;
+  GradCall c;
+  c.per_field = true;
+  int64_t rows = 0, dim = 0;
+  for (int f = 0; f < num_fields; ++f) {
+    const cti_ebag_table& t = tables[f];
+    if (t.rows < 1) return set_error(CTI_EBAG_EINVAL, "tables[%d].rows must be >= 1 (got %lld)", f, (long long)t.rows);
+    if (t.dim < 1) return set_error(CTI_EBAG_EINVAL, "tables[%d].dim must be >= 1 (got %d)", f, t.dim);
+    if (t.row_stride < t.dim) return set_error(CTI_EBAG_EINVAL, "tables[%d].row_stride %lld < dim %d", f, (long long)t.row_stride, t.dim);
+    if (t.out_col < 0 || t.out_col + static_cast<int64_t>(t.dim) > grad_row_stride)
+      return set_error(CTI_EBAG_EINVAL, "tables[%d]: columns [%d, %lld) outside the gradient's row of %lld", f, t.out_col,
+                       (long long)t.out_col + t.dim, (long long)grad_row_stride);
+    if (!t.data) return set_error(CTI_EBAG_EINVAL, "tables[%d].data is NULL", f);
+    if (compact && t.dim != tables[0].dim)
+      return set_error(CTI_EBAG_EUNSUPPORTED, "rows_out needs tables of one width (%d, %d)", tables[0].dim, t.dim);
+    if (padding_idx < -1 || padding_idx >= t.rows)
+      return set_error(CTI_EBAG_EINVAL, "padding_idx %lld outside tables[%d]", (long long)padding_idx, f);
+    int same = f;
+    for (int k = 0; k < f && same == f; ++k)
+      if (tables[k].data == t.data) same = k;
+    if (same < f && (tables[same].rows != t.rows || tables[same].dim != t.dim || tables[same].row_stride != t.row_stride))
+      return set_error(CTI_EBAG_EINVAL, "tables[%d] and tables[%d] share data but not their shape", same, f);
+    c.src.base[f] = same < f ? c.src.base[same] : static_cast<uint32_t>(rows);
+    if (same == f) {
+      if (t.rows >= kGradMostRows || rows + t.rows >= kGradMostRows)
+        return set_error(CTI_EBAG_EUNSUPPORTED, "more than 2^31 - 2 rows of tables");
+      rows += t.rows;
+    }
+    c.src.rows[f] = static_cast<uint32_t>(t.rows);
+    c.fields.data[f] = static_cast<char*>(const_cast<void*>(t.data));
+    c.fields.stride[f] = t.row_stride;
+    c.fields.base[f] = c.src.base[f];
+    c.fields.dim[f] = t.dim;
+    c.fields.col[f] = t.out_col;
+    if (t.dim > dim) dim = t.dim;
+  }
+  const int64_t bags = batch_size * num_fields;
+  int rc = check_gradient(grad_dtype, out_dtype, index_type, nnz, bags, dim, compact, count_out, rows, capacity);
+  if (rc != CTI_EBAG_OK) return rc;
+  const bool any = nnz > 0 && bags > 0;
+  if ((any && (!grad || !values || !offsets)) || (compact && any && !out))
+    return set_error(CTI_EBAG_EINVAL, "NULL device pointer among grad/values/offsets/out");
+  c.src.ids = values;
+  c.src.offsets = offsets;
+  c.src.n = any ? nnz : 0;
+  c.src.batch = batch_size;
+  c.src.bags = bags;
+  c.src.fields = num_fields;
+  c.src.ids64 = index_type == CTI_EBAG_I64;
+  c.src.offs64 = 1;
+  c.src.per_field = 1;
+  c.src.total = static_cast<uint32_t>(rows);
+  c.src.padding = padding_idx;
+  c.src.inv_len = pooling == CTI_EBAG_MEAN ? static_cast<float*>(workspace) : nullptr;
+  c.sum.grad = static_cast<const char*>(grad);
+  c.sum.grad_stride = grad_row_stride;
+  c.sum.dim = static_cast<int32_t>(dim);
+  c.sum.scale = 1.f;
+  c.sum.out = static_cast<char*>(out);
+  c.sum.rows_out = rows_out;
+  c.sum.count_out = count_out;
+  c.grad_dtype = grad_dtype;
+  c.out_dtype = out_dtype;
+  c.capacity = capacity;
+  c.workspace = workspace;
+  c.workspace_bytes = workspace_bytes;
+  rc = check_workspace(c, pooling == CTI_EBAG_MEAN ? bags : 0, dim);
+  return rc != CTI_EBAG_OK ? rc : run_gradient(c, static_cast<hipStream_t>(stream));
+}

@@ -1,0 +1,676 @@
+// Dropout, and the layer norm with dropout and the residual's addition in it, forward and backward, for
+// MI355X (gfx950).
+//
+//   dropout:   y = residual + keep(row, col) * x / (1 - p)
+//   forward:   h = residual + keep * x / (1 - p), stored in x's type; y = (h - mean) * rstd * gamma + beta of
+//              what is stored, so that the backward pass differentiates what the forward pass computed
+//   backward:  z = (h - mean) * rstd, a = g * gamma
+//              dh = rstd * (a - mean(a) - z * mean(a * z)) + grad_h      (the residual's gradient)
+//              dx = keep * dh / (1 - p);  dgamma = sum over rows of g * z;  dbeta = sum over rows of g
+// all in fp32 (sums too), one rounding to the outputs' types. The mask is never stored: it is a function of
+// seed, offset, row and column.
+//
+// Bound by HBM, each array read or written once; the generator's multiplications come next. A row lies in
+// the registers of 8 lanes (64 columns) to 512 threads (16,384 columns), chunks of 8 columns a thread; wider
+// rows take a loop form. The backward pass adds up dgamma and dbeta in registers over the rows of a
+// workgroup, which go to the workspace as one fp32 row each; a second kernel adds those up in their order.
+// No atomics: results are the same bits in every run.
+#include <stdint.h>
+
+#include "ebag_train.h"
+
+namespace cti {
+namespace {
+
+// ---------------------------------------------------------------------------------------------
+// Dropout
+// ---------------------------------------------------------------------------------------------
+constexpr int kDropThreads = 256;
+
+struct DropParams {
+  const char* x;
+  const char* res;  // NULL: no residual
+  char* y;
+  int64_t cols;
+  uint32_t first_row;
+  uint32_t chunks;   // of this launch
+  uint32_t per_row;
+  ChunkDivide div;
+  Dropout drop;
+  int32_t stream_out;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kDropThreads) dropout_kernel(const DropParams p) {
+  const uint32_t c = blockIdx.x * kDropThreads + threadIdx.x;
+  if (c >= p.chunks) return;
+  const uint32_t row = p.div.quotient(c), chunk = c - row * p.per_row;
+  const int64_t col = static_cast<int64_t>(chunk) * 8, at = (static_cast<int64_t>(row) * p.cols + col) * Elem<T>::kBytes;
+  const int live = p.cols - col < 8 ? static_cast<int>(p.cols - col) : 8;
+  float v[8], r[8];
+  load8<T>(p.x + at, live, v);
+  if (p.res) load8<T>(p.res + at, live, r);
+  Dropout d = p.drop;
+  if (d.threshold) {
+    load_state(d);
+    apply_dropout(d, p.first_row + row, chunk, v);
+  }
+  if (p.res) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += r[e];
+  }
+  with_stream(p.stream_out, [&](auto stream) { store8<T, decltype(stream)::value>(p.y + at, live, v); });
+}
+
+// ---------------------------------------------------------------------------------------------
+// Norm
+// ---------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ void round8(float* v) {
+  if constexpr (std::is_same<T, bf16_t>::value) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const uint32_t w = pack_bf16x2(v[e], v[e + 1]);
+      v[e] = __uint_as_float(w << 16);
+      v[e + 1] = __uint_as_float(w & 0xffff0000u);
+    }
+  } else if constexpr (std::is_same<T, f16_t>::value) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = f16_bits_to_f32(f32_to_f16_bits(v[e]));
+  }
+}
+
+// A chunk of 8 columns as loaded; columns past the row are +0.
+template <typename T>
+struct Chunk {
+  static constexpr int kWords = Elem<T>::kBytes / 2;
+  uint4 raw[kWords];
+  __device__ __forceinline__ void load(const char* p, int live) {
+    constexpr int VEC = 16 / Elem<T>::kBytes;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      raw[i] = live > i * VEC ? load_raw<T, VEC>(p + i * 16, live - i * VEC) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ void unpack(float* v) const {
+    constexpr int VEC = 16 / Elem<T>::kBytes;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) unpack16(raw[i], v + i * VEC, T{});
+  }
+};
+
+// N sums over the LANES threads that hold a row, in a fixed order. s_red: N * LANES / 64 floats.
+template <int LANES, int N>
+__device__ __forceinline__ void row_sums(float* v, float* s_red) {
+  if constexpr (LANES <= kWave) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+#pragma unroll
+      for (int m = 1; m < LANES; m <<= 1) v[k] += shfl_xor_f32(v[k], m);
+    }
+  } else {
+    block_sum_n<LANES / kWave, N>(v, s_red);
+  }
+}
+
+struct TrainNormParams {
+  const char* x;
+  const char* res;
+  const void* gamma;
+  const void* beta;
+  char* h;  // NULL: h is x
+  char* y;
+  float* mean;
+  float* rstd;
+  int64_t rows;
+  int64_t cols;
+  uint32_t first_row;
+  float eps;
+  Dropout drop;
+  int32_t stream_out;
+};
+
+template <int LANES>
+struct Block {
+  static constexpr int kThreads = LANES < 256 ? 256 : LANES;
+  static constexpr int kSide = kThreads / LANES;  // rows side by side
+  static constexpr int kReds = LANES <= kWave ? 1 : 2 * LANES / kWave;
+};
+
+template <typename T, typename PT, int LANES, int K>
+__global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_kernel(const TrainNormParams p) {
+  __shared__ float s_red[Block<LANES>::kReds];
+  const int t = static_cast<int>(threadIdx.x), lane = t % LANES;
+  const int64_t want = static_cast<int64_t>(blockIdx.x) * Block<LANES>::kSide + t / LANES;
+  const bool there = want < p.rows;  // the lanes of a row past the end take part in the shuffles
+  const int64_t row = there ? want : p.rows - 1;
+  const int cols = static_cast<int>(p.cols);
+  const int64_t at = row * p.cols * Elem<T>::kBytes;
+  Dropout d = p.drop;
+  if (d.threshold) load_state(d);
+  float v[K][8], s = 0.f;
+  Chunk<T> x[K], r[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (lane + k * LANES) * 8;
+    x[k].load(p.x + at + c * Elem<T>::kBytes, cols - c);
+    if (p.res) r[k].load(p.res + at + c * Elem<T>::kBytes, cols - c);
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (lane + k * LANES) * 8;
+    x[k].unpack(v[k]);
+    if (d.threshold) apply_dropout(d, p.first_row + static_cast<uint32_t>(row), static_cast<uint32_t>(c / 8), v[k]);
+    if (p.res) {
+      float w[8];
+      r[k].unpack(w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[k][e] += w[e];
+    }
+    if (p.h) {
+      round8<T>(v[k]);
+      if (there && c < cols)
+        with_stream(p.stream_out, [&](auto st) { store8<T, decltype(st)::value>(p.h + at + c * Elem<T>::kBytes, cols - c, v[k]); });
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += v[k][e];  // columns past the row are +0: dropped or kept
+  }
+  const float n = static_cast<float>(cols);
+  row_sums<LANES, 1>(&s, s_red);
+  const float mean = s / n;
+  float q = 0.f;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (lane + k * LANES) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[k][e] = c + e < cols ? v[k][e] - mean : 0.f;
+      q += v[k][e] * v[k][e];
+    }
+  }
+  row_sums<LANES, 1>(&q, s_red);
+  const float rstd = 1.0f / __builtin_sqrtf(q / n + p.eps);
+  if (!there) return;
+  if (lane == 0) {
+    p.mean[row] = mean;
+    p.rstd[row] = rstd;
+  }
+  with_stream(p.stream_out, [&](auto st) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (lane + k * LANES) * 8;
+      if (c < cols) {
+        float gm[8], bt[8];
+        load8<PT>(static_cast<const char*>(p.gamma) + c * Elem<PT>::kBytes, cols - c, gm);
+        load8<PT>(static_cast<const char*>(p.beta) + c * Elem<PT>::kBytes, cols - c, bt);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gm[e] = v[k][e] * rstd * gm[e] + bt[e];
+        store8<T, decltype(st)::value>(p.y + at + c * Elem<T>::kBytes, cols - c, gm);
+      }
+    }
+  });
+}
+
+// Rows of any width: a workgroup reads its row three times (h is made again each time).
+constexpr int kWideThreads = 1024;
+template <typename T>
+__device__ __forceinline__ void wide_h(const TrainNormParams& p, const Dropout& d, int64_t row, int64_t c, float* v) {
+  const int64_t at = (row * p.cols + c) * Elem<T>::kBytes;
+  const int live = p.cols - c < 8 ? static_cast<int>(p.cols - c) : 8;
+  load8<T>(p.x + at, live, v);
+  if (d.threshold) apply_dropout(d, p.first_row + static_cast<uint32_t>(row), static_cast<uint32_t>(c / 8), v);
+  if (p.res) {
+    float w[8];
+    load8<T>(p.res + at, live, w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += w[e];
+  }
+  if (p.h) round8<T>(v);
+}
+
+template <typename T, typename PT>
+__global__ void __launch_bounds__(kWideThreads) train_norm_wide_kernel(const TrainNormParams p) {
+  __shared__ float s_red[2 * kWideThreads / kWave];
+  const int64_t row = blockIdx.x, t = threadIdx.x;
+  Dropout d = p.drop;
+  if (d.threshold) load_state(d);
+  float s = 0.f, v[8];
+  for (int64_t c = t * 8; c < p.cols; c += kWideThreads * 8) {
+    wide_h<T>(p, d, row, c, v);
+    if (p.h) store8<T>(p.h + (row * p.cols + c) * Elem<T>::kBytes, p.cols - c < 8 ? static_cast<int>(p.cols - c) : 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += v[e];
+  }
+  const float n = static_cast<float>(p.cols);
+  row_sums<kWideThreads, 1>(&s, s_red);
+  const float mean = s / n;
+  float q = 0.f;
+  for (int64_t c = t * 8; c < p.cols; c += kWideThreads * 8) {
+    wide_h<T>(p, d, row, c, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float w = c + e < p.cols ? v[e] - mean : 0.f;
+      q += w * w;
+    }
+  }
+  row_sums<kWideThreads, 1>(&q, s_red);
+  const float rstd = 1.0f / __builtin_sqrtf(q / n + p.eps);
+  if (t == 0) {
+    p.mean[row] = mean;
+    p.rstd[row] = rstd;
+  }
+  for (int64_t c = t * 8; c < p.cols; c += kWideThreads * 8) {
+    const int live = p.cols - c < 8 ? static_cast<int>(p.cols - c) : 8;
+    float gm[8], bt[8];
+    wide_h<T>(p, d, row, c, v);
+    load8<PT>(static_cast<const char*>(p.gamma) + c * Elem<PT>::kBytes, live, gm);
+    load8<PT>(static_cast<const char*>(p.beta) + c * Elem<PT>::kBytes, live, bt);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (v[e] - mean) * rstd * gm[e] + bt[e];
+    store8<T>(p.y + (row * p.cols + c) * Elem<T>::kBytes, live, v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Norm, backward
+// ---------------------------------------------------------------------------------------------
+struct NormBackParams {
+  const char* g;
+  const char* h;
+  const char* grad_h;  // NULL: none
+  const float* mean;
+  const float* rstd;
+  const void* gamma;
+  char* dh;  // NULL: not asked for (or the same as dx)
+  char* dx;
+  float* partial;  // [workgroup][dgamma, dbeta][whole chunks]
+  int64_t rows;
+  int64_t cols;
+  Dropout drop;
+  int32_t stream_out;
+};
+
+template <typename T, typename PT, int LANES, int K>
+__global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel(const NormBackParams p) {
+  constexpr int SIDE = Block<LANES>::kSide;
+  __shared__ float s_red[Block<LANES>::kReds];
+  __shared__ float s_acc[SIDE > 1 ? 2 * Block<LANES>::kThreads * 8 * K : 1];
+  const int t = static_cast<int>(threadIdx.x), lane = t % LANES;
+  const int cols = static_cast<int>(p.cols);
+  const float n = static_cast<float>(cols);
+  Dropout d = p.drop;
+  if (d.threshold) load_state(d);
+  float dgamma[K][8], dbeta[K][8], gamma[K][8];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (lane + k * LANES) * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gamma[k][e] = dgamma[k][e] = dbeta[k][e] = 0.f;
+    if (c < cols) load8<PT>(static_cast<const char*>(p.gamma) + c * Elem<PT>::kBytes, cols - c, gamma[k]);
+  }
+  const int64_t step = static_cast<int64_t>(gridDim.x) * SIDE;
+  struct Row {
+    Chunk<T> g[K], h[K], gh[K];
+    float mean, rstd;
+  };
+  const auto fetch = [&](int64_t row, Row& r) {
+    const int64_t at = row * p.cols * Elem<T>::kBytes;
+    r.mean = p.mean[row];
+    r.rstd = p.rstd[row];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (lane + k * LANES) * 8;
+      const int64_t o = at + c * Elem<T>::kBytes;
+      r.g[k].load(p.g + o, cols - c);
+      r.h[k].load(p.h + o, cols - c);
+      if (p.grad_h) r.gh[k].load(p.grad_h + o, cols - c);
+    }
+  };
+  // whole rounds of rows: a group past the last row repeats it and leaves its results out
+  const int64_t mine = static_cast<int64_t>(blockIdx.x) * SIDE + t / LANES;
+  Row now, next;
+  fetch(mine < p.rows ? mine : p.rows - 1, now);
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * SIDE; base < p.rows; base += step) {
+    const int64_t row = base + t / LANES;
+    const bool there = row < p.rows;
+    if (base + step < p.rows) fetch(row + step < p.rows ? row + step : p.rows - 1, next);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (lane + k * LANES) * 8;
+      float g[8], h[8];
+      now.g[k].unpack(g);
+      now.h[k].unpack(h);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float z = c + e < cols ? (h[e] - now.mean) * now.rstd : 0.f;
+        const float a = g[e] * gamma[k][e];
+        s[0] += a;
+        s[1] += a * z;
+        if (there) {
+          dgamma[k][e] += g[e] * z;
+          dbeta[k][e] += g[e];
+        }
+      }
+    }
+    row_sums<LANES, 2>(s, s_red);
+    const float m0 = s[0] / n, m1 = s[1] / n;
+    if (there) {
+      const int64_t at = row * p.cols * Elem<T>::kBytes;
+      with_stream(p.stream_out, [&](auto st) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          const int c = (lane + k * LANES) * 8;
+          if (c < cols) {
+            float g[8], h[8], v[8];
+            now.g[k].unpack(g);
+            now.h[k].unpack(h);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float z = (h[e] - now.mean) * now.rstd;
+              v[e] = now.rstd * (g[e] * gamma[k][e] - m0 - z * m1);
+            }
+            if (p.grad_h) {
+              now.gh[k].unpack(g);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] += g[e];
+            }
+            if (p.dh) store8<T, decltype(st)::value>(p.dh + at + c * Elem<T>::kBytes, cols - c, v);
+            if (d.threshold) apply_dropout(d, static_cast<uint32_t>(row), static_cast<uint32_t>(c / 8), v);
+            store8<T, decltype(st)::value>(p.dx + at + c * Elem<T>::kBytes, cols - c, v);
+          }
+        }
+      });
+    }
+    now = next;
+  }
+  // the workgroup's sums: of the rows side by side through LDS, in their order
+  const int64_t width = ceil_div(p.cols, 8) * 8;
+  float* const out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * width;
+  if constexpr (SIDE > 1) {
+    const int wide = LANES * K * 8;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = (lane + k * LANES) * 8 + e;
+        s_acc[(t / LANES) * wide + c] = dgamma[k][e];
+        s_acc[(SIDE + t / LANES) * wide + c] = dbeta[k][e];
+      }
+    }
+    __syncthreads();
+    for (int i = t; i < 2 * wide; i += Block<LANES>::kThreads) {
+      const int which = i / wide, c = i % wide;
+      float sum = 0.f;
+      for (int r = 0; r < SIDE; ++r) sum += s_acc[(which * SIDE + r) * wide + c];
+      if (c < width) out[which * width + c] = sum;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (lane + k * LANES) * 8;
+      if (c < cols) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          *reinterpret_cast<float4*>(out + c + e) = make_float4(dgamma[k][e], dgamma[k][e + 1], dgamma[k][e + 2], dgamma[k][e + 3]);
+          *reinterpret_cast<float4*>(out + width + c + e) = make_float4(dbeta[k][e], dbeta[k][e + 1], dbeta[k][e + 2], dbeta[k][e + 3]);
+        }
+      }
+    }
+  }
+}
+
+// Rows of any width: the workgroup's sums lie in the workspace, where a thread adds its columns' row by row.
+template <typename T, typename PT>
+__global__ void __launch_bounds__(kWideThreads) train_norm_back_wide_kernel(const NormBackParams p) {
+  __shared__ float s_red[2 * kWideThreads / kWave];
+  const int64_t t = threadIdx.x;
+  const float n = static_cast<float>(p.cols);
+  Dropout d = p.drop;
+  if (d.threshold) load_state(d);
+  const int64_t width = ceil_div(p.cols, 8) * 8;
+  float* const out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * width;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    const bool first = row == static_cast<int64_t>(blockIdx.x);
+    float s[2] = {0.f, 0.f};
+    for (int64_t c = t * 8; c < p.cols; c += kWideThreads * 8) {
+      const int live = p.cols - c < 8 ? static_cast<int>(p.cols - c) : 8;
+      const int64_t at = (row * p.cols + c) * Elem<T>::kBytes;
+      float g[8], h[8], gamma[8];
+      load8<T>(p.g + at, live, g);
+      load8<T>(p.h + at, live, h);
+      load8<PT>(static_cast<const char*>(p.gamma) + c * Elem<PT>::kBytes, live, gamma);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float z = e < live ? (h[e] - mean) * rstd : 0.f, a = g[e] * gamma[e];
+        s[0] += a;
+        s[1] += a * z;
+        float* const sums = out + c + e;
+        sums[0] = (first ? 0.f : sums[0]) + g[e] * z;
+        sums[width] = (first ? 0.f : sums[width]) + g[e];
+      }
+    }
+    row_sums<kWideThreads, 2>(s, s_red);
+    const float m0 = s[0] / n, m1 = s[1] / n;
+    for (int64_t c = t * 8; c < p.cols; c += kWideThreads * 8) {
+      const int live = p.cols - c < 8 ? static_cast<int>(p.cols - c) : 8;
+      const int64_t at = (row * p.cols + c) * Elem<T>::kBytes;
+      float g[8], h[8], gamma[8], v[8];
+      load8<T>(p.g + at, live, g);
+      load8<T>(p.h + at, live, h);
+      load8<PT>(static_cast<const char*>(p.gamma) + c * Elem<PT>::kBytes, live, gamma);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = rstd * (g[e] * gamma[e] - m0 - (h[e] - mean) * rstd * m1);
+      if (p.grad_h) {
+        load8<T>(p.grad_h + at, live, g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += g[e];
+      }
+      if (p.dh) store8<T>(p.dh + at, live, v);
+      if (d.threshold) apply_dropout(d, static_cast<uint32_t>(row), static_cast<uint32_t>(c / 8), v);
+      store8<T>(p.dx + at, live, v);
+    }
+  }
+}
+
+// dgamma (blockIdx.y 0) and dbeta (1): the workgroups' sums, 16 of them side by side, then those in order.
+constexpr int kParamThreads = 256, kParamQuads = 16;
+template <typename PT>
+__global__ void __launch_bounds__(kParamThreads) train_norm_params_kernel(const float* partial, int workgroups, int64_t cols,
+                                                                          char* dgamma, char* dbeta) {
+  constexpr int ROWS = kParamThreads / kParamQuads;
+  __shared__ float4 s_sum[kParamThreads];
+  const int t = static_cast<int>(threadIdx.x), q = t % kParamQuads, r = t / kParamQuads;
+  const int64_t width = ceil_div(cols, 8) * 8, c = (static_cast<int64_t>(blockIdx.x) * kParamQuads + q) * 4;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (c < width) {
+    const float* const from = partial + static_cast<int64_t>(blockIdx.y) * width + c;
+#pragma unroll 4
+    for (int w = r; w < workgroups; w += ROWS) {
+      const float4 v = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(w) * 2 * width);
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+  }
+  s_sum[t] = sum;
+  __syncthreads();
+  if (r != 0 || c >= cols) return;
+  for (int i = 1; i < ROWS; ++i) {
+    const float4 v = s_sum[i * kParamQuads + q];
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+  }
+  const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+  store_vec<PT, 4>((blockIdx.y ? dbeta : dgamma) + c * Elem<PT>::kBytes, cols - c < 4 ? static_cast<int>(cols - c) : 4, v);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------------
+// f(LANES, K) for the register form of a width, as types.
+template <int V>
+using Const = std::integral_constant<int, V>;
+template <typename F>
+void with_form(const TrainNormForm& form, F&& f) {
+  if (form.lanes == 8) f(Const<8>{}, Const<1>{});
+  else if (form.lanes == 16) f(Const<16>{}, Const<1>{});
+  else if (form.lanes == 32) f(Const<32>{}, Const<1>{});
+  else if (form.lanes == 64 && form.chunks == 1) f(Const<64>{}, Const<1>{});
+  else if (form.lanes == 64) f(Const<64>{}, Const<2>{});
+  else if (form.lanes == 256 && form.chunks == 1) f(Const<256>{}, Const<1>{});
+  else if (form.lanes == 256 && form.chunks == 2) f(Const<256>{}, Const<2>{});
+  else if (form.lanes == 256) f(Const<256>{}, Const<4>{});
+  else f(Const<512>{}, Const<4>{});
+}
+
+int check_norm(int64_t rows, int64_t cols, int32_t dtype, int32_t param_dtype) {
+  if (rows < 0) return set_error(CTI_EBAG_EINVAL, "rows must be >= 0 (got %lld)", (long long)rows);
+  if (cols < 1) return set_error(CTI_EBAG_EINVAL, "cols must be >= 1 (got %lld)", (long long)cols);
+  if (!float_dtype(dtype)) return set_error(CTI_EBAG_EINVAL, "unknown dtype code %d", dtype);
+  if (!float_dtype(param_dtype)) return set_error(CTI_EBAG_EINVAL, "unknown parameter dtype code %d", param_dtype);
+  if (rows > INT32_MAX) return set_error(CTI_EBAG_EUNSUPPORTED, "more than 2^31 - 1 rows (%lld)", (long long)rows);
+  if (cols > INT32_MAX / 8) return set_error(CTI_EBAG_EUNSUPPORTED, "more than 2^28 - 1 columns (%lld)", (long long)cols);
+  return CTI_EBAG_OK;
+}
+
+}  // namespace
+}  // namespace cti
+
+using namespace cti;
+
+extern "C" int cti_ebag_dropout(const void* x, const void* residual, void* y, int64_t rows, int64_t cols, int32_t dtype, double p,
+                                uint64_t seed, uint64_t offset, const int64_t* state, void* stream) {
+  clear_error();
+  const int rc = check_norm(rows, cols, dtype, dtype);
+  if (rc != CTI_EBAG_OK) return rc;
+  DropParams a{};
+  if (!set_dropout(&a.drop, p, seed, offset, state)) return set_error(CTI_EBAG_EINVAL, "p must be in [0, 1] (got %g)", p);
+  if (rows == 0) return CTI_EBAG_OK;
+  if (!x || !y) return set_error(CTI_EBAG_EINVAL, "NULL device pointer among x/y");
+  const int64_t row_bytes = cols * dtype_bytes(dtype);
+  a.cols = cols;
+  a.per_row = static_cast<uint32_t>(ceil_div(cols, 8));
+  a.div = ChunkDivide::by(a.per_row);
+  a.stream_out = rows * row_bytes >= kStreamOutBytes;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const int64_t per_launch = kMostChunks / a.per_row;  // rows
+  for (int64_t r = 0; r < rows; r += per_launch) {
+    const int64_t now = rows - r < per_launch ? rows - r : per_launch;
+    a.x = static_cast<const char*>(x) + r * row_bytes;
+    a.res = residual ? static_cast<const char*>(residual) + r * row_bytes : nullptr;
+    a.y = static_cast<char*>(y) + r * row_bytes;
+    a.first_row = static_cast<uint32_t>(r);
+    a.chunks = static_cast<uint32_t>(now * a.per_row);
+    const dim3 grid((a.chunks + kDropThreads - 1) / kDropThreads), block(kDropThreads);
+    with_type(dtype, [&](auto t) { hipLaunchKernelGGL((dropout_kernel<decltype(t)>), grid, block, 0, s, a); });
+  }
+  return check_launch("dropout");
+}
+
+extern "C" int cti_ebag_dropout_layernorm(const void* x, const void* residual, void* h, void* y, int64_t rows, int64_t cols,
+                                          int32_t dtype, const void* gamma, const void* beta, int32_t param_dtype, float eps, double p,
+                                          uint64_t seed, uint64_t offset, const int64_t* state, float* mean, float* rstd,
+                                          void* stream) {
+  clear_error();
+  const int rc = check_norm(rows, cols, dtype, param_dtype);
+  if (rc != CTI_EBAG_OK) return rc;
+  if (!(eps >= 0.f)) return set_error(CTI_EBAG_EINVAL, "eps must be >= 0");
+  TrainNormParams a{};
+  if (!set_dropout(&a.drop, p, seed, offset, state)) return set_error(CTI_EBAG_EINVAL, "p must be in [0, 1] (got %g)", p);
+  const bool plain = !residual && a.drop.threshold == 0;
+  if (rows == 0) return CTI_EBAG_OK;
+  if (!x || !y || !gamma || !beta || !mean || !rstd)
+    return set_error(CTI_EBAG_EINVAL, "NULL device pointer among x/y/gamma/beta/mean/rstd");
+  if (!plain && !h) return set_error(CTI_EBAG_EINVAL, "h is NULL: a call with dropout or a residual writes it");
+  const int64_t row_bytes = cols * dtype_bytes(dtype);
+  a.gamma = gamma;
+  a.beta = beta;
+  a.cols = cols;
+  a.eps = eps;
+  a.stream_out = rows * row_bytes >= kStreamOutBytes;
+  const TrainNormForm form = train_norm_form(cols);
+  const int threads = form.lanes == 0 ? kWideThreads : form.lanes < 256 ? 256 : form.lanes;
+  const int side = form.lanes > 0 && form.lanes < 256 ? 256 / form.lanes : 1;
+  const int64_t per_launch = (int64_t{1} << 31) / threads * side;  // rows: below 2^32 threads
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  for (int64_t r = 0; r < rows; r += per_launch) {
+    a.rows = rows - r < per_launch ? rows - r : per_launch;
+    a.x = static_cast<const char*>(x) + r * row_bytes;
+    a.res = residual ? static_cast<const char*>(residual) + r * row_bytes : nullptr;
+    a.h = h ? static_cast<char*>(h) + r * row_bytes : nullptr;
+    a.y = static_cast<char*>(y) + r * row_bytes;
+    a.mean = mean + r;
+    a.rstd = rstd + r;
+    a.first_row = static_cast<uint32_t>(r);
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.rows, side))), block(threads);
+    with_types(dtype, param_dtype, [&](auto t, auto pt) {
+      using T = decltype(t);
+      using PT = decltype(pt);
+      if (form.lanes == 0) {
+        hipLaunchKernelGGL((train_norm_wide_kernel<T, PT>), grid, block, 0, s, a);
+      } else {
+        with_form(form, [&](auto lanes, auto k) {
+          hipLaunchKernelGGL((train_norm_kernel<T, PT, decltype(lanes)::value, decltype(k)::value>), grid, block, 0, s, a);
+        });
+      }
+    });
+  }
+  return check_launch("dropout_layernorm");
+}
+
+extern "C" int64_t cti_ebag_dropout_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols) {
+  return rows <= 0 || cols < 1 || rows > INT32_MAX || cols > INT32_MAX / 8 ? 0 : train_norm_workspace_bytes(rows, cols);
+}
+
+extern "C" int cti_ebag_dropout_layernorm_backward(const void* grad, const void* h, const void* grad_h, const float* mean,
+                                                   const float* rstd, int64_t rows, int64_t cols, int32_t dtype, const void* gamma,
+                                                   int32_t param_dtype, double p, uint64_t seed, uint64_t offset,
+                                                   const int64_t* state, void* dx, void* dresidual, void* dgamma, void* dbeta,
+                                                   void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  const int rc = check_norm(rows, cols, dtype, param_dtype);
+  if (rc != CTI_EBAG_OK) return rc;
+  NormBackParams a{};
+  if (!set_dropout(&a.drop, p, seed, offset, state)) return set_error(CTI_EBAG_EINVAL, "p must be in [0, 1] (got %g)", p);
+  if (!dgamma || !dbeta || (rows > 0 && (!grad || !h || !mean || !rstd || !gamma || !dx)))
+    return set_error(CTI_EBAG_EINVAL, "NULL device pointer among grad/h/mean/rstd/gamma/dx/dgamma/dbeta");
+  const int64_t need = train_norm_workspace_bytes(rows, cols);
+  if (rows > 0 && (!workspace || workspace_bytes < need))
+    return set_error(CTI_EBAG_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0),
+                     (long long)need);
+  if (rows > 0 && reinterpret_cast<uintptr_t>(workspace) % 16) return set_error(CTI_EBAG_EINVAL, "workspace is not 16-byte aligned");
+  a.g = static_cast<const char*>(grad);
+  a.h = static_cast<const char*>(h);
+  a.grad_h = static_cast<const char*>(grad_h);
+  a.mean = mean;
+  a.rstd = rstd;
+  a.gamma = gamma;
+  a.dh = static_cast<char*>(dresidual);
+  a.dx = static_cast<char*>(dx);
+  a.partial = static_cast<float*>(workspace);
+  a.rows = rows;
+  a.cols = cols;
+  a.stream_out = rows * cols * dtype_bytes(dtype) >= kStreamOutBytes;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const TrainNormForm form = train_norm_form(cols);
+  const int64_t workgroups = rows > 0 ? train_norm_workgroups(rows, cols) : 0;
+  const dim3 grid(static_cast<unsigned>(workgroups));
+  const dim3 block(form.lanes == 0 ? kWideThreads : form.lanes < 256 ? 256 : form.lanes);
+  if (rows > 0) {
+    with_types(dtype, param_dtype, [&](auto t, auto pt) {
+      using T = decltype(t);
+      using PT = decltype(pt);
+      if (form.lanes == 0) {
+        hipLaunchKernelGGL((train_norm_back_wide_kernel<T, PT>), grid, block, 0, s, a);
+      } else {
+        with_form(form, [&](auto lanes, auto k) {
+          hipLaunchKernelGGL((train_norm_back_kernel<T, PT, decltype(lanes)::value, decltype(k)::value>), grid, block, 0, s, a);
+        });
+      }
+    });
+  }
+  with_type(param_dtype, [&](auto pt) {
+    hipLaunchKernelGGL((train_norm_params_kernel<decltype(pt)>), dim3(static_cast<unsigned>(ceil_div(cols, kParamQuads * 4)), 2),
+                       dim3(kParamThreads), 0, s, a.partial, static_cast<int>(workgroups), cols, static_cast<char*>(dgamma),
+                       static_cast<char*>(dbeta));
+  });
+  return check_launch("dropout_layernorm_backward");
+}

@@ -1,0 +1,105 @@
+// Rules of the training operators that are arithmetic on sizes alone: plain C++, so that a test can hold them
+// against what the kernels behind them assume, without a GPU.
+#pragma once
+
+#include <stdint.h>
+
+#include <initializer_list>
+
+namespace cti {
+
+constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// n / d for n < 2^31 by one multiplication (Granlund and Montgomery, 1994): m = floor(2^(31 + s) / d) + 1 with
+// s = ceil(log2 d) is off by at most d <= 2^s, so n times that stays below 2^(31 + s).
+struct ChunkDivide {
+  uint32_t m, shift;
+  static constexpr ChunkDivide by(uint32_t d) {
+    uint32_t s = 0;
+    while (s < 32 && (uint64_t{1} << s) < d) ++s;
+    return {static_cast<uint32_t>((uint64_t{1} << (31 + s)) / d + 1), 31 + s};
+  }
+  constexpr uint32_t quotient(uint32_t n) const { return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> shift); }
+};
+
+constexpr int64_t kMostChunks = int64_t{1} << 30;  // of 8 columns, a launch
+
+constexpr int kGradTile = 4096;
+constexpr int64_t kGradMostIds = int64_t{1} << 30;        // ids and bags: 32-bit numbers, and launches below 2^32 threads
+constexpr int64_t kGradMostRows = (int64_t{1} << 31) - 1;  // rows of all tables are fewer: the number itself is a key
+constexpr int64_t kGradMostDim = int64_t{1} << 22;
+constexpr int64_t kGradTilesUnscanned = 256;
+constexpr int64_t kGradHeadsUnscanned = 4096;
+
+struct GradPlan {
+  int64_t tiles;
+  int bits, digit_bits;
+  int log_lanes, run, blocks;  // lanes of a group, ids of a group, blocks of 64 vectors of columns
+  int64_t workgroups;
+  int64_t key[2], unit[2], counts, totals, heads, last_rank, inv_len, partial, bytes;  // places in the workspace
+};
+
+// The gradient of n ids in tables of `rows` rows, the widest of `dim` columns; mean_bags: bags under mean pooling, else 0.
+inline GradPlan grad_plan(int64_t n, int64_t mean_bags, int64_t dim, int elem_bytes, uint32_t rows) {
+  GradPlan p{};
+  p.tiles = ceil_div(n, kGradTile);
+  while (p.bits < 32 && (rows >> p.bits)) ++p.bits;  // of the key `rows` itself
+  const int passes = (p.bits + 7) / 8;
+  p.digit_bits = (p.bits + passes - 1) / passes;
+  const int vec = 16 / elem_bytes;
+  const int64_t vectors = ceil_div(dim, vec);
+  while (p.log_lanes < 6 && (int64_t{1} << p.log_lanes) < vectors) ++p.log_lanes;
+  p.blocks = static_cast<int>(ceil_div(vectors, 64));
+  const int groups = 256 >> p.log_lanes;
+  p.run = 2048 / groups < 32 ? 2048 / groups : 32;
+  if (ceil_div(n, int64_t{groups} * p.run) * p.blocks < 1024) p.run = 8;
+  p.workgroups = ceil_div(n, int64_t{groups} * p.run);
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += ceil_div(bytes, 256) * 256;
+    return here;
+  };
+  for (int i = 0; i < 2; ++i) {
+    p.key[i] = take(n * 4);
+    p.unit[i] = take(n * 4);
+  }
+  p.counts = take(p.tiles * 1024);
+  p.totals = take(1024);
+  p.heads = take((p.workgroups + 1) * 4);
+  p.last_rank = take(p.workgroups * 4);
+  p.inv_len = take(mean_bags * 4);
+  p.partial = take(p.workgroups * p.blocks * 2 * (int64_t{vec} << p.log_lanes) * 4);
+  p.bytes = at;
+  return p;
+}
+
+// The register form of the norm with dropout: `lanes` threads hold a row, `chunks` chunks of 8 columns each (1, 2 or 4);
+// lanes 0: the loop form.
+struct TrainNormForm {
+  int lanes, chunks;
+};
+inline TrainNormForm train_norm_form(int64_t cols) {
+  const int64_t n = ceil_div(cols, 8);
+  for (const int lanes : {8, 16, 32, 64})
+    if (n <= lanes) return {lanes, 1};
+  if (n <= 128) return {64, 2};
+  if (n <= 256) return {256, 1};
+  if (n <= 512) return {256, 2};
+  if (n <= 1024) return {256, 4};
+  if (n <= 2048) return {512, 4};
+  return {0, 0};
+}
+// Workgroups of the norm's backward pass: each adds up gamma's and beta's gradients over its rows.
+inline int64_t train_norm_workgroups(int64_t rows, int64_t cols) {
+  const TrainNormForm f = train_norm_form(cols);
+  const int64_t side = f.lanes > 0 && f.lanes < 256 ? 256 / f.lanes : 1;  // rows side by side
+  const int64_t most = f.lanes == 0 ? 128 : 512;
+  const int64_t n = ceil_div(rows, side);
+  return n < most ? n : most;
+}
+inline int64_t train_norm_workspace_bytes(int64_t rows, int64_t cols) {
+  return rows <= 0 ? 0 : train_norm_workgroups(rows, cols) * 2 * ceil_div(cols, 8) * 8 * 4;
+}
+
+}  // namespace cti

@@ -9,7 +9,9 @@ and ``linear`` maps them to d_model (online_best/infer.py:1085). ``forward`` poo
 the pooled block in place and runs ``linear``; ``forward(batch, fused_linear=True)`` instead runs
 one matrix-core kernel that applies the LayerNorm to the pooled block's tiles as it loads them
 and multiplies them with the Linear's weight (``layer_norm_linear``, after ``layer_norm_stats``).
-Like the reference's Triton kernels, the pooling and the LayerNorm are forward-only (inference).
+Like the reference's Triton kernels, the pooling and the LayerNorm of these calls are forward-only
+(inference); ``forward_train`` is the same encoder with gradients for all of its parameters, and with
+dropout on the pooled block.
 
 ``quantize_int8_()`` is the reference's int8 switch (``_USE_INT8_EMB``, online_best/infer.py:893
 and :976-1026): the table is row-quantised once on the device and every later ``pooled`` reads
@@ -28,6 +30,7 @@ from .ops import (fused_all_slots_embedding, fused_all_slots_embedding_int8,
                   fused_all_slots_embedding_int8_layernorm, fused_all_slots_embedding_layernorm,
                   layer_norm, layer_norm_int8, layer_norm_linear, layer_norm_stats, linear_int8,
                   quantize_embedding_int8)
+from .training import dropout_add_layer_norm, fused_embedding_train
 
 
 class RepEncoder(nn.Module):
@@ -165,3 +168,18 @@ class RepEncoder(nn.Module):
         with torch.no_grad():
             fused_embs = layer_norm(fused_embs, norm.weight.detach(), norm.bias.detach(), norm.eps, out=fused_embs)
         return self.linear(fused_embs)
+
+    def forward_train(self, batch: dict, dropout: float = 0.0, seed=0, offset: int = 0, sparse_grad: bool = False) -> torch.Tensor:
+        """``linear(input_norm(dropout(pooled)))``, differentiable in the table, ``input_norm`` and ``linear``.
+
+        The table's gradient comes from the ids sorted on the device (0 for the embedding's ``padding_idx``, as
+        ``nn.Embedding`` defines it; the forward pass reads that row like any), whole or with ``sparse_grad`` as a
+        sparse tensor of the rows that occur. Dropout is the LayerNorm kernel's own, with ``seed`` and ``offset`` as in
+        ``dropout`` (give every step an offset of its own); nothing of it is stored. Without dropout the result is
+        ``forward``'s up to the order of the LayerNorm's sums."""
+        if self._int8_weight is not None or self._int8_linear is not None:
+            raise ValueError("an int8 encoder is not trained: dequantize_() and dequantize_linear_() first")
+        norm = self.input_norm
+        flat_values, val_offsets, flat_row_offsets, _ = self.flat_inputs(batch)
+        pooled = fused_embedding_train(flat_values, val_offsets, flat_row_offsets, self.emb.weight, self.emb.padding_idx, sparse_grad)
+        return self.linear(dropout_add_layer_norm(pooled, norm.weight, norm.bias, norm.eps, p=dropout, seed=seed, offset=offset)[0])

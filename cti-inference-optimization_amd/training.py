@@ -1,0 +1,646 @@
+"""Operators of a training step in front of and behind the encoder: the embedding lookup with a scale, the
+gradients of tables behind lookups and pooled bags, dropout, and the layer norm with dropout and the
+residual's addition in it.
+
+The reference's kernels are forward-only; what its modules would train is what torch's do
+(``nn.Embedding`` with ``padding_idx`` and ``nn.LayerNorm``, online_best/infer.py:948-950), and the
+gradients here are theirs. Each operator comes as plain calls, forward and backward, that a training
+loop or a captured graph makes itself (``embedding_lookup_backward``, ``embedding_bag_backward``,
+``fused_all_slots_embedding_backward``, ``dropout_backward``, ``dropout_add_layer_norm_backward``), and
+``embedding_lookup``, ``dropout``, ``dropout_add_layer_norm``, ``embedding_bag_train`` and
+``fused_embedding_train`` take part in autograd by themselves where an input requires a gradient.
+
+Gradients of tables come whole, or as the rows that occur (``compact``): ``rows`` (their numbers, ascending,
+then -1), their sums and how many they are, all on the device, so that nothing waits for the count. The ids
+are sorted for it and no sum is taken by atomics: results are the same bits in every run.
+
+Dropout's mask is a function of seed, offset, row and column that both directions compute: nothing is stored.
+A training loop gives each layer and step an offset of its own. ``seed`` may be an int64 tensor of two
+numbers on the device, (seed, offset), to which the call's own offset is added: for captured graphs, which
+replay the numbers that a call was given but read what lies in the tensor.
+
+Arguments are validated on the host (no device synchronisation): ``ValueError`` / ``TypeError`` for
+malformed calls, ``EbagError`` when the C ABI reports a failure. Everything runs on torch's current stream;
+workspaces come from torch's allocator for the call.
+"""
+from __future__ import annotations
+
+import functools
+from typing import Optional, Sequence
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _capi
+from .ops import (_check_flat_layout, _check_output, _launch, _require_on, _same_offset_type, _table_descs,
+                  embedding_bag_pooled, fused_all_slots_embedding)
+
+_INDEX_TYPES = (torch.int64, torch.int32)
+
+
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _check_index(name: str, t: torch.Tensor, index: Optional[int] = None) -> int:
+    index = _require_on(name, t, index)
+    if t.dtype not in _INDEX_TYPES:
+        raise TypeError(f"{name} must be int64 or int32 (got {t.dtype})")
+    return index
+
+
+def _check_padding(padding_idx: Optional[int], rows: int) -> int:
+    if padding_idx is None:
+        return -1
+    if not 0 <= padding_idx < rows:
+        raise ValueError(f"padding_idx {padding_idx} outside [0, {rows - 1}]")
+    return int(padding_idx)
+
+
+def _check_dim(dim: int) -> None:
+    if dim >= 2 ** 31:  # ctypes drops the bits above
+        raise _capi.EbagError(_capi.EUNSUPPORTED, f"dim {dim} >= 2^31")
+
+
+# ------------------------------------------------------------------------------------------------
+# Lookup
+# ------------------------------------------------------------------------------------------------
+def _lookup(ids, weight, scale, out, out_dtype):
+    if not isinstance(weight, torch.Tensor) or not weight.is_cuda:
+        _require_on("weight", weight)
+    index = weight.get_device()
+    _check_index("ids", ids, index)
+    if weight.dim() != 2 or weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
+        raise ValueError("weight must be a row-major 2-D tensor with unit column stride")
+    rows, dim = weight.shape
+    if rows < 1 or dim < 1:
+        raise ValueError(f"weight has shape {tuple(weight.shape)}: no rows or no columns")
+    _check_dim(dim)
+    code = _capi.dtype_code(weight.dtype)
+    shape = (*ids.shape, dim)
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype or weight.dtype, device=weight.device)
+    else:
+        _check_output("out", out, shape, out_dtype or out.dtype, index)
+    _launch(index, _capi.lib().cti_ebag_lookup, ids.data_ptr(), _capi.index_code(ids.dtype), ids.numel(), weight.data_ptr(), code,
+            rows, weight.stride(0), dim, scale, out.data_ptr(), _capi.dtype_code(out.dtype))
+    return out
+
+
+class _Lookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding_idx, out_dtype, sparse_grad):
+        ctx.save_for_backward(ids)
+        ctx.info = (weight.shape[0], weight.shape[1], weight.dtype, scale, padding_idx, sparse_grad)
+        return _lookup(ids, weight, scale, None, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        ids, = ctx.saved_tensors
+        rows, dim, dtype, scale, padding_idx, sparse_grad = ctx.info
+        got = embedding_lookup_backward(grad.contiguous(), ids, rows, scale, padding_idx, grad_dtype=dtype, compact=sparse_grad)
+        return (_sparse(got, rows, dim) if sparse_grad else got), None, None, None, None, None
+
+
+def _sparse(got, rows: int, dim: int) -> torch.Tensor:
+    """Compact rows as a sparse tensor of torch; waits for their count."""
+    numbers, sums, count = got
+    n = int(count.item())
+    return torch.sparse_coo_tensor(numbers[:n].unsqueeze(0), sums[:n], (rows, dim), is_coalesced=True, check_invariants=False)
+
+
+def embedding_lookup(
+    ids: torch.Tensor,
+    weight: torch.Tensor,
+    scale: float = 1.0,
+    padding_idx: Optional[int] = None,
+    out: Optional[torch.Tensor] = None,
+    out_dtype: Optional[torch.dtype] = None,
+    sparse_grad: bool = False,
+) -> torch.Tensor:
+    """Rows of a table, scaled: ``out[..., :] = scale * weight[clamp(ids[...], 0, rows - 1)]`` in fp32, rounded
+    once to ``out_dtype`` (the table's type by default; or ``out``'s).
+
+    ``ids`` int64 or int32 of any shape, contiguous; ``weight`` ``[rows, dim]`` fp32 / bf16 / fp16 with unit
+    column stride. Ids outside the table are clamped, as everywhere in this package. Returns ``out`` of shape
+    ``ids.shape + (dim,)``; ``out`` overlaps no input.
+
+    Differentiable in ``weight`` (``out`` must then be None): the gradient is ``embedding_lookup_backward``'s,
+    0 for row ``padding_idx``, which the lookup itself reads like any row. With ``sparse_grad`` it is a
+    sparse tensor of the rows that occur, each once, whose making waits for their count (not within a captured graph).
+    """
+    scale = float(scale)
+    if _needs_grad(weight):
+        if out is not None:
+            raise ValueError("out does not combine with a gradient: detach the weight or leave out None")
+        if isinstance(weight, torch.Tensor) and weight.dim() == 2:
+            _check_padding(padding_idx, weight.shape[0])
+        return _Lookup.apply(weight, ids, scale, padding_idx, out_dtype, sparse_grad)
+    return _lookup(ids, weight, scale, out, out_dtype)
+
+
+# ------------------------------------------------------------------------------------------------
+# Gradients of tables
+# ------------------------------------------------------------------------------------------------
+@functools.lru_cache(maxsize=4096)
+def _backward_workspace(nnz: int, bags: int, rows: int, dim: int, pooling: int) -> int:
+    return _capi.lib().cti_ebag_backward_workspace_bytes(nnz, bags, rows, dim, pooling)
+
+
+def _workspace(nnz, bags, rows, dim, pooling, device):
+    """(the workspace, its address, its bytes); kept alive until the launches are enqueued."""
+    size = _backward_workspace(nnz, bags, rows, dim, pooling)
+    if size <= 0:
+        return None, None, 0
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), size
+
+
+def _compact_output(out, nnz: int, rows: int, dim: int, dtype, device, index: int):
+    """Buffers of the compact form, checked or new: (numbers, sums, count), and their capacity."""
+    need = max(1, min(nnz, rows))
+    if out is None:
+        return (torch.empty(need, dtype=torch.int64, device=device), torch.empty(need, dim, dtype=dtype, device=device),
+                torch.empty(1, dtype=torch.int64, device=device)), need
+    if not isinstance(out, (tuple, list)) or len(out) != 3:
+        raise ValueError("out of the compact form is (rows, grads, count)")
+    numbers, sums, count = out
+    _require_on("out[0] (rows)", numbers, index)
+    if numbers.dim() != 1 or numbers.dtype != torch.int64 or numbers.numel() < need:
+        raise ValueError(f"out[0] (rows) must be 1-D int64 with at least {need} entries")
+    _check_output("out[1] (grads)", sums, (numbers.numel(), dim), dtype or sums.dtype, index)
+    _check_output("out[2] (count)", count, (1,), torch.int64, index)
+    return (numbers, sums, count), numbers.numel()
+
+
+def embedding_lookup_backward(
+    grad: torch.Tensor,
+    ids: torch.Tensor,
+    num_rows: int,
+    scale: float = 1.0,
+    padding_idx: Optional[int] = None,
+    grad_dtype: Optional[torch.dtype] = None,
+    compact: bool = False,
+    out=None,
+):
+    """The gradient of ``embedding_lookup``'s table of ``num_rows`` rows: row v is ``scale`` times the sum of
+    ``grad``'s rows whose id, clamped, is v; row ``padding_idx`` is 0.
+
+    ``grad`` ``ids.shape + (dim,)`` fp32 / bf16 / fp16, contiguous. Sums in fp32, in an order that the sizes alone
+    fix, rounded once to ``grad_dtype`` (``grad``'s type by default; or ``out``'s). Returns ``[num_rows, dim]``
+    (``out``), or with ``compact`` ``(rows, grads, count)``: the numbers of the rows that occur, ascending, then -1;
+    their sums, where what lies behind the last row is left as it was; and how many they are, int64 ``[1]``. There
+    ``out`` is a tuple of three such buffers of any capacity of at least ``min(ids, num_rows)`` (and 1) rows.
+    Nothing waits for the device. ``out`` overlaps no input.
+    """
+    index = _require_on("grad", grad)
+    _check_index("ids", ids, index)
+    if grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape or grad.shape[-1] < 1:
+        raise ValueError(f"grad has shape {tuple(grad.shape)}, expected {tuple(ids.shape)} and columns")
+    dim, n, num_rows = grad.shape[-1], ids.numel(), int(num_rows)
+    _check_dim(dim)
+    if num_rows < 1:
+        raise ValueError(f"num_rows must be >= 1, got {num_rows}")
+    padding = _check_padding(padding_idx, num_rows)
+    code = _capi.dtype_code(grad.dtype)
+    numbers = count = None
+    capacity = 0
+    if compact:
+        got, capacity = _compact_output(out, n, num_rows, dim, grad_dtype or (grad.dtype if out is None else None), grad.device, index)
+        numbers, out, count = got
+    elif out is None:
+        out = torch.empty(num_rows, dim, dtype=grad_dtype or grad.dtype, device=grad.device)
+    else:
+        _check_output("out", out, (num_rows, dim), grad_dtype or out.dtype, index)
+    ws, ws_ptr, ws_bytes = _workspace(n, n, num_rows, dim, _capi.SUM, grad.device)
+    _launch(index, _capi.lib().cti_ebag_lookup_backward, grad.data_ptr(), code, ids.data_ptr(), _capi.index_code(ids.dtype), n,
+            num_rows, dim, float(scale), padding, out.data_ptr(), _capi.dtype_code(out.dtype),
+            numbers.data_ptr() if compact else None, count.data_ptr() if compact else None, capacity, ws_ptr, ws_bytes)
+    return (numbers, out, count) if compact else out
+
+
+def fused_all_slots_embedding_backward(
+    grad: torch.Tensor,
+    flat_values: torch.Tensor,
+    val_offsets: torch.Tensor,
+    flat_row_offsets: torch.Tensor,
+    batch_size: int,
+    emb_dim: int,
+    max_idx: int,
+    pooling: str = "sum",
+    padding_idx: Optional[int] = None,
+    grad_dtype: Optional[torch.dtype] = None,
+    compact: bool = False,
+    out=None,
+):
+    """The gradient of ``fused_all_slots_embedding``'s table (``max_idx + 1`` rows), given ``grad`` ``[B,
+    S*emb_dim]``, the gradient of its output: row v is the sum over ids that are v, clamped, of their bag's part of
+    ``grad`` (under ``pooling="mean"`` divided by the bag's length); row ``padding_idx`` is 0.
+
+    The batch's arguments as ``fused_all_slots_embedding`` takes them; the bags lie in ``flat_values`` in the order of
+    slots and samples, as ``collate_flat_layout``, ``pack_slots`` and ``merge_batches`` lay them out (a batch whose
+    offsets descend gives unspecified sums). The rest as in ``embedding_lookup_backward``.
+    """
+    index = _require_on("grad", grad)
+    icode, ocode = _check_flat_layout(flat_values, val_offsets, flat_row_offsets, grad, grad.device)
+    val_offsets = _same_offset_type(val_offsets, flat_row_offsets, flat_values.numel())
+    batch_size, emb_dim, max_idx = int(batch_size), int(emb_dim), int(max_idx)
+    slots, n = val_offsets.numel(), flat_values.numel()
+    if batch_size < 0 or emb_dim < 1 or max_idx < 0:
+        raise ValueError(f"batch_size {batch_size}, emb_dim {emb_dim}, max_idx {max_idx}: expected >= 0, >= 1, >= 0")
+    _check_dim(emb_dim)
+    if flat_row_offsets.numel() != slots * (batch_size + 1):
+        raise ValueError(f"flat_row_offsets has {flat_row_offsets.numel()} entries, expected {slots} * ({batch_size} + 1)")
+    if tuple(grad.shape) != (batch_size, slots * emb_dim):
+        raise ValueError(f"grad has shape {tuple(grad.shape)}, expected ({batch_size}, {slots * emb_dim})")
+    padding = _check_padding(padding_idx, max_idx + 1)
+    code, pool = _capi.dtype_code(grad.dtype), _capi.pooling_code(pooling)
+    numbers = count = None
+    capacity = 0
+    if compact:
+        got, capacity = _compact_output(out, n, max_idx + 1, emb_dim, grad_dtype or (grad.dtype if out is None else None), grad.device,
+                                        index)
+        numbers, out, count = got
+    elif out is None:
+        out = torch.empty(max_idx + 1, emb_dim, dtype=grad_dtype or grad.dtype, device=grad.device)
+    else:
+        _check_output("out", out, (max_idx + 1, emb_dim), grad_dtype or out.dtype, index)
+    ws, ws_ptr, ws_bytes = _workspace(n, batch_size * slots, max_idx + 1, emb_dim, pool, grad.device)
+    _launch(index, _capi.lib().cti_ebag_fused_all_slots_backward, grad.data_ptr(), code, flat_values.data_ptr(), icode,
+            val_offsets.data_ptr(), flat_row_offsets.data_ptr(), ocode, batch_size, slots, emb_dim, max_idx, n, pool, padding,
+            out.data_ptr(), _capi.dtype_code(out.dtype), numbers.data_ptr() if compact else None,
+            count.data_ptr() if compact else None, capacity, ws_ptr, ws_bytes)
+    return (numbers, out, count) if compact else out
+
+
+def embedding_bag_backward(
+    grad: torch.Tensor,
+    values: torch.Tensor,
+    offsets: torch.Tensor,
+    tables: Sequence[torch.Tensor],
+    pooling: str = "sum",
+    padding_idx: Optional[int] = None,
+    grad_dtype: Optional[torch.dtype] = None,
+    compact: bool = False,
+    out=None,
+):
+    """The gradients of ``embedding_bag_pooled``'s tables, given ``grad`` ``[B, sum(D_f)]``, the gradient of its
+    output. ``values``, ``offsets`` and ``tables`` as that call takes them (offsets ascend; tables are float tensors,
+    of which only shape, type and identity are read; at most 64).
+
+    Returns a list with the gradient ``[V_f, D_f]`` of each field's table, of ``grad_dtype`` (the tables' type by
+    default); fields that share a table (the same tensor) share its gradient (the same tensor). ``out``: such a list.
+    With ``compact`` (tables of one width) ``(rows, grads, count)`` as in ``embedding_lookup_backward``, where row r
+    of a table has the number (rows of the tables before it, shared ones counted once) + r. ``padding_idx`` is every
+    table's.
+    """
+    index = _require_on("grad", grad)
+    dev = grad.device
+    descs, table_dev, code, width, dtype = _table_descs(tables)
+    if code == _capi.I8:
+        raise TypeError("int8 tables have no gradient")
+    if table_dev != dev:
+        raise ValueError(f"tables are on {table_dev}, grad on {dev}")
+    _check_index("values", values, index)
+    _require_on("offsets", offsets, index)
+    fields = len(tables)
+    if offsets.dtype != torch.int64:
+        raise TypeError(f"offsets must be int64 (got {offsets.dtype})")
+    if offsets.numel() < 1 or (offsets.numel() - 1) % fields:
+        raise ValueError(f"offsets has {offsets.numel()} entries; expected F*B+1 with F={fields}")
+    batch = (offsets.numel() - 1) // fields
+    if tuple(grad.shape) != (batch, width):
+        raise ValueError(f"grad has shape {tuple(grad.shape)}, expected ({batch}, {width})")
+    if width >= 2 ** 31:
+        raise _capi.EbagError(_capi.EUNSUPPORTED, f"{width} columns >= 2^31")
+    pool = _capi.pooling_code(pooling)
+    first = {}  # a table's identity -> the first field that has it
+    same = []
+    for f, t in enumerate(tables):
+        same.append(first.setdefault((t.data_ptr(), tuple(t.shape), t.stride()), f))
+    padding = min(_check_padding(padding_idx, t.shape[0]) for t in tables)
+    rows = sum(tables[f].shape[0] for f in set(same))
+    dim = max(t.shape[1] for t in tables)
+    odt = grad_dtype or dtype
+    n = values.numel()
+    numbers = sums = count = None
+    capacity = 0
+    if compact:
+        got, capacity = _compact_output(out, n, rows, dim, odt, dev, index)
+        numbers, sums, count = got
+        grads = None
+        for f in range(fields):  # tells tables apart, even those without rows of their own in memory
+            descs[f].data = same[f] + 1
+            descs[f].row_stride = descs[f].dim
+    else:
+        if out is None:
+            made = {f: torch.empty(tuple(tables[f].shape), dtype=odt, device=dev) for f in set(same)}
+            grads = [made[f] for f in same]
+        else:
+            grads = list(out)
+            if len(grads) != fields:
+                raise ValueError(f"out has {len(grads)} tensors for {fields} tables")
+            for f, g in enumerate(grads):
+                _check_output(f"out[{f}]", g, tuple(tables[f].shape), odt, index)
+                if (g.data_ptr() == grads[same[f]].data_ptr()) is False:
+                    raise ValueError(f"out[{f}] and out[{same[f]}] are gradients of one table: expected one tensor")
+            if len({g.data_ptr() for g in grads}) != len(set(same)):
+                raise ValueError("out: gradients of different tables share memory")
+        for f, g in enumerate(grads):
+            descs[f].data, descs[f].row_stride = g.data_ptr(), g.shape[1]
+    ws, ws_ptr, ws_bytes = _workspace(n, batch * fields, rows, dim, pool, dev)
+    _launch(index, _capi.lib().cti_ebag_backward, grad.data_ptr(), _capi.dtype_code(grad.dtype), width, values.data_ptr(),
+            _capi.index_code(values.dtype), n, offsets.data_ptr(), batch, fields, descs, pool, padding,
+            _capi.dtype_code(sums.dtype if compact else odt), sums.data_ptr() if compact else None,
+            numbers.data_ptr() if compact else None, count.data_ptr() if compact else None, capacity, ws_ptr, ws_bytes)
+    return (numbers, sums, count) if compact else grads
+
+
+class _PooledTables(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, values, offsets, pooling, padding_idx, out_dtype, *tables):
+        ctx.save_for_backward(values, offsets, *tables)
+        ctx.info = (pooling, padding_idx)
+        return embedding_bag_pooled(values, offsets, tables, pooling, out_dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        values, offsets, *tables = ctx.saved_tensors
+        grads = embedding_bag_backward(grad.contiguous(), values, offsets, tables, ctx.info[0], ctx.info[1])
+        seen = set()
+        for f, g in enumerate(grads):  # autograd adds up the fields' gradients of one table: its sum is in the first
+            if g.data_ptr() in seen:
+                grads[f] = None
+            seen.add(g.data_ptr())
+        return (None, None, None, None, None, *grads)
+
+
+def embedding_bag_train(
+    values: torch.Tensor,
+    offsets: torch.Tensor,
+    tables: Sequence[torch.Tensor],
+    pooling: str = "sum",
+    padding_idx: Optional[int] = None,
+    out_dtype: Optional[torch.dtype] = None,
+) -> torch.Tensor:
+    """``embedding_bag_pooled`` of float tables, differentiable in them (``embedding_bag_backward``)."""
+    for t in tables:
+        _check_padding(padding_idx, t.shape[0])
+    return _PooledTables.apply(values, offsets, pooling, padding_idx, out_dtype, *tables)
+
+
+class _PooledShared(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, flat_values, val_offsets, flat_row_offsets, batch_size, padding_idx, sparse_grad):
+        ctx.save_for_backward(flat_values, val_offsets, flat_row_offsets)
+        rows, dim = weight.shape
+        ctx.info = (rows, dim, batch_size, padding_idx, sparse_grad)
+        out = torch.empty(batch_size, val_offsets.numel() * dim, dtype=weight.dtype, device=weight.device)
+        return fused_all_slots_embedding(flat_values, val_offsets, flat_row_offsets, weight, out, batch_size, dim, rows - 1)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        rows, dim, batch_size, padding_idx, sparse_grad = ctx.info
+        got = fused_all_slots_embedding_backward(grad.contiguous(), *ctx.saved_tensors, batch_size, dim, rows - 1,
+                                                 padding_idx=padding_idx, compact=sparse_grad)
+        return (_sparse(got, rows, dim) if sparse_grad else got), None, None, None, None, None, None
+
+
+def fused_embedding_train(
+    flat_values: torch.Tensor,
+    val_offsets: torch.Tensor,
+    flat_row_offsets: torch.Tensor,
+    weight: torch.Tensor,
+    padding_idx: Optional[int] = None,
+    sparse_grad: bool = False,
+) -> torch.Tensor:
+    """The fused step of a flat-layout batch, ``[B, S*D]`` as ``fused_all_slots_embedding`` pools it, differentiable in
+    the table (``fused_all_slots_embedding_backward``; ``padding_idx`` and ``sparse_grad`` as in
+    ``embedding_lookup``)."""
+    slots = val_offsets.numel()
+    if slots < 1 or flat_row_offsets.numel() % slots:
+        raise ValueError(f"flat_row_offsets has {flat_row_offsets.numel()} entries for {slots} slots")
+    _check_padding(padding_idx, weight.shape[0])
+    return _PooledShared.apply(weight, flat_values, val_offsets, flat_row_offsets, flat_row_offsets.numel() // slots - 1, padding_idx,
+                               sparse_grad)
+
+
+# ------------------------------------------------------------------------------------------------
+# Dropout
+# ------------------------------------------------------------------------------------------------
+def _check_seed(p, seed, offset, index: int):
+    """(p, seed, offset, the state's address) as the library takes them."""
+    p, offset = float(p), int(offset)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"p must be in [0, 1], got {p}")
+    if not 0 <= offset < 2 ** 64:
+        raise ValueError(f"offset must be in [0, 2^64), got {offset}")
+    if isinstance(seed, torch.Tensor):
+        _require_on("seed", seed, index)
+        if seed.dtype != torch.int64 or seed.numel() != 2:
+            raise ValueError(f"seed must be an int or an int64 tensor of 2 (seed, offset), got {tuple(seed.shape)} {seed.dtype}")
+        return p, 0, offset, seed.data_ptr()
+    seed = int(seed)
+    if not 0 <= seed < 2 ** 64:
+        raise ValueError(f"seed must be in [0, 2^64), got {seed}")
+    return p, seed, offset, None
+
+
+def _rows_of(name: str, x) -> tuple:
+    """(device index, type code, rows, columns) of a contiguous tensor of rows."""
+    index = _require_on(name, x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name} must have columns, got shape {tuple(x.shape)}")
+    return index, _capi.dtype_code(x.dtype), x.numel() // x.shape[-1], x.shape[-1]
+
+
+def _check_like(name: str, t, x, index: int) -> int:
+    _require_on(name, t, index)
+    if t.shape != x.shape or t.dtype != x.dtype:
+        raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype}, got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr()
+
+
+def _dropout(x, p, seed, offset, residual, out):
+    index, code, rows, cols = _rows_of("x", x)
+    p, seed, offset, state = _check_seed(p, seed, offset, index)
+    res = None if residual is None else _check_like("residual", residual, x, index)
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _check_like("out", out, x, index)
+    _launch(index, _capi.lib().cti_ebag_dropout, x.data_ptr(), res, out.data_ptr(), rows, cols, code, p, seed, offset, state)
+    return out
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset):
+        ctx.state = None if isinstance(seed, torch.Tensor) else (p, seed, offset)
+        if ctx.state is None:
+            ctx.save_for_backward(seed)
+            ctx.rest = (p, offset)
+        return _dropout(x, p, seed, offset, residual, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        p, seed, offset = ctx.state or (ctx.rest[0], ctx.saved_tensors[0], ctx.rest[1])
+        dx = _dropout(grad.contiguous(), p, seed, offset, None, None) if ctx.needs_input_grad[0] else None
+        return dx, (grad if ctx.needs_input_grad[1] else None), None, None, None
+
+
+def dropout(
+    x: torch.Tensor,
+    p: float,
+    seed,
+    offset: int = 0,
+    residual: Optional[torch.Tensor] = None,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``residual + (kept ? x / (1 - p) : 0)`` in fp32, rounded once to x's type; without a residual the dropout alone.
+
+    ``x`` (fp32 / bf16 / fp16, contiguous, any shape; its last dimension are the columns, the others the rows) is kept
+    where 16 bits of Philox4x32-10 with key ``seed`` and counter (row, column / 8, ``offset``) reach
+    ``t = round(65536 p)``; p counts as t / 65536, for the factor too. Dropped elements give 0 whatever x is (NaN too).
+    ``seed`` is a number below 2^64, or an int64 tensor (seed, offset) on the device. ``out`` may be x or residual.
+    Differentiable in ``x`` and ``residual`` (``out`` must then be None); the mask is made again for it, not stored.
+    """
+    if _needs_grad(x, residual):
+        if out is not None:
+            raise ValueError("out does not combine with a gradient: detach the inputs or leave out None")
+        return _Dropout.apply(x, residual, p, seed, offset)
+    return _dropout(x, p, seed, offset, residual, out)
+
+
+def dropout_backward(grad: torch.Tensor, p: float, seed, offset: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The gradient of ``dropout``'s ``x`` (that of its residual is ``grad`` itself); ``out`` may be ``grad``."""
+    return _dropout(grad, p, seed, offset, None, out)
+
+
+# ------------------------------------------------------------------------------------------------
+# Layer norm
+# ------------------------------------------------------------------------------------------------
+def _check_param(name: str, t, cols: int, index: int):
+    _require_on(name, t, index)
+    if t.numel() != cols:
+        raise ValueError(f"{name} has {t.numel()} elements, expected {cols}")
+
+
+def _threshold(p: float) -> int:
+    return int(p * 65536.0 + 0.5)
+
+
+def _norm(x, weight, bias, eps, residual, p, seed, offset):
+    index, code, rows, cols = _rows_of("x", x)
+    _check_param("weight", weight, cols, index)
+    _check_param("bias", bias, cols, index)
+    if weight.dtype != bias.dtype:
+        raise TypeError(f"weight and bias dtypes differ ({weight.dtype} vs {bias.dtype})")
+    p, seed, offset, state = _check_seed(p, seed, offset, index)
+    res = None if residual is None else _check_like("residual", residual, x, index)
+    y = torch.empty_like(x)
+    h = torch.empty_like(x) if residual is not None or _threshold(p) else None
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    _launch(index, _capi.lib().cti_ebag_dropout_layernorm, x.data_ptr(), res, None if h is None else h.data_ptr(), y.data_ptr(), rows,
+            cols, code, weight.data_ptr(), bias.data_ptr(), _capi.dtype_code(weight.dtype), eps, p, seed, offset, state,
+            mean.data_ptr(), rstd.data_ptr())
+    return y, h, mean, rstd
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, p, seed, offset):
+        y, h, mean, rstd = _norm(x, weight, bias, eps, residual, p, seed, offset)
+        on_device = isinstance(seed, torch.Tensor)
+        ctx.save_for_backward(x if h is None else h, mean, rstd, weight, *((seed,) if on_device else ()))
+        ctx.info = (p, None if on_device else seed, offset, residual is not None, h is not None)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(mean, rstd)
+        return (y, mean, rstd) if h is None else (y, mean, rstd, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _mean, _rstd, grad_h=None):
+        h, mean, rstd, weight, *rest = ctx.saved_tensors
+        p, seed, offset, residual, _ = ctx.info
+        grad = torch.zeros_like(h) if grad is None else grad.contiguous()
+        dx, dweight, dbias, dres = dropout_add_layer_norm_backward(
+            grad, h, mean, rstd, weight, None if grad_h is None else grad_h.contiguous(), residual, p, rest[0] if rest else seed, offset)
+        return dx, dres, dweight.view_as(weight), dbias.view_as(weight), None, None, None, None
+
+
+def dropout_add_layer_norm(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    bias: torch.Tensor,
+    eps: float = 1e-5,
+    residual: Optional[torch.Tensor] = None,
+    p: float = 0.0,
+    seed=0,
+    offset: int = 0,
+):
+    """``h = residual + dropout(x, p, seed, offset)`` (rounded to x's type) and its LayerNorm in one pass over memory.
+
+    ``x`` (and ``residual``) ``[..., cols]`` fp32 / bf16 / fp16, contiguous, ``weight`` and ``bias`` ``[cols]`` of one of
+    these types. Returns ``(y, h, mean, rstd)``: ``y = (h - mean) * rstd * weight + bias`` of h as it is stored, rounded
+    once; ``mean`` and ``rstd`` fp32, one a row. Without dropout and residual h is x itself. ``p``, ``seed`` and
+    ``offset`` as in ``dropout``. Differentiable in x, residual, weight and bias, through y and h.
+    """
+    eps = float(eps)
+    if _needs_grad(x, residual, weight, bias):
+        y, mean, rstd, *h = _Norm.apply(x, residual, weight, bias, eps, p, seed, offset)
+        return y, (h[0] if h else x), mean, rstd
+    y, h, mean, rstd = _norm(x, weight, bias, eps, residual, p, seed, offset)
+    return y, (x if h is None else h), mean, rstd
+
+
+@functools.lru_cache(maxsize=4096)
+def _norm_workspace(rows: int, cols: int) -> int:
+    return _capi.lib().cti_ebag_dropout_layernorm_backward_workspace_bytes(rows, cols)
+
+
+def dropout_add_layer_norm_backward(
+    grad: torch.Tensor,
+    h: torch.Tensor,
+    mean: torch.Tensor,
+    rstd: torch.Tensor,
+    weight: torch.Tensor,
+    grad_h: Optional[torch.Tensor] = None,
+    residual: bool = False,
+    p: float = 0.0,
+    seed=0,
+    offset: int = 0,
+):
+    """The gradients of ``dropout_add_layer_norm``: ``grad`` is that of y, ``grad_h`` what arrives at h itself (the
+    residual stream's, or None), ``h``, ``mean`` and ``rstd`` are what it returned. Returns ``(dx, dweight, dbias,
+    dresidual)``; ``dresidual`` is None unless ``residual`` is set, and dx itself without dropout. dweight and dbias
+    are summed in fp32 over the rows, in a fixed order, and rounded once to the weight's type.
+    """
+    index, code, rows, cols = _rows_of("h", h)
+    _check_like("grad", grad, h, index)
+    gh = None if grad_h is None else _check_like("grad_h", grad_h, h, index)
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        _require_on(name, t, index)
+        if t.dtype != torch.float32 or t.numel() != rows:
+            raise ValueError(f"{name} must be a contiguous float32 tensor of {rows} elements")
+    _check_param("weight", weight, cols, index)
+    p, seed, offset, state = _check_seed(p, seed, offset, index)
+    param = _capi.dtype_code(weight.dtype)
+    dx = torch.empty_like(h)
+    dres = None
+    if residual:
+        dres = torch.empty_like(h) if _threshold(p) else dx
+    dweight = torch.empty(cols, dtype=weight.dtype, device=h.device)
+    dbias = torch.empty_like(dweight)
+    size = _norm_workspace(rows, cols)
+    ws = torch.empty(size, dtype=torch.uint8, device=h.device) if size > 0 else None
+    _launch(index, _capi.lib().cti_ebag_dropout_layernorm_backward, grad.data_ptr(), h.data_ptr(), gh, mean.data_ptr(), rstd.data_ptr(),
+            rows, cols, code, weight.data_ptr(), param, p, seed, offset, state, dx.data_ptr(),
+            dres.data_ptr() if dres is not None and dres is not dx else None, dweight.data_ptr(), dbias.data_ptr(),
+            None if ws is None else ws.data_ptr(), size)
+    return dx, dweight, dbias, dres

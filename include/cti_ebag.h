@@ -535,6 +535,111 @@ int64_t cti_ebag_linear_int8_workspace_bytes(int64_t rows, int32_t cols, int32_t
 /* The same where q or weight starts at no 16-byte address (both are copied to the workspace where that is faster). */
 int64_t cti_ebag_linear_int8_workspace_bytes_unaligned(int64_t rows, int32_t cols, int32_t out_features, int32_t gate);
 
+/* ---------------------------------------------------------------------------------------------
+ * Training: the lookup with a scale, the gradients of the tables, dropout, and the layer norm with dropout
+ * and the residual's addition in it. (No counterpart in the reference, whose kernels are forward-only; its model's
+ * nn.Embedding and nn.LayerNorm, online_best/infer.py:948-950, define the gradients.) Results are deterministic: no sum is
+ * taken by atomics.
+ * --------------------------------------------------------------------------------------------- */
+
+/*
+ * out[i] = scale * weight[clamp(ids[i], 0, rows - 1)] in fp32, rounded once to `out_dtype`.
+ *   ids      n of `index_type`
+ *   weight   [rows, row_stride] of `dtype` (F32 / BF16 / F16), the first `dim` columns used
+ *   out      [n, dim] contiguous, overlapping no input
+ */
+int cti_ebag_lookup(const void* ids, int32_t index_type, int64_t n, const void* weight, int32_t dtype, int64_t rows,
+                    int64_t row_stride, int32_t dim, float scale, void* out, int32_t out_dtype, void* stream);
+
+/*
+ * Gradient of cti_ebag_lookup's table: for every row v
+ *   d[v] = scale * sum over i with clamp(ids[i]) = v of grad[i]          (fp32, one rounding to `out_dtype`)
+ * and 0 for row padding_idx (-1: none; nn.Embedding's padding_idx). The ids are sorted and each row's
+ * contributions added in an order that the sizes alone fix.
+ *   grad     [n, dim] of `grad_dtype`, contiguous
+ *   rows_out NULL: out is the whole gradient [rows, dim], rows without an id are 0.
+ *            Else the rows that occur, in ascending order: rows_out [capacity] their numbers, then -1;
+ *            out [capacity, dim] their sums (rows behind the last are left as they were); count_out [1] how many.
+ *            capacity >= min(n, rows)
+ *   workspace  device scratch of at least cti_ebag_backward_workspace_bytes(n, n, rows, dim, CTI_EBAG_SUM)
+ *            bytes, 16-byte aligned (CTI_EBAG_EWORKSPACE otherwise; none needed for n = 0)
+ * n at most 2^30, rows at most 2^31 - 2, dim at most 2^22. No two arrays overlap.
+ */
+int cti_ebag_lookup_backward(const void* grad, int32_t grad_dtype, const void* ids, int32_t index_type, int64_t n, int64_t rows,
+                             int32_t dim, float scale, int64_t padding_idx, void* out, int32_t out_dtype, int64_t* rows_out,
+                             int64_t* count_out, int64_t capacity, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Gradient of the shared table of cti_ebag_fused_all_slots_typed (rows = max_idx + 1), given the gradient of
+ * its output: grad [batch_size, num_slots * emb_dim] of `grad_dtype`, contiguous.
+ *   d[v] = sum over bags (b, s) and their ids with clamp(id) = v of grad[b, s] (MEAN: grad[b, s] / length of the bag)
+ * The bags lie in `values` in the order of slots and samples, as every builder of this library lays them out
+ * (a slot's offsets ascend, and the slots); ids between bags count for none. Offsets are clipped to [0, nnz].
+ * The rest as for cti_ebag_lookup_backward; the workspace's query takes bags = batch_size * num_slots.
+ */
+int cti_ebag_fused_all_slots_backward(const void* grad, int32_t grad_dtype, const void* values, int32_t index_type,
+                                      const void* val_offsets, const void* row_offsets, int32_t offset_type, int64_t batch_size,
+                                      int32_t num_slots, int32_t emb_dim, int64_t max_idx, int64_t nnz, int32_t pooling,
+                                      int64_t padding_idx, void* out, int32_t out_dtype, int64_t* rows_out, int64_t* count_out,
+                                      int64_t capacity, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of the tables of cti_ebag_forward (global offsets, ascending). tables[f] (host) describes the table's
+ * GRADIENT, of `out_dtype`: `data` is written (tables of the same `data` are one table that fields share, and have the
+ * same shape), `out_col` and `dim` are the field's columns in grad [batch_size, grad_row_stride]; row_scale is ignored. At
+ * most 64 fields. padding_idx is every table's.
+ * With rows_out the tables' `data` only tells shared ones apart and nothing is written there: table t's row r
+ * has the number (rows of the tables before t, each counted once) + r, out is [capacity, dim], the tables
+ * have one width. The workspace's query takes rows of all (distinct) tables and the widest dim.
+ */
+int cti_ebag_backward(const void* grad, int32_t grad_dtype, int64_t grad_row_stride, const void* values, int32_t index_type,
+                      int64_t nnz, const int64_t* offsets, int64_t batch_size, int32_t num_fields, const cti_ebag_table* tables,
+                      int32_t pooling, int64_t padding_idx, int32_t out_dtype, void* out, int64_t* rows_out, int64_t* count_out,
+                      int64_t capacity, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace that the gradient of `nnz` ids in `bags` bags needs (0 for no ids and for arguments out of range). */
+int64_t cti_ebag_backward_workspace_bytes(int64_t nnz, int64_t bags, int64_t rows, int32_t dim, int32_t pooling);
+
+/*
+ * Dropout with a mask that is a function of (seed, offset, row, column) and never stored:
+ *   y = residual + (kept ? x * 65536 / (65536 - t) : 0),  t = floor(65536 p + 1/2), in fp32, rounded once.
+ * Philox4x32-10 with counter (row, column / 8, offset low, offset high) and key (seed low, seed high) gives four words; the
+ * 16 bits of column c are the low (c even) or high half of word (c % 8) / 2; the element is dropped where they are below t.
+ * Dropped elements give 0 whatever x is. The gradient is the same call on the output's gradient, without a residual.
+ *   x, residual (or NULL), y   [rows, cols] contiguous, of `dtype`; y may be x or residual
+ *   state    NULL, or two int64 on the device that are added to seed and offset (for captured graphs: what changes between
+ *            replays changes there)
+ * rows at most 2^31 - 1, cols at most 2^28 - 1.
+ */
+int cti_ebag_dropout(const void* x, const void* residual, void* y, int64_t rows, int64_t cols, int32_t dtype, double p,
+                     uint64_t seed, uint64_t offset, const int64_t* state, void* stream);
+
+/*
+ * h = residual + dropout(x) as cti_ebag_dropout makes it, rounded to `dtype`; y = LayerNorm(h) of what is stored:
+ * mean, rstd = 1/sqrt(var + eps) (fp32 [rows]), y = (h - mean) * rstd * gamma + beta, rounded once.
+ *   h        [rows, cols], or NULL where there is neither dropout (t = 0) nor a residual (h is x)
+ * No output overlaps another array.
+ */
+int cti_ebag_dropout_layernorm(const void* x, const void* residual, void* h, void* y, int64_t rows, int64_t cols, int32_t dtype,
+                               const void* gamma, const void* beta, int32_t param_dtype, float eps, double p, uint64_t seed,
+                               uint64_t offset, const int64_t* state, float* mean, float* rstd, void* stream);
+
+/*
+ * Its gradients, with z = (h - mean) * rstd and a = grad * gamma:
+ *   dresidual = rstd * (a - mean(a) - z * mean(a * z)) + grad_h      dx = dropout(dresidual)
+ *   dgamma = sum over rows of grad * z      dbeta = sum over rows of grad
+ * in fp32, dx from the unrounded sum, each rounded once (dgamma and dbeta to `param_dtype`).
+ *   grad, h  [rows, cols] of `dtype`; grad_h: the gradient that arrives at h itself, or NULL
+ *   dresidual  NULL: not written (without dropout it is dx)
+ *   workspace  at least cti_ebag_dropout_layernorm_backward_workspace_bytes(rows, cols), 16-byte aligned
+ * No output overlaps another array. rows = 0 gives dgamma = dbeta = 0.
+ */
+int cti_ebag_dropout_layernorm_backward(const void* grad, const void* h, const void* grad_h, const float* mean, const float* rstd,
+                                        int64_t rows, int64_t cols, int32_t dtype, const void* gamma, int32_t param_dtype, double p,
+                                        uint64_t seed, uint64_t offset, const int64_t* state, void* dx, void* dresidual,
+                                        void* dgamma, void* dbeta, void* workspace, int64_t workspace_bytes, void* stream);
+int64_t cti_ebag_dropout_layernorm_backward_workspace_bytes(int64_t rows, int64_t cols);
+
 #ifdef __cplusplus
 }
 #endif
