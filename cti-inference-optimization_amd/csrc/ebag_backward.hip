@@ -496,7 +496,8 @@ struct SumParams {
   int64_t grad_stride;    // elements between units' groups of `fields` (per-field), else dim
   uint32_t total;
   int32_t dim;            // the widest field's
-  int32_t log_lanes;      // lanes that cover a block of columns
+  int32_t log_lanes;      // lanes that cover a block of columns, each with `lane_cols`
+  int32_t lane_cols;
   int32_t run;            // ids a lane group
   int32_t workgroups;
   float scale;
@@ -561,13 +562,12 @@ __global__ void __launch_bounds__(kScanThreads) grad_heads_scan_kernel(uint32_t*
   }
 }
 
-// Columns of lane `lane` of block `block`: VEC from the first on; the last vector ends with the row and
+// The first of the `cols` columns of lane `lane` of block `block`; the last vector ends with the row and
 // overlaps the one before it (both come to the same sums). A row narrower than a vector is lane 0's.
-template <int VEC>
-__device__ __forceinline__ int first_column(int block, int lane, int dim) {
-  const int c = (block * kWave + lane) * VEC;
+__device__ __forceinline__ int first_column(int block, int lane, int dim, int cols) {
+  const int c = (block * kWave + lane) * cols;
   if (c >= dim) return -1;
-  return c + VEC <= dim ? c : (dim >= VEC ? dim - VEC : 0);
+  return c + cols <= dim ? c : (dim >= cols ? dim - cols : 0);
 }
 
 template <typename T, typename OT, typename FIELDS>
@@ -602,6 +602,40 @@ struct Sums {
   }
 };
 
+// Distinct keys that begin in the runs before this workgroup's, and all of them. s_sum: 2 * wavefronts words.
+__device__ __forceinline__ uint32_t keys_begun(const SumParams& p, uint32_t* total, uint32_t (*s_sum)[kSumThreads / kWave]) {
+  if (p.heads_scanned) {
+    *total = p.heads[p.workgroups];
+    return p.heads[blockIdx.x];
+  }
+  const int t = static_cast<int>(threadIdx.x);
+  uint32_t all = 0, begun = 0;
+#pragma unroll 8
+  for (int i = t; i < p.workgroups; i += kSumThreads) {
+    const uint32_t c = p.heads[i];
+    all += c;
+    begun += i < static_cast<int>(blockIdx.x) ? c : 0u;
+  }
+#pragma unroll
+  for (int m = 1; m < kWave; m <<= 1) {
+    all += static_cast<uint32_t>(shfl_i32(static_cast<int>(all), lane_id() ^ m));
+    begun += static_cast<uint32_t>(shfl_i32(static_cast<int>(begun), lane_id() ^ m));
+  }
+  if (lane_id() == 0) {
+    s_sum[0][t / kWave] = all;
+    s_sum[1][t / kWave] = begun;
+  }
+  __syncthreads();
+  all = begun = 0;
+#pragma unroll
+  for (int w = 0; w < kSumThreads / kWave; ++w) {
+    all += s_sum[0][w];
+    begun += s_sum[1][w];
+  }
+  *total = all;
+  return begun;
+}
+
 // A workgroup's run of the sorted ids: `run` for each of its kSumThreads >> log_lanes lane groups.
 // blockIdx.x: the run; blockIdx.y: the block of 64 vectors of columns.
 template <typename T, typename OT, typename FIELDS>
@@ -625,33 +659,8 @@ __global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p
   }
   uint32_t begun = 0;  // distinct keys before this run
   if (p.rows_out) {
-    uint32_t all = 0;
-    if (p.heads_scanned) {
-      begun = p.heads[blockIdx.x];
-      all = p.heads[p.workgroups];
-    } else {
-      for (int i = t; i < p.workgroups; i += kSumThreads) {
-        const uint32_t c = p.heads[i];
-        all += c;
-        begun += i < static_cast<int>(blockIdx.x) ? c : 0u;
-      }
-#pragma unroll
-      for (int m = 1; m < kWave; m <<= 1) {
-        all += static_cast<uint32_t>(shfl_i32(static_cast<int>(all), lane_id() ^ m));
-        begun += static_cast<uint32_t>(shfl_i32(static_cast<int>(begun), lane_id() ^ m));
-      }
-      if (lane_id() == 0) {
-        s_sum[0][t / kWave] = all;
-        s_sum[1][t / kWave] = begun;
-      }
-      __syncthreads();
-      all = begun = 0;
-#pragma unroll
-      for (int w = 0; w < kSumThreads / kWave; ++w) {
-        all += s_sum[0][w];
-        begun += s_sum[1][w];
-      }
-    }
+    uint32_t all;
+    begun = keys_begun(p, &all, s_sum);
     if (blockIdx.x == 0 && block == 0 && t == 0) *p.count_out = all;
   }
   __syncthreads();
@@ -701,7 +710,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p
         for (int e = 0; e < VEC; ++e) s_part[0][t * VEC + e] = acc[e];
       } else if (cur < p.total) {
         const uint32_t unit = s_unit[i];
-        const int dim = S::width(p, fs, unit), c0 = first_column<VEC>(block, lane, dim);
+        const int dim = S::width(p, fs, unit), c0 = first_column(block, lane, dim, VEC);
         if (c0 >= 0) {
           char* const row = S::target(p, fs, cur, unit, p.rows_out ? s_rank[i] : 0u);
           float v[VEC];
@@ -724,7 +733,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p
           const uint32_t unit = s_unit[i];
           int dim;
           const char* const row = S::row(p, fs, unit, &dim);
-          const int c0 = first_column<VEC>(block, lane, dim);
+          const int c0 = first_column(block, lane, dim, VEC);
           if (c0 >= 0) raw[u] = load_raw<T, VEC>(row + static_cast<int64_t>(c0) * Elem<T>::kBytes, dim - c0);
           if (p.inv_len) w[u] = p.inv_len[unit];
         }
@@ -782,7 +791,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p
           } else if (s_key[w * p.run + 1] < p.total) {
             const int i = w * p.run;
             const uint32_t unit = s_unit[i];
-            const int dim = S::width(p, fs, unit), c0 = first_column<VEC>(block, l, dim);
+            const int dim = S::width(p, fs, unit), c0 = first_column(block, l, dim, VEC);
             if (c0 >= 0 && c0 + e < dim)
               store_one(reinterpret_cast<OT*>(S::target(p, fs, s_key[i + 1], unit, p.rows_out ? s_rank[i] : 0u)) + c0 + e,
                         carry * p.scale, false);
@@ -800,12 +809,236 @@ __global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p
   }
 }
 
+// The same for rows of at least kWalkCols columns that lie one behind the other in grad: a whole wavefront
+// walks its ids, so that keys, rows' addresses and the ends of keys are scalars: an id costs a load and its
+// additions. (Lane groups of 16 lanes for 128 bf16 columns: 917,504 ids 64 us, the end of a key in one of
+// four groups stopping the others; so: see below.) COLS columns a lane; a wavefront takes `run` ids, 128 at most.
+constexpr int kWalkWaves = kSumThreads / kWave;
+constexpr int kWalkBatches = 2;
+
+template <typename T, int COLS>
+struct LaneCols {  // COLS columns as loaded
+  static constexpr int kBytes = COLS * Elem<T>::kBytes;
+  static constexpr int kWords = (kBytes + 3) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (kBytes == 2) w[0] = *reinterpret_cast<const uint16_t*>(p);
+    else if constexpr (kBytes == 4) w[0] = *reinterpret_cast<const u32_any*>(p);
+    else if constexpr (kBytes == 8) { const u32x2 v = *reinterpret_cast<const u32x2_any*>(p); w[0] = v.x, w[1] = v.y; }
+    else { const uint4 v = load16_any(p); w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w; }
+  }
+  __device__ __forceinline__ float value(int e) const {
+    if constexpr (Elem<T>::kBytes == 4) return __uint_as_float(w[e]);
+    else if constexpr (std::is_same<T, bf16_t>::value) return __uint_as_float(e % 2 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    else return f16_bits_to_f32(e % 2 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu);
+  }
+};
+
+template <typename OT, int COLS>
+__device__ __forceinline__ void store_cols(char* p, const float* v) {
+  if constexpr (COLS >= 4) {
+    store_vec<OT, COLS>(p, COLS, v);
+  } else if constexpr (Elem<OT>::kBytes == 4) {
+    if constexpr (COLS == 2) *reinterpret_cast<u32x2_any*>(p) = u32x2{__float_as_uint(v[0]), __float_as_uint(v[1])};
+    else *reinterpret_cast<float*>(p) = v[0];
+  } else if constexpr (COLS == 2) {
+    *reinterpret_cast<u32_any*>(p) = Packed<OT>::pair(v[0], v[1]);
+  } else {
+    store_one(reinterpret_cast<OT*>(p), v[0], false);
+  }
+}
+
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+
+template <typename T, typename OT, typename FIELDS, int COLS, bool MEAN>
+__global__ void __launch_bounds__(kSumThreads) grad_walk_kernel(const SumParams p, const FIELDS fs) {
+  using S = Sums<T, OT, FIELDS>;
+  constexpr int AHEAD = COLS * Elem<T>::kBytes >= 16 ? 8 : 16;  // rows whose loads are in flight
+  __shared__ float s_part[2][kWalkWaves][kWave * COLS];
+  __shared__ uint32_t s_flag[2][kWalkWaves], s_key[kWalkWaves], s_unit[kWalkWaves], s_rank[kWalkWaves], s_heads[kWalkWaves];
+  __shared__ uint32_t s_sum[2][kSumThreads / kWave];
+  const int t = static_cast<int>(threadIdx.x), lane = lane_id();
+  const int w = __builtin_amdgcn_readfirstlane(t / kWave);
+  const int block = static_cast<int>(blockIdx.y);
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kWalkWaves + w) * p.run;  // the wavefront's
+  const int64_t rest = p.n - first;
+  const int have = rest <= 0 ? 0 : rest < p.run ? static_cast<int>(rest) : p.run;
+  uint32_t key[kWalkBatches], unit[kWalkBatches];
+  float weight[kWalkBatches];
+  uint64_t begins[kWalkBatches];  // whose key is another than the id's before
+  int live = 0;                   // ids that are not dropped: those come last
+  uint32_t heads = 0;
+  const uint32_t before = have && first > 0 ? p.key[first - 1] : 0xffffffffu;  // no key is that large
+  const uint32_t behind = have && first + have < p.n ? p.key[first + have] : 0xffffffffu;
+#pragma unroll
+  for (int b = 0; b < kWalkBatches; ++b) {
+    const int i = b * kWave + lane;
+    const bool in = i < have;
+    key[b] = in ? p.key[first + i] : 0xffffffffu;
+    unit[b] = in ? p.unit[first + i] : 0u;
+  }
+#pragma unroll
+  for (int b = 0; b < kWalkBatches; ++b) {
+    uint32_t prev = static_cast<uint32_t>(shfl_i32(static_cast<int>(key[b]), lane - 1));
+    const uint32_t last = b == 0 ? before : lane_value(key[b > 0 ? b - 1 : 0], kWave - 1);
+    if (lane == 0) prev = last;
+    const bool kept = key[b] < p.total;
+    begins[b] = __ballot(kept && key[b] != prev);
+    live += __popcll(__ballot(kept));
+    heads += static_cast<uint32_t>(__popcll(begins[b]));
+    weight[b] = MEAN && kept ? p.inv_len[unit[b]] : 1.f;
+  }
+  const uint32_t first_key = lane_value(key[0], 0);
+  bool open = live > 0 && before == first_key;  // the first key began before
+  uint32_t rank = 0;                            // of the current key
+  if (p.rows_out) {
+    uint32_t all;
+    if (lane == 0) s_heads[w] = heads;
+    rank = keys_begun(p, &all, s_sum);
+    if (p.heads_scanned) __syncthreads();
+    if (blockIdx.x == 0 && block == 0 && t == 0) *p.count_out = all;
+    for (int i = 0; i < w; ++i) rank += s_heads[i];
+    rank = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(rank)));
+    if (block == 0) {
+      uint32_t r = rank;
+#pragma unroll
+      for (int b = 0; b < kWalkBatches; ++b) {
+        if ((begins[b] >> lane) & 1) p.rows_out[r + static_cast<uint32_t>(__popcll(begins[b] & ((uint64_t{1} << lane) - 1)))] = key[b];
+        r += static_cast<uint32_t>(__popcll(begins[b]));
+      }
+      if (have && lane == 0 && (w == kWalkWaves - 1 || rest <= p.run)) p.last_rank[blockIdx.x] = r - 1u;
+    }
+    rank -= 1u;
+  }
+  uint32_t flag0 = 0, flag1 = 0;
+  const int c0 = first_column(block, lane, p.dim, COLS);
+  const uint32_t first_unit = lane_value(unit[0], 0), first_rank = rank;
+  float acc[COLS];
+#pragma unroll
+  for (int e = 0; e < COLS; ++e) acc[e] = 0.f;
+  const int64_t row_bytes = static_cast<int64_t>(p.dim) * Elem<T>::kBytes;
+  const uint32_t lane_at = static_cast<uint32_t>(c0 < 0 ? 0 : c0) * Elem<T>::kBytes;  // lanes without columns read the first
+  uint32_t cur_key = first_key, cur_unit = first_unit;
+  const auto finish = [&]() {
+    if (open) {
+      flag0 = 1;
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) s_part[0][w][lane * COLS + e] = acc[e];
+      open = false;
+    } else {
+      char* const row = S::target(p, fs, cur_key, cur_unit, rank);
+      float v[COLS];
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) v[e] = acc[e] * p.scale;
+      if (c0 >= 0) store_cols<OT, COLS>(row + static_cast<uint32_t>(c0) * Elem<OT>::kBytes, v);
+    }
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) acc[e] = 0.f;
+  };
+  bool any = false;
+#pragma unroll
+  for (int b = 0; b < kWalkBatches; ++b) {
+    const int now = live - b * kWave < kWave ? live - b * kWave : kWave;
+    if (now <= 0) break;
+    LaneCols<T, COLS> rows[2][AHEAD];
+    const auto fetch = [&](int i0, LaneCols<T, COLS>* to) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int i = i0 + u < now ? i0 + u : now - 1;
+        to[u].load(p.grad + static_cast<int64_t>(lane_value(unit[b], i)) * row_bytes + lane_at);
+      }
+    };
+    const auto add = [&](int i0, const LaneCols<T, COLS>* from) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int i = i0 + u;
+        if (i < now) {
+          if ((begins[b] >> i) & 1) {
+            if (any) finish();
+            cur_key = lane_value(key[b], i);
+            cur_unit = lane_value(unit[b], i);
+            rank += 1u;
+          }
+          any = true;
+          if constexpr (MEAN) {
+            const float f = __uint_as_float(lane_value(__float_as_uint(weight[b]), i));
+#pragma unroll
+            for (int e = 0; e < COLS; ++e) acc[e] = __builtin_fmaf(from[u].value(e), f, acc[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < COLS; ++e) acc[e] += from[u].value(e);
+          }
+        }
+      }
+    };
+    fetch(0, rows[0]);
+    for (int i0 = 0; i0 < now; i0 += 2 * AHEAD) {
+      if (i0 + AHEAD < now) fetch(i0 + AHEAD, rows[1]);
+      add(i0, rows[0]);
+      if (i0 + 2 * AHEAD < now) fetch(i0 + 2 * AHEAD, rows[0]);
+      add(i0 + AHEAD, rows[1]);
+    }
+  }
+  if (any) {
+    if (live == have && behind == cur_key) {  // goes on behind the wavefront's ids
+      const int which = open ? 0 : 1;
+      if (open) flag0 = 2;
+      else flag1 = 1;
+#pragma unroll
+      for (int e = 0; e < COLS; ++e) s_part[which][w][lane * COLS + e] = acc[e];
+    } else {
+      finish();
+    }
+  }
+  if (lane == 0) {
+    s_flag[0][w] = flag0;
+    s_flag[1][w] = flag1;
+    s_key[w] = first_key;
+    s_unit[w] = first_unit;
+    s_rank[w] = first_rank;
+  }
+  __syncthreads();
+
+  // Keys that cross wavefronts, in their order; a thread adds up its columns' parts.
+  constexpr int SLOTS = kWave * COLS;
+  float* const mine = p.partial + (static_cast<int64_t>(block) * p.workgroups + blockIdx.x) * 2 * SLOTS;
+  bool head = s_flag[0][0] != 0;  // the first key began before the workgroup's ids
+  for (int slot = t; slot < SLOTS; slot += kSumThreads) {
+    bool began = head, carrying = head;
+    float carry = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWalkWaves; ++i) {
+      const uint32_t f0 = s_flag[0][i];
+      if (f0) {
+        carry += s_part[0][i][slot];
+        if (f0 == 1) {
+          if (began) {
+            mine[slot] = carry;
+          } else {
+            const int at = first_column(block, slot / COLS, p.dim, COLS);
+            if (at >= 0)
+              store_one(reinterpret_cast<OT*>(S::target(p, fs, s_key[i], s_unit[i], s_rank[i])) + at + slot % COLS, carry * p.scale, false);
+          }
+          began = carrying = false;
+          carry = 0.f;
+        }
+      }
+      if (s_flag[1][i]) {
+        carry = s_part[1][i][slot];
+        carrying = true;
+      }
+    }
+    if (carrying) mine[began ? slot : SLOTS + slot] = carry;
+  }
+}
+
 // Keys that cross workgroups: the workgroup in whose run one begins and goes on adds up its own part and, in order of the
 // runs, those of the runs it crosses.
 template <typename T, typename OT, typename FIELDS>
 __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams p, const FIELDS fs) {
   using S = Sums<T, OT, FIELDS>;
-  constexpr int VEC = S::VEC;
   __shared__ float4 s_part[kSumThreads];
   const int t = static_cast<int>(threadIdx.x), lanes = 1 << p.log_lanes, groups = kSumThreads >> p.log_lanes;
   const int64_t ids = static_cast<int64_t>(groups) * p.run, first = static_cast<int64_t>(blockIdx.x) * ids;
@@ -823,7 +1056,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams 
     follow += c;
     if (c < kSumThreads) break;
   }
-  const int slots = lanes * VEC, quads = slots / 4, rows = kSumThreads / quads;  // rows of parts side by side
+  const int slots = lanes * p.lane_cols, quads = slots / 4, rows = kSumThreads / quads;  // rows of parts side by side
   const int64_t row_floats = 2 * static_cast<int64_t>(slots);
   const float* const mine = p.partial + (static_cast<int64_t>(block) * p.workgroups + blockIdx.x) * row_floats;
   const int q = t % quads, r = t / quads;
@@ -848,8 +1081,8 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams 
   OT* const row = reinterpret_cast<OT*>(S::target(p, fs, key, unit, rank));
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    const int slot = q * 4 + k, c0 = first_column<VEC>(block, slot / VEC, dim);
-    if (c0 >= 0 && c0 + slot % VEC < dim) store_one(row + c0 + slot % VEC, v[k] * p.scale, false);
+    const int slot = q * 4 + k, c0 = first_column(block, slot / p.lane_cols, dim, p.lane_cols);
+    if (c0 >= 0 && c0 + slot % p.lane_cols < dim) store_one(row + c0 + slot % p.lane_cols, v[k] * p.scale, false);
   }
 }
 
@@ -897,22 +1130,35 @@ struct GradCall {
   SumParams sum{};
   SumFields fields{};
   bool per_field = false;
+  bool even = true;   // the units' rows lie one behind the other in grad, all of sum.dim columns
+  bool walk = false;  // the plan's
   int32_t grad_dtype = 0, out_dtype = 0;
   int64_t capacity = 0;
   void* workspace = nullptr;
   int64_t workspace_bytes = 0;
 };
 
+template <typename T, typename OT, typename FIELDS, int COLS>
+void launch_walk(const SumParams& p, const FIELDS& fs, dim3 grid, hipStream_t s) {
+  if constexpr (COLS * Elem<T>::kBytes <= 16) {
+    if (p.inv_len) hipLaunchKernelGGL((grad_walk_kernel<T, OT, FIELDS, COLS, true>), grid, dim3(kSumThreads), 0, s, p, fs);
+    else hipLaunchKernelGGL((grad_walk_kernel<T, OT, FIELDS, COLS, false>), grid, dim3(kSumThreads), 0, s, p, fs);
+  }
+}
 template <typename T, typename OT, typename FIELDS>
-void launch_sums(const SumParams& p, const FIELDS& fs, int blocks, hipStream_t s) {
+void launch_sums(const SumParams& p, const FIELDS& fs, int blocks, bool walk, hipStream_t s) {
   const dim3 grid(static_cast<unsigned>(p.workgroups), static_cast<unsigned>(blocks));
-  hipLaunchKernelGGL((grad_sum_kernel<T, OT, FIELDS>), grid, dim3(kSumThreads), 0, s, p, fs);
+  if (!walk) hipLaunchKernelGGL((grad_sum_kernel<T, OT, FIELDS>), grid, dim3(kSumThreads), 0, s, p, fs);
+  else if (p.lane_cols == 1) launch_walk<T, OT, FIELDS, 1>(p, fs, grid, s);
+  else if (p.lane_cols == 2) launch_walk<T, OT, FIELDS, 2>(p, fs, grid, s);
+  else if (p.lane_cols == 4) launch_walk<T, OT, FIELDS, 4>(p, fs, grid, s);
+  else launch_walk<T, OT, FIELDS, 8>(p, fs, grid, s);
   if (p.workgroups > 1) hipLaunchKernelGGL((grad_join_kernel<T, OT, FIELDS>), grid, dim3(kSumThreads), 0, s, p, fs);
 }
 template <typename T, typename OT>
 void launch_sums_for(const GradCall& c, int blocks, hipStream_t s) {
-  if (c.per_field) launch_sums<T, OT, SumFields>(c.sum, c.fields, blocks, s);
-  else launch_sums<T, OT, NoFields>(c.sum, NoFields{}, blocks, s);
+  if (c.per_field) launch_sums<T, OT, SumFields>(c.sum, c.fields, blocks, c.walk, s);
+  else launch_sums<T, OT, NoFields>(c.sum, NoFields{}, blocks, c.walk, s);
 }
 template <typename T>
 void launch_sums_typed(const GradCall& c, int blocks, hipStream_t s) {
@@ -951,7 +1197,7 @@ int run_gradient(GradCall& c, hipStream_t s) {
   if (n == 0) return check_launch("gradient");
 
   c.src.by_batch = ChunkDivide::by(static_cast<uint32_t>(c.src.batch));
-  const GradPlan plan = grad_plan(n, c.src.inv_len ? c.src.bags : 0, c.sum.dim, dtype_bytes(c.grad_dtype), c.src.total);
+  const GradPlan plan = grad_plan(n, c.src.inv_len ? c.src.bags : 0, c.sum.dim, dtype_bytes(c.grad_dtype), c.src.total, c.even);
   char* const ws = static_cast<char*>(c.workspace);
   SortBuffers buf[2] = {{reinterpret_cast<uint32_t*>(ws + plan.key[0]), reinterpret_cast<uint32_t*>(ws + plan.unit[0])},
                         {reinterpret_cast<uint32_t*>(ws + plan.key[1]), reinterpret_cast<uint32_t*>(ws + plan.unit[1])}};
@@ -987,7 +1233,9 @@ int run_gradient(GradCall& c, hipStream_t s) {
   p.n = n;
   p.total = c.src.total;
   p.partial = reinterpret_cast<float*>(ws + plan.partial);
+  c.walk = plan.walk;
   p.log_lanes = plan.log_lanes;
+  p.lane_cols = plan.lane_cols;
   p.run = plan.run;
   p.workgroups = static_cast<int32_t>(plan.workgroups);
   p.fields = c.src.fields;
@@ -1032,11 +1280,10 @@ int check_gradient(int32_t grad_dtype, int32_t out_dtype, int32_t index_type, in
 
 int check_workspace(const GradCall& c, int64_t bags, int64_t dim) {
   if (c.src.n == 0) return CTI_EBAG_OK;
-  const int64_t need = grad_plan(c.src.n, bags, dim, 2, c.src.total).bytes, need4 = grad_plan(c.src.n, bags, dim, 4, c.src.total).bytes;
-  const int64_t most = need > need4 ? need : need4;
-  if (!c.workspace || c.workspace_bytes < most)
+  const int64_t need = grad_workspace_bytes(c.src.n, bags, dim, c.src.total);
+  if (!c.workspace || c.workspace_bytes < need)
     return set_error(CTI_EBAG_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)(c.workspace ? c.workspace_bytes : 0),
-                     (long long)most);
+                     (long long)need);
   if (reinterpret_cast<uintptr_t>(c.workspace) % 16) return set_error(CTI_EBAG_EINVAL, "workspace is not 16-byte aligned");
   return CTI_EBAG_OK;
 }
@@ -1086,9 +1333,7 @@ extern "C" int cti_ebag_lookup(const void* ids, int32_t index_type, int64_t n, c
 extern "C" int64_t cti_ebag_backward_workspace_bytes(int64_t nnz, int64_t bags, int64_t rows, int32_t dim, int32_t pooling) {
   if (nnz <= 0 || bags < 0 || rows < 1 || dim < 1 || nnz > kGradMostIds || bags > kGradMostIds || rows >= kGradMostRows) return 0;
   const int64_t b = pooling == CTI_EBAG_MEAN ? bags : 0;
-  const int64_t two = grad_plan(nnz, b, dim, 2, static_cast<uint32_t>(rows)).bytes;
-  const int64_t four = grad_plan(nnz, b, dim, 4, static_cast<uint32_t>(rows)).bytes;
-  return two > four ? two : four;
+  return grad_workspace_bytes(nnz, b, dim, static_cast<uint32_t>(rows));
 }
 
 extern "C" int cti_ebag_lookup_backward(const void* grad, int32_t grad_dtype, const void* ids, int32_t index_type, int64_t n,
@@ -1225,7 +1470,9 @@ extern "C" int cti_ebag_backward(const void* grad, int32_t grad_dtype, int64_t g
     c.fields.dim[f] = t.dim;
     c.fields.col[f] = t.out_col;
     if (t.dim > dim) dim = t.dim;
+    c.even = c.even && t.dim == tables[0].dim && t.out_col == static_cast<int64_t>(f) * t.dim;
   }
+  c.even = c.even && grad_row_stride == num_fields * dim;
   const int64_t bags = batch_size * num_fields;
   int rc = check_gradient(grad_dtype, out_dtype, index_type, nnz, bags, dim, compact, count_out, rows, capacity);
   if (rc != CTI_EBAG_OK) return rc;

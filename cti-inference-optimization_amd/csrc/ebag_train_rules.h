@@ -31,29 +31,46 @@ constexpr int64_t kGradMostDim = int64_t{1} << 22;
 constexpr int64_t kGradTilesUnscanned = 256;
 constexpr int64_t kGradHeadsUnscanned = 4096;
 
+constexpr int kGradWalkCols = 64;  // narrower rows would leave most of a wavefront idle
+
 struct GradPlan {
   int64_t tiles;
   int bits, digit_bits;
-  int log_lanes, run, blocks;  // lanes of a group, ids of a group, blocks of 64 vectors of columns
+  bool walk;      // a wavefront for each run of ids, else lane groups
+  int lane_cols;  // columns a lane
+  int log_lanes, run, blocks;  // lanes of a group, ids of a group, blocks of 64 lanes' columns
   int64_t workgroups;
   int64_t key[2], unit[2], counts, totals, heads, last_rank, inv_len, partial, bytes;  // places in the workspace
 };
 
-// The gradient of n ids in tables of `rows` rows, the widest of `dim` columns; mean_bags: bags under mean pooling, else 0.
-inline GradPlan grad_plan(int64_t n, int64_t mean_bags, int64_t dim, int elem_bytes, uint32_t rows) {
+// The gradient of n ids in tables of `rows` rows, the widest of `dim` columns; mean_bags: bags under mean pooling, else 0;
+// even: all rows of grad have `dim` columns and lie one behind the other.
+inline GradPlan grad_plan(int64_t n, int64_t mean_bags, int64_t dim, int elem_bytes, uint32_t rows, bool even) {
   GradPlan p{};
   p.tiles = ceil_div(n, kGradTile);
   while (p.bits < 32 && (rows >> p.bits)) ++p.bits;  // of the key `rows` itself
   const int passes = (p.bits + 7) / 8;
   p.digit_bits = (p.bits + passes - 1) / passes;
   const int vec = 16 / elem_bytes;
-  const int64_t vectors = ceil_div(dim, vec);
-  while (p.log_lanes < 6 && (int64_t{1} << p.log_lanes) < vectors) ++p.log_lanes;
-  p.blocks = static_cast<int>(ceil_div(vectors, 64));
-  const int groups = 256 >> p.log_lanes;
-  p.run = 2048 / groups < 32 ? 2048 / groups : 32;
-  if (ceil_div(n, int64_t{groups} * p.run) * p.blocks < 1024) p.run = 8;
-  p.workgroups = ceil_div(n, int64_t{groups} * p.run);
+  p.walk = even && dim >= kGradWalkCols;
+  if (p.walk) {
+    p.log_lanes = 6;
+    p.lane_cols = 1;
+    while (p.lane_cols < vec && 64 * p.lane_cols < dim) p.lane_cols *= 2;
+    p.blocks = static_cast<int>(ceil_div(dim, 64 * p.lane_cols));
+    // enough wavefronts to fill the card, ids enough for each to keep its loads in flight
+    p.run = 128;
+    while (p.run > 16 && ceil_div(n, p.run) * p.blocks < 4096) p.run /= 2;
+  } else {
+    p.lane_cols = vec;
+    const int64_t vectors = ceil_div(dim, vec);
+    while (p.log_lanes < 6 && (int64_t{1} << p.log_lanes) < vectors) ++p.log_lanes;
+    p.blocks = static_cast<int>(ceil_div(vectors, 64));
+    const int groups = 256 >> p.log_lanes;
+    p.run = 2048 / groups < 32 ? 2048 / groups : 32;
+    if (ceil_div(n, int64_t{groups} * p.run) * p.blocks < 1024) p.run = 8;
+  }
+  p.workgroups = ceil_div(n, int64_t{256 >> p.log_lanes} * p.run);
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -69,9 +86,20 @@ inline GradPlan grad_plan(int64_t n, int64_t mean_bags, int64_t dim, int elem_by
   p.heads = take((p.workgroups + 1) * 4);
   p.last_rank = take(p.workgroups * 4);
   p.inv_len = take(mean_bags * 4);
-  p.partial = take(p.workgroups * p.blocks * 2 * (int64_t{vec} << p.log_lanes) * 4);
+  p.partial = take(p.workgroups * p.blocks * 2 * (int64_t{p.lane_cols} << p.log_lanes) * 4);
   p.bytes = at;
   return p;
+}
+
+// Bytes that every form of a gradient of these sizes fits in.
+inline int64_t grad_workspace_bytes(int64_t n, int64_t mean_bags, int64_t dim, uint32_t rows) {
+  int64_t most = 0;
+  for (const int elem_bytes : {2, 4})
+    for (const bool even : {false, true}) {
+      const int64_t bytes = grad_plan(n, mean_bags, dim, elem_bytes, rows, even).bytes;
+      most = bytes > most ? bytes : most;
+    }
+  return most;
 }
 
 // The register form of the norm with dropout: `lanes` threads hold a row, `chunks` chunks of 8 columns each (1, 2 or 4);

@@ -40,8 +40,8 @@ def test_mask_keeps_the_stated_share(p):
 
 
 class Plan(ctypes.Structure):
-    _fields_ = [("tiles", ctypes.c_int64), ("bits", ctypes.c_int), ("digit_bits", ctypes.c_int), ("log_lanes", ctypes.c_int),
-                ("run", ctypes.c_int), ("blocks", ctypes.c_int), ("workgroups", ctypes.c_int64), ("key", ctypes.c_int64 * 2),
+    _fields_ = [("tiles", ctypes.c_int64), ("bits", ctypes.c_int), ("digit_bits", ctypes.c_int), ("walk", ctypes.c_bool),
+                ("lane_cols", ctypes.c_int), ("log_lanes", ctypes.c_int), ("run", ctypes.c_int), ("blocks", ctypes.c_int), ("workgroups", ctypes.c_int64), ("key", ctypes.c_int64 * 2),
                 ("unit", ctypes.c_int64 * 2), ("counts", ctypes.c_int64), ("totals", ctypes.c_int64), ("heads", ctypes.c_int64),
                 ("last_rank", ctypes.c_int64), ("inv_len", ctypes.c_int64), ("partial", ctypes.c_int64), ("bytes", ctypes.c_int64)]
 
@@ -53,8 +53,8 @@ def rules(tmp_path_factory):
         '#include "ebag_train_rules.h"\n'
         "using namespace cti;\n"
         'extern "C" uint32_t divide(uint32_t n, uint32_t d) { return ChunkDivide::by(d).quotient(n); }\n'
-        'extern "C" void plan(int64_t n, int64_t bags, int64_t dim, int elem, uint32_t rows, GradPlan* p) {\n'
-        "  *p = grad_plan(n, bags, dim, elem, rows);\n}\n"
+        'extern "C" void plan(int64_t n, int64_t bags, int64_t dim, int elem, uint32_t rows, int even, GradPlan* p) {\n'
+        "  *p = grad_plan(n, bags, dim, elem, rows, even);\n}\n"
         'extern "C" int form(int64_t cols, int* chunks) {\n'
         "  const TrainNormForm f = train_norm_form(cols);\n  *chunks = f.chunks;\n  return f.lanes;\n}\n"
         'extern "C" int64_t norm_groups(int64_t rows, int64_t cols) { return train_norm_workgroups(rows, cols); }\n'
@@ -63,7 +63,8 @@ def rules(tmp_path_factory):
                     str(work / "rules.so")], check=True)
     lib = ctypes.CDLL(str(work / "rules.so"))
     lib.divide.argtypes, lib.divide.restype = [ctypes.c_uint32] * 2, ctypes.c_uint32
-    lib.plan.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_uint32, ctypes.POINTER(Plan)]
+    lib.plan.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_uint32, ctypes.c_int,
+                         ctypes.POINTER(Plan)]
     lib.form.argtypes = [ctypes.c_int64, ctypes.POINTER(ctypes.c_int)]
     for f in (lib.norm_groups, lib.norm_bytes):
         f.argtypes, f.restype = [ctypes.c_int64] * 2, ctypes.c_int64
@@ -87,21 +88,26 @@ def test_gradient_plan_holds_what_the_kernels_assume(rules):
         n, dim = int(2 ** rng.uniform(0, 30)), int(2 ** rng.uniform(0, 22))
         rows, elem = int(2 ** rng.uniform(0, 30.99)), rng.choice([2, 4])
         bags = rng.choice([0, int(2 ** rng.uniform(0, 30))])
-        rules.plan(n, bags, dim, elem, rows, ctypes.byref(p))
-        vec = 16 // elem
+        even = rng.random() < 0.5
+        rules.plan(n, bags, dim, elem, rows, even, ctypes.byref(p))
         assert p.tiles == -(-n // 4096)
         # every key, the dropped ids' key `rows` too, has its bits; digits are at most 8 bits
         assert rows < 2 ** p.bits and p.digit_bits <= 8 and -(-p.bits // p.digit_bits) == -(-p.bits // 8)
         # lane groups cover a block of columns; blocks cover the row, and fit the grid
-        assert p.log_lanes <= 6 and (1 << p.log_lanes) * vec * p.blocks >= dim and p.blocks <= 65535
+        assert p.log_lanes <= 6 and (1 << p.log_lanes) * p.lane_cols * p.blocks >= dim and p.blocks <= 65535
         assert p.blocks == 1 or p.log_lanes == 6
+        assert p.lane_cols in (1, 2, 4, 8) and p.lane_cols * elem <= 16 and (p.blocks - 1) * 64 * p.lane_cols < dim
+        if p.walk:
+            assert even and dim >= 64 and p.log_lanes == 6 and p.run <= 128 and p.lane_cols <= dim
+        else:
+            assert p.lane_cols * elem == 16
         groups = 256 >> p.log_lanes
         assert groups * p.run <= 2048 and p.workgroups == -(-n // (groups * p.run))
         assert p.workgroups * 256 < 2 ** 32 and p.workgroups < 2 ** 31
         # parts of the workspace, in their order, neither overlap nor end before what is written there
         ends = [(p.key[0], n * 4), (p.unit[0], n * 4), (p.key[1], n * 4), (p.unit[1], n * 4), (p.counts, p.tiles * 1024),
                 (p.totals, 1024), (p.heads, (p.workgroups + 1) * 4), (p.last_rank, p.workgroups * 4), (p.inv_len, bags * 4),
-                (p.partial, p.workgroups * p.blocks * 2 * (vec << p.log_lanes) * 4), (p.bytes, 0)]
+                (p.partial, p.workgroups * p.blocks * 2 * (p.lane_cols << p.log_lanes) * 4), (p.bytes, 0)]
         for (a, size), (b, _) in zip(ends, ends[1:]):
             assert a % 256 == 0 and a + size <= b
 
