@@ -10,11 +10,10 @@
 //
 // 1. Keys: (table's first row number + clamped id, u) for each id; ids of the padding row and ids in no bag
 //    get the key `total`, which sorts last and is dropped. Bags are found from their starts in the tile.
-// 2. A radix sort by digits of at most 8 bits, least significant first, in tiles of 4,096: counts of every
-//    tile, then ranks within the tile (one ballot a bit finds the lanes of a wavefront that hold the same
-//    digit), the tile put in order in LDS and written out in runs. Every tile adds up the counts of the
-//    others itself where they are few (no further launch), else a scan kernel does. A single tile is sorted
-//    in LDS, all digits in one launch.
+// 2. A radix sort by digits of at most 11 bits, least significant first, in tiles of 4,096: counts of every
+//    tile, their sums over the tiles, then ranks within the tile (one ballot a bit finds the lanes of a
+//    wavefront that hold the same digit), the tile put in order in LDS and written out in runs. Few tiles add
+//    up the counts of the others themselves. A single tile is sorted in LDS, all digits in one launch.
 // 3. Sums: a workgroup takes a run of the sorted list, lane groups that cover a row's columns walk shares of
 //    it, several rows' loads in flight, and write a table row where its key ends inside the share. What
 //    crosses shares is added in LDS, what crosses workgroups goes to the workspace as fp32 rows, at most two
@@ -78,7 +77,6 @@ constexpr int kTile = kGradTile;  // keys a workgroup sorts
 constexpr int kSortThreads = 512;
 constexpr int kSortWaves = kSortThreads / kWave;
 constexpr int kItems = kTile / kSortThreads;  // keys a thread
-constexpr int kDigits = 256;
 constexpr int kMaxFields = 64;
 
 // Where the ids' bags and tables are.
@@ -117,66 +115,86 @@ __device__ __forceinline__ int64_t bag_edge(const GradSource& s, int64_t j, int 
   return clamp_i64(v, 0, s.n);
 }
 
-// How many bags start at or before p (the bags start in order): a search of 64 places a step. Called by a
-// whole wavefront, p uniform.
-__device__ __forceinline__ int64_t bags_started(const GradSource& s, int64_t p) {
-  int64_t lo = 0, hi = s.bags;  // the answer lies in [lo, hi]
-  while (lo < hi) {
-    const int64_t step = (hi - lo + kWave - 1) / kWave;
-    const int64_t j = lo + step * (lane_id() + 1) - 1;  // lane's last bag of its share
-    const bool started = j < hi && bag_edge(s, j, 0) <= p;
-    const int k = __popcll(__ballot(started));
-    lo += step * k;
-    const int64_t top = lo + step - 1;  // this bag has not started, or is past the end
-    if (top < hi) hi = top;
-  }
-  return lo;
-}
-
-// The key of id i of field f.
-__device__ __forceinline__ uint32_t grad_key(const GradSource& s, int64_t i, int f) {
+// The key of an id of field f.
+__device__ __forceinline__ uint32_t grad_key(const GradSource& s, int64_t id, int f) {
   const uint32_t at = s.per_field ? f : 0;
-  const int64_t id = load_id(s.ids, s.ids64, i, s.rows[at]);
+  id = clamp_i64(id, 0, static_cast<int64_t>(s.rows[at]) - 1);
   return id == s.padding ? s.total : s.base[at] + static_cast<uint32_t>(id);
 }
 
-constexpr int kMostBags = 4 * kTile;  // bags whose starts a tile looks through; with more, each id searches
+constexpr int kMostBags = 8 * kTile;  // bags whose starts a tile looks through; with more, each id searches
 
 // Keys and u of the tile's ids: item k of a thread is id tile * kTile + item_index(k). s_bag: kTile words.
 __device__ __forceinline__ int item_index(int k) {
   return (static_cast<int>(threadIdx.x) / kWave) * (kItems * kWave) + k * kWave + lane_id();
 }
 
+// The ids' own loads are under way while their bags are found: the tile's first bag by a search of 512 places a
+// step, the others by reading edges from there on, 512 at a time. Bag j's start is event 2 (j - lo) + 2 at its place,
+// its end event 2 (j - lo) + 3 at the place behind; the largest event up to an id is its bag's start (even), or an
+// end: the id lies in no bag. (Ends looked up id by id, a search of 64 places and one for the tile's last id:
+// 917,504 ids in 114,688 bags 16 us.)
 __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uint32_t* key, uint32_t* unit, int32_t* s_bag,
-                                          int64_t* s_range) {
+                                          int32_t* s_wave) {
   const int64_t first = tile * kTile;
+  const int t = static_cast<int>(threadIdx.x);
+  int64_t id[kItems];
+  const auto load_ids = [&](auto type) {
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      const int64_t i = first + item_index(k);
+      id[k] = static_cast<const decltype(type)*>(s.ids)[i < s.n ? i : s.n - 1];
+    }
+  };
+  if (s.ids64) load_ids(int64_t{});
+  else load_ids(int32_t{});
   if (!s.offsets) {
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       const int64_t i = first + item_index(k);
-      key[k] = i < s.n ? grad_key(s, i, 0) : 0xffffffffu;
+      key[k] = i < s.n ? grad_key(s, id[k], 0) : 0xffffffffu;
       unit[k] = static_cast<uint32_t>(i);
     }
     return;
   }
-  const int t = static_cast<int>(threadIdx.x);
-  const int64_t last = first + kTile < s.n ? first + kTile : s.n;
-  if (t < 2 * kWave) {
-    const int64_t r = bags_started(s, t < kWave ? first : last - 1);
-    if (lane_id() == 0) s_range[t / kWave] = r;
+  const int64_t last = (first + kTile < s.n ? first + kTile : s.n) - 1;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) s_bag[t + k * kSortThreads] = 0;
+  // bags that start at or before the first id
+  int64_t lo = 0, hi = s.bags;
+  while (lo < hi) {  // lo grows or hi falls in every step, whatever the offsets hold
+    const int64_t step = (hi - lo + kSortThreads - 1) / kSortThreads;
+    const int64_t j = lo + step * (t + 1) - 1;  // the thread's last bag of its share
+    const int started = __syncthreads_count(j < hi && bag_edge(s, j, 0) <= first);
+    lo += step * started;
+    if (lo + step - 1 < hi) hi = lo + step - 1;
   }
-  for (int i = t; i < kTile; i += kSortThreads) s_bag[i] = 0;
-  __syncthreads();
-  // bags [lo, hi) start in the tile after its first id; bag lo - 1 (or none) holds the first one
-  const int64_t lo = s_range[0], hi = s_range[1];
-  const bool scan = hi - lo <= kMostBags;
-  if (scan) {
-    // s_bag[p] = 1 + the last of them that starts at p, relative to lo; then the largest up to each place
-    for (int64_t j = lo + t; j < hi; j += kSortThreads) {
-      const int64_t at = bag_edge(s, j, 0) - first;
-      if (at >= 0 && at < kTile) atomicMax(&s_bag[at], static_cast<int32_t>(j - lo) + 1);
+  lo -= 1;  // the bag that holds the first id, or -1
+  // edges of bags lo, lo + 1, ... until one starts behind the tile
+  int64_t begun = 0;
+  bool scan = true;
+  for (int64_t j0 = lo;; j0 += kSortThreads) {
+    const int64_t j = j0 + t;
+    bool in = false;
+    if (j < s.bags) {
+      const int64_t a = j >= 0 ? bag_edge(s, j, 0) : 0, b = j >= 0 ? bag_edge(s, j, 1) : 0;
+      in = a <= last;
+      if (in && j >= 0) {
+        const int32_t event = static_cast<int32_t>(j - lo) * 2 + 2;
+        const int64_t at = a > first ? a - first : 0, end = b - first;
+        if (b > a) atomicMax(&s_bag[at], event);
+        if (end >= 0 && first + end <= last) atomicMax(&s_bag[end], event + 1);
+      }
     }
-    __syncthreads();
+    const int c = __syncthreads_count(in);
+    begun += c;
+    if (c < kSortThreads) break;
+    if (begun > kMostBags) {
+      scan = false;
+      break;
+    }
+  }
+  if (scan) {
     constexpr int kRun = kTile / kSortThreads;
     int32_t m[kRun], top = 0;
 #pragma unroll
@@ -191,12 +209,11 @@ __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uin
       const int32_t o = shfl_i32(before, lane_id() - d);
       if (lane_id() >= d) before = o > before ? o : before;
     }
-    __shared__ int32_t s_top[kSortWaves];
-    if (lane_id() == kWave - 1) s_top[t / kWave] = before;
+    if (lane_id() == kWave - 1) s_wave[t / kWave] = before;
     int32_t carry = shfl_i32(before, lane_id() - 1);
     if (lane_id() == 0) carry = 0;
     __syncthreads();
-    for (int w = 0; w < t / kWave; ++w) carry = s_top[w] > carry ? s_top[w] : carry;
+    for (int w = 0; w < t / kWave; ++w) carry = s_wave[w] > carry ? s_wave[w] : carry;
 #pragma unroll
     for (int k = 0; k < kRun; ++k) s_bag[t * kRun + k] = m[k] > carry ? m[k] : carry;
     __syncthreads();
@@ -207,36 +224,94 @@ __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uin
     key[k] = 0xffffffffu;
     unit[k] = 0u;
     if (i >= s.n) continue;
+    key[k] = s.total;
     int64_t j;
     if (scan) {
-      j = lo - 1 + s_bag[item_index(k)];
+      const int32_t event = s_bag[item_index(k)];
+      if (event == 0 || event % 2) continue;  // in no bag
+      j = lo + event / 2 - 1;
     } else {
-      int64_t a = lo, b = hi;  // bags started at or before i
+      int64_t a = lo + 1, b = s.bags;  // bags started at or before i
       while (a < b) {
         const int64_t mid = (a + b) / 2;
         if (bag_edge(s, mid, 0) <= i) a = mid + 1;
         else b = mid;
       }
       j = a - 1;
+      if (j < 0 || i >= bag_edge(s, j, 1)) continue;
     }
-    key[k] = s.total;
-    if (j < 0 || j >= s.bags || i >= bag_edge(s, j, 1)) continue;  // in no bag
     const int64_t f = s.by_batch.quotient(static_cast<uint32_t>(j));
-    key[k] = grad_key(s, i, static_cast<int>(f));
+    key[k] = grad_key(s, id[k], static_cast<int>(f));
     unit[k] = static_cast<uint32_t>((j - f * s.batch) * s.fields + f);
   }
 }
 
 // ---------------------------------------------------------------------------------------------
-// Gradient: sort
+// Gradient: rows without ids
 // ---------------------------------------------------------------------------------------------
-struct SortBuffers {
-  uint32_t* key;
-  uint32_t* unit;
+// What is written before the sums: zeros to whole tables, -1 to the compact form's numbers. It rides on the
+// sort's launches, whose few workgroups wait on latency: workgroups behind the sort's take shares of 64 KiB.
+constexpr int64_t kFillShare = 64 << 10;
+struct GradFill {
+  char* data[kMaxFields];
+  int64_t bytes[kMaxFields];       // rows * row_bytes
+  int64_t row_bytes[kMaxFields];   // to be written
+  int64_t row_stride[kMaxFields];  // bytes between rows
+  int32_t tables;
+  uint32_t value;
+  int32_t sort_groups;  // workgroups of this launch that sort
+  int32_t first_share;  // share of the first one behind them
 };
 
-// Exclusive sums over the first kDigits threads' values (the others pass 0); s_scan: kSortWaves words.
-__device__ __forceinline__ uint32_t digit_scan(uint32_t v, uint32_t* s_scan) {
+__device__ __forceinline__ void fill_share(const GradFill& f, int64_t share) {
+  int i = 0;
+  for (; i < f.tables; ++i) {
+    const int64_t shares = (f.bytes[i] + kFillShare - 1) / kFillShare;
+    if (share < shares) break;
+    share -= shares;
+  }
+  if (i == f.tables) return;
+  char* const data = f.data[i];
+  const int64_t a = share * kFillShare, b = a + kFillShare < f.bytes[i] ? a + kFillShare : f.bytes[i];
+  const int t = static_cast<int>(threadIdx.x);
+  if (f.row_stride[i] == f.row_bytes[i]) {
+    const u32x4 v = {f.value, f.value, f.value, f.value};
+    const int64_t whole = a + (b - a) / 16 * 16;
+#pragma unroll 8
+    for (int64_t at = a + t * 16; at < whole; at += blockDim.x * 16) *reinterpret_cast<u32x4_any*>(data + at) = v;
+    for (int64_t at = whole + t * 2; at < b; at += blockDim.x * 2) *reinterpret_cast<uint16_t*>(data + at) = static_cast<uint16_t>(f.value);
+  } else {
+    for (int64_t at = a + t * 2; at < b; at += blockDim.x * 2) {
+      const int64_t row = at / f.row_bytes[i];
+      *reinterpret_cast<uint16_t*>(data + row * f.row_stride[i] + (at - row * f.row_bytes[i])) = static_cast<uint16_t>(f.value);
+    }
+  }
+}
+
+// Whether the workgroup is one behind the sort's; then its share is written.
+__device__ __forceinline__ bool fills(const GradFill& f) {
+  const int extra = static_cast<int>(blockIdx.x) - f.sort_groups;
+  if (extra < 0) return false;
+  fill_share(f, static_cast<int64_t>(f.first_share) + extra);
+  return true;
+}
+
+// ---------------------------------------------------------------------------------------------
+// Gradient: sort
+// ---------------------------------------------------------------------------------------------
+// (key, u) of every id. Digits of up to kGradDigitBits = 11 bits (21 bits, two million rows, in two passes: 917,504
+// ids 46 us; in three of 7 bits, each tile adding up the counts of all tiles, 74).
+typedef uint2 Pair;
+
+// The tile of a workgroup: runs of tiles to each of the 8 XCDs, to which workgroups go in turn, so that what
+// neighbouring tiles write side by side meets in one L2.
+__device__ __forceinline__ int64_t tile_of(int64_t group, int64_t tiles) {
+  const int64_t per = tiles / 8, more = tiles % 8, xcd = group % 8;
+  return xcd * per + (xcd < more ? xcd : more) + group / 8;
+}
+
+// Exclusive sums over the workgroup's threads; s_scan: kSortWaves words.
+__device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* s_scan) {
   const int t = static_cast<int>(threadIdx.x);
   uint32_t x = v;
 #pragma unroll
@@ -249,226 +324,252 @@ __device__ __forceinline__ uint32_t digit_scan(uint32_t v, uint32_t* s_scan) {
   __syncthreads();
   uint32_t before = 0;
 #pragma unroll
-  for (int w = 0; w < kDigits / kWave; ++w) before += w < t / kWave ? s_scan[w] : 0u;
+  for (int w = 0; w < kSortWaves; ++w) before += w < t / kWave ? s_scan[w] : 0u;
   return before + x - v;
 }
 
-// Places of the tile's keys in the tile sorted by one digit (stable): place[k] of item k. s_start[d] is the
-// first place of digit d.
-__device__ __forceinline__ void tile_places(const uint32_t* key, int shift, int bits, uint32_t* place, uint32_t* s_hist,
+// Places of the tile's keys in the tile sorted by one digit (stable): place[k] of item k. s_hist: kSortWaves << bits
+// numbers; s_start[d] is the first place of digit d. A thread holds digits 4 t to 4 t + 3; counts[4] of them are the tile's.
+__device__ __forceinline__ void tile_places(const uint32_t* key, int shift, int bits, uint32_t* place, uint16_t* s_hist,
                                             uint32_t* s_start, uint32_t* s_scan) {
-  const int t = static_cast<int>(threadIdx.x), w = t / kWave;
-  const uint32_t mask = (1u << bits) - 1u;
-  for (int i = t; i < kSortWaves * kDigits; i += kSortThreads) s_hist[i] = 0u;
+  const int t = static_cast<int>(threadIdx.x), w = t / kWave, digits = 1 << bits;
+  const uint32_t mask = digits - 1;
+  uint2* const hist4 = reinterpret_cast<uint2*>(s_hist);
+  for (int i = t; i < kSortWaves * digits / 4; i += kSortThreads) hist4[i] = make_uint2(0u, 0u);
   __syncthreads();
-  volatile uint32_t* const mine = s_hist + w * kDigits;
-  const uint64_t below = (uint64_t{1} << lane_id()) - 1;
+  // the lanes with the same digit, of every item before the first one's turn, so that no ballot waits for LDS: where a
+  // lane's bit is like the lane's own (m: its bit in every place), same & ~(ones ^ m) keeps it
+  uint32_t lo[kItems], hi[kItems];
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) lo[k] = hi[k] = ~0u;
+#pragma unroll
+  for (int b = 0; b < kGradDigitBits; ++b) {
+    if (b < bits) {
+#pragma unroll
+      for (int k = 0; k < kItems; ++k) {
+        const uint32_t m = static_cast<uint32_t>(static_cast<int32_t>((key[k] >> shift) << (31 - b)) >> 31);
+        const uint64_t ones = __ballot(m != 0u);
+        lo[k] = __builtin_amdgcn_bitop3_b32(lo[k], static_cast<uint32_t>(ones), m, 0x90);
+        hi[k] = __builtin_amdgcn_bitop3_b32(hi[k], static_cast<uint32_t>(ones >> 32), m, 0x90);
+      }
+    }
+  }
+  volatile uint16_t* const mine = s_hist + w * digits;
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const uint32_t d = (key[k] >> shift) & mask;
-    uint64_t same = ~uint64_t{0};
-    for (int b = 0; b < bits; ++b) {
-      const bool one = (d >> b) & 1u;
-      const uint64_t ones = __ballot(one);
-      same &= one ? ones : ~ones;
-    }
     const uint32_t seen = mine[d];
-    const uint32_t rank = static_cast<uint32_t>(__popcll(same & below));
+    const uint32_t rank = __builtin_amdgcn_mbcnt_hi(hi[k], __builtin_amdgcn_mbcnt_lo(lo[k], 0u));  // lanes before this one
     place[k] = seen + rank;
     __builtin_amdgcn_wave_barrier();
-    if (rank == 0) mine[d] = seen + static_cast<uint32_t>(__popcll(same));
+    if (rank == 0) mine[d] = static_cast<uint16_t>(seen + static_cast<uint32_t>(__popc(lo[k]) + __popc(hi[k])));
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  uint32_t sum = 0;
-  if (t < kDigits) {
+  uint32_t sum[4] = {0u, 0u, 0u, 0u};
+  if (4 * t < digits) {
 #pragma unroll
     for (int i = 0; i < kSortWaves; ++i) {
-      const uint32_t c = s_hist[i * kDigits + t];
-      s_hist[i * kDigits + t] = sum;
-      sum += c;
+      const uint2 c = hist4[i * (digits / 4) + t];
+      hist4[i * (digits / 4) + t] = make_uint2(sum[0] | (sum[1] << 16), sum[2] | (sum[3] << 16));
+      sum[0] += c.x & 0xffffu, sum[1] += c.x >> 16, sum[2] += c.y & 0xffffu, sum[3] += c.y >> 16;
     }
   }
-  const uint32_t start = digit_scan(sum, s_scan);
-  if (t < kDigits) s_start[t] = start;
+  uint32_t start = group_scan(sum[0] + sum[1] + sum[2] + sum[3], s_scan);
+  if (4 * t < digits) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s_start[4 * t + i] = start;
+      start += sum[i];
+    }
+  }
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const uint32_t d = (key[k] >> shift) & mask;
-    place[k] += s_start[d] + s_hist[w * kDigits + d];
+    place[k] += s_start[d] + s_hist[w * digits + d];
   }
 }
 
 // All ids in one tile: keys and every digit in one launch.
-__global__ void __launch_bounds__(kSortThreads) grad_sort_tile_kernel(const GradSource s, SortBuffers out, int bits) {
-  __shared__ uint32_t s_key[kTile], s_unit[kTile];
-  __shared__ uint32_t s_hist[kSortWaves * kDigits], s_start[kDigits], s_scan[kSortWaves];
-  __shared__ int64_t s_range[2];
+__global__ void __launch_bounds__(kSortThreads) grad_sort_tile_kernel(const GradSource s, Pair* out, int all_bits, int digit_bits,
+                                                                      const GradFill fill) {
+  if (fills(fill)) return;
+  __shared__ Pair s_pair[kTile];
+  __shared__ uint16_t s_hist[kSortWaves * kGradDigits];
+  __shared__ uint32_t s_start[kGradDigits], s_scan[kSortWaves];
   uint32_t key[kItems], unit[kItems], place[kItems];
-  tile_keys(s, 0, key, unit, reinterpret_cast<int32_t*>(s_key), s_range);
-  for (int shift = 0; shift < bits; shift += 8) {
-    const int now = bits - shift < 8 ? bits - shift : 8;
-    tile_places(key, shift, now, place, s_hist, s_start, s_scan);
+  tile_keys(s, 0, key, unit, reinterpret_cast<int32_t*>(s_pair), reinterpret_cast<int32_t*>(s_scan));
+  for (int shift = 0; shift < all_bits; shift += digit_bits) {
+    tile_places(key, shift, digit_bits, place, s_hist, s_start, s_scan);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) s_pair[place[k]] = make_uint2(key[k], unit[k]);
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      s_key[place[k]] = key[k];
-      s_unit[place[k]] = unit[k];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      key[k] = s_key[item_index(k)];
-      unit[k] = s_unit[item_index(k)];
+      const Pair v = s_pair[item_index(k)];
+      key[k] = v.x;
+      unit[k] = v.y;
     }
     __syncthreads();
   }
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const int i = item_index(k);
-    if (i < s.n) {
-      out.key[i] = key[k];
-      out.unit[i] = unit[k];
-    }
+    if (i < s.n) out[i] = make_uint2(key[k], unit[k]);
   }
 }
 
 __device__ __forceinline__ void tile_count(const uint32_t* key, int64_t live, int shift, int bits, uint32_t* counts,
                                            uint32_t* s_hist) {
-  const int t = static_cast<int>(threadIdx.x);
-  const uint32_t mask = (1u << bits) - 1u;
-  __syncthreads();
-  for (int i = t; i < kDigits; i += kSortThreads) s_hist[i] = 0u;
+  const int t = static_cast<int>(threadIdx.x), digits = 1 << bits;
+  const uint32_t mask = digits - 1;
+  for (int i = t; i < digits; i += kSortThreads) s_hist[i] = 0u;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < kItems; ++k)
     if (item_index(k) < live) atomicAdd(&s_hist[(key[k] >> shift) & mask], 1u);
   __syncthreads();
-  for (int i = t; i < kDigits; i += kSortThreads) counts[i] = s_hist[i];
+  for (int i = t; i < digits; i += kSortThreads) counts[i] = s_hist[i];
 }
 
 // Keys of every tile and the counts of their first digit.
-__global__ void __launch_bounds__(kSortThreads) grad_keys_kernel(const GradSource s, SortBuffers out, uint32_t* counts, int bits) {
+__global__ void __launch_bounds__(kSortThreads) grad_keys_kernel(const GradSource s, Pair* out, uint32_t* counts, int bits,
+                                                                 const GradFill fill) {
+  if (fills(fill)) return;
   __shared__ int32_t s_bag[kTile];
-  __shared__ uint32_t s_hist[kDigits];
-  __shared__ int64_t s_range[2];
+  __shared__ uint32_t s_hist[kGradDigits];
+  __shared__ int32_t s_wave[kSortWaves];
   uint32_t key[kItems], unit[kItems];
-  tile_keys(s, blockIdx.x, key, unit, s_bag, s_range);
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kTile;
+  const int64_t tile = tile_of(blockIdx.x, fill.sort_groups), first = tile * kTile;
+  tile_keys(s, tile, key, unit, s_bag, s_wave);
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const int64_t i = first + item_index(k);
-    if (i < s.n) {
-      out.key[i] = key[k];
-      out.unit[i] = unit[k];
+    if (i < s.n) out[i] = make_uint2(key[k], unit[k]);
+  }
+  tile_count(key, s.n - first, 0, bits, counts + (tile << bits), s_hist);
+}
+
+__global__ void __launch_bounds__(kSortThreads) grad_count_kernel(const Pair* in, int64_t n, int shift, int bits, uint32_t* counts,
+                                                                  const GradFill fill) {
+  if (fills(fill)) return;
+  __shared__ uint32_t s_hist[kGradDigits];
+  uint32_t key[kItems];
+  const int64_t tile = tile_of(blockIdx.x, fill.sort_groups), first = tile * kTile;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = first + item_index(k);
+    key[k] = in[i < n ? i : n - 1].x;
+  }
+  tile_count(key, n - first, shift, bits, counts + (tile << bits), s_hist);
+}
+
+// counts[tile][digit] -> how many of the digit lie in tiles before it; totals[digit]. A lane takes a digit, the wavefronts
+// runs of tiles, up to kScanHeld of them in registers.
+constexpr int kScanThreads = 1024, kScanWaves = kScanThreads / kWave, kScanHeld = 16;
+__global__ void __launch_bounds__(kScanThreads) grad_scan_kernel(uint32_t* counts, uint32_t* totals, int64_t tiles, int bits,
+                                                                 const GradFill fill) {
+  if (fills(fill)) return;
+  __shared__ uint32_t s_sum[kScanWaves][kWave];
+  const int w = static_cast<int>(threadIdx.x) / kWave;
+  const int64_t digit = static_cast<int64_t>(blockIdx.x) * kWave + lane_id(), digits = int64_t{1} << bits;
+  const bool there = digit < digits;
+  const int64_t per = (tiles + kScanWaves - 1) / kScanWaves;
+  const int64_t a = per * w < tiles ? per * w : tiles, b = a + per < tiles ? a + per : tiles;
+  uint32_t* const col = counts + digit;
+  uint32_t held[kScanHeld], sum = 0;
+  const bool hold = per <= kScanHeld;
+  if (hold) {
+#pragma unroll
+    for (int k = 0; k < kScanHeld; ++k) held[k] = there && a + k < b ? col[(a + k) << bits] : 0u;
+#pragma unroll
+    for (int k = 0; k < kScanHeld; ++k) sum += held[k];
+  } else if (there) {
+#pragma unroll 8
+    for (int64_t i = a; i < b; ++i) sum += col[i << bits];
+  }
+  s_sum[w][lane_id()] = sum;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kScanWaves; ++i) {
+    const uint32_t c = s_sum[i][lane_id()];
+    before += i < w ? c : 0u;
+    all += c;
+  }
+  if (!there) return;
+  if (w == 0) totals[digit] = all;
+  if (hold) {
+#pragma unroll
+    for (int k = 0; k < kScanHeld; ++k) {
+      if (a + k < b) col[(a + k) << bits] = before;
+      before += held[k];
+    }
+  } else {
+    for (int64_t i = a; i < b; ++i) {
+      const uint32_t c = col[i << bits];
+      col[i << bits] = before;
+      before += c;
     }
   }
-  tile_count(key, s.n - first, 0, bits, counts + static_cast<int64_t>(blockIdx.x) * kDigits, s_hist);
 }
 
-__global__ void __launch_bounds__(kSortThreads) grad_count_kernel(const uint32_t* keys, int64_t n, int shift, int bits,
-                                                                  uint32_t* counts) {
-  __shared__ uint32_t s_hist[kDigits];
-  uint32_t key[kItems];
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * kTile;
-#pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int64_t i = first + item_index(k);
-    key[k] = i < n ? keys[i] : 0u;
-  }
-  tile_count(key, n - first, shift, bits, counts + static_cast<int64_t>(blockIdx.x) * kDigits, s_hist);
-}
-
-// counts[tile][digit] -> how many of the digit lie in tiles before it; totals[digit]. A workgroup takes four
-// digits, a thread a run of tiles.
-constexpr int kScanThreads = 256;
-__global__ void __launch_bounds__(kScanThreads) grad_scan_kernel(uint32_t* counts, uint32_t* totals, int64_t tiles) {
-  __shared__ uint4 s_sum[kScanThreads];
-  const int t = static_cast<int>(threadIdx.x);
-  const int64_t per = (tiles + kScanThreads - 1) / kScanThreads;
-  const int64_t a = per * t < tiles ? per * t : tiles, b = a + per < tiles ? a + per : tiles;
-  uint4* const col = reinterpret_cast<uint4*>(counts) + blockIdx.x;
-  uint4 sum = make_uint4(0u, 0u, 0u, 0u);
-  for (int64_t i = a; i < b; ++i) {
-    const uint4 c = col[i * (kDigits / 4)];
-    sum.x += c.x, sum.y += c.y, sum.z += c.z, sum.w += c.w;
-  }
-  s_sum[t] = sum;
-  __syncthreads();
-  uint4 before = make_uint4(0u, 0u, 0u, 0u);
-  for (int i = 0; i < kScanThreads; ++i) {
-    if (i == t) sum = before;
-    const uint4 c = s_sum[i];
-    before.x += c.x, before.y += c.y, before.z += c.z, before.w += c.w;
-  }
-  if (t == 0) reinterpret_cast<uint4*>(totals)[blockIdx.x] = before;
-  for (int64_t i = a; i < b; ++i) {
-    const uint4 c = col[i * (kDigits / 4)];
-    col[i * (kDigits / 4)] = sum;
-    sum.x += c.x, sum.y += c.y, sum.z += c.z, sum.w += c.w;
-  }
-}
-
-// One digit: the tile in order, written to its places. totals NULL: counts are the tiles' own.
-__global__ void __launch_bounds__(kSortThreads) grad_scatter_kernel(SortBuffers in, SortBuffers out, int64_t n, int shift, int bits,
-                                                                    const uint32_t* counts, const uint32_t* totals, int tiles) {
-  __shared__ uint32_t s_key[kTile], s_unit[kTile];
-  __shared__ uint32_t s_hist[kSortWaves * kDigits], s_start[kDigits], s_scan[kSortWaves], s_base[kDigits];
-  const int t = static_cast<int>(threadIdx.x), tile = static_cast<int>(blockIdx.x);
-  const int64_t first = static_cast<int64_t>(tile) * kTile;
+// One digit: the tile in order, written to its places. totals NULL: counts are the few tiles' own.
+__global__ void __launch_bounds__(kSortThreads) grad_scatter_kernel(const Pair* in, Pair* out, int64_t n, int shift, int bits,
+                                                                    const uint32_t* counts, const uint32_t* totals,
+                                                                    const GradFill fill) {
+  if (fills(fill)) return;
+  __shared__ Pair s_pair[kTile];
+  __shared__ uint16_t s_hist[kSortWaves * kGradDigits];
+  __shared__ uint32_t s_start[kGradDigits], s_scan[kSortWaves];
+  const int t = static_cast<int>(threadIdx.x), digits = 1 << bits;
+  const int64_t tile = tile_of(blockIdx.x, fill.sort_groups), first = tile * kTile;
   uint32_t key[kItems], unit[kItems], place[kItems];
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const int64_t i = first + item_index(k);
-    key[k] = i < n ? in.key[i] : 0xffffffffu;
-    unit[k] = i < n ? in.unit[i] : 0u;
+    const Pair v = in[i < n ? i : n - 1];
+    key[k] = i < n ? v.x : 0xffffffffu;
+    unit[k] = v.y;
   }
-  uint32_t before = 0, total = 0;
-  if (totals) {
-    if (t < kDigits) {
-      before = counts[static_cast<int64_t>(tile) * kDigits + t];
-      total = totals[t];
-    }
-  } else {
-    // a wavefront adds up every kSortWaves-th tile, a lane four digits
+  uint4 before = make_uint4(0u, 0u, 0u, 0u), total = before;
+  if (4 * t < digits) {
     const uint4* const c4 = reinterpret_cast<const uint4*>(counts);
-    uint4 b4 = make_uint4(0u, 0u, 0u, 0u), t4 = b4;
-#pragma unroll 8
-    for (int i = t / kWave; i < tiles; i += kSortWaves) {
-      const uint4 c = c4[i * (kDigits / 4) + lane_id()];
-      t4.x += c.x, t4.y += c.y, t4.z += c.z, t4.w += c.w;
-      if (i < tile) b4.x += c.x, b4.y += c.y, b4.z += c.z, b4.w += c.w;
-    }
-    reinterpret_cast<uint4*>(s_key)[t] = b4;  // [wavefront][digit]
-    reinterpret_cast<uint4*>(s_unit)[t] = t4;
-    __syncthreads();
-    if (t < kDigits) {
-#pragma unroll
-      for (int w = 0; w < kSortWaves; ++w) {
-        before += s_key[w * kDigits + t];
-        total += s_unit[w * kDigits + t];
+    if (totals) {
+      before = c4[tile * (digits / 4) + t];
+      total = reinterpret_cast<const uint4*>(totals)[t];
+    } else {
+#pragma unroll 16
+      for (int i = 0; i < fill.sort_groups; ++i) {
+        const uint4 c = c4[i * (digits / 4) + t];
+        const uint32_t m = i < tile ? ~0u : 0u;  // (a branch would wait for every load)
+        total.x += c.x, total.y += c.y, total.z += c.z, total.w += c.w;
+        before.x += c.x & m, before.y += c.y & m, before.z += c.z & m, before.w += c.w & m;
       }
     }
   }
-  const uint32_t digits_before = digit_scan(total, s_scan);
-  if (t < kDigits) s_base[t] = digits_before + before;
+  const uint32_t base = group_scan(total.x + total.y + total.z + total.w, s_scan);
   tile_places(key, shift, bits, place, s_hist, s_start, s_scan);
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    s_key[place[k]] = key[k];
-    s_unit[place[k]] = unit[k];
+  for (int k = 0; k < kItems; ++k) s_pair[place[k]] = make_uint2(key[k], unit[k]);
+  __syncthreads();
+  if (4 * t < digits) {  // s_start becomes the way from a place in the tile to the place in the list
+    uint32_t* const at = s_start + 4 * t;
+    at[0] = base + before.x - at[0];
+    at[1] = base + total.x + before.y - at[1];
+    at[2] = base + total.x + total.y + before.z - at[2];
+    at[3] = base + total.x + total.y + total.z + before.w - at[3];
   }
   __syncthreads();
-  const uint32_t mask = (1u << bits) - 1u;
   const int64_t live = n - first;
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const int i = item_index(k);
     if (i < live) {  // keys past the end are the tile's last: their digit is the largest and they come last
-      const uint32_t v = s_key[i], d = (v >> shift) & mask;
-      const uint32_t to = s_base[d] + static_cast<uint32_t>(i) - s_start[d];
-      out.key[to] = v;
-      out.unit[to] = s_unit[i];
+      const Pair v = s_pair[i];
+      out[s_start[(v.x >> shift) & (digits - 1)] + static_cast<uint32_t>(i)] = v;
     }
   }
 }
@@ -482,8 +583,7 @@ constexpr int kSumAhead = 8;    // rows a lane group loads at once
 
 struct SumParams {
   const char* grad;
-  const uint32_t* key;
-  const uint32_t* unit;
+  const Pair* ids;        // sorted
   const float* inv_len;
   const uint32_t* heads;  // compact: distinct keys that begin in each workgroup's run (or before it: scanned)
   int32_t heads_scanned;
@@ -502,6 +602,7 @@ struct SumParams {
   int32_t workgroups;
   float scale;
   int32_t fields;
+  int32_t per_field;      // tables in SumFields
   ChunkDivide by_fields;
 };
 // A table for each field.
@@ -515,7 +616,7 @@ struct SumFields {
 struct NoFields {};
 
 // Distinct keys that begin in each run of `ids`.
-__global__ void __launch_bounds__(kSumThreads) grad_heads_kernel(const uint32_t* key, int64_t n, uint32_t total, int ids,
+__global__ void __launch_bounds__(kSumThreads) grad_heads_kernel(const Pair* sorted, int64_t n, uint32_t total, int ids,
                                                                  uint32_t* heads) {
   __shared__ uint32_t s_sum[kSumThreads / kWave];
   const int64_t first = static_cast<int64_t>(blockIdx.x) * ids;
@@ -523,8 +624,8 @@ __global__ void __launch_bounds__(kSumThreads) grad_heads_kernel(const uint32_t*
   for (int i = static_cast<int>(threadIdx.x); i < ids; i += kSumThreads) {
     const int64_t at = first + i;
     if (at < n) {
-      const uint32_t k = key[at];
-      c += k < total && (at == 0 || key[at - 1] != k) ? 1u : 0u;
+      const uint32_t k = sorted[at].x;
+      c += k < total && (at == 0 || sorted[at - 1].x != k) ? 1u : 0u;
     }
   }
 #pragma unroll
@@ -654,8 +755,9 @@ __global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p
   const int live = static_cast<int>(p.n - first < ids ? p.n - first : ids);
   for (int i = t; i < live + 2; i += kSumThreads) {
     const int64_t at = first + i - 1;
-    s_key[i] = at >= 0 && at < p.n ? p.key[at] : 0xffffffffu;  // no key is that large
-    if (i < live) s_unit[i] = p.unit[first + i];
+    const Pair v = at >= 0 && at < p.n ? p.ids[at] : make_uint2(0xffffffffu, 0u);  // no key is that large
+    s_key[i] = v.x;
+    if (i > 0 && i <= live) s_unit[i - 1] = v.y;
   }
   uint32_t begun = 0;  // distinct keys before this run
   if (p.rows_out) {
@@ -852,12 +954,16 @@ __device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) {
   return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
 
-template <typename T, typename OT, typename FIELDS, int COLS, bool MEAN>
-__global__ void __launch_bounds__(kSumThreads) grad_walk_kernel(const SumParams p, const FIELDS fs) {
-  using S = Sums<T, OT, FIELDS>;
+// Wavefronts a SIMD that the registers leave room for: all of a launch of a million ids at once where an id's columns are few.
+template <int BYTES>
+constexpr int kWalkPerSimd = BYTES <= 4 ? 8 : 4;
+
+template <typename T, typename OT, int COLS, bool MEAN>
+__global__ void __launch_bounds__(kSumThreads, (kWalkPerSimd<COLS * Elem<T>::kBytes>)) grad_walk_kernel(const SumParams p, const SumFields fs) {
   constexpr int AHEAD = COLS * Elem<T>::kBytes >= 16 ? 8 : 16;  // rows whose loads are in flight
   __shared__ float s_part[2][kWalkWaves][kWave * COLS];
-  __shared__ uint32_t s_flag[2][kWalkWaves], s_key[kWalkWaves], s_unit[kWalkWaves], s_rank[kWalkWaves], s_heads[kWalkWaves];
+  __shared__ uint32_t s_flag[2][kWalkWaves], s_heads[kWalkWaves];
+  __shared__ char* s_target[kWalkWaves];  // of each wavefront's first key
   __shared__ uint32_t s_sum[2][kSumThreads / kWave];
   const int t = static_cast<int>(threadIdx.x), lane = lane_id();
   const int w = __builtin_amdgcn_readfirstlane(t / kWave);
@@ -870,14 +976,15 @@ __global__ void __launch_bounds__(kSumThreads) grad_walk_kernel(const SumParams 
   uint64_t begins[kWalkBatches];  // whose key is another than the id's before
   int live = 0;                   // ids that are not dropped: those come last
   uint32_t heads = 0;
-  const uint32_t before = have && first > 0 ? p.key[first - 1] : 0xffffffffu;  // no key is that large
-  const uint32_t behind = have && first + have < p.n ? p.key[first + have] : 0xffffffffu;
+  const uint32_t before = have && first > 0 ? p.ids[first - 1].x : 0xffffffffu;  // no key is that large
+  const uint32_t behind = have && first + have < p.n ? p.ids[first + have].x : 0xffffffffu;
 #pragma unroll
   for (int b = 0; b < kWalkBatches; ++b) {
     const int i = b * kWave + lane;
     const bool in = i < have;
-    key[b] = in ? p.key[first + i] : 0xffffffffu;
-    unit[b] = in ? p.unit[first + i] : 0u;
+    const Pair v = in ? p.ids[first + i] : make_uint2(0xffffffffu, 0u);
+    key[b] = v.x;
+    unit[b] = v.y;
   }
 #pragma unroll
   for (int b = 0; b < kWalkBatches; ++b) {
@@ -892,7 +999,24 @@ __global__ void __launch_bounds__(kSumThreads) grad_walk_kernel(const SumParams 
   }
   const uint32_t first_key = lane_value(key[0], 0);
   bool open = live > 0 && before == first_key;  // the first key began before
-  uint32_t rank = 0;                            // of the current key
+  const int c0 = first_column(block, lane, p.dim, COLS);
+  const uint32_t lane_at = static_cast<uint32_t>(c0 < 0 ? 0 : c0) * Elem<T>::kBytes;  // lanes without columns read the first
+  uint64_t source[kWalkBatches];  // each id's row of grad
+#pragma unroll
+  for (int b = 0; b < kWalkBatches; ++b)
+    source[b] = reinterpret_cast<uint64_t>(p.grad) + static_cast<uint64_t>(unit[b]) * (static_cast<uint64_t>(p.dim) * Elem<T>::kBytes);
+  const auto of_lane = [&](uint64_t v, int i) {
+    return reinterpret_cast<char*>((static_cast<uint64_t>(lane_value(static_cast<uint32_t>(v >> 32), i)) << 32) |
+                                   lane_value(static_cast<uint32_t>(v), i));
+  };
+  LaneCols<T, COLS> rows[2][AHEAD];
+  const auto fetch = [&](int b, int i0, LaneCols<T, COLS>* to) {
+    const int last = (live - b * kWave < kWave ? live - b * kWave : kWave) - 1;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) to[u].load(of_lane(source[b], i0 + u < last ? i0 + u : last) + lane_at);
+  };
+  if (live > 0) fetch(0, 0, rows[0]);  // under way while the places of the sums are found
+  uint32_t rank = 0;
   if (p.rows_out) {
     uint32_t all;
     if (lane == 0) s_heads[w] = heads;
@@ -901,26 +1025,30 @@ __global__ void __launch_bounds__(kSumThreads) grad_walk_kernel(const SumParams 
     if (blockIdx.x == 0 && block == 0 && t == 0) *p.count_out = all;
     for (int i = 0; i < w; ++i) rank += s_heads[i];
     rank = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(rank)));
-    if (block == 0) {
-      uint32_t r = rank;
-#pragma unroll
-      for (int b = 0; b < kWalkBatches; ++b) {
-        if ((begins[b] >> lane) & 1) p.rows_out[r + static_cast<uint32_t>(__popcll(begins[b] & ((uint64_t{1} << lane) - 1)))] = key[b];
-        r += static_cast<uint32_t>(__popcll(begins[b]));
-      }
-      if (have && lane == 0 && (w == kWalkWaves - 1 || rest <= p.run)) p.last_rank[blockIdx.x] = r - 1u;
-    }
-    rank -= 1u;
   }
+  // Where the sum of each id's key goes: a lane for an id, so that no key's end waits for its table's numbers.
+  uint64_t target[kWalkBatches];
+#pragma unroll
+  for (int b = 0; b < kWalkBatches; ++b) {
+    target[b] = 0;
+    if (p.rows_out) {
+      const uint32_t r = rank + static_cast<uint32_t>(__popcll(begins[b] & (~uint64_t{0} >> (kWave - 1 - lane)))) - 1u;
+      if (block == 0 && ((begins[b] >> lane) & 1)) p.rows_out[r] = key[b];
+      rank += static_cast<uint32_t>(__popcll(begins[b]));
+      target[b] = reinterpret_cast<uint64_t>(p.out + static_cast<int64_t>(r) * p.dim * Elem<OT>::kBytes);
+    } else if (key[b] < p.total) {
+      target[b] = reinterpret_cast<uint64_t>(
+          p.per_field ? Sums<T, OT, SumFields>::target(p, fs, key[b], unit[b], 0u)
+                      : p.out + static_cast<int64_t>(key[b]) * p.dim * Elem<OT>::kBytes);
+    }
+  }
+  if (p.rows_out && block == 0 && have && lane == 0 && (w == kWalkWaves - 1 || rest <= p.run)) p.last_rank[blockIdx.x] = rank - 1u;
   uint32_t flag0 = 0, flag1 = 0;
-  const int c0 = first_column(block, lane, p.dim, COLS);
-  const uint32_t first_unit = lane_value(unit[0], 0), first_rank = rank;
   float acc[COLS];
 #pragma unroll
   for (int e = 0; e < COLS; ++e) acc[e] = 0.f;
-  const int64_t row_bytes = static_cast<int64_t>(p.dim) * Elem<T>::kBytes;
-  const uint32_t lane_at = static_cast<uint32_t>(c0 < 0 ? 0 : c0) * Elem<T>::kBytes;  // lanes without columns read the first
-  uint32_t cur_key = first_key, cur_unit = first_unit;
+  char* const first_target = of_lane(target[0], 0);
+  char* cur_target = first_target;
   const auto finish = [&]() {
     if (open) {
       flag0 = 1;
@@ -928,61 +1056,53 @@ __global__ void __launch_bounds__(kSumThreads) grad_walk_kernel(const SumParams 
       for (int e = 0; e < COLS; ++e) s_part[0][w][lane * COLS + e] = acc[e];
       open = false;
     } else {
-      char* const row = S::target(p, fs, cur_key, cur_unit, rank);
       float v[COLS];
 #pragma unroll
       for (int e = 0; e < COLS; ++e) v[e] = acc[e] * p.scale;
-      if (c0 >= 0) store_cols<OT, COLS>(row + static_cast<uint32_t>(c0) * Elem<OT>::kBytes, v);
+      if (c0 >= 0) store_cols<OT, COLS>(cur_target + static_cast<uint32_t>(c0) * Elem<OT>::kBytes, v);
     }
 #pragma unroll
     for (int e = 0; e < COLS; ++e) acc[e] = 0.f;
   };
-  bool any = false;
 #pragma unroll
   for (int b = 0; b < kWalkBatches; ++b) {
     const int now = live - b * kWave < kWave ? live - b * kWave : kWave;
     if (now <= 0) break;
-    LaneCols<T, COLS> rows[2][AHEAD];
-    const auto fetch = [&](int i0, LaneCols<T, COLS>* to) {
+    const auto add = [&](int i, const LaneCols<T, COLS>& row) {
+      if ((begins[b] >> i) & 1) {
+        if (b + i > 0) finish();
+        cur_target = of_lane(target[b], i);
+      }
+      if constexpr (MEAN) {
+        const float f = __uint_as_float(lane_value(__float_as_uint(weight[b]), i));
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int i = i0 + u < now ? i0 + u : now - 1;
-        to[u].load(p.grad + static_cast<int64_t>(lane_value(unit[b], i)) * row_bytes + lane_at);
+        for (int e = 0; e < COLS; ++e) acc[e] = __builtin_fmaf(row.value(e), f, acc[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < COLS; ++e) acc[e] += row.value(e);
       }
     };
-    const auto add = [&](int i0, const LaneCols<T, COLS>* from) {
+    const auto add_all = [&](int i0, const LaneCols<T, COLS>* from) {
+      if (i0 + AHEAD <= now) {
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int i = i0 + u;
-        if (i < now) {
-          if ((begins[b] >> i) & 1) {
-            if (any) finish();
-            cur_key = lane_value(key[b], i);
-            cur_unit = lane_value(unit[b], i);
-            rank += 1u;
-          }
-          any = true;
-          if constexpr (MEAN) {
-            const float f = __uint_as_float(lane_value(__float_as_uint(weight[b]), i));
+        for (int u = 0; u < AHEAD; ++u) add(i0 + u, from[u]);
+      } else {
 #pragma unroll
-            for (int e = 0; e < COLS; ++e) acc[e] = __builtin_fmaf(from[u].value(e), f, acc[e]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < COLS; ++e) acc[e] += from[u].value(e);
-          }
-        }
+        for (int u = 0; u < AHEAD; ++u)
+          if (i0 + u < now) add(i0 + u, from[u]);
       }
     };
-    fetch(0, rows[0]);
+    if (b > 0) fetch(b, 0, rows[0]);
     for (int i0 = 0; i0 < now; i0 += 2 * AHEAD) {
-      if (i0 + AHEAD < now) fetch(i0 + AHEAD, rows[1]);
-      add(i0, rows[0]);
-      if (i0 + 2 * AHEAD < now) fetch(i0 + 2 * AHEAD, rows[0]);
-      add(i0 + AHEAD, rows[1]);
+      if (i0 + AHEAD < now) fetch(b, i0 + AHEAD, rows[1]);
+      add_all(i0, rows[0]);
+      if (i0 + 2 * AHEAD < now) fetch(b, i0 + 2 * AHEAD, rows[0]);
+      add_all(i0 + AHEAD, rows[1]);
     }
   }
-  if (any) {
-    if (live == have && behind == cur_key) {  // goes on behind the wavefront's ids
+  if (live > 0) {
+    const uint32_t last_key = lane_value(live > kWave ? key[1] : key[0], (live - 1) % kWave);
+    if (live == have && behind == last_key) {  // goes on behind the wavefront's ids
       const int which = open ? 0 : 1;
       if (open) flag0 = 2;
       else flag1 = 1;
@@ -995,9 +1115,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_walk_kernel(const SumParams 
   if (lane == 0) {
     s_flag[0][w] = flag0;
     s_flag[1][w] = flag1;
-    s_key[w] = first_key;
-    s_unit[w] = first_unit;
-    s_rank[w] = first_rank;
+    s_target[w] = first_target;
   }
   __syncthreads();
 
@@ -1019,7 +1137,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_walk_kernel(const SumParams 
           } else {
             const int at = first_column(block, slot / COLS, p.dim, COLS);
             if (at >= 0)
-              store_one(reinterpret_cast<OT*>(S::target(p, fs, s_key[i], s_unit[i], s_rank[i])) + at + slot % COLS, carry * p.scale, false);
+              store_one(reinterpret_cast<OT*>(s_target[i]) + at + slot % COLS, carry * p.scale, false);
           }
           began = carrying = false;
           carry = 0.f;
@@ -1045,14 +1163,14 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams 
   const int block = static_cast<int>(blockIdx.y);
   const int64_t next = first + ids;
   if (next >= p.n) return;
-  const uint32_t key = p.key[next - 1];
-  if (key >= p.total || p.key[next] != key) return;                 // ends with the run
-  if (first > 0 && p.key[first] == key && p.key[first - 1] == key) return;  // began in a run before
+  const uint32_t key = p.ids[next - 1].x;
+  if (key >= p.total || p.ids[next].x != key) return;                       // ends with the run
+  if (first > 0 && p.ids[first].x == key && p.ids[first - 1].x == key) return;  // began in a run before
   // runs that begin with the key
   int follow = 0;
   for (int at = static_cast<int>(blockIdx.x) + 1;; at += kSumThreads) {
     const int64_t i = static_cast<int64_t>(at + t) * ids;
-    const int c = __syncthreads_count(at + t < p.workgroups && i < p.n && p.key[i] == key);
+    const int c = __syncthreads_count(at + t < p.workgroups && i < p.n && p.ids[i].x == key);
     follow += c;
     if (c < kSumThreads) break;
   }
@@ -1061,7 +1179,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams 
   const float* const mine = p.partial + (static_cast<int64_t>(block) * p.workgroups + blockIdx.x) * row_floats;
   const int q = t % quads, r = t / quads;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
   for (int h = r; h < follow; h += rows) {
     const float4 v = *reinterpret_cast<const float4*>(mine + (h + 1) * row_floats + q * 4);
     sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
@@ -1075,7 +1193,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams 
     sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
   }
   const uint32_t rank = p.rows_out ? p.last_rank[blockIdx.x] : 0u;
-  const uint32_t unit = p.unit[next - 1];
+  const uint32_t unit = p.ids[next - 1].y;
   const int dim = S::width(p, fs, unit);
   const float v[4] = {sum.x, sum.y, sum.z, sum.w};
   OT* const row = reinterpret_cast<OT*>(S::target(p, fs, key, unit, rank));
@@ -1094,32 +1212,9 @@ __global__ void __launch_bounds__(256) grad_lengths_kernel(const GradSource s) {
   s.inv_len[(j - f * s.batch) * s.fields + f] = len > 0 ? 1.0f / static_cast<float>(len) : 1.0f;
 }
 
-// Rows of zeros: blockIdx.y is the table.
-struct FillParams {
-  char* data[kMaxFields];
-  int64_t rows[kMaxFields];
-  int64_t row_bytes[kMaxFields];   // to clear
-  int64_t row_stride[kMaxFields];  // bytes
-};
-__global__ void __launch_bounds__(256) grad_fill_rows_kernel(const FillParams p) {
-  const int f = static_cast<int>(blockIdx.y);
-  char* const data = p.data[f];
-  if (!data) return;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, all = static_cast<int64_t>(gridDim.x) * 256;
-  if (p.row_stride[f] == p.row_bytes[f]) {
-    const int64_t bytes = p.rows[f] * p.row_bytes[f], whole = bytes / 16;
-    for (int64_t i = at; i < whole; i += all) *reinterpret_cast<u32x4_any*>(data + i * 16) = u32x4{0u, 0u, 0u, 0u};
-    for (int64_t i = whole * 16 + at * 2; i < bytes; i += all * 2) *reinterpret_cast<uint16_t*>(data + i) = 0;
-    return;
-  }
-  for (int64_t r = at / kWave; r < p.rows[f]; r += all / kWave)
-    for (int64_t i = lane_id() * 2; i < p.row_bytes[f]; i += kWave * 2)
-      *reinterpret_cast<uint16_t*>(data + r * p.row_stride[f] + i) = 0;
-}
-__global__ void __launch_bounds__(256) grad_fill_numbers_kernel(int64_t* rows, int64_t capacity, int64_t* count) {
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  for (int64_t i = at; i < capacity; i += static_cast<int64_t>(gridDim.x) * 256) rows[i] = -1;
-  if (at == 0) *count = 0;
+__global__ void __launch_bounds__(kSortThreads) grad_fill_kernel(const GradFill f, int64_t* count_out) {
+  fill_share(f, blockIdx.x);
+  if (count_out && blockIdx.x == 0 && threadIdx.x == 0) *count_out = 0;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -1138,27 +1233,30 @@ struct GradCall {
   int64_t workspace_bytes = 0;
 };
 
-template <typename T, typename OT, typename FIELDS, int COLS>
-void launch_walk(const SumParams& p, const FIELDS& fs, dim3 grid, hipStream_t s) {
+template <typename T, typename OT, int COLS>
+void launch_walk(const SumParams& p, const SumFields& fs, dim3 grid, hipStream_t s) {
   if constexpr (COLS * Elem<T>::kBytes <= 16) {
-    if (p.inv_len) hipLaunchKernelGGL((grad_walk_kernel<T, OT, FIELDS, COLS, true>), grid, dim3(kSumThreads), 0, s, p, fs);
-    else hipLaunchKernelGGL((grad_walk_kernel<T, OT, FIELDS, COLS, false>), grid, dim3(kSumThreads), 0, s, p, fs);
+    if (p.inv_len) hipLaunchKernelGGL((grad_walk_kernel<T, OT, COLS, true>), grid, dim3(kSumThreads), 0, s, p, fs);
+    else hipLaunchKernelGGL((grad_walk_kernel<T, OT, COLS, false>), grid, dim3(kSumThreads), 0, s, p, fs);
   }
 }
 template <typename T, typename OT, typename FIELDS>
-void launch_sums(const SumParams& p, const FIELDS& fs, int blocks, bool walk, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(p.workgroups), static_cast<unsigned>(blocks));
-  if (!walk) hipLaunchKernelGGL((grad_sum_kernel<T, OT, FIELDS>), grid, dim3(kSumThreads), 0, s, p, fs);
-  else if (p.lane_cols == 1) launch_walk<T, OT, FIELDS, 1>(p, fs, grid, s);
-  else if (p.lane_cols == 2) launch_walk<T, OT, FIELDS, 2>(p, fs, grid, s);
-  else if (p.lane_cols == 4) launch_walk<T, OT, FIELDS, 4>(p, fs, grid, s);
-  else launch_walk<T, OT, FIELDS, 8>(p, fs, grid, s);
+void launch_groups(const SumParams& p, const FIELDS& fs, bool walked, dim3 grid, hipStream_t s) {
+  if (!walked) hipLaunchKernelGGL((grad_sum_kernel<T, OT, FIELDS>), grid, dim3(kSumThreads), 0, s, p, fs);
   if (p.workgroups > 1) hipLaunchKernelGGL((grad_join_kernel<T, OT, FIELDS>), grid, dim3(kSumThreads), 0, s, p, fs);
 }
 template <typename T, typename OT>
 void launch_sums_for(const GradCall& c, int blocks, hipStream_t s) {
-  if (c.per_field) launch_sums<T, OT, SumFields>(c.sum, c.fields, blocks, c.walk, s);
-  else launch_sums<T, OT, NoFields>(c.sum, NoFields{}, blocks, c.walk, s);
+  const SumParams& p = c.sum;
+  const dim3 grid(static_cast<unsigned>(p.workgroups), static_cast<unsigned>(blocks));
+  if (c.walk) {
+    if (p.lane_cols == 1) launch_walk<T, OT, 1>(p, c.fields, grid, s);
+    else if (p.lane_cols == 2) launch_walk<T, OT, 2>(p, c.fields, grid, s);
+    else if (p.lane_cols == 4) launch_walk<T, OT, 4>(p, c.fields, grid, s);
+    else launch_walk<T, OT, 8>(p, c.fields, grid, s);
+  }
+  if (c.per_field) launch_groups<T, OT, SumFields>(p, c.fields, c.walk, grid, s);
+  else launch_groups<T, OT, NoFields>(p, NoFields{}, c.walk, grid, s);
 }
 template <typename T>
 void launch_sums_typed(const GradCall& c, int blocks, hipStream_t s) {
@@ -1173,34 +1271,39 @@ void launch_sums_typed(const GradCall& c, int blocks, hipStream_t s) {
 int run_gradient(GradCall& c, hipStream_t s) {
   const int64_t n = c.src.n;
   const bool compact = c.sum.rows_out != nullptr;
+  GradFill fill{};
+  int64_t shares = 0;
+  const auto fill_table = [&](char* data, int64_t rows, int64_t row_bytes, int64_t row_stride) {
+    for (int k = 0; k < fill.tables; ++k)
+      if (fill.data[k] == data) return;  // fields that share a table
+    const int i = fill.tables++;
+    fill.data[i] = data;
+    fill.bytes[i] = rows * row_bytes;
+    fill.row_bytes[i] = row_bytes;
+    fill.row_stride[i] = row_stride;
+    shares += (fill.bytes[i] + kFillShare - 1) / kFillShare;
+  };
+  const int eb = dtype_bytes(c.out_dtype);
   if (compact) {
-    const int64_t blocks = (c.capacity + 255) / 256;
-    hipLaunchKernelGGL(grad_fill_numbers_kernel, dim3(static_cast<unsigned>(blocks < 1 ? 1 : blocks > 1024 ? 1024 : blocks)), dim3(256),
-                       0, s, c.sum.rows_out, c.capacity, c.sum.count_out);
+    fill.value = 0xffffffffu;
+    fill_table(reinterpret_cast<char*>(c.sum.rows_out), c.capacity, 8, 8);
+  } else if (c.per_field) {
+    for (int f = 0; f < c.src.fields; ++f)
+      fill_table(c.fields.data[f], c.src.rows[f], static_cast<int64_t>(c.fields.dim[f]) * eb, c.fields.stride[f] * eb);
   } else {
-    FillParams f{};
-    const int eb = dtype_bytes(c.out_dtype), tables = c.per_field ? c.src.fields : 1;
-    int64_t most = 0;
-    for (int i = 0; i < tables; ++i) {
-      f.data[i] = c.per_field ? c.fields.data[i] : c.sum.out;
-      f.rows[i] = c.src.rows[i];
-      f.row_bytes[i] = static_cast<int64_t>(c.per_field ? c.fields.dim[i] : c.sum.dim) * eb;
-      f.row_stride[i] = c.per_field ? c.fields.stride[i] * eb : f.row_bytes[i];
-      for (int k = 0; k < i; ++k)
-        if (f.data[k] == f.data[i]) f.data[i] = nullptr;  // fields that share a table
-      if (f.data[i] && f.rows[i] * f.row_bytes[i] > most) most = f.rows[i] * f.row_bytes[i];
-    }
-    int64_t blocks = (most + 16 * 256 - 1) / (16 * 256);
-    if (blocks > 4096) blocks = 4096;
-    hipLaunchKernelGGL(grad_fill_rows_kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(tables)), dim3(256), 0, s, f);
+    fill_table(c.sum.out, c.src.rows[0], static_cast<int64_t>(c.sum.dim) * eb, static_cast<int64_t>(c.sum.dim) * eb);
   }
-  if (n == 0) return check_launch("gradient");
+  if (shares > kGradMostShares) return set_error(CTI_EBAG_EUNSUPPORTED, "tables of more than 2^38 bytes");
+  if (n == 0) {
+    hipLaunchKernelGGL(grad_fill_kernel, dim3(static_cast<unsigned>(shares > 0 ? shares : 1)), dim3(kSortThreads), 0, s, fill,
+                       c.sum.count_out);
+    return check_launch("gradient");
+  }
 
   c.src.by_batch = ChunkDivide::by(static_cast<uint32_t>(c.src.batch));
   const GradPlan plan = grad_plan(n, c.src.inv_len ? c.src.bags : 0, c.sum.dim, dtype_bytes(c.grad_dtype), c.src.total, c.even);
   char* const ws = static_cast<char*>(c.workspace);
-  SortBuffers buf[2] = {{reinterpret_cast<uint32_t*>(ws + plan.key[0]), reinterpret_cast<uint32_t*>(ws + plan.unit[0])},
-                        {reinterpret_cast<uint32_t*>(ws + plan.key[1]), reinterpret_cast<uint32_t*>(ws + plan.unit[1])}};
+  Pair* const buf[2] = {reinterpret_cast<Pair*>(ws + plan.ids[0]), reinterpret_cast<Pair*>(ws + plan.ids[1])};
   uint32_t* const counts = reinterpret_cast<uint32_t*>(ws + plan.counts);
   uint32_t* const totals = reinterpret_cast<uint32_t*>(ws + plan.totals);
   if (c.src.inv_len) {
@@ -1208,28 +1311,39 @@ int run_gradient(GradCall& c, hipStream_t s) {
     c.sum.inv_len = c.src.inv_len;
     hipLaunchKernelGGL(grad_lengths_kernel, dim3(static_cast<unsigned>((c.src.bags + 255) / 256)), dim3(256), 0, s, c.src);
   }
+  // the shares of the fill are dealt to the sort's launches evenly
+  const bool scan = plan.tiles > kGradTilesUnscanned;
+  const int launches = plan.tiles == 1 ? 1 : (scan ? 3 : 2) * static_cast<int>(ceil_div(plan.bits, plan.digit_bits));
+  int launch = 0;
+  const auto grid = [&](int64_t groups) {
+    fill.sort_groups = static_cast<int32_t>(groups);
+    fill.first_share = static_cast<int32_t>(shares * launch / launches);
+    ++launch;
+    return dim3(static_cast<unsigned>(groups + shares * launch / launches - fill.first_share));
+  };
+  const dim3 threads(kSortThreads);
   int at = 0;
   if (plan.tiles == 1) {
-    hipLaunchKernelGGL(grad_sort_tile_kernel, dim3(1), dim3(kSortThreads), 0, s, c.src, buf[0], plan.bits);
+    const dim3 g = grid(1);
+    hipLaunchKernelGGL(grad_sort_tile_kernel, g, threads, 0, s, c.src, buf[0], plan.bits, plan.digit_bits, fill);
   } else {
-    const dim3 tiles(static_cast<unsigned>(plan.tiles));
-    const bool scan = plan.tiles > kGradTilesUnscanned;
-    for (int shift = 0; shift < plan.bits; shift += plan.digit_bits) {
-      const int bits = plan.bits - shift < plan.digit_bits ? plan.bits - shift : plan.digit_bits;
-      if (shift == 0) {
-        hipLaunchKernelGGL(grad_keys_kernel, tiles, dim3(kSortThreads), 0, s, c.src, buf[0], counts, bits);
-      } else {
-        hipLaunchKernelGGL(grad_count_kernel, tiles, dim3(kSortThreads), 0, s, buf[at].key, n, shift, bits, counts);
+    const int bits = plan.digit_bits;
+    for (int shift = 0; shift < plan.bits; shift += bits) {
+      dim3 g = grid(plan.tiles);
+      if (shift == 0) hipLaunchKernelGGL(grad_keys_kernel, g, threads, 0, s, c.src, buf[0], counts, bits, fill);
+      else hipLaunchKernelGGL(grad_count_kernel, g, threads, 0, s, buf[at], n, shift, bits, counts, fill);
+      if (scan) {
+        g = grid(ceil_div(int64_t{1} << bits, kWave));
+        hipLaunchKernelGGL(grad_scan_kernel, g, dim3(kScanThreads), 0, s, counts, totals, plan.tiles, bits, fill);
       }
-      if (scan) hipLaunchKernelGGL(grad_scan_kernel, dim3(kDigits / 4), dim3(kScanThreads), 0, s, counts, totals, plan.tiles);
-      hipLaunchKernelGGL(grad_scatter_kernel, tiles, dim3(kSortThreads), 0, s, buf[at], buf[1 - at], n, shift, bits, counts,
-                         scan ? totals : nullptr, static_cast<int>(plan.tiles));
+      g = grid(plan.tiles);
+      hipLaunchKernelGGL(grad_scatter_kernel, g, threads, 0, s, buf[at], buf[1 - at], n, shift, bits, counts,
+                         scan ? totals : nullptr, fill);
       at = 1 - at;
     }
   }
   SumParams& p = c.sum;
-  p.key = buf[at].key;
-  p.unit = buf[at].unit;
+  p.ids = buf[at];
   p.n = n;
   p.total = c.src.total;
   p.partial = reinterpret_cast<float*>(ws + plan.partial);
@@ -1239,12 +1353,13 @@ int run_gradient(GradCall& c, hipStream_t s) {
   p.run = plan.run;
   p.workgroups = static_cast<int32_t>(plan.workgroups);
   p.fields = c.src.fields;
+  p.per_field = c.per_field;
   p.by_fields = ChunkDivide::by(static_cast<uint32_t>(c.src.fields));
   if (compact) {
     uint32_t* const heads = reinterpret_cast<uint32_t*>(ws + plan.heads);
     p.heads = heads;
     p.last_rank = reinterpret_cast<uint32_t*>(ws + plan.last_rank);
-    hipLaunchKernelGGL(grad_heads_kernel, dim3(static_cast<unsigned>(plan.workgroups)), dim3(kSumThreads), 0, s, p.key, n, p.total,
+    hipLaunchKernelGGL(grad_heads_kernel, dim3(static_cast<unsigned>(plan.workgroups)), dim3(kSumThreads), 0, s, p.ids, n, p.total,
                        static_cast<int>(plan.run * (kSumThreads >> plan.log_lanes)), heads);
     p.heads_scanned = plan.workgroups > kGradHeadsUnscanned;
     if (p.heads_scanned)

@@ -28,7 +28,9 @@ constexpr int kGradTile = 4096;
 constexpr int64_t kGradMostIds = int64_t{1} << 30;        // ids and bags: 32-bit numbers, and launches below 2^32 threads
 constexpr int64_t kGradMostRows = (int64_t{1} << 31) - 1;  // rows of all tables are fewer: the number itself is a key
 constexpr int64_t kGradMostDim = int64_t{1} << 22;
-constexpr int64_t kGradTilesUnscanned = 256;
+constexpr int64_t kGradMostShares = int64_t{1} << 22;     // of the fill: with the tiles, below 2^32 threads
+constexpr int kGradDigitBits = 11, kGradDigits = 1 << kGradDigitBits;
+constexpr int64_t kGradTilesUnscanned = 16;
 constexpr int64_t kGradHeadsUnscanned = 4096;
 
 constexpr int kGradWalkCols = 64;  // narrower rows would leave most of a wavefront idle
@@ -40,7 +42,7 @@ struct GradPlan {
   int lane_cols;  // columns a lane
   int log_lanes, run, blocks;  // lanes of a group, ids of a group, blocks of 64 lanes' columns
   int64_t workgroups;
-  int64_t key[2], unit[2], counts, totals, heads, last_rank, inv_len, partial, bytes;  // places in the workspace
+  int64_t ids[2], counts, totals, heads, last_rank, inv_len, partial, bytes;  // places in the workspace
 };
 
 // The gradient of n ids in tables of `rows` rows, the widest of `dim` columns; mean_bags: bags under mean pooling, else 0;
@@ -49,8 +51,9 @@ inline GradPlan grad_plan(int64_t n, int64_t mean_bags, int64_t dim, int elem_by
   GradPlan p{};
   p.tiles = ceil_div(n, kGradTile);
   while (p.bits < 32 && (rows >> p.bits)) ++p.bits;  // of the key `rows` itself
-  const int passes = (p.bits + 7) / 8;
+  const int passes = (p.bits + kGradDigitBits - 1) / kGradDigitBits;
   p.digit_bits = (p.bits + passes - 1) / passes;
+  if (p.digit_bits < 2) p.digit_bits = 2;  // a thread holds four digits
   const int vec = 16 / elem_bytes;
   p.walk = even && dim >= kGradWalkCols;
   if (p.walk) {
@@ -77,12 +80,9 @@ inline GradPlan grad_plan(int64_t n, int64_t mean_bags, int64_t dim, int elem_by
     at += ceil_div(bytes, 256) * 256;
     return here;
   };
-  for (int i = 0; i < 2; ++i) {
-    p.key[i] = take(n * 4);
-    p.unit[i] = take(n * 4);
-  }
-  p.counts = take(p.tiles * 1024);
-  p.totals = take(1024);
+  for (int i = 0; i < 2; ++i) p.ids[i] = take(n * 8);
+  p.counts = take((p.tiles << p.digit_bits) * 4);
+  p.totals = take(kGradDigits * 4);
   p.heads = take((p.workgroups + 1) * 4);
   p.last_rank = take(p.workgroups * 4);
   p.inv_len = take(mean_bags * 4);

@@ -41,8 +41,8 @@ def test_mask_keeps_the_stated_share(p):
 
 class Plan(ctypes.Structure):
     _fields_ = [("tiles", ctypes.c_int64), ("bits", ctypes.c_int), ("digit_bits", ctypes.c_int), ("walk", ctypes.c_bool),
-                ("lane_cols", ctypes.c_int), ("log_lanes", ctypes.c_int), ("run", ctypes.c_int), ("blocks", ctypes.c_int), ("workgroups", ctypes.c_int64), ("key", ctypes.c_int64 * 2),
-                ("unit", ctypes.c_int64 * 2), ("counts", ctypes.c_int64), ("totals", ctypes.c_int64), ("heads", ctypes.c_int64),
+                ("lane_cols", ctypes.c_int), ("log_lanes", ctypes.c_int), ("run", ctypes.c_int), ("blocks", ctypes.c_int), ("workgroups", ctypes.c_int64), ("ids", ctypes.c_int64 * 2),
+                ("counts", ctypes.c_int64), ("totals", ctypes.c_int64), ("heads", ctypes.c_int64),
                 ("last_rank", ctypes.c_int64), ("inv_len", ctypes.c_int64), ("partial", ctypes.c_int64), ("bytes", ctypes.c_int64)]
 
 
@@ -91,8 +91,8 @@ def test_gradient_plan_holds_what_the_kernels_assume(rules):
         even = rng.random() < 0.5
         rules.plan(n, bags, dim, elem, rows, even, ctypes.byref(p))
         assert p.tiles == -(-n // 4096)
-        # every key, the dropped ids' key `rows` too, has its bits; digits are at most 8 bits
-        assert rows < 2 ** p.bits and p.digit_bits <= 8 and -(-p.bits // p.digit_bits) == -(-p.bits // 8)
+        # every key, the dropped ids' key `rows` too, has its bits; digits have 2 to 11
+        assert rows < 2 ** p.bits and 2 <= p.digit_bits <= 11 and -(-p.bits // p.digit_bits) == -(-p.bits // 11)
         # lane groups cover a block of columns; blocks cover the row, and fit the grid
         assert p.log_lanes <= 6 and (1 << p.log_lanes) * p.lane_cols * p.blocks >= dim and p.blocks <= 65535
         assert p.blocks == 1 or p.log_lanes == 6
@@ -105,8 +105,7 @@ def test_gradient_plan_holds_what_the_kernels_assume(rules):
         assert groups * p.run <= 2048 and p.workgroups == -(-n // (groups * p.run))
         assert p.workgroups * 256 < 2 ** 32 and p.workgroups < 2 ** 31
         # parts of the workspace, in their order, neither overlap nor end before what is written there
-        ends = [(p.key[0], n * 4), (p.unit[0], n * 4), (p.key[1], n * 4), (p.unit[1], n * 4), (p.counts, p.tiles * 1024),
-                (p.totals, 1024), (p.heads, (p.workgroups + 1) * 4), (p.last_rank, p.workgroups * 4), (p.inv_len, bags * 4),
+        ends = [(p.ids[0], n * 8), (p.ids[1], n * 8), (p.counts, (p.tiles << p.digit_bits) * 4), (p.totals, 2048 * 4), (p.heads, (p.workgroups + 1) * 4), (p.last_rank, p.workgroups * 4), (p.inv_len, bags * 4),
                 (p.partial, p.workgroups * p.blocks * 2 * (p.lane_cols << p.log_lanes) * 4), (p.bytes, 0)]
         for (a, size), (b, _) in zip(ends, ends[1:]):
             assert a % 256 == 0 and a + size <= b
