@@ -51,22 +51,43 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int32_t ids64, int64
   return clamp_i64(id, 0, rows - 1);
 }
 
-// A thread takes 8 columns of a row. Bound by HBM where the rows are many, by the latency of an id's load
-// and a row's behind it where they are few.
+// A thread takes four chunks of 8 columns, their loads under way together (one: 16,384 rows of 4,096 bf16 columns 48 us).
+// Bound by HBM where the rows are many, by the latency of an id's load and a row's behind it where they are few.
+constexpr int kLookupChunks = 4;
 template <typename T, typename OT>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupParams p) {
-  const uint32_t c = blockIdx.x * kLookupThreads + threadIdx.x;
-  if (c >= p.chunks) return;
-  const uint32_t i = p.div.quotient(c);
-  const int col = static_cast<int>(c - i * p.per_row) * 8;
-  const int64_t id = load_id(p.ids, p.ids64, i, p.rows);
-  float v[8];
-  const int live = p.dim - col;
-  load8<T>(p.weight + id * p.row_bytes + static_cast<int64_t>(col) * Elem<T>::kBytes, live, v);
+  constexpr int VEC = 16 / Elem<T>::kBytes, WORDS = 8 / VEC;
+  const uint32_t first = blockIdx.x * (kLookupThreads * kLookupChunks) + threadIdx.x;
+  uint32_t row[kLookupChunks];
+  int col[kLookupChunks];
+  int64_t id[kLookupChunks];
+  uint4 raw[kLookupChunks][WORDS];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] *= p.scale;
+  for (int k = 0; k < kLookupChunks; ++k) {
+    const uint32_t c = first + k * kLookupThreads, at = c < p.chunks ? c : p.chunks - 1;
+    row[k] = p.div.quotient(at);
+    col[k] = static_cast<int>(at - row[k] * p.per_row) * 8;
+    id[k] = load_id(p.ids, p.ids64, row[k], p.rows);
+  }
+#pragma unroll
+  for (int k = 0; k < kLookupChunks; ++k) {
+    const char* const from = p.weight + id[k] * p.row_bytes + static_cast<int64_t>(col[k]) * Elem<T>::kBytes;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i)
+      raw[k][i] = p.dim - col[k] > i * VEC ? load_raw<T, VEC>(from + i * 16, p.dim - col[k] - i * VEC) : make_uint4(0u, 0u, 0u, 0u);
+  }
   with_stream(p.stream_out, [&](auto stream) {
-    store8<OT, decltype(stream)::value>(p.out + (static_cast<int64_t>(i) * p.dim + col) * Elem<OT>::kBytes, live, v);
+#pragma unroll
+    for (int k = 0; k < kLookupChunks; ++k) {
+      if (first + k * kLookupThreads < p.chunks) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) unpack16(raw[k][i], v + i * VEC, T{});
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= p.scale;
+        store8<OT, decltype(stream)::value>(p.out + (static_cast<int64_t>(row[k]) * p.dim + col[k]) * Elem<OT>::kBytes, p.dim - col[k], v);
+      }
+    }
   });
 }
 
@@ -129,8 +150,8 @@ __device__ __forceinline__ int item_index(int k) {
   return (static_cast<int>(threadIdx.x) / kWave) * (kItems * kWave) + k * kWave + lane_id();
 }
 
-// The ids' own loads are under way while their bags are found: the tile's first bag by a search of 512 places a
-// step, the others by reading edges from there on, 512 at a time. Bag j's start is event 2 (j - lo) + 2 at its place,
+// The ids' own loads are under way while their bags are found: the tile's first bag to within 512 by a search of 512
+// places a step, the others by reading edges from there on, 1,024 at a time. Bag j's start is event 2 (j - lo) + 2 at its place,
 // its end event 2 (j - lo) + 3 at the place behind; the largest event up to an id is its bag's start (even), or an
 // end: the id lies in no bag. (Ends looked up id by id, a search of 64 places and one for the tile's last id:
 // 917,504 ids in 114,688 bags 16 us.)
@@ -160,34 +181,42 @@ __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uin
   const int64_t last = (first + kTile < s.n ? first + kTile : s.n) - 1;
 #pragma unroll
   for (int k = 0; k < kItems; ++k) s_bag[t + k * kSortThreads] = 0;
-  // bags that start at or before the first id
+  // bags that start at or before the first id: `lo` at least, `hi` at most
   int64_t lo = 0, hi = s.bags;
-  while (lo < hi) {  // lo grows or hi falls in every step, whatever the offsets hold
+  while (hi - lo > kSortThreads) {  // lo grows or hi falls in every step, whatever the offsets hold
     const int64_t step = (hi - lo + kSortThreads - 1) / kSortThreads;
     const int64_t j = lo + step * (t + 1) - 1;  // the thread's last bag of its share
     const int started = __syncthreads_count(j < hi && bag_edge(s, j, 0) <= first);
     lo += step * started;
     if (lo + step - 1 < hi) hi = lo + step - 1;
   }
-  lo -= 1;  // the bag that holds the first id, or -1
-  // edges of bags lo, lo + 1, ... until one starts behind the tile
+  lo = lo > 0 ? lo - 1 : 0;
+  // edges of bags lo, lo + 1, ... until one starts behind the tile, two a thread; those before the tile leave nothing
+  __syncthreads();
   int64_t begun = 0;
   bool scan = true;
-  for (int64_t j0 = lo;; j0 += kSortThreads) {
-    const int64_t j = j0 + t;
-    bool in = false;
-    if (j < s.bags) {
-      const int64_t a = j >= 0 ? bag_edge(s, j, 0) : 0, b = j >= 0 ? bag_edge(s, j, 1) : 0;
-      in = a <= last;
-      if (in && j >= 0) {
-        const int32_t event = static_cast<int32_t>(j - lo) * 2 + 2;
-        const int64_t at = a > first ? a - first : 0, end = b - first;
-        if (b > a) atomicMax(&s_bag[at], event);
-        if (end >= 0 && first + end <= last) atomicMax(&s_bag[end], event + 1);
+  for (int64_t j0 = lo;; j0 += 2 * kSortThreads) {
+    int64_t a[2], b[2];
+    bool in[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t j = j0 + h * kSortThreads + t;
+      in[h] = j < s.bags;
+      a[h] = in[h] ? bag_edge(s, j, 0) : 0;
+      b[h] = in[h] ? bag_edge(s, j, 1) : 0;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      in[h] = in[h] && a[h] <= last;
+      if (in[h] && b[h] > first) {
+        const int32_t event = static_cast<int32_t>(j0 + h * kSortThreads + t - lo) * 2 + 2;
+        const int64_t at = a[h] > first ? a[h] - first : 0;
+        if (b[h] > a[h]) atomicMax(&s_bag[at], event);
+        if (b[h] <= last) atomicMax(&s_bag[b[h] - first], event + 1);
       }
     }
-    const int c = __syncthreads_count(in);
-    begun += c;
+    const int c = __syncthreads_count(in[1]);
+    begun += 2 * c;
     if (c < kSortThreads) break;
     if (begun > kMostBags) {
       scan = false;
@@ -231,7 +260,7 @@ __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uin
       if (event == 0 || event % 2) continue;  // in no bag
       j = lo + event / 2 - 1;
     } else {
-      int64_t a = lo + 1, b = s.bags;  // bags started at or before i
+      int64_t a = lo, b = s.bags;  // bags started at or before i
       while (a < b) {
         const int64_t mid = (a + b) / 2;
         if (bag_edge(s, mid, 0) <= i) a = mid + 1;
@@ -1184,14 +1213,20 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams 
   const int block = static_cast<int>(blockIdx.y);
   const int64_t next = first + ids;
   if (next >= p.n) return;
-  const uint32_t key = p.ids[next - 1].x;
-  if (key >= p.total || p.ids[next].x != key) return;                       // ends with the run
-  if (first > 0 && p.ids[first].x == key && p.ids[first - 1].x == key) return;  // began in a run before
+  // (all of these loads at once: one after the other, as far as each was needed, 7.2 us where no key crosses far)
+  const int64_t h0 = (static_cast<int64_t>(blockIdx.x) + 1 + t) * ids;
+  const uint32_t key = p.ids[next - 1].x, key_next = p.ids[next].x, key_first = p.ids[first].x;
+  const uint32_t key_before = first > 0 ? p.ids[first - 1].x : 0xffffffffu;
+  const uint32_t key_run = h0 < p.n ? p.ids[h0].x : 0xffffffffu;
+  const uint32_t unit = p.ids[next - 1].y;
+  const uint32_t rank = p.rows_out ? p.last_rank[blockIdx.x] : 0u;
+  if (key >= p.total || key_next != key) return;           // ends with the run
+  if (key_first == key && key_before == key) return;       // began in a run before
   // runs that begin with the key
-  int follow = 0;
-  for (int at = static_cast<int>(blockIdx.x) + 1;; at += kSumThreads) {
-    const int64_t i = static_cast<int64_t>(at + t) * ids;
-    const int c = __syncthreads_count(at + t < p.workgroups && i < p.n && p.ids[i].x == key);
+  int follow = __syncthreads_count(key_run == key);
+  for (int at = static_cast<int>(blockIdx.x) + 1 + kSumThreads; follow % kSumThreads == 0; at += kSumThreads) {
+    const int64_t i = (static_cast<int64_t>(at) + t) * ids;
+    const int c = __syncthreads_count(i < p.n && p.ids[i].x == key);
     follow += c;
     if (c < kSumThreads) break;
   }
@@ -1213,8 +1248,6 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams 
     const float4 v = s_part[i * quads + q];
     sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
   }
-  const uint32_t rank = p.rows_out ? p.last_rank[blockIdx.x] : 0u;
-  const uint32_t unit = p.ids[next - 1].y;
   const int dim = S::width(p, fs, unit);
   const float v[4] = {sum.x, sum.y, sum.z, sum.w};
   OT* const row = reinterpret_cast<OT*>(S::target(p, fs, key, unit, rank));
@@ -1458,7 +1491,7 @@ extern "C" int cti_ebag_lookup(const void* ids, int32_t index_type, int64_t n, c
     p.ids = static_cast<const char*>(ids) + i * (p.ids64 ? 8 : 4);
     p.out = static_cast<char*>(out) + i * dim * dtype_bytes(out_dtype);
     p.chunks = static_cast<uint32_t>(now * p.per_row);
-    const dim3 grid((p.chunks + kLookupThreads - 1) / kLookupThreads), block(kLookupThreads);
+    const dim3 grid(static_cast<unsigned>(ceil_div(p.chunks, kLookupThreads * kLookupChunks))), block(kLookupThreads);
     with_types(dtype, out_dtype, [&](auto t, auto o) {
       hipLaunchKernelGGL((lookup_kernel<decltype(t), decltype(o)>), grid, block, 0, s, p);
     });

@@ -98,17 +98,52 @@ struct Chunk {
   }
 };
 
-// N sums over the LANES threads that hold a row, in a fixed order. s_red: N * LANES / 64 floats.
+// v + v of the lane across, by the cross-lane forms of the VALU: 5 steps of about 10 cycles where a trip through the LDS
+// crossbar is 60 (16,384 x 4,096 bf16 backward, one reduction a row: see the kernel).
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+// Sum over each LANES lanes side by side, the same bits in all of them: pairs, quads (permutations within four lanes), eights
+// and sixteens (a row's halves, then the row, mirrored), rows and halves of the wavefront swapped.
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
+  static_assert(LANES == 8 || LANES == 16 || LANES == 32 || LANES == 64, "a power of two of lanes");
+  v = add_dpp<0xb1>(v);   // lanes 1 0 3 2
+  v = add_dpp<0x4e>(v);   // lanes 2 3 0 1
+  v = add_dpp<0x141>(v);  // 7 - lane of each eight
+  if constexpr (LANES >= 16) v = add_dpp<0x140>(v);  // 15 - lane of each sixteen
+  if constexpr (LANES >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (LANES == 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return v;
+}
+
+// N sums over the LANES threads that hold a row, in a fixed order. s_red: N * LANES / 64 floats that no thread still reads from
+// another use (callers take turns between two: then one barrier is enough).
 template <int LANES, int N>
 __device__ __forceinline__ void row_sums(float* v, float* s_red) {
-  if constexpr (LANES <= kWave) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = lane_sum<(LANES < kWave ? LANES : kWave)>(v[k]);
+  if constexpr (LANES > kWave) {
+    constexpr int WAVES = LANES / kWave;
+    if (lane_id() == 0) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) s_red[k * WAVES + threadIdx.x / kWave] = v[k];
+    }
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < N; ++k) {
+      float t = 0.f;
 #pragma unroll
-      for (int m = 1; m < LANES; m <<= 1) v[k] += shfl_xor_f32(v[k], m);
+      for (int i = 0; i < WAVES; ++i) t += s_red[k * WAVES + i];
+      v[k] = t;
     }
-  } else {
-    block_sum_n<LANES / kWave, N>(v, s_red);
   }
 }
 
@@ -133,12 +168,12 @@ template <int LANES>
 struct Block {
   static constexpr int kThreads = LANES < 256 ? 256 : LANES;
   static constexpr int kSide = kThreads / LANES;  // rows side by side
-  static constexpr int kReds = LANES <= kWave ? 1 : 2 * LANES / kWave;
+  static constexpr int kReds = LANES <= kWave ? 1 : 2 * LANES / kWave;  // one use of row_sums
 };
 
 template <typename T, typename PT, int LANES, int K>
 __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_kernel(const TrainNormParams p) {
-  __shared__ float s_red[Block<LANES>::kReds];
+  __shared__ float s_red[2][Block<LANES>::kReds];
   const int t = static_cast<int>(threadIdx.x), lane = t % LANES;
   const int64_t want = static_cast<int64_t>(blockIdx.x) * Block<LANES>::kSide + t / LANES;
   const bool there = want < p.rows;  // the lanes of a row past the end take part in the shuffles
@@ -175,7 +210,7 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_kernel(cons
     for (int e = 0; e < 8; ++e) s += v[k][e];  // columns past the row are +0: dropped or kept
   }
   const float n = static_cast<float>(cols);
-  row_sums<LANES, 1>(&s, s_red);
+  row_sums<LANES, 1>(&s, s_red[0]);
   const float mean = s / n;
   float q = 0.f;
 #pragma unroll
@@ -187,7 +222,7 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_kernel(cons
       q += v[k][e] * v[k][e];
     }
   }
-  row_sums<LANES, 1>(&q, s_red);
+  row_sums<LANES, 1>(&q, s_red[1]);
   const float rstd = 1.0f / __builtin_sqrtf(q / n + p.eps);
   if (!there) return;
   if (lane == 0) {
@@ -229,7 +264,7 @@ __device__ __forceinline__ void wide_h(const TrainNormParams& p, const Dropout& 
 
 template <typename T, typename PT>
 __global__ void __launch_bounds__(kWideThreads) train_norm_wide_kernel(const TrainNormParams p) {
-  __shared__ float s_red[2 * kWideThreads / kWave];
+  __shared__ float s_red[2][kWideThreads / kWave];
   const int64_t row = blockIdx.x, t = threadIdx.x;
   Dropout d = p.drop;
   if (d.threshold) load_state(d);
@@ -241,7 +276,7 @@ __global__ void __launch_bounds__(kWideThreads) train_norm_wide_kernel(const Tra
     for (int e = 0; e < 8; ++e) s += v[e];
   }
   const float n = static_cast<float>(p.cols);
-  row_sums<kWideThreads, 1>(&s, s_red);
+  row_sums<kWideThreads, 1>(&s, s_red[0]);
   const float mean = s / n;
   float q = 0.f;
   for (int64_t c = t * 8; c < p.cols; c += kWideThreads * 8) {
@@ -252,7 +287,7 @@ __global__ void __launch_bounds__(kWideThreads) train_norm_wide_kernel(const Tra
       q += w * w;
     }
   }
-  row_sums<kWideThreads, 1>(&q, s_red);
+  row_sums<kWideThreads, 1>(&q, s_red[1]);
   const float rstd = 1.0f / __builtin_sqrtf(q / n + p.eps);
   if (t == 0) {
     p.mean[row] = mean;
@@ -292,7 +327,8 @@ struct NormBackParams {
 template <typename T, typename PT, int LANES, int K>
 __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel(const NormBackParams p) {
   constexpr int SIDE = Block<LANES>::kSide;
-  __shared__ float s_red[Block<LANES>::kReds];
+  __shared__ float s_red[2][Block<LANES>::kReds];
+  int turn = 0;
   __shared__ float s_acc[SIDE > 1 ? 2 * Block<LANES>::kThreads * 8 * K : 1];
   const int t = static_cast<int>(threadIdx.x), lane = t % LANES;
   const int cols = static_cast<int>(p.cols);
@@ -352,7 +388,8 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
         }
       }
     }
-    row_sums<LANES, 2>(s, s_red);
+    row_sums<LANES, 2>(s, s_red[turn]);
+    turn ^= 1;
     const float m0 = s[0] / n, m1 = s[1] / n;
     if (there) {
       const int64_t at = row * p.cols * Elem<T>::kBytes;
@@ -422,7 +459,8 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
 // Rows of any width: the workgroup's sums lie in the workspace, where a thread adds its columns' row by row.
 template <typename T, typename PT>
 __global__ void __launch_bounds__(kWideThreads) train_norm_back_wide_kernel(const NormBackParams p) {
-  __shared__ float s_red[2 * kWideThreads / kWave];
+  __shared__ float s_red[2][2 * kWideThreads / kWave];
+  int turn = 0;
   const int64_t t = threadIdx.x;
   const float n = static_cast<float>(p.cols);
   Dropout d = p.drop;
@@ -450,7 +488,8 @@ __global__ void __launch_bounds__(kWideThreads) train_norm_back_wide_kernel(cons
         sums[width] = (first ? 0.f : sums[width]) + g[e];
       }
     }
-    row_sums<kWideThreads, 2>(s, s_red);
+    row_sums<kWideThreads, 2>(s, s_red[turn]);
+    turn ^= 1;
     const float m0 = s[0] / n, m1 = s[1] / n;
     for (int64_t c = t * 8; c < p.cols; c += kWideThreads * 8) {
       const int live = p.cols - c < 8 ? static_cast<int>(p.cols - c) : 8;
