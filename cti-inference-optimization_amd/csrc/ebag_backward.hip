@@ -53,36 +53,32 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int32_t ids64, int64
 
 // A thread takes four chunks of 8 columns, their loads under way together (one: 16,384 rows of 4,096 bf16 columns 48 us).
 // Bound by HBM where the rows are many, by the latency of an id's load and a row's behind it where they are few.
+// The last chunk of a row ends with it and overlaps the one before (the same values twice); rows of less than 8 columns are
+// one chunk.
 constexpr int kLookupChunks = 4;
 template <typename T, typename OT>
 __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupParams p) {
-  constexpr int VEC = 16 / Elem<T>::kBytes, WORDS = 8 / VEC;
   const uint32_t first = blockIdx.x * (kLookupThreads * kLookupChunks) + threadIdx.x;
   uint32_t row[kLookupChunks];
   int col[kLookupChunks];
   int64_t id[kLookupChunks];
-  uint4 raw[kLookupChunks][WORDS];
+  Chunk<T> x[kLookupChunks];
 #pragma unroll
   for (int k = 0; k < kLookupChunks; ++k) {
     const uint32_t c = first + k * kLookupThreads, at = c < p.chunks ? c : p.chunks - 1;
     row[k] = p.div.quotient(at);
     col[k] = static_cast<int>(at - row[k] * p.per_row) * 8;
+    if (p.dim >= 8 && col[k] + 8 > p.dim) col[k] = p.dim - 8;
     id[k] = load_id(p.ids, p.ids64, row[k], p.rows);
   }
 #pragma unroll
-  for (int k = 0; k < kLookupChunks; ++k) {
-    const char* const from = p.weight + id[k] * p.row_bytes + static_cast<int64_t>(col[k]) * Elem<T>::kBytes;
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i)
-      raw[k][i] = p.dim - col[k] > i * VEC ? load_raw<T, VEC>(from + i * 16, p.dim - col[k] - i * VEC) : make_uint4(0u, 0u, 0u, 0u);
-  }
+  for (int k = 0; k < kLookupChunks; ++k) x[k].load(p.weight + id[k] * p.row_bytes, col[k], p.dim);
   with_stream(p.stream_out, [&](auto stream) {
 #pragma unroll
     for (int k = 0; k < kLookupChunks; ++k) {
       if (first + k * kLookupThreads < p.chunks) {
         float v[8];
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) unpack16(raw[k][i], v + i * VEC, T{});
+        x[k].unpack(v, col[k], p.dim);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= p.scale;
         store8<OT, decltype(stream)::value>(p.out + (static_cast<int64_t>(row[k]) * p.dim + col[k]) * Elem<OT>::kBytes, p.dim - col[k], v);
@@ -96,7 +92,6 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupPara
 // ---------------------------------------------------------------------------------------------
 constexpr int kTile = kGradTile;  // keys a workgroup sorts
 constexpr int kSortThreads = 512;
-constexpr int kSortWaves = kSortThreads / kWave;
 constexpr int kItems = kTile / kSortThreads;  // keys a thread
 constexpr int kMaxFields = 64;
 
@@ -145,9 +140,10 @@ __device__ __forceinline__ uint32_t grad_key(const GradSource& s, int64_t id, in
 
 constexpr int kMostBags = 8 * kTile;  // bags whose starts a tile looks through; with more, each id searches
 
-// Keys and u of the tile's ids: item k of a thread is id tile * kTile + item_index(k). s_bag: kTile words.
+// Keys and u of the tile's ids (THREADS * ITEMS): item k of a thread is the tile's id item_index(k). s_bag: a word for each.
+template <int ITEMS = kItems>
 __device__ __forceinline__ int item_index(int k) {
-  return (static_cast<int>(threadIdx.x) / kWave) * (kItems * kWave) + k * kWave + lane_id();
+  return (static_cast<int>(threadIdx.x) / kWave) * (ITEMS * kWave) + k * kWave + lane_id();
 }
 
 // The ids' own loads are under way while their bags are found: the tile's first bag to within 512 by a search of 512
@@ -155,15 +151,16 @@ __device__ __forceinline__ int item_index(int k) {
 // its end event 2 (j - lo) + 3 at the place behind; the largest event up to an id is its bag's start (even), or an
 // end: the id lies in no bag. (Ends looked up id by id, a search of 64 places and one for the tile's last id:
 // 917,504 ids in 114,688 bags 16 us.)
+template <int THREADS, int ITEMS>
 __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uint32_t* key, uint32_t* unit, int32_t* s_bag,
                                           int32_t* s_wave) {
-  const int64_t first = tile * kTile;
+  const int64_t first = tile * (THREADS * ITEMS);
   const int t = static_cast<int>(threadIdx.x);
-  int64_t id[kItems];
+  int64_t id[ITEMS];
   const auto load_ids = [&](auto type) {
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const int64_t i = first + item_index(k);
+    for (int k = 0; k < ITEMS; ++k) {
+      const int64_t i = first + item_index<ITEMS>(k);
       id[k] = static_cast<const decltype(type)*>(s.ids)[i < s.n ? i : s.n - 1];
     }
   };
@@ -171,20 +168,20 @@ __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uin
   else load_ids(int32_t{});
   if (!s.offsets) {
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const int64_t i = first + item_index(k);
+    for (int k = 0; k < ITEMS; ++k) {
+      const int64_t i = first + item_index<ITEMS>(k);
       key[k] = i < s.n ? grad_key(s, id[k], 0) : 0xffffffffu;
       unit[k] = static_cast<uint32_t>(i);
     }
     return;
   }
-  const int64_t last = (first + kTile < s.n ? first + kTile : s.n) - 1;
+  const int64_t last = (first + THREADS * ITEMS < s.n ? first + THREADS * ITEMS : s.n) - 1;
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) s_bag[t + k * kSortThreads] = 0;
+  for (int k = 0; k < ITEMS; ++k) s_bag[t + k * THREADS] = 0;
   // bags that start at or before the first id: `lo` at least, `hi` at most
   int64_t lo = 0, hi = s.bags;
-  while (hi - lo > kSortThreads) {  // lo grows or hi falls in every step, whatever the offsets hold
-    const int64_t step = (hi - lo + kSortThreads - 1) / kSortThreads;
+  while (hi - lo > THREADS) {  // lo grows or hi falls in every step, whatever the offsets hold
+    const int64_t step = (hi - lo + THREADS - 1) / THREADS;
     const int64_t j = lo + step * (t + 1) - 1;  // the thread's last bag of its share
     const int started = __syncthreads_count(j < hi && bag_edge(s, j, 0) <= first);
     lo += step * started;
@@ -195,12 +192,12 @@ __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uin
   __syncthreads();
   int64_t begun = 0;
   bool scan = true;
-  for (int64_t j0 = lo;; j0 += 2 * kSortThreads) {
+  for (int64_t j0 = lo;; j0 += 2 * THREADS) {
     int64_t a[2], b[2];
     bool in[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int64_t j = j0 + h * kSortThreads + t;
+      const int64_t j = j0 + h * THREADS + t;
       in[h] = j < s.bags;
       a[h] = in[h] ? bag_edge(s, j, 0) : 0;
       b[h] = in[h] ? bag_edge(s, j, 1) : 0;
@@ -209,7 +206,7 @@ __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uin
     for (int h = 0; h < 2; ++h) {
       in[h] = in[h] && a[h] <= last;
       if (in[h] && b[h] > first) {
-        const int32_t event = static_cast<int32_t>(j0 + h * kSortThreads + t - lo) * 2 + 2;
+        const int32_t event = static_cast<int32_t>(j0 + h * THREADS + t - lo) * 2 + 2;
         const int64_t at = a[h] > first ? a[h] - first : 0;
         if (b[h] > a[h]) atomicMax(&s_bag[at], event);
         if (b[h] <= last) atomicMax(&s_bag[b[h] - first], event + 1);
@@ -217,14 +214,14 @@ __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uin
     }
     const int c = __syncthreads_count(in[1]);
     begun += 2 * c;
-    if (c < kSortThreads) break;
+    if (c < THREADS) break;
     if (begun > kMostBags) {
       scan = false;
       break;
     }
   }
   if (scan) {
-    constexpr int kRun = kTile / kSortThreads;
+    constexpr int kRun = ITEMS;
     int32_t m[kRun], top = 0;
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {
@@ -248,15 +245,15 @@ __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uin
     __syncthreads();
   }
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int64_t i = first + item_index(k);
+  for (int k = 0; k < ITEMS; ++k) {
+    const int64_t i = first + item_index<ITEMS>(k);
     key[k] = 0xffffffffu;
     unit[k] = 0u;
     if (i >= s.n) continue;
     key[k] = s.total;
     int64_t j;
     if (scan) {
-      const int32_t event = s_bag[item_index(k)];
+      const int32_t event = s_bag[item_index<ITEMS>(k)];
       if (event == 0 || event % 2) continue;  // in no bag
       j = lo + event / 2 - 1;
     } else {
@@ -339,7 +336,8 @@ __device__ __forceinline__ int64_t tile_of(int64_t group, int64_t tiles) {
   return xcd * per + (xcd < more ? xcd : more) + group / 8;
 }
 
-// Exclusive sums over the workgroup's threads; s_scan: kSortWaves words.
+// Exclusive sums over the workgroup's threads; s_scan: a word for each wavefront.
+template <int THREADS>
 __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* s_scan) {
   const int t = static_cast<int>(threadIdx.x);
   uint32_t x = v;
@@ -353,29 +351,30 @@ __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* s_scan) {
   __syncthreads();
   uint32_t before = 0;
 #pragma unroll
-  for (int w = 0; w < kSortWaves; ++w) before += w < t / kWave ? s_scan[w] : 0u;
+  for (int w = 0; w < THREADS / kWave; ++w) before += w < t / kWave ? s_scan[w] : 0u;
   return before + x - v;
 }
 
-// Places of the tile's keys in the tile sorted by one digit (stable): place[k] of item k. s_hist: kSortWaves << bits
+// Places of the tile's keys in the tile sorted by one digit (stable): place[k] of item k. s_hist: wavefronts << bits
 // numbers; s_start[d] is the first place of digit d. A thread holds digits 4 t to 4 t + 3; counts[4] of them are the tile's.
+template <int THREADS, int ITEMS>
 __device__ __forceinline__ void tile_places(const uint32_t* key, int shift, int bits, uint32_t* place, uint16_t* s_hist,
                                             uint32_t* s_start, uint32_t* s_scan) {
   const int t = static_cast<int>(threadIdx.x), w = t / kWave, digits = 1 << bits;
   const uint32_t mask = digits - 1;
   uint2* const hist4 = reinterpret_cast<uint2*>(s_hist);
-  for (int i = t; i < kSortWaves * digits / 4; i += kSortThreads) hist4[i] = make_uint2(0u, 0u);
+  for (int i = t; i < THREADS / kWave * digits / 4; i += THREADS) hist4[i] = make_uint2(0u, 0u);
   __syncthreads();
   // the lanes with the same digit, of every item before the first one's turn, so that no ballot waits for LDS: where a
   // lane's bit is like the lane's own (m: its bit in every place), same & ~(ones ^ m) keeps it
-  uint32_t lo[kItems], hi[kItems];
+  uint32_t lo[ITEMS], hi[ITEMS];
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) lo[k] = hi[k] = ~0u;
+  for (int k = 0; k < ITEMS; ++k) lo[k] = hi[k] = ~0u;
 #pragma unroll
   for (int b = 0; b < kGradDigitBits; ++b) {
     if (b < bits) {
 #pragma unroll
-      for (int k = 0; k < kItems; ++k) {
+      for (int k = 0; k < ITEMS; ++k) {
         const uint32_t m = static_cast<uint32_t>(static_cast<int32_t>((key[k] >> shift) << (31 - b)) >> 31);
         const uint64_t ones = __ballot(m != 0u);
         lo[k] = __builtin_amdgcn_bitop3_b32(lo[k], static_cast<uint32_t>(ones), m, 0x90);
@@ -385,7 +384,7 @@ __device__ __forceinline__ void tile_places(const uint32_t* key, int shift, int 
   }
   volatile uint16_t* const mine = s_hist + w * digits;
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
+  for (int k = 0; k < ITEMS; ++k) {
     const uint32_t d = (key[k] >> shift) & mask;
     const uint32_t seen = mine[d];
     const uint32_t rank = __builtin_amdgcn_mbcnt_hi(hi[k], __builtin_amdgcn_mbcnt_lo(lo[k], 0u));  // lanes before this one
@@ -398,13 +397,13 @@ __device__ __forceinline__ void tile_places(const uint32_t* key, int shift, int 
   uint32_t sum[4] = {0u, 0u, 0u, 0u};
   if (4 * t < digits) {
 #pragma unroll
-    for (int i = 0; i < kSortWaves; ++i) {
+    for (int i = 0; i < THREADS / kWave; ++i) {
       const uint2 c = hist4[i * (digits / 4) + t];
       hist4[i * (digits / 4) + t] = make_uint2(sum[0] | (sum[1] << 16), sum[2] | (sum[3] << 16));
       sum[0] += c.x & 0xffffu, sum[1] += c.x >> 16, sum[2] += c.y & 0xffffu, sum[3] += c.y >> 16;
     }
   }
-  uint32_t start = group_scan(sum[0] + sum[1] + sum[2] + sum[3], s_scan);
+  uint32_t start = group_scan<THREADS>(sum[0] + sum[1] + sum[2] + sum[3], s_scan);
   if (4 * t < digits) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -414,38 +413,42 @@ __device__ __forceinline__ void tile_places(const uint32_t* key, int shift, int 
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
+  for (int k = 0; k < ITEMS; ++k) {
     const uint32_t d = (key[k] >> shift) & mask;
     place[k] += s_start[d] + s_hist[w * digits + d];
   }
 }
 
-// All ids in one tile: keys and every digit in one launch.
-__global__ void __launch_bounds__(kSortThreads) grad_sort_tile_kernel(const GradSource s, Pair* out, int all_bits, int digit_bits,
-                                                                      const GradFill fill) {
+// All ids in one tile of up to kGradIdsAlone: keys and every digit in one launch (5,001 ids of 10 bits: 10 us, in two
+// launches 15; 16,384 ids of 15 bits: 35 us in one workgroup, 37 in four launches of four).
+template <int THREADS, int ITEMS>
+__global__ void __launch_bounds__(THREADS) grad_sort_tile_kernel(const GradSource s, Pair* out, int all_bits, int digit_bits,
+                                                                 const GradFill fill) {
   if (fills(fill)) return;
-  __shared__ Pair s_pair[kTile];
-  __shared__ uint16_t s_hist[kSortWaves * kGradDigits];
-  __shared__ uint32_t s_start[kGradDigits], s_scan[kSortWaves];
-  uint32_t key[kItems], unit[kItems], place[kItems];
-  tile_keys(s, 0, key, unit, reinterpret_cast<int32_t*>(s_pair), reinterpret_cast<int32_t*>(s_scan));
+  constexpr int HIST = THREADS / kWave * kGradDigits;
+  __shared__ Pair s_pair[THREADS * ITEMS > HIST / 4 ? THREADS * ITEMS : HIST / 4];  // the digits' numbers, then the pairs
+  __shared__ uint32_t s_start[kGradDigits], s_scan[THREADS / kWave];
+  uint16_t* const s_hist = reinterpret_cast<uint16_t*>(s_pair);
+  uint32_t key[ITEMS], unit[ITEMS], place[ITEMS];
+  tile_keys<THREADS, ITEMS>(s, 0, key, unit, reinterpret_cast<int32_t*>(s_pair), reinterpret_cast<int32_t*>(s_scan));
+  __syncthreads();
   for (int shift = 0; shift < all_bits; shift += digit_bits) {
-    tile_places(key, shift, digit_bits, place, s_hist, s_start, s_scan);
+    tile_places<THREADS, ITEMS>(key, shift, digit_bits, place, s_hist, s_start, s_scan);
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) s_pair[place[k]] = make_uint2(key[k], unit[k]);
+    for (int k = 0; k < ITEMS; ++k) s_pair[place[k]] = make_uint2(key[k], unit[k]);
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kItems; ++k) {
-      const Pair v = s_pair[item_index(k)];
+    for (int k = 0; k < ITEMS; ++k) {
+      const Pair v = s_pair[item_index<ITEMS>(k)];
       key[k] = v.x;
       unit[k] = v.y;
     }
     __syncthreads();
   }
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int i = item_index(k);
+  for (int k = 0; k < ITEMS; ++k) {
+    const int i = item_index<ITEMS>(k);
     if (i < s.n) out[i] = make_uint2(key[k], unit[k]);
   }
 }
@@ -469,10 +472,10 @@ __global__ void __launch_bounds__(kSortThreads) grad_keys_kernel(const GradSourc
   if (fills(fill)) return;
   __shared__ int32_t s_bag[kTile];
   __shared__ uint32_t s_hist[kGradDigits];
-  __shared__ int32_t s_wave[kSortWaves];
+  __shared__ int32_t s_wave[kSortThreads / kWave];
   uint32_t key[kItems], unit[kItems];
   const int64_t tile = tile_of(blockIdx.x, fill.sort_groups), first = tile * kTile;
-  tile_keys(s, tile, key, unit, s_bag, s_wave);
+  tile_keys<kSortThreads, kItems>(s, tile, key, unit, s_bag, s_wave);
 #pragma unroll
   for (int k = 0; k < kItems; ++k) {
     const int64_t i = first + item_index(k);
@@ -551,8 +554,8 @@ __global__ void __launch_bounds__(kSortThreads) grad_scatter_kernel(const Pair* 
                                                                     const GradFill fill) {
   if (fills(fill)) return;
   __shared__ Pair s_pair[kTile];
-  __shared__ uint16_t s_hist[kSortWaves * kGradDigits];
-  __shared__ uint32_t s_start[kGradDigits], s_scan[kSortWaves];
+  __shared__ uint16_t s_hist[kSortThreads / kWave * kGradDigits];
+  __shared__ uint32_t s_start[kGradDigits], s_scan[kSortThreads / kWave];
   const int t = static_cast<int>(threadIdx.x), digits = 1 << bits;
   const int64_t tile = tile_of(blockIdx.x, fill.sort_groups), first = tile * kTile;
   uint32_t key[kItems], unit[kItems], place[kItems];
@@ -579,8 +582,8 @@ __global__ void __launch_bounds__(kSortThreads) grad_scatter_kernel(const Pair* 
       }
     }
   }
-  const uint32_t base = group_scan(total.x + total.y + total.z + total.w, s_scan);
-  tile_places(key, shift, bits, place, s_hist, s_start, s_scan);
+  const uint32_t base = group_scan<kSortThreads>(total.x + total.y + total.z + total.w, s_scan);
+  tile_places<kSortThreads, kItems>(key, shift, bits, place, s_hist, s_start, s_scan);
 #pragma unroll
   for (int k = 0; k < kItems; ++k) s_pair[place[k]] = make_uint2(key[k], unit[k]);
   __syncthreads();
@@ -1367,7 +1370,8 @@ int run_gradient(GradCall& c, hipStream_t s) {
   }
   // the shares of the fill are dealt to the sort's launches evenly
   const bool scan = plan.tiles > kGradTilesUnscanned;
-  const int launches = plan.tiles == 1 ? 1 : (scan ? 3 : 2) * static_cast<int>(ceil_div(plan.bits, plan.digit_bits));
+  const bool alone = n <= kGradIdsAlone;
+  const int launches = alone ? 1 : (scan ? 3 : 2) * static_cast<int>(ceil_div(plan.bits, plan.digit_bits));
   int launch = 0;
   const auto grid = [&](int64_t groups) {
     fill.sort_groups = static_cast<int32_t>(groups);
@@ -1377,9 +1381,10 @@ int run_gradient(GradCall& c, hipStream_t s) {
   };
   const dim3 threads(kSortThreads);
   int at = 0;
-  if (plan.tiles == 1) {
+  if (alone) {
     const dim3 g = grid(1);
-    hipLaunchKernelGGL(grad_sort_tile_kernel, g, threads, 0, s, c.src, buf[0], plan.bits, plan.digit_bits, fill);
+    if (n <= 4096) hipLaunchKernelGGL((grad_sort_tile_kernel<512, 8>), g, threads, 0, s, c.src, buf[0], plan.bits, plan.digit_bits, fill);
+    else hipLaunchKernelGGL((grad_sort_tile_kernel<1024, 8>), g, dim3(1024), 0, s, c.src, buf[0], plan.bits, plan.digit_bits, fill);
   } else {
     const int bits = plan.digit_bits;
     for (int shift = 0; shift < plan.bits; shift += bits) {

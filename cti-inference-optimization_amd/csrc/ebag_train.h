@@ -24,6 +24,64 @@ __device__ __forceinline__ void load8(const char* p, int live, float* v) {
   }
 }
 
+// 8 columns of a row from column c on, as loaded; what lies past the row's `cols` is +0. Rows of at least 8 columns are read
+// by whole vectors, at any address: a chunk past the row's end as the last 8 columns, moved to their places when they are
+// unpacked. (Read one by one, they would be waited for in a branch, and every other load with them.)
+// WHOLE: the row's width is a multiple of 8 (columns from the row's end on are its last 8, for lanes that leave them out).
+template <typename T, bool WHOLE = false>
+struct Chunk {
+  static constexpr int kVecs = Elem<T>::kBytes / 2;
+  uint4 raw[kVecs];
+  __device__ __forceinline__ void load(const char* row, int c, int cols) {
+    if (WHOLE || cols >= 8) {
+      const char* const p = row + static_cast<int64_t>(c + 8 <= cols ? c : cols - 8) * Elem<T>::kBytes;
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) raw[i] = load16_any(p + i * 16);
+    } else {
+      uint32_t w[4 * kVecs] = {};
+#pragma unroll
+      for (int e = 0; e < 7; ++e) {
+        if (c + e < cols) {
+          const char* const p = row + (c + e) * Elem<T>::kBytes;
+          if constexpr (Elem<T>::kBytes == 4) w[e] = *reinterpret_cast<const uint32_t*>(p);
+          else w[e / 2] |= static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(p)) << (16 * (e % 2));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) raw[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+  }
+  __device__ __forceinline__ void unpack(float* v, int c, int cols) const {
+    constexpr int VEC = 16 / Elem<T>::kBytes, N = 4 * kVecs;
+    if (WHOLE || c + 8 <= cols || cols < 8) {
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i) unpack16(raw[i], v + i * VEC, T{});
+      return;
+    }
+    const int by = c + 8 - cols < 8 ? c + 8 - cols : 8;  // columns to move by
+    uint32_t w[N];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) w[4 * i] = raw[i].x, w[4 * i + 1] = raw[i].y, w[4 * i + 2] = raw[i].z, w[4 * i + 3] = raw[i].w;
+#pragma unroll
+    for (int step = 8; step * Elem<T>::kBytes >= 4; step /= 2) {
+      const int words = step * Elem<T>::kBytes / 4;
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = by & step ? (i + words < N ? w[i + words] : 0u) : w[i];
+    }
+    if constexpr (Elem<T>::kBytes == 2) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = by & 1 ? (w[i] >> 16) | (i + 1 < N ? w[i + 1] << 16 : 0u) : w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) unpack16(make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]), v + i * VEC, T{});
+  }
+  // What was unpacked before is forgotten, and unpacked again when it is needed: else the compiler keeps both forms.
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) asm("" : "+v"(raw[i].x), "+v"(raw[i].y), "+v"(raw[i].z), "+v"(raw[i].w));
+  }
+};
+
 // One vector of 16 bytes, as loaded, of which the first `live` elements are there.
 template <typename T, int VEC>
 __device__ __forceinline__ uint4 load_raw(const char* p, int live) {
@@ -97,6 +155,18 @@ inline void with_type(int32_t dtype, F&& f) {
     default: f(f16_t{}); break;
   }
 }
+// 8 parameters of a type known at run time, from column c on.
+__device__ __forceinline__ void load_params8(const void* p, int32_t dtype, int c, int cols, float* v) {
+  const auto load = [&](auto t) {
+    Chunk<decltype(t)> x;
+    x.load(static_cast<const char*>(p), c, cols);
+    x.unpack(v, c, cols);
+  };
+  if (dtype == CTI_EBAG_F32) load(float{});
+  else if (dtype == CTI_EBAG_BF16) load(bf16_t{});
+  else load(f16_t{});
+}
+
 template <typename F>
 inline void with_types(int32_t a, int32_t b, F&& f) {
   with_type(a, [&](auto t) { with_type(b, [&](auto o) { f(t, o); }); });

@@ -45,21 +45,25 @@ __global__ void __launch_bounds__(kDropThreads) dropout_kernel(const DropParams 
   const uint32_t c = blockIdx.x * kDropThreads + threadIdx.x;
   if (c >= p.chunks) return;
   const uint32_t row = p.div.quotient(c), chunk = c - row * p.per_row;
-  const int64_t col = static_cast<int64_t>(chunk) * 8, at = (static_cast<int64_t>(row) * p.cols + col) * Elem<T>::kBytes;
-  const int live = p.cols - col < 8 ? static_cast<int>(p.cols - col) : 8;
-  float v[8], r[8];
-  load8<T>(p.x + at, live, v);
-  if (p.res) load8<T>(p.res + at, live, r);
+  const int cols = static_cast<int>(p.cols), col = static_cast<int>(chunk) * 8;
+  const int64_t row_at = static_cast<int64_t>(row) * p.cols * Elem<T>::kBytes;
+  Chunk<T> x, res;
+  float v[8];
+  x.load(p.x + row_at, col, cols);
+  if (p.res) res.load(p.res + row_at, col, cols);
+  x.unpack(v, col, cols);
   Dropout d = p.drop;
   if (d.threshold) {
     load_state(d);
     apply_dropout(d, p.first_row + row, chunk, v);
   }
   if (p.res) {
+    float r[8];
+    res.unpack(r, col, cols);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += r[e];
   }
-  with_stream(p.stream_out, [&](auto stream) { store8<T, decltype(stream)::value>(p.y + at, live, v); });
+  with_stream(p.stream_out, [&](auto stream) { store8<T, decltype(stream)::value>(p.y + row_at + static_cast<int64_t>(col) * Elem<T>::kBytes, cols - col, v); });
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -79,24 +83,6 @@ __device__ __forceinline__ void round8(float* v) {
     for (int e = 0; e < 8; ++e) v[e] = f16_bits_to_f32(f32_to_f16_bits(v[e]));
   }
 }
-
-// A chunk of 8 columns as loaded; columns past the row are +0.
-template <typename T>
-struct Chunk {
-  static constexpr int kWords = Elem<T>::kBytes / 2;
-  uint4 raw[kWords];
-  __device__ __forceinline__ void load(const char* p, int live) {
-    constexpr int VEC = 16 / Elem<T>::kBytes;
-#pragma unroll
-    for (int i = 0; i < kWords; ++i)
-      raw[i] = live > i * VEC ? load_raw<T, VEC>(p + i * 16, live - i * VEC) : make_uint4(0u, 0u, 0u, 0u);
-  }
-  __device__ __forceinline__ void unpack(float* v) const {
-    constexpr int VEC = 16 / Elem<T>::kBytes;
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) unpack16(raw[i], v + i * VEC, T{});
-  }
-};
 
 // v + v of the lane across, by the cross-lane forms of the VALU: 5 steps of about 10 cycles where a trip through the LDS
 // crossbar is 60 (16,384 x 4,096 bf16 backward, one reduction a row: see the kernel).
@@ -124,7 +110,7 @@ __device__ __forceinline__ float lane_sum(float v) {
   return v;
 }
 
-// N sums over the LANES threads that hold a row, in a fixed order. s_red: N * LANES / 64 floats that no thread still reads from
+// N sums over the LANES threads that hold a row, in a fixed order. s_red: N floats a wavefront that no thread still reads from
 // another use (callers take turns between two: then one barrier is enough).
 template <int LANES, int N>
 __device__ __forceinline__ void row_sums(float* v, float* s_red) {
@@ -132,16 +118,17 @@ __device__ __forceinline__ void row_sums(float* v, float* s_red) {
   for (int k = 0; k < N; ++k) v[k] = lane_sum<(LANES < kWave ? LANES : kWave)>(v[k]);
   if constexpr (LANES > kWave) {
     constexpr int WAVES = LANES / kWave;
+    float* const mine = s_red + threadIdx.x / LANES * (N * WAVES);  // the row's, of those side by side
     if (lane_id() == 0) {
 #pragma unroll
-      for (int k = 0; k < N; ++k) s_red[k * WAVES + threadIdx.x / kWave] = v[k];
+      for (int k = 0; k < N; ++k) mine[k * WAVES + threadIdx.x % LANES / kWave] = v[k];
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       float t = 0.f;
 #pragma unroll
-      for (int i = 0; i < WAVES; ++i) t += s_red[k * WAVES + i];
+      for (int i = 0; i < WAVES; ++i) t += mine[k * WAVES + i];
       v[k] = t;
     }
   }
@@ -161,6 +148,7 @@ struct TrainNormParams {
   uint32_t first_row;
   float eps;
   Dropout drop;
+  int32_t param_dtype;
   int32_t stream_out;
 };
 
@@ -168,10 +156,10 @@ template <int LANES>
 struct Block {
   static constexpr int kThreads = LANES < 256 ? 256 : LANES;
   static constexpr int kSide = kThreads / LANES;  // rows side by side
-  static constexpr int kReds = LANES <= kWave ? 1 : 2 * LANES / kWave;  // one use of row_sums
+  static constexpr int kReds = LANES <= kWave ? 1 : 2 * kThreads / kWave;  // one use of row_sums
 };
 
-template <typename T, typename PT, int LANES, int K>
+template <typename T, int LANES, int K>
 __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_kernel(const TrainNormParams p) {
   __shared__ float s_red[2][Block<LANES>::kReds];
   const int t = static_cast<int>(threadIdx.x), lane = t % LANES;
@@ -187,17 +175,17 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_kernel(cons
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (lane + k * LANES) * 8;
-    x[k].load(p.x + at + c * Elem<T>::kBytes, cols - c);
-    if (p.res) r[k].load(p.res + at + c * Elem<T>::kBytes, cols - c);
+    x[k].load(p.x + at, c, cols);
+    if (p.res) r[k].load(p.res + at, c, cols);
   }
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (lane + k * LANES) * 8;
-    x[k].unpack(v[k]);
+    x[k].unpack(v[k], c, cols);
     if (d.threshold) apply_dropout(d, p.first_row + static_cast<uint32_t>(row), static_cast<uint32_t>(c / 8), v[k]);
     if (p.res) {
       float w[8];
-      r[k].unpack(w);
+      r[k].unpack(w, c, cols);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[k][e] += w[e];
     }
@@ -235,8 +223,8 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_kernel(cons
       const int c = (lane + k * LANES) * 8;
       if (c < cols) {
         float gm[8], bt[8];
-        load8<PT>(static_cast<const char*>(p.gamma) + c * Elem<PT>::kBytes, cols - c, gm);
-        load8<PT>(static_cast<const char*>(p.beta) + c * Elem<PT>::kBytes, cols - c, bt);
+        load_params8(p.gamma, p.param_dtype, c, cols, gm);
+        load_params8(p.beta, p.param_dtype, c, cols, bt);
 #pragma unroll
         for (int e = 0; e < 8; ++e) gm[e] = v[k][e] * rstd * gm[e] + bt[e];
         store8<T, decltype(st)::value>(p.y + at + c * Elem<T>::kBytes, cols - c, gm);
@@ -262,7 +250,7 @@ __device__ __forceinline__ void wide_h(const TrainNormParams& p, const Dropout& 
   if (p.h) round8<T>(v);
 }
 
-template <typename T, typename PT>
+template <typename T>
 __global__ void __launch_bounds__(kWideThreads) train_norm_wide_kernel(const TrainNormParams p) {
   __shared__ float s_red[2][kWideThreads / kWave];
   const int64_t row = blockIdx.x, t = threadIdx.x;
@@ -297,8 +285,8 @@ __global__ void __launch_bounds__(kWideThreads) train_norm_wide_kernel(const Tra
     const int live = p.cols - c < 8 ? static_cast<int>(p.cols - c) : 8;
     float gm[8], bt[8];
     wide_h<T>(p, d, row, c, v);
-    load8<PT>(static_cast<const char*>(p.gamma) + c * Elem<PT>::kBytes, live, gm);
-    load8<PT>(static_cast<const char*>(p.beta) + c * Elem<PT>::kBytes, live, bt);
+    load_params8(p.gamma, p.param_dtype, static_cast<int>(c), static_cast<int>(p.cols), gm);
+    load_params8(p.beta, p.param_dtype, static_cast<int>(c), static_cast<int>(p.cols), bt);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (v[e] - mean) * rstd * gm[e] + bt[e];
     store8<T>(p.y + (row * p.cols + c) * Elem<T>::kBytes, live, v);
@@ -321,10 +309,11 @@ struct NormBackParams {
   int64_t rows;
   int64_t cols;
   Dropout drop;
+  int32_t param_dtype;
   int32_t stream_out;
 };
 
-template <typename T, typename PT, int LANES, int K>
+template <typename T, int LANES, int K, bool WHOLE>
 __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel(const NormBackParams p) {
   constexpr int SIDE = Block<LANES>::kSide;
   __shared__ float s_red[2][Block<LANES>::kReds];
@@ -335,54 +324,60 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
   const float n = static_cast<float>(cols);
   Dropout d = p.drop;
   if (d.threshold) load_state(d);
+  // The next row's loads are under way while this one is worked on; four chunks a thread leave no registers for that, nor for
+  // the row itself next to the sums: it is read again (from L2).
+  constexpr bool AHEAD = LANES * K <= 1024;
   float dgamma[K][8], dbeta[K][8], gamma[K][8];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (lane + k * LANES) * 8;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) gamma[k][e] = dgamma[k][e] = dbeta[k][e] = 0.f;
-    if (c < cols) load8<PT>(static_cast<const char*>(p.gamma) + c * Elem<PT>::kBytes, cols - c, gamma[k]);
+    for (int e = 0; e < 8; ++e) dgamma[k][e] = dbeta[k][e] = 0.f;
+    load_params8(p.gamma, p.param_dtype, c, cols, gamma[k]);
   }
   const int64_t step = static_cast<int64_t>(gridDim.x) * SIDE;
   struct Row {
-    Chunk<T> g[K], h[K], gh[K];
+    Chunk<T, WHOLE> g[K], h[K], gh[K];
     float mean, rstd;
   };
-  const auto fetch = [&](int64_t row, Row& r) {
+  const auto fetch = [&](int64_t row, Row& r, bool all = true) {
     const int64_t at = row * p.cols * Elem<T>::kBytes;
     r.mean = p.mean[row];
     r.rstd = p.rstd[row];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (lane + k * LANES) * 8;
-      const int64_t o = at + c * Elem<T>::kBytes;
-      r.g[k].load(p.g + o, cols - c);
-      r.h[k].load(p.h + o, cols - c);
-      if (p.grad_h) r.gh[k].load(p.grad_h + o, cols - c);
+      r.g[k].load(p.g + at, c, cols);
+      r.h[k].load(p.h + at, c, cols);
+      if (all && p.grad_h) r.gh[k].load(p.grad_h + at, c, cols);
     }
   };
   // whole rounds of rows: a group past the last row repeats it and leaves its results out
   const int64_t mine = static_cast<int64_t>(blockIdx.x) * SIDE + t / LANES;
   Row now, next;
-  fetch(mine < p.rows ? mine : p.rows - 1, now);
+  if constexpr (AHEAD) fetch(mine < p.rows ? mine : p.rows - 1, now);
   for (int64_t base = static_cast<int64_t>(blockIdx.x) * SIDE; base < p.rows; base += step) {
     const int64_t row = base + t / LANES;
     const bool there = row < p.rows;
-    if (base + step < p.rows) fetch(row + step < p.rows ? row + step : p.rows - 1, next);
+    if constexpr (AHEAD) {
+      if (base + step < p.rows) fetch(row + step < p.rows ? row + step : p.rows - 1, next);
+    } else {
+      fetch(there ? row : p.rows - 1, now, false);
+    }
     float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = (lane + k * LANES) * 8;
       float g[8], h[8];
-      now.g[k].unpack(g);
-      now.h[k].unpack(h);
+      now.g[k].unpack(g, c, cols);
+      now.h[k].unpack(h, c, cols);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float z = c + e < cols ? (h[e] - now.mean) * now.rstd : 0.f;
-        const float a = g[e] * gamma[k][e];
-        s[0] += a;
-        s[1] += a * z;
-        if (there) {
+        const bool in = WHOLE ? c < cols : c + e < cols;
+        const float z = (h[e] - now.mean) * now.rstd, a = g[e] * gamma[k][e];
+        s[0] += in ? a : 0.f;
+        s[1] += in ? a * z : 0.f;
+        if (there) {  // (of columns past the row: left out below)
           dgamma[k][e] += g[e] * z;
           dbeta[k][e] += g[e];
         }
@@ -390,6 +385,15 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
     }
     row_sums<LANES, 2>(s, s_red[turn]);
     turn ^= 1;
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        now.g[k].forget();
+        now.h[k].forget();
+      }
+    } else {
+      fetch(there ? row : p.rows - 1, now);
+    }
     const float m0 = s[0] / n, m1 = s[1] / n;
     if (there) {
       const int64_t at = row * p.cols * Elem<T>::kBytes;
@@ -399,15 +403,15 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
           const int c = (lane + k * LANES) * 8;
           if (c < cols) {
             float g[8], h[8], v[8];
-            now.g[k].unpack(g);
-            now.h[k].unpack(h);
+            now.g[k].unpack(g, c, cols);
+            now.h[k].unpack(h, c, cols);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float z = (h[e] - now.mean) * now.rstd;
               v[e] = now.rstd * (g[e] * gamma[k][e] - m0 - z * m1);
             }
             if (p.grad_h) {
-              now.gh[k].unpack(g);
+              now.gh[k].unpack(g, c, cols);
 #pragma unroll
               for (int e = 0; e < 8; ++e) v[e] += g[e];
             }
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
         }
       });
     }
-    now = next;
+    if constexpr (AHEAD) now = next;
   }
   // the workgroup's sums: of the rows side by side through LDS, in their order
   const int64_t width = ceil_div(p.cols, 8) * 8;
@@ -457,7 +461,7 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
 }
 
 // Rows of any width: the workgroup's sums lie in the workspace, where a thread adds its columns' row by row.
-template <typename T, typename PT>
+template <typename T>
 __global__ void __launch_bounds__(kWideThreads) train_norm_back_wide_kernel(const NormBackParams p) {
   __shared__ float s_red[2][2 * kWideThreads / kWave];
   int turn = 0;
@@ -477,7 +481,7 @@ __global__ void __launch_bounds__(kWideThreads) train_norm_back_wide_kernel(cons
       float g[8], h[8], gamma[8];
       load8<T>(p.g + at, live, g);
       load8<T>(p.h + at, live, h);
-      load8<PT>(static_cast<const char*>(p.gamma) + c * Elem<PT>::kBytes, live, gamma);
+      load_params8(p.gamma, p.param_dtype, static_cast<int>(c), static_cast<int>(p.cols), gamma);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float z = e < live ? (h[e] - mean) * rstd : 0.f, a = g[e] * gamma[e];
@@ -497,7 +501,7 @@ __global__ void __launch_bounds__(kWideThreads) train_norm_back_wide_kernel(cons
       float g[8], h[8], gamma[8], v[8];
       load8<T>(p.g + at, live, g);
       load8<T>(p.h + at, live, h);
-      load8<PT>(static_cast<const char*>(p.gamma) + c * Elem<PT>::kBytes, live, gamma);
+      load_params8(p.gamma, p.param_dtype, static_cast<int>(c), static_cast<int>(p.cols), gamma);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = rstd * (g[e] * gamma[e] - m0 - (h[e] - mean) * rstd * m1);
       if (p.grad_h) {
@@ -512,19 +516,19 @@ __global__ void __launch_bounds__(kWideThreads) train_norm_back_wide_kernel(cons
   }
 }
 
-// dgamma (blockIdx.y 0) and dbeta (1): the workgroups' sums, 16 of them side by side, then those in order.
-constexpr int kParamThreads = 256, kParamQuads = 16;
-template <typename PT>
-__global__ void __launch_bounds__(kParamThreads) train_norm_params_kernel(const float* partial, int workgroups, int64_t cols,
-                                                                          char* dgamma, char* dbeta) {
-  constexpr int ROWS = kParamThreads / kParamQuads;
-  __shared__ float4 s_sum[kParamThreads];
+// dgamma (blockIdx.y 0) and dbeta (1): the workgroups' sums, ROWS of them side by side, then those in order. 64 for many
+// (1,024 workgroups' of 1,021 columns: 16 side by side 7.9 us, 64 5.9; 128 workgroups' of 3,584: 3.3 and 4.6).
+constexpr int kParamQuads = 16;
+template <typename PT, int ROWS>
+__global__ void __launch_bounds__(ROWS * kParamQuads) train_norm_params_kernel(const float* partial, int workgroups, int64_t cols,
+                                                                               char* dgamma, char* dbeta) {
+  __shared__ float4 s_sum[ROWS * kParamQuads];
   const int t = static_cast<int>(threadIdx.x), q = t % kParamQuads, r = t / kParamQuads;
   const int64_t width = ceil_div(cols, 8) * 8, c = (static_cast<int64_t>(blockIdx.x) * kParamQuads + q) * 4;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   if (c < width) {
     const float* const from = partial + static_cast<int64_t>(blockIdx.y) * width + c;
-#pragma unroll 4
+#pragma unroll 8
     for (int w = r; w < workgroups; w += ROWS) {
       const float4 v = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(w) * 2 * width);
       sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
@@ -557,6 +561,19 @@ void with_form(const TrainNormForm& form, F&& f) {
   else if (form.lanes == 256 && form.chunks == 1) f(Const<256>{}, Const<1>{});
   else if (form.lanes == 256 && form.chunks == 2) f(Const<256>{}, Const<2>{});
   else if (form.lanes == 256) f(Const<256>{}, Const<4>{});
+  else f(Const<512>{}, Const<4>{});
+}
+
+template <typename F>
+void with_back_form(const TrainNormForm& form, F&& f) {
+  if (form.lanes == 8) f(Const<8>{}, Const<1>{});
+  else if (form.lanes == 16) f(Const<16>{}, Const<1>{});
+  else if (form.lanes == 32) f(Const<32>{}, Const<1>{});
+  else if (form.lanes == 64) f(Const<64>{}, Const<1>{});
+  else if (form.lanes == 128) f(Const<128>{}, Const<1>{});
+  else if (form.lanes == 256) f(Const<256>{}, Const<1>{});
+  else if (form.chunks == 1) f(Const<512>{}, Const<1>{});
+  else if (form.chunks == 2) f(Const<512>{}, Const<2>{});
   else f(Const<512>{}, Const<4>{});
 }
 
@@ -624,6 +641,7 @@ extern "C" int cti_ebag_dropout_layernorm(const void* x, const void* residual, v
   a.beta = beta;
   a.cols = cols;
   a.eps = eps;
+  a.param_dtype = param_dtype;
   a.stream_out = rows * row_bytes >= kStreamOutBytes;
   const TrainNormForm form = train_norm_form(cols);
   const int threads = form.lanes == 0 ? kWideThreads : form.lanes < 256 ? 256 : form.lanes;
@@ -640,14 +658,13 @@ extern "C" int cti_ebag_dropout_layernorm(const void* x, const void* residual, v
     a.rstd = rstd + r;
     a.first_row = static_cast<uint32_t>(r);
     const dim3 grid(static_cast<unsigned>(ceil_div(a.rows, side))), block(threads);
-    with_types(dtype, param_dtype, [&](auto t, auto pt) {
+    with_type(dtype, [&](auto t) {
       using T = decltype(t);
-      using PT = decltype(pt);
       if (form.lanes == 0) {
-        hipLaunchKernelGGL((train_norm_wide_kernel<T, PT>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((train_norm_wide_kernel<T>), grid, block, 0, s, a);
       } else {
         with_form(form, [&](auto lanes, auto k) {
-          hipLaunchKernelGGL((train_norm_kernel<T, PT, decltype(lanes)::value, decltype(k)::value>), grid, block, 0, s, a);
+          hipLaunchKernelGGL((train_norm_kernel<T, decltype(lanes)::value, decltype(k)::value>), grid, block, 0, s, a);
         });
       }
     });
@@ -687,29 +704,35 @@ extern "C" int cti_ebag_dropout_layernorm_backward(const void* grad, const void*
   a.partial = static_cast<float*>(workspace);
   a.rows = rows;
   a.cols = cols;
+  a.param_dtype = param_dtype;
   a.stream_out = rows * cols * dtype_bytes(dtype) >= kStreamOutBytes;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const TrainNormForm form = train_norm_form(cols);
+  const TrainNormForm form = train_norm_back_form(cols);
   const int64_t workgroups = rows > 0 ? train_norm_workgroups(rows, cols) : 0;
   const dim3 grid(static_cast<unsigned>(workgroups));
   const dim3 block(form.lanes == 0 ? kWideThreads : form.lanes < 256 ? 256 : form.lanes);
   if (rows > 0) {
-    with_types(dtype, param_dtype, [&](auto t, auto pt) {
+    with_type(dtype, [&](auto t) {
       using T = decltype(t);
-      using PT = decltype(pt);
       if (form.lanes == 0) {
-        hipLaunchKernelGGL((train_norm_back_wide_kernel<T, PT>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((train_norm_back_wide_kernel<T>), grid, block, 0, s, a);
       } else {
-        with_form(form, [&](auto lanes, auto k) {
-          hipLaunchKernelGGL((train_norm_back_kernel<T, PT, decltype(lanes)::value, decltype(k)::value>), grid, block, 0, s, a);
+        with_back_form(form, [&](auto lanes, auto k) {
+          constexpr int LANES = decltype(lanes)::value, K = decltype(k)::value;
+          if (cols % 8 == 0) hipLaunchKernelGGL((train_norm_back_kernel<T, LANES, K, true>), grid, block, 0, s, a);
+          else hipLaunchKernelGGL((train_norm_back_kernel<T, LANES, K, false>), grid, block, 0, s, a);
         });
       }
     });
   }
   with_type(param_dtype, [&](auto pt) {
-    hipLaunchKernelGGL((train_norm_params_kernel<decltype(pt)>), dim3(static_cast<unsigned>(ceil_div(cols, kParamQuads * 4)), 2),
-                       dim3(kParamThreads), 0, s, a.partial, static_cast<int>(workgroups), cols, static_cast<char*>(dgamma),
-                       static_cast<char*>(dbeta));
+    using PT = decltype(pt);
+    const dim3 sums(static_cast<unsigned>(ceil_div(cols, kParamQuads * 4)), 2);
+    const int n = static_cast<int>(workgroups);
+    char* const dg = static_cast<char*>(dgamma);
+    char* const db = static_cast<char*>(dbeta);
+    if (n <= 256) hipLaunchKernelGGL((train_norm_params_kernel<PT, 16>), sums, dim3(16 * kParamQuads), 0, s, a.partial, n, cols, dg, db);
+    else hipLaunchKernelGGL((train_norm_params_kernel<PT, 64>), sums, dim3(64 * kParamQuads), 0, s, a.partial, n, cols, dg, db);
   });
   return check_launch("dropout_layernorm_backward");
 }

@@ -30,6 +30,7 @@ constexpr int64_t kGradMostRows = (int64_t{1} << 31) - 1;  // rows of all tables
 constexpr int64_t kGradMostDim = int64_t{1} << 22;
 constexpr int64_t kGradMostShares = int64_t{1} << 22;     // of the fill: with the tiles, below 2^32 threads
 constexpr int kGradDigitBits = 11, kGradDigits = 1 << kGradDigitBits;
+constexpr int64_t kGradIdsAlone = 8192;  // ids that one workgroup sorts
 constexpr int64_t kGradTilesUnscanned = 16;
 constexpr int64_t kGradHeadsUnscanned = 4096;
 
@@ -118,11 +119,22 @@ inline TrainNormForm train_norm_form(int64_t cols) {
   if (n <= 2048) return {512, 4};
   return {0, 0};
 }
-// Workgroups of the norm's backward pass: each adds up gamma's and beta's gradients over its rows.
+// The backward pass holds three arrays' chunks, the parameters' gradients and the next row's loads: one chunk a thread
+// as far as 512 threads go (112 registers, four wavefronts a SIMD; 4,096 columns by 256 threads of two chunks take 187, two
+// wavefronts: no faster), then two, then four that are read again instead of held.
+inline TrainNormForm train_norm_back_form(int64_t cols) {
+  const int64_t n = ceil_div(cols, 8);
+  for (const int lanes : {8, 16, 32, 64, 128, 256, 512})
+    if (n <= lanes) return {lanes, 1};
+  if (n <= 1024) return {512, 2};
+  if (n <= 2048) return {512, 4};
+  return {0, 0};
+}
+// Workgroups of the backward pass: as many as are resident (each adds up gamma's and beta's gradients over its rows).
 inline int64_t train_norm_workgroups(int64_t rows, int64_t cols) {
-  const TrainNormForm f = train_norm_form(cols);
+  const TrainNormForm f = train_norm_back_form(cols);
   const int64_t side = f.lanes > 0 && f.lanes < 256 ? 256 / f.lanes : 1;  // rows side by side
-  const int64_t most = f.lanes == 0 ? 128 : 512;
+  const int64_t most = f.lanes == 0 ? 128 : f.lanes < 512 ? 1024 : f.chunks == 1 ? 512 : 256;
   const int64_t n = ceil_div(rows, side);
   return n < most ? n : most;
 }

@@ -25,7 +25,9 @@ workspaces come from torch's allocator for the call.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -36,10 +38,17 @@ from .ops import (_check_flat_layout, _check_output, _launch, _require_on, _same
                   embedding_bag_pooled, fused_all_slots_embedding)
 
 _INDEX_TYPES = (torch.int64, torch.int32)
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+_grad_enabled = torch.is_grad_enabled
+
+
+def _any_requires_grad(*tensors) -> bool:
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def _check_index(name: str, t: torch.Tensor, index: Optional[int] = None) -> int:
@@ -76,14 +85,18 @@ def _lookup(ids, weight, scale, out, out_dtype):
     if rows < 1 or dim < 1:
         raise ValueError(f"weight has shape {tuple(weight.shape)}: no rows or no columns")
     _check_dim(dim)
-    code = _capi.dtype_code(weight.dtype)
+    dtype = weight.dtype
+    code = out_code = _capi.dtype_code(dtype)
     shape = (*ids.shape, dim)
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype or weight.dtype, device=weight.device)
+        if out_dtype is not None:
+            dtype, out_code = out_dtype, _capi.dtype_code(out_dtype)
+        out = torch.empty(shape, dtype=dtype, device=weight.device)
     else:
         _check_output("out", out, shape, out_dtype or out.dtype, index)
+        out_code = _capi.dtype_code(out.dtype)
     _launch(index, _capi.lib().cti_ebag_lookup, ids.data_ptr(), _capi.index_code(ids.dtype), ids.numel(), weight.data_ptr(), code,
-            rows, weight.stride(0), dim, scale, out.data_ptr(), _capi.dtype_code(out.dtype))
+            rows, weight.stride(0), dim, scale, out.data_ptr(), out_code)
     return out
 
 
@@ -131,10 +144,10 @@ def embedding_lookup(
     sparse tensor of the rows that occur, each once, whose making waits for their count (not within a captured graph).
     """
     scale = float(scale)
-    if _needs_grad(weight):
+    if _grad_enabled() and isinstance(weight, torch.Tensor) and weight.requires_grad:
         if out is not None:
             raise ValueError("out does not combine with a gradient: detach the weight or leave out None")
-        if isinstance(weight, torch.Tensor) and weight.dim() == 2:
+        if weight.dim() == 2:
             _check_padding(padding_idx, weight.shape[0])
         return _Lookup.apply(weight, ids, scale, padding_idx, out_dtype, sparse_grad)
     return _lookup(ids, weight, scale, out, out_dtype)
@@ -297,64 +310,90 @@ def embedding_bag_backward(
     """
     index = _require_on("grad", grad)
     dev = grad.device
-    descs, table_dev, code, width, dtype = _table_descs(tables)
-    if code == _capi.I8:
-        raise TypeError("int8 tables have no gradient")
-    if table_dev != dev:
-        raise ValueError(f"tables are on {table_dev}, grad on {dev}")
+    fields = len(tables)
+    if not _plain_tables(tables, index):
+        code, table_dev = _table_descs(tables)[2:0:-1]  # explains what is wrong with them
+        if code == _capi.I8:
+            raise TypeError("int8 tables have no gradient")
+        raise ValueError(f"tables are on {table_dev}, grad on {dev}" if table_dev != dev else "a table has no columns")
+    dtype = tables[0].dtype
+    shapes, pointers = [t.shape for t in tables], [t.data_ptr() for t in tables]
+    width = sum(shape[1] for shape in shapes)
     _check_index("values", values, index)
     _require_on("offsets", offsets, index)
-    fields = len(tables)
     if offsets.dtype != torch.int64:
         raise TypeError(f"offsets must be int64 (got {offsets.dtype})")
     if offsets.numel() < 1 or (offsets.numel() - 1) % fields:
         raise ValueError(f"offsets has {offsets.numel()} entries; expected F*B+1 with F={fields}")
     batch = (offsets.numel() - 1) // fields
-    if tuple(grad.shape) != (batch, width):
+    if grad.shape != (batch, width):
         raise ValueError(f"grad has shape {tuple(grad.shape)}, expected ({batch}, {width})")
     if width >= 2 ** 31:
         raise _capi.EbagError(_capi.EUNSUPPORTED, f"{width} columns >= 2^31")
     pool = _capi.pooling_code(pooling)
-    first = {}  # a table's identity -> the first field that has it
-    same = []
-    for f, t in enumerate(tables):
-        same.append(first.setdefault((t.data_ptr(), tuple(t.shape), t.stride()), f))
-    padding = min(_check_padding(padding_idx, t.shape[0]) for t in tables)
-    rows = sum(tables[f].shape[0] for f in set(same))
-    dim = max(t.shape[1] for t in tables)
+    same, rows = list(range(fields)), 0  # the first field with the table
+    if len(set(pointers)) == fields:
+        rows = sum(shape[0] for shape in shapes)
+    else:
+        first = {}  # a table is its address, shape and strides
+        for f, t in enumerate(tables):
+            same[f] = first.setdefault((pointers[f], shapes[f], t.stride()), f)
+            rows += shapes[f][0] if same[f] == f else 0
+    padding = _check_padding(padding_idx, min(shape[0] for shape in shapes))
+    dim = max(shape[1] for shape in shapes)
     odt = grad_dtype or dtype
     n = values.numel()
-    numbers = sums = count = None
+    numbers = sums = count = grads = None
     capacity = 0
     if compact:
         got, capacity = _compact_output(out, n, rows, dim, odt, dev, index)
         numbers, sums, count = got
-        grads = None
-        for f in range(fields):  # tells tables apart, even those without rows of their own in memory
-            descs[f].data = same[f] + 1
-            descs[f].row_stride = descs[f].dim
-    else:
-        if out is None:
-            made = {f: torch.empty(tuple(tables[f].shape), dtype=odt, device=dev) for f in set(same)}
-            grads = [made[f] for f in same]
+        pointers = [f + 1 for f in same]  # only tells the tables apart
+    elif out is None:
+        if same[-1] == fields - 1 and shapes.count(shapes[0]) == fields:  # tables alike: one allocation
+            grads = list(torch.empty((fields, *shapes[0]), dtype=odt, device=dev).unbind(0))
         else:
-            grads = list(out)
-            if len(grads) != fields:
-                raise ValueError(f"out has {len(grads)} tensors for {fields} tables")
-            for f, g in enumerate(grads):
-                _check_output(f"out[{f}]", g, tuple(tables[f].shape), odt, index)
-                if (g.data_ptr() == grads[same[f]].data_ptr()) is False:
-                    raise ValueError(f"out[{f}] and out[{same[f]}] are gradients of one table: expected one tensor")
-            if len({g.data_ptr() for g in grads}) != len(set(same)):
-                raise ValueError("out: gradients of different tables share memory")
+            made = {f: torch.empty(shapes[f], dtype=odt, device=dev) for f in set(same)}
+            grads = [made[f] for f in same]
+        pointers = [g.data_ptr() for g in grads]
+    else:
+        grads = list(out)
+        if len(grads) != fields:
+            raise ValueError(f"out has {len(grads)} tensors for {fields} tables")
         for f, g in enumerate(grads):
-            descs[f].data, descs[f].row_stride = g.data_ptr(), g.shape[1]
+            _check_output(f"out[{f}]", g, shapes[f], odt, index)
+        pointers = [g.data_ptr() for g in grads]
+        if any(pointers[f] != pointers[same[f]] for f in range(fields)) or len(set(pointers)) != len(set(same)):
+            raise ValueError("out: fields of one table expect one tensor, and different tables different ones")
+    # cti_ebag_table of every field: data, rows, row_stride, dim, out_col, row_scale
+    descs, col = [], 0
+    for (v, d), at in zip(shapes, pointers):
+        descs += (at, v, d, d, col, 0)
+        col += d
+    packed = struct.pack("QqqiiQ" * fields, *descs)
     ws, ws_ptr, ws_bytes = _workspace(n, batch * fields, rows, dim, pool, dev)
     _launch(index, _capi.lib().cti_ebag_backward, grad.data_ptr(), _capi.dtype_code(grad.dtype), width, values.data_ptr(),
-            _capi.index_code(values.dtype), n, offsets.data_ptr(), batch, fields, descs, pool, padding,
+            _capi.index_code(values.dtype), n, offsets.data_ptr(), batch, fields,
+            ctypes.cast(ctypes.c_char_p(packed), ctypes.POINTER(_capi.Table)), pool, padding,
             _capi.dtype_code(sums.dtype if compact else odt), sums.data_ptr() if compact else None,
             numbers.data_ptr() if compact else None, count.data_ptr() if compact else None, capacity, ws_ptr, ws_bytes)
     return (numbers, sums, count) if compact else grads
+
+
+def _plain_tables(tables, index: int) -> bool:
+    """Whether these are float tables of one type on device `index`, row-major, with rows and columns."""
+    if not tables:
+        return False
+    dtype = getattr(tables[0], "dtype", None)
+    if dtype not in _FLOATS:
+        return False
+    for t in tables:
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.dim() == 2 and t.get_device() == index):
+            return False
+        v, d = t.shape
+        if v < 1 or d < 1 or not (t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= d)):
+            return False
+    return True
 
 
 class _PooledTables(torch.autograd.Function):
@@ -509,7 +548,7 @@ def dropout(
     ``seed`` is a number below 2^64, or an int64 tensor (seed, offset) on the device. ``out`` may be x or residual.
     Differentiable in ``x`` and ``residual`` (``out`` must then be None); the mask is made again for it, not stored.
     """
-    if _needs_grad(x, residual):
+    if _grad_enabled() and _any_requires_grad(x, residual):
         if out is not None:
             raise ValueError("out does not combine with a gradient: detach the inputs or leave out None")
         return _Dropout.apply(x, residual, p, seed, offset)
@@ -571,7 +610,7 @@ class _Norm(torch.autograd.Function):
         grad = torch.zeros_like(h) if grad is None else grad.contiguous()
         dx, dweight, dbias, dres = dropout_add_layer_norm_backward(
             grad, h, mean, rstd, weight, None if grad_h is None else grad_h.contiguous(), residual, p, rest[0] if rest else seed, offset)
-        return dx, dres, dweight.view_as(weight), dbias.view_as(weight), None, None, None, None
+        return dx, dres, dweight, dbias, None, None, None, None
 
 
 def dropout_add_layer_norm(
@@ -592,7 +631,7 @@ def dropout_add_layer_norm(
     ``offset`` as in ``dropout``. Differentiable in x, residual, weight and bias, through y and h.
     """
     eps = float(eps)
-    if _needs_grad(x, residual, weight, bias):
+    if _grad_enabled() and _any_requires_grad(x, residual, weight, bias):
         y, mean, rstd, *h = _Norm.apply(x, residual, weight, bias, eps, p, seed, offset)
         return y, (h[0] if h else x), mean, rstd
     y, h, mean, rstd = _norm(x, weight, bias, eps, residual, p, seed, offset)
@@ -635,8 +674,7 @@ def dropout_add_layer_norm_backward(
     dres = None
     if residual:
         dres = torch.empty_like(h) if _threshold(p) else dx
-    dweight = torch.empty(cols, dtype=weight.dtype, device=h.device)
-    dbias = torch.empty_like(dweight)
+    dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
     size = _norm_workspace(rows, cols)
     ws = torch.empty(size, dtype=torch.uint8, device=h.device) if size > 0 else None
     _launch(index, _capi.lib().cti_ebag_dropout_layernorm_backward, grad.data_ptr(), h.data_ptr(), gh, mean.data_ptr(), rstd.data_ptr(),

@@ -57,6 +57,8 @@ def rules(tmp_path_factory):
         "  *p = grad_plan(n, bags, dim, elem, rows, even);\n}\n"
         'extern "C" int form(int64_t cols, int* chunks) {\n'
         "  const TrainNormForm f = train_norm_form(cols);\n  *chunks = f.chunks;\n  return f.lanes;\n}\n"
+        'extern "C" int back_form(int64_t cols, int* chunks) {\n'
+        "  const TrainNormForm f = train_norm_back_form(cols);\n  *chunks = f.chunks;\n  return f.lanes;\n}\n"
         'extern "C" int64_t norm_groups(int64_t rows, int64_t cols) { return train_norm_workgroups(rows, cols); }\n'
         'extern "C" int64_t norm_bytes(int64_t rows, int64_t cols) { return train_norm_workspace_bytes(rows, cols); }\n')
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", f"-I{CSRC}", str(work / "rules.cpp"), "-o",
@@ -65,7 +67,8 @@ def rules(tmp_path_factory):
     lib.divide.argtypes, lib.divide.restype = [ctypes.c_uint32] * 2, ctypes.c_uint32
     lib.plan.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_uint32, ctypes.c_int,
                          ctypes.POINTER(Plan)]
-    lib.form.argtypes = [ctypes.c_int64, ctypes.POINTER(ctypes.c_int)]
+    for f in (lib.form, lib.back_form):
+        f.argtypes = [ctypes.c_int64, ctypes.POINTER(ctypes.c_int)]
     for f in (lib.norm_groups, lib.norm_bytes):
         f.argtypes, f.restype = [ctypes.c_int64] * 2, ctypes.c_int64
     return lib
@@ -116,11 +119,13 @@ def test_norm_forms_cover_their_rows(rules):
     for cols in [*range(1, 600), 1023, 1024, 1025, 2047, 2049, 4095, 4097, 8191, 8192, 8193, 16383, 16384]:
         lanes = rules.form(cols, ctypes.byref(chunks))
         assert lanes * chunks.value * 8 >= cols and lanes in (8, 16, 32, 64, 256, 512)
+        lanes = rules.back_form(cols, ctypes.byref(chunks))
+        assert lanes * chunks.value * 8 >= cols and lanes in (8, 16, 32, 64, 128, 256, 512, 1024)
         for rows in (1, 3, 100, 10 ** 6):
             groups = rules.norm_groups(rows, cols)
-            assert 1 <= groups <= 512 and rules.norm_bytes(rows, cols) == groups * 2 * -(-cols // 8) * 8 * 4
+            assert 1 <= groups <= 1024 and rules.norm_bytes(rows, cols) == groups * 2 * -(-cols // 8) * 8 * 4
     for cols in (16385, 10 ** 6):
-        assert rules.form(cols, ctypes.byref(chunks)) == 0 and 1 <= rules.norm_groups(1000, cols) <= 128
+        assert rules.form(cols, ctypes.byref(chunks)) == 0 and rules.back_form(cols, ctypes.byref(chunks)) == 0 and 1 <= rules.norm_groups(1000, cols) <= 128
 
 
 # ---------------------------------------------------------------------------------------------
