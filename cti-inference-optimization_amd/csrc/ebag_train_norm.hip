@@ -324,15 +324,22 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
   const float n = static_cast<float>(cols);
   Dropout d = p.drop;
   if (d.threshold) load_state(d);
-  // The next row's loads are under way while this one is worked on; four chunks a thread leave no registers for that, nor for
-  // the row itself next to the sums: it is read again (from L2).
-  constexpr bool AHEAD = LANES * K <= 1024;
-  float dgamma[K][8], dbeta[K][8], gamma[K][8];
+  // The next row's loads are under way while this one is worked on (fp32 rows of 1,024 threads leave no registers for it).
+  constexpr bool AHEAD = LANES < 1024 || Elem<T>::kBytes == 2;
+  // gamma's and beta's gradients: in registers, or in LDS where a thread's are the float4s of its chunks, four arrays of them
+  constexpr bool IN_LDS = LANES == 1024;
+  __shared__ float4 s_sums[IN_LDS ? 4 * LANES * K : 1];
+  float dgamma[IN_LDS ? 1 : K][8], dbeta[IN_LDS ? 1 : K][8], gamma[K][8];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (lane + k * LANES) * 8;
+    if constexpr (IN_LDS) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dgamma[k][e] = dbeta[k][e] = 0.f;
+      for (int j = 0; j < 4; ++j) s_sums[(j * K + k) * LANES + lane] = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dgamma[k][e] = dbeta[k][e] = 0.f;
+    }
     load_params8(p.gamma, p.param_dtype, c, cols, gamma[k]);
   }
   const int64_t step = static_cast<int64_t>(gridDim.x) * SIDE;
@@ -377,10 +384,20 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
         const float z = (h[e] - now.mean) * now.rstd, a = g[e] * gamma[k][e];
         s[0] += in ? a : 0.f;
         s[1] += in ? a * z : 0.f;
-        if (there) {  // (of columns past the row: left out below)
+        if constexpr (IN_LDS) {
+          h[e] = g[e] * z;
+        } else if (there) {  // (of columns past the row: left out below)
           dgamma[k][e] += g[e] * z;
           dbeta[k][e] += g[e];
         }
+      }
+      if constexpr (IN_LDS) {  // one row a workgroup: it is there
+        const auto add = [&](int j, const float* v) {
+          float4& at = s_sums[(j * K + k) * LANES + lane];
+          const float4 o = at;
+          at = make_float4(o.x + v[0], o.y + v[1], o.z + v[2], o.w + v[3]);
+        };
+        add(0, h), add(1, h + 4), add(2, g), add(3, g + 4);
       }
     }
     row_sums<LANES, 2>(s, s_red[turn]);
@@ -445,6 +462,16 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
       for (int r = 0; r < SIDE; ++r) sum += s_acc[(which * SIDE + r) * wide + c];
       if (c < width) out[which * width + c] = sum;
     }
+  } else if constexpr (IN_LDS) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (lane + k * LANES) * 8;
+      if (c < cols) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<float4*>(out + (j / 2) * width + c + (j % 2) * 4) = s_sums[(j * K + k) * LANES + lane];
+      }
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -460,59 +487,89 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
   }
 }
 
-// Rows of any width: the workgroup's sums lie in the workspace, where a thread adds its columns' row by row.
+// Rows of any width: a workgroup a row, read twice (the second time from L2) ...
 template <typename T>
 __global__ void __launch_bounds__(kWideThreads) train_norm_back_wide_kernel(const NormBackParams p) {
   __shared__ float s_red[2][2 * kWideThreads / kWave];
   int turn = 0;
-  const int64_t t = threadIdx.x;
-  const float n = static_cast<float>(p.cols);
+  const int t = static_cast<int>(threadIdx.x), cols = static_cast<int>(p.cols);
+  const float n = static_cast<float>(cols);
   Dropout d = p.drop;
   if (d.threshold) load_state(d);
-  const int64_t width = ceil_div(p.cols, 8) * 8;
-  float* const out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * width;
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const float mean = p.mean[row], rstd = p.rstd[row];
-    const bool first = row == static_cast<int64_t>(blockIdx.x);
-    float s[2] = {0.f, 0.f};
-    for (int64_t c = t * 8; c < p.cols; c += kWideThreads * 8) {
-      const int live = p.cols - c < 8 ? static_cast<int>(p.cols - c) : 8;
-      const int64_t at = (row * p.cols + c) * Elem<T>::kBytes;
-      float g[8], h[8], gamma[8];
-      load8<T>(p.g + at, live, g);
-      load8<T>(p.h + at, live, h);
-      load_params8(p.gamma, p.param_dtype, static_cast<int>(c), static_cast<int>(p.cols), gamma);
+    const int64_t at = row * p.cols * Elem<T>::kBytes;
+    float s[2] = {0.f, 0.f}, g[8], h[8], gamma[8];
+    const auto load = [&](int c) {
+      Chunk<T> gc, hc;
+      gc.load(p.g + at, c, cols);
+      hc.load(p.h + at, c, cols);
+      load_params8(p.gamma, p.param_dtype, c, cols, gamma);
+      gc.unpack(g, c, cols);
+      hc.unpack(h, c, cols);
+    };
+    for (int c = t * 8; c < cols; c += kWideThreads * 8) {
+      load(c);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float z = e < live ? (h[e] - mean) * rstd : 0.f, a = g[e] * gamma[e];
+        const float z = c + e < cols ? (h[e] - mean) * rstd : 0.f, a = g[e] * gamma[e];
         s[0] += a;
         s[1] += a * z;
-        float* const sums = out + c + e;
-        sums[0] = (first ? 0.f : sums[0]) + g[e] * z;
-        sums[width] = (first ? 0.f : sums[width]) + g[e];
       }
     }
     row_sums<kWideThreads, 2>(s, s_red[turn]);
     turn ^= 1;
     const float m0 = s[0] / n, m1 = s[1] / n;
-    for (int64_t c = t * 8; c < p.cols; c += kWideThreads * 8) {
-      const int live = p.cols - c < 8 ? static_cast<int>(p.cols - c) : 8;
-      const int64_t at = (row * p.cols + c) * Elem<T>::kBytes;
-      float g[8], h[8], gamma[8], v[8];
-      load8<T>(p.g + at, live, g);
-      load8<T>(p.h + at, live, h);
-      load_params8(p.gamma, p.param_dtype, static_cast<int>(c), static_cast<int>(p.cols), gamma);
+    for (int c = t * 8; c < cols; c += kWideThreads * 8) {
+      load(c);
+      float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = rstd * (g[e] * gamma[e] - m0 - (h[e] - mean) * rstd * m1);
       if (p.grad_h) {
-        load8<T>(p.grad_h + at, live, g);
+        Chunk<T> gh;
+        gh.load(p.grad_h + at, c, cols);
+        gh.unpack(g, c, cols);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += g[e];
       }
-      if (p.dh) store8<T>(p.dh + at, live, v);
+      const int64_t to = at + static_cast<int64_t>(c) * Elem<T>::kBytes;
+      if (p.dh) store8<T>(p.dh + to, cols - c, v);
       if (d.threshold) apply_dropout(d, static_cast<uint32_t>(row), static_cast<uint32_t>(c / 8), v);
-      store8<T>(p.dx + at, live, v);
+      store8<T>(p.dx + to, cols - c, v);
     }
+  }
+}
+// ... and the parameters' gradients of 2,048 columns over a share of the rows (blockIdx.y), read once more.
+constexpr int kColumnThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kColumnThreads) train_norm_columns_kernel(const NormBackParams p) {
+  const int cols = static_cast<int>(p.cols);
+  const int64_t first = (static_cast<int64_t>(blockIdx.x) * kColumnThreads + threadIdx.x) * 8;
+  if (first >= cols) return;
+  const int c = static_cast<int>(first);
+  float dgamma[8] = {}, dbeta[8] = {};
+#pragma unroll 4
+  for (int64_t row = blockIdx.y; row < p.rows; row += gridDim.y) {
+    const int64_t at = row * p.cols * Elem<T>::kBytes;
+    Chunk<T> gc, hc;
+    gc.load(p.g + at, c, cols);
+    hc.load(p.h + at, c, cols);
+    const float mean = p.mean[row], rstd = p.rstd[row];
+    float g[8], h[8];
+    gc.unpack(g, c, cols);
+    hc.unpack(h, c, cols);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      dgamma[e] += g[e] * ((h[e] - mean) * rstd);
+      dbeta[e] += g[e];
+    }
+  }
+  const int64_t width = ceil_div(p.cols, 8) * 8;
+  float* const out = p.partial + static_cast<int64_t>(blockIdx.y) * 2 * width + c;
+#pragma unroll
+  for (int e = 0; e < 8; e += 4) {
+    *reinterpret_cast<float4*>(out + e) = make_float4(dgamma[e], dgamma[e + 1], dgamma[e + 2], dgamma[e + 3]);
+    *reinterpret_cast<float4*>(out + width + e) = make_float4(dbeta[e], dbeta[e + 1], dbeta[e + 2], dbeta[e + 3]);
   }
 }
 
@@ -572,9 +629,9 @@ void with_back_form(const TrainNormForm& form, F&& f) {
   else if (form.lanes == 64) f(Const<64>{}, Const<1>{});
   else if (form.lanes == 128) f(Const<128>{}, Const<1>{});
   else if (form.lanes == 256) f(Const<256>{}, Const<1>{});
-  else if (form.chunks == 1) f(Const<512>{}, Const<1>{});
-  else if (form.chunks == 2) f(Const<512>{}, Const<2>{});
-  else f(Const<512>{}, Const<4>{});
+  else if (form.lanes == 512 && form.chunks == 1) f(Const<512>{}, Const<1>{});
+  else if (form.lanes == 512) f(Const<512>{}, Const<2>{});
+  else f(Const<1024>{}, Const<2>{});
 }
 
 int check_norm(int64_t rows, int64_t cols, int32_t dtype, int32_t param_dtype) {
@@ -715,7 +772,9 @@ extern "C" int cti_ebag_dropout_layernorm_backward(const void* grad, const void*
     with_type(dtype, [&](auto t) {
       using T = decltype(t);
       if (form.lanes == 0) {
-        hipLaunchKernelGGL((train_norm_back_wide_kernel<T>), grid, block, 0, s, a);
+        const unsigned blocks = static_cast<unsigned>(ceil_div(cols, kColumnThreads * 8));
+        hipLaunchKernelGGL((train_norm_back_wide_kernel<T>), dim3(static_cast<unsigned>(rows < 4096 ? rows : 4096)), block, 0, s, a);
+        hipLaunchKernelGGL((train_norm_columns_kernel<T>), dim3(blocks, static_cast<unsigned>(workgroups)), dim3(kColumnThreads), 0, s, a);
       } else {
         with_back_form(form, [&](auto lanes, auto k) {
           constexpr int LANES = decltype(lanes)::value, K = decltype(k)::value;

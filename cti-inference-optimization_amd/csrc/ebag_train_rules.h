@@ -121,20 +121,22 @@ inline TrainNormForm train_norm_form(int64_t cols) {
 }
 // The backward pass holds three arrays' chunks, the parameters' gradients and the next row's loads: one chunk a thread
 // as far as 512 threads go (112 registers, four wavefronts a SIMD; 4,096 columns by 256 threads of two chunks take 187, two
-// wavefronts: no faster), then two, then four that are read again instead of held.
+// wavefronts: no faster), then two, then two of 1,024 threads with the gradients in LDS (2 x 16,384 fp32 numbers; in
+// registers they spill: 4,096 rows of 14,336 bf16 164 us).
 inline TrainNormForm train_norm_back_form(int64_t cols) {
   const int64_t n = ceil_div(cols, 8);
   for (const int lanes : {8, 16, 32, 64, 128, 256, 512})
     if (n <= lanes) return {lanes, 1};
   if (n <= 1024) return {512, 2};
-  if (n <= 2048) return {512, 4};
+  if (n <= 2048) return {1024, 2};
   return {0, 0};
 }
 // Workgroups of the backward pass: as many as are resident (each adds up gamma's and beta's gradients over its rows).
 inline int64_t train_norm_workgroups(int64_t rows, int64_t cols) {
   const TrainNormForm f = train_norm_back_form(cols);
   const int64_t side = f.lanes > 0 && f.lanes < 256 ? 256 / f.lanes : 1;  // rows side by side
-  const int64_t most = f.lanes == 0 ? 128 : f.lanes < 512 ? 1024 : f.chunks == 1 ? 512 : 256;
+  // (wider rows: workgroups for each 2,048 columns, four a CU in all)
+  const int64_t most = f.lanes == 0 ? ceil_div(1024, ceil_div(cols, 2048)) : f.lanes < 512 ? 1024 : f.chunks == 1 ? 512 : 256;
   const int64_t n = ceil_div(rows, side);
   return n < most ? n : most;
 }

@@ -125,7 +125,7 @@ def test_norm_forms_cover_their_rows(rules):
             groups = rules.norm_groups(rows, cols)
             assert 1 <= groups <= 1024 and rules.norm_bytes(rows, cols) == groups * 2 * -(-cols // 8) * 8 * 4
     for cols in (16385, 10 ** 6):
-        assert rules.form(cols, ctypes.byref(chunks)) == 0 and rules.back_form(cols, ctypes.byref(chunks)) == 0 and 1 <= rules.norm_groups(1000, cols) <= 128
+        assert rules.form(cols, ctypes.byref(chunks)) == 0 and rules.back_form(cols, ctypes.byref(chunks)) == 0 and 1 <= rules.norm_groups(1000, cols) <= 128 and rules.norm_groups(3, 2 ** 28 - 1) == 1
 
 
 # ---------------------------------------------------------------------------------------------
