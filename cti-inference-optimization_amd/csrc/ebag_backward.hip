@@ -453,6 +453,141 @@ __global__ void __launch_bounds__(THREADS) grad_sort_tile_kernel(const GradSourc
   }
 }
 
+// Up to kGradIdsRanged ids in one launch without counts: a workgroup for each range of keys (the `range_bits` top ones) reads
+// all of them, keeps its own in LDS in their order, as (the key's other bits, position), sorts these and writes them behind the
+// ids of the ranges before, which it has counted on the way. Nothing waits for another workgroup; a range that holds every
+// id takes as long as one workgroup takes for them. (16,384 ids of 15 bits in four tiles and four launches: 37 us.)
+constexpr int kRangeThreads = 1024, kRangeWaves = kRangeThreads / kWave;
+static_assert(kGradIdsRanged <= (1 << kGradPositionBits), "a position has its bits");
+template <int ITEMS>
+__global__ void __launch_bounds__(kRangeThreads) grad_sort_ranges_kernel(const GradSource s, const Pair* in, Pair* out, int key_bits,
+                                                                         const GradFill fill) {
+  if (fills(fill)) return;
+  // (8 bits where two workgroups, of which the other fills, then fit a CU)
+  constexpr int DIGIT_BITS = ITEMS == 32 ? 9 : 8, DIGITS = 1 << DIGIT_BITS;
+  __shared__ uint32_t s_val[kRangeThreads * ITEMS];
+  __shared__ uint16_t s_hist[kRangeWaves * DIGITS];
+  __shared__ uint32_t s_start[DIGITS], s_scan[kRangeWaves], s_count[2][kRangeWaves];
+  const int t = static_cast<int>(threadIdx.x), w = t / kWave, n = static_cast<int>(s.n);
+  const uint32_t range = blockIdx.x;
+  // a wavefront reads `rows` times 64 ids side by side
+  const int rows = (n + kRangeThreads - 1) / kRangeThreads;
+  uint32_t v[ITEMS], kept = 0, mine = 0, below = 0;
+  const auto read = [&](auto key_of) {
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const int i = (w * rows + k) * kWave + lane_id();
+      v[k] = key_of(k < rows && i < n ? i : n - 1);
+    }
+  };
+  if (in) read([&](int i) { return in[i].x; });
+  else if (s.ids64) read([&](int i) { return grad_key(s, static_cast<const int64_t*>(s.ids)[i], 0); });
+  else read([&](int i) { return grad_key(s, static_cast<const int32_t*>(s.ids)[i], 0); });
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    if (k < rows) {
+      const bool there = (w * rows + k) * kWave + lane_id() < n;
+      const uint32_t r = v[k] >> key_bits;
+      const bool own = there && r == range;
+      kept |= (own ? 1u : 0u) << (k % 32);
+      mine += static_cast<uint32_t>(__popcll(__ballot(own)));
+      below += static_cast<uint32_t>(__popcll(__ballot(there && r < range)));
+    }
+  }
+  if (lane_id() == 0) {
+    s_count[0][w] = mine;
+    s_count[1][w] = below;
+  }
+  __syncthreads();
+  uint32_t at = 0, m = 0, base = 0;
+#pragma unroll
+  for (int i = 0; i < kRangeWaves; ++i) {
+    at += i < w ? s_count[0][i] : 0u;
+    m += s_count[0][i];
+    base += s_count[1][i];
+  }
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    if (k < rows) {
+      const bool own = (kept >> (k % 32)) & 1u;
+      const uint64_t lanes = __ballot(own);
+      const uint32_t place = at + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
+                                                            __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0u));
+      const uint32_t position = static_cast<uint32_t>((w * rows + k) * kWave + lane_id());
+      if (own) s_val[place] = ((v[k] & ((1u << key_bits) - 1u)) << kGradPositionBits) | position;
+      at += static_cast<uint32_t>(__popcll(lanes));
+    }
+  }
+  __syncthreads();
+  const int per = static_cast<int>((m + kRangeThreads - 1) / kRangeThreads);  // items a thread
+  const int passes = (key_bits + DIGIT_BITS - 1) / DIGIT_BITS;
+  const int digit_bits = passes > 0 ? ((key_bits + passes - 1) / passes < 2 ? 2 : (key_bits + passes - 1) / passes) : 0;
+  for (int shift = 0; m > 1 && shift < key_bits; shift += digit_bits) {
+    const int digits = 1 << digit_bits;
+    const uint32_t mask = digits - 1;
+    uint2* const hist4 = reinterpret_cast<uint2*>(s_hist);
+    for (int i = t; i < kRangeWaves * digits / 4; i += kRangeThreads) hist4[i] = make_uint2(0u, 0u);
+    __syncthreads();
+    volatile uint16_t* const hist = s_hist + w * digits;
+    uint32_t place[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      if (k < per) {
+        const uint32_t i = static_cast<uint32_t>((w * per + k) * kWave + lane_id());
+        v[k] = i < m ? s_val[i] : ~0u;  // past the end: the largest digit, and last
+        const uint32_t d = (v[k] >> (kGradPositionBits + shift)) & mask;
+        uint32_t lo = ~0u, hi = ~0u;
+#pragma unroll
+        for (int b = 0; b < DIGIT_BITS; ++b) {
+          if (b < digit_bits) {
+            const uint32_t own = static_cast<uint32_t>(static_cast<int32_t>(d << (31 - b)) >> 31);
+            const uint64_t ones = __ballot(own != 0u);
+            lo = __builtin_amdgcn_bitop3_b32(lo, static_cast<uint32_t>(ones), own, 0x90);
+            hi = __builtin_amdgcn_bitop3_b32(hi, static_cast<uint32_t>(ones >> 32), own, 0x90);
+          }
+        }
+        const uint32_t seen = hist[d];
+        const uint32_t rank = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0u));
+        place[k] = seen + rank;
+        __builtin_amdgcn_wave_barrier();
+        if (rank == 0) hist[d] = static_cast<uint16_t>(seen + static_cast<uint32_t>(__popc(lo) + __popc(hi)));
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    __syncthreads();
+    uint32_t sum[4] = {0u, 0u, 0u, 0u};
+    if (4 * t < digits) {
+#pragma unroll
+      for (int i = 0; i < kRangeWaves; ++i) {
+        const uint2 c = hist4[i * (digits / 4) + t];
+        hist4[i * (digits / 4) + t] = make_uint2(sum[0] | (sum[1] << 16), sum[2] | (sum[3] << 16));
+        sum[0] += c.x & 0xffffu, sum[1] += c.x >> 16, sum[2] += c.y & 0xffffu, sum[3] += c.y >> 16;
+      }
+    }
+    uint32_t start = group_scan<kRangeThreads>(sum[0] + sum[1] + sum[2] + sum[3], s_scan);
+    if (4 * t < digits) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s_start[4 * t + i] = start;
+        start += sum[i];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      if (k < per) {
+        const uint32_t d = (v[k] >> (kGradPositionBits + shift)) & mask;
+        s_val[place[k] + s_start[d] + s_hist[w * digits + d]] = v[k];
+      }
+    }
+    __syncthreads();
+  }
+  for (uint32_t i = t; i < m; i += kRangeThreads) {
+    const uint32_t x = s_val[i], position = x & ((1u << kGradPositionBits) - 1u);
+    out[base + i] = make_uint2((range << key_bits) | (x >> kGradPositionBits), in ? in[position].y : position);
+  }
+}
+
 __device__ __forceinline__ void tile_count(const uint32_t* key, int64_t live, int shift, int bits, uint32_t* counts,
                                            uint32_t* s_hist) {
   const int t = static_cast<int>(threadIdx.x), digits = 1 << bits;
@@ -466,7 +601,7 @@ __device__ __forceinline__ void tile_count(const uint32_t* key, int64_t live, in
   for (int i = t; i < digits; i += kSortThreads) counts[i] = s_hist[i];
 }
 
-// Keys of every tile and the counts of their first digit.
+// Keys of every tile and (counts not NULL) the counts of their first digit.
 __global__ void __launch_bounds__(kSortThreads) grad_keys_kernel(const GradSource s, Pair* out, uint32_t* counts, int bits,
                                                                  const GradFill fill) {
   if (fills(fill)) return;
@@ -481,7 +616,7 @@ __global__ void __launch_bounds__(kSortThreads) grad_keys_kernel(const GradSourc
     const int64_t i = first + item_index(k);
     if (i < s.n) out[i] = make_uint2(key[k], unit[k]);
   }
-  tile_count(key, s.n - first, 0, bits, counts + (tile << bits), s_hist);
+  if (counts) tile_count(key, s.n - first, 0, bits, counts + (tile << bits), s_hist);
 }
 
 __global__ void __launch_bounds__(kSortThreads) grad_count_kernel(const Pair* in, int64_t n, int shift, int bits, uint32_t* counts,
@@ -1370,8 +1505,10 @@ int run_gradient(GradCall& c, hipStream_t s) {
   }
   // the shares of the fill are dealt to the sort's launches evenly
   const bool scan = plan.tiles > kGradTilesUnscanned;
-  const bool alone = n <= kGradIdsAlone;
-  const int launches = alone ? 1 : (scan ? 3 : 2) * static_cast<int>(ceil_div(plan.bits, plan.digit_bits));
+  const bool bags = c.src.offsets != nullptr, alone = bags && n <= kGradIdsAlone;
+  const int range_bits = alone ? 0 : grad_range_bits(n, plan.bits);
+  const int launches = alone ? 1 : range_bits > 0 ? (bags ? 2 : 1)
+                             : (scan ? 3 : 2) * static_cast<int>(ceil_div(plan.bits, plan.digit_bits));
   int launch = 0;
   const auto grid = [&](int64_t groups) {
     fill.sort_groups = static_cast<int32_t>(groups);
@@ -1385,6 +1522,19 @@ int run_gradient(GradCall& c, hipStream_t s) {
     const dim3 g = grid(1);
     if (n <= 4096) hipLaunchKernelGGL((grad_sort_tile_kernel<512, 8>), g, threads, 0, s, c.src, buf[0], plan.bits, plan.digit_bits, fill);
     else hipLaunchKernelGGL((grad_sort_tile_kernel<1024, 8>), g, dim3(1024), 0, s, c.src, buf[0], plan.bits, plan.digit_bits, fill);
+  } else if (range_bits > 0) {
+    const Pair* keys = nullptr;
+    if (bags) {
+      const dim3 g = grid(plan.tiles);
+      hipLaunchKernelGGL(grad_keys_kernel, g, threads, 0, s, c.src, buf[0], static_cast<uint32_t*>(nullptr), 0, fill);
+      keys = buf[0];
+      at = 1;
+    }
+    const dim3 g = grid(int64_t{1} << range_bits);
+    const int key_bits = plan.bits - range_bits;
+    if (n <= 8 * kRangeThreads) hipLaunchKernelGGL((grad_sort_ranges_kernel<8>), g, dim3(kRangeThreads), 0, s, c.src, keys, buf[at], key_bits, fill);
+    else if (n <= 16 * kRangeThreads) hipLaunchKernelGGL((grad_sort_ranges_kernel<16>), g, dim3(kRangeThreads), 0, s, c.src, keys, buf[at], key_bits, fill);
+    else hipLaunchKernelGGL((grad_sort_ranges_kernel<32>), g, dim3(kRangeThreads), 0, s, c.src, keys, buf[at], key_bits, fill);
   } else {
     const int bits = plan.digit_bits;
     for (int shift = 0; shift < plan.bits; shift += bits) {

@@ -30,7 +30,9 @@ constexpr int64_t kGradMostRows = (int64_t{1} << 31) - 1;  // rows of all tables
 constexpr int64_t kGradMostDim = int64_t{1} << 22;
 constexpr int64_t kGradMostShares = int64_t{1} << 22;     // of the fill: with the tiles, below 2^32 threads
 constexpr int kGradDigitBits = 11, kGradDigits = 1 << kGradDigitBits;
-constexpr int64_t kGradIdsAlone = 8192;  // ids that one workgroup sorts
+constexpr int64_t kGradIdsAlone = 8192;    // in bags: ids that one workgroup finds and sorts
+constexpr int64_t kGradIdsRanged = 32768;  // ids that are sorted by ranges of keys
+constexpr int kGradPositionBits = 15, kGradKeyBits = 32 - kGradPositionBits;  // ids that one workgroup sorts
 constexpr int64_t kGradTilesUnscanned = 16;
 constexpr int64_t kGradHeadsUnscanned = 4096;
 
@@ -90,6 +92,18 @@ inline GradPlan grad_plan(int64_t n, int64_t mean_bags, int64_t dim, int elem_by
   p.partial = take(p.workgroups * p.blocks * 2 * (int64_t{p.lane_cols} << p.log_lanes) * 4);
   p.bytes = at;
   return p;
+}
+
+// Bits of the ranges of keys by which n ids of `bits` bits are sorted in one launch, a workgroup for each range: 64 ranges (of
+// 16,384 tokens 256 each), fewer where that leaves less than 64 ids each, and as many as leave a key its 17 bits next to a
+// position. 0: by digits, in tiles.
+inline int grad_range_bits(int64_t n, int bits) {
+  if (n > kGradIdsRanged) return 0;
+  int r = 6;
+  while (r > 1 && (n >> r) < 64) --r;
+  if (bits - r > kGradKeyBits) r = bits - kGradKeyBits;
+  if (r >= bits) r = bits - 1;
+  return r < 1 || r > 8 ? 0 : r;
 }
 
 // Bytes that every form of a gradient of these sizes fits in.

@@ -426,6 +426,8 @@ def embedding_bag_train(
 ) -> torch.Tensor:
     """``embedding_bag_pooled`` of float tables, differentiable in them (``embedding_bag_backward``)."""
     for t in tables:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("tables must be tensors: int8 pairs have no gradient")
         _check_padding(padding_idx, t.shape[0])
     return _PooledTables.apply(values, offsets, pooling, padding_idx, out_dtype, *tables)
 

@@ -55,6 +55,7 @@ def rules(tmp_path_factory):
         'extern "C" uint32_t divide(uint32_t n, uint32_t d) { return ChunkDivide::by(d).quotient(n); }\n'
         'extern "C" void plan(int64_t n, int64_t bags, int64_t dim, int elem, uint32_t rows, int even, GradPlan* p) {\n'
         "  *p = grad_plan(n, bags, dim, elem, rows, even);\n}\n"
+        'extern "C" int range_bits(int64_t n, int bits) { return grad_range_bits(n, bits); }\n'
         'extern "C" int form(int64_t cols, int* chunks) {\n'
         "  const TrainNormForm f = train_norm_form(cols);\n  *chunks = f.chunks;\n  return f.lanes;\n}\n"
         'extern "C" int back_form(int64_t cols, int* chunks) {\n'
@@ -112,6 +113,18 @@ def test_gradient_plan_holds_what_the_kernels_assume(rules):
                 (p.partial, p.workgroups * p.blocks * 2 * (p.lane_cols << p.log_lanes) * 4), (p.bytes, 0)]
         for (a, size), (b, _) in zip(ends, ends[1:]):
             assert a % 256 == 0 and a + size <= b
+
+
+def test_ranges_of_keys_leave_a_word_for_key_and_position(rules):
+    rules.range_bits.argtypes = [ctypes.c_int64, ctypes.c_int]
+    for n in [1, 2, 63, 64, 100, 127, 128, 129, 1000, 4096, 8191, 8193, 16384, 32767, 32768, 32769, 10 ** 6]:
+        for bits in range(1, 32):
+            r = rules.range_bits(n, bits)
+            if n > 32768:
+                assert r == 0
+            if r:
+                # positions have 15 bits, the rest of a key 17; a key keeps a bit outside its range's
+                assert 1 <= r <= 8 and r < bits and bits - r <= 17 and n <= 2 ** 15
 
 
 def test_norm_forms_cover_their_rows(rules):
