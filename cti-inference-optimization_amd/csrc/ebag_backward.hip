@@ -765,6 +765,7 @@ struct SumParams {
   int32_t dim;            // the widest field's
   int32_t log_lanes;      // lanes that cover a block of columns, each with `lane_cols`
   int32_t lane_cols;
+  int32_t out_dtype;
   int32_t run;            // ids a lane group
   int32_t workgroups;
   float scale;
@@ -838,7 +839,20 @@ __device__ __forceinline__ int first_column(int block, int lane, int dim, int co
   return c + cols <= dim ? c : (dim >= cols ? dim - cols : 0);
 }
 
-template <typename T, typename OT, typename FIELDS>
+// f(OT{}) for the type of the sums (the walk below knows it when it is built: 45 us against 42, a key's end being a place in
+// every unrolled step).
+template <typename F>
+__device__ __forceinline__ void with_out_type(const SumParams& p, F&& f) {
+  if (p.out_dtype == CTI_EBAG_F32) f(float{});
+  else if (p.out_dtype == CTI_EBAG_BF16) f(bf16_t{});
+  else f(f16_t{});
+}
+// One element of a row of sums.
+__device__ __forceinline__ void put_sum(const SumParams& p, char* row, int col, float v) {
+  with_out_type(p, [&](auto o) { store_one(reinterpret_cast<decltype(o)*>(row) + col, v, false); });
+}
+
+template <typename T, typename FIELDS>
 struct Sums {
   static constexpr int VEC = 16 / Elem<T>::kBytes;
   static constexpr bool kPerField = !std::is_same<FIELDS, NoFields>::value;
@@ -856,12 +870,13 @@ struct Sums {
   }
   // The row that a key's sum goes to; rank: its number among the distinct keys.
   __device__ static __forceinline__ char* target(const SumParams& p, const FIELDS& fs, uint32_t key, uint32_t unit, uint32_t rank) {
-    if (p.rows_out) return p.out + static_cast<int64_t>(rank) * p.dim * Elem<OT>::kBytes;
+    const int bytes = p.out_dtype == CTI_EBAG_F32 ? 4 : 2;
+    if (p.rows_out) return p.out + static_cast<int64_t>(rank) * p.dim * bytes;
     if constexpr (kPerField) {
       const uint32_t f = unit - p.by_fields.quotient(unit) * static_cast<uint32_t>(p.fields);
-      return fs.data[f] + static_cast<int64_t>(key - fs.base[f]) * fs.stride[f] * Elem<OT>::kBytes;
+      return fs.data[f] + static_cast<int64_t>(key - fs.base[f]) * fs.stride[f] * bytes;
     } else {
-      return p.out + static_cast<int64_t>(key) * p.dim * Elem<OT>::kBytes;
+      return p.out + static_cast<int64_t>(key) * p.dim * bytes;
     }
   }
   __device__ static __forceinline__ int width(const SumParams& p, const FIELDS& fs, uint32_t unit) {
@@ -906,9 +921,9 @@ __device__ __forceinline__ uint32_t keys_begun(const SumParams& p, uint32_t* tot
 
 // A workgroup's run of the sorted ids: `run` for each of its kSumThreads >> log_lanes lane groups.
 // blockIdx.x: the run; blockIdx.y: the block of 64 vectors of columns.
-template <typename T, typename OT, typename FIELDS>
+template <typename T, typename FIELDS>
 __global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p, const FIELDS fs) {
-  using S = Sums<T, OT, FIELDS>;
+  using S = Sums<T, FIELDS>;
   constexpr int VEC = S::VEC;
   __shared__ uint32_t s_key[kSumMost + 2];  // one before, one behind
   __shared__ uint32_t s_unit[kSumMost];
@@ -985,7 +1000,9 @@ __global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p
           float v[VEC];
 #pragma unroll
           for (int e = 0; e < VEC; ++e) v[e] = acc[e] * p.scale;
-          store_vec<OT, VEC>(row + static_cast<int64_t>(c0) * Elem<OT>::kBytes, dim - c0, v);
+          with_out_type(p, [&](auto o) {
+            store_vec<decltype(o), VEC>(row + static_cast<int64_t>(c0) * Elem<decltype(o)>::kBytes, dim - c0, v);
+          });
         }
       }
       open = false;
@@ -1062,8 +1079,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p
             const uint32_t unit = s_unit[i];
             const int dim = S::width(p, fs, unit), c0 = first_column(block, l, dim, VEC);
             if (c0 >= 0 && c0 + e < dim)
-              store_one(reinterpret_cast<OT*>(S::target(p, fs, s_key[i + 1], unit, p.rows_out ? s_rank[i] : 0u)) + c0 + e,
-                        carry * p.scale, false);
+              put_sum(p, S::target(p, fs, s_key[i + 1], unit, p.rows_out ? s_rank[i] : 0u), c0 + e, carry * p.scale);
           }
           before = carrying = false;
           carry = 0.f;
@@ -1223,7 +1239,7 @@ __global__ void __launch_bounds__(kSumThreads, (kWalkPerSimd<COLS * Elem<T>::kBy
       target[b] = reinterpret_cast<uint64_t>(p.out + static_cast<int64_t>(r) * p.dim * Elem<OT>::kBytes);
     } else if (key[b] < p.total) {
       target[b] = reinterpret_cast<uint64_t>(
-          p.per_field ? Sums<T, OT, SumFields>::target(p, fs, key[b], unit[b], 0u)
+          p.per_field ? Sums<T, SumFields>::target(p, fs, key[b], unit[b], 0u)
                       : p.out + static_cast<int64_t>(key[b]) * p.dim * Elem<OT>::kBytes);
     }
   }
@@ -1244,7 +1260,9 @@ __global__ void __launch_bounds__(kSumThreads, (kWalkPerSimd<COLS * Elem<T>::kBy
       float v[COLS];
 #pragma unroll
       for (int e = 0; e < COLS; ++e) v[e] = acc[e] * p.scale;
-      if (c0 >= 0) store_cols<OT, COLS>(cur_target + static_cast<uint32_t>(c0) * Elem<OT>::kBytes, v);
+      if (c0 >= 0) {
+        store_cols<OT, COLS>(cur_target + static_cast<uint32_t>(c0) * Elem<OT>::kBytes, v);
+      }
     }
 #pragma unroll
     for (int e = 0; e < COLS; ++e) acc[e] = 0.f;
@@ -1268,14 +1286,9 @@ __global__ void __launch_bounds__(kSumThreads, (kWalkPerSimd<COLS * Elem<T>::kBy
       }
     };
     const auto add_all = [&](int i0, const LaneCols<T, COLS>* from) {
-      if (i0 + AHEAD <= now) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) add(i0 + u, from[u]);
-      } else {
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u)
-          if (i0 + u < now) add(i0 + u, from[u]);
-      }
+      for (int u = 0; u < AHEAD; ++u)
+        if (i0 + u < now) add(i0 + u, from[u]);
     };
     if (b > 0) fetch(b, 0, rows[0]);
     for (int i0 = 0; i0 < now; i0 += 2 * AHEAD) {
@@ -1342,9 +1355,9 @@ __global__ void __launch_bounds__(kSumThreads, (kWalkPerSimd<COLS * Elem<T>::kBy
 
 // Keys that cross workgroups: the workgroup in whose run one begins and goes on adds up its own part and, in order of the
 // runs, those of the runs it crosses.
-template <typename T, typename OT, typename FIELDS>
+template <typename FIELDS>
 __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams p, const FIELDS fs) {
-  using S = Sums<T, OT, FIELDS>;
+  using S = Sums<float, FIELDS>;  // (grad itself is not read)
   __shared__ float4 s_part[kSumThreads];
   const int t = static_cast<int>(threadIdx.x), lanes = 1 << p.log_lanes, groups = kSumThreads >> p.log_lanes;
   const int64_t ids = static_cast<int64_t>(groups) * p.run, first = static_cast<int64_t>(blockIdx.x) * ids;
@@ -1388,11 +1401,11 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams 
   }
   const int dim = S::width(p, fs, unit);
   const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-  OT* const row = reinterpret_cast<OT*>(S::target(p, fs, key, unit, rank));
+  char* const row = S::target(p, fs, key, unit, rank);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int slot = q * 4 + k, c0 = first_column(block, slot / p.lane_cols, dim, p.lane_cols);
-    if (c0 >= 0 && c0 + slot % p.lane_cols < dim) store_one(row + c0 + slot % p.lane_cols, v[k] * p.scale, false);
+    if (c0 >= 0 && c0 + slot % p.lane_cols < dim) put_sum(p, row, c0 + slot % p.lane_cols, v[k] * p.scale);
   }
 }
 
@@ -1425,38 +1438,35 @@ struct GradCall {
   int64_t workspace_bytes = 0;
 };
 
-template <typename T, typename OT, int COLS>
+template <typename T, int COLS>
 void launch_walk(const SumParams& p, const SumFields& fs, dim3 grid, hipStream_t s) {
   if constexpr (COLS * Elem<T>::kBytes <= 16) {
-    if (p.inv_len) hipLaunchKernelGGL((grad_walk_kernel<T, OT, COLS, true>), grid, dim3(kSumThreads), 0, s, p, fs);
-    else hipLaunchKernelGGL((grad_walk_kernel<T, OT, COLS, false>), grid, dim3(kSumThreads), 0, s, p, fs);
+    with_type(p.out_dtype, [&](auto o) {
+      using OT = decltype(o);
+      if (p.inv_len) hipLaunchKernelGGL((grad_walk_kernel<T, OT, COLS, true>), grid, dim3(kSumThreads), 0, s, p, fs);
+      else hipLaunchKernelGGL((grad_walk_kernel<T, OT, COLS, false>), grid, dim3(kSumThreads), 0, s, p, fs);
+    });
   }
 }
-template <typename T, typename OT, typename FIELDS>
-void launch_groups(const SumParams& p, const FIELDS& fs, bool walked, dim3 grid, hipStream_t s) {
-  if (!walked) hipLaunchKernelGGL((grad_sum_kernel<T, OT, FIELDS>), grid, dim3(kSumThreads), 0, s, p, fs);
-  if (p.workgroups > 1) hipLaunchKernelGGL((grad_join_kernel<T, OT, FIELDS>), grid, dim3(kSumThreads), 0, s, p, fs);
-}
-template <typename T, typename OT>
-void launch_sums_for(const GradCall& c, int blocks, hipStream_t s) {
+void launch_sums(const GradCall& c, int blocks, hipStream_t s) {
   const SumParams& p = c.sum;
-  const dim3 grid(static_cast<unsigned>(p.workgroups), static_cast<unsigned>(blocks));
-  if (c.walk) {
-    if (p.lane_cols == 1) launch_walk<T, OT, 1>(p, c.fields, grid, s);
-    else if (p.lane_cols == 2) launch_walk<T, OT, 2>(p, c.fields, grid, s);
-    else if (p.lane_cols == 4) launch_walk<T, OT, 4>(p, c.fields, grid, s);
-    else launch_walk<T, OT, 8>(p, c.fields, grid, s);
-  }
-  if (c.per_field) launch_groups<T, OT, SumFields>(p, c.fields, c.walk, grid, s);
-  else launch_groups<T, OT, NoFields>(p, NoFields{}, c.walk, grid, s);
-}
-template <typename T>
-void launch_sums_typed(const GradCall& c, int blocks, hipStream_t s) {
-  switch (c.out_dtype) {
-    case CTI_EBAG_F32: launch_sums_for<T, float>(c, blocks, s); break;
-    case CTI_EBAG_BF16: launch_sums_for<T, bf16_t>(c, blocks, s); break;
-    default: launch_sums_for<T, f16_t>(c, blocks, s); break;
-  }
+  const dim3 grid(static_cast<unsigned>(p.workgroups), static_cast<unsigned>(blocks)), threads(kSumThreads);
+  with_type(c.grad_dtype, [&](auto t) {
+    using T = decltype(t);
+    if (c.walk) {
+      if (p.lane_cols == 1) launch_walk<T, 1>(p, c.fields, grid, s);
+      else if (p.lane_cols == 2) launch_walk<T, 2>(p, c.fields, grid, s);
+      else if (p.lane_cols == 4) launch_walk<T, 4>(p, c.fields, grid, s);
+      else launch_walk<T, 8>(p, c.fields, grid, s);
+    } else if (c.per_field) {
+      hipLaunchKernelGGL((grad_sum_kernel<T, SumFields>), grid, threads, 0, s, p, c.fields);
+    } else {
+      hipLaunchKernelGGL((grad_sum_kernel<T, NoFields>), grid, threads, 0, s, p, NoFields{});
+    }
+  });
+  if (p.workgroups == 1) return;
+  if (c.per_field) hipLaunchKernelGGL((grad_join_kernel<SumFields>), grid, threads, 0, s, p, c.fields);
+  else hipLaunchKernelGGL((grad_join_kernel<NoFields>), grid, threads, 0, s, p, NoFields{});
 }
 
 // The sort and the sums of a call whose arguments are checked.
@@ -1574,11 +1584,8 @@ int run_gradient(GradCall& c, hipStream_t s) {
     if (p.heads_scanned)
       hipLaunchKernelGGL(grad_heads_scan_kernel, dim3(1), dim3(kScanThreads), 0, s, heads, plan.workgroups);
   }
-  switch (c.grad_dtype) {
-    case CTI_EBAG_F32: launch_sums_typed<float>(c, plan.blocks, s); break;
-    case CTI_EBAG_BF16: launch_sums_typed<bf16_t>(c, plan.blocks, s); break;
-    default: launch_sums_typed<f16_t>(c, plan.blocks, s); break;
-  }
+  p.out_dtype = c.out_dtype;
+  launch_sums(c, plan.blocks, s);
   return check_launch("gradient");
 }
 
