@@ -613,11 +613,12 @@ void with_form(const TrainNormForm& form, F&& f) {
   if (form.lanes == 8) f(Const<8>{}, Const<1>{});
   else if (form.lanes == 16) f(Const<16>{}, Const<1>{});
   else if (form.lanes == 32) f(Const<32>{}, Const<1>{});
-  else if (form.lanes == 64 && form.chunks == 1) f(Const<64>{}, Const<1>{});
-  else if (form.lanes == 64) f(Const<64>{}, Const<2>{});
+  else if (form.lanes == 64) f(Const<64>{}, Const<1>{});
+  else if (form.lanes == 128) f(Const<128>{}, Const<1>{});
   else if (form.lanes == 256 && form.chunks == 1) f(Const<256>{}, Const<1>{});
-  else if (form.lanes == 256 && form.chunks == 2) f(Const<256>{}, Const<2>{});
-  else if (form.lanes == 256) f(Const<256>{}, Const<4>{});
+  else if (form.lanes == 256) f(Const<256>{}, Const<2>{});
+  else if (form.chunks == 1) f(Const<512>{}, Const<1>{});
+  else if (form.chunks == 2) f(Const<512>{}, Const<2>{});
   else f(Const<512>{}, Const<4>{});
 }
 
@@ -700,7 +701,7 @@ extern "C" int cti_ebag_dropout_layernorm(const void* x, const void* residual, v
   a.eps = eps;
   a.param_dtype = param_dtype;
   a.stream_out = rows * row_bytes >= kStreamOutBytes;
-  const TrainNormForm form = train_norm_form(cols);
+  const TrainNormForm form = train_norm_form(cols, dtype_bytes(dtype));
   const int threads = form.lanes == 0 ? kWideThreads : form.lanes < 256 ? 256 : form.lanes;
   const int side = form.lanes > 0 && form.lanes < 256 ? 256 / form.lanes : 1;
   const int64_t per_launch = (int64_t{1} << 31) / threads * side;  // rows: below 2^32 threads

@@ -74,30 +74,38 @@ def _check_dim(dim: int) -> None:
 # ------------------------------------------------------------------------------------------------
 # Lookup
 # ------------------------------------------------------------------------------------------------
+# A call's way through Python takes as long as a small kernel: what these operators check on every call is one expression, explained
+# only when it fails (as in ops.py).
 def _lookup(ids, weight, scale, out, out_dtype):
-    if not isinstance(weight, torch.Tensor) or not weight.is_cuda:
-        _require_on("weight", weight)
-    index = weight.get_device()
-    _check_index("ids", ids, index)
-    if weight.dim() != 2 or weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]:
+    if not (isinstance(weight, torch.Tensor) and isinstance(ids, torch.Tensor) and weight.is_cuda and ids.is_cuda
+            and weight.dim() == 2 and (weight.is_contiguous() or _row_major(weight)) and ids.is_contiguous()
+            and (ids.dtype is torch.int64 or ids.dtype is torch.int32) and ids.get_device() == weight.get_device()):
+        if not isinstance(weight, torch.Tensor) or not weight.is_cuda:
+            _require_on("weight", weight)
+        _check_index("ids", ids, weight.get_device())
         raise ValueError("weight must be a row-major 2-D tensor with unit column stride")
+    index = weight.get_device()
     rows, dim = weight.shape
-    if rows < 1 or dim < 1:
+    if rows < 1 or not 1 <= dim < 2 ** 31:
+        if rows >= 1 and dim >= 1:
+            _check_dim(dim)
         raise ValueError(f"weight has shape {tuple(weight.shape)}: no rows or no columns")
-    _check_dim(dim)
     dtype = weight.dtype
     code = out_code = _capi.dtype_code(dtype)
-    shape = (*ids.shape, dim)
     if out is None:
         if out_dtype is not None:
             dtype, out_code = out_dtype, _capi.dtype_code(out_dtype)
-        out = torch.empty(shape, dtype=dtype, device=weight.device)
+        out = torch.empty(*ids.shape, dim, dtype=dtype, device=weight.device)
     else:
-        _check_output("out", out, shape, out_dtype or out.dtype, index)
+        _check_output("out", out, (*ids.shape, dim), out_dtype or out.dtype, index)
         out_code = _capi.dtype_code(out.dtype)
-    _launch(index, _capi.lib().cti_ebag_lookup, ids.data_ptr(), _capi.index_code(ids.dtype), ids.numel(), weight.data_ptr(), code,
-            rows, weight.stride(0), dim, scale, out.data_ptr(), out_code)
+    _launch(index, _capi.lib().cti_ebag_lookup, ids.data_ptr(), _capi.I64 if ids.dtype is torch.int64 else _capi.I32, ids.numel(),
+            weight.data_ptr(), code, rows, weight.stride(0), dim, scale, out.data_ptr(), out_code)
     return out
+
+
+def _row_major(t: torch.Tensor) -> bool:
+    return t.stride(1) == 1 and t.stride(0) >= t.shape[1]
 
 
 class _Lookup(torch.autograd.Function):
@@ -391,7 +399,7 @@ def _plain_tables(tables, index: int) -> bool:
         if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.dim() == 2 and t.get_device() == index):
             return False
         v, d = t.shape
-        if v < 1 or d < 1 or not (t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= d)):
+        if v < 1 or d < 1 or not (t.is_contiguous() or _row_major(t)):
             return False
     return True
 
@@ -492,6 +500,10 @@ def _check_seed(p, seed, offset, index: int):
 
 def _rows_of(name: str, x) -> tuple:
     """(device index, type code, rows, columns) of a contiguous tensor of rows."""
+    if isinstance(x, torch.Tensor) and x.is_cuda and x.is_contiguous():
+        shape = x.shape
+        if len(shape) == 2 and shape[1] >= 1:
+            return x.get_device(), _capi.dtype_code(x.dtype), shape[0], shape[1]
     index = _require_on(name, x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name} must have columns, got shape {tuple(x.shape)}")
@@ -499,8 +511,9 @@ def _rows_of(name: str, x) -> tuple:
 
 
 def _check_like(name: str, t, x, index: int) -> int:
-    _require_on(name, t, index)
-    if t.shape != x.shape or t.dtype != x.dtype:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == index and t.is_contiguous() and t.dtype is x.dtype
+            and t.shape == x.shape):
+        _require_on(name, t, index)
         raise ValueError(f"{name} must be {tuple(x.shape)} {x.dtype}, got {tuple(t.shape)} {t.dtype}")
     return t.data_ptr()
 
@@ -565,10 +578,19 @@ def dropout_backward(grad: torch.Tensor, p: float, seed, offset: int = 0, out: O
 # ------------------------------------------------------------------------------------------------
 # Layer norm
 # ------------------------------------------------------------------------------------------------
-def _check_param(name: str, t, cols: int, index: int):
-    _require_on(name, t, index)
-    if t.numel() != cols:
+def _check_param(name: str, t, cols: int, index: int) -> int:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == index and t.is_contiguous() and t.numel() == cols):
+        _require_on(name, t, index)
         raise ValueError(f"{name} has {t.numel()} elements, expected {cols}")
+    return t.data_ptr()
+
+
+def _check_stats(name: str, t, rows: int, index: int) -> int:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.get_device() == index and t.is_contiguous() and t.dtype is torch.float32
+            and t.numel() == rows):
+        _require_on(name, t, index)
+        raise ValueError(f"{name} must be a contiguous float32 tensor of {rows} elements")
+    return t.data_ptr()
 
 
 def _threshold(p: float) -> int:
@@ -577,19 +599,18 @@ def _threshold(p: float) -> int:
 
 def _norm(x, weight, bias, eps, residual, p, seed, offset):
     index, code, rows, cols = _rows_of("x", x)
-    _check_param("weight", weight, cols, index)
-    _check_param("bias", bias, cols, index)
-    if weight.dtype != bias.dtype:
+    gamma, beta = _check_param("weight", weight, cols, index), _check_param("bias", bias, cols, index)
+    if weight.dtype is not bias.dtype:
         raise TypeError(f"weight and bias dtypes differ ({weight.dtype} vs {bias.dtype})")
+    param = _capi.dtype_code(weight.dtype)
     p, seed, offset, state = _check_seed(p, seed, offset, index)
     res = None if residual is None else _check_like("residual", residual, x, index)
     y = torch.empty_like(x)
     h = torch.empty_like(x) if residual is not None or _threshold(p) else None
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean = torch.empty(*x.shape[:-1], dtype=torch.float32, device=x.device) if x.dim() > 1 else torch.empty((), dtype=torch.float32, device=x.device)
     rstd = torch.empty_like(mean)
     _launch(index, _capi.lib().cti_ebag_dropout_layernorm, x.data_ptr(), res, None if h is None else h.data_ptr(), y.data_ptr(), rows,
-            cols, code, weight.data_ptr(), bias.data_ptr(), _capi.dtype_code(weight.dtype), eps, p, seed, offset, state,
-            mean.data_ptr(), rstd.data_ptr())
+            cols, code, gamma, beta, param, eps, p, seed, offset, state, mean.data_ptr(), rstd.data_ptr())
     return y, h, mean, rstd
 
 
@@ -663,13 +684,10 @@ def dropout_add_layer_norm_backward(
     are summed in fp32 over the rows, in a fixed order, and rounded once to the weight's type.
     """
     index, code, rows, cols = _rows_of("h", h)
-    _check_like("grad", grad, h, index)
+    g = _check_like("grad", grad, h, index)
     gh = None if grad_h is None else _check_like("grad_h", grad_h, h, index)
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        _require_on(name, t, index)
-        if t.dtype != torch.float32 or t.numel() != rows:
-            raise ValueError(f"{name} must be a contiguous float32 tensor of {rows} elements")
-    _check_param("weight", weight, cols, index)
+    stats = _check_stats("mean", mean, rows, index), _check_stats("rstd", rstd, rows, index)
+    gamma = _check_param("weight", weight, cols, index)
     p, seed, offset, state = _check_seed(p, seed, offset, index)
     param = _capi.dtype_code(weight.dtype)
     dx = torch.empty_like(h)
@@ -679,8 +697,8 @@ def dropout_add_layer_norm_backward(
     dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
     size = _norm_workspace(rows, cols)
     ws = torch.empty(size, dtype=torch.uint8, device=h.device) if size > 0 else None
-    _launch(index, _capi.lib().cti_ebag_dropout_layernorm_backward, grad.data_ptr(), h.data_ptr(), gh, mean.data_ptr(), rstd.data_ptr(),
-            rows, cols, code, weight.data_ptr(), param, p, seed, offset, state, dx.data_ptr(),
+    _launch(index, _capi.lib().cti_ebag_dropout_layernorm_backward, g, h.data_ptr(), gh, *stats,
+            rows, cols, code, gamma, param, p, seed, offset, state, dx.data_ptr(),
             dres.data_ptr() if dres is not None and dres is not dx else None, dweight.data_ptr(), dbias.data_ptr(),
             None if ws is None else ws.data_ptr(), size)
     return dx, dweight, dbias, dres

@@ -56,8 +56,8 @@ def rules(tmp_path_factory):
         'extern "C" void plan(int64_t n, int64_t bags, int64_t dim, int elem, uint32_t rows, int even, GradPlan* p) {\n'
         "  *p = grad_plan(n, bags, dim, elem, rows, even);\n}\n"
         'extern "C" int range_bits(int64_t n, int bits) { return grad_range_bits(n, bits); }\n'
-        'extern "C" int form(int64_t cols, int* chunks) {\n'
-        "  const TrainNormForm f = train_norm_form(cols);\n  *chunks = f.chunks;\n  return f.lanes;\n}\n"
+        'extern "C" int form(int64_t cols, int elem, int* chunks) {\n'
+        "  const TrainNormForm f = train_norm_form(cols, elem);\n  *chunks = f.chunks;\n  return f.lanes;\n}\n"
         'extern "C" int back_form(int64_t cols, int* chunks) {\n'
         "  const TrainNormForm f = train_norm_back_form(cols);\n  *chunks = f.chunks;\n  return f.lanes;\n}\n"
         'extern "C" int64_t norm_groups(int64_t rows, int64_t cols) { return train_norm_workgroups(rows, cols); }\n'
@@ -68,8 +68,8 @@ def rules(tmp_path_factory):
     lib.divide.argtypes, lib.divide.restype = [ctypes.c_uint32] * 2, ctypes.c_uint32
     lib.plan.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_uint32, ctypes.c_int,
                          ctypes.POINTER(Plan)]
-    for f in (lib.form, lib.back_form):
-        f.argtypes = [ctypes.c_int64, ctypes.POINTER(ctypes.c_int)]
+    lib.form.argtypes = [ctypes.c_int64, ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
+    lib.back_form.argtypes = [ctypes.c_int64, ctypes.POINTER(ctypes.c_int)]
     for f in (lib.norm_groups, lib.norm_bytes):
         f.argtypes, f.restype = [ctypes.c_int64] * 2, ctypes.c_int64
     return lib
@@ -130,15 +130,16 @@ def test_ranges_of_keys_leave_a_word_for_key_and_position(rules):
 def test_norm_forms_cover_their_rows(rules):
     chunks = ctypes.c_int()
     for cols in [*range(1, 600), 1023, 1024, 1025, 2047, 2049, 4095, 4097, 8191, 8192, 8193, 16383, 16384]:
-        lanes = rules.form(cols, ctypes.byref(chunks))
-        assert lanes * chunks.value * 8 >= cols and lanes in (8, 16, 32, 64, 256, 512)
+        for elem in (2, 4):
+            lanes = rules.form(cols, elem, ctypes.byref(chunks))
+            assert lanes * chunks.value * 8 >= cols and lanes in (8, 16, 32, 64, 128, 256, 512)
         lanes = rules.back_form(cols, ctypes.byref(chunks))
         assert lanes * chunks.value * 8 >= cols and lanes in (8, 16, 32, 64, 128, 256, 512, 1024)
         for rows in (1, 3, 100, 10 ** 6):
             groups = rules.norm_groups(rows, cols)
             assert 1 <= groups <= 1024 and rules.norm_bytes(rows, cols) == groups * 2 * -(-cols // 8) * 8 * 4
     for cols in (16385, 10 ** 6):
-        assert rules.form(cols, ctypes.byref(chunks)) == 0 and rules.back_form(cols, ctypes.byref(chunks)) == 0 and 1 <= rules.norm_groups(1000, cols) <= 128 and rules.norm_groups(3, 2 ** 28 - 1) == 1
+        assert rules.form(cols, 2, ctypes.byref(chunks)) == 0 and rules.back_form(cols, ctypes.byref(chunks)) == 0 and 1 <= rules.norm_groups(1000, cols) <= 128 and rules.norm_groups(3, 2 ** 28 - 1) == 1
 
 
 # ---------------------------------------------------------------------------------------------
