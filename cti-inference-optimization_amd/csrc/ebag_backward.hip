@@ -13,11 +13,17 @@
 // 2. A radix sort by digits of at most 11 bits, least significant first, in tiles of 4,096: counts of every
 //    tile, their sums over the tiles, then ranks within the tile (one ballot a bit finds the lanes of a
 //    wavefront that hold the same digit), the tile put in order in LDS and written out in runs. Few tiles add
-//    up the counts of the others themselves. A single tile is sorted in LDS, all digits in one launch.
-// 3. Sums: a workgroup takes a run of the sorted list, lane groups that cover a row's columns walk shares of
-//    it, several rows' loads in flight, and write a table row where its key ends inside the share. What
-//    crosses shares is added in LDS, what crosses workgroups goes to the workspace as fp32 rows, at most two
-//    a workgroup, and a second kernel adds these up.
+//    up the counts of the others themselves. Up to 32,768 ids are sorted in one launch, by ranges of keys; up to
+//    8,192 ids in bags in the launch that finds their bags.
+// 3. Sums: a workgroup takes a run of the sorted list, wavefronts (or, for narrow rows and tables of several
+//    widths, lane groups that cover a row's columns) walk shares of it, several rows' loads in flight, and write
+//    a table row where its key ends inside the share. What crosses shares is added in LDS, what crosses
+//    workgroups goes to the workspace as fp32 rows, at most two a workgroup, and a second kernel adds these up.
+//
+// Measured (917,504 ids in 114,688 bags of 128 bf16 columns, Zipf ids of 2M rows, 146,000 of them hit): keys 13 us,
+// sort 42, the rows' numbers 4, sums 42 (235 MB gathered from the memory-side cache; the pooling kernel takes 29 for
+// the same rows in bags of 64, with a tenth of the rows to write), join 7. The sort is bound by its launches' latency
+// (4 to 13 us each), the sums by the gather.
 #include <stdint.h>
 
 #include "ebag_train.h"
@@ -51,7 +57,8 @@ __device__ __forceinline__ int64_t load_id(const void* ids, int32_t ids64, int64
   return clamp_i64(id, 0, rows - 1);
 }
 
-// A thread takes four chunks of 8 columns, their loads under way together (one: 16,384 rows of 4,096 bf16 columns 48 us).
+// A thread takes four chunks of 8 columns, their loads under way together (16,384 rows of 4,096 bf16 columns:
+// 35 us, 4.9 TB/s of minimal bytes; one chunk a thread 38).
 // Bound by HBM where the rows are many, by the latency of an id's load and a row's behind it where they are few.
 // The last chunk of a row ends with it and overlaps the one before (the same values twice); rows of less than 8 columns are
 // one chunk.
@@ -150,7 +157,7 @@ __device__ __forceinline__ int item_index(int k) {
 // places a step, the others by reading edges from there on, 1,024 at a time. Bag j's start is event 2 (j - lo) + 2 at its place,
 // its end event 2 (j - lo) + 3 at the place behind; the largest event up to an id is its bag's start (even), or an
 // end: the id lies in no bag. (Ends looked up id by id, a search of 64 places and one for the tile's last id:
-// 917,504 ids in 114,688 bags 16 us.)
+// 917,504 ids in 114,688 bags 16 us, 13 so.)
 template <int THREADS, int ITEMS>
 __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uint32_t* key, uint32_t* unit, int32_t* s_bag,
                                           int32_t* s_wave) {
@@ -326,7 +333,7 @@ __device__ __forceinline__ bool fills(const GradFill& f) {
 // Gradient: sort
 // ---------------------------------------------------------------------------------------------
 // (key, u) of every id. Digits of up to kGradDigitBits = 11 bits (21 bits, two million rows, in two passes: 917,504
-// ids 46 us; in three of 7 bits, each tile adding up the counts of all tiles, 74).
+// ids 55 us with their keys; in three of 7 bits, each tile adding up the counts of all tiles, 74).
 typedef uint2 Pair;
 
 // The tile of a workgroup: runs of tiles to each of the 8 XCDs, to which workgroups go in turn, so that what
@@ -456,7 +463,8 @@ __global__ void __launch_bounds__(THREADS) grad_sort_tile_kernel(const GradSourc
 // Up to kGradIdsRanged ids in one launch without counts: a workgroup for each range of keys (the `range_bits` top ones) reads
 // all of them, keeps its own in LDS in their order, as (the key's other bits, position), sorts these and writes them behind the
 // ids of the ranges before, which it has counted on the way. Nothing waits for another workgroup; a range that holds every
-// id takes as long as one workgroup takes for them. (16,384 ids of 15 bits in four tiles and four launches: 37 us.)
+// id takes as long as one workgroup takes for them. (16,384 ids of 15 bits: 24 us beside a fill of 131 MB, which takes 20 by
+// itself; in four tiles and four launches 37. 5,001 ids of 10 bits: 8.6.)
 constexpr int kRangeThreads = 1024, kRangeWaves = kRangeThreads / kWave;
 static_assert(kGradIdsRanged <= (1 << kGradPositionBits), "a position has its bits");
 template <int ITEMS>
@@ -1096,13 +1104,13 @@ __global__ void __launch_bounds__(kSumThreads) grad_sum_kernel(const SumParams p
 
 // The same for rows of at least kWalkCols columns that lie one behind the other in grad: a whole wavefront
 // walks its ids, so that keys, rows' addresses and the ends of keys are scalars: an id costs a load and its
-// additions. (Lane groups of 16 lanes for 128 bf16 columns: 917,504 ids 64 us, the end of a key in one of
-// four groups stopping the others; so: see below.) COLS columns a lane; a wavefront takes `run` ids, 128 at most.
+// additions. (917,504 ids of 128 bf16 columns: 42 us. Lane groups of 16 lanes took 64, the end of a key in one of four
+// groups stopping the others.) COLS columns a lane; a wavefront takes `run` ids, 128 at most.
 constexpr int kWalkWaves = kSumThreads / kWave;
 constexpr int kWalkBatches = 2;
 
 // Addresses that went through lanes' registers are numbers: as pointers of no address space they would be loaded by flat
-// instructions, which complete in no order, so that every wait is for all of them (917,504 ids: 42.7 us).
+// instructions, which complete in no order, so that every wait is for all of them.
 template <typename V>
 using Global = __attribute__((address_space(1))) V;
 
@@ -1364,7 +1372,7 @@ __global__ void __launch_bounds__(kSumThreads) grad_join_kernel(const SumParams 
   const int block = static_cast<int>(blockIdx.y);
   const int64_t next = first + ids;
   if (next >= p.n) return;
-  // (all of these loads at once: one after the other, as far as each was needed, 7.2 us where no key crosses far)
+  // (all of these loads at once: each is a microsecond away)
   const int64_t h0 = (static_cast<int64_t>(blockIdx.x) + 1 + t) * ids;
   const uint32_t key = p.ids[next - 1].x, key_next = p.ids[next].x, key_first = p.ids[first].x;
   const uint32_t key_before = first > 0 ? p.ids[first - 1].x : 0xffffffffu;

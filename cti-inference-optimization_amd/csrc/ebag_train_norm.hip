@@ -12,9 +12,13 @@
 //
 // Bound by HBM, each array read or written once; the generator's multiplications come next. A row lies in
 // the registers of 8 lanes (64 columns) to 512 threads (16,384 columns), chunks of 8 columns a thread; wider
-// rows take a loop form. The backward pass adds up dgamma and dbeta in registers over the rows of a
-// workgroup, which go to the workspace as one fp32 row each; a second kernel adds those up in their order.
-// No atomics: results are the same bits in every run.
+// rows take a loop form. The backward pass adds up dgamma and dbeta over the rows of a workgroup, in registers
+// or (8,193 to 16,384 columns) in LDS, which go to the workspace as one fp32 row each; a second kernel adds those
+// up in their order. No atomics: results are the same bits in every run.
+//
+// Measured (16,384 x 4,096 bf16; a copy of 1 GiB reaches 5.2 TB/s here): dropout 44 us, with a residual 71 (6.1 and 5.7
+// TB/s); forward with dropout and residual 95 (5.6); backward with grad_h and both gradients out 137 (4.9), and the
+// parameters' sums 6.
 #include <stdint.h>
 
 #include "ebag_train.h"
