@@ -14,7 +14,8 @@
 // the registers of 8 lanes (64 columns) to 512 threads (16,384 columns), chunks of 8 columns a thread; wider
 // rows take a loop form. The backward pass adds up dgamma and dbeta over the rows of a workgroup, in registers
 // or (8,193 to 16,384 columns) in LDS, which go to the workspace as one fp32 row each; a second kernel adds those
-// up in their order. No atomics: results are the same bits in every run.
+// up in their order (up to 256 rows of up to 8,192 columns: in the same launch, by workgroups that read the rows once
+// more). No atomics: results are the same bits in every run.
 //
 // Measured (16,384 x 4,096 bf16; a copy of 1 GiB reaches 5.2 TB/s here): dropout 44 us, with a residual 71 (6.1 and 5.7
 // TB/s); forward with dropout and residual 95 (5.6); backward with grad_h and both gradients out 137 (4.9), and the
@@ -310,19 +311,73 @@ struct NormBackParams {
   char* dh;  // NULL: not asked for (or the same as dx)
   char* dx;
   float* partial;  // [workgroup][dgamma, dbeta][whole chunks]
+  char* dgamma;    // few rows: written by the workgroups behind the first row_groups
+  char* dbeta;
   int64_t rows;
   int64_t cols;
   Dropout drop;
   int32_t param_dtype;
   int32_t stream_out;
+  int32_t row_groups;  // workgroups that take rows
+  int32_t few;
 };
+
+// gamma's and beta's gradients of kTrainNormFewCols columns over all rows: 16 threads take a row's chunks, the others further
+// rows; their sums are added in order. s_sum: 16 floats a thread.
+template <typename T, int THREADS>
+__device__ __forceinline__ void few_rows_columns(const NormBackParams& p, int block, float* s_sum) {
+  constexpr int WIDE = kTrainNormFewCols / 8, SIDE = THREADS / WIDE;
+  const int t = static_cast<int>(threadIdx.x), lane = t % WIDE, cols = static_cast<int>(p.cols);
+  const int c = block * kTrainNormFewCols + lane * 8;
+  float sums[16] = {};
+  if (c < cols) {
+#pragma unroll 8
+    for (int row = t / WIDE; row < static_cast<int>(p.rows); row += SIDE) {
+      const int64_t at = static_cast<int64_t>(row) * p.cols * Elem<T>::kBytes;
+      Chunk<T> gc, hc;
+      gc.load(p.g + at, c, cols);
+      hc.load(p.h + at, c, cols);
+      const float mean = p.mean[row], rstd = p.rstd[row];
+      float g[8], h[8];
+      gc.unpack(g, c, cols);
+      hc.unpack(h, c, cols);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        sums[e] += g[e] * ((h[e] - mean) * rstd);
+        sums[8 + e] += g[e];
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 16; ++e) s_sum[e * THREADS + t] = sums[e];
+  __syncthreads();
+  if (t >= 2 * WIDE) return;
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = 0.f;
+    for (int r = 0; r < SIDE; ++r) v[e] += s_sum[((t / WIDE) * 8 + e) * THREADS + r * WIDE + lane];
+  }
+  if (c >= cols) return;
+  char* const out = t < WIDE ? p.dgamma : p.dbeta;
+  if (p.param_dtype == CTI_EBAG_F32) store8<float>(out + static_cast<int64_t>(c) * 4, cols - c, v);
+  else if (p.param_dtype == CTI_EBAG_BF16) store8<bf16_t>(out + static_cast<int64_t>(c) * 2, cols - c, v);
+  else store8<f16_t>(out + static_cast<int64_t>(c) * 2, cols - c, v);
+}
 
 template <typename T, int LANES, int K, bool WHOLE>
 __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel(const NormBackParams p) {
   constexpr int SIDE = Block<LANES>::kSide;
   __shared__ float s_red[2][Block<LANES>::kReds];
   int turn = 0;
-  __shared__ float s_acc[SIDE > 1 ? 2 * Block<LANES>::kThreads * 8 * K : 1];
+  constexpr bool IN_LDS = LANES == 1024;
+  __shared__ float s_acc[IN_LDS ? 1 : SIDE > 1 ? 2 * Block<LANES>::kThreads * 8 * K : 16 * Block<LANES>::kThreads];
+  if constexpr (!IN_LDS) {
+    if (static_cast<int>(blockIdx.x) >= p.row_groups) {
+      few_rows_columns<T, Block<LANES>::kThreads>(p, static_cast<int>(blockIdx.x) - p.row_groups, s_acc);
+      return;
+    }
+  }
   const int t = static_cast<int>(threadIdx.x), lane = t % LANES;
   const int cols = static_cast<int>(p.cols);
   const float n = static_cast<float>(cols);
@@ -331,7 +386,6 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
   // The next row's loads are under way while this one is worked on (fp32 rows of 1,024 threads leave no registers for it).
   constexpr bool AHEAD = LANES < 1024 || Elem<T>::kBytes == 2;
   // gamma's and beta's gradients: in registers, or in LDS where a thread's are the float4s of its chunks, four arrays of them
-  constexpr bool IN_LDS = LANES == 1024;
   __shared__ float4 s_sums[IN_LDS ? 4 * LANES * K : 1];
   float dgamma[IN_LDS ? 1 : K][8], dbeta[IN_LDS ? 1 : K][8], gamma[K][8];
 #pragma unroll
@@ -346,7 +400,7 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
     }
     load_params8(p.gamma, p.param_dtype, c, cols, gamma[k]);
   }
-  const int64_t step = static_cast<int64_t>(gridDim.x) * SIDE;
+  const int64_t step = static_cast<int64_t>(p.row_groups) * SIDE;
   struct Row {
     Chunk<T, WHOLE> g[K], h[K], gh[K];
     float mean, rstd;
@@ -445,6 +499,7 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
     }
     if constexpr (AHEAD) now = next;
   }
+  if (p.few) return;
   // the workgroup's sums: of the rows side by side through LDS, in their order
   const int64_t width = ceil_div(p.cols, 8) * 8;
   float* const out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * width;
@@ -751,10 +806,10 @@ extern "C" int cti_ebag_dropout_layernorm_backward(const void* grad, const void*
   if (!dgamma || !dbeta || (rows > 0 && (!grad || !h || !mean || !rstd || !gamma || !dx)))
     return set_error(CTI_EBAG_EINVAL, "NULL device pointer among grad/h/mean/rstd/gamma/dx/dgamma/dbeta");
   const int64_t need = train_norm_workspace_bytes(rows, cols);
-  if (rows > 0 && (!workspace || workspace_bytes < need))
+  if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(CTI_EBAG_EWORKSPACE, "workspace of %lld bytes, %lld needed", (long long)(workspace ? workspace_bytes : 0),
                      (long long)need);
-  if (rows > 0 && reinterpret_cast<uintptr_t>(workspace) % 16) return set_error(CTI_EBAG_EINVAL, "workspace is not 16-byte aligned");
+  if (need > 0 && reinterpret_cast<uintptr_t>(workspace) % 16) return set_error(CTI_EBAG_EINVAL, "workspace is not 16-byte aligned");
   a.g = static_cast<const char*>(grad);
   a.h = static_cast<const char*>(h);
   a.grad_h = static_cast<const char*>(grad_h);
@@ -771,7 +826,12 @@ extern "C" int cti_ebag_dropout_layernorm_backward(const void* grad, const void*
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const TrainNormForm form = train_norm_back_form(cols);
   const int64_t workgroups = rows > 0 ? train_norm_workgroups(rows, cols) : 0;
-  const dim3 grid(static_cast<unsigned>(workgroups));
+  const bool few = rows > 0 && train_norm_few(rows, cols);
+  a.dgamma = static_cast<char*>(dgamma);
+  a.dbeta = static_cast<char*>(dbeta);
+  a.row_groups = static_cast<int32_t>(workgroups);
+  a.few = few;
+  const dim3 grid(static_cast<unsigned>(workgroups + (few ? ceil_div(cols, kTrainNormFewCols) : 0)));
   const dim3 block(form.lanes == 0 ? kWideThreads : form.lanes < 256 ? 256 : form.lanes);
   if (rows > 0) {
     with_type(dtype, [&](auto t) {
@@ -789,6 +849,7 @@ extern "C" int cti_ebag_dropout_layernorm_backward(const void* grad, const void*
       }
     });
   }
+  if (few) return check_launch("dropout_layernorm_backward");
   with_type(param_dtype, [&](auto pt) {
     using PT = decltype(pt);
     const dim3 sums(static_cast<unsigned>(ceil_div(cols, kParamQuads * 4)), 2);

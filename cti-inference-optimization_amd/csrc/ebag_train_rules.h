@@ -155,8 +155,16 @@ inline int64_t train_norm_workgroups(int64_t rows, int64_t cols) {
   const int64_t n = ceil_div(rows, side);
   return n < 1 ? 0 : ceil_div(n, ceil_div(n, most));  // as many rows to each
 }
+// Few rows: the parameters' gradients come from workgroups of the same launch that read all rows of 128 columns once more (from
+// L2) instead of a second launch that adds up the first one's sums. Calls one after another, one launch against two: 128 x 3,584
+// 9.5 against 13.4 us (4.9 against 8.2 in a graph), 256 x 8,192 9.2 against 15.9, 256 x 256 9.5 against 13.5 (6.2 against 6.0);
+// 255 x 1,021, whose chunks are loaded by elements, 11.4 against 13.6 (11.6 against 7.7). 512 x 3,584 still 11.7 against 17.7, but
+// in a graph 512 x 1,024 9.8 against 8.1 and 1,024 x 1,024 18.1 against 11.0.
+constexpr int64_t kTrainNormFewRows = 256;
+constexpr int kTrainNormFewCols = 128;
+inline bool train_norm_few(int64_t rows, int64_t cols) { return rows <= kTrainNormFewRows && cols <= 8192; }
 inline int64_t train_norm_workspace_bytes(int64_t rows, int64_t cols) {
-  return rows <= 0 ? 0 : train_norm_workgroups(rows, cols) * 2 * ceil_div(cols, 8) * 8 * 4;
+  return rows <= 0 || train_norm_few(rows, cols) ? 0 : train_norm_workgroups(rows, cols) * 2 * ceil_div(cols, 8) * 8 * 4;
 }
 
 }  // namespace cti

@@ -631,7 +631,8 @@ int cti_ebag_dropout_layernorm(const void* x, const void* residual, void* h, voi
  * in fp32, dx from the unrounded sum, each rounded once (dgamma and dbeta to `param_dtype`).
  *   grad, h  [rows, cols] of `dtype`; grad_h: the gradient that arrives at h itself, or NULL
  *   dresidual  NULL: not written (without dropout it is dx)
- *   workspace  at least cti_ebag_dropout_layernorm_backward_workspace_bytes(rows, cols), 16-byte aligned
+ *   workspace  at least cti_ebag_dropout_layernorm_backward_workspace_bytes(rows, cols), 16-byte aligned; may be NULL where
+ *            that is 0 (few rows)
  * No output overlaps another array. rows = 0 gives dgamma = dbeta = 0.
  */
 int cti_ebag_dropout_layernorm_backward(const void* grad, const void* h, const void* grad_h, const float* mean, const float* rstd,

@@ -379,6 +379,12 @@ def test_norm_rows(pkg, dev, rows, cols, dtype, params):
     check_norm(pkg, dev, rows, cols, dtype, params, 0.2, True, False)
 
 
+@pytest.mark.parametrize("cols", [1, 9, 64, 127, 128, 129, 256, 333, 512, 1021, 2048, 3584, 4096, 5000, 8191, 8192, 8193])
+@pytest.mark.parametrize("rows,dtype,params", [(256, "bf16", "bf16"), (257, "bf16", "f32"), (300, "f32", "f16")])
+def test_norm_rows_around_the_single_launch(pkg, dev, rows, cols, dtype, params):
+    check_norm(pkg, dev, rows, cols, dtype, params, 0.1, True, True)
+
+
 def test_norm_extremes(pkg, dev):
     check_norm(pkg, dev, 40, 512, "f32", "f32", 0.0, False, False, shift=100.0)  # a mean far from 0
     check_norm(pkg, dev, 5, 256, "bf16", "bf16", 1.0, True, True)                # everything dropped
