@@ -27,6 +27,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import itertools
 import struct
 from typing import Optional, Sequence
 
@@ -319,14 +320,14 @@ def embedding_bag_backward(
     index = _require_on("grad", grad)
     dev = grad.device
     fields = len(tables)
-    if not _plain_tables(tables, index):
+    shapes, pointers, alike = _plain_tables(tables, index)
+    if shapes is None:
         code, table_dev = _table_descs(tables)[2:0:-1]  # explains what is wrong with them
         if code == _capi.I8:
             raise TypeError("int8 tables have no gradient")
         raise ValueError(f"tables are on {table_dev}, grad on {dev}" if table_dev != dev else "a table has no columns")
     dtype = tables[0].dtype
-    shapes, pointers = [t.shape for t in tables], [t.data_ptr() for t in tables]
-    width = sum(shape[1] for shape in shapes)
+    width = fields * shapes[0][1] if alike else sum(shape[1] for shape in shapes)
     _check_index("values", values, index)
     _require_on("offsets", offsets, index)
     if offsets.dtype != torch.int64:
@@ -347,8 +348,8 @@ def embedding_bag_backward(
         for f, t in enumerate(tables):
             same[f] = first.setdefault((pointers[f], shapes[f], t.stride()), f)
             rows += shapes[f][0] if same[f] == f else 0
-    padding = _check_padding(padding_idx, min(shape[0] for shape in shapes))
-    dim = max(shape[1] for shape in shapes)
+    padding = _check_padding(padding_idx, shapes[0][0] if alike else min(shape[0] for shape in shapes))
+    dim = shapes[0][1] if alike else max(shape[1] for shape in shapes)
     odt = grad_dtype or dtype
     n = values.numel()
     numbers = sums = count = grads = None
@@ -358,12 +359,15 @@ def embedding_bag_backward(
         numbers, sums, count = got
         pointers = [f + 1 for f in same]  # only tells the tables apart
     elif out is None:
-        if same[-1] == fields - 1 and shapes.count(shapes[0]) == fields:  # tables alike: one allocation
-            grads = list(torch.empty((fields, *shapes[0]), dtype=odt, device=dev).unbind(0))
+        if alike and rows == fields * shapes[0][0]:  # tables alike and none shared: one allocation
+            whole = torch.empty((rows, dim), dtype=odt, device=dev)
+            grads = list(torch.unsafe_chunk(whole, fields))
+            size = shapes[0][0] * dim * whole.element_size()
+            pointers = range(whole.data_ptr(), whole.data_ptr() + fields * size, size)
         else:
             made = {f: torch.empty(shapes[f], dtype=odt, device=dev) for f in set(same)}
             grads = [made[f] for f in same]
-        pointers = [g.data_ptr() for g in grads]
+            pointers = [g.data_ptr() for g in grads]
     else:
         grads = list(out)
         if len(grads) != fields:
@@ -374,10 +378,15 @@ def embedding_bag_backward(
         if any(pointers[f] != pointers[same[f]] for f in range(fields)) or len(set(pointers)) != len(set(same)):
             raise ValueError("out: fields of one table expect one tensor, and different tables different ones")
     # cti_ebag_table of every field: data, rows, row_stride, dim, out_col, row_scale
-    descs, col = [], 0
-    for (v, d), at in zip(shapes, pointers):
-        descs += (at, v, d, d, col, 0)
-        col += d
+    descs = [0] * (6 * fields)
+    descs[0::6] = pointers
+    if alike:
+        descs[1::6], descs[2::6], descs[3::6] = [shapes[0][0]] * fields, [dim] * fields, [dim] * fields
+        descs[4::6] = range(0, width, dim)
+    else:
+        descs[1::6], dims = [shape[0] for shape in shapes], [shape[1] for shape in shapes]
+        descs[2::6], descs[3::6] = dims, dims
+        descs[4::6] = itertools.accumulate(dims[:-1], initial=0)
     packed = struct.pack("QqqiiQ" * fields, *descs)
     ws, ws_ptr, ws_bytes = _workspace(n, batch * fields, rows, dim, pool, dev)
     _launch(index, _capi.lib().cti_ebag_backward, grad.data_ptr(), _capi.dtype_code(grad.dtype), width, values.data_ptr(),
@@ -388,20 +397,27 @@ def embedding_bag_backward(
     return (numbers, sums, count) if compact else grads
 
 
-def _plain_tables(tables, index: int) -> bool:
-    """Whether these are float tables of one type on device `index`, row-major, with rows and columns."""
+def _plain_tables(tables, index: int):
+    """(shapes, addresses, whether the shapes are all the same) of float tables of one type on device `index`, row-major,
+    with rows and columns; (None, None, False) if that is not what they are."""
+    bad = None, None, False
     if not tables:
-        return False
+        return bad
     dtype = getattr(tables[0], "dtype", None)
     if dtype not in _FLOATS:
-        return False
+        return bad
+    shapes, pointers = [], []
     for t in tables:
-        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.dim() == 2 and t.get_device() == index):
-            return False
-        v, d = t.shape
-        if v < 1 or d < 1 or not (t.is_contiguous() or _row_major(t)):
-            return False
-    return True
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype is dtype and t.get_device() == index
+                and (t.is_contiguous() or t.dim() == 2 and _row_major(t))):
+            return bad
+        shapes.append(t.shape)
+        pointers.append(t.data_ptr())
+    alike = shapes.count(shapes[0]) == len(shapes)
+    for shape in shapes[:1] if alike else shapes:
+        if len(shape) != 2 or shape[0] < 1 or shape[1] < 1:
+            return bad
+    return shapes, pointers, alike
 
 
 class _PooledTables(torch.autograd.Function):
