@@ -463,8 +463,9 @@ __global__ void __launch_bounds__(THREADS) grad_sort_tile_kernel(const GradSourc
 // Up to kGradIdsRanged ids in one launch without counts: a workgroup for each range of keys (the `range_bits` top ones) reads
 // all of them, keeps its own in LDS in their order, as (the key's other bits, position), sorts these and writes them behind the
 // ids of the ranges before, which it has counted on the way. Nothing waits for another workgroup; a range that holds every
-// id takes as long as one workgroup takes for them. (16,384 ids of 15 bits: 24 us beside a fill of 131 MB, which takes 20 by
-// itself; in four tiles and four launches 37. 5,001 ids of 10 bits: 8.6.)
+// id takes as long as one workgroup takes for them. (19 bits without a fill: 8,192 ids 10 us, 16,384 13, 32,768 19; with the sort's
+// steps unrolled for a range of any size alone, their conditions held as scalars, 12, 16 and 25. Beside a fill of 131 MB, which
+// takes 20 by itself, 16,384 ids in four tiles and four launches 37.)
 constexpr int kRangeThreads = 1024, kRangeWaves = kRangeThreads / kWave;
 static_assert(kGradIdsRanged <= (1 << kGradPositionBits), "a position has its bits");
 template <int ITEMS>
@@ -480,26 +481,32 @@ __global__ void __launch_bounds__(kRangeThreads) grad_sort_ranges_kernel(const G
   const uint32_t range = blockIdx.x;
   // a wavefront reads `rows` times 64 ids side by side
   const int rows = (n + kRangeThreads - 1) / kRangeThreads;
+  const int first = w * rows * kWave + lane_id(), end = (w + 1) * rows * kWave < n ? (w + 1) * rows * kWave : n;
   uint32_t v[ITEMS], kept = 0, mine = 0, below = 0;
   const auto read = [&](auto key_of) {
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      const int i = (w * rows + k) * kWave + lane_id();
-      v[k] = key_of(k < rows && i < n ? i : n - 1);
+    for (int g = 0; g < ITEMS; g += 8) {  // (a condition an item would hold a scalar each)
+      if (g < rows) {
+#pragma unroll
+        for (int k = g; k < g + 8; ++k) v[k] = key_of(first + k * kWave < end ? first + k * kWave : n - 1);
+      }
     }
   };
   if (in) read([&](int i) { return in[i].x; });
   else if (s.ids64) read([&](int i) { return grad_key(s, static_cast<const int64_t*>(s.ids)[i], 0); });
   else read([&](int i) { return grad_key(s, static_cast<const int32_t*>(s.ids)[i], 0); });
 #pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    if (k < rows) {
-      const bool there = (w * rows + k) * kWave + lane_id() < n;
-      const uint32_t r = v[k] >> key_bits;
-      const bool own = there && r == range;
-      kept |= (own ? 1u : 0u) << (k % 32);
-      mine += static_cast<uint32_t>(__popcll(__ballot(own)));
-      below += static_cast<uint32_t>(__popcll(__ballot(there && r < range)));
+  for (int g = 0; g < ITEMS; g += 8) {
+    if (g < rows) {
+#pragma unroll
+      for (int k = g; k < g + 8; ++k) {
+        const bool there = first + k * kWave < end;
+        const uint32_t r = v[k] >> key_bits;
+        const bool own = there && r == range;
+        kept |= (own ? 1u : 0u) << k;
+        mine += static_cast<uint32_t>(__popcll(__ballot(own)));
+        below += static_cast<uint32_t>(__popcll(__ballot(there && r < range)));
+      }
     }
   }
   if (lane_id() == 0) {
@@ -515,81 +522,88 @@ __global__ void __launch_bounds__(kRangeThreads) grad_sort_ranges_kernel(const G
     base += s_count[1][i];
   }
 #pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    if (k < rows) {
-      const bool own = (kept >> (k % 32)) & 1u;
-      const uint64_t lanes = __ballot(own);
-      const uint32_t place = at + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
-                                                            __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0u));
-      const uint32_t position = static_cast<uint32_t>((w * rows + k) * kWave + lane_id());
-      if (own) s_val[place] = ((v[k] & ((1u << key_bits) - 1u)) << kGradPositionBits) | position;
-      at += static_cast<uint32_t>(__popcll(lanes));
+  for (int g = 0; g < ITEMS; g += 8) {
+    if (g < rows) {
+#pragma unroll
+      for (int k = g; k < g + 8; ++k) {
+        const bool own = (kept >> k) & 1u;
+        const uint64_t lanes = __ballot(own);
+        const uint32_t place = at + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32),
+                                                              __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0u));
+        if (own) s_val[place] = ((v[k] & ((1u << key_bits) - 1u)) << kGradPositionBits) | static_cast<uint32_t>(first + k * kWave);
+        at += static_cast<uint32_t>(__popcll(lanes));
+      }
     }
   }
   __syncthreads();
   const int per = static_cast<int>((m + kRangeThreads - 1) / kRangeThreads);  // items a thread
   const int passes = (key_bits + DIGIT_BITS - 1) / DIGIT_BITS;
   const int digit_bits = passes > 0 ? ((key_bits + passes - 1) / passes < 2 ? 2 : (key_bits + passes - 1) / passes) : 0;
-  for (int shift = 0; m > 1 && shift < key_bits; shift += digit_bits) {
-    const int digits = 1 << digit_bits;
-    const uint32_t mask = digits - 1;
-    uint2* const hist4 = reinterpret_cast<uint2*>(s_hist);
-    for (int i = t; i < kRangeWaves * digits / 4; i += kRangeThreads) hist4[i] = make_uint2(0u, 0u);
-    __syncthreads();
-    volatile uint16_t* const hist = s_hist + w * digits;
-    uint32_t place[ITEMS];
+  const auto sort = [&](auto most) {
+    constexpr int PER = decltype(most)::value;  // per <= PER; ranges are mostly small, and code that is skipped is still fetched
+    for (int shift = 0; m > 1 && shift < key_bits; shift += digit_bits) {
+      const int digits = 1 << digit_bits;
+      const uint32_t mask = digits - 1;
+      uint2* const hist4 = reinterpret_cast<uint2*>(s_hist);
+      for (int i = t; i < kRangeWaves * digits / 4; i += kRangeThreads) hist4[i] = make_uint2(0u, 0u);
+      __syncthreads();
+      volatile uint16_t* const hist = s_hist + w * digits;
+      uint32_t x[PER], place[PER];
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      if (k < per) {
-        const uint32_t i = static_cast<uint32_t>((w * per + k) * kWave + lane_id());
-        v[k] = i < m ? s_val[i] : ~0u;  // past the end: the largest digit, and last
-        const uint32_t d = (v[k] >> (kGradPositionBits + shift)) & mask;
-        uint32_t lo = ~0u, hi = ~0u;
+      for (int k = 0; k < PER; ++k) {
+        if (k < per) {
+          const uint32_t i = static_cast<uint32_t>((w * per + k) * kWave + lane_id());
+          x[k] = i < m ? s_val[i] : ~0u;  // past the end: the largest digit, and last
+          const uint32_t d = (x[k] >> (kGradPositionBits + shift)) & mask;
+          uint32_t lo = ~0u, hi = ~0u;
 #pragma unroll
-        for (int b = 0; b < DIGIT_BITS; ++b) {
-          if (b < digit_bits) {
-            const uint32_t own = static_cast<uint32_t>(static_cast<int32_t>(d << (31 - b)) >> 31);
-            const uint64_t ones = __ballot(own != 0u);
-            lo = __builtin_amdgcn_bitop3_b32(lo, static_cast<uint32_t>(ones), own, 0x90);
-            hi = __builtin_amdgcn_bitop3_b32(hi, static_cast<uint32_t>(ones >> 32), own, 0x90);
+          for (int b = 0; b < DIGIT_BITS; ++b) {
+            if (b < digit_bits) {
+              const uint32_t own = static_cast<uint32_t>(static_cast<int32_t>(d << (31 - b)) >> 31);
+              const uint64_t ones = __ballot(own != 0u);
+              lo = __builtin_amdgcn_bitop3_b32(lo, static_cast<uint32_t>(ones), own, 0x90);
+              hi = __builtin_amdgcn_bitop3_b32(hi, static_cast<uint32_t>(ones >> 32), own, 0x90);
+            }
           }
+          const uint32_t seen = hist[d];
+          const uint32_t rank = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0u));
+          place[k] = seen + rank;
+          __builtin_amdgcn_wave_barrier();
+          if (rank == 0) hist[d] = static_cast<uint16_t>(seen + static_cast<uint32_t>(__popc(lo) + __popc(hi)));
+          __builtin_amdgcn_wave_barrier();
         }
-        const uint32_t seen = hist[d];
-        const uint32_t rank = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0u));
-        place[k] = seen + rank;
-        __builtin_amdgcn_wave_barrier();
-        if (rank == 0) hist[d] = static_cast<uint16_t>(seen + static_cast<uint32_t>(__popc(lo) + __popc(hi)));
-        __builtin_amdgcn_wave_barrier();
       }
-    }
-    __syncthreads();
-    uint32_t sum[4] = {0u, 0u, 0u, 0u};
-    if (4 * t < digits) {
+      __syncthreads();
+      uint32_t sum[4] = {0u, 0u, 0u, 0u};
+      if (4 * t < digits) {
 #pragma unroll
-      for (int i = 0; i < kRangeWaves; ++i) {
-        const uint2 c = hist4[i * (digits / 4) + t];
-        hist4[i * (digits / 4) + t] = make_uint2(sum[0] | (sum[1] << 16), sum[2] | (sum[3] << 16));
-        sum[0] += c.x & 0xffffu, sum[1] += c.x >> 16, sum[2] += c.y & 0xffffu, sum[3] += c.y >> 16;
+        for (int i = 0; i < kRangeWaves; ++i) {
+          const uint2 c = hist4[i * (digits / 4) + t];
+          hist4[i * (digits / 4) + t] = make_uint2(sum[0] | (sum[1] << 16), sum[2] | (sum[3] << 16));
+          sum[0] += c.x & 0xffffu, sum[1] += c.x >> 16, sum[2] += c.y & 0xffffu, sum[3] += c.y >> 16;
+        }
       }
-    }
-    uint32_t start = group_scan<kRangeThreads>(sum[0] + sum[1] + sum[2] + sum[3], s_scan);
-    if (4 * t < digits) {
+      uint32_t start = group_scan<kRangeThreads>(sum[0] + sum[1] + sum[2] + sum[3], s_scan);
+      if (4 * t < digits) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s_start[4 * t + i] = start;
-        start += sum[i];
+        for (int i = 0; i < 4; ++i) {
+          s_start[4 * t + i] = start;
+          start += sum[i];
+        }
       }
-    }
-    __syncthreads();
+      __syncthreads();
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      if (k < per) {
-        const uint32_t d = (v[k] >> (kGradPositionBits + shift)) & mask;
-        s_val[place[k] + s_start[d] + s_hist[w * digits + d]] = v[k];
+      for (int k = 0; k < PER; ++k) {
+        if (k < per) {
+          const uint32_t d = (x[k] >> (kGradPositionBits + shift)) & mask;
+          s_val[place[k] + s_start[d] + s_hist[w * digits + d]] = x[k];
+        }
       }
+      __syncthreads();
     }
-    __syncthreads();
-  }
+  };
+  if (per <= 2) sort(std::integral_constant<int, 2>{});
+  else sort(std::integral_constant<int, ITEMS>{});
   for (uint32_t i = t; i < m; i += kRangeThreads) {
     const uint32_t x = s_val[i], position = x & ((1u << kGradPositionBits) - 1u);
     out[base + i] = make_uint2((range << key_bits) | (x >> kGradPositionBits), in ? in[position].y : position);
@@ -609,22 +623,28 @@ __device__ __forceinline__ void tile_count(const uint32_t* key, int64_t live, in
   for (int i = t; i < digits; i += kSortThreads) counts[i] = s_hist[i];
 }
 
-// Keys of every tile and (counts not NULL) the counts of their first digit.
+// Fewer ids a tile where few ids are sorted by ranges, which need no tiles of 4,096: more workgroups, fewer bags for each (21,500
+// ids in 7,168 bags beside half a fill of 72 MB: 15 us, so 11; 512 ids a tile 10.6).
+constexpr int kRangeKeyItems = 2;
+// Keys of every tile of ITEMS ids a thread and (tiles of 4,096) the counts of their first digit.
+template <int ITEMS>
 __global__ void __launch_bounds__(kSortThreads) grad_keys_kernel(const GradSource s, Pair* out, uint32_t* counts, int bits,
                                                                  const GradFill fill) {
   if (fills(fill)) return;
-  __shared__ int32_t s_bag[kTile];
-  __shared__ uint32_t s_hist[kGradDigits];
+  __shared__ int32_t s_bag[kSortThreads * ITEMS];
   __shared__ int32_t s_wave[kSortThreads / kWave];
-  uint32_t key[kItems], unit[kItems];
-  const int64_t tile = tile_of(blockIdx.x, fill.sort_groups), first = tile * kTile;
-  tile_keys<kSortThreads, kItems>(s, tile, key, unit, s_bag, s_wave);
+  uint32_t key[ITEMS], unit[ITEMS];
+  const int64_t tile = tile_of(blockIdx.x, fill.sort_groups), first = tile * (kSortThreads * ITEMS);
+  tile_keys<kSortThreads, ITEMS>(s, tile, key, unit, s_bag, s_wave);
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int64_t i = first + item_index(k);
+  for (int k = 0; k < ITEMS; ++k) {
+    const int64_t i = first + item_index<ITEMS>(k);
     if (i < s.n) out[i] = make_uint2(key[k], unit[k]);
   }
-  if (counts) tile_count(key, s.n - first, 0, bits, counts + (tile << bits), s_hist);
+  if constexpr (ITEMS == kItems) {
+    __shared__ uint32_t s_hist[kGradDigits];
+    tile_count(key, s.n - first, 0, bits, counts + (tile << bits), s_hist);
+  }
 }
 
 __global__ void __launch_bounds__(kSortThreads) grad_count_kernel(const Pair* in, int64_t n, int shift, int bits, uint32_t* counts,
@@ -1543,8 +1563,8 @@ int run_gradient(GradCall& c, hipStream_t s) {
   } else if (range_bits > 0) {
     const Pair* keys = nullptr;
     if (bags) {
-      const dim3 g = grid(plan.tiles);
-      hipLaunchKernelGGL(grad_keys_kernel, g, threads, 0, s, c.src, buf[0], static_cast<uint32_t*>(nullptr), 0, fill);
+      const dim3 g = grid(ceil_div(n, kSortThreads * kRangeKeyItems));
+      hipLaunchKernelGGL((grad_keys_kernel<kRangeKeyItems>), g, threads, 0, s, c.src, buf[0], static_cast<uint32_t*>(nullptr), 0, fill);
       keys = buf[0];
       at = 1;
     }
@@ -1557,7 +1577,7 @@ int run_gradient(GradCall& c, hipStream_t s) {
     const int bits = plan.digit_bits;
     for (int shift = 0; shift < plan.bits; shift += bits) {
       dim3 g = grid(plan.tiles);
-      if (shift == 0) hipLaunchKernelGGL(grad_keys_kernel, g, threads, 0, s, c.src, buf[0], counts, bits, fill);
+      if (shift == 0) hipLaunchKernelGGL((grad_keys_kernel<kItems>), g, threads, 0, s, c.src, buf[0], counts, bits, fill);
       else hipLaunchKernelGGL(grad_count_kernel, g, threads, 0, s, buf[at], n, shift, bits, counts, fill);
       if (scan) {
         g = grid(ceil_div(int64_t{1} << bits, kWave));

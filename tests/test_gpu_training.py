@@ -114,6 +114,31 @@ def test_lookup_gradient_of_hot_rows(pkg, dev, n, dim, shape):
     check_gradient(pkg, dev, grad, ids[torch.randperm(ids.numel(), generator=torch.Generator().manual_seed(1))], rows, padding=7)
 
 
+@pytest.mark.parametrize("n", [2047, 2048, 2049, 8193, 16385, 24576, 32768])
+def test_lookup_gradient_of_one_range_of_rows(pkg, dev, n):
+    """All ids in neighbouring rows at one end of a large table: one workgroup of the sort holds them, others none or a few."""
+    rows = 200_000
+    ids = randint(n, rows - 40, rows + 5, n)
+    check_gradient(pkg, dev, randn(n, n, 16), ids, rows)
+    ids[::1000] = 3
+    ids[5::700] = 100_001
+    check_gradient(pkg, dev, randn(n + 1, n, 16), ids, rows, padding=rows - 1)
+
+
+@pytest.mark.parametrize("fields,batch,long", [(9, 800, None), (2, 900, (1000, 3000)), (3, 30, (40, 20_000)), (1, 20_000, (7, 1024)),
+                                               (1, 18_000, (17_999, 1025))])
+def test_gradient_of_bags_in_small_tiles(pkg, dev, fields, batch, long):
+    """Some ten thousand ids in bags: empty and short ones, one over many tiles, one that ends with or just behind a tile."""
+    rows, dim, empty = 700, 24, 0.9 if batch >= 18_000 else 0.2
+    lens, values, _, val_offsets, row_offsets = make_bags(batch, fields, batch, [rows] * fields, 10, empty=empty, long=long)
+    assert 8192 < values.numel() <= 32768
+    grad = randn(batch, batch, fields * dim)
+    parts = bag_contributions(lens, values, grad, [dim] * fields, "sum")
+    want, absolute, count = ref.table_gradient(torch.cat([p[1] for p in parts]), torch.cat([p[0] for p in parts]).clamp(0, rows - 1), rows)
+    got = pkg.fused_all_slots_embedding_backward(grad.to(dev), values.to(dev), val_offsets.to(dev), row_offsets.to(dev), batch, dim, rows - 1)
+    ref.assert_within(got, want, ref.gradient_bound(want, absolute, count, torch.float32))
+
+
 def test_lookup_gradient_of_many_ids(pkg, dev):
     """More tiles than a workgroup adds up by itself, more runs than heads are summed in place."""
     n, rows = 1_300_000, 40_000
