@@ -319,7 +319,6 @@ struct NormBackParams {
   int32_t param_dtype;
   int32_t stream_out;
   int32_t row_groups;  // workgroups that take rows
-  int32_t few;
 };
 
 // gamma's and beta's gradients of kTrainNormFewCols columns over all rows: 16 threads take a row's chunks, the others further
@@ -365,14 +364,16 @@ __device__ __forceinline__ void few_rows_columns(const NormBackParams& p, int bl
   else store8<f16_t>(out + static_cast<int64_t>(c) * 2, cols - c, v);
 }
 
-template <typename T, int LANES, int K, bool WHOLE>
+// FEW: the parameters' gradients are the workgroups' behind the first row_groups (a kernel of its own: as a branch of this one
+// their registers leave the rows a wavefront less a SIMD, 4,096 x 3,584 bf16 28 -> 36 us).
+template <typename T, int LANES, int K, bool WHOLE, bool FEW>
 __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel(const NormBackParams p) {
   constexpr int SIDE = Block<LANES>::kSide;
   __shared__ float s_red[2][Block<LANES>::kReds];
   int turn = 0;
   constexpr bool IN_LDS = LANES == 1024;
-  __shared__ float s_acc[IN_LDS ? 1 : SIDE > 1 ? 2 * Block<LANES>::kThreads * 8 * K : 16 * Block<LANES>::kThreads];
-  if constexpr (!IN_LDS) {
+  __shared__ float s_acc[FEW ? 16 * Block<LANES>::kThreads : SIDE > 1 ? 2 * Block<LANES>::kThreads * 8 * K : 1];
+  if constexpr (FEW) {
     if (static_cast<int>(blockIdx.x) >= p.row_groups) {
       few_rows_columns<T, Block<LANES>::kThreads>(p, static_cast<int>(blockIdx.x) - p.row_groups, s_acc);
       return;
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(Block<LANES>::kThreads) train_norm_back_kernel
     }
     if constexpr (AHEAD) now = next;
   }
-  if (p.few) return;
+  if constexpr (FEW) return;
   // the workgroup's sums: of the rows side by side through LDS, in their order
   const int64_t width = ceil_div(p.cols, 8) * 8;
   float* const out = p.partial + static_cast<int64_t>(blockIdx.x) * 2 * width;
@@ -830,7 +831,6 @@ extern "C" int cti_ebag_dropout_layernorm_backward(const void* grad, const void*
   a.dgamma = static_cast<char*>(dgamma);
   a.dbeta = static_cast<char*>(dbeta);
   a.row_groups = static_cast<int32_t>(workgroups);
-  a.few = few;
   const dim3 grid(static_cast<unsigned>(workgroups + (few ? ceil_div(cols, kTrainNormFewCols) : 0)));
   const dim3 block(form.lanes == 0 ? kWideThreads : form.lanes < 256 ? 256 : form.lanes);
   if (rows > 0) {
@@ -843,8 +843,16 @@ extern "C" int cti_ebag_dropout_layernorm_backward(const void* grad, const void*
       } else {
         with_back_form(form, [&](auto lanes, auto k) {
           constexpr int LANES = decltype(lanes)::value, K = decltype(k)::value;
-          if (cols % 8 == 0) hipLaunchKernelGGL((train_norm_back_kernel<T, LANES, K, true>), grid, block, 0, s, a);
-          else hipLaunchKernelGGL((train_norm_back_kernel<T, LANES, K, false>), grid, block, 0, s, a);
+          if (few) {
+            if constexpr (LANES < 1024) {  // up to 8,192 columns
+              if (cols % 8 == 0) hipLaunchKernelGGL((train_norm_back_kernel<T, LANES, K, true, true>), grid, block, 0, s, a);
+              else hipLaunchKernelGGL((train_norm_back_kernel<T, LANES, K, false, true>), grid, block, 0, s, a);
+            }
+          } else if (cols % 8 == 0) {
+            hipLaunchKernelGGL((train_norm_back_kernel<T, LANES, K, true, false>), grid, block, 0, s, a);
+          } else {
+            hipLaunchKernelGGL((train_norm_back_kernel<T, LANES, K, false, false>), grid, block, 0, s, a);
+          }
         });
       }
     });
