@@ -312,21 +312,32 @@ def embedding_bag_backward(
     of which only shape, type and identity are read; at most 64).
 
     Returns a list with the gradient ``[V_f, D_f]`` of each field's table, of ``grad_dtype`` (the tables' type by
-    default); fields that share a table (the same tensor) share its gradient (the same tensor). ``out``: such a list.
+    default); fields that share a table (the same memory, shape and strides) share its gradient (the same tensor). ``out``: such a
+    list.
     With ``compact`` (tables of one width) ``(rows, grads, count)`` as in ``embedding_lookup_backward``, where row r
     of a table has the number (rows of the tables before it, shared ones counted once) + r. ``padding_idx`` is every
     table's.
     """
     index = _require_on("grad", grad)
-    dev = grad.device
-    fields = len(tables)
     shapes, pointers, alike = _plain_tables(tables, index)
     if shapes is None:
         code, table_dev = _table_descs(tables)[2:0:-1]  # explains what is wrong with them
         if code == _capi.I8:
             raise TypeError("int8 tables have no gradient")
-        raise ValueError(f"tables are on {table_dev}, grad on {dev}" if table_dev != dev else "a table has no columns")
-    dtype = tables[0].dtype
+        raise ValueError(f"tables are on {table_dev}, grad on {grad.device}" if table_dev != grad.device else "a table has no columns")
+    same = None  # the first field with the table
+    if len(set(pointers)) != len(pointers):
+        first = {}  # a table is its address, shape and strides
+        same = [first.setdefault((pointers[f], shapes[f], t.stride()), f) for f, t in enumerate(tables)]
+    return _bag_gradients(index, grad, values, offsets, shapes, alike, tables[0].dtype, same, pooling, padding_idx, grad_dtype, compact, out)
+
+
+def _bag_gradients(index, grad, values, offsets, shapes, alike, dtype, same, pooling, padding_idx, grad_dtype=None, compact=False,
+                   out=None):
+    """``embedding_bag_backward`` of tables of these shapes (``alike``: all the same) and this type; ``same[f]``: the first field with
+    field f's table (None: no field shares one)."""
+    dev = grad.device
+    fields = len(shapes)
     width = fields * shapes[0][1] if alike else sum(shape[1] for shape in shapes)
     _check_index("values", values, index)
     _require_on("offsets", offsets, index)
@@ -340,14 +351,10 @@ def embedding_bag_backward(
     if width >= 2 ** 31:
         raise _capi.EbagError(_capi.EUNSUPPORTED, f"{width} columns >= 2^31")
     pool = _capi.pooling_code(pooling)
-    same, rows = list(range(fields)), 0  # the first field with the table
-    if len(set(pointers)) == fields:
-        rows = sum(shape[0] for shape in shapes)
+    if same is None:
+        same, rows = range(fields), sum(shape[0] for shape in shapes)
     else:
-        first = {}  # a table is its address, shape and strides
-        for f, t in enumerate(tables):
-            same[f] = first.setdefault((pointers[f], shapes[f], t.stride()), f)
-            rows += shapes[f][0] if same[f] == f else 0
+        rows = sum(shapes[f][0] for f in set(same))
     padding = _check_padding(padding_idx, shapes[0][0] if alike else min(shape[0] for shape in shapes))
     dim = shapes[0][1] if alike else max(shape[1] for shape in shapes)
     odt = grad_dtype or dtype
@@ -422,22 +429,21 @@ def _plain_tables(tables, index: int):
 
 class _PooledTables(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, values, offsets, pooling, padding_idx, out_dtype, *tables):
+    def forward(ctx, values, offsets, pooling, padding_idx, out_dtype, same, *tables):
         ctx.save_for_backward(values, offsets, *tables)
-        ctx.info = (pooling, padding_idx)
+        ctx.info = (pooling, padding_idx, same)
         return embedding_bag_pooled(values, offsets, tables, pooling, out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         values, offsets, *tables = ctx.saved_tensors
-        grads = embedding_bag_backward(grad.contiguous(), values, offsets, tables, ctx.info[0], ctx.info[1])
-        seen = set()
-        for f, g in enumerate(grads):  # autograd adds up the fields' gradients of one table: its sum is in the first
-            if g.data_ptr() in seen:
-                grads[f] = None
-            seen.add(g.data_ptr())
-        return (None, None, None, None, None, *grads)
+        pooling, padding_idx, same = ctx.info
+        shapes = [t.shape for t in tables]
+        grads = _bag_gradients(grad.get_device(), grad.contiguous(), values, offsets, shapes, len(set(shapes)) == 1, tables[0].dtype,
+                               same, pooling, padding_idx)
+        # autograd adds up the fields' gradients of one table: its sum is in the first
+        return (None, None, None, None, None, None, *(g if same[f] == f else None for f, g in enumerate(grads)))
 
 
 def embedding_bag_train(
@@ -448,12 +454,17 @@ def embedding_bag_train(
     padding_idx: Optional[int] = None,
     out_dtype: Optional[torch.dtype] = None,
 ) -> torch.Tensor:
-    """``embedding_bag_pooled`` of float tables, differentiable in them (``embedding_bag_backward``)."""
+    """``embedding_bag_pooled`` of float tables, differentiable in them (``embedding_bag_backward``). Fields share a table where they
+    are given the same tensor. Tensors that only share memory, a table and what ``detach()`` makes of it among them, are tables of
+    their own, as autograd sees them.
+    """
     for t in tables:
         if not isinstance(t, torch.Tensor):
             raise TypeError("tables must be tensors: int8 pairs have no gradient")
         _check_padding(padding_idx, t.shape[0])
-    return _PooledTables.apply(values, offsets, pooling, padding_idx, out_dtype, *tables)
+    first = {}
+    same = [first.setdefault(id(t), f) for f, t in enumerate(tables)]
+    return _PooledTables.apply(values, offsets, pooling, padding_idx, out_dtype, same, *tables)
 
 
 class _PooledShared(torch.autograd.Function):

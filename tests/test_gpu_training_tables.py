@@ -1,0 +1,80 @@
+"""Which table a gradient belongs to: fields with the same tensor share one, tensors over the same memory do not, and tables
+that need no gradient take none."""
+import pytest
+import torch
+
+import _training as ref
+
+pytestmark = pytest.mark.gpu
+
+BATCH, ROWS, DIM = 30, 40, 24
+
+
+def randn(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+def make_fields(fields, seed=0, rows=ROWS, max_len=6):
+    """(values, global offsets, per field the ids and the samples that they belong to)"""
+    gen = torch.Generator().manual_seed(seed)
+    lens = torch.randint(0, max_len + 1, (fields, BATCH), generator=gen)
+    values = torch.randint(-1, rows + 1, (int(lens.sum()),), generator=gen)
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), lens.reshape(-1).cumsum(0)])
+    parts = [(values[offsets[f * BATCH]:offsets[(f + 1) * BATCH]].clamp(0, rows - 1), torch.repeat_interleave(torch.arange(BATCH), lens[f]))
+             for f in range(fields)]
+    return values, offsets, parts
+
+
+def assert_gradient(got, parts, grad, fields, dim=DIM, rows=ROWS, padding=None, mean=False):
+    """`got` is the sum over these fields' ids."""
+    ids = torch.cat([parts[f][0] for f in fields])
+    g = torch.cat([grad[:, f * dim:(f + 1) * dim][parts[f][1]] for f in fields])
+    weights = None
+    if mean:
+        weights = torch.cat([1.0 / torch.bincount(parts[f][1], minlength=BATCH)[parts[f][1]].double() for f in fields])
+    want, absolute, count = ref.table_gradient(g, ids, rows, padding=padding, weights=weights)
+    ref.assert_within(got, want, ref.gradient_bound(want, absolute, count, got.dtype, mean))
+
+
+@pytest.mark.parametrize("detached", [(0,), (1,), (0, 2), (1, 2)])
+def test_a_table_and_its_detached_alias(pkg, dev, detached):
+    """The gradient is cut off where the table is detached, in any order of the fields."""
+    fields = 3
+    values, offsets, parts = make_fields(fields)
+    grad = randn(1, BATCH, fields * DIM)
+    w = randn(2, ROWS, DIM).to(dev).requires_grad_()
+    tables = [w.detach() if f in detached else w for f in range(fields)]
+    pkg.embedding_bag_train(values.to(dev), offsets.to(dev), tables).backward(grad.to(dev))
+    assert w.grad is not None
+    assert_gradient(w.grad, parts, grad, [f for f in range(fields) if f not in detached])
+
+
+def test_two_leaves_over_one_memory(pkg, dev):
+    values, offsets, parts = make_fields(4)
+    grad = randn(1, BATCH, 4 * DIM)
+    a = randn(2, ROWS, DIM).to(dev).requires_grad_()
+    b = a.detach().requires_grad_()
+    pkg.embedding_bag_train(values.to(dev), offsets.to(dev), [a, b, b, a]).backward(grad.to(dev))
+    assert_gradient(a.grad, parts, grad, [0, 3])
+    assert_gradient(b.grad, parts, grad, [1, 2])
+
+
+def test_views_of_one_table_add_up(pkg, dev):
+    """A table and a view of it that autograd knows: both fields' gradients arrive at the leaf."""
+    values, offsets, parts = make_fields(3)
+    grad = randn(1, BATCH, 3 * DIM)
+    w = randn(2, ROWS, DIM).to(dev).requires_grad_()
+    pkg.embedding_bag_train(values.to(dev), offsets.to(dev), [w, w.view_as(w), w]).backward(grad.to(dev))
+    want, absolute, count = ref.table_gradient(torch.cat([grad[:, f * DIM:(f + 1) * DIM][parts[f][1]] for f in range(3)]),
+                                               torch.cat([p[0] for p in parts]), ROWS)
+    # two sums, each rounded, and their sum: two roundings more
+    ref.assert_within(w.grad, want, ref.gradient_bound(want, absolute, count + 2, torch.float32))
+
+
+def test_a_shared_table_has_one_gradient(pkg, dev):
+    values, offsets, parts = make_fields(4)
+    grad = randn(1, BATCH, 4 * DIM)
+    a, b = (randn(s, ROWS, DIM).to(dev).requires_grad_() for s in (2, 3))
+    pkg.embedding_bag_train(values.to(dev), offsets.to(dev), [a, b, a, b], "mean", padding_idx=1).backward(grad.to(dev))
+    assert_gradient(a.grad, parts, grad, [0, 2], padding=1, mean=True)
+    assert_gradient(b.grad, parts, grad, [1, 3], padding=1, mean=True)

@@ -1,0 +1,68 @@
+"""The differentiable pooling's way through autograd without a GPU: its two launches replaced by loops."""
+import importlib
+
+import pytest
+import torch
+
+BATCH, ROWS, DIM = 5, 7, 4
+
+
+@pytest.fixture
+def loops(pkg, monkeypatch):
+    """The training module with bags pooled, and their gradients summed, by loops on the CPU."""
+    module = importlib.import_module(pkg.__name__ + ".training")
+
+    def pooled(values, offsets, tables, pooling="sum", out_dtype=None):
+        fields = len(tables)
+        batch = (offsets.numel() - 1) // fields
+        return torch.cat([torch.stack([tables[f][values[offsets[f * batch + b]:offsets[f * batch + b + 1]]].sum(0) for b in range(batch)])
+                          for f in range(fields)], 1)
+
+    def gradients(index, grad, values, offsets, shapes, alike, dtype, same, *rest, **kw):
+        batch, col, sums = grad.shape[0], 0, {}
+        for f, (rows, dim) in enumerate(shapes):
+            out = sums.setdefault(same[f] if same is not None else f, torch.zeros(rows, dim, dtype=dtype))
+            for b in range(batch):
+                for i in values[offsets[f * batch + b]:offsets[f * batch + b + 1]]:
+                    out[i] += grad[b, col:col + dim]
+            col += dim
+        return [sums[same[f] if same is not None else f] for f in range(len(shapes))]
+
+    monkeypatch.setattr(module, "embedding_bag_pooled", pooled)
+    monkeypatch.setattr(module, "_bag_gradients", gradients)
+    return module
+
+
+def make_fields(fields):
+    gen = torch.Generator().manual_seed(fields)
+    lens = torch.randint(0, 4, (fields * BATCH,), generator=gen)
+    return torch.randint(0, ROWS, (int(lens.sum()),), generator=gen), torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)])
+
+
+def wanted(values, offsets, grad, fields):
+    out = torch.zeros(ROWS, DIM)
+    for f in fields:
+        for b in range(BATCH):
+            for i in values[offsets[f * BATCH + b]:offsets[f * BATCH + b + 1]]:
+                out[i] += grad[b, f * DIM:(f + 1) * DIM]
+    return out
+
+
+@pytest.mark.parametrize("detached", [(0,), (1,), (0, 2), (1, 2)])
+def test_a_detached_alias_adds_nothing(loops, detached):
+    values, offsets = make_fields(3)
+    w = torch.randn(ROWS, DIM, requires_grad=True)
+    out = loops.embedding_bag_train(values, offsets, [w.detach() if f in detached else w for f in range(3)])
+    grad = torch.arange(out.numel(), dtype=torch.float32).view_as(out)  # whole numbers: sums are exact in any order
+    out.backward(grad)
+    assert torch.equal(w.grad, wanted(values, offsets, grad, [f for f in range(3) if f not in detached]))
+
+
+def test_leaves_over_one_memory_and_shared_tensors(loops):
+    values, offsets = make_fields(4)
+    a = torch.randn(ROWS, DIM, requires_grad=True)
+    b = a.detach().requires_grad_()
+    out = loops.embedding_bag_train(values, offsets, [a, b, b, a])
+    grad = torch.arange(out.numel(), dtype=torch.float32).view_as(out)
+    out.backward(grad)
+    assert torch.equal(a.grad, wanted(values, offsets, grad, [0, 3])) and torch.equal(b.grad, wanted(values, offsets, grad, [1, 2]))
