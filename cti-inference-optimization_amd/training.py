@@ -430,18 +430,17 @@ def _plain_tables(tables, index: int):
 class _PooledTables(torch.autograd.Function):
     @staticmethod
     def forward(ctx, values, offsets, pooling, padding_idx, out_dtype, same, *tables):
-        ctx.save_for_backward(values, offsets, *tables)
-        ctx.info = (pooling, padding_idx, same)
+        ctx.save_for_backward(values, offsets)  # of the tables, only what the gradient needs to know: they may change until then
+        ctx.info = (pooling, padding_idx, same, [t.shape for t in tables], tables[0].dtype)
         return embedding_bag_pooled(values, offsets, tables, pooling, out_dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        values, offsets, *tables = ctx.saved_tensors
-        pooling, padding_idx, same = ctx.info
-        shapes = [t.shape for t in tables]
-        grads = _bag_gradients(grad.get_device(), grad.contiguous(), values, offsets, shapes, len(set(shapes)) == 1, tables[0].dtype,
-                               same, pooling, padding_idx)
+        values, offsets = ctx.saved_tensors
+        pooling, padding_idx, same, shapes, dtype = ctx.info
+        grads = _bag_gradients(grad.get_device(), grad.contiguous(), values, offsets, shapes, len(set(shapes)) == 1, dtype, same,
+                               pooling, padding_idx)
         # autograd adds up the fields' gradients of one table: its sum is in the first
         return (None, None, None, None, None, None, *(g if same[f] == f else None for f, g in enumerate(grads)))
 

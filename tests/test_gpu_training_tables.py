@@ -78,3 +78,17 @@ def test_a_shared_table_has_one_gradient(pkg, dev):
     pkg.embedding_bag_train(values.to(dev), offsets.to(dev), [a, b, a, b], "mean", padding_idx=1).backward(grad.to(dev))
     assert_gradient(a.grad, parts, grad, [0, 2], padding=1, mean=True)
     assert_gradient(b.grad, parts, grad, [1, 3], padding=1, mean=True)
+
+
+def test_tables_may_change_before_the_backward_pass(pkg, dev):
+    """As with the other differentiable operators: the gradient reads no table."""
+    values, offsets, parts = make_fields(2)
+    grad = randn(1, BATCH, 2 * DIM)
+    tables = [randn(s, ROWS, DIM).to(dev).requires_grad_() for s in (2, 3)]
+    out = pkg.embedding_bag_train(values.to(dev), offsets.to(dev), tables)
+    with torch.no_grad():
+        for t in tables:
+            t.add_(1.0)
+    out.backward(grad.to(dev))
+    for f, t in enumerate(tables):
+        assert_gradient(t.grad, parts, grad, [f])

@@ -66,3 +66,16 @@ def test_leaves_over_one_memory_and_shared_tensors(loops):
     grad = torch.arange(out.numel(), dtype=torch.float32).view_as(out)
     out.backward(grad)
     assert torch.equal(a.grad, wanted(values, offsets, grad, [0, 3])) and torch.equal(b.grad, wanted(values, offsets, grad, [1, 2]))
+
+
+def test_tables_may_change_before_the_backward_pass(loops):
+    """The gradient reads no table: an optimizer's step in between is no fault."""
+    values, offsets = make_fields(2)
+    a, b = (torch.randn(ROWS, DIM, requires_grad=True) for _ in range(2))
+    out = loops.embedding_bag_train(values, offsets, [a, b])
+    with torch.no_grad():
+        a.add_(1.0)
+        b.zero_()
+    grad = torch.arange(out.numel(), dtype=torch.float32).view_as(out)
+    out.backward(grad)
+    assert torch.equal(a.grad, wanted(values, offsets, grad, [0])) and torch.equal(b.grad, wanted(values, offsets, grad, [1]))
