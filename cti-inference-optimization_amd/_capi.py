@@ -168,6 +168,11 @@ SIGNATURES = {
         ctypes.c_int,
         [_P, _I32, _I64, _P, _I32, _I64, _P, _I64, _I32, ctypes.POINTER(Table), _I32, _I64, _I32, _P, _P, _P, _I64, _P, _I64, _P],
     ),
+    "cti_ebag_backward_fields": (
+        ctypes.c_int,
+        [_P, _I32, _I64, _P, _I32, _I64, _P, _I64, _I32, ctypes.POINTER(Table), ctypes.c_uint64, _I32, _I64, _I32, _P, _P, _P, _I64, _P,
+         _I64, _P],
+    ),
     "cti_ebag_backward_workspace_bytes": (ctypes.c_int64, [_I64, _I64, _I64, _I32, _I32]),
     "cti_ebag_dropout": (
         ctypes.c_int,

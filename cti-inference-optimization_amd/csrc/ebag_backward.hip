@@ -1519,7 +1519,7 @@ int run_gradient(GradCall& c, hipStream_t s) {
     fill_table(reinterpret_cast<char*>(c.sum.rows_out), c.capacity, 8, 8);
   } else if (c.per_field) {
     for (int f = 0; f < c.src.fields; ++f)
-      fill_table(c.fields.data[f], c.src.rows[f], static_cast<int64_t>(c.fields.dim[f]) * eb, c.fields.stride[f] * eb);
+      if (c.fields.data[f]) fill_table(c.fields.data[f], c.src.rows[f], static_cast<int64_t>(c.fields.dim[f]) * eb, c.fields.stride[f] * eb);
   } else {
     fill_table(c.sum.out, c.src.rows[0], static_cast<int64_t>(c.sum.dim) * eb, static_cast<int64_t>(c.sum.dim) * eb);
   }
@@ -1782,11 +1782,11 @@ extern "C" int cti_ebag_fused_all_slots_backward(const void* grad, int32_t grad_
   return rc != CTI_EBAG_OK ? rc : run_gradient(c, static_cast<hipStream_t>(stream));
 }
 
-extern "C" int cti_ebag_backward(const void* grad, int32_t grad_dtype, int64_t grad_row_stride, const void* values,
-                                 int32_t index_type, int64_t nnz, const int64_t* offsets, int64_t batch_size, int32_t num_fields,
-                                 const cti_ebag_table* tables, int32_t pooling, int64_t padding_idx, int32_t out_dtype, void* out,
-                                 int64_t* rows_out, int64_t* count_out, int64_t capacity, void* workspace, int64_t workspace_bytes,
-                                 void* stream) {
+extern "C" int cti_ebag_backward_fields(const void* grad, int32_t grad_dtype, int64_t grad_row_stride, const void* values,
+                                        int32_t index_type, int64_t nnz, const int64_t* offsets, int64_t batch_size,
+                                        int32_t num_fields, const cti_ebag_table* tables, uint64_t wanted, int32_t pooling,
+                                        int64_t padding_idx, int32_t out_dtype, void* out, int64_t* rows_out, int64_t* count_out,
+                                        int64_t capacity, void* workspace, int64_t workspace_bytes, void* stream) {
   clear_error();
   if (batch_size < 0) return set_error(CTI_EBAG_EINVAL, "batch_size must be >= 0 (got %lld)", (long long)batch_size);
   if (num_fields < 1) return set_error(CTI_EBAG_EINVAL, "num_fields must be >= 1 (got %d)", num_fields);
@@ -1794,26 +1794,35 @@ extern "C" int cti_ebag_backward(const void* grad, int32_t grad_dtype, int64_t g
   if (!tables) return set_error(CTI_EBAG_EINVAL, "tables is NULL");
   if (pooling != CTI_EBAG_SUM && pooling != CTI_EBAG_MEAN) return set_error(CTI_EBAG_EINVAL, "unknown pooling mode %d", pooling);
   if (batch_size > kGradMostIds) return set_error(CTI_EBAG_EUNSUPPORTED, "batch_size %lld (2^30 at most)", (long long)batch_size);
+  if (num_fields < kMaxFields) wanted &= (uint64_t{1} << num_fields) - 1;
+  if (!wanted) return set_error(CTI_EBAG_EINVAL, "no field has a gradient");
   const bool compact = rows_out != nullptr;
+  const int first_wanted = __builtin_ctzll(wanted);
   GradCall c;
   c.per_field = true;
   int64_t rows = 0, dim = 0;
   for (int f = 0; f < num_fields; ++f) {
     const cti_ebag_table& t = tables[f];
-    if (t.rows < 1) return set_error(CTI_EBAG_EINVAL, "tables[%d].rows must be >= 1 (got %lld)", f, (long long)t.rows);
+    const bool with = (wanted >> f) & 1;
+    if (with && t.rows < 1) return set_error(CTI_EBAG_EINVAL, "tables[%d].rows must be >= 1 (got %lld)", f, (long long)t.rows);
     if (t.dim < 1) return set_error(CTI_EBAG_EINVAL, "tables[%d].dim must be >= 1 (got %d)", f, t.dim);
-    if (t.row_stride < t.dim) return set_error(CTI_EBAG_EINVAL, "tables[%d].row_stride %lld < dim %d", f, (long long)t.row_stride, t.dim);
+    if (with && t.row_stride < t.dim)
+      return set_error(CTI_EBAG_EINVAL, "tables[%d].row_stride %lld < dim %d", f, (long long)t.row_stride, t.dim);
     if (t.out_col < 0 || t.out_col + static_cast<int64_t>(t.dim) > grad_row_stride)
       return set_error(CTI_EBAG_EINVAL, "tables[%d]: columns [%d, %lld) outside the gradient's row of %lld", f, t.out_col,
                        (long long)t.out_col + t.dim, (long long)grad_row_stride);
+    c.even = c.even && t.dim == tables[0].dim && t.out_col == static_cast<int64_t>(f) * t.dim;
+    c.fields.dim[f] = t.dim;
+    c.fields.col[f] = t.out_col;
+    if (!with) continue;
     if (!t.data) return set_error(CTI_EBAG_EINVAL, "tables[%d].data is NULL", f);
-    if (compact && t.dim != tables[0].dim)
-      return set_error(CTI_EBAG_EUNSUPPORTED, "rows_out needs tables of one width (%d, %d)", tables[0].dim, t.dim);
+    if (compact && t.dim != tables[first_wanted].dim)
+      return set_error(CTI_EBAG_EUNSUPPORTED, "rows_out needs tables of one width (%d, %d)", tables[first_wanted].dim, t.dim);
     if (padding_idx < -1 || padding_idx >= t.rows)
       return set_error(CTI_EBAG_EINVAL, "padding_idx %lld outside tables[%d]", (long long)padding_idx, f);
     int same = f;
-    for (int k = 0; k < f && same == f; ++k)
-      if (tables[k].data == t.data) same = k;
+    for (int k = first_wanted; k < f && same == f; ++k)
+      if (((wanted >> k) & 1) && tables[k].data == t.data) same = k;
     if (same < f && (tables[same].rows != t.rows || tables[same].dim != t.dim || tables[same].row_stride != t.row_stride))
       return set_error(CTI_EBAG_EINVAL, "tables[%d] and tables[%d] share data but not their shape", same, f);
     c.src.base[f] = same < f ? c.src.base[same] : static_cast<uint32_t>(rows);
@@ -1826,10 +1835,13 @@ extern "C" int cti_ebag_backward(const void* grad, int32_t grad_dtype, int64_t g
     c.fields.data[f] = static_cast<char*>(const_cast<void*>(t.data));
     c.fields.stride[f] = t.row_stride;
     c.fields.base[f] = c.src.base[f];
-    c.fields.dim[f] = t.dim;
-    c.fields.col[f] = t.out_col;
     if (t.dim > dim) dim = t.dim;
-    c.even = c.even && t.dim == tables[0].dim && t.out_col == static_cast<int64_t>(f) * t.dim;
+  }
+  // Fields without a gradient: a table of one row, whose number is the dropped ids' key.
+  for (int f = 0; f < num_fields; ++f) {
+    if ((wanted >> f) & 1) continue;
+    c.src.base[f] = static_cast<uint32_t>(rows);
+    c.src.rows[f] = 1;
   }
   c.even = c.even && grad_row_stride == num_fields * dim;
   const int64_t bags = batch_size * num_fields;
@@ -1864,4 +1876,14 @@ extern "C" int cti_ebag_backward(const void* grad, int32_t grad_dtype, int64_t g
   c.workspace_bytes = workspace_bytes;
   rc = check_workspace(c, pooling == CTI_EBAG_MEAN ? bags : 0, dim);
   return rc != CTI_EBAG_OK ? rc : run_gradient(c, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int cti_ebag_backward(const void* grad, int32_t grad_dtype, int64_t grad_row_stride, const void* values,
+                                 int32_t index_type, int64_t nnz, const int64_t* offsets, int64_t batch_size, int32_t num_fields,
+                                 const cti_ebag_table* tables, int32_t pooling, int64_t padding_idx, int32_t out_dtype, void* out,
+                                 int64_t* rows_out, int64_t* count_out, int64_t capacity, void* workspace, int64_t workspace_bytes,
+                                 void* stream) {
+  return cti_ebag_backward_fields(grad, grad_dtype, grad_row_stride, values, index_type, nnz, offsets, batch_size, num_fields, tables,
+                                  ~uint64_t{0}, pooling, padding_idx, out_dtype, out, rows_out, count_out, capacity, workspace,
+                                  workspace_bytes, stream);
 }

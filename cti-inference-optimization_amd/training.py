@@ -333,9 +333,10 @@ def embedding_bag_backward(
 
 
 def _bag_gradients(index, grad, values, offsets, shapes, alike, dtype, same, pooling, padding_idx, grad_dtype=None, compact=False,
-                   out=None):
+                   out=None, wanted=None):
     """``embedding_bag_backward`` of tables of these shapes (``alike``: all the same) and this type; ``same[f]``: the first field with
-    field f's table (None: no field shares one)."""
+    field f's table (None: no field shares one); ``wanted[f]``: whether its table has a gradient (None: every field's; the whole
+    form alone, which gives None for the others)."""
     dev = grad.device
     fields = len(shapes)
     width = fields * shapes[0][1] if alike else sum(shape[1] for shape in shapes)
@@ -351,12 +352,13 @@ def _bag_gradients(index, grad, values, offsets, shapes, alike, dtype, same, poo
     if width >= 2 ** 31:
         raise _capi.EbagError(_capi.EUNSUPPORTED, f"{width} columns >= 2^31")
     pool = _capi.pooling_code(pooling)
+    with_grad = shapes if wanted is None else [shape for f, shape in enumerate(shapes) if wanted[f]]
     if same is None:
-        same, rows = range(fields), sum(shape[0] for shape in shapes)
+        same, rows = range(fields), sum(shape[0] for shape in with_grad)
     else:
-        rows = sum(shapes[f][0] for f in set(same))
-    padding = _check_padding(padding_idx, shapes[0][0] if alike else min(shape[0] for shape in shapes))
-    dim = shapes[0][1] if alike else max(shape[1] for shape in shapes)
+        rows = sum(shapes[f][0] for f in set(same) if wanted is None or wanted[f])
+    padding = _check_padding(padding_idx, shapes[0][0] if alike else min(shape[0] for shape in with_grad))
+    dim = shapes[0][1] if alike else max(shape[1] for shape in with_grad)
     odt = grad_dtype or dtype
     n = values.numel()
     numbers = sums = count = grads = None
@@ -372,9 +374,9 @@ def _bag_gradients(index, grad, values, offsets, shapes, alike, dtype, same, poo
             size = shapes[0][0] * dim * whole.element_size()
             pointers = range(whole.data_ptr(), whole.data_ptr() + fields * size, size)
         else:
-            made = {f: torch.empty(shapes[f], dtype=odt, device=dev) for f in set(same)}
+            made = {f: torch.empty(shapes[f], dtype=odt, device=dev) if wanted is None or wanted[f] else None for f in set(same)}
             grads = [made[f] for f in same]
-            pointers = [g.data_ptr() for g in grads]
+            pointers = [0 if g is None else g.data_ptr() for g in grads]
     else:
         grads = list(out)
         if len(grads) != fields:
@@ -396,9 +398,10 @@ def _bag_gradients(index, grad, values, offsets, shapes, alike, dtype, same, poo
         descs[4::6] = itertools.accumulate(dims[:-1], initial=0)
     packed = struct.pack("QqqiiQ" * fields, *descs)
     ws, ws_ptr, ws_bytes = _workspace(n, batch * fields, rows, dim, pool, dev)
-    _launch(index, _capi.lib().cti_ebag_backward, grad.data_ptr(), _capi.dtype_code(grad.dtype), width, values.data_ptr(),
+    mask = 2 ** 64 - 1 if wanted is None else sum(1 << f for f in range(fields) if wanted[f])
+    _launch(index, _capi.lib().cti_ebag_backward_fields, grad.data_ptr(), _capi.dtype_code(grad.dtype), width, values.data_ptr(),
             _capi.index_code(values.dtype), n, offsets.data_ptr(), batch, fields,
-            ctypes.cast(ctypes.c_char_p(packed), ctypes.POINTER(_capi.Table)), pool, padding,
+            ctypes.cast(ctypes.c_char_p(packed), ctypes.POINTER(_capi.Table)), mask, pool, padding,
             _capi.dtype_code(sums.dtype if compact else odt), sums.data_ptr() if compact else None,
             numbers.data_ptr() if compact else None, count.data_ptr() if compact else None, capacity, ws_ptr, ws_bytes)
     return (numbers, sums, count) if compact else grads
@@ -439,8 +442,9 @@ class _PooledTables(torch.autograd.Function):
     def backward(ctx, grad):
         values, offsets = ctx.saved_tensors
         pooling, padding_idx, same, shapes, dtype = ctx.info
+        wanted = ctx.needs_input_grad[6:]
         grads = _bag_gradients(grad.get_device(), grad.contiguous(), values, offsets, shapes, len(set(shapes)) == 1, dtype, same,
-                               pooling, padding_idx)
+                               pooling, padding_idx, wanted=None if all(wanted) else wanted)
         # autograd adds up the fields' gradients of one table: its sum is in the first
         return (None, None, None, None, None, None, *(g if same[f] == f else None for f, g in enumerate(grads)))
 
@@ -455,7 +459,7 @@ def embedding_bag_train(
 ) -> torch.Tensor:
     """``embedding_bag_pooled`` of float tables, differentiable in them (``embedding_bag_backward``). Fields share a table where they
     are given the same tensor. Tensors that only share memory, a table and what ``detach()`` makes of it among them, are tables of
-    their own, as autograd sees them.
+    their own, as autograd sees them. Tables that require no gradient take no memory and no sums in the backward pass.
     """
     for t in tables:
         if not isinstance(t, torch.Tensor):

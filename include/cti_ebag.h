@@ -597,6 +597,17 @@ int cti_ebag_backward(const void* grad, int32_t grad_dtype, int64_t grad_row_str
                       int32_t pooling, int64_t padding_idx, int32_t out_dtype, void* out, int64_t* rows_out, int64_t* count_out,
                       int64_t capacity, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * The same for some of the fields: bit f of `wanted` says whether field f's table has a gradient (bits from num_fields on count
+ * for nothing; one field at least). Of a field without one only dim and out_col are read, and its ids count for none. Tables,
+ * rows and the widest dim above are then those of the fields that have one.
+ */
+int cti_ebag_backward_fields(const void* grad, int32_t grad_dtype, int64_t grad_row_stride, const void* values, int32_t index_type,
+                             int64_t nnz, const int64_t* offsets, int64_t batch_size, int32_t num_fields,
+                             const cti_ebag_table* tables, uint64_t wanted, int32_t pooling, int64_t padding_idx, int32_t out_dtype,
+                             void* out, int64_t* rows_out, int64_t* count_out, int64_t capacity, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
 /* Bytes of workspace that the gradient of `nnz` ids in `bags` bags needs (0 for no ids and for arguments out of range). */
 int64_t cti_ebag_backward_workspace_bytes(int64_t nnz, int64_t bags, int64_t rows, int32_t dim, int32_t pooling);
 

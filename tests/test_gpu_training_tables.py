@@ -92,3 +92,43 @@ def test_tables_may_change_before_the_backward_pass(pkg, dev):
     out.backward(grad.to(dev))
     for f, t in enumerate(tables):
         assert_gradient(t.grad, parts, grad, [f])
+
+
+@pytest.mark.parametrize("dims", [(24, 24, 24, 24), (128, 128, 128, 128), (7, 64, 300, 1)])
+@pytest.mark.parametrize("frozen", [(0,), (3,), (1, 2), (0, 2, 3)])
+@pytest.mark.parametrize("padding", [None, 0, 5])
+@pytest.mark.parametrize("max_len", [6, 200])  # ids of one tile, and of several
+def test_frozen_tables_take_no_part(pkg, dev, dims, frozen, padding, max_len):
+    gen = torch.Generator().manual_seed(max_len)
+    rows, fields = (40, 9, 17, 30), len(dims)
+    lens = torch.randint(0, max_len + 1, (fields, BATCH), generator=gen)
+    values = torch.randint(-1, 41, (int(lens.sum()),), generator=gen)
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), lens.reshape(-1).cumsum(0)])
+    grad = randn(1, BATCH, sum(dims))
+    tables = [randn(f, rows[f], dims[f]).to(dev).requires_grad_(f not in frozen) for f in range(fields)]
+    pkg.embedding_bag_train(values.to(dev), offsets.to(dev), tables, "mean", padding_idx=padding).backward(grad.to(dev))
+    for f, t in enumerate(tables):
+        if f in frozen:
+            assert t.grad is None
+            continue
+        ids = values[offsets[f * BATCH]:offsets[(f + 1) * BATCH]].clamp(0, rows[f] - 1)
+        sample = torch.repeat_interleave(torch.arange(BATCH), lens[f])
+        col = sum(dims[:f])
+        want, absolute, count = ref.table_gradient(grad[:, col:col + dims[f]][sample], ids, rows[f], padding=padding,
+                                                   weights=1.0 / lens[f][sample].double())
+        ref.assert_within(t.grad, want, ref.gradient_bound(want, absolute, count, torch.float32, True), f"field {f}")
+
+
+def test_frozen_tables_take_no_memory(pkg, dev):
+    values, offsets, parts = make_fields(2)
+    big = torch.zeros(2 ** 20, DIM, device=dev)  # 96 MiB
+    w = randn(2, ROWS, DIM).to(dev).requires_grad_()
+    grad = randn(1, BATCH, 2 * DIM)
+    out = pkg.embedding_bag_train(values.to(dev), offsets.to(dev), [big, w])
+    grad_dev = grad.to(dev)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out.backward(grad_dev)
+    assert torch.cuda.max_memory_allocated() - before < 2 ** 24
+    assert_gradient(w.grad, parts, grad, [1])

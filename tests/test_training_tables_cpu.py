@@ -18,7 +18,8 @@ def loops(pkg, monkeypatch):
         return torch.cat([torch.stack([tables[f][values[offsets[f * batch + b]:offsets[f * batch + b + 1]]].sum(0) for b in range(batch)])
                           for f in range(fields)], 1)
 
-    def gradients(index, grad, values, offsets, shapes, alike, dtype, same, *rest, **kw):
+    def gradients(index, grad, values, offsets, shapes, alike, dtype, same, *rest, wanted=None, **kw):
+        module.asked.append(wanted)
         batch, col, sums = grad.shape[0], 0, {}
         for f, (rows, dim) in enumerate(shapes):
             out = sums.setdefault(same[f] if same is not None else f, torch.zeros(rows, dim, dtype=dtype))
@@ -26,8 +27,9 @@ def loops(pkg, monkeypatch):
                 for i in values[offsets[f * batch + b]:offsets[f * batch + b + 1]]:
                     out[i] += grad[b, col:col + dim]
             col += dim
-        return [sums[same[f] if same is not None else f] for f in range(len(shapes))]
+        return [sums[same[f] if same is not None else f] if wanted is None or wanted[f] else None for f in range(len(shapes))]
 
+    monkeypatch.setattr(module, "asked", [], raising=False)
     monkeypatch.setattr(module, "embedding_bag_pooled", pooled)
     monkeypatch.setattr(module, "_bag_gradients", gradients)
     return module
@@ -79,3 +81,51 @@ def test_tables_may_change_before_the_backward_pass(loops):
     grad = torch.arange(out.numel(), dtype=torch.float32).view_as(out)
     out.backward(grad)
     assert torch.equal(a.grad, wanted(values, offsets, grad, [0])) and torch.equal(b.grad, wanted(values, offsets, grad, [1]))
+
+
+def test_only_tables_that_require_a_gradient_get_one(loops):
+    values, offsets = make_fields(4)
+    a, b, frozen = torch.randn(ROWS, DIM, requires_grad=True), torch.randn(ROWS, DIM, requires_grad=True), torch.randn(ROWS, DIM)
+    out = loops.embedding_bag_train(values, offsets, [frozen, a, frozen, b])
+    grad = torch.arange(out.numel(), dtype=torch.float32).view_as(out)
+    out.backward(grad)
+    assert [tuple(w) for w in loops.asked] == [(False, True, False, True)] and frozen.grad is None
+    assert torch.equal(a.grad, wanted(values, offsets, grad, [1])) and torch.equal(b.grad, wanted(values, offsets, grad, [3]))
+    out = loops.embedding_bag_train(values, offsets, [a, b, a, b])
+    out.backward(grad)
+    assert loops.asked[1] is None
+
+
+def test_gradient_of_some_fields_refuses(pkg):
+    """The C ABI; addresses are numbers that nothing reads. Of a field without a gradient only its columns are looked at."""
+    c, lib = pkg._capi, pkg.load_library()
+
+    def call(wanted, second=None, **kw):
+        descs = (c.Table * 2)()
+        rest = dict(data=8192, rows=20, row_stride=8, dim=8, out_col=8)
+        for d, t in zip(descs, (dict(data=4096, rows=10, row_stride=8, dim=8, out_col=0), {**rest, **(second or {})})):
+            for k, v in t.items():
+                setattr(d, k, v)
+        a = dict(grad=64, gdt=c.F32, stride=16, v=64, it=c.I64, nnz=4, offs=64, batch=2, fields=2, tables=descs, wanted=wanted, pool=c.SUM,
+                 pad=-1, odt=c.F32, out=None, rows_out=None, count=None, cap=0, ws=None, ws_bytes=0)
+        a.update(kw)
+        status = lib.cti_ebag_backward_fields(*a.values(), None)
+        return status, c.last_error()
+
+    for mask in (0, 4, 2 ** 64 - 4):
+        status, error = call(mask)
+        assert status == c.EINVAL and "no field" in error
+    for second in (dict(data=None), dict(rows=0), dict(row_stride=0), dict(data=4096), dict(rows=2 ** 31)):
+        assert call(3, second)[0] in (c.EINVAL, c.EUNSUPPORTED), second
+        status, error = call(1, second)  # as far as the workspace, which is checked last
+        assert status == c.EWORKSPACE and "needed" in error, second
+    for second in (dict(dim=0), dict(out_col=9), dict(out_col=-1)):
+        assert call(1, second)[0] == c.EINVAL, second
+    status, error = call(2, pad=10)  # the first table's rows do not count
+    assert status == c.EWORKSPACE, error
+    status, error = call(1, pad=10)
+    assert status == c.EINVAL and "padding" in error
+    # one width is asked of the tables that have a gradient
+    compact = dict(rows_out=64, count=64, cap=4, out=64)
+    assert call(3, dict(dim=4, row_stride=4), **compact)[0] == c.EUNSUPPORTED
+    assert call(1, dict(dim=4, row_stride=4), **compact)[0] == c.EWORKSPACE
