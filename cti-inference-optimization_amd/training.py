@@ -72,6 +72,16 @@ def _check_dim(dim: int) -> None:
         raise _capi.EbagError(_capi.EUNSUPPORTED, f"dim {dim} >= 2^31")
 
 
+_MOST_IDS, _MOST_ROWS, _MOST_COLUMNS, _MOST_FIELDS = 2 ** 30, 2 ** 31 - 2, 2 ** 22, 64  # of a gradient, as the library has them
+
+
+def _check_gradient(ids: int, bags: int, rows: int, dim: int) -> None:
+    """Refuse in the forward pass what its backward pass would."""
+    if ids > _MOST_IDS or bags > _MOST_IDS or rows > _MOST_ROWS or dim > _MOST_COLUMNS:
+        raise _capi.EbagError(_capi.EUNSUPPORTED, f"no gradient for {ids} ids in {bags} bags of {rows} rows of {dim} columns: at most 2^30 "
+                                                  "ids and bags, 2^31 - 2 rows of tables, 2^22 columns")
+
+
 # ------------------------------------------------------------------------------------------------
 # Lookup
 # ------------------------------------------------------------------------------------------------
@@ -148,7 +158,8 @@ def embedding_lookup(
     column stride. Ids outside the table are clamped, as everywhere in this package. Returns ``out`` of shape
     ``ids.shape + (dim,)``; ``out`` overlaps no input.
 
-    Differentiable in ``weight`` (``out`` must then be None): the gradient is ``embedding_lookup_backward``'s,
+    Differentiable in ``weight`` (``out`` must then be None, and the limits are the gradient's: 2^30 ids, 2^31 - 2 rows, 2^22
+    columns): the gradient is ``embedding_lookup_backward``'s,
     0 for row ``padding_idx``, which the lookup itself reads like any row. With ``sparse_grad`` it is a
     sparse tensor of the rows that occur, each once, whose making waits for their count (not within a captured graph).
     """
@@ -156,8 +167,9 @@ def embedding_lookup(
     if _grad_enabled() and isinstance(weight, torch.Tensor) and weight.requires_grad:
         if out is not None:
             raise ValueError("out does not combine with a gradient: detach the weight or leave out None")
-        if weight.dim() == 2:
+        if weight.dim() == 2 and isinstance(ids, torch.Tensor):
             _check_padding(padding_idx, weight.shape[0])
+            _check_gradient(ids.numel(), 0, *weight.shape)
         return _Lookup.apply(weight, ids, scale, padding_idx, out_dtype, sparse_grad)
     return _lookup(ids, weight, scale, out, out_dtype)
 
@@ -459,7 +471,8 @@ def embedding_bag_train(
 ) -> torch.Tensor:
     """``embedding_bag_pooled`` of float tables, differentiable in them (``embedding_bag_backward``). Fields share a table where they
     are given the same tensor. Tensors that only share memory, a table and what ``detach()`` makes of it among them, are tables of
-    their own, as autograd sees them. Tables that require no gradient take no memory and no sums in the backward pass.
+    their own, as autograd sees them. Tables that require no gradient take no memory and no sums in the backward pass. Where one
+    requires it there are at most 64 fields, 2^30 ids and bags, 2^31 - 2 rows of such tables and 2^22 columns of each.
     """
     for t in tables:
         if not isinstance(t, torch.Tensor):
@@ -467,6 +480,12 @@ def embedding_bag_train(
         _check_padding(padding_idx, t.shape[0])
     first = {}
     same = [first.setdefault(id(t), f) for f, t in enumerate(tables)]
+    trained = [t for f, t in enumerate(tables) if same[f] == f and t.requires_grad]
+    if trained and _grad_enabled():
+        if len(tables) > _MOST_FIELDS:
+            raise _capi.EbagError(_capi.EUNSUPPORTED, f"no gradient for {len(tables)} fields: at most {_MOST_FIELDS} in a call")
+        if isinstance(values, torch.Tensor) and isinstance(offsets, torch.Tensor):
+            _check_gradient(values.numel(), offsets.numel() - 1, sum(t.shape[0] for t in trained), max(t.shape[-1] for t in trained))
     return _PooledTables.apply(values, offsets, pooling, padding_idx, out_dtype, same, *tables)
 
 
@@ -497,14 +516,16 @@ def fused_embedding_train(
     sparse_grad: bool = False,
 ) -> torch.Tensor:
     """The fused step of a flat-layout batch, ``[B, S*D]`` as ``fused_all_slots_embedding`` pools it, differentiable in
-    the table (``fused_all_slots_embedding_backward``; ``padding_idx`` and ``sparse_grad`` as in
+    the table (``fused_all_slots_embedding_backward``; ``padding_idx``, ``sparse_grad`` and the limits, of bags too, as in
     ``embedding_lookup``)."""
     slots = val_offsets.numel()
     if slots < 1 or flat_row_offsets.numel() % slots:
         raise ValueError(f"flat_row_offsets has {flat_row_offsets.numel()} entries for {slots} slots")
     _check_padding(padding_idx, weight.shape[0])
-    return _PooledShared.apply(weight, flat_values, val_offsets, flat_row_offsets, flat_row_offsets.numel() // slots - 1, padding_idx,
-                               sparse_grad)
+    batch_size = flat_row_offsets.numel() // slots - 1
+    if _grad_enabled() and weight.requires_grad:
+        _check_gradient(flat_values.numel(), slots * batch_size, weight.shape[0], weight.shape[-1])
+    return _PooledShared.apply(weight, flat_values, val_offsets, flat_row_offsets, batch_size, padding_idx, sparse_grad)
 
 
 # ------------------------------------------------------------------------------------------------

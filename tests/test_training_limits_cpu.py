@@ -1,0 +1,84 @@
+"""What a gradient cannot do is refused where the differentiable call is made, not in the backward pass."""
+import importlib
+
+import pytest
+import torch
+
+
+@pytest.fixture
+def training(pkg):
+    return importlib.import_module(pkg.__name__ + ".training")
+
+
+def wide(rows, dim):
+    """A table of any shape that takes no memory."""
+    return torch.zeros(1).expand(rows, dim).requires_grad_()
+
+
+def test_limits_are_the_librarys(pkg, training):
+    """Each limit passes, and one more does not, in Python as in C (ids, rows, columns; n = 0 launches nothing that matters here: the
+    call ends at its NULL pointers or its workspace)."""
+    c, lib = pkg._capi, pkg.load_library()
+
+    def lookup(n, rows, dim):
+        return lib.cti_ebag_lookup_backward(64, c.F32, 64, c.I64, n, rows, dim, 1.0, -1, 64, c.F32, None, None, 0, None, 0, None)
+
+    ids, rows, dim = training._MOST_IDS, training._MOST_ROWS, training._MOST_COLUMNS
+    for sizes in ((ids, 10, 8), (4, rows, 8), (4, 10, dim)):
+        training._check_gradient(sizes[0], 0, *sizes[1:])
+        assert lookup(*sizes) == c.EWORKSPACE, sizes
+    for sizes in ((ids + 1, 10, 8), (4, rows + 1, 8), (4, 10, dim + 1)):
+        with pytest.raises(pkg.EbagError):
+            training._check_gradient(sizes[0], 0, *sizes[1:])
+        assert lookup(*sizes) == c.EUNSUPPORTED, sizes
+    with pytest.raises(pkg.EbagError):
+        training._check_gradient(4, ids + 1, 10, 8)
+
+    def fields(n):
+        descs = (c.Table * n)()
+        for f, d in enumerate(descs):
+            d.data, d.rows, d.row_stride, d.dim, d.out_col = 4096 * (f + 1), 10, 8, 8, 8 * f
+        return lib.cti_ebag_backward(64, c.F32, 8 * n, 64, c.I64, 4, 64, 2, n, descs, c.SUM, -1, c.F32, None, None, None, 0, None, 0, None)
+
+    assert fields(training._MOST_FIELDS) == c.EWORKSPACE and fields(training._MOST_FIELDS + 1) == c.EUNSUPPORTED
+
+
+def test_more_fields_than_a_gradient_has(pkg):
+    values, offsets = torch.zeros(65, dtype=torch.int64), torch.arange(66)
+    with pytest.raises(pkg.EbagError, match="65 fields"):
+        pkg.embedding_bag_train(values, offsets, [torch.zeros(5, 8, requires_grad=True)] * 65)
+    with pytest.raises(ValueError, match="GPU tensor"):  # without a gradient the limit is not there
+        pkg.embedding_bag_train(values, offsets, [torch.zeros(5, 8)] * 65)
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU tensor"):
+        pkg.embedding_bag_train(values, offsets, [torch.zeros(5, 8, requires_grad=True)] * 65)
+
+
+@pytest.mark.parametrize("rows,dim", [(2 ** 31 - 1, 4), (5, 2 ** 22 + 1)])
+def test_tables_past_the_limits(pkg, rows, dim):
+    ids, offsets = torch.zeros(4, dtype=torch.int64), torch.tensor([0, 2, 4])
+    for call in (lambda w: pkg.embedding_lookup(ids, w), lambda w: pkg.embedding_bag_train(ids, offsets, [w]),
+                 lambda w: pkg.fused_embedding_train(ids, offsets[:1], offsets, w)):
+        with pytest.raises(pkg.EbagError, match="no gradient"):
+            call(wide(rows, dim))
+    half = [wide(2 ** 30, 4), wide(2 ** 30, 4)]
+    with pytest.raises(pkg.EbagError, match="no gradient"):  # rows of all tables that have a gradient count
+        pkg.embedding_bag_train(ids, torch.arange(5), half)
+    with pytest.raises(ValueError, match="GPU tensor"):
+        pkg.embedding_bag_train(ids, torch.arange(5), [half[0], half[1].detach()])
+
+
+def test_ids_and_bags_past_the_limits(pkg):
+    def numbers(n):
+        return torch.zeros(1, dtype=torch.int64).expand(n)
+
+    few, w, most = numbers(4), torch.zeros(5, 8, requires_grad=True), 2 ** 30
+    for call in (lambda k: pkg.embedding_lookup(numbers(most + k), w),
+                 lambda k: pkg.embedding_bag_train(numbers(most + k), numbers(2), [w]),
+                 lambda k: pkg.embedding_bag_train(few, numbers(most + 1 + k), [w]),
+                 lambda k: pkg.fused_embedding_train(numbers(most + k), few[:1], few[:2], w),
+                 lambda k: pkg.fused_embedding_train(few, few[:1], numbers(most + 1 + k), w)):
+        with pytest.raises(pkg.EbagError, match="no gradient"):
+            call(1)
+    for call in (lambda: pkg.embedding_lookup(numbers(most), w), lambda: pkg.embedding_bag_train(few, numbers(most + 1), [w])):
+        with pytest.raises(ValueError, match="GPU tensor"):  # the limits themselves pass
+            call()
