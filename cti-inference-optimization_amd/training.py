@@ -8,7 +8,8 @@ gradients here are theirs. Each operator comes as plain calls, forward and backw
 loop or a captured graph makes itself (``embedding_lookup_backward``, ``embedding_bag_backward``,
 ``fused_all_slots_embedding_backward``, ``dropout_backward``, ``dropout_add_layer_norm_backward``), and
 ``embedding_lookup``, ``dropout``, ``dropout_add_layer_norm``, ``embedding_bag_train`` and
-``fused_embedding_train`` take part in autograd by themselves where an input requires a gradient.
+``fused_embedding_train`` take part in autograd by themselves where an input requires a gradient, in reverse
+mode and once; inputs with a tangent (forward mode) are refused.
 
 Gradients of tables come whole, or as the rows that occur (``compact``): ``rows`` (their numbers, ascending,
 then -1), their sums and how many they are, all on the device, so that nothing waits for the count. The ids
@@ -32,6 +33,7 @@ import struct
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi
@@ -50,6 +52,14 @@ def _any_requires_grad(*tensors) -> bool:
         if t is not None and t.requires_grad:
             return True
     return False
+
+
+def _refuse_tangents(*tensors) -> None:
+    """There is no forward mode, and a dual tensor has no requires_grad by which it would take autograd's way and be refused there."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # -1 outside of dual levels: unpack_dual takes as long as a small kernel
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("an input has a tangent: this operator is differentiated in reverse mode only")
 
 
 def _check_index(name: str, t: torch.Tensor, index: Optional[int] = None) -> int:
@@ -164,6 +174,7 @@ def embedding_lookup(
     sparse tensor of the rows that occur, each once, whose making waits for their count (not within a captured graph).
     """
     scale = float(scale)
+    _refuse_tangents(weight)
     if _grad_enabled() and isinstance(weight, torch.Tensor) and weight.requires_grad:
         if out is not None:
             raise ValueError("out does not combine with a gradient: detach the weight or leave out None")
@@ -478,6 +489,7 @@ def embedding_bag_train(
         if not isinstance(t, torch.Tensor):
             raise TypeError("tables must be tensors: int8 pairs have no gradient")
         _check_padding(padding_idx, t.shape[0])
+    _refuse_tangents(*tables)
     first = {}
     same = [first.setdefault(id(t), f) for f, t in enumerate(tables)]
     trained = [t for f, t in enumerate(tables) if same[f] == f and t.requires_grad]
@@ -522,6 +534,7 @@ def fused_embedding_train(
     if slots < 1 or flat_row_offsets.numel() % slots:
         raise ValueError(f"flat_row_offsets has {flat_row_offsets.numel()} entries for {slots} slots")
     _check_padding(padding_idx, weight.shape[0])
+    _refuse_tangents(weight)
     batch_size = flat_row_offsets.numel() // slots - 1
     if _grad_enabled() and weight.requires_grad:
         _check_gradient(flat_values.numel(), slots * batch_size, weight.shape[0], weight.shape[-1])
@@ -614,6 +627,7 @@ def dropout(
     ``seed`` is a number below 2^64, or an int64 tensor (seed, offset) on the device. ``out`` may be x or residual.
     Differentiable in ``x`` and ``residual`` (``out`` must then be None); the mask is made again for it, not stored.
     """
+    _refuse_tangents(x, residual)
     if _grad_enabled() and _any_requires_grad(x, residual):
         if out is not None:
             raise ValueError("out does not combine with a gradient: detach the inputs or leave out None")
@@ -705,6 +719,7 @@ def dropout_add_layer_norm(
     ``offset`` as in ``dropout``. Differentiable in x, residual, weight and bias, through y and h.
     """
     eps = float(eps)
+    _refuse_tangents(x, residual, weight, bias)
     if _grad_enabled() and _any_requires_grad(x, residual, weight, bias):
         y, mean, rstd, *h = _Norm.apply(x, residual, weight, bias, eps, p, seed, offset)
         return y, (h[0] if h else x), mean, rstd

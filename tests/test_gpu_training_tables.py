@@ -132,3 +132,17 @@ def test_frozen_tables_take_no_memory(pkg, dev):
     out.backward(grad_dev)
     assert torch.cuda.max_memory_allocated() - before < 2 ** 24
     assert_gradient(w.grad, parts, grad, [1])
+
+
+def test_tangents_are_refused(pkg, dev):
+    """Forward mode: no result without its tangent."""
+    w, x, one = randn(1, ROWS, DIM).to(dev), randn(2, 6, DIM).to(dev), torch.ones(DIM, device=dev)
+    ids = torch.arange(6, device=dev)
+    for call, t in ((lambda t: pkg.embedding_lookup(ids, t), w), (lambda t: pkg.dropout(t, 0.5, 1), x),
+                    (lambda t: pkg.dropout(x, 0.5, 1, residual=t), x), (lambda t: pkg.dropout_add_layer_norm(t, one, one), x),
+                    (lambda t: pkg.dropout_add_layer_norm(x, t, one), one),
+                    (lambda t: pkg.embedding_bag_train(ids, torch.tensor([0, 3, 6], device=dev), [t]), w)):
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(ValueError, match="tangent"):
+                call(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
+            call(t)

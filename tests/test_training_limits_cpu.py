@@ -82,3 +82,38 @@ def test_ids_and_bags_past_the_limits(pkg):
     for call in (lambda: pkg.embedding_lookup(numbers(most), w), lambda: pkg.embedding_bag_train(few, numbers(most + 1), [w])):
         with pytest.raises(ValueError, match="GPU tensor"):  # the limits themselves pass
             call()
+
+
+def operators(pkg):
+    """name, call of one tensor, that tensor's shape: every input through which an operator is differentiable."""
+    ids, offsets = torch.zeros(4, dtype=torch.int64), torch.tensor([0, 2, 4])
+    x, one = torch.ones(4, 8), torch.ones(8)
+    return [("lookup", lambda w: pkg.embedding_lookup(ids, w), (5, 8)), ("dropout", lambda t: pkg.dropout(t, 0.5, 1), (4, 8)),
+            ("dropout residual", lambda t: pkg.dropout(x, 0.5, 1, residual=t), (4, 8)),
+            ("norm", lambda t: pkg.dropout_add_layer_norm(t, one, one), (4, 8)),
+            ("norm residual", lambda t: pkg.dropout_add_layer_norm(x, one, one, residual=t), (4, 8)),
+            ("norm weight", lambda t: pkg.dropout_add_layer_norm(x, t, one), (8,)),
+            ("norm bias", lambda t: pkg.dropout_add_layer_norm(x, one, t), (8,)),
+            ("bags", lambda t: pkg.embedding_bag_train(ids, offsets, [t]), (5, 8)),
+            ("second table", lambda t: pkg.embedding_bag_train(ids, torch.arange(5), [torch.zeros(5, 8), t]), (5, 8)),
+            ("fused", lambda t: pkg.fused_embedding_train(ids, offsets[:1], offsets, t), (5, 8))]
+
+
+@pytest.mark.parametrize("which", range(10))
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused(pkg, which, grad):
+    """A dual tensor's tangent is not dropped without a word; outside of it the operator goes its way (here to its refusal of a
+    CPU tensor)."""
+    name, call, shape = operators(pkg)[which]
+    t = torch.ones(shape)
+    with torch.set_grad_enabled(grad):
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(t, torch.ones(shape))
+            with pytest.raises(ValueError, match="tangent"):
+                call(dual)
+            with pytest.raises(ValueError, match="GPU tensor"):
+                call(t)
+        with pytest.raises(ValueError, match="tangent"):
+            torch.func.jvp(call, (t,), (t,))
+        with pytest.raises(ValueError, match="GPU tensor"):
+            call(t)
