@@ -363,7 +363,7 @@ __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* s_scan) {
 }
 
 // Places of the tile's keys in the tile sorted by one digit (stable): place[k] of item k. s_hist: wavefronts << bits
-// numbers; s_start[d] is the first place of digit d. A thread holds digits 4 t to 4 t + 3; counts[4] of them are the tile's.
+// numbers, 16-byte aligned; s_start[d] is the first place of digit d. A thread holds digits 4 t to 4 t + 3; counts[4] of them are the tile's.
 template <int THREADS, int ITEMS>
 __device__ __forceinline__ void tile_places(const uint32_t* key, int shift, int bits, uint32_t* place, uint16_t* s_hist,
                                             uint32_t* s_start, uint32_t* s_scan) {
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(kRangeThreads) grad_sort_ranges_kernel(const G
   // (8 bits where two workgroups, of which the other fills, then fit a CU)
   constexpr int DIGIT_BITS = ITEMS == 32 ? 9 : 8, DIGITS = 1 << DIGIT_BITS;
   __shared__ uint32_t s_val[kRangeThreads * ITEMS];
-  __shared__ uint16_t s_hist[kRangeWaves * DIGITS];
+  __shared__ __align__(16) uint16_t s_hist[kRangeWaves * DIGITS];
   __shared__ uint32_t s_start[DIGITS], s_scan[kRangeWaves], s_count[2][kRangeWaves];
   const int t = static_cast<int>(threadIdx.x), w = t / kWave, n = static_cast<int>(s.n);
   const uint32_t range = blockIdx.x;
@@ -717,7 +717,7 @@ __global__ void __launch_bounds__(kSortThreads) grad_scatter_kernel(const Pair* 
                                                                     const GradFill fill) {
   if (fills(fill)) return;
   __shared__ Pair s_pair[kTile];
-  __shared__ uint16_t s_hist[kSortThreads / kWave * kGradDigits];
+  __shared__ __align__(16) uint16_t s_hist[kSortThreads / kWave * kGradDigits];
   __shared__ uint32_t s_start[kGradDigits], s_scan[kSortThreads / kWave];
   const int t = static_cast<int>(threadIdx.x), digits = 1 << bits;
   const int64_t tile = tile_of(blockIdx.x, fill.sort_groups), first = tile * kTile;
