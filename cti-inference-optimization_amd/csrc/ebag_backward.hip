@@ -284,7 +284,7 @@ __device__ __forceinline__ void tile_keys(const GradSource& s, int64_t tile, uin
 // ---------------------------------------------------------------------------------------------
 // What is written before the sums: zeros to whole tables, -1 to the compact form's numbers. It rides on the
 // sort's launches, whose few workgroups wait on latency: workgroups behind the sort's take shares of 64 KiB.
-constexpr int64_t kFillShare = 64 << 10;
+constexpr int64_t kFillShare = kGradFillShare;
 struct GradFill {
   char* data[kMaxFields];
   int64_t bytes[kMaxFields];       // rows * row_bytes
@@ -1523,7 +1523,7 @@ int run_gradient(GradCall& c, hipStream_t s) {
   } else {
     fill_table(c.sum.out, c.src.rows[0], static_cast<int64_t>(c.sum.dim) * eb, static_cast<int64_t>(c.sum.dim) * eb);
   }
-  if (shares > kGradMostShares) return set_error(CTI_EBAG_EUNSUPPORTED, "tables of more than 2^38 bytes");
+  if (shares > kGradMostShares) return set_error(CTI_EBAG_EUNSUPPORTED, "a gradient of more than 2^38 - 2^25 bytes");
   if (n == 0) {
     hipLaunchKernelGGL(grad_fill_kernel, dim3(static_cast<unsigned>(shares > 0 ? shares : 1)), dim3(kSortThreads), 0, s, fill,
                        c.sum.count_out);

@@ -28,7 +28,10 @@ constexpr int kGradTile = 4096;
 constexpr int64_t kGradMostIds = int64_t{1} << 30;        // ids and bags: 32-bit numbers, and launches below 2^32 threads
 constexpr int64_t kGradMostRows = (int64_t{1} << 31) - 1;  // rows of all tables are fewer: the number itself is a key
 constexpr int64_t kGradMostDim = int64_t{1} << 22;
-constexpr int64_t kGradMostShares = int64_t{1} << 22;     // of the fill: with the tiles, below 2^32 threads
+constexpr int64_t kGradFillShare = 64 << 10;  // bytes that a workgroup fills
+// Shares of the fill that one launch of the sort may take beside its own workgroups and stay below 2^32 threads: launches of 1,024
+// threads have 256 workgroups at most (one, a range of keys each, or 64 digits each), launches of 512 one for each tile.
+constexpr int64_t kGradMostShares = (int64_t{1} << 22) - 512;
 constexpr int kGradDigitBits = 11, kGradDigits = 1 << kGradDigitBits;
 constexpr int64_t kGradIdsAlone = 8192;    // in bags: ids that one workgroup finds and sorts
 constexpr int64_t kGradIdsRanged = 32768;  // ids that are sorted by ranges of keys

@@ -563,7 +563,7 @@ int cti_ebag_lookup(const void* ids, int32_t index_type, int64_t n, const void* 
  *            capacity >= min(n, rows)
  *   workspace  device scratch of at least cti_ebag_backward_workspace_bytes(n, n, rows, dim, CTI_EBAG_SUM)
  *            bytes, 16-byte aligned (CTI_EBAG_EWORKSPACE otherwise; none needed for n = 0)
- * n at most 2^30, rows at most 2^31 - 2, dim at most 2^22. No two arrays overlap.
+ * n at most 2^30, rows at most 2^31 - 2, dim at most 2^22, a whole gradient at most 2^38 - 2^25 bytes. No two arrays overlap.
  */
 int cti_ebag_lookup_backward(const void* grad, int32_t grad_dtype, const void* ids, int32_t index_type, int64_t n, int64_t rows,
                              int32_t dim, float scale, int64_t padding_idx, void* out, int32_t out_dtype, int64_t* rows_out,

@@ -1,5 +1,8 @@
 """What a gradient cannot do is refused where the differentiable call is made, not in the backward pass."""
+import ctypes
 import importlib
+import os
+import subprocess
 
 import pytest
 import torch
@@ -117,3 +120,29 @@ def test_tangents_are_refused(pkg, which, grad):
             torch.func.jvp(call, (t,), (t,))
         with pytest.raises(ValueError, match="GPU tensor"):
             call(t)
+
+
+def test_fill_beside_the_sort_stays_within_a_launch(pkg, tmp_path):
+    """The most shares of the fill, with the most workgroups of each kind of launch that takes them, are fewer than 2^32 threads; the
+    library refuses one share more."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cti-inference-optimization_amd", "csrc")
+    (tmp_path / "rules.cpp").write_text(
+        '#include "ebag_train_rules.h"\nusing namespace cti;\n'
+        'extern "C" int64_t shares() { return kGradMostShares; }\n'
+        'extern "C" int64_t share() { return kGradFillShare; }\n'
+        'extern "C" int range_bits(int64_t n, int bits) { return grad_range_bits(n, bits); }\n'
+        'extern "C" int64_t tiles(int64_t n) { return grad_plan(n, 0, 8, 2, 100, false).tiles; }\n')
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", f"-I{csrc}", str(tmp_path / "rules.cpp"), "-o",
+                    str(tmp_path / "rules.so")], check=True)
+    lib = ctypes.CDLL(str(tmp_path / "rules.so"))
+    for f in (lib.shares, lib.share, lib.tiles):
+        f.restype = ctypes.c_int64
+    lib.tiles.argtypes, lib.range_bits.argtypes = [ctypes.c_int64], [ctypes.c_int64, ctypes.c_int]
+    ranges = max(1 << lib.range_bits(n, bits) for n in (1, 64, 128, 4096, 8193, 32768) for bits in range(1, 32))
+    for groups, threads in ((1, 1024), (ranges, 1024), (2048 // 64, 1024), (lib.tiles(2 ** 30), 512)):
+        assert (lib.shares() + groups) * threads < 2 ** 32, (groups, threads)
+    c, row = pkg._capi, 2 ** 18  # bytes of a row of 2^16 fp32 columns, four shares
+    rows = lib.shares() * lib.share() // row + 1
+    # without ids: it ends at the limit, or at a launch
+    status = pkg.load_library().cti_ebag_lookup_backward(None, c.F32, None, c.I64, 0, rows, 2 ** 16, 1.0, -1, 64, c.F32, None, None, 0, None, 0, None)
+    assert status == c.EUNSUPPORTED and "2^38" in c.last_error()
