@@ -6,7 +6,7 @@
 // u_i is the gradient's row that id i contributed to (the id's own position, or its bag), w_i is 1 or, under
 // mean pooling, 1 / length of the bag. No contribution is added by an atomic: the ids are sorted (stably, so
 // in order of position), and each table row's contributions are added in fp32 in an order that the sizes
-// alone fix, rounded once. Rows are the same bits in every run.
+// and the ids fix, rounded once. The same call gives the same bits in every run.
 //
 // 1. Keys: (table's first row number + clamped id, u) for each id; ids of the padding row and ids in no bag
 //    get the key `total`, which sorts last and is dropped. Bags are found from their starts in the tile.

@@ -232,8 +232,8 @@ def embedding_lookup_backward(
     """The gradient of ``embedding_lookup``'s table of ``num_rows`` rows: row v is ``scale`` times the sum of
     ``grad``'s rows whose id, clamped, is v; row ``padding_idx`` is 0.
 
-    ``grad`` ``ids.shape + (dim,)`` fp32 / bf16 / fp16, contiguous. Sums in fp32, in an order that the sizes alone
-    fix, rounded once to ``grad_dtype`` (``grad``'s type by default; or ``out``'s). Returns ``[num_rows, dim]``
+    ``grad`` ``ids.shape + (dim,)`` fp32 / bf16 / fp16, contiguous. Sums in fp32, in an order that sizes and ids
+    fix (the same call gives the same bits in every run), rounded once to ``grad_dtype`` (``grad``'s type by default; or ``out``'s). Returns ``[num_rows, dim]``
     (``out``), or with ``compact`` ``(rows, grads, count)``: the numbers of the rows that occur, ascending, then -1;
     their sums, where what lies behind the last row is left as it was; and how many they are, int64 ``[1]``. There
     ``out`` is a tuple of three such buffers of any capacity of at least ``min(ids, num_rows)`` (and 1) rows.

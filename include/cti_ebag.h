@@ -555,7 +555,7 @@ int cti_ebag_lookup(const void* ids, int32_t index_type, int64_t n, const void* 
  * Gradient of cti_ebag_lookup's table: for every row v
  *   d[v] = scale * sum over i with clamp(ids[i]) = v of grad[i]          (fp32, one rounding to `out_dtype`)
  * and 0 for row padding_idx (-1: none; nn.Embedding's padding_idx). The ids are sorted and each row's
- * contributions added in an order that the sizes alone fix.
+ * contributions added in an order that the sizes and the ids fix: the same call gives the same bits in every run.
  *   grad     [n, dim] of `grad_dtype`, contiguous
  *   rows_out NULL: out is the whole gradient [rows, dim], rows without an id are 0.
  *            Else the rows that occur, in ascending order: rows_out [capacity] their numbers, then -1;
