@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(kLookupThreads) lookup_kernel(const LookupPara
     const uint32_t c = first + k * kLookupThreads, at = c < p.chunks ? c : p.chunks - 1;
     row[k] = p.div.quotient(at);
     col[k] = static_cast<int>(at - row[k] * p.per_row) * 8;
-    if (p.dim >= 8 && col[k] + 8 > p.dim) col[k] = p.dim - 8;
+    if (p.dim >= 8) col[k] = chunk_start(col[k], p.dim);
     id[k] = load_id(p.ids, p.ids64, row[k], p.rows);
   }
 #pragma unroll

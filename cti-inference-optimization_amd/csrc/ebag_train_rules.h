@@ -22,6 +22,10 @@ struct ChunkDivide {
   constexpr uint32_t quotient(uint32_t n) const { return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> shift); }
 };
 
+// Where the 8 columns of the chunk at column c of a row of `cols` (8 or more) begin in the lookup: the row's last 8 for a chunk that
+// would end behind it. (Nothing is added to c, which comes close to 2^31 in the widest rows.)
+constexpr int chunk_start(int c, int cols) { return c <= cols - 8 ? c : cols - 8; }
+
 constexpr int64_t kMostChunks = int64_t{1} << 30;  // of 8 columns, a launch
 
 constexpr int kGradTile = 4096;

@@ -146,3 +146,24 @@ def test_fill_beside_the_sort_stays_within_a_launch(pkg, tmp_path):
     # without ids: it ends at the limit, or at a launch
     status = pkg.load_library().cti_ebag_lookup_backward(None, c.F32, None, c.I64, 0, rows, 2 ** 16, 1.0, -1, 64, c.F32, None, None, 0, None, 0, None)
     assert status == c.EUNSUPPORTED and "2^38" in c.last_error()
+
+
+def test_chunks_of_the_widest_rows(tmp_path):
+    """A chunk's 8 columns lie within its row, also in rows of 2^31 - 1 columns; arithmetic that wraps ends the program."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "cti-inference-optimization_amd", "csrc")
+    (tmp_path / "chunks.cpp").write_text('''
+#include "ebag_train_rules.h"
+#include <cstdio>
+int main() {
+  for (int64_t cols : {8, 9, 15, 16, 1021, (1 << 28) - 1, (1 << 28), 2147483640, 2147483641, 2147483646, 2147483647})
+    for (int64_t chunk = 0; chunk * 8 < cols; chunk = chunk == 2 && cols > 64 ? (cols - 1) / 8 - 2 : chunk + 1) {
+      const int64_t at = cti::chunk_start(static_cast<int>(chunk * 8), static_cast<int>(cols));
+      const int64_t want = chunk * 8 + 8 <= cols ? chunk * 8 : cols - 8;
+      if (at != want || at < 0 || at + 8 > cols) return std::printf("%lld %lld: %lld", (long long)cols, (long long)chunk, (long long)at), 1;
+    }
+}''')
+    subprocess.run(["g++", "-std=c++17", "-O1", "-ftrapv", f"-I{csrc}", str(tmp_path / "chunks.cpp"), "-o", str(tmp_path / "chunks")], check=True)
+    subprocess.run([str(tmp_path / "chunks")], check=True)
+    # and the lookup, which alone takes rows of more than 2^28 columns, goes by it
+    text = open(os.path.join(csrc, "ebag_backward.hip")).read()
+    assert "chunk_start(col[k], p.dim)" in text and "col[k] + 8" not in text
