@@ -688,6 +688,7 @@ class _Norm(torch.autograd.Function):
         ctx.info = (p, None if on_device else seed, offset, residual is not None, h is not None)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(mean, rstd)
+        ctx.bias_shape = bias.shape  # the weight's has as many elements, not always the same dimensions
         return (y, mean, rstd) if h is None else (y, mean, rstd, h)
 
     @staticmethod
@@ -698,7 +699,7 @@ class _Norm(torch.autograd.Function):
         grad = torch.zeros_like(h) if grad is None else grad.contiguous()
         dx, dweight, dbias, dres = dropout_add_layer_norm_backward(
             grad, h, mean, rstd, weight, None if grad_h is None else grad_h.contiguous(), residual, p, rest[0] if rest else seed, offset)
-        return dx, dres, dweight, dbias, None, None, None, None
+        return dx, dres, dweight, dbias.view(ctx.bias_shape), None, None, None, None
 
 
 def dropout_add_layer_norm(

@@ -146,3 +146,18 @@ def test_tangents_are_refused(pkg, dev):
             with pytest.raises(ValueError, match="tangent"):
                 call(torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)))
             call(t)
+
+
+@pytest.mark.parametrize("shapes", [((1, 24), (24,)), ((24,), (1, 24)), ((24, 1, 1), (2, 12))])
+def test_norm_parameters_of_any_dimensions(pkg, dev, shapes):
+    """Accepted by the forward pass where they have as many elements as columns; each gradient has its parameter's shape."""
+    x, gy = randn(1, 6, 24).to(dev).requires_grad_(), randn(2, 6, 24).to(dev)
+    w, b = (randn(3 + i, *s).to(dev).requires_grad_() for i, s in enumerate(shapes))
+    flat = [t.detach().reshape(24).requires_grad_() for t in (w, b)]
+    y = pkg.dropout_add_layer_norm(x, w, b)[0]
+    y.backward(gy)
+    dx, x.grad = x.grad, None
+    pkg.dropout_add_layer_norm(x, *flat)[0].backward(gy)
+    assert torch.equal(dx, x.grad)
+    for t, f in zip((w, b), flat):
+        assert t.grad.shape == t.shape and torch.equal(t.grad.reshape(24), f.grad)
