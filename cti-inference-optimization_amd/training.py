@@ -181,7 +181,9 @@ def embedding_lookup(
         if weight.dim() == 2 and isinstance(ids, torch.Tensor):
             _check_padding(padding_idx, weight.shape[0])
             _check_gradient(ids.numel(), 0, *weight.shape)
-        return _Lookup.apply(weight, ids, scale, padding_idx, out_dtype, sparse_grad)
+            return _Lookup.apply(weight, ids, scale, padding_idx, out_dtype, sparse_grad)
+    elif padding_idx is not None and isinstance(weight, torch.Tensor) and weight.dim() == 2:
+        _check_padding(padding_idx, weight.shape[0])
     return _lookup(ids, weight, scale, out, out_dtype)
 
 
@@ -456,9 +458,10 @@ def _plain_tables(tables, index: int):
 class _PooledTables(torch.autograd.Function):
     @staticmethod
     def forward(ctx, values, offsets, pooling, padding_idx, out_dtype, same, *tables):
+        out = embedding_bag_pooled(values, offsets, tables, pooling, out_dtype)
         ctx.save_for_backward(values, offsets)  # of the tables, only what the gradient needs to know: they may change until then
         ctx.info = (pooling, padding_idx, same, [t.shape for t in tables], tables[0].dtype)
-        return embedding_bag_pooled(values, offsets, tables, pooling, out_dtype)
+        return out
 
     @staticmethod
     @once_differentiable
@@ -485,9 +488,11 @@ def embedding_bag_train(
     their own, as autograd sees them. Tables that require no gradient take no memory and no sums in the backward pass. Where one
     requires it there are at most 64 fields, 2^30 ids and bags, 2^31 - 2 rows of such tables and 2^22 columns of each.
     """
-    for t in tables:
+    for f, t in enumerate(tables):
         if not isinstance(t, torch.Tensor):
             raise TypeError("tables must be tensors: int8 pairs have no gradient")
+        if t.dim() != 2:
+            raise ValueError(f"tables[{f}] must be 2-D, got shape {tuple(t.shape)}")
         _check_padding(padding_idx, t.shape[0])
     _refuse_tangents(*tables)
     first = {}
@@ -497,7 +502,7 @@ def embedding_bag_train(
         if len(tables) > _MOST_FIELDS:
             raise _capi.EbagError(_capi.EUNSUPPORTED, f"no gradient for {len(tables)} fields: at most {_MOST_FIELDS} in a call")
         if isinstance(values, torch.Tensor) and isinstance(offsets, torch.Tensor):
-            _check_gradient(values.numel(), offsets.numel() - 1, sum(t.shape[0] for t in trained), max(t.shape[-1] for t in trained))
+            _check_gradient(values.numel(), offsets.numel() - 1, sum(t.shape[0] for t in trained), max(t.shape[1] for t in trained))
     return _PooledTables.apply(values, offsets, pooling, padding_idx, out_dtype, same, *tables)
 
 
@@ -530,14 +535,19 @@ def fused_embedding_train(
     """The fused step of a flat-layout batch, ``[B, S*D]`` as ``fused_all_slots_embedding`` pools it, differentiable in
     the table (``fused_all_slots_embedding_backward``; ``padding_idx``, ``sparse_grad`` and the limits, of bags too, as in
     ``embedding_lookup``)."""
+    for name, t in (("flat_values", flat_values), ("val_offsets", val_offsets), ("flat_row_offsets", flat_row_offsets), ("weight", weight)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be 2-D [V, D], got shape {tuple(weight.shape)}")
     slots = val_offsets.numel()
-    if slots < 1 or flat_row_offsets.numel() % slots:
+    if slots < 1 or flat_row_offsets.numel() < slots or flat_row_offsets.numel() % slots:
         raise ValueError(f"flat_row_offsets has {flat_row_offsets.numel()} entries for {slots} slots")
     _check_padding(padding_idx, weight.shape[0])
     _refuse_tangents(weight)
     batch_size = flat_row_offsets.numel() // slots - 1
     if _grad_enabled() and weight.requires_grad:
-        _check_gradient(flat_values.numel(), slots * batch_size, weight.shape[0], weight.shape[-1])
+        _check_gradient(flat_values.numel(), slots * batch_size, *weight.shape)
     return _PooledShared.apply(weight, flat_values, val_offsets, flat_row_offsets, batch_size, padding_idx, sparse_grad)
 
 

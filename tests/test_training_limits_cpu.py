@@ -167,3 +167,31 @@ int main() {
     # and the lookup, which alone takes rows of more than 2^28 columns, goes by it
     text = open(os.path.join(csrc, "ebag_backward.hip")).read()
     assert "chunk_start(col[k], p.dim)" in text and "col[k] + 8" not in text
+
+
+def test_malformed_calls_are_explained(pkg):
+    """The package's errors, with or without a gradient, where an IndexError or a message of torch's stood, or nothing."""
+    ids, offsets = torch.zeros(4, dtype=torch.int64), torch.tensor([0, 2, 4])
+    table, flat = torch.zeros(5, 8), torch.zeros(8)
+    for grad in (False, True):
+        w, v, s = (t.clone().requires_grad_(grad) for t in (table, flat, torch.zeros(())))
+        for bad in (-1, 5):
+            for call in (lambda: pkg.embedding_lookup(ids, w, padding_idx=bad), lambda: pkg.embedding_bag_train(ids, offsets, [w], padding_idx=bad),
+                         lambda: pkg.fused_embedding_train(ids, offsets[:1], offsets, w, padding_idx=bad)):
+                with pytest.raises(ValueError, match="padding_idx"):
+                    call()
+        for t in (v, s):
+            with pytest.raises(ValueError):
+                pkg.embedding_lookup(ids, t)
+            with pytest.raises(ValueError, match="2-D"):
+                pkg.embedding_bag_train(ids, offsets, [w, t])
+            with pytest.raises(ValueError, match="2-D"):
+                pkg.fused_embedding_train(ids, offsets[:1], offsets, t)
+        for call in (lambda: pkg.embedding_lookup([1, 2], w), lambda: pkg.embedding_bag_train([1, 2], offsets, [w]),
+                     lambda: pkg.fused_embedding_train(ids, [0], offsets, w), lambda: pkg.fused_embedding_train(ids, offsets[:1], None, w)):
+            with pytest.raises((TypeError, ValueError), match="must be a (torch.Tensor|GPU tensor)"):
+                call()
+        with pytest.raises(ValueError, match="entries for"):
+            pkg.fused_embedding_train(ids, offsets[:1], offsets[:0], w)
+    with pytest.raises(ValueError, match="at least one table"):
+        pkg.embedding_bag_train(ids, offsets, [])
