@@ -176,10 +176,11 @@ class RepEncoder(nn.Module):
         ``nn.Embedding`` defines it; the forward pass reads that row like any), whole or with ``sparse_grad`` as a
         sparse tensor of the rows that occur. Dropout is the LayerNorm kernel's own, with ``seed`` and ``offset`` as in
         ``dropout`` (give every step an offset of its own); nothing of it is stored. Without dropout the result is
-        ``forward``'s up to the order of the LayerNorm's sums."""
+        ``forward``'s up to the order of the LayerNorm's sums. A batch's ``_tile_order`` is followed as in ``pooled``."""
         if self._int8_weight is not None or self._int8_linear is not None:
             raise ValueError("an int8 encoder is not trained: dequantize_() and dequantize_linear_() first")
         norm = self.input_norm
         flat_values, val_offsets, flat_row_offsets, _ = self.flat_inputs(batch)
-        pooled = fused_embedding_train(flat_values, val_offsets, flat_row_offsets, self.emb.weight, self.emb.padding_idx, sparse_grad)
+        pooled = fused_embedding_train(flat_values, val_offsets, flat_row_offsets, self.emb.weight, self.emb.padding_idx, sparse_grad,
+                                       batch.get("_tile_order"))
         return self.linear(dropout_add_layer_norm(pooled, norm.weight, norm.bias, norm.eps, p=dropout, seed=seed, offset=offset)[0])

@@ -508,12 +508,13 @@ def embedding_bag_train(
 
 class _PooledShared(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, flat_values, val_offsets, flat_row_offsets, batch_size, padding_idx, sparse_grad):
+    def forward(ctx, weight, flat_values, val_offsets, flat_row_offsets, batch_size, padding_idx, sparse_grad, tile_order):
         ctx.save_for_backward(flat_values, val_offsets, flat_row_offsets)
         rows, dim = weight.shape
         ctx.info = (rows, dim, batch_size, padding_idx, sparse_grad)
         out = torch.empty(batch_size, val_offsets.numel() * dim, dtype=weight.dtype, device=weight.device)
-        return fused_all_slots_embedding(flat_values, val_offsets, flat_row_offsets, weight, out, batch_size, dim, rows - 1)
+        return fused_all_slots_embedding(flat_values, val_offsets, flat_row_offsets, weight, out, batch_size, dim, rows - 1,
+                                         tile_order=tile_order)
 
     @staticmethod
     @once_differentiable
@@ -521,7 +522,7 @@ class _PooledShared(torch.autograd.Function):
         rows, dim, batch_size, padding_idx, sparse_grad = ctx.info
         got = fused_all_slots_embedding_backward(grad.contiguous(), *ctx.saved_tensors, batch_size, dim, rows - 1,
                                                  padding_idx=padding_idx, compact=sparse_grad)
-        return (_sparse(got, rows, dim) if sparse_grad else got), None, None, None, None, None, None
+        return (_sparse(got, rows, dim) if sparse_grad else got), None, None, None, None, None, None, None
 
 
 def fused_embedding_train(
@@ -531,10 +532,12 @@ def fused_embedding_train(
     weight: torch.Tensor,
     padding_idx: Optional[int] = None,
     sparse_grad: bool = False,
+    tile_order: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """The fused step of a flat-layout batch, ``[B, S*D]`` as ``fused_all_slots_embedding`` pools it, differentiable in
     the table (``fused_all_slots_embedding_backward``; ``padding_idx``, ``sparse_grad`` and the limits, of bags too, as in
-    ``embedding_lookup``)."""
+    ``embedding_lookup``). ``tile_order``: the batch's dispatch order for the forward pass, as ``fused_all_slots_embedding`` takes
+    it."""
     for name, t in (("flat_values", flat_values), ("val_offsets", val_offsets), ("flat_row_offsets", flat_row_offsets), ("weight", weight)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
@@ -548,7 +551,7 @@ def fused_embedding_train(
     batch_size = flat_row_offsets.numel() // slots - 1
     if _grad_enabled() and weight.requires_grad:
         _check_gradient(flat_values.numel(), slots * batch_size, *weight.shape)
-    return _PooledShared.apply(weight, flat_values, val_offsets, flat_row_offsets, batch_size, padding_idx, sparse_grad)
+    return _PooledShared.apply(weight, flat_values, val_offsets, flat_row_offsets, batch_size, padding_idx, sparse_grad, tile_order)
 
 
 # ------------------------------------------------------------------------------------------------

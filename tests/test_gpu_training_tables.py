@@ -161,3 +161,30 @@ def test_norm_parameters_of_any_dimensions(pkg, dev, shapes):
     assert torch.equal(dx, x.grad)
     for t, f in zip((w, b), flat):
         assert t.grad.shape == t.shape and torch.equal(t.grad.reshape(24), f.grad)
+
+
+def test_training_step_follows_the_batchs_tile_order(pkg, dev, monkeypatch):
+    """As pooled() does, and with the same result bit for bit."""
+    import sys
+
+    slots, dim, batch, rows = 28, 128, 64, 500
+    gen = torch.Generator().manual_seed(1)
+    lens = torch.randint(0, 12, (slots, batch), generator=gen)
+    values = torch.randint(0, rows, (int(lens.sum()),), generator=gen)
+    row_offsets = torch.zeros(slots, batch + 1, dtype=torch.int64)
+    row_offsets[:, 1:] = lens.cumsum(1)
+    val_offsets = (lens.sum(1).cumsum(0) - lens.sum(1)).to(dev)
+    order = pkg.make_tile_order(row_offsets.reshape(-1), batch, slots, torch.bfloat16, dim).to(dev)
+    enc = pkg.RepEncoder(rows, dim, slot_num=slots, d_model=16).to(dev).bfloat16()
+    flat = {"_flat_values": values.to(dev), "_val_offsets": val_offsets, "_flat_row_offsets": row_offsets.reshape(-1).to(dev)}
+    module, seen = sys.modules[pkg.__name__ + ".training"], []
+    pooled = module.fused_all_slots_embedding
+    monkeypatch.setattr(module, "fused_all_slots_embedding", lambda *a, **kw: (seen.append(kw.get("tile_order")), pooled(*a, **kw))[1])
+    out = []
+    for case in (flat, {**flat, "_tile_order": order}):
+        enc.zero_grad()
+        y = enc.forward_train(case, dropout=0.2, seed=3, offset=1)
+        y.float().square().sum().backward()
+        out.append([y.detach(), *(p.grad.clone() for p in enc.parameters())])
+    assert seen[0] is None and seen[1] is order
+    assert all(torch.equal(a, b) for a, b in zip(*out))
