@@ -486,7 +486,11 @@ def embedding_bag_train(
     """``embedding_bag_pooled`` of float tables, differentiable in them (``embedding_bag_backward``). Fields share a table where they
     are given the same tensor. Tensors that only share memory, a table and what ``detach()`` makes of it among them, are tables of
     their own, as autograd sees them. Tables that require no gradient take no memory and no sums in the backward pass. Where one
-    requires it there are at most 64 fields, 2^30 ids and bags, 2^31 - 2 rows of such tables and 2^22 columns of each.
+    requires it there are at most 64 fields, 2^30 ids and bags, 2^31 - 2 rows of such tables and 2^22 columns of each, the offsets
+    ascend (else the gradients are unspecified), and gradients are whole (``embedding_bag_backward`` has the compact form).
+
+    Row ``padding_idx`` of every table gets the gradient 0, and that is all: unlike ``nn.EmbeddingBag``'s, the forward pass reads the
+    row like any other, and its ids count in a mean's length.
     """
     for f, t in enumerate(tables):
         if not isinstance(t, torch.Tensor):
@@ -537,7 +541,11 @@ def fused_embedding_train(
     """The fused step of a flat-layout batch, ``[B, S*D]`` as ``fused_all_slots_embedding`` pools it, differentiable in
     the table (``fused_all_slots_embedding_backward``; ``padding_idx``, ``sparse_grad`` and the limits, of bags too, as in
     ``embedding_lookup``). ``tile_order``: the batch's dispatch order for the forward pass, as ``fused_all_slots_embedding`` takes
-    it."""
+    it.
+
+    The bags have to lie in ``flat_values`` in the order of slots and samples, none over another, as ``collate_flat_layout``,
+    ``pack_slots`` and ``merge_batches`` lay them out. The forward pass pools any other batch too (slots in another order, bags
+    that share ids), but its gradient is unspecified, without an error."""
     for name, t in (("flat_values", flat_values), ("val_offsets", val_offsets), ("flat_row_offsets", flat_row_offsets), ("weight", weight)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
