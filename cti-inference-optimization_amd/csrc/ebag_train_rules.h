@@ -162,13 +162,15 @@ inline int64_t train_norm_workgroups(int64_t rows, int64_t cols) {
   const int64_t n = ceil_div(rows, side);
   return n < 1 ? 0 : ceil_div(n, ceil_div(n, most));  // as many rows to each
 }
-// Few rows: the parameters' gradients come from workgroups of the same launch that read all rows of 128 columns once more (from
-// L2) instead of a second launch that adds up the first one's sums. Calls one after another, one launch against two: 128 x 3,584
-// 9.5 against 13.4 us (4.9 against 8.2 in a graph), 256 x 8,192 9.2 against 15.9, 256 x 256 9.5 against 13.5 (6.2 against 6.0);
-// 255 x 1,021, whose chunks are loaded by elements, 11.4 against 13.6 (11.6 against 7.7). 512 x 3,584 still 11.7 against 17.7, but
-// in a graph 512 x 1,024 9.8 against 8.1 and 1,024 x 1,024 18.1 against 11.0.
+// Few rows: the parameters' gradients come from workgroups of the same launch that read all rows of some columns once more (from
+// L2) instead of a second launch that adds up the first one's sums: 64 columns each where up to 256 threads hold a row (2,048
+// columns), else 128. Backward passes one after another in a graph, one launch against two (us, fp16): 128 x 3,584 4.5 against 7.8,
+// 256 x 8,192 7.6 against 15.8, 256 x 1,024 5.0 against 6.7, 255 x 1,021 6.7 against 7.4, 255 x 8,191 12.0 against 18.9; narrow odd
+// rows are level (255 x 333: 7.0 and 7.2) or lose (255 x 77: 7.7 and 5.9). By calls the host takes 12 with one launch, 17 with
+// two. More rows lose: in a graph 512 x 1,024 was 9.8 against 8.1 and 1,024 x 1,024 18.1 against 11.0 (128 columns each). 64 columns a
+// workgroup for wide rows too: 256 x 3,584 8.1 for 6.6; 128 for all: 255 x 1,021 9.6 for 6.7.
 constexpr int64_t kTrainNormFewRows = 256;
-constexpr int kTrainNormFewCols = 128;
+constexpr int train_norm_few_cols(int lanes) { return lanes <= 256 ? 64 : 128; }
 inline bool train_norm_few(int64_t rows, int64_t cols) { return rows <= kTrainNormFewRows && cols <= 8192; }
 inline int64_t train_norm_workspace_bytes(int64_t rows, int64_t cols) {
   return rows <= 0 || train_norm_few(rows, cols) ? 0 : train_norm_workgroups(rows, cols) * 2 * ceil_div(cols, 8) * 8 * 4;
