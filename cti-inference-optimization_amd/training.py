@@ -379,7 +379,7 @@ def _bag_gradients(index, grad, values, offsets, shapes, alike, dtype, same, poo
     pool = _capi.pooling_code(pooling)
     with_grad = shapes if wanted is None else [shape for f, shape in enumerate(shapes) if wanted[f]]
     if same is None:
-        same, rows = range(fields), sum(shape[0] for shape in with_grad)
+        same, rows = range(fields), len(with_grad) * shapes[0][0] if alike else sum(shape[0] for shape in with_grad)
     else:
         rows = sum(shapes[f][0] for f in set(same) if wanted is None or wanted[f])
     padding = _check_padding(padding_idx, shapes[0][0] if alike else min(shape[0] for shape in with_grad))
