@@ -361,7 +361,7 @@ def _bag_gradients(index, grad, values, offsets, shapes, alike, dtype, same, poo
                    out=None, wanted=None):
     """``embedding_bag_backward`` of tables of these shapes (``alike``: all the same) and this type; ``same[f]``: the first field with
     field f's table (None: no field shares one); ``wanted[f]``: whether its table has a gradient (None: every field's; the whole
-    form alone, which gives None for the others)."""
+    form gives None for the others, the compact one does not count their rows)."""
     dev = grad.device
     fields = len(shapes)
     width = fields * shapes[0][1] if alike else sum(shape[1] for shape in shapes)
@@ -457,22 +457,35 @@ def _plain_tables(tables, index: int):
 
 class _PooledTables(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, values, offsets, pooling, padding_idx, out_dtype, same, *tables):
+    def forward(ctx, values, offsets, pooling, padding_idx, out_dtype, sparse_grad, same, *tables):
         out = embedding_bag_pooled(values, offsets, tables, pooling, out_dtype)
         ctx.save_for_backward(values, offsets)  # of the tables, only what the gradient needs to know: they may change until then
-        ctx.info = (pooling, padding_idx, same, [t.shape for t in tables], tables[0].dtype)
+        ctx.info = (pooling, padding_idx, sparse_grad, same, [t.shape for t in tables], tables[0].dtype)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         values, offsets = ctx.saved_tensors
-        pooling, padding_idx, same, shapes, dtype = ctx.info
-        wanted = ctx.needs_input_grad[6:]
+        pooling, padding_idx, sparse_grad, same, shapes, dtype = ctx.info
+        wanted = ctx.needs_input_grad[7:]
         grads = _bag_gradients(grad.get_device(), grad.contiguous(), values, offsets, shapes, len(set(shapes)) == 1, dtype, same,
-                               pooling, padding_idx, wanted=None if all(wanted) else wanted)
+                               pooling, padding_idx, compact=sparse_grad, wanted=None if all(wanted) else wanted)
         # autograd adds up the fields' gradients of one table: its sum is in the first
-        return (None, None, None, None, None, None, *(g if same[f] == f else None for f, g in enumerate(grads)))
+        first = [f for f in range(len(shapes)) if same[f] == f and wanted[f]]
+        by_field = dict(zip(first, _sparse_tables(grads, [shapes[f] for f in first])) if sparse_grad else ((f, grads[f]) for f in first))
+        return (None,) * 7 + tuple(by_field.get(f) for f in range(len(shapes)))
+
+
+def _sparse_tables(got, shapes):
+    """Compact rows of tables of these shapes, numbered one table behind the other, as a sparse tensor of torch each; waits for
+    their count."""
+    numbers, sums, count = got
+    numbers = numbers[:int(count.item())]
+    starts = [0, *itertools.accumulate(shape[0] for shape in shapes)]
+    ends = torch.searchsorted(numbers, torch.tensor(starts, device=numbers.device)).tolist()
+    return [torch.sparse_coo_tensor((numbers[a:b] - start).unsqueeze(0), sums[a:b], shape, is_coalesced=True, check_invariants=False)
+            for a, b, start, shape in zip(ends, ends[1:], starts, shapes)]
 
 
 def embedding_bag_train(
@@ -482,12 +495,14 @@ def embedding_bag_train(
     pooling: str = "sum",
     padding_idx: Optional[int] = None,
     out_dtype: Optional[torch.dtype] = None,
+    sparse_grad: bool = False,
 ) -> torch.Tensor:
     """``embedding_bag_pooled`` of float tables, differentiable in them (``embedding_bag_backward``). Fields share a table where they
     are given the same tensor. Tensors that only share memory, a table and what ``detach()`` makes of it among them, are tables of
     their own, as autograd sees them. Tables that require no gradient take no memory and no sums in the backward pass. Where one
-    requires it there are at most 64 fields, 2^30 ids and bags, 2^31 - 2 rows of such tables and 2^22 columns of each, the offsets
-    ascend (else the gradients are unspecified), and gradients are whole (``embedding_bag_backward`` has the compact form).
+    requires it there are at most 64 fields, 2^30 ids and bags, 2^31 - 2 rows of such tables and 2^22 columns of each, and the
+    offsets ascend (else the gradients are unspecified). With ``sparse_grad`` (such tables then have one width) gradients are sparse
+    tensors of the rows that occur, as ``embedding_lookup``'s, and their making waits for their count.
 
     Row ``padding_idx`` of every table gets the gradient 0, and that is all: unlike ``nn.EmbeddingBag``'s, the forward pass reads the
     row like any other, and its ids count in a mean's length.
@@ -505,9 +520,11 @@ def embedding_bag_train(
     if trained and _grad_enabled():
         if len(tables) > _MOST_FIELDS:
             raise _capi.EbagError(_capi.EUNSUPPORTED, f"no gradient for {len(tables)} fields: at most {_MOST_FIELDS} in a call")
+        if sparse_grad and len({t.shape[1] for t in trained}) > 1:
+            raise _capi.EbagError(_capi.EUNSUPPORTED, "sparse gradients need tables of one width")
         if isinstance(values, torch.Tensor) and isinstance(offsets, torch.Tensor):
             _check_gradient(values.numel(), offsets.numel() - 1, sum(t.shape[0] for t in trained), max(t.shape[1] for t in trained))
-    return _PooledTables.apply(values, offsets, pooling, padding_idx, out_dtype, same, *tables)
+    return _PooledTables.apply(values, offsets, pooling, padding_idx, out_dtype, sparse_grad, same, *tables)
 
 
 class _PooledShared(torch.autograd.Function):

@@ -188,3 +188,52 @@ def test_training_step_follows_the_batchs_tile_order(pkg, dev, monkeypatch):
         out.append([y.detach(), *(p.grad.clone() for p in enc.parameters())])
     assert seen[0] is None and seen[1] is order
     assert all(torch.equal(a, b) for a, b in zip(*out))
+
+
+@pytest.mark.parametrize("frozen", [(), (0,), (1, 4)])
+@pytest.mark.parametrize("padding,pooling,max_len", [(None, "sum", 6), (0, "mean", 6), (3, "sum", 300), (None, "mean", 0)])
+def test_sparse_gradients_of_tables_per_field(pkg, dev, frozen, padding, pooling, max_len):
+    """The rows that occur, each once and in order, with the whole gradients' bits where the same call gives these; tables that
+    share, frozen ones between; no ids at all."""
+    values, offsets, parts = make_fields(5, seed=max_len, rows=ROWS, max_len=max_len)
+    grad = randn(1, BATCH, 5 * DIM).to(dev)
+    a, b, c, d = (randn(s, ROWS + 7 * s, DIM).to(dev) for s in (0, 1, 2, 3))
+    tables = [a, b, c, a, d]  # field 3 shares field 0's
+    for f in frozen:
+        tables[f] = tables[f].detach()
+    leaves = {id(t): t.requires_grad_() for f, t in enumerate(tables) if f not in frozen}
+    grads = []
+    for sparse in (False, True):
+        for t in leaves.values():
+            t.grad = None
+        out = pkg.embedding_bag_train(values.to(dev), offsets.to(dev), tables, pooling, padding_idx=padding, sparse_grad=sparse)
+        out.backward(grad)
+        grads.append([t.grad for t in leaves.values()])
+    for whole, sparse in zip(*grads):
+        assert sparse.is_sparse and sparse.shape == whole.shape and sparse.dtype == whole.dtype
+        rows = sparse._indices()[0]  # (torch drops the mark that they are in order)
+        assert bool((rows[1:] > rows[:-1]).all()) and torch.equal(sparse.to_dense(), whole)
+        assert padding is None or not bool((rows == padding).any())
+    assert all(tables[f].grad is None for f in frozen)
+    ids = [p[0].unique() for p in parts]
+    first = list(leaves.values())[0]
+    if first is a:  # fields 0 and 3
+        occur = torch.cat([ids[0], ids[3]]).unique()
+        occur = occur[occur != padding] if padding is not None else occur
+        # ids of the larger tables are not clamped to ROWS there, but a has ROWS rows
+        assert torch.equal(grads[1][0]._indices()[0].cpu(), occur)
+
+
+def test_sparse_gradients_train(pkg, dev):
+    """An optimizer of torch's takes them; rows without ids stay."""
+    values, offsets, parts = make_fields(2)
+    tables = [torch.nn.Parameter(randn(s, 1000, DIM).to(dev)) for s in (2, 3)]
+    before = [t.detach().clone() for t in tables]
+    opt = torch.optim.SparseAdam(tables, lr=0.1)
+    pkg.embedding_bag_train(values.to(dev), offsets.to(dev), tables, sparse_grad=True).square().sum().backward()
+    opt.step()
+    for f, t in enumerate(tables):
+        touched = torch.zeros(1000, dtype=torch.bool)
+        ids = values[offsets[f * BATCH]:offsets[(f + 1) * BATCH]].clamp(0, 999)
+        touched[ids] = True
+        assert torch.equal((t.detach() != before[f]).any(1).cpu(), touched)

@@ -129,3 +129,31 @@ def test_gradient_of_some_fields_refuses(pkg):
     compact = dict(rows_out=64, count=64, cap=4, out=64)
     assert call(3, dict(dim=4, row_stride=4), **compact)[0] == c.EUNSUPPORTED
     assert call(1, dict(dim=4, row_stride=4), **compact)[0] == c.EWORKSPACE
+
+
+def test_rows_of_several_tables_are_told_apart(pkg):
+    """Compact rows are numbered one table behind the other."""
+    module = importlib.import_module(pkg.__name__ + ".training")
+    shapes = [(4, 3), (1, 3), (6, 3), (2, 3)]
+    numbers = torch.tensor([0, 3, 5, 9, 10, 11, 12, -1, -1])
+    sums = torch.arange(9 * 3, dtype=torch.float32).view(9, 3)
+    got = module._sparse_tables((numbers, sums, torch.tensor([7])), shapes)
+    want = torch.zeros(13, 3)
+    want[numbers[:7]] = sums[:7]
+    at = 0
+    for g, shape in zip(got, shapes):
+        assert g.shape == shape and torch.equal(g.to_dense(), want[at:at + shape[0]])
+        at += shape[0]
+    assert [g._nnz() for g in got] == [2, 0, 3, 2]
+    none = module._sparse_tables((numbers, sums, torch.tensor([0])), shapes)
+    assert [g._nnz() for g in none] == [0, 0, 0, 0]
+
+
+def test_sparse_gradients_need_one_width(pkg):
+    ids, offsets = torch.zeros(4, dtype=torch.int64), torch.arange(5)
+    wide, narrow = torch.zeros(5, 8, requires_grad=True), torch.zeros(5, 4, requires_grad=True)
+    with pytest.raises(pkg.EbagError, match="one width"):
+        pkg.embedding_bag_train(ids, offsets, [wide, narrow], sparse_grad=True)
+    for tables, sparse in (([wide, narrow.detach()], True), ([wide, narrow], False)):  # only of those that have a gradient
+        with pytest.raises(ValueError, match="GPU tensor"):
+            pkg.embedding_bag_train(ids, offsets, tables, sparse_grad=sparse)
