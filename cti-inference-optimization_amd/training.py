@@ -457,24 +457,27 @@ def _plain_tables(tables, index: int):
 
 class _PooledTables(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, values, offsets, pooling, padding_idx, out_dtype, sparse_grad, same, *tables):
+    def forward(ctx, values, offsets, pooling, padding_idx, out_dtype, sparse_grad, known, *tables):
         out = embedding_bag_pooled(values, offsets, tables, pooling, out_dtype)
         ctx.save_for_backward(values, offsets)  # of the tables, only what the gradient needs to know: they may change until then
-        ctx.info = (pooling, padding_idx, sparse_grad, same, [t.shape for t in tables], tables[0].dtype)
+        ctx.info = (pooling, padding_idx, sparse_grad, *known, tables[0].dtype)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         values, offsets = ctx.saved_tensors
-        pooling, padding_idx, sparse_grad, same, shapes, dtype = ctx.info
+        pooling, padding_idx, sparse_grad, shapes, alike, same, dtype = ctx.info
         wanted = ctx.needs_input_grad[7:]
-        grads = _bag_gradients(grad.get_device(), grad.contiguous(), values, offsets, shapes, len(set(shapes)) == 1, dtype, same,
-                               pooling, padding_idx, compact=sparse_grad, wanted=None if all(wanted) else wanted)
-        # autograd adds up the fields' gradients of one table: its sum is in the first
-        first = [f for f in range(len(shapes)) if same[f] == f and wanted[f]]
-        by_field = dict(zip(first, _sparse_tables(grads, [shapes[f] for f in first])) if sparse_grad else ((f, grads[f]) for f in first))
-        return (None,) * 7 + tuple(by_field.get(f) for f in range(len(shapes)))
+        grads = _bag_gradients(grad.get_device(), grad.contiguous(), values, offsets, shapes, alike, dtype, same, pooling, padding_idx,
+                               compact=sparse_grad, wanted=None if all(wanted) else wanted)
+        if sparse_grad:
+            first = [f for f in range(len(shapes)) if wanted[f] and (same is None or same[f] == f)]
+            made = dict(zip(first, _sparse_tables(grads, [shapes[f] for f in first])))
+            grads = [made.get(f) for f in range(len(shapes))]
+        elif same is not None:  # autograd adds up the fields' gradients of one table: its sum is in the first
+            grads = [g if same[f] == f else None for f, g in enumerate(grads)]
+        return (None, None, None, None, None, None, None, *grads)
 
 
 def _sparse_tables(got, shapes):
@@ -507,24 +510,35 @@ def embedding_bag_train(
     Row ``padding_idx`` of every table gets the gradient 0, and that is all: unlike ``nn.EmbeddingBag``'s, the forward pass reads the
     row like any other, and its ids count in a mean's length.
     """
+    shapes = []  # looked up once: for 28 tables each pass over them takes as long as a launch
     for f, t in enumerate(tables):
         if not isinstance(t, torch.Tensor):
             raise TypeError("tables must be tensors: int8 pairs have no gradient")
-        if t.dim() != 2:
-            raise ValueError(f"tables[{f}] must be 2-D, got shape {tuple(t.shape)}")
-        _check_padding(padding_idx, t.shape[0])
+        shape = t.shape
+        if len(shape) != 2:
+            raise ValueError(f"tables[{f}] must be 2-D, got shape {tuple(shape)}")
+        shapes.append(shape)
+    if padding_idx is not None and shapes:
+        _check_padding(padding_idx, min(shape[0] for shape in shapes))
     _refuse_tangents(*tables)
-    first = {}
-    same = [first.setdefault(id(t), f) for f, t in enumerate(tables)]
-    trained = [t for f, t in enumerate(tables) if same[f] == f and t.requires_grad]
-    if trained and _grad_enabled():
-        if len(tables) > _MOST_FIELDS:
-            raise _capi.EbagError(_capi.EUNSUPPORTED, f"no gradient for {len(tables)} fields: at most {_MOST_FIELDS} in a call")
-        if sparse_grad and len({t.shape[1] for t in trained}) > 1:
+    fields = len(shapes)
+    alike = fields > 0 and shapes.count(shapes[0]) == fields
+    same = None  # the first field with the table
+    if len(set(map(id, tables))) != fields:
+        first = {}
+        same = [first.setdefault(id(t), f) for f, t in enumerate(tables)]
+    needs = [t.requires_grad for t in tables]
+    if True in needs and _grad_enabled():
+        if fields > _MOST_FIELDS:
+            raise _capi.EbagError(_capi.EUNSUPPORTED, f"no gradient for {fields} fields: at most {_MOST_FIELDS} in a call")
+        trained = [shape for f, shape in enumerate(shapes) if needs[f] and (same is None or same[f] == f)]
+        dim = trained[0][1] if alike else max(shape[1] for shape in trained)
+        if sparse_grad and not alike and min(shape[1] for shape in trained) != dim:
             raise _capi.EbagError(_capi.EUNSUPPORTED, "sparse gradients need tables of one width")
         if isinstance(values, torch.Tensor) and isinstance(offsets, torch.Tensor):
-            _check_gradient(values.numel(), offsets.numel() - 1, sum(t.shape[0] for t in trained), max(t.shape[1] for t in trained))
-    return _PooledTables.apply(values, offsets, pooling, padding_idx, out_dtype, sparse_grad, same, *tables)
+            rows = len(trained) * trained[0][0] if alike else sum(shape[0] for shape in trained)
+            _check_gradient(values.numel(), offsets.numel() - 1, rows, dim)
+    return _PooledTables.apply(values, offsets, pooling, padding_idx, out_dtype, sparse_grad, (shapes, alike, same), *tables)
 
 
 class _PooledShared(torch.autograd.Function):
@@ -726,7 +740,7 @@ class _Norm(torch.autograd.Function):
         ctx.info = (p, None if on_device else seed, offset, residual is not None, h is not None)
         ctx.set_materialize_grads(False)
         ctx.mark_non_differentiable(mean, rstd)
-        ctx.bias_shape = bias.shape  # the weight's has as many elements, not always the same dimensions
+        ctx.bias_shape = None if bias.shape == weight.shape else bias.shape  # as many elements, not always the same dimensions
         return (y, mean, rstd) if h is None else (y, mean, rstd, h)
 
     @staticmethod
@@ -737,7 +751,7 @@ class _Norm(torch.autograd.Function):
         grad = torch.zeros_like(h) if grad is None else grad.contiguous()
         dx, dweight, dbias, dres = dropout_add_layer_norm_backward(
             grad, h, mean, rstd, weight, None if grad_h is None else grad_h.contiguous(), residual, p, rest[0] if rest else seed, offset)
-        return dx, dres, dweight, dbias.view(ctx.bias_shape), None, None, None, None
+        return dx, dres, dweight, dbias if ctx.bias_shape is None else dbias.view(ctx.bias_shape), None, None, None, None
 
 
 def dropout_add_layer_norm(
