@@ -17,7 +17,7 @@
 // up in their order (up to 256 rows of up to 8,192 columns: in the same launch, by workgroups that read the rows once
 // more). No atomics: results are the same bits in every run.
 //
-// Measured (16,384 x 4,096 bf16; a copy of 1 GiB reaches 5.2 TB/s here): dropout 44 us, with a residual 71 (6.1 and 5.7
+// Measured (16,384 x 4,096 bf16; a read and a write of 1 GiB reach 6.25 TB/s here): dropout 44 us, with a residual 71 (6.1 and 5.7
 // TB/s); forward with dropout and residual 95 (5.6); backward with grad_h and both gradients out 137 (4.9), and the
 // parameters' sums 6.
 #include <stdint.h>
