@@ -176,7 +176,8 @@ class RepEncoder(nn.Module):
         ``nn.Embedding`` defines it; the forward pass reads that row like any), whole or with ``sparse_grad`` as a
         sparse tensor of the rows that occur. Dropout is the LayerNorm kernel's own, with ``seed`` and ``offset`` as in
         ``dropout`` (give every step an offset of its own); nothing of it is stored. Without dropout the result is
-        ``forward``'s up to the order of the LayerNorm's sums. A batch's ``_tile_order`` is followed as in ``pooled``."""
+        ``forward``'s up to the order of the LayerNorm's sums. A batch's ``_tile_order`` is followed as in ``pooled``.
+        Its bags have to lie in order (``fused_embedding_train``), as every builder of this package lays them out."""
         if self._int8_weight is not None or self._int8_linear is not None:
             raise ValueError("an int8 encoder is not trained: dequantize_() and dequantize_linear_() first")
         norm = self.input_norm

@@ -237,3 +237,49 @@ def test_sparse_gradients_train(pkg, dev):
         ids = values[offsets[f * BATCH]:offsets[(f + 1) * BATCH]].clamp(0, 999)
         touched[ids] = True
         assert torch.equal((t.detach() != before[f]).any(1).cpu(), touched)
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_any_mix_of_tables(pkg, dev, seed):
+    """Fields with tables of their own, shared ones, detached aliases and leaves over one memory, frozen ones; widths alike or not;
+    every type; sum and mean; a long bag; whole and sparse."""
+    import random
+
+    rng, gen = random.Random(seed), torch.Generator().manual_seed(seed)
+    types = [torch.float32, torch.bfloat16, torch.float16]
+    fields, batch = rng.choice([1, 2, 5, 13, 64]), rng.choice([1, 7, 33, 200])
+    dims = [rng.choice([1, 8, 24, 64, 65, 128, 256])] * fields if rng.random() < 0.5 else [rng.choice([1, 7, 64, 100, 129]) for _ in range(fields)]
+    dtype, out_dtype, pooling, padding = rng.choice(types), rng.choice([None, *types]), rng.choice(["sum", "mean"]), rng.choice([None, 0])
+    tables = []
+    for f in range(fields):
+        other = rng.randrange(f) if f and rng.random() < 0.4 else None
+        if other is not None and dims[other] == dims[f]:
+            tables.append(tables[other] if rng.random() < 0.5 else tables[other].detach().requires_grad_(rng.random() < 0.5))
+        else:
+            table = torch.randn(rng.choice([1, 5, 100, 3000]), dims[f], generator=gen).to(dtype)
+            tables.append(table.to(dev).requires_grad_(rng.random() < 0.7 or f == 0))
+    rows = [t.shape[0] for t in tables]
+    lens = torch.randint(0, rng.choice([1, 4, 30]) + 1, (fields, batch), generator=gen)
+    if rng.random() < 0.4:
+        lens[rng.randrange(fields), rng.randrange(batch)] = rng.choice([100, 9000])
+    values = torch.cat([torch.randint(-1, rows[f] + 1, (int(lens[f].sum()),), generator=gen) for f in range(fields)])
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), lens.reshape(-1).cumsum(0)])
+    trained = {id(t): t for t in tables if t.requires_grad}
+    sparse = len({t.shape[1] for t in trained.values()}) == 1 and rng.random() < 0.5
+    out = pkg.embedding_bag_train(values.to(dev, rng.choice([torch.int64, torch.int32])), offsets.to(dev), tables, pooling, padding, out_dtype,
+                                  sparse_grad=sparse)
+    grad = torch.randn(out.shape, generator=gen).to(out.dtype)
+    out.backward(grad.to(dev))
+    assert all(t.grad is None for t in tables if not t.requires_grad)
+    for t in trained.values():
+        ids, parts, weights = [], [], []
+        for f in range(fields):
+            if tables[f] is t:
+                sample = torch.repeat_interleave(torch.arange(batch), lens[f])
+                ids.append(values[offsets[f * batch]:offsets[(f + 1) * batch]].clamp(0, rows[f] - 1))
+                parts.append(grad[:, sum(dims[:f]):sum(dims[:f + 1])].double()[sample])
+                weights.append(1.0 / lens[f][sample].double() if pooling == "mean" else torch.ones(sample.numel(), dtype=torch.float64))
+        want, absolute, count = ref.table_gradient(torch.cat(parts), torch.cat(ids), t.shape[0], padding=padding, weights=torch.cat(weights))
+        assert t.grad.is_sparse == sparse
+        ref.assert_within(t.grad.to_dense() if sparse else t.grad, want,
+                          ref.gradient_bound(want, absolute, count, t.dtype, pooling == "mean"))
